@@ -351,6 +351,251 @@ def add(a, b, stream=None):
 
 
 # ---------------------------------------------------------------------------
+# a KV cache held in 4 bits
+# ---------------------------------------------------------------------------
+class _Kv4Struct(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("k", "k_scales", "k_biases", "v", "v_scales", "v_biases")] + [
+        (n, ctypes.c_int) for n in ("n_kv_heads", "capacity", "group_size", "bits")]
+
+
+KV4_COUNTER_BYTES = 65536  # BMX_KV4_COUNTER_BYTES
+
+
+class Kv4Cache:
+    """bmx_kv4: one layer's keys and values as MLX affine 4-bit rows of 128
+    values, group size 64 -- k, v [n_kv_heads, capacity, 16] int32 (packed
+    words), *_scales and *_biases [n_kv_heads, capacity, 2] bf16, contiguous,
+    on one GPU.  The object holds the tensors, in attributes of these names,
+    and describes them to the library as they are now."""
+
+    def __init__(self, k, k_scales, k_biases, v, v_scales, v_biases):
+        torch = _torch()
+        ts = (k, k_scales, k_biases, v, v_scales, v_biases)
+        _require_cuda(*ts)
+        if k.dim() != 3 or k.shape[2] != 16 or v.shape != k.shape:
+            raise BmxError(BMX_E_SHAPE, f"k and v must be [n_kv_heads, capacity, 16], got {tuple(k.shape)}, "
+                                        f"{tuple(v.shape)}")
+        if any(w.dtype not in (torch.int32, torch.uint32) for w in (k, v)):
+            raise BmxError(BMX_E_ARG, "k and v must be int32 or uint32 words")
+        for t in (k_scales, k_biases, v_scales, v_biases):
+            if t.shape != (*k.shape[:2], 2):
+                raise BmxError(BMX_E_SHAPE, f"scales and biases must be {(*k.shape[:2], 2)}, got {tuple(t.shape)}")
+            if t.dtype != torch.bfloat16:
+                raise BmxError(BMX_E_ARG, "scales and biases must be bfloat16")
+        _same_device(*ts)
+        self.k, self.k_scales, self.k_biases, self.v, self.v_scales, self.v_biases = ts
+        self.n_kv_heads, self.capacity, self.device = k.shape[0], k.shape[1], k.device
+        self._struct = _Kv4Struct(*[t.data_ptr() for t in ts], self.n_kv_heads, self.capacity, 64, 4)
+        self._ref = ctypes.addressof(self._struct)
+
+    @classmethod
+    def empty(cls, n_kv_heads, capacity, device="cuda"):
+        """A zero-filled cache (every row reads back as zeros)."""
+        torch = _torch()
+        t = []
+        for _ in range(2):
+            t.append(torch.zeros(n_kv_heads, capacity, 16, dtype=torch.int32, device=device))
+            t += [torch.zeros(n_kv_heads, capacity, 2, dtype=torch.bfloat16, device=device) for _ in range(2)]
+        return cls(*t)
+
+
+def _same_device(t, *others):
+    for o in others:
+        if o.device != t.device:
+            raise BmxError(BMX_E_ARG, f"tensors on {t.device} and {o.device}")
+
+
+def _elsewhere(device):
+    """Whether a call's tensors live on another GPU than the current one (it
+    then runs again with theirs current, on that device's current stream)."""
+    return device.index != _torch().cuda.current_device()
+
+
+def _on_stream(stream, device):
+    """A context in which torch allocates on `stream`, the one that uses the
+    memory (None: the current stream, a context that does nothing)."""
+    torch = _torch()
+    if stream is not None and not isinstance(stream, torch.cuda.Stream):
+        stream = torch.cuda.ExternalStream(stream.cuda_stream, device=device)
+    return torch.cuda.stream(stream)
+
+
+def _empty(stream, device, dtype, *shape):
+    torch = _torch()
+    if stream is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    with _on_stream(stream, device):
+        return torch.empty(shape, dtype=dtype, device=device)
+
+
+def _bf16(*ts):
+    for t in ts:
+        if t.dtype != _T.bfloat16:
+            raise BmxError(BMX_E_ARG, f"bfloat16 tensors expected, got {t.dtype}")
+
+
+def kv4_write(k, v, cache, offset, stream=None):
+    """Quantizes keys and values [n_kv_heads, M, 128] bf16 into cache rows
+    offset .. offset+M-1.  k and v may be strided views with contiguous rows:
+    rows of a bf16 cache, or projection rows seen as
+    x.view(M, n_kv_heads, 128).transpose(0, 1)."""
+    torch = _torch()
+    if _elsewhere(cache.device):
+        with torch.cuda.device(cache.device):
+            return kv4_write(k, v, cache, offset, stream)
+    _same_device(cache.k, k, v)
+    _bf16(k, v)
+    st = []
+    for t in (k, v):
+        if t.dim() != 3 or t.shape != k.shape or t.shape[0] != cache.n_kv_heads:
+            raise BmxError(BMX_E_SHAPE, f"k and v must be [{cache.n_kv_heads}, M, 128], got {tuple(t.shape)}")
+        s0, s1, s2 = t.stride()
+        if s2 != 1:
+            raise BmxError(BMX_E_ARG, "the 128 values of a row must be contiguous")
+        st += [s0 if t.shape[0] > 1 else 0, s1 if t.shape[1] > 1 else 0]
+    call("bmx_kv4_write", k.data_ptr(), st[0], st[1], v.data_ptr(), st[2], st[3], cache._ref, k.shape[1], k.shape[2],
+         offset, _stream(stream))
+
+
+def kv4_read(cache, start, stop, stream=None):
+    """Cache rows [start, stop) as bf16 (k, v), each [n_kv_heads, stop - start, 128]."""
+    torch = _torch()
+    if _elsewhere(cache.device):
+        with torch.cuda.device(cache.device):
+            return kv4_read(cache, start, stop, stream)
+    if not 0 <= start <= stop <= cache.capacity:
+        raise BmxError(BMX_E_KV_CAPACITY, f"rows [{start}, {stop}) of capacity {cache.capacity}")
+    M = stop - start
+    k, v = _empty(stream, cache.device, torch.bfloat16, 2, cache.n_kv_heads, M, 128).unbind(0)
+    if M:
+        call("bmx_kv4_read", cache._ref, k.data_ptr(), v.data_ptr(), M, 128, start, _stream(stream))
+    return k, v
+
+
+def qk_norm_rope_kv4(q, k, v, q_norm, k_norm, cache, offset, position=None, eps=1e-6, theta=1e6, stream=None):
+    """qk_norm_rope_kv into a 4-bit cache: raw projection rows q [M, Hq*128],
+    k, v [M, Hkv*128]; the new rows go to cache rows offset .. offset+M-1,
+    rotated for text positions position .. position+M-1 (None: offset; rows
+    and positions differ once rows were evicted).  Returns q_out [Hq, M, 128]."""
+    torch = _torch()
+    if _elsewhere(cache.device):
+        with torch.cuda.device(cache.device):
+            return qk_norm_rope_kv4(q, k, v, q_norm, k_norm, cache, offset, position, eps, theta, stream)
+    _require_cuda(q, k, v, q_norm, k_norm)
+    _same_device(cache.k, q, k, v, q_norm, k_norm)
+    _bf16(q, k, v, q_norm, k_norm)
+    M = q.shape[0]
+    if q.dim() != 2 or q.shape[1] % 128 or k.shape != (M, cache.n_kv_heads * 128) or v.shape != k.shape:
+        raise BmxError(BMX_E_SHAPE, f"q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}: [M, Hq*128] and "
+                                    f"[M, {cache.n_kv_heads}*128] expected")
+    if q_norm.shape != (128,) or k_norm.shape != (128,):
+        raise BmxError(BMX_E_SHAPE, "q_norm and k_norm must hold 128 weights")
+    Hq = q.shape[1] // 128
+    out = _empty(stream, cache.device, torch.bfloat16, Hq, M, 128)
+    call("bmx_qk_norm_rope_kv4", q.data_ptr(), k.data_ptr(), v.data_ptr(), q_norm.data_ptr(), k_norm.data_ptr(),
+         out.data_ptr(), cache._ref, M, Hq, 128, offset, offset if position is None else position, eps, theta,
+         _stream(stream))
+    return out
+
+
+def attention_kv4_workspace(n_heads, n_kv_heads, M, L, weigh=False, device="cuda", stream=None):
+    """A workspace for attention_kv4 calls of M queries that end at row L
+    (weigh: with weights), its counters zeroed.  It serves one call at a time."""
+    torch = _torch()
+    nbytes = load().bmx_attention_kv4_workspace_bytes(n_heads, n_kv_heads, M, L, int(bool(weigh)))
+    if not nbytes:
+        raise BmxError(BMX_E_SHAPE, f"{n_heads} heads over {n_kv_heads}, M={M}, L={L}")
+    with _on_stream(stream, device):
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        ws[:KV4_COUNTER_BYTES].zero_()
+    return ws
+
+
+def attention_kv4(q, cache, offset, scale=None, weights=None, workspace=None, out=None, stream=None):
+    """GQA attention of q [Hq, M, 128] over rows [0, offset + M) of a 4-bit
+    cache, query t seeing rows up to offset + t; returns [M, Hq*128] bf16.
+    weights (fp32 [n_kv_heads, capacity]) has every row's softmax weights, over
+    the queries and the q heads of its kv head, added to it in place.
+    workspace: from attention_kv4_workspace (None: one for this call)."""
+    torch = _torch()
+    if _elsewhere(cache.device):
+        with torch.cuda.device(cache.device):
+            return attention_kv4(q, cache, offset, scale, weights, workspace, out, stream)
+    _require_cuda(q)
+    _same_device(cache.k, q)
+    _bf16(q)
+    if q.dim() != 3 or q.shape[0] == 0 or q.shape[0] % cache.n_kv_heads:
+        raise BmxError(BMX_E_SHAPE, f"q must be [Hq, M, 128] with Hq a multiple of {cache.n_kv_heads}, got "
+                                    f"{tuple(q.shape)}")
+    Hq, M, D = q.shape
+    if weights is not None:
+        _kv4_weights(weights, cache)
+    if out is None:
+        out = _empty(stream, cache.device, torch.bfloat16, M, Hq * D)
+    else:
+        _require_cuda(out)
+        _same_device(cache.k, out)
+        _bf16(out)
+        if out.numel() != M * Hq * D:
+            raise BmxError(BMX_E_SHAPE, f"out must hold [{M}, {Hq * D}], got {tuple(out.shape)}")
+    if M == 0:
+        return out
+    if not 0 <= offset <= cache.capacity - M:
+        raise BmxError(BMX_E_KV_CAPACITY, f"rows {offset} .. {offset + M - 1}, capacity {cache.capacity}")
+    if workspace is None:
+        workspace = attention_kv4_workspace(Hq, cache.n_kv_heads, M, offset + M, weights is not None, cache.device,
+                                            stream)
+    else:
+        _require_cuda(workspace)
+        _same_device(cache.k, workspace)
+    call("bmx_attention_gqa_kv4", q.data_ptr(), cache._ref, out.data_ptr(), _ptr(weights), Hq, M, D, offset,
+         1.0 / D ** 0.5 if scale is None else scale, workspace.data_ptr(),
+         workspace.numel() * workspace.element_size(), _stream(stream))
+    return out
+
+
+def _kv4_weights(w, cache):
+    _require_cuda(w)
+    _same_device(cache.k, w)
+    if w.dtype != _T.float32:
+        raise BmxError(BMX_E_ARG, "weights must be float32")
+    if w.shape != (cache.n_kv_heads, cache.capacity):
+        raise BmxError(BMX_E_SHAPE, f"weights must be {(cache.n_kv_heads, cache.capacity)}, got {tuple(w.shape)}")
+
+
+def kv4_evict(cache, weights, length, budget, sink=4, recent=0, into=None, weights_into=None, kept=None, stream=None):
+    """Cuts `length` cached rows per kv head to `budget`: the first `sink`,
+    the last `recent`, and of those between the ones with the largest weights
+    (attention_kv4's, fp32 [n_kv_heads, capacity]; ties to the lower row), in
+    their old order.  In place, or into another cache `into` with its own
+    weights_into; weights move along, and are zero from `budget` on.
+    Returns kept [n_kv_heads, budget] int32, the rows' old numbers."""
+    torch = _torch()
+    if _elsewhere(cache.device):
+        with torch.cuda.device(cache.device):
+            return kv4_evict(cache, weights, length, budget, sink, recent, into, weights_into, kept, stream)
+    if (into is None) != (weights_into is None):
+        raise BmxError(BMX_E_ARG, "into and weights_into go together")
+    if into is None:
+        into, weights_into = cache, weights
+    _same_device(cache.k, into.k)
+    _kv4_weights(weights, cache)
+    _kv4_weights(weights_into, into)
+    if budget < 1:
+        raise BmxError(BMX_E_SHAPE, f"budget={budget}")
+    if kept is None:
+        kept = _empty(stream, cache.device, torch.int32, cache.n_kv_heads, budget)
+    else:
+        _require_cuda(kept)
+        _same_device(cache.k, kept)
+        if kept.dtype != torch.int32 or kept.shape != (cache.n_kv_heads, budget):
+            raise BmxError(BMX_E_ARG, f"kept must be int32 {(cache.n_kv_heads, budget)}")
+    call("bmx_kv4_evict", cache._ref, weights.data_ptr(), into._ref, weights_into.data_ptr(), kept.data_ptr(), length,
+         budget, sink, recent, 128, _stream(stream))
+    return kept
+
+
+# ---------------------------------------------------------------------------
 # Qwen3 model / KV cache / generation (host mirror of the reference's
 # Qwen3, KvCache, LoadedModel::generate_text and speculative::generate)
 # ---------------------------------------------------------------------------

@@ -262,6 +262,101 @@ int bmx_silu_mul(const bmx_bf16 *gate, const bmx_bf16 *up, bmx_bf16 *y, int64_t 
 int bmx_add(const bmx_bf16 *a, const bmx_bf16 *b, bmx_bf16 *y, int64_t n, void *stream);
 
 /* ------------------------------------------------------------------ */
+/* A KV cache held in 4 bits                                            */
+/* ------------------------------------------------------------------ */
+
+/* One layer's keys and values as MLX affine 4-bit rows of 128 values in two
+ * groups of 64, the format of the quantized weights: k and v
+ * [n_kv_heads, capacity, 16] words of eight nibbles (value d of a row in
+ * bits 4 (d % 8) of word d / 8), scales and biases [n_kv_heads, capacity, 2];
+ * a value is scale * nibble + bias.  144 bytes per row and kv head, K and V
+ * together, where bf16 takes 512.  k and v, all scales and biases: 16-byte
+ * aligned device pointers; the struct itself is host memory, read during the
+ * call.  group_size must be 64 and bits 4 (BMX_E_UNSUPPORTED).  `capacity`
+ * may be up to 2^24 rows (BMX_E_SHAPE).
+ * No counterpart in the reference, whose KvCache is in the activations' type
+ * (crates/base-mlx-core/src/model/qwen3.rs:109-162). */
+typedef struct {
+  uint32_t *k;
+  bmx_bf16 *k_scales, *k_biases;
+  uint32_t *v;
+  bmx_bf16 *v_scales, *v_biases;
+  int n_kv_heads, capacity;
+  int group_size, bits;
+} bmx_kv4;
+
+/* Quantizes M rows of keys and values into cache rows offset .. offset+M-1:
+ * row t of kv head h is the 128 values from k + h * k_head_stride +
+ * t * k_row_stride (v alike; strides in values, multiples of 8, not negative;
+ * k and v 16-byte aligned), so a bf16 cache [n_kv_heads, capacity, 128]
+ * and projection rows [M, n_kv_heads * 128] both serve.  Per group
+ *   bias = min x, scale = bf16((max x - min x) / 15),
+ *   nibble = round((x - bias) / scale) to even, at most 15 (scale 0: 0)
+ * in fp32.  A group that holds a NaN or an infinity, or whose range
+ * overflows fp32, gets NaN for scale and bias.  Rows outside the range stay
+ * as they are; offset + M > capacity returns BMX_E_KV_CAPACITY and writes
+ * nothing; M = 0 is a no-op.
+ * The 4-bit form of the write mlx_ext::slice_update makes
+ * (crates/base-mlx-core/src/model/qwen3.rs:431-489). */
+int bmx_kv4_write(const bmx_bf16 *k, int64_t k_head_stride, int64_t k_row_stride, const bmx_bf16 *v,
+                  int64_t v_head_stride, int64_t v_row_stride, const bmx_kv4 *cache, int M, int head_dim, int offset,
+                  void *stream);
+
+/* Cache rows start .. start+M-1 as bf16: k and v [n_kv_heads, M, 128]
+ * (16-byte aligned), each value as bmx_dequantize_affine gives it. */
+int bmx_kv4_read(const bmx_kv4 *cache, bmx_bf16 *k, bmx_bf16 *v, int M, int head_dim, int start, void *stream);
+
+/* bmx_qk_norm_rope_kv into a 4-bit cache: the normed, rotated keys and the
+ * values of M new tokens go to cache rows offset .. offset+M-1, quantized
+ * as bmx_kv4_write does it (the same bits as the two calls), the queries to
+ * q_out [n_heads, M, 128].  `position` is the first token's position in the
+ * text: it sets the rotation and is not the row once rows have been evicted.
+ * Replaces: the same sequence of Qwen3::forward_internal as
+ *   bmx_qk_norm_rope_kv (crates/base-mlx-core/src/model/qwen3.rs:392-489). */
+int bmx_qk_norm_rope_kv4(const bmx_bf16 *q, const bmx_bf16 *k, const bmx_bf16 *v, const bmx_bf16 *q_norm,
+                         const bmx_bf16 *k_norm, bmx_bf16 *q_out, const bmx_kv4 *cache, int M, int n_heads,
+                         int head_dim, int offset, int64_t position, float eps, float theta, void *stream);
+
+/* bmx_attention_gqa over a 4-bit cache: M queries q [n_heads, M, 128] over
+ * rows 0 .. offset+M-1, out [M, n_heads*128]; query t sees rows
+ * j <= offset + t.  Keys and values enter as scale * nibble + bias without a
+ * rounding to bf16 between.  With `weights` (fp32 [n_kv_heads, capacity], or
+ * NULL) the call also adds to weights[h][j] the softmax weights that row j
+ * drew, over the q heads of kv head h and the M queries; entries past
+ * offset+M-1 stay as they are.  The order of every sum is fixed: equal calls
+ * give equal bits.  `workspace` is as for bmx_attention_gqa (the first
+ * BMX_KV4_COUNTER_BYTES of it zero-filled before its first use; every call
+ * leaves them zero; 16-byte aligned; calls that share one must not run
+ * concurrently) but not optional: bmx_attention_kv4_workspace_bytes for the
+ * call's n_heads, n_kv_heads, M, L = offset + M and weights != NULL, or more
+ * (BMX_E_ARG otherwise, nothing enqueued).  A call of many queries unpacks
+ * the cache to bf16 there once: 512 bytes per row and kv head.
+ * Replaces: mlx_rs::fast::scaled_dot_product_attention as
+ *   bmx_attention_gqa does (crates/base-mlx-core/src/model/qwen3.rs:491-518);
+ *   the reference has no quantized cache and no eviction. */
+#define BMX_KV4_COUNTER_BYTES 65536
+int bmx_attention_gqa_kv4(const bmx_bf16 *q, const bmx_kv4 *cache, bmx_bf16 *out, float *weights, int n_heads, int M,
+                          int head_dim, int offset, float scale, void *workspace, size_t workspace_bytes,
+                          void *stream);
+/* Bytes of workspace bmx_attention_gqa_kv4 needs for offset + M = L (0 for
+ * arguments it would refuse).  Host only. */
+size_t bmx_attention_kv4_workspace_bytes(int n_heads, int n_kv_heads, int M, int L, int weigh);
+
+/* Cuts a cache of `length` rows per kv head down to `budget` (1 <= budget <=
+ * length): each kv head keeps its first `sink` rows, its last `recent` rows
+ * and, of those between, the budget - sink - recent whose weights are
+ * largest (equal weights: the lower row; a NaN counts as larger than any
+ * number), and they become rows 0 .. budget-1 of `into` in their old order.
+ * weights_into [n_kv_heads, into->capacity] gets their weights, and zeros
+ * from `budget` on; kept [n_kv_heads, budget] their old row numbers.
+ * into may be the cache itself (the same struct or equal pointers), and
+ * weights_into weights, both then in place; otherwise nothing of `into` may
+ * overlap the cache.  Rows of `into` from `budget` on stay as they are.
+ * sink, recent >= 0, sink + recent <= budget. */
+int bmx_kv4_evict(const bmx_kv4 *cache, const float *weights, const bmx_kv4 *into, float *weights_into,
+                  int32_t *kept, int length, int budget, int sink, int recent, int head_dim, void *stream);
+
+/* ------------------------------------------------------------------ */
 /* Qwen3 model, KV cache, generation                                   */
 /* ------------------------------------------------------------------ */
 
