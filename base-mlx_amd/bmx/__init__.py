@@ -499,8 +499,9 @@ def qk_norm_rope_kv4(q, k, v, q_norm, k_norm, cache, offset, position=None, eps=
 
 
 def attention_kv4_workspace(n_heads, n_kv_heads, M, L, weigh=False, device="cuda", stream=None):
-    """A workspace for attention_kv4 calls of M queries that end at row L
-    (weigh: with weights), its counters zeroed.  It serves one call at a time."""
+    """A workspace for attention_kv4 calls of up to M queries that end at up
+    to row L (weigh: with weights), its counters zeroed.  It serves one call
+    at a time."""
     torch = _torch()
     nbytes = load().bmx_attention_kv4_workspace_bytes(n_heads, n_kv_heads, M, L, int(bool(weigh)))
     if not nbytes:

@@ -338,8 +338,9 @@ int bmx_qk_norm_rope_kv4(const bmx_bf16 *q, const bmx_bf16 *k, const bmx_bf16 *v
 int bmx_attention_gqa_kv4(const bmx_bf16 *q, const bmx_kv4 *cache, bmx_bf16 *out, float *weights, int n_heads, int M,
                           int head_dim, int offset, float scale, void *workspace, size_t workspace_bytes,
                           void *stream);
-/* Bytes of workspace bmx_attention_gqa_kv4 needs for offset + M = L (0 for
- * arguments it would refuse).  Host only. */
+/* Bytes of workspace that are enough for every bmx_attention_gqa_kv4 call of
+ * these heads with up to M queries and offset + M up to L, with weights if
+ * `weigh` (0 for arguments it would refuse).  Host only. */
 size_t bmx_attention_kv4_workspace_bytes(int n_heads, int n_kv_heads, int M, int L, int weigh);
 
 /* Cuts a cache of `length` rows per kv head down to `budget` (1 <= budget <=

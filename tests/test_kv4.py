@@ -122,6 +122,19 @@ def test_attention_workspace_query_refuses_what_the_call_refuses():
     assert q(65535, 1, 1 << 20, 1 << 24, 0) == 0  # more query rows than one call takes
 
 
+def test_attention_workspace_grows_with_the_call():
+    """One sized for the largest call serves the smaller ones."""
+    q = bmx.load().bmx_attention_kv4_workspace_bytes
+    for hq, hkv in ((32, 8), (6, 2), (300, 150)):
+        for weigh in (0, 1):
+            last = 0
+            for M in (1, 2, 3, 8, 15, 64, 300, 1000, 5000):
+                row = [q(hq, hkv, M, L, weigh) for L in (5000, 5001, 9000, 20000, 200000)]
+                assert row == sorted(row) and row[0] >= last
+                last = row[0]
+            assert q(hq, hkv, 8, 9000, 1) > q(hq, hkv, 8, 9000, 0)
+
+
 def test_evict_refusals():
     f = entry_points(kv4())["evict"]
     for n in ("w", "w_into", "kept"):
