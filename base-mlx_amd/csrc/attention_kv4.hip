@@ -21,6 +21,7 @@
 #include <math.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "kv4.h"
 
@@ -36,6 +37,8 @@ constexpr int kOs = kKv4Dim + 4;           // LDS stride of an output row
 
 typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8_t;
 typedef __attribute__((ext_vector_type(4))) float f32x4_t;
+typedef __attribute__((ext_vector_type(16))) float f32x16_t;
+typedef __attribute__((ext_vector_type(2))) float f32x2_t;
 typedef __attribute__((ext_vector_type(2))) unsigned u32x2_t;
 typedef __attribute__((ext_vector_type(4))) unsigned u32x4_t;
 
@@ -46,7 +49,7 @@ struct Kv4AttnParams {
   float* weights;     // [Hkv, cap], or null
   unsigned* cnt;      // arrival counters, cnt_stride words apart, zero between calls
   float2* lse;        // [Hq, M] (max * c2, log2 of the sum), or null
-  uint4* qp;          // [Hq, M] the three pieces of Q_0 and Q_1, with lse
+  uint4* qp;          // [Hq, M, 17] the queries as the weights' kernel takes them, with lse
   float* part_o;      // [Hq, M, ns, 128]
   float* part_ml;     // [Hq, M, ns, 2]
   int Hq, M, offset;
@@ -60,6 +63,11 @@ struct Kv4AttnParams {
 
 __device__ __forceinline__ f32x4_t mfma(u32x4_t a, u32x4_t b, f32x4_t c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c,
+                                                 0, 0, 0);
+}
+
+__device__ __forceinline__ f32x16_t mfma32(u32x4_t a, u32x4_t b, f32x16_t c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c,
                                                  0, 0, 0);
 }
 
@@ -79,8 +87,8 @@ __device__ __forceinline__ u32x4_t word_pairs(uint32_t w, const PairK& k) {
 }
 __device__ __forceinline__ float lo_f(uint32_t w) { return __uint_as_float(w << 16); }
 __device__ __forceinline__ float hi_f(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
-__device__ __forceinline__ uint32_t pack_bf(float a, float b) {
-  return static_cast<uint32_t>(f2bf(a)) | (static_cast<uint32_t>(f2bf(b)) << 16);
+__device__ __forceinline__ uint32_t pack_bf(float a, float b) {  // one v_cvt_pk_bf16_f32
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2_t{a, b}, bf16x2_t));
 }
 __device__ __forceinline__ uint32_t dpp_ror8(uint32_t v) {
   return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0x128, 0xF, 0xF, false));
@@ -114,6 +122,23 @@ __device__ __forceinline__ float2 load_part(const float* p) {
   return make_float2(__uint_as_float(static_cast<uint32_t>(v)), __uint_as_float(static_cast<uint32_t>(v >> 32)));
 }
 
+// Q_0 and Q_1 of a query row, each in three bf16 pieces that add up to it
+__device__ __forceinline__ u32x4_t q_pieces(const float (&qs)[2]) {
+  const float h0 = round_bf(qs[0]), h1 = round_bf(qs[1]);
+  const float m0 = round_bf(qs[0] - h0), m1 = round_bf(qs[1] - h1);
+  return u32x4_t{pack_bf(h0, h1), pack_bf(m0, m1), pack_bf(qs[0] - h0 - m0, qs[1] - h1 - m1), 0u};
+}
+// ... kept for the weights with the row's fragments, in the order their
+// lanes g take them: 64 bytes per g, then the pieces (17 words of 16 bytes)
+constexpr int kQueryWords = 17;
+__device__ __forceinline__ void store_query(const Kv4AttnParams& p, int64_t row, int g, const u32x4_t (&qf)[2][2],
+                                            const float (&qs)[2]) {
+  u32x4_t* dst = reinterpret_cast<u32x4_t*>(p.qp) + row * kQueryWords;
+#pragma unroll
+  for (int k = 0; k < 4; k++) dst[4 * g + k] = qf[k >> 1][k & 1];
+  if (g == 0) dst[16] = q_pieces(qs);
+}
+
 // One output row's 4 dims, and the row's softmax statistics for the weights.
 __device__ __forceinline__ void finish_row(const Kv4AttnParams& p, int kvh, int r, int d, float4 o, float m, float l) {
   const int rep = p.Hq / p.c.n_kv_heads, t = r % p.M, h = kvh * rep + r / p.M;
@@ -123,7 +148,148 @@ __device__ __forceinline__ void finish_row(const Kv4AttnParams& p, int kvh, int 
   if (p.lse && d == 0) p.lse[static_cast<int64_t>(kvh) * rep * p.M + r] = make_float2(m * p.c2, log2f(l));
 }
 
-// A workgroup of NW waves: one kv head, 16 query rows (row r = j * M + t:
+template <int NW, int ROWS, int NT>
+struct JoinLds {
+  alignas(16) float os[NW][ROWS][kOs];
+  float ms[NW][NT * ROWS], ls[NW][NT * ROWS], wt[NT * ROWS][kMaxSplits], fin[NT * ROWS][2];
+  int last;
+};
+
+// The end of a workgroup: each wave hands in, for rows n * ROWS + li of the
+// tile (lanes li < ROWS), its maximum m and sum l over its keys, and in lane
+// (li, g) the products acc[n][y][nibble][i] of the dims described at the
+// kernel, to which x[n][y] adds.
+template <int NW, int ROWS, int NT>
+__device__ __forceinline__ void join_and_finish(const Kv4AttnParams& p, JoinLds<NW, ROWS, NT>& sm, int kvh, int split,
+                                                int r0, int RT, const float (&ma)[NT], const float (&la)[NT],
+                                                const f32x4_t (&acc)[NT][2][4], const float (&x)[NT][2]) {
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, li = lane & 15, g = lane >> 4;
+  const int64_t row0 = static_cast<int64_t>(kvh) * (p.Hq / p.c.n_kv_heads) * p.M + r0;
+  // ---- the waves' sums joined: weights exp2((m_w - m) c2) ----
+  float m[NT];
+#pragma unroll
+  for (int n = 0; n < NT; n++) {
+    m[n] = la[n] != la[n] ? la[n] : ma[n];  // a NaN score: the row stays NaN
+    if (g == 0 && li < ROWS) {
+      sm.ms[wave][n * ROWS + li] = m[n];
+      sm.ls[wave][n * ROWS + li] = la[n];
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int n = 0; n < NT; n++) {
+    if (n > 0) __syncthreads();  // the rows before have been read
+    if (li < ROWS) {
+      float mm = sm.ms[0][n * ROWS + li];
+#pragma unroll
+      for (int w = 1; w < NW; w++) mm = fmaxf(mm, sm.ms[w][n * ROWS + li]);
+      const float f = m[n] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m[n] - mm) * p.c2);
+#pragma unroll
+      for (int y = 0; y < 2; y++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          const int a = 4 * g + i;  // row of A: word a % 8, half a / 8
+          *reinterpret_cast<float4*>(&sm.os[wave][li][64 * y + 8 * (a & 7) + 4 * (a >> 3)]) =
+              make_float4((acc[n][y][0][i] + x[n][y]) * f, (acc[n][y][1][i] + x[n][y]) * f,
+                          (acc[n][y][2][i] + x[n][y]) * f, (acc[n][y][3][i] + x[n][y]) * f);
+        }
+    }
+    __syncthreads();
+    for (int it = tid; it < min(ROWS, RT - n * ROWS) * 32; it += 64 * NW) {
+      const int rr = it >> 5, r = n * ROWS + rr, d = 4 * (it & 31);
+      float mm = sm.ms[0][r];
+#pragma unroll
+      for (int w = 1; w < NW; w++) mm = fmaxf(mm, sm.ms[w][r]);
+      float sum = 0.0f;
+      float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+      for (int w = 0; w < NW; w++) {
+        const float f = sm.ms[w][r] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((sm.ms[w][r] - mm) * p.c2);
+        sum = __builtin_fmaf(f, sm.ls[w][r], sum);
+        const float4 v = *reinterpret_cast<const float4*>(&sm.os[w][rr][d]);
+        o.x += v.x;
+        o.y += v.y;
+        o.z += v.z;
+        o.w += v.w;
+      }
+      if (sum != sum) mm = sum;
+      if (p.ns == 1) {
+        finish_row(p, kvh, r0 + r, d, o, mm, sum);
+      } else {
+        const int64_t at = (row0 + r) * p.ns + split;
+        store_part(p.part_o + at * kKv4Dim + d, o.x, o.y);
+        store_part(p.part_o + at * kKv4Dim + d + 2, o.z, o.w);
+        if (d == 0) store_part(p.part_ml + at * 2, mm, sum);
+      }
+    }
+  }
+  if (p.ns == 1) return;
+
+  // ---- the last workgroup of a (kv head, row tile) merges its splits ----
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  if (tid == 0) {
+    unsigned* c = p.cnt + (static_cast<int64_t>(blockIdx.z) * gridDim.x + kvh) * p.cnt_stride;
+    const unsigned n = __hip_atomic_fetch_add(c, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    sm.last = n == static_cast<unsigned>(p.ns - 1);
+    if (sm.last) __hip_atomic_store(c, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  __syncthreads();
+  if (!sm.last) return;
+  // a wave per row, a lane per split: the splits' weights
+  for (int r = wave; r < RT; r += NW) {
+    float2 ml = make_float2(-INFINITY, 0.0f);
+    if (lane < p.ns) ml = load_part(p.part_ml + ((row0 + r) * p.ns + lane) * 2);
+    const float mm = max_xor32(max_xor16(row16_max(ml.x)));
+    const float f = ml.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((ml.x - mm) * p.c2);
+    const float sum = lanes_sum(f * ml.y, 64);
+    sm.wt[r][lane] = f;
+    if (lane == 0) {
+      sm.fin[r][0] = mm;
+      sm.fin[r][1] = sum;
+    }
+  }
+  __syncthreads();
+  // (row, 4 dims) per thread, and the splits over as many threads as there are
+  constexpr int kThreads = 64 * NW;
+  const int items = RT * 32, groups = max(1, kThreads / items);
+  const int n = tid / items;  // this thread's group; those past the last have none
+  float* red = &sm.os[0][0][0];
+  for (int it = tid - n * items; it < items && n < groups; it += kThreads) {
+    const int r = it >> 5, d = 4 * (it & 31);
+    const float* src = p.part_o + (row0 + r) * p.ns * kKv4Dim + d;
+    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 8
+    for (int s = n; s < p.ns; s += groups) {
+      const float2 u = load_part(src + static_cast<int64_t>(s) * kKv4Dim);
+      const float2 v = load_part(src + static_cast<int64_t>(s) * kKv4Dim + 2);
+      const float f = sm.wt[r][s];
+      o.x = __builtin_fmaf(f, u.x, o.x);
+      o.y = __builtin_fmaf(f, u.y, o.y);
+      o.z = __builtin_fmaf(f, v.x, o.z);
+      o.w = __builtin_fmaf(f, v.y, o.w);
+    }
+    if (groups == 1)
+      finish_row(p, kvh, r0 + r, d, o, sm.fin[r][0], sm.fin[r][1]);
+    else
+      *reinterpret_cast<float4*>(&red[(n * items + it) * 4]) = o;
+  }
+  if (groups == 1) return;
+  __syncthreads();
+  for (int it = tid; it < items; it += kThreads) {
+    float4 o = *reinterpret_cast<const float4*>(&red[it * 4]);
+    for (int k = 1; k < groups; k++) {
+      const float4 v = *reinterpret_cast<const float4*>(&red[(k * items + it) * 4]);
+      o.x += v.x;
+      o.y += v.y;
+      o.z += v.z;
+      o.w += v.w;
+    }
+    finish_row(p, kvh, r0 + (it >> 5), 4 * (it & 31), o, sm.fin[it >> 5][0], sm.fin[it >> 5][1]);
+  }
+}
+
+// A workgroup of NW waves: one kv head, 16 NT query rows (row r = j * M + t:
 // head kvh * rep + j, token t), one split of the keys; a wave takes 32 keys
 // a step, with its own running maximum and sums.
 //   Lanes: li = lane % 16, g = lane / 16.
@@ -137,17 +303,19 @@ __device__ __forceinline__ void finish_row(const Kv4AttnParams& p, int kvh, int 
 //     4 (li / 8) + i.  Lane li < 8 loads a word of the even key of a pair,
 //     lane li + 8 the same word of the odd key, and they swap halves.
 // The next step's K is loaded once the scores are done, its V once P V is.
-template <int NW>
-__global__ void __launch_bounds__(64 * NW) kv4_split_kernel(const Kv4AttnParams p) {
-  __shared__ __align__(16) float os[NW][kRows][kOs];
-  __shared__ float ms[NW][kRows], ls[NW][kRows], wt[kRows][kMaxSplits], fin[kRows][2];
-  __shared__ int last;
+// Bound by the VALU: per step about 180 instructions for the nibbles and
+// scales, which NT row tiles share, and 110 per tile.
+template <int NW, int NT>
+__global__ void __launch_bounds__(64 * NW) kv4_rows_kernel(const Kv4AttnParams p) {
+  __shared__ JoinLds<NW, kRows, NT> sm;
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, li = lane & 15, g = lane >> 4;
-  const int kvh = blockIdx.x, split = blockIdx.y, r0 = blockIdx.z * kRows;
-  const int M = p.M, R = p.Hq / p.c.n_kv_heads * M, RT = min(kRows, R - r0), L = p.offset + M;
+  const int kvh = blockIdx.x, split = blockIdx.y, r0 = blockIdx.z * (NT * kRows);
+  const int M = p.M, R = p.Hq / p.c.n_kv_heads * M, RT = min(NT * kRows, R - r0), L = p.offset + M;
   const int64_t row0 = static_cast<int64_t>(kvh) * R + r0;
-  // rows' tokens: query li sees keys < lim; the tile's first and last token
-  const int lim = p.offset + (r0 + min(li, RT - 1)) % M + 1;
+  // rows' tokens: a query sees keys < lim; the tile's first and last token
+  int lim[NT];
+#pragma unroll
+  for (int n = 0; n < NT; n++) lim[n] = p.offset + (r0 + min(n * kRows + li, RT - 1)) % M + 1;
   const int t0 = r0 % M, tmin = t0 + RT > M ? 0 : t0, tmax = t0 + RT > M ? M - 1 : t0 + RT - 1;
   const int all_see = p.offset + tmin + 1, kend = p.offset + tmax + 1;
   const PairK nk;
@@ -194,12 +362,15 @@ __global__ void __launch_bounds__(64 * NW) kv4_split_kernel(const Kv4AttnParams 
   load_k(b);
   load_v(b);
 
-  // ---- the query fragments, in the pair order of a word, and their sums ----
-  u32x4_t qf[2][2];
-  f32x4_t start[2];  // -16 Q_y of query li
-  u32x4_t qp;        // lanes g = 0: Q_0, Q_1 in three bf16 pieces each
-  {
-    const uint16_t* qr = p.q + (row0 + min(li, RT - 1)) * kKv4Dim + 16 * g;
+  // ---- the query fragments, in the pair order of a word, and their sums;
+  // two row tiles' fragments would not fit the registers next to the rest
+  // (94 spilled), so every wave reads them from LDS each step ----
+  __shared__ u32x4_t ql[NT][5][64];
+  float start[NT][2];  // -16 Q_y of the query
+#pragma unroll
+  for (int n = 0; n < NT; n++) {
+    const uint16_t* qr = p.q + (row0 + min(n * kRows + li, RT - 1)) * kKv4Dim + 16 * g;
+    u32x4_t qf[2][2];
     float qs[2];
 #pragma unroll
     for (int y = 0; y < 2; y++) {
@@ -216,97 +387,82 @@ __global__ void __launch_bounds__(64 * NW) kv4_split_kernel(const Kv4AttnParams 
         qf[y][e] = u32x4_t{d.x, d.y, d.z, d.w};
       }
       qs[y] = add_xor32(add_xor16(qs[y]));
-      start[y] = f32x4_t{-16.0f, -16.0f, -16.0f, -16.0f} * qs[y];
+      start[n][y] = -16.0f * qs[y];
     }
-    const float h0 = round_bf(qs[0]), h1 = round_bf(qs[1]);
-    const float m0 = round_bf(qs[0] - h0), m1 = round_bf(qs[1] - h1);
-    qp = u32x4_t{pack_bf(h0, h1), pack_bf(m0, m1), pack_bf(qs[0] - h0 - m0, qs[1] - h1 - m1), 0u};
-    if (p.qp && split == 0 && wave == 0 && g == 0 && li < RT) p.qp[row0 + li] = make_uint4(qp.x, qp.y, qp.z, 0u);
-    if (g != 0) qp = u32x4_t{0u, 0u, 0u, 0u};
+    if (p.qp && split == 0 && wave == 0 && n * kRows + li < RT) store_query(p, row0 + n * kRows + li, g, qf, qs);
+    if (wave == 0) {
+      u32x4_t pieces = q_pieces(qs);  // Q_0, Q_1 in three bf16 pieces each, for lanes g = 0
+      if (g != 0) pieces = u32x4_t{0u, 0u, 0u, 0u};
+#pragma unroll
+      for (int k = 0; k < 4; k++) ql[n][k][lane] = qf[k >> 1][k & 1];
+      ql[n][4][lane] = pieces;
+    }
   }
+  __syncthreads();
 
   const f32x4_t zero = {0.0f, 0.0f, 0.0f, 0.0f};
-  f32x4_t acc[2][4], ones[2], edge = zero;
+  // edge: rows 0, 1 sum p~ b, rows 2, 3 sum p~ s, rows 4, 5 -23.5 sum p', of
+  // groups 0 and 1
+  f32x4_t acc[NT][2][4], edge[NT];
+  float m[NT], l[NT], slow[NT][2];
 #pragma unroll
-  for (int y = 0; y < 2; y++) {
-    ones[y] = zero;
+  for (int n = 0; n < NT; n++) {
+    edge[n] = zero;
+    m[n] = -INFINITY;
+    l[n] = slow[n][0] = slow[n][1] = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 4; i++) acc[y][i] = zero;
+    for (int y = 0; y < 2; y++)
+#pragma unroll
+      for (int i = 0; i < 4; i++) acc[n][y][i] = zero;
   }
-  float m = -INFINITY, l = 0.0f, slow[2] = {0.0f, 0.0f};
-  constexpr uint32_t kCentre = 0xC1BCC1BCu;  // bf16 -23.5 twice
+  const uint32_t centre[2] = {li == 4 ? 0xC1BCC1BCu : 0u, li == 5 ? 0xC1BCC1BCu : 0u};  // bf16 -23.5 twice
   const uint32_t half_sel = li < 8 ? 0x01000504u : 0x07060302u;
-  const uint32_t odd_sel = li & 1 ? 0x07060302u : 0x05040100u;
+  // (selector 0x0c gives a zero byte: rows from 4 on take nothing)
+  const uint32_t odd_sel = li >= 4 ? 0x0c0c0c0cu : li & 1 ? 0x07060302u : 0x05040100u;
 
-  for (; b < b_end; b += NW) {
+  auto step = [&](auto cut_) {
+    constexpr bool cut = decltype(cut_)::value;  // some row does not see some key
+    asm volatile("" ::: "memory");  // (the fragments stay in LDS: not moved out of the loop)
     // ---- scores ----
-    float sc[8];
+    float sc[NT][8];
 #pragma unroll
     for (int t = 0; t < 2; t++) {
-      f32x4_t d0 = start[0], d1 = start[1];
-      d0 = mfma(word_pairs(kw[t][0].x, nk), qf[0][0], d0);
-      d1 = mfma(word_pairs(kw[t][1].x, nk), qf[1][0], d1);
-      d0 = mfma(word_pairs(kw[t][0].y, nk), qf[0][1], d0);
-      d1 = mfma(word_pairs(kw[t][1].y, nk), qf[1][1], d1);
-      const f32x4_t db = mfma(u32x4_t{kb[t], kb[t], kb[t], kb[t]}, qp, zero);
+      f32x4_t d0[NT], d1[NT], db[NT];
 #pragma unroll
-      for (int i = 0; i < 4; i++)
-        sc[4 * t + i] =
-            __builtin_fmaf(lo_f(ks[t][i]), d0[i], __builtin_fmaf(hi_f(ks[t][i]), d1[i], db[i]));
-    }
-    load_k(b + NW);
-    // ---- running softmax: the maximum over all keys of query li ----
-    const int key0 = b * kKeys + 4 * g;
-    const bool cut = b * kKeys + kKeys > all_see;  // uniform: some row does not see some key
-    if (cut) {
+      for (int n = 0; n < NT; n++) {
+        d0[n] = f32x4_t{start[n][0], start[n][0], start[n][0], start[n][0]};
+        d1[n] = f32x4_t{start[n][1], start[n][1], start[n][1], start[n][1]};
+      }
 #pragma unroll
-      for (int e = 0; e < 8; e++)
-        if (key0 + (e & 3) + 16 * (e >> 2) >= lim) sc[e] = -INFINITY;
-    }
-    float bm = sc[0];
+      for (int e = 0; e < 2; e++) {
+        const u32x4_t a0 = word_pairs(kw[t][0][e], nk), a1 = word_pairs(kw[t][1][e], nk);
 #pragma unroll
-    for (int e = 1; e < 8; e++) bm = fmaxf(bm, sc[e]);
-    bm = max_xor32(max_xor16(bm));
-    if (__any(bm > m)) {
-      const float mn = fmaxf(m, bm);
-      const float a = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - mn) * p.c2);
-      m = mn;
-      l *= a;
-      edge *= a;
+        for (int n = 0; n < NT; n++) {
+          d0[n] = mfma(a0, ql[n][e][lane], d0[n]);
+          d1[n] = mfma(a1, ql[n][2 + e][lane], d1[n]);
+        }
+      }
 #pragma unroll
-      for (int y = 0; y < 2; y++) {
-        slow[y] *= a;
-        ones[y] *= a;
+      for (int n = 0; n < NT; n++) db[n] = mfma(u32x4_t{kb[t], kb[t], kb[t], kb[t]}, ql[n][4][lane], zero);
 #pragma unroll
-        for (int i = 0; i < 4; i++) acc[y][i] *= a;
+      for (int i = 0; i < 4; i++) {
+        const float s0 = lo_f(ks[t][i]), s1 = hi_f(ks[t][i]);
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+          sc[n][4 * t + i] = __builtin_fmaf(s0, d0[n][i], __builtin_fmaf(s1, d1[n][i], db[n][i]));
       }
     }
-    const float mc = m == -INFINITY ? 0.0f : m * p.c2;
-    float pr[8];
-#pragma unroll
-    for (int e = 0; e < 8; e++) pr[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[e], p.c2, -mc));
-    if (cut) {
-#pragma unroll
-      for (int e = 0; e < 8; e++)
-        if (key0 + (e & 3) + 16 * (e >> 2) >= lim) pr[e] = 0.0f;
-    }
-    l += ((pr[0] + pr[1]) + (pr[2] + pr[3])) + ((pr[4] + pr[5]) + (pr[6] + pr[7]));
-    // ---- P V ----
-    float ps[2][8];
-    uint32_t sw[8];
-#pragma unroll
-    for (int e = 0; e < 8; e++) {
-      sw[e] = vs[e >> 2][e & 3];
-      ps[0][e] = pr[e] * lo_f(sw[e]);
-      ps[1][e] = pr[e] * hi_f(sw[e]);
-    }
+    load_k(b + NW);
+    // ---- running softmax: the maximum over all keys of a query ----
+    const int key0 = b * kKeys + 4 * g;
+    u32x4_t pb[NT][2], pt[NT];
     bool odd = false;
-    if (cut) {
+    u32x4_t bw[2];
+    if constexpr (cut) {
       // rows that a query does not see weigh nothing in it, whatever their
       // scales and biases are: its P V column has zeros for them, and biases
       // that are not finite go to the lanes' own sums of the rows that see
       // them, not into the product that every query shares
-      u32x4_t bw[2];
 #pragma unroll
       for (int t = 0; t < 2; t++) {
         bw[t] = load4(vbr, key0 * 4 + t * 64);
@@ -317,41 +473,75 @@ __global__ void __launch_bounds__(64 * NW) kv4_split_kernel(const Kv4AttnParams 
         }
       }
       odd = __any(odd);
+    }
 #pragma unroll
-      for (int e = 0; e < 8; e++) {
-        const bool seen = key0 + (e & 3) + 16 * (e >> 2) < lim;
-        if (!seen) ps[0][e] = ps[1][e] = 0.0f;
-        if (odd && seen) {
-          slow[0] += lo_f(bw[e >> 2][e & 3]) * 0.0f;  // 0 or NaN
-          slow[1] += hi_f(bw[e >> 2][e & 3]) * 0.0f;
+    for (int n = 0; n < NT; n++) {
+      if constexpr (cut) {
+#pragma unroll
+        for (int e = 0; e < 8; e++)
+          if (key0 + (e & 3) + 16 * (e >> 2) >= lim[n]) sc[n][e] = -INFINITY;
+      }
+      float bm = sc[n][0];
+#pragma unroll
+      for (int e = 1; e < 8; e++) bm = fmaxf(bm, sc[n][e]);
+      bm = max_xor32(max_xor16(bm));
+      if (__any(bm > m[n])) {
+        const float mn = fmaxf(m[n], bm);
+        const float a = m[n] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m[n] - mn) * p.c2);
+        m[n] = mn;
+        l[n] *= a;
+        edge[n] *= a;
+#pragma unroll
+        for (int y = 0; y < 2; y++) {
+          slow[n][y] *= a;
+#pragma unroll
+          for (int i = 0; i < 4; i++) acc[n][y][i] *= a;
         }
       }
-    }
-    u32x4_t pb[2], pt;
+      const float mc = m[n] == -INFINITY ? 0.0f : m[n] * p.c2;
+      float pr[8], ps[2][8];
 #pragma unroll
-    for (int j = 0; j < 4; j++) {
-      pb[0][j] = pack_bf(ps[0][2 * j], ps[0][2 * j + 1]);
-      pb[1][j] = pack_bf(ps[1][2 * j], ps[1][2 * j + 1]);
-      pt[j] = pack_bf(pr[2 * j], pr[2 * j + 1]);
+      for (int e = 0; e < 8; e++) {
+        pr[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[n][e], p.c2, -mc));
+        ps[0][e] = pr[e] * lo_f(vs[e >> 2][e & 3]);
+        ps[1][e] = pr[e] * hi_f(vs[e >> 2][e & 3]);
+        if constexpr (cut) {
+          const bool seen = key0 + (e & 3) + 16 * (e >> 2) < lim[n];
+          if (!seen) pr[e] = ps[0][e] = ps[1][e] = 0.0f;
+          if (odd && seen) {
+            slow[n][0] += lo_f(bw[e >> 2][e & 3]) * 0.0f;  // 0 or NaN
+            slow[n][1] += hi_f(bw[e >> 2][e & 3]) * 0.0f;
+          }
+        }
+      }
+      l[n] += ((pr[0] + pr[1]) + (pr[2] + pr[3])) + ((pr[4] + pr[5]) + (pr[6] + pr[7]));
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        pb[n][0][j] = pack_bf(ps[0][2 * j], ps[0][2 * j + 1]);
+        pb[n][1][j] = pack_bf(ps[1][2 * j], ps[1][2 * j + 1]);
+        pt[n][j] = pack_bf(pr[2 * j], pr[2 * j + 1]);
+      }
     }
+    // ---- P V ----
 #pragma unroll
     for (int y = 0; y < 2; y++) {
       uint32_t v[4];
 #pragma unroll
       for (int j = 0; j < 4; j++) v[j] = __builtin_amdgcn_perm(vw[y][j], dpp_ror8(vw[y][j]), half_sel);
-      acc[y][0] = mfma(u32x4_t{nibble_pair<0>(v[0], nk), nibble_pair<0>(v[1], nk), nibble_pair<0>(v[2], nk),
-                               nibble_pair<0>(v[3], nk)}, pb[y], acc[y][0]);
-      acc[y][1] = mfma(u32x4_t{nibble_pair<1>(v[0], nk), nibble_pair<1>(v[1], nk), nibble_pair<1>(v[2], nk),
-                               nibble_pair<1>(v[3], nk)}, pb[y], acc[y][1]);
-      acc[y][2] = mfma(u32x4_t{nibble_pair<2>(v[0], nk), nibble_pair<2>(v[1], nk), nibble_pair<2>(v[2], nk),
-                               nibble_pair<2>(v[3], nk)}, pb[y], acc[y][2]);
-      acc[y][3] = mfma(u32x4_t{nibble_pair<3>(v[0], nk), nibble_pair<3>(v[1], nk), nibble_pair<3>(v[2], nk),
-                               nibble_pair<3>(v[3], nk)}, pb[y], acc[y][3]);
-      ones[y] = mfma(u32x4_t{kCentre, kCentre, kCentre, kCentre}, pb[y], ones[y]);
+      const u32x4_t a[4] = {
+          {nibble_pair<0>(v[0], nk), nibble_pair<0>(v[1], nk), nibble_pair<0>(v[2], nk), nibble_pair<0>(v[3], nk)},
+          {nibble_pair<1>(v[0], nk), nibble_pair<1>(v[1], nk), nibble_pair<1>(v[2], nk), nibble_pair<1>(v[3], nk)},
+          {nibble_pair<2>(v[0], nk), nibble_pair<2>(v[1], nk), nibble_pair<2>(v[2], nk), nibble_pair<2>(v[3], nk)},
+          {nibble_pair<3>(v[0], nk), nibble_pair<3>(v[1], nk), nibble_pair<3>(v[2], nk), nibble_pair<3>(v[3], nk)}};
+#pragma unroll
+      for (int n = 0; n < NT; n++) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) acc[n][y][i] = mfma(a[i], pb[n][y], acc[n][y][i]);
+        edge[n] = mfma(u32x4_t{centre[y], centre[y], centre[y], centre[y]}, pb[n][y], edge[n]);
+      }
     }
     {
-      // rows 0..3 of A: b_0, b_1, s_0, s_1 of the step's keys (the other
-      // rows' results are not used)
+      // rows 0..3 of A: b_0, b_1, s_0, s_1 of the step's keys
       u32x4_t a;
 #pragma unroll
       for (int j = 0; j < 4; j++) {
@@ -363,138 +553,585 @@ __global__ void __launch_bounds__(64 * NW) kv4_split_kernel(const Kv4AttnParams 
           if ((a[j] & 0x7f800000u) == 0x7f800000u) a[j] &= 0xffffu;
         }
       }
-      edge = mfma(a, pt, edge);
+#pragma unroll
+      for (int n = 0; n < NT; n++) edge[n] = mfma(a, pt[n], edge[n]);
     }
     load_v(b + NW);
-  }
+  };
+  // the steps whose keys every row sees, then the others
+  const int b_full = min(b_end, all_see / kKeys);
+  for (; b < b_full; b += NW) step(std::false_type{});
+  for (; b < b_end; b += NW) step(std::true_type{});
 
-  // ---- the waves' sums joined: weights exp2((m_w - m) c2) ----
-  l = add_xor32(add_xor16(l));
-  if (l != l) m = l;  // a NaN score: the row stays NaN
-  if (g == 0) {
-    ms[wave][li] = m;
-    ls[wave][li] = l;
+  float x[NT][2];  // what every dim of a group gets besides its product
+#pragma unroll
+  for (int n = 0; n < NT; n++) {
+    l[n] = add_xor32(add_xor16(l[n]));
+#pragma unroll
+    for (int y = 0; y < 2; y++)
+      x[n][y] = __shfl(edge[n][y], 16 + li, 64) +
+                __builtin_fmaf(7.5f, __shfl(edge[n][2 + y], li, 64), __shfl(edge[n][y], li, 64)) +
+                add_xor32(add_xor16(slow[n][y]));
   }
-  __syncthreads();
+  join_and_finish<NW, kRows, NT>(p, sm, kvh, split, r0, RT, m, l, acc, x);
+}
+
+// Up to RC = 4 or 8 query rows.  The scores of T = 16 / RC key tiles share one
+// 16 x 16 result: column li is query li % RC over tile li / RC, so a lane
+// holds 4 scores of a step of 16 T keys, for as many keys' scales, where the
+// kernel above would hold 4 T with most of them for no query.  Every tile is
+// multiplied with all 16 columns (the queries RC by RC again) and each lane
+// takes the result of its tile; P goes back as a B operand with zeros where a
+// column's tile is not the product's, two tiles to a product.  The columns of
+// a query are added at the end.  The sums over a lane's own keys that take
+// p', s and b (see the top) are fp32 here.
+// One token over 131072 rows, 32 heads of 8: 44 us with the kernel above.
+template <int RC, int NW>
+__global__ void __launch_bounds__(64 * NW) kv4_few_kernel(const Kv4AttnParams p) {
+  constexpr int T = 16 / RC, kStep = 16 * T;
+  __shared__ JoinLds<NW, RC, 1> sm;
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, li = lane & 15, g = lane >> 4;
+  const int qi = li % RC, blk = li / RC;
+  const int kvh = blockIdx.x, split = blockIdx.y;
+  const int M = p.M, R = p.Hq / p.c.n_kv_heads * M, L = p.offset + M;
+  const int64_t row0 = static_cast<int64_t>(kvh) * R;
+  const int lim = p.offset + min(qi, R - 1) % M + 1;
+  const PairK nk;
+
+  const int64_t slot = static_cast<int64_t>(kvh) * p.c.capacity;
+  const __amdgpu_buffer_rsrc_t kwr = rsrc(p.c.k, slot * kKv4Words, L * 64);
+  const __amdgpu_buffer_rsrc_t vwr = rsrc(p.c.v, slot * kKv4Words, L * 64);
+  const __amdgpu_buffer_rsrc_t ksr = rsrc(reinterpret_cast<const uint32_t*>(p.c.k_scales), slot, L * 4);
+  const __amdgpu_buffer_rsrc_t kbr = rsrc(reinterpret_cast<const uint32_t*>(p.c.k_biases), slot, L * 4);
+  const __amdgpu_buffer_rsrc_t vsr = rsrc(reinterpret_cast<const uint32_t*>(p.c.v_scales), slot, L * 4);
+  const __amdgpu_buffer_rsrc_t vbr = rsrc(reinterpret_cast<const uint32_t*>(p.c.v_biases), slot, L * 4);
+
+  u32x2_t kw[T][2];        // [tile][group]: words of key li
+  uint32_t vw[T / 2][2][4];  // [tile pair][group][key pair]
+  u32x4_t ks, kb, vs, vb;  // the lane's 4 keys: 16 blk + 4g ..
+  auto load_k = [&](int b) {
+    const int w = (b * kStep + li) * 64 + 8 * g, s = (b * kStep + 16 * blk + 4 * g) * 4;
+#pragma unroll
+    for (int t = 0; t < T; t++)
+#pragma unroll
+      for (int y = 0; y < 2; y++) kw[t][y] = load2(kwr, w + t * 1024 + y * 32);
+    ks = load4(ksr, s);
+    kb = load4(kbr, s);
+  };
+  auto load_v = [&](int b) {
+    const int w = (b * kStep + 4 * g + (li >> 3)) * 64 + 4 * (li & 7), s = (b * kStep + 16 * blk + 4 * g) * 4;
+#pragma unroll
+    for (int u = 0; u < T / 2; u++)
+#pragma unroll
+      for (int j = 0; j < 4; j++)
+#pragma unroll
+        for (int y = 0; y < 2; y++)
+          vw[u][y][j] = load1(vwr, w + (32 * u + (j & 1) * 2 + (j >> 1) * 16) * 64 + y * 32);
+    vs = load4(vsr, s);
+    vb = load4(vbr, s);
+  };
+
+  const int b_end = min((L + kStep - 1) / kStep, (split + 1) * p.bps * NW);
+  int b = split * p.bps * NW + wave;
+  load_k(b);
+  load_v(b);
+
+  u32x4_t qf[2][2];
+  float qs[2];  // Q_y of query qi
   {
-    float mm = ms[0][li];
+    const uint16_t* qr = p.q + (row0 + min(qi, R - 1)) * kKv4Dim + 16 * g;
 #pragma unroll
-    for (int w = 1; w < NW; w++) mm = fmaxf(mm, ms[w][li]);
-    const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - mm) * p.c2);
-    float x[2];
+    for (int y = 0; y < 2; y++) {
+      qs[y] = 0.0f;
 #pragma unroll
-    for (int y = 0; y < 2; y++)
-      x[y] = ones[y][0] + __builtin_fmaf(7.5f, __shfl(edge[2 + y], li, 64), __shfl(edge[y], li, 64)) +
-             add_xor32(add_xor16(slow[y]));
+      for (int e = 0; e < 2; e++) {
+        uint4 d = *reinterpret_cast<const uint4*>(qr + 64 * y + 8 * e);
+        d.x ^= p.flip;
+        d.y ^= p.flip;
+        d.z ^= p.flip;
+        d.w ^= p.flip;
+        qs[y] += gemv_unit_sum(d);
+        d = permute_pairs(d);
+        qf[y][e] = u32x4_t{d.x, d.y, d.z, d.w};
+      }
+      qs[y] = add_xor32(add_xor16(qs[y]));
+    }
+    if (p.qp && split == 0 && wave == 0 && li < R) store_query(p, row0 + li, g, qf, qs);
+  }
+  const float st[2] = {-16.0f * qs[0], -16.0f * qs[1]};
+
+  f32x4_t accs[1][2][4], (&acc)[2][4] = accs[0];
 #pragma unroll
-    for (int y = 0; y < 2; y++)
+  for (int y = 0; y < 2; y++)
+#pragma unroll
+    for (int i = 0; i < 4; i++) acc[y][i] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+  float m = -INFINITY, l = 0.0f, add[2] = {0.0f, 0.0f};
+  const uint32_t half_sel = li < 8 ? 0x01000504u : 0x07060302u;
+
+  auto step = [&](auto cut_) {
+    constexpr bool cut = decltype(cut_)::value;
+    f32x4_t d0[T], d1[T];
+#pragma unroll
+    for (int t = 0; t < T; t++) {
+      const f32x4_t s0 = {st[0], st[0], st[0], st[0]}, s1 = {st[1], st[1], st[1], st[1]};
+      d0[t] = mfma(word_pairs(kw[t][0].x, nk), qf[0][0], s0);
+      d1[t] = mfma(word_pairs(kw[t][1].x, nk), qf[1][0], s1);
+      d0[t] = mfma(word_pairs(kw[t][0].y, nk), qf[0][1], d0[t]);
+      d1[t] = mfma(word_pairs(kw[t][1].y, nk), qf[1][1], d1[t]);
+    }
+#pragma unroll
+    for (int n = 1; n < T; n *= 2)  // the lane's tile
+#pragma unroll
+      for (int t = 0; t < T; t += 2 * n)
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          d0[t][i] = blk & n ? d0[t + n][i] : d0[t][i];
+          d1[t][i] = blk & n ? d1[t + n][i] : d1[t][i];
+        }
+    float sc[4], pr[4], ps[2][4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      sc[i] = __builtin_fmaf(lo_f(kb[i]), qs[0], hi_f(kb[i]) * qs[1]);
+      sc[i] = __builtin_fmaf(lo_f(ks[i]), d0[0][i], __builtin_fmaf(hi_f(ks[i]), d1[0][i], sc[i]));
+    }
+    load_k(b + NW);
+    const int key0 = b * kStep + 16 * blk + 4 * g;
+    if constexpr (cut) {
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+        if (key0 + i >= lim) sc[i] = -INFINITY;
+    }
+    float bm = fmaxf(fmaxf(sc[0], sc[1]), fmaxf(sc[2], sc[3]));
+    if constexpr (RC == 4) bm = fmaxf(bm, dpp_f32<0x124>(bm));
+    bm = fmaxf(bm, dpp_f32<0x128>(bm));
+    bm = max_xor32(max_xor16(bm));
+    if (__any(bm > m)) {
+      const float mn = fmaxf(m, bm);
+      const float a = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - mn) * p.c2);
+      m = mn;
+      l *= a;
+#pragma unroll
+      for (int y = 0; y < 2; y++) {
+        add[y] *= a;
+#pragma unroll
+        for (int i = 0; i < 4; i++) acc[y][i] *= a;
+      }
+    }
+    const float mc = m == -INFINITY ? 0.0f : m * p.c2;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      pr[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[i], p.c2, -mc));
+      ps[0][i] = pr[i] * lo_f(vs[i]);
+      ps[1][i] = pr[i] * hi_f(vs[i]);
+    }
+    // rows that a query does not see weigh nothing in it, whatever their
+    // scales and biases are
+    float mid[2][4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      mid[0][i] = __builtin_fmaf(7.5f, ps[0][i], pr[i] * lo_f(vb[i]));
+      mid[1][i] = __builtin_fmaf(7.5f, ps[1][i], pr[i] * hi_f(vb[i]));
+      if constexpr (cut) {
+        if (key0 + i >= lim) pr[i] = ps[0][i] = ps[1][i] = mid[0][i] = mid[1][i] = 0.0f;
+      }
+    }
+    l += (pr[0] + pr[1]) + (pr[2] + pr[3]);
+    uint32_t pb[2][2];
+#pragma unroll
+    for (int y = 0; y < 2; y++) {
+      pb[y][0] = pack_bf(ps[y][0], ps[y][1]);
+      pb[y][1] = pack_bf(ps[y][2], ps[y][3]);
+      const float sum = (lo_f(pb[y][0]) + hi_f(pb[y][0])) + (lo_f(pb[y][1]) + hi_f(pb[y][1]));
+      add[y] += __builtin_fmaf(-23.5f, sum, (mid[y][0] + mid[y][1]) + (mid[y][2] + mid[y][3]));
+    }
+#pragma unroll
+    for (int u = 0; u < T / 2; u++)
+#pragma unroll
+      for (int y = 0; y < 2; y++) {
+        const u32x4_t pv = {blk == 2 * u ? pb[y][0] : 0u, blk == 2 * u ? pb[y][1] : 0u,
+                            blk == 2 * u + 1 ? pb[y][0] : 0u, blk == 2 * u + 1 ? pb[y][1] : 0u};
+        uint32_t v[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) v[j] = __builtin_amdgcn_perm(vw[u][y][j], dpp_ror8(vw[u][y][j]), half_sel);
+        acc[y][0] = mfma(u32x4_t{nibble_pair<0>(v[0], nk), nibble_pair<0>(v[1], nk), nibble_pair<0>(v[2], nk),
+                                 nibble_pair<0>(v[3], nk)}, pv, acc[y][0]);
+        acc[y][1] = mfma(u32x4_t{nibble_pair<1>(v[0], nk), nibble_pair<1>(v[1], nk), nibble_pair<1>(v[2], nk),
+                                 nibble_pair<1>(v[3], nk)}, pv, acc[y][1]);
+        acc[y][2] = mfma(u32x4_t{nibble_pair<2>(v[0], nk), nibble_pair<2>(v[1], nk), nibble_pair<2>(v[2], nk),
+                                 nibble_pair<2>(v[3], nk)}, pv, acc[y][2]);
+        acc[y][3] = mfma(u32x4_t{nibble_pair<3>(v[0], nk), nibble_pair<3>(v[1], nk), nibble_pair<3>(v[2], nk),
+                                 nibble_pair<3>(v[3], nk)}, pv, acc[y][3]);
+      }
+    load_v(b + NW);
+  };
+  const int b_full = min(b_end, (p.offset + 1) / kStep);  // every row sees keys 0 .. offset
+  for (; b < b_full; b += NW) step(std::false_type{});
+  for (; b < b_end; b += NW) step(std::true_type{});
+
+  // the columns of a query together
+  auto columns = [&](float v) {
+    if constexpr (RC == 4) v += dpp_f32<0x124>(v);
+    return v + dpp_f32<0x128>(v);
+  };
+  float xs[1][2], (&x)[2] = xs[0];
+#pragma unroll
+  for (int y = 0; y < 2; y++) {
+    x[y] = add_xor32(add_xor16(columns(add[y])));
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+#pragma unroll
+      for (int e = 0; e < 4; e++) acc[y][i][e] = columns(acc[y][i][e]);
+  }
+  const float ms[1] = {m}, ls[1] = {add_xor32(add_xor16(columns(l)))};
+  join_and_finish<NW, RC, 1>(p, sm, kvh, split, 0, R, ms, ls, accs, xs);
+}
+
+// Many query rows: 32 RW of one kv head per workgroup of 8 waves, wave w with
+// rows 32 (w % RW) ..; the waves that share rows take different key tiles of
+// 32.  An iteration's keys are unpacked once, by all waves, into LDS (two
+// buffers: the next iteration's while this one's are multiplied), so the
+// nibbles cost a row tile 1 / RW of what they cost above.
+//   K as 16 + n in the pair order of a word, [key][128], rows 272 bytes
+//   apart; scores by v_mfma_f32_32x32x16_bf16, transposed: lane (query
+//   l % 32, h = l / 32) holds keys 8 j + 4 h + i.  One more product adds
+//   b_g Q_g - 16 s_g Q_g: its k index runs over biases (lanes h = 0) and
+//   scales (h = 1), each against the three pieces of Q_0 and Q_1.
+//   V as bf16(s n + b), transposed: [dim][key], the keys of a half tile in
+//   the order the score lanes hold them (16 k + 4 h + i, 16 k + 8 + 4 h + i),
+//   so P is its own B operand; 16-byte pieces swizzled by the dim.  Rounding V
+//   (by 2^-8 at most, as a bf16 cache would) saves the two scaled copies of
+//   P and three products a tile.
+// A value that is not finite (its scale or bias is not) goes to LDS as 0 and
+// marks the iteration; the rows that see it become NaN by themselves.
+template <int RW>
+__global__ void __launch_bounds__(512) kv4_tile_kernel(const Kv4AttnParams p) {
+  constexpr int KW = 8 / RW, TPW = RW == 8 ? 2 : 1, KPI = kKeys * KW * TPW;
+  constexpr int W = KPI / 32;     // words of K per thread
+  constexpr int VJ = KPI / 64;    // (quad of keys, half word) jobs of V per thread
+  constexpr int KS = kKv4Dim + 8;
+  struct Stage {
+    alignas(16) uint16_t kt[KPI][KS];
+    alignas(16) uint16_t vt[kKv4Dim][KPI];
+    alignas(16) uint32_t sb[2][KPI];  // K's biases, scales
+  };
+  struct Join {
+    alignas(16) float os[4][kKeys][kOs];
+    float ms[4][kKeys], ls[4][kKeys];
+  };
+  constexpr size_t kLds = sizeof(Stage) * 2 > sizeof(Join) ? sizeof(Stage) * 2 : sizeof(Join);
+  __shared__ __align__(16) char lds[kLds];
+  __shared__ int mark[2];
+  Stage* const st = reinterpret_cast<Stage*>(lds);
+  Join& jn = *reinterpret_cast<Join*>(lds);
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, lr = lane & 31, h = lane >> 5;
+  const int rwi = wave % RW, kwi = wave / RW;
+  const int kvh = blockIdx.x, split = blockIdx.y;
+  const int M = p.M, R = p.Hq / p.c.n_kv_heads * M, L = p.offset + M;
+  const int r0 = blockIdx.z * (kKeys * RW), rw0 = r0 + kKeys * rwi;  // first row of the workgroup, of the wave
+  const int RT = min(kKeys * RW, R - r0), n = min(kKeys, R - rw0);   // their rows (n <= 0: none)
+  const int64_t row0 = static_cast<int64_t>(kvh) * R;
+  const int row = min(rw0 + lr, R - 1);
+  const int lim = p.offset + row % M + 1;
+  int all_see = 0, kend = 0;  // keys that every row, any row of the wave sees
+  if (n > 0) {
+    const int t0 = rw0 % M;
+    all_see = p.offset + (t0 + n > M ? 0 : t0) + 1;
+    kend = p.offset + (t0 + n > M ? M - 1 : t0 + n - 1) + 1;
+  }
+  const int tw = r0 % M, kend_wg = p.offset + (tw + RT > M ? M - 1 : tw + RT - 1) + 1;
+  const PairK nk;
+
+  const int64_t slot = static_cast<int64_t>(kvh) * p.c.capacity;
+  const __amdgpu_buffer_rsrc_t kwr = rsrc(p.c.k, slot * kKv4Words, L * 64);
+  const __amdgpu_buffer_rsrc_t vwr = rsrc(p.c.v, slot * kKv4Words, L * 64);
+  const __amdgpu_buffer_rsrc_t ksr = rsrc(reinterpret_cast<const uint32_t*>(p.c.k_scales), slot, L * 4);
+  const __amdgpu_buffer_rsrc_t kbr = rsrc(reinterpret_cast<const uint32_t*>(p.c.k_biases), slot, L * 4);
+  const __amdgpu_buffer_rsrc_t vsr = rsrc(reinterpret_cast<const uint32_t*>(p.c.v_scales), slot, L * 4);
+  const __amdgpu_buffer_rsrc_t vbr = rsrc(reinterpret_cast<const uint32_t*>(p.c.v_biases), slot, L * 4);
+
+  // ---- staging: this thread's part of an iteration ----
+  uint32_t gk[W], gsb = 0;
+  uint32_t gv[VJ][4];
+  u32x4_t gs[VJ], gb[VJ];
+  const int k_key = tid / (16 / W), k_word = W * (tid % (16 / W));
+  auto fetch = [&](int it) {
+    const int key0 = it * KPI;
+    if constexpr (W == 2) {
+      const u32x2_t w = load2(kwr, (key0 + k_key) * 64 + 4 * k_word);
+      gk[0] = w.x;
+      gk[1] = w.y;
+    } else {
+      const u32x4_t w = load4(kwr, (key0 + k_key) * 64 + 4 * k_word);
+#pragma unroll
+      for (int i = 0; i < W; i++) gk[i] = w[i];
+    }
+    if (tid < 2 * KPI) gsb = tid < KPI ? load1(kbr, (key0 + tid) * 4) : load1(ksr, (key0 + tid - KPI) * 4);
+#pragma unroll
+    for (int v = 0; v < VJ; v++) {
+      const int job = tid + 512 * v, hw = job & 31, quad = job >> 5;
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+        gv[v][i] = __builtin_amdgcn_raw_buffer_load_b16(vwr, (key0 + 4 * quad + i) * 64 + 2 * hw, 0, 0);
+      gs[v] = load4(vsr, (key0 + 4 * quad) * 4);
+      gb[v] = load4(vbr, (key0 + 4 * quad) * 4);
+    }
+  };
+  auto stage = [&](int it, int buf) {
+    Stage& s = st[buf];
+#pragma unroll
+    for (int i = 0; i < W; i++)
+      *reinterpret_cast<u32x4_t*>(&s.kt[k_key][8 * (k_word + i)]) = word_pairs(gk[i], nk);
+    if (tid < 2 * KPI) (&s.sb[0][0])[tid] = gsb;
+#pragma unroll
+    for (int v = 0; v < VJ; v++) {
+      const int job = tid + 512 * v, hw = job & 31, quad = job >> 5;
+      const int r = quad & 7, pair = 4 * (quad >> 3) + 2 * (r >> 2) + (r & 1);
+      float sv[4], cv[4];
+      bool bad = false;
 #pragma unroll
       for (int i = 0; i < 4; i++) {
-        const int a = 4 * g + i;  // row of A: word a % 8, half a / 8
-        *reinterpret_cast<float4*>(&os[wave][li][64 * y + 8 * (a & 7) + 4 * (a >> 3)]) =
-            make_float4((acc[y][0][i] + x[y]) * f, (acc[y][1][i] + x[y]) * f, (acc[y][2][i] + x[y]) * f,
-                        (acc[y][3][i] + x[y]) * f);
+        sv[i] = hw < 16 ? lo_f(gs[v][i]) : hi_f(gs[v][i]);
+        const float b = hw < 16 ? lo_f(gb[v][i]) : hi_f(gb[v][i]);
+        cv[i] = __builtin_fmaf(-16.0f, sv[i], b);
+        if (!(__builtin_fmaf(15.0f, fabsf(sv[i]), fabsf(b)) <= 3.402823466e38f)) {
+          bad = true;
+          sv[i] = cv[i] = 0.0f;
+        }
       }
-  }
-  __syncthreads();
-  for (int it = tid; it < RT * 32; it += 64 * NW) {
-    const int r = it >> 5, d = 4 * (it & 31);
-    float mm = ms[0][r];
+      if (bad) atomicMax(&mark[buf], it + 1);
+      const uint32_t p01 = gv[v][0] | (gv[v][1] << 16), p23 = gv[v][2] | (gv[v][3] << 16);
+      const uint32_t a[4] = {nibble_pair<0>(p01, nk), nibble_pair<1>(p01, nk), nibble_pair<2>(p01, nk),
+                             nibble_pair<3>(p01, nk)};
+      const uint32_t b[4] = {nibble_pair<0>(p23, nk), nibble_pair<1>(p23, nk), nibble_pair<2>(p23, nk),
+                             nibble_pair<3>(p23, nk)};
 #pragma unroll
-    for (int w = 1; w < NW; w++) mm = fmaxf(mm, ms[w][r]);
-    float sum = 0.0f;
-    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-    for (int w = 0; w < NW; w++) {
-      const float f = ms[w][r] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((ms[w][r] - mm) * p.c2);
-      sum = __builtin_fmaf(f, ls[w][r], sum);
-      const float4 v = *reinterpret_cast<const float4*>(&os[w][r][d]);
-      o.x += v.x;
-      o.y += v.y;
-      o.z += v.z;
-      o.w += v.w;
+      for (int i = 0; i < 4; i++)
+        *reinterpret_cast<u32x2_t*>(&s.vt[4 * hw + i][((pair ^ (hw & 7)) * 2 + ((r >> 1) & 1)) * 4]) =
+            u32x2_t{pack_bf(__builtin_fmaf(sv[0], lo_f(a[i]), cv[0]), __builtin_fmaf(sv[1], hi_f(a[i]), cv[1])),
+                    pack_bf(__builtin_fmaf(sv[2], lo_f(b[i]), cv[2]), __builtin_fmaf(sv[3], hi_f(b[i]), cv[3]))};
     }
-    if (sum != sum) mm = sum;
-    if (p.ns == 1) {
-      finish_row(p, kvh, r0 + r, d, o, mm, sum);
-    } else {
-      const int64_t at = (row0 + r) * p.ns + split;
-      store_part(p.part_o + at * kKv4Dim + d, o.x, o.y);
-      store_part(p.part_o + at * kKv4Dim + d + 2, o.z, o.w);
-      if (d == 0) store_part(p.part_ml + at * 2, mm, sum);
-    }
-  }
-  if (p.ns == 1) return;
+  };
 
-  // ---- the last workgroup of a (kv head, row tile) merges its splits ----
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-  __syncthreads();
-  if (tid == 0) {
-    unsigned* c = p.cnt + (static_cast<int64_t>(blockIdx.z) * gridDim.x + kvh) * p.cnt_stride;
-    const unsigned n = __hip_atomic_fetch_add(c, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    last = n == static_cast<unsigned>(p.ns - 1);
-    if (last) __hip_atomic_store(c, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  }
-  __syncthreads();
-  if (!last) return;
-  // a wave per row, a lane per split: the splits' weights
-  for (int r = wave; r < RT; r += NW) {
-    float2 ml = make_float2(-INFINITY, 0.0f);
-    if (lane < p.ns) ml = load_part(p.part_ml + ((row0 + r) * p.ns + lane) * 2);
-    const float mm = max_xor32(max_xor16(row16_max(ml.x)));
-    const float f = ml.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((ml.x - mm) * p.c2);
-    const float sum = lanes_sum(f * ml.y, 64);
-    wt[r][lane] = f;
-    if (lane == 0) {
-      fin[r][0] = mm;
-      fin[r][1] = sum;
+  const int iters = (kend_wg + KPI - 1) / KPI;
+  const int it0 = split * p.bps, it1 = min(iters, it0 + p.bps);
+  if (tid < 2) mark[tid] = 0;
+  if (it0 < it1) fetch(it0);
+
+  // ---- the query fragments: word 2 k + h of step k, in its pair order ----
+  u32x4_t qf[8], pieces;
+  {
+    const uint16_t* qr = p.q + (row0 + row) * kKv4Dim + 8 * h;
+    float qs[2];
+#pragma unroll
+    for (int y = 0; y < 2; y++) {
+      qs[y] = 0.0f;
+#pragma unroll
+      for (int k = 0; k < 4; k++) {
+        uint4 d = *reinterpret_cast<const uint4*>(qr + 64 * y + 16 * k);
+        d.x ^= p.flip;
+        d.y ^= p.flip;
+        d.z ^= p.flip;
+        d.w ^= p.flip;
+        qs[y] += gemv_unit_sum(d);
+        d = permute_pairs(d);
+        qf[4 * y + k] = u32x4_t{d.x, d.y, d.z, d.w};
+      }
+      qs[y] = add_xor32(qs[y]);
     }
+    if (p.qp && split == 0 && kwi == 0 && lr < n) {
+      u32x4_t* dst = reinterpret_cast<u32x4_t*>(p.qp) + (row0 + row) * kQueryWords;
+#pragma unroll
+      for (int k = 0; k < 8; k++) dst[4 * (k & 3) + 2 * (k >> 2) + h] = qf[k];
+      if (h == 0) dst[16] = q_pieces(qs);
+    }
+    const float f = h ? -16.0f : 1.0f, qh[2] = {f * qs[0], f * qs[1]};
+    pieces = q_pieces(qh);
   }
-  __syncthreads();
-  // (row, 4 dims) per thread, and the splits over as many threads as there are
-  constexpr int kThreads = 64 * NW;
-  const int items = RT * 32, groups = max(1, kThreads / items);
-  const int n = tid / items;  // this thread's group; those past the last have none
-  float* red = &os[0][0][0];
-  for (int it = tid - n * items; it < items && n < groups; it += kThreads) {
-    const int r = it >> 5, d = 4 * (it & 31);
-    const float* src = p.part_o + (row0 + r) * p.ns * kKv4Dim + d;
-    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 8
-    for (int s = n; s < p.ns; s += groups) {
-      const float2 u = load_part(src + static_cast<int64_t>(s) * kKv4Dim);
-      const float2 v = load_part(src + static_cast<int64_t>(s) * kKv4Dim + 2);
-      const float f = wt[r][s];
-      if (f != 0.0f) {
-        o.x = __builtin_fmaf(f, u.x, o.x);
-        o.y = __builtin_fmaf(f, u.y, o.y);
-        o.z = __builtin_fmaf(f, v.x, o.z);
-        o.w = __builtin_fmaf(f, v.y, o.w);
+
+  f32x16_t acc[4];
+#pragma unroll
+  for (int d = 0; d < 4; d++)
+#pragma unroll
+    for (int i = 0; i < 16; i++) acc[d][i] = 0.0f;
+  float m = -INFINITY, l = 0.0f, poison[2] = {0.0f, 0.0f};
+
+  auto multiply = [&](int it, int buf, int tile) {
+    const Stage& s = st[buf];
+    const int key0 = it * KPI + kKeys * tile, kl = kKeys * tile;
+    if (key0 >= kend) return;  // uniform in the wave
+    f32x16_t d0, d1, db;
+#pragma unroll
+    for (int i = 0; i < 16; i++) d0[i] = d1[i] = db[i] = 0.0f;
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+      d0 = mfma32(*reinterpret_cast<const u32x4_t*>(&s.kt[kl + lr][8 * (2 * k + h)]), qf[k], d0);
+      d1 = mfma32(*reinterpret_cast<const u32x4_t*>(&s.kt[kl + lr][8 * (2 * k + 8 + h)]), qf[4 + k], d1);
+    }
+    const uint32_t w = s.sb[h][kl + lr];
+    db = mfma32(u32x4_t{w, w, w, w}, pieces, db);
+    float sc[16];
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      const u32x4_t s4 = *reinterpret_cast<const u32x4_t*>(&s.sb[1][kl + 8 * j + 4 * h]);
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+        sc[4 * j + i] =
+            __builtin_fmaf(lo_f(s4[i]), d0[4 * j + i], __builtin_fmaf(hi_f(s4[i]), d1[4 * j + i], db[4 * j + i]));
+    }
+    const bool cut = key0 + kKeys > all_see;
+    if (cut) {
+#pragma unroll
+      for (int e = 0; e < 16; e++)
+        if (key0 + 8 * (e >> 2) + 4 * h + (e & 3) >= lim) sc[e] = -INFINITY;
+    }
+    float bm = sc[0];
+#pragma unroll
+    for (int e = 1; e < 16; e++) bm = fmaxf(bm, sc[e]);
+    bm = max_xor32(bm);
+    if (__any(bm > m)) {
+      const float mn = fmaxf(m, bm);
+      const float a = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - mn) * p.c2);
+      m = mn;
+      l *= a;
+#pragma unroll
+      for (int d = 0; d < 4; d++) acc[d] *= a;
+    }
+    const float mc = m == -INFINITY ? 0.0f : m * p.c2;
+#pragma unroll
+    for (int e = 0; e < 16; e++) sc[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[e], p.c2, -mc));
+    if (cut) {
+#pragma unroll
+      for (int e = 0; e < 16; e++)
+        if (key0 + 8 * (e >> 2) + 4 * h + (e & 3) >= lim) sc[e] = 0.0f;
+    }
+    float sum = 0.0f;
+    u32x4_t pb[2];
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      sum += (sc[4 * j] + sc[4 * j + 1]) + (sc[4 * j + 2] + sc[4 * j + 3]);
+      pb[j >> 1][2 * (j & 1)] = pack_bf(sc[4 * j], sc[4 * j + 1]);
+      pb[j >> 1][2 * (j & 1) + 1] = pack_bf(sc[4 * j + 2], sc[4 * j + 3]);
+    }
+    l += sum;
+#pragma unroll
+    for (int k = 0; k < 2; k++)
+#pragma unroll
+      for (int d = 0; d < 4; d++)
+        acc[d] = mfma32(*reinterpret_cast<const u32x4_t*>(
+                            &s.vt[32 * d + lr][((4 * tile + 2 * k + h) ^ ((lr >> 2) & 7)) * 8]),
+                        pb[k], acc[d]);
+    if (mark[buf] == it + 1) {  // some value of the iteration is not finite
+      for (int e = 0; e < 16; e++) {
+        const int key = key0 + 8 * (e >> 2) + 4 * h + (e & 3);
+        const uint32_t sw = load1(vsr, key * 4), bw = load1(vbr, key * 4);
+        if (key < lim) {
+          if (!(__builtin_fmaf(15.0f, fabsf(lo_f(sw)), fabsf(lo_f(bw))) <= 3.402823466e38f)) poison[0] = NAN;
+          if (!(__builtin_fmaf(15.0f, fabsf(hi_f(sw)), fabsf(hi_f(bw))) <= 3.402823466e38f)) poison[1] = NAN;
+        }
       }
     }
-    if (groups == 1)
-      finish_row(p, kvh, r0 + r, d, o, fin[r][0], fin[r][1]);
-    else
-      *reinterpret_cast<float4*>(&red[(n * items + it) * 4]) = o;
-  }
-  if (groups == 1) return;
+  };
+
+  __syncthreads();  // (the marks are cleared)
+  if (it0 < it1) stage(it0, 0);
+  if (it0 + 1 < it1) fetch(it0 + 1);
   __syncthreads();
-  for (int it = tid; it < items; it += kThreads) {
-    float4 o = *reinterpret_cast<const float4*>(&red[it * 4]);
-    for (int k = 1; k < groups; k++) {
-      const float4 v = *reinterpret_cast<const float4*>(&red[(k * items + it) * 4]);
-      o.x += v.x;
-      o.y += v.y;
-      o.z += v.z;
-      o.w += v.w;
-    }
-    finish_row(p, kvh, r0 + (it >> 5), 4 * (it & 31), o, fin[it >> 5][0], fin[it >> 5][1]);
+  for (int it = it0; it < it1; it++) {
+    const int buf = (it - it0) & 1;
+#pragma unroll
+    for (int t = 0; t < TPW; t++) multiply(it, buf, kwi * TPW + t);
+    if (it + 1 < it1) stage(it + 1, buf ^ 1);
+    if (it + 2 < it1) fetch(it + 2);
+    __syncthreads();
   }
+
+  l = add_xor32(l);
+  if (l != l) m = l;  // a NaN score: the row stays NaN
+#pragma unroll
+  for (int d = 0; d < 4; d++) acc[d] += add_xor32(poison[d >> 1]);
+  // ---- waves of the same rows, two by two ----
+#pragma unroll
+  for (int half = KW / 2; half > 0; half >>= 1) {
+    const int sl = (kwi & (half - 1)) * RW + rwi;
+    if (kwi >= half && kwi < 2 * half) {
+#pragma unroll
+      for (int d = 0; d < 4; d++)
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+          *reinterpret_cast<float4*>(&jn.os[sl][lr][32 * d + 8 * j + 4 * h]) =
+              make_float4(acc[d][4 * j], acc[d][4 * j + 1], acc[d][4 * j + 2], acc[d][4 * j + 3]);
+      if (h == 0) {
+        jn.ms[sl][lr] = m;
+        jn.ls[sl][lr] = l;
+      }
+    }
+    __syncthreads();
+    if (kwi < half) {
+      const float mo = jn.ms[sl][lr], lo = jn.ls[sl][lr], mm = fmaxf(m, mo);
+      const float a = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - mm) * p.c2);
+      const float b = mo == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((mo - mm) * p.c2);
+      l = __builtin_fmaf(l, a, lo * b);
+      m = l != l ? l : mm;
+#pragma unroll
+      for (int d = 0; d < 4; d++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          const float4 v = *reinterpret_cast<const float4*>(&jn.os[sl][lr][32 * d + 8 * j + 4 * h]);
+          acc[d][4 * j] = __builtin_fmaf(acc[d][4 * j], a, v.x * b);
+          acc[d][4 * j + 1] = __builtin_fmaf(acc[d][4 * j + 1], a, v.y * b);
+          acc[d][4 * j + 2] = __builtin_fmaf(acc[d][4 * j + 2], a, v.z * b);
+          acc[d][4 * j + 3] = __builtin_fmaf(acc[d][4 * j + 3], a, v.w * b);
+        }
+    }
+    __syncthreads();
+  }
+  if (kwi > 0 || lr >= n) return;
+#pragma unroll
+  for (int d = 0; d < 4; d++)
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      const float4 o = make_float4(acc[d][4 * j], acc[d][4 * j + 1], acc[d][4 * j + 2], acc[d][4 * j + 3]);
+      const int dim = 32 * d + 8 * j + 4 * h;
+      if (p.ns == 1)
+        finish_row(p, kvh, row, dim, o, m, l);
+      else
+        *reinterpret_cast<float4*>(p.part_o + ((row0 + row) * p.ns + split) * kKv4Dim + dim) = o;
+    }
+  if (p.ns > 1 && h == 0)
+    *reinterpret_cast<float2*>(p.part_ml + ((row0 + row) * p.ns + split) * 2) = make_float2(m, l);
+}
+
+// Joins the splits of kv4_tile_kernel: 32 lanes per row, 4 dims each.
+__global__ void __launch_bounds__(256) kv4_merge_kernel(const Kv4AttnParams p) {
+  const int R = p.Hq / p.c.n_kv_heads * p.M;
+  const int64_t rows = static_cast<int64_t>(p.c.n_kv_heads) * R;
+  const int64_t at = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  const int d = 4 * (threadIdx.x & 31);
+  if (at >= rows) return;
+  const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + at * p.ns;
+  const float* po = p.part_o + at * p.ns * kKv4Dim + d;
+  float m = -INFINITY, l = 0.0f;
+  for (int s = 0; s < p.ns; s++) m = fmaxf(m, ml[s].x);
+  float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+  for (int s = 0; s < p.ns; s++) {
+    const float2 v = ml[s];
+    const float f = v.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((v.x - m) * p.c2);
+    const float4 u = *reinterpret_cast<const float4*>(po + static_cast<int64_t>(s) * kKv4Dim);
+    l = __builtin_fmaf(f, v.y, l);
+    o.x = __builtin_fmaf(f, u.x, o.x);
+    o.y = __builtin_fmaf(f, u.y, o.y);
+    o.z = __builtin_fmaf(f, u.z, o.z);
+    o.w = __builtin_fmaf(f, u.w, o.w);
+  }
+  finish_row(p, static_cast<int>(at / R), static_cast<int>(at % R), d, o, m, l);
 }
 
 // weights[h][j] += sum over the query rows of exp2(S c2 - max c2 - log2 sum).
-// A wave holds 32 keys unpacked and walks the query rows 16 at a time; rw
-// waves of a workgroup share keys and take every rw-th row tile.
+// A wave holds 32 keys unpacked and walks the query rows 16 at a time, the
+// next rows' queries loaded ahead; rw waves of a workgroup share keys and
+// take every rw-th row tile.  The start of the accumulators, -16 Q_g, comes
+// from the matrix cores too: a product of the pieces with -16.
 constexpr int kWeighWaves = 8;
 __global__ void __launch_bounds__(64 * kWeighWaves) kv4_weigh_kernel(const Kv4AttnParams p) {
   __shared__ float red[kWeighWaves][kKeys];
@@ -504,6 +1141,7 @@ __global__ void __launch_bounds__(64 * kWeighWaves) kv4_weigh_kernel(const Kv4At
   const int M = p.M, R = p.Hq / p.c.n_kv_heads * M, L = p.offset + M;
   const int tiles = (R + kRows - 1) / kRows;
   const int64_t slot = static_cast<int64_t>(kvh) * p.c.capacity, row0 = static_cast<int64_t>(kvh) * R;
+  const f32x4_t zero = {0.0f, 0.0f, 0.0f, 0.0f};
   const PairK nk;
   float acc[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
   if (b * kKeys < L) {
@@ -511,8 +1149,20 @@ __global__ void __launch_bounds__(64 * kWeighWaves) kv4_weigh_kernel(const Kv4At
     const __amdgpu_buffer_rsrc_t ksr = rsrc(reinterpret_cast<const uint32_t*>(p.c.k_scales), slot, L * 4);
     const __amdgpu_buffer_rsrc_t kbr = rsrc(reinterpret_cast<const uint32_t*>(p.c.k_biases), slot, L * 4);
     u32x4_t ka[2][2][2];  // [tile][group][word]
-    u32x4_t kb[2];
+    uint32_t kb[2];
     float ks[2][8];
+    // the queries of row tile rt
+    u32x4_t qf[4], qp;
+    float2 st;
+    auto load_q = [&](int rt) {
+      const int64_t row = row0 + min(rt * kRows + li, R - 1);
+      const u32x4_t* src = reinterpret_cast<const u32x4_t*>(p.qp) + row * kQueryWords;
+#pragma unroll
+      for (int k = 0; k < 4; k++) qf[k] = src[4 * g + k];
+      qp = src[16];
+      st = p.lse[row];
+    };
+    load_q(rs);
 #pragma unroll
     for (int t = 0; t < 2; t++) {
       const int key = b * kKeys + 16 * t;
@@ -522,8 +1172,7 @@ __global__ void __launch_bounds__(64 * kWeighWaves) kv4_weigh_kernel(const Kv4At
         ka[t][y][0] = word_pairs(w.x, nk);
         ka[t][y][1] = word_pairs(w.y, nk);
       }
-      const uint32_t bw = load1(kbr, (key + li) * 4);
-      kb[t] = u32x4_t{bw, bw, bw, bw};
+      kb[t] = load1(kbr, (key + li) * 4);
       const u32x4_t s = load4(ksr, (key + 4 * g) * 4);
 #pragma unroll
       for (int i = 0; i < 4; i++) {
@@ -532,45 +1181,44 @@ __global__ void __launch_bounds__(64 * kWeighWaves) kv4_weigh_kernel(const Kv4At
       }
     }
     for (int rt = rs; rt < tiles; rt += p.rw) {
-      const int r = rt * kRows + li, rc = min(r, R - 1);
+      const int r = rt * kRows + li;
       const int t0 = rt * kRows % M, n = min(kRows, R - rt * kRows);
       const int tmax = t0 + n > M ? M - 1 : t0 + n - 1, tmin = t0 + n > M ? 0 : t0;
-      if (b * kKeys > p.offset + tmax) continue;  // uniform: none of these rows sees any of these keys
-      const uint16_t* qr = p.q + (row0 + rc) * kKv4Dim + 16 * g;
-      u32x4_t qf[2][2];
-#pragma unroll
-      for (int y = 0; y < 2; y++)
-#pragma unroll
-        for (int e = 0; e < 2; e++) {
-          uint4 d = *reinterpret_cast<const uint4*>(qr + 64 * y + 8 * e);
-          d = permute_pairs(d);
-          qf[y][e] = u32x4_t{d.x ^ p.flip, d.y ^ p.flip, d.z ^ p.flip, d.w ^ p.flip};
-        }
-      const uint4 pieces = p.qp[row0 + rc];
-      const float2 st = p.lse[row0 + rc];
-      const u32x4_t qp = g ? u32x4_t{0u, 0u, 0u, 0u} : u32x4_t{pieces.x, pieces.y, pieces.z, 0u};
-      const float q0 = lo_f(pieces.x) + lo_f(pieces.y) + lo_f(pieces.z);
-      const float q1 = hi_f(pieces.x) + hi_f(pieces.y) + hi_f(pieces.z);
-      const f32x4_t one = {-16.0f, -16.0f, -16.0f, -16.0f};
+      const bool none = b * kKeys > p.offset + tmax;  // uniform: none of these rows sees any of these keys
       const bool cut = n < kRows || b * kKeys + kKeys > p.offset + tmin + 1;
       const int lim = r < R ? p.offset + r % M + 1 : 0;
+      const u32x4_t pieces = g ? u32x4_t{0u, 0u, 0u, 0u} : qp;
+      const float mc = st.x, lg = st.y;
+      f32x4_t d[2][3];
+      if (!none) {
+        // rows all alike: -16 Q_0, -16 Q_1
+        const f32x4_t s0 = mfma(u32x4_t{0xC180u, 0xC180u, 0xC180u, 0u}, pieces, zero);
+        const f32x4_t s1 = mfma(u32x4_t{0xC1800000u, 0xC1800000u, 0xC1800000u, 0u}, pieces, zero);
 #pragma unroll
-      for (int t = 0; t < 2; t++) {
-        f32x4_t d0 = one * q0, d1 = one * q1;
-        d0 = mfma(ka[t][0][0], qf[0][0], d0);
-        d1 = mfma(ka[t][1][0], qf[1][0], d1);
-        d0 = mfma(ka[t][0][1], qf[0][1], d0);
-        d1 = mfma(ka[t][1][1], qf[1][1], d1);
-        const f32x4_t db = mfma(kb[t], qp, f32x4_t{0.0f, 0.0f, 0.0f, 0.0f});
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-          const int e = 4 * t + i;
-          const float s = __builtin_fmaf(ks[0][e], d0[i], __builtin_fmaf(ks[1][e], d1[i], db[i]));
-          float w = __builtin_amdgcn_exp2f(__builtin_fmaf(s, p.c2, -st.x) - st.y);
-          if (cut && b * kKeys + 16 * t + 4 * g + i >= lim) w = 0.0f;
-          acc[e] += w;
+        for (int t = 0; t < 2; t++) {
+          d[t][0] = mfma(ka[t][0][0], qf[0], s0);
+          d[t][1] = mfma(ka[t][1][0], qf[2], s1);
+          d[t][0] = mfma(ka[t][0][1], qf[1], d[t][0]);
+          d[t][1] = mfma(ka[t][1][1], qf[3], d[t][1]);
+          d[t][2] = mfma(u32x4_t{kb[t], kb[t], kb[t], kb[t]}, pieces, zero);
         }
       }
+      load_q(min(rt + p.rw, tiles - 1));
+      if (none) continue;
+      float w[8];
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        const int t = e >> 2, i = e & 3;
+        const float s = __builtin_fmaf(ks[0][e], d[t][0][i], __builtin_fmaf(ks[1][e], d[t][1][i], d[t][2][i]));
+        w[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s, p.c2, -mc) - lg);
+      }
+      if (cut) {
+#pragma unroll
+        for (int e = 0; e < 8; e++)
+          if (b * kKeys + 16 * (e >> 2) + 4 * g + (e & 3) >= lim) w[e] = 0.0f;
+      }
+#pragma unroll
+      for (int e = 0; e < 8; e++) acc[e] += w[e];
     }
   }
   // over the 16 queries of a lane row, then over the waves that share keys
@@ -595,14 +1243,15 @@ bool attn_shape_ok(int Hq, int Hkv, int M, int64_t L) {
   if (Hkv <= 0 || Hkv > 65535 || Hq <= 0 || Hq > 65535 || Hq % Hkv || M <= 0 || L < M || L > kKv4MaxCapacity ||
       static_cast<int64_t>(Hq) * M > kMaxQueryRows)
     return false;
-  return (static_cast<int64_t>(Hq / Hkv) * M + kRows - 1) / kRows <= 65535;  // row tiles: grid z
+  return (static_cast<int64_t>(Hq / Hkv) * M + 255) / 256 <= 65535;  // row tiles: grid z
 }
 
-constexpr int kSplitWaves = 8;
-constexpr int kSplitGrid = 512;  // workgroups that a call's splits aim at
+constexpr int kSplitGrid = 256;  // workgroups that a call's splits aim at (twice as many of 4 waves)
 
 // Where the keys of a call are split, and where its workspace's parts are.
 struct Kv4Plan {
+  int rc;  // query rows of the kernel: 4, 8, 16, 64, 128, 256
+  int nw;  // its waves
   int tiles, ns, bps, cnt_stride;
   size_t lse, qp, part_o, part_ml, bytes;  // byte offsets; the counters come first
 };
@@ -610,13 +1259,17 @@ struct Kv4Plan {
 Kv4Plan make_plan(int Hq, int Hkv, int M, int L, bool weigh) {
   Kv4Plan a{};
   const int64_t R = static_cast<int64_t>(Hq / Hkv) * M;
-  a.tiles = static_cast<int>((R + kRows - 1) / kRows);
+  a.rc = R <= 4 ? 4 : R <= 8 ? 8 : R <= 2 * kRows ? kRows : R <= 64 ? 64 : R <= 128 ? 128 : 256;
+  a.tiles = static_cast<int>((R + a.rc - 1) / a.rc);
   const int64_t pairs = static_cast<int64_t>(Hkv) * a.tiles;
-  const int steps = (L + kKeys * kSplitWaves - 1) / (kKeys * kSplitWaves);
-  const int64_t want = std::max<int64_t>(1, kSplitGrid / pairs);
+  a.nw = a.rc < kRows && L <= 16384 ? 4 : 8;
+  // keys of a split's unit: a step of every wave, or an iteration
+  const int keys = a.rc == 4 ? 64 * a.nw : a.rc <= kRows ? 32 * a.nw : a.rc == 64 ? 128 : 64;
+  const int steps = (L + keys - 1) / keys;
+  const int64_t want = std::max<int64_t>(1, (a.rc < kRows && a.nw == 4 ? 2 * kSplitGrid : kSplitGrid) / pairs);
   int ns = static_cast<int>(std::min<int64_t>({want, steps, kMaxSplits}));
   a.cnt_stride = pairs <= 128 ? 128 : 16;
-  if (pairs * a.cnt_stride * 4 > BMX_KV4_COUNTER_BYTES) ns = 1;
+  if (a.rc <= kRows && pairs * a.cnt_stride * 4 > BMX_KV4_COUNTER_BYTES) ns = 1;
   a.bps = (steps + ns - 1) / ns;
   a.ns = (steps + a.bps - 1) / a.bps;
   const size_t rows = static_cast<size_t>(Hq) * M;
@@ -625,7 +1278,7 @@ Kv4Plan make_plan(int Hq, int Hkv, int M, int L, bool weigh) {
   if (weigh) at += rows * sizeof(float2);
   at = (at + 15) & ~static_cast<size_t>(15);
   a.qp = at;
-  if (weigh) at += rows * sizeof(uint4);
+  if (weigh) at += rows * kQueryWords * sizeof(uint4);
   a.part_o = at;
   if (a.ns > 1) at += rows * a.ns * kKv4Dim * sizeof(float);
   a.part_ml = at;
@@ -639,9 +1292,9 @@ Kv4Plan make_plan(int Hq, int Hkv, int M, int L, bool weigh) {
 // partials have a bound that grows with M and L, as the rest does.
 size_t plan_bound(int Hq, int M, int L, bool weigh) {
   const size_t rows = static_cast<size_t>(Hq) * M;
-  const size_t steps = (static_cast<size_t>(L) + kKeys * kSplitWaves - 1) / (kKeys * kSplitWaves);
-  const size_t parts = std::min<size_t>(rows * std::min<size_t>(steps, kMaxSplits), kSplitGrid * kRows);
-  return BMX_KV4_COUNTER_BYTES + (weigh ? rows * (sizeof(float2) + sizeof(uint4)) + 16 : 0) +
+  const size_t steps = (static_cast<size_t>(L) + 63) / 64;  // the smallest a split may be
+  const size_t parts = std::min<size_t>(rows * std::min<size_t>(steps, kMaxSplits), static_cast<size_t>(kSplitGrid) * 256);
+  return BMX_KV4_COUNTER_BYTES + (weigh ? rows * (sizeof(float2) + kQueryWords * sizeof(uint4)) + 16 : 0) +
          parts * (kKv4Dim + 2) * sizeof(float);
 }
 
@@ -691,18 +1344,31 @@ extern "C" int bmx_attention_gqa_kv4(const bmx_bf16* q, const bmx_kv4* cache, bm
   p.ns = a.ns;
   p.bps = a.bps;
   p.cnt_stride = a.cnt_stride;
-  hipLaunchKernelGGL(kv4_split_kernel<kSplitWaves>, dim3(Hkv, a.ns, a.tiles), dim3(64 * kSplitWaves), 0,
-                     as_stream(stream), p);
+  const dim3 grid(Hkv, a.ns, a.tiles), block(64 * a.nw);
+  const hipStream_t st = as_stream(stream);
+  if (a.rc == 4 && a.nw == 4) hipLaunchKernelGGL((kv4_few_kernel<4, 4>), grid, block, 0, st, p);
+  else if (a.rc == 4) hipLaunchKernelGGL((kv4_few_kernel<4, 8>), grid, block, 0, st, p);
+  else if (a.rc == 8 && a.nw == 4) hipLaunchKernelGGL((kv4_few_kernel<8, 4>), grid, block, 0, st, p);
+  else if (a.rc == 8) hipLaunchKernelGGL((kv4_few_kernel<8, 8>), grid, block, 0, st, p);
+  else if (a.rc == kRows) hipLaunchKernelGGL((kv4_rows_kernel<8, 1>), grid, block, 0, st, p);
+  else if (a.rc == 64) hipLaunchKernelGGL(kv4_tile_kernel<2>, grid, block, 0, st, p);
+  else if (a.rc == 128) hipLaunchKernelGGL(kv4_tile_kernel<4>, grid, block, 0, st, p);
+  else hipLaunchKernelGGL(kv4_tile_kernel<8>, grid, block, 0, st, p);
   if (int rc = check_launch("attention_kv4")) return rc;
-  if (!weights) return BMX_OK;
-  p.rw = 1;
-  while (p.rw < kWeighWaves && p.rw < a.tiles) p.rw *= 2;
-  const int keys = kKeys * (kWeighWaves / p.rw);
-  if ((L + keys - 1) / keys > 65535) {
-    // (fewer key groups: waves do not share keys)
-    p.rw = 1;
+  if (a.rc > kRows && a.ns > 1) {
+    const int64_t rows = static_cast<int64_t>(n_heads) * M;
+    hipLaunchKernelGGL(kv4_merge_kernel, dim3(static_cast<unsigned>((rows + 7) / 8)), dim3(256), 0, st, p);
+    if (int rc = check_launch("attention_kv4 merge")) return rc;
   }
+  if (!weights) return BMX_OK;
+  // waves that share keys: as many as bring 2048 waves (two per SIMD) or have
+  // a row tile each
+  const int64_t rt = (static_cast<int64_t>(n_heads / Hkv) * M + kRows - 1) / kRows;
+  const int64_t key_waves = static_cast<int64_t>(Hkv) * ((L + kKeys - 1) / kKeys);
+  p.rw = 1;
+  while (p.rw < kWeighWaves && p.rw < rt && key_waves * p.rw < 2048) p.rw *= 2;
   const int per = kKeys * (kWeighWaves / p.rw);
-  hipLaunchKernelGGL(kv4_weigh_kernel, dim3(Hkv, (L + per - 1) / per), dim3(64 * kWeighWaves), 0, as_stream(stream), p);
+  const int groups = (L + per - 1) / per;  // at most 65535: kKv4MaxCapacity
+  hipLaunchKernelGGL(kv4_weigh_kernel, dim3(Hkv, groups), dim3(64 * kWeighWaves), 0, as_stream(stream), p);
   return check_launch("attention_kv4 weights");
 }

@@ -12,7 +12,7 @@ namespace bmx {
 
 constexpr int kKv4Dim = 128;                 // head_dim
 constexpr int kKv4Words = 16;                // words per row
-constexpr int kKv4MaxCapacity = 1 << 24;     // rows: a head's words stay below 2^31 bytes
+constexpr int kKv4MaxCapacity = 65535 * 256;  // rows: a head's words stay below 2^31 bytes, 256 keys a grid row
 
 // Checks of the struct itself; `what` names the entry point.
 int check_kv4(const char* what, const bmx_kv4* c, int head_dim);

@@ -273,7 +273,7 @@ int bmx_add(const bmx_bf16 *a, const bmx_bf16 *b, bmx_bf16 *y, int64_t n, void *
  * together, where bf16 takes 512.  k and v, all scales and biases: 16-byte
  * aligned device pointers; the struct itself is host memory, read during the
  * call.  group_size must be 64 and bits 4 (BMX_E_UNSUPPORTED).  `capacity`
- * may be up to 2^24 rows (BMX_E_SHAPE).
+ * may be up to 16776960 rows (BMX_E_SHAPE).
  * No counterpart in the reference, whose KvCache is in the activations' type
  * (crates/base-mlx-core/src/model/qwen3.rs:109-162). */
 typedef struct {

@@ -60,7 +60,7 @@ def test_cache_struct_refusals(op):
     assert entry_points(kv4())[op](D=64) == bmx.BMX_E_UNSUPPORTED
     assert entry_points(kv4(n_kv_heads=0))[op]() == bmx.BMX_E_SHAPE
     assert entry_points(kv4(capacity=0))[op]() == bmx.BMX_E_SHAPE
-    assert entry_points(kv4(capacity=(1 << 24) + 1))[op]() == bmx.BMX_E_SHAPE
+    assert entry_points(kv4(capacity=16776961))[op]() == bmx.BMX_E_SHAPE
 
 
 @pytest.mark.parametrize("op", ("write", "read", "rope", "attention"))
@@ -116,10 +116,10 @@ def test_attention_refusals():
 def test_attention_workspace_query_refuses_what_the_call_refuses():
     q = bmx.load().bmx_attention_kv4_workspace_bytes
     assert q(4, 3, 1, 10, 0) == 0 and q(0, 1, 1, 10, 0) == 0 and q(4, 0, 1, 10, 0) == 0
-    assert q(4, 2, 0, 10, 0) == 0 and q(4, 2, 11, 10, 0) == 0 and q(4, 2, 1, (1 << 24) + 1, 0) == 0
+    assert q(4, 2, 0, 10, 0) == 0 and q(4, 2, 11, 10, 0) == 0 and q(4, 2, 1, 16776961, 0) == 0
     assert q(4, 2, -5, 10, 0) == 0 and q(4, 2, 1, -1, 0) == 0
-    assert q(4, 2, 1, 1 << 24, 1) > 0
-    assert q(65535, 1, 1 << 20, 1 << 24, 0) == 0  # more query rows than one call takes
+    assert q(4, 2, 1, 16776960, 1) > 0
+    assert q(65535, 1, 1 << 20, 16776960, 0) == 0  # more query rows than one call takes
 
 
 def test_attention_workspace_grows_with_the_call():
