@@ -71,6 +71,14 @@ __device__ __forceinline__ f32x16_t mfma32(u32x4_t a, u32x4_t b, f32x16_t c) {
                                                  0, 0, 0);
 }
 
+// The wave's number as a scalar, so branches on it cost no lane masks
+__device__ __forceinline__ int wave_id() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
+
+// Whether a running maximum m moves to its step's maximum bm: only where the
+// weights exp2((bm - m) c2) would pass 2^8.  Until then m stays, P goes up to
+// 2^8, and the products so far need no rescaling.
+__device__ __forceinline__ bool moves(float bm, float m, float c2) { return bm > m && !((bm - m) * c2 <= 8.0f); }
+
 // The masks of the nibble pairs, held in registers (a gfx9 and-or takes no
 // literal)
 struct PairK {
@@ -163,7 +171,7 @@ template <int NW, int ROWS, int NT>
 __device__ __forceinline__ void join_and_finish(const Kv4AttnParams& p, JoinLds<NW, ROWS, NT>& sm, int kvh, int split,
                                                 int r0, int RT, const float (&ma)[NT], const float (&la)[NT],
                                                 const f32x4_t (&acc)[NT][2][4], const float (&x)[NT][2]) {
-  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, li = lane & 15, g = lane >> 4;
+  const int tid = threadIdx.x, wave = wave_id(), lane = tid & 63, li = lane & 15, g = lane >> 4;
   const int64_t row0 = static_cast<int64_t>(kvh) * (p.Hq / p.c.n_kv_heads) * p.M + r0;
   // ---- the waves' sums joined: weights exp2((m_w - m) c2) ----
   float m[NT];
@@ -308,7 +316,7 @@ __device__ __forceinline__ void join_and_finish(const Kv4AttnParams& p, JoinLds<
 template <int NW, int NT>
 __global__ void __launch_bounds__(64 * NW) kv4_rows_kernel(const Kv4AttnParams p) {
   __shared__ JoinLds<NW, kRows, NT> sm;
-  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, li = lane & 15, g = lane >> 4;
+  const int tid = threadIdx.x, wave = wave_id(), lane = tid & 63, li = lane & 15, g = lane >> 4;
   const int kvh = blockIdx.x, split = blockIdx.y, r0 = blockIdx.z * (NT * kRows);
   const int M = p.M, R = p.Hq / p.c.n_kv_heads * M, RT = min(NT * kRows, R - r0), L = p.offset + M;
   const int64_t row0 = static_cast<int64_t>(kvh) * R + r0;
@@ -485,7 +493,7 @@ __global__ void __launch_bounds__(64 * NW) kv4_rows_kernel(const Kv4AttnParams p
 #pragma unroll
       for (int e = 1; e < 8; e++) bm = fmaxf(bm, sc[n][e]);
       bm = max_xor32(max_xor16(bm));
-      if (__any(bm > m[n])) {
+      if (__any(moves(bm, m[n], p.c2))) {
         const float mn = fmaxf(m[n], bm);
         const float a = m[n] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m[n] - mn) * p.c2);
         m[n] = mn;
@@ -590,7 +598,7 @@ template <int RC, int NW>
 __global__ void __launch_bounds__(64 * NW) kv4_few_kernel(const Kv4AttnParams p) {
   constexpr int T = 16 / RC, kStep = 16 * T;
   __shared__ JoinLds<NW, RC, 1> sm;
-  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, li = lane & 15, g = lane >> 4;
+  const int tid = threadIdx.x, wave = wave_id(), lane = tid & 63, li = lane & 15, g = lane >> 4;
   const int qi = li % RC, blk = li / RC;
   const int kvh = blockIdx.x, split = blockIdx.y;
   const int M = p.M, R = p.Hq / p.c.n_kv_heads * M, L = p.offset + M;
@@ -705,7 +713,7 @@ __global__ void __launch_bounds__(64 * NW) kv4_few_kernel(const Kv4AttnParams p)
     if constexpr (RC == 4) bm = fmaxf(bm, dpp_f32<0x124>(bm));
     bm = fmaxf(bm, dpp_f32<0x128>(bm));
     bm = max_xor32(max_xor16(bm));
-    if (__any(bm > m)) {
+    if (__any(moves(bm, m, p.c2))) {
       const float mn = fmaxf(m, bm);
       const float a = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - mn) * p.c2);
       m = mn;
@@ -786,6 +794,16 @@ __global__ void __launch_bounds__(64 * NW) kv4_few_kernel(const Kv4AttnParams p)
   join_and_finish<NW, RC, 1>(p, sm, kvh, split, 0, R, ms, ls, accs, xs);
 }
 
+__device__ __forceinline__ u32x4_t lds_read(const uint16_t* p) { return *reinterpret_cast<const u32x4_t*>(p); }
+// Reads before it stay before it, and so ahead of the branches that follow
+__device__ __forceinline__ void reads_go_out() { asm volatile("" ::: "memory"); }
+
+constexpr float kFloatMax = 3.402823466e38f;
+// Whether every value of a group of scale s and bias b is a finite number
+__device__ __forceinline__ bool kv4_finite(float s, float b) {
+  return __builtin_fmaf(15.0f, fabsf(s), fabsf(b)) <= kFloatMax;
+}
+
 // Many query rows: 32 RW of one kv head per workgroup of 8 waves, wave w with
 // rows 32 (w % RW) ..; the waves that share rows take different key tiles of
 // 32.  An iteration's keys are unpacked once, by all waves, into LDS (two
@@ -813,6 +831,7 @@ __global__ void __launch_bounds__(512) kv4_tile_kernel(const Kv4AttnParams p) {
     alignas(16) uint16_t kt[KPI][KS];
     alignas(16) uint16_t vt[kKv4Dim][KPI];
     alignas(16) uint32_t sb[2][KPI];  // K's biases, scales
+    alignas(16) float sf[2][KPI];     // the scales of group 0, group 1
   };
   struct Join {
     alignas(16) float os[4][kKeys][kOs];
@@ -823,12 +842,25 @@ __global__ void __launch_bounds__(512) kv4_tile_kernel(const Kv4AttnParams p) {
   __shared__ int mark[2];
   Stage* const st = reinterpret_cast<Stage*>(lds);
   Join& jn = *reinterpret_cast<Join*>(lds);
-  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, lr = lane & 31, h = lane >> 5;
+  const int tid = threadIdx.x, wave = wave_id(), lane = tid & 63, lr = lane & 31, h = lane >> 5;
   const int rwi = wave % RW, kwi = wave / RW;
   const int kvh = blockIdx.x, split = blockIdx.y;
   const int M = p.M, R = p.Hq / p.c.n_kv_heads * M, L = p.offset + M;
-  const int r0 = blockIdx.z * (kKeys * RW), rw0 = r0 + kKeys * rwi;  // first row of the workgroup, of the wave
-  const int RT = min(kKeys * RW, R - r0), n = min(kKeys, R - rw0);   // their rows (n <= 0: none)
+  // the 32-row tile of wave number i: with 8, spread over the rows, so that
+  // the two waves of a SIMD (and so all workgroups) see about as many keys
+  // together, however the causal mask cuts them
+  const int z = blockIdx.z, zs = gridDim.z;
+  auto tile_of = [&](int i) {
+    if constexpr (RW < 8) return z * RW + i;
+    const int o = i < 4 ? i : 11 - i;
+    return o * zs + (o & 1 ? zs - 1 - z : z);
+  };
+  // keys that any row of a tile sees
+  auto end_of = [&](int first, int rows) {
+    const int t0 = first % M;
+    return p.offset + (t0 + rows > M ? M - 1 : t0 + rows - 1) + 1;
+  };
+  const int rw0 = kKeys * tile_of(rwi), n = min(kKeys, R - rw0);  // first row, rows (n <= 0: none)
   const int64_t row0 = static_cast<int64_t>(kvh) * R;
   const int row = min(rw0 + lr, R - 1);
   const int lim = p.offset + row % M + 1;
@@ -836,9 +868,13 @@ __global__ void __launch_bounds__(512) kv4_tile_kernel(const Kv4AttnParams p) {
   if (n > 0) {
     const int t0 = rw0 % M;
     all_see = p.offset + (t0 + n > M ? 0 : t0) + 1;
-    kend = p.offset + (t0 + n > M ? M - 1 : t0 + n - 1) + 1;
+    kend = end_of(rw0, n);
   }
-  const int tw = r0 % M, kend_wg = p.offset + (tw + RT > M ? M - 1 : tw + RT - 1) + 1;
+  int kend_wg = 0;
+  for (int i = 0; i < RW; i++) {
+    const int first = kKeys * tile_of(i);
+    if (first < R) kend_wg = max(kend_wg, end_of(first, min(kKeys, R - first)));
+  }
   const PairK nk;
 
   const int64_t slot = static_cast<int64_t>(kvh) * p.c.capacity;
@@ -881,24 +917,34 @@ __global__ void __launch_bounds__(512) kv4_tile_kernel(const Kv4AttnParams p) {
 #pragma unroll
     for (int i = 0; i < W; i++)
       *reinterpret_cast<u32x4_t*>(&s.kt[k_key][8 * (k_word + i)]) = word_pairs(gk[i], nk);
-    if (tid < 2 * KPI) (&s.sb[0][0])[tid] = gsb;
+    if (tid < 2 * KPI) {
+      (&s.sb[0][0])[tid] = gsb;
+      if (tid >= KPI) {
+        s.sf[0][tid - KPI] = lo_f(gsb);
+        s.sf[1][tid - KPI] = hi_f(gsb);
+      }
+    }
 #pragma unroll
     for (int v = 0; v < VJ; v++) {
       const int job = tid + 512 * v, hw = job & 31, quad = job >> 5;
       const int r = quad & 7, pair = 4 * (quad >> 3) + 2 * (r >> 2) + (r & 1);
-      float sv[4], cv[4];
-      bool bad = false;
+      float sv[4], cv[4], most = 0.0f;
+      const uint32_t half = hw < 16 ? 0x01000c0cu : 0x03020c0cu;  // the group's scale as a float
 #pragma unroll
       for (int i = 0; i < 4; i++) {
-        sv[i] = hw < 16 ? lo_f(gs[v][i]) : hi_f(gs[v][i]);
-        const float b = hw < 16 ? lo_f(gb[v][i]) : hi_f(gb[v][i]);
+        sv[i] = __uint_as_float(__builtin_amdgcn_perm(0u, gs[v][i], half));
+        const float b = __uint_as_float(__builtin_amdgcn_perm(0u, gb[v][i], half));
         cv[i] = __builtin_fmaf(-16.0f, sv[i], b);
-        if (!(__builtin_fmaf(15.0f, fabsf(sv[i]), fabsf(b)) <= 3.402823466e38f)) {
-          bad = true;
-          sv[i] = cv[i] = 0.0f;
-        }
+        most += __builtin_fmaf(15.0f, fabsf(sv[i]), fabsf(b));
       }
-      if (bad) atomicMax(&mark[buf], it + 1);
+      if (!(most <= kFloatMax)) {  // one of them, or just their sum
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+          if (!kv4_finite(sv[i], __uint_as_float(__builtin_amdgcn_perm(0u, gb[v][i], half)))) {
+            sv[i] = cv[i] = 0.0f;
+            atomicMax(&mark[buf], it + 1);
+          }
+      }
       const uint32_t p01 = gv[v][0] | (gv[v][1] << 16), p23 = gv[v][2] | (gv[v][3] << 16);
       const uint32_t a[4] = {nibble_pair<0>(p01, nk), nibble_pair<1>(p01, nk), nibble_pair<2>(p01, nk),
                              nibble_pair<3>(p01, nk)};
@@ -955,29 +1001,43 @@ __global__ void __launch_bounds__(512) kv4_tile_kernel(const Kv4AttnParams p) {
     for (int i = 0; i < 16; i++) acc[d][i] = 0.0f;
   float m = -INFINITY, l = 0.0f, poison[2] = {0.0f, 0.0f};
 
-  auto multiply = [&](int it, int buf, int tile) {
+  // K's fragments of the tile to come: read while P V of the one before runs
+  u32x4_t kf[8];
+  auto read_k = [&](int buf, int tile) {
+#pragma unroll
+    for (int k = 0; k < 8; k++) kf[k] = lds_read(&st[buf].kt[kKeys * tile + lr][8 * (2 * k + h)]);
+    reads_go_out();
+  };
+  auto multiply = [&](int it, int buf, int tile, bool more) {
     const Stage& s = st[buf];
     const int key0 = it * KPI + kKeys * tile, kl = kKeys * tile;
     if (key0 >= kend) return;  // uniform in the wave
     f32x16_t d0, d1, db;
 #pragma unroll
     for (int i = 0; i < 16; i++) d0[i] = d1[i] = db[i] = 0.0f;
+    const uint32_t w = s.sb[h][kl + lr];
+    const bool marked = __builtin_amdgcn_readfirstlane(mark[buf]) == it + 1;  // some value of the iteration is not finite
 #pragma unroll
     for (int k = 0; k < 4; k++) {
-      d0 = mfma32(*reinterpret_cast<const u32x4_t*>(&s.kt[kl + lr][8 * (2 * k + h)]), qf[k], d0);
-      d1 = mfma32(*reinterpret_cast<const u32x4_t*>(&s.kt[kl + lr][8 * (2 * k + 8 + h)]), qf[4 + k], d1);
+      d0 = mfma32(kf[k], qf[k], d0);
+      d1 = mfma32(kf[4 + k], qf[4 + k], d1);
     }
-    const uint32_t w = s.sb[h][kl + lr];
     db = mfma32(u32x4_t{w, w, w, w}, pieces, db);
     float sc[16];
 #pragma unroll
     for (int j = 0; j < 4; j++) {
-      const u32x4_t s4 = *reinterpret_cast<const u32x4_t*>(&s.sb[1][kl + 8 * j + 4 * h]);
+      const f32x4_t s0 = *reinterpret_cast<const f32x4_t*>(&s.sf[0][kl + 8 * j + 4 * h]);
+      const f32x4_t s1 = *reinterpret_cast<const f32x4_t*>(&s.sf[1][kl + 8 * j + 4 * h]);
 #pragma unroll
       for (int i = 0; i < 4; i++)
-        sc[4 * j + i] =
-            __builtin_fmaf(lo_f(s4[i]), d0[4 * j + i], __builtin_fmaf(hi_f(s4[i]), d1[4 * j + i], db[4 * j + i]));
+        sc[4 * j + i] = __builtin_fmaf(s0[i], d0[4 * j + i], __builtin_fmaf(s1[i], d1[4 * j + i], db[4 * j + i]));
     }
+    // V's fragments, on their way while the weights are computed
+    u32x4_t vf[8];
+#pragma unroll
+    for (int k = 0; k < 8; k++)
+      vf[k] = lds_read(&s.vt[32 * (k & 3) + lr][((4 * tile + 2 * (k >> 2) + h) ^ ((lr >> 2) & 7)) * 8]);
+    reads_go_out();
     const bool cut = key0 + kKeys > all_see;
     if (cut) {
 #pragma unroll
@@ -988,7 +1048,7 @@ __global__ void __launch_bounds__(512) kv4_tile_kernel(const Kv4AttnParams p) {
 #pragma unroll
     for (int e = 1; e < 16; e++) bm = fmaxf(bm, sc[e]);
     bm = max_xor32(bm);
-    if (__any(bm > m)) {
+    if (__any(moves(bm, m, p.c2))) {
       const float mn = fmaxf(m, bm);
       const float a = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - mn) * p.c2);
       m = mn;
@@ -1013,20 +1073,16 @@ __global__ void __launch_bounds__(512) kv4_tile_kernel(const Kv4AttnParams p) {
       pb[j >> 1][2 * (j & 1) + 1] = pack_bf(sc[4 * j + 2], sc[4 * j + 3]);
     }
     l += sum;
+    if (more) read_k(buf, tile + 1);
 #pragma unroll
-    for (int k = 0; k < 2; k++)
-#pragma unroll
-      for (int d = 0; d < 4; d++)
-        acc[d] = mfma32(*reinterpret_cast<const u32x4_t*>(
-                            &s.vt[32 * d + lr][((4 * tile + 2 * k + h) ^ ((lr >> 2) & 7)) * 8]),
-                        pb[k], acc[d]);
-    if (mark[buf] == it + 1) {  // some value of the iteration is not finite
+    for (int k = 0; k < 8; k++) acc[k & 3] = mfma32(vf[k], pb[k >> 2], acc[k & 3]);
+    if (marked) {
       for (int e = 0; e < 16; e++) {
         const int key = key0 + 8 * (e >> 2) + 4 * h + (e & 3);
         const uint32_t sw = load1(vsr, key * 4), bw = load1(vbr, key * 4);
         if (key < lim) {
-          if (!(__builtin_fmaf(15.0f, fabsf(lo_f(sw)), fabsf(lo_f(bw))) <= 3.402823466e38f)) poison[0] = NAN;
-          if (!(__builtin_fmaf(15.0f, fabsf(hi_f(sw)), fabsf(hi_f(bw))) <= 3.402823466e38f)) poison[1] = NAN;
+          if (!kv4_finite(lo_f(sw), lo_f(bw))) poison[0] = NAN;
+          if (!kv4_finite(hi_f(sw), hi_f(bw))) poison[1] = NAN;
         }
       }
     }
@@ -1038,10 +1094,19 @@ __global__ void __launch_bounds__(512) kv4_tile_kernel(const Kv4AttnParams p) {
   __syncthreads();
   for (int it = it0; it < it1; it++) {
     const int buf = (it - it0) & 1;
+    // the two waves of a SIMD (w and w + 4) unpack at different ends of the
+    // iteration: between barriers one's VALU work falls on the other's products
+    read_k(buf, kwi * TPW);
+    if (wave >= 4) {
+      if (it + 1 < it1) stage(it + 1, buf ^ 1);
+      if (it + 2 < it1) fetch(it + 2);
+    }
 #pragma unroll
-    for (int t = 0; t < TPW; t++) multiply(it, buf, kwi * TPW + t);
-    if (it + 1 < it1) stage(it + 1, buf ^ 1);
-    if (it + 2 < it1) fetch(it + 2);
+    for (int t = 0; t < TPW; t++) multiply(it, buf, kwi * TPW + t, t + 1 < TPW);
+    if (wave < 4) {
+      if (it + 1 < it1) stage(it + 1, buf ^ 1);
+      if (it + 2 < it1) fetch(it + 2);
+    }
     __syncthreads();
   }
 
@@ -1135,7 +1200,7 @@ __global__ void __launch_bounds__(256) kv4_merge_kernel(const Kv4AttnParams p) {
 constexpr int kWeighWaves = 8;
 __global__ void __launch_bounds__(64 * kWeighWaves) kv4_weigh_kernel(const Kv4AttnParams p) {
   __shared__ float red[kWeighWaves][kKeys];
-  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, li = lane & 15, g = lane >> 4;
+  const int tid = threadIdx.x, wave = wave_id(), lane = tid & 63, li = lane & 15, g = lane >> 4;
   const int kvh = blockIdx.x, kg = kWeighWaves / p.rw;  // key blocks per workgroup
   const int b = blockIdx.y * kg + wave / p.rw, rs = wave % p.rw;
   const int M = p.M, R = p.Hq / p.c.n_kv_heads * M, L = p.offset + M;
