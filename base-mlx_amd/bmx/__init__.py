@@ -591,8 +591,10 @@ def kv4_evict(cache, weights, length, budget, sink=4, recent=0, into=None, weigh
         _same_device(cache.k, kept)
         if kept.dtype != torch.int32 or kept.shape != (cache.n_kv_heads, budget):
             raise BmxError(BMX_E_ARG, f"kept must be int32 {(cache.n_kv_heads, budget)}")
+    nbytes = load().bmx_kv4_evict_workspace_bytes(cache.n_kv_heads, length)
+    ws = _empty(stream, cache.device, torch.uint8, nbytes) if nbytes else None
     call("bmx_kv4_evict", cache._ref, weights.data_ptr(), into._ref, weights_into.data_ptr(), kept.data_ptr(), length,
-         budget, sink, recent, 128, _stream(stream))
+         budget, sink, recent, 128, _ptr(ws), nbytes, _stream(stream))
     return kept
 
 

@@ -89,7 +89,8 @@ SIGNATURES = {
     "bmx_attention_gqa_kv4": (c_int, [c_p, c_p, c_p, c_p, c_int, c_int, c_int, c_int, c_f, c_p, ctypes.c_size_t,
                                       c_p]),
     "bmx_attention_kv4_workspace_bytes": (ctypes.c_size_t, [c_int, c_int, c_int, c_int, c_int]),
-    "bmx_kv4_evict": (c_int, [c_p, c_p, c_p, c_p, c_p, c_int, c_int, c_int, c_int, c_int, c_p]),
+    "bmx_kv4_evict": (c_int, [c_p, c_p, c_p, c_p, c_p, c_int, c_int, c_int, c_int, c_int, c_p, ctypes.c_size_t, c_p]),
+    "bmx_kv4_evict_workspace_bytes": (ctypes.c_size_t, [c_int, c_int]),
     "bmx_argmax_rows": (c_int, [c_p, c_i64, c_i64, c_p, c_p]),
     "bmx_silu_mul": (c_int, [c_p, c_p, c_p, c_i64, c_p]),
     "bmx_add": (c_int, [c_p, c_p, c_p, c_i64, c_p]),

@@ -58,7 +58,7 @@ struct Kv4AttnParams {
   int ns;             // key splits
   int bps;            // steps of all waves per split
   int cnt_stride;
-  int rw;             // weigh: waves of a workgroup that share keys
+  float* sums;        // [row ranges, Hkv, L] of the weights
 };
 
 __device__ __forceinline__ f32x4_t mfma(u32x4_t a, u32x4_t b, f32x4_t c) {
@@ -1150,156 +1150,193 @@ __global__ void __launch_bounds__(512) kv4_tile_kernel(const Kv4AttnParams p) {
     }
     __syncthreads();
   }
-  if (kwi > 0 || lr >= n) return;
+  if (kwi > 0 || n <= 0) return;
+  if (p.ns == 1) {
+    if (lr >= n) return;
+#pragma unroll
+    for (int d = 0; d < 4; d++)
+#pragma unroll
+      for (int j = 0; j < 4; j++)
+        finish_row(p, kvh, row, 32 * d + 8 * j + 4 * h,
+                   make_float4(acc[d][4 * j], acc[d][4 * j + 1], acc[d][4 * j + 2], acc[d][4 * j + 3]), m, l);
+    return;
+  }
+  // partials in the lanes' order, so a store writes 1 KB in one piece
+  const int64_t unit = (static_cast<int64_t>(kvh) * ((R + kKeys - 1) / kKeys) + tile_of(rwi)) * p.ns + split;
+  f32x4_t* po = reinterpret_cast<f32x4_t*>(p.part_o) + unit * (kKeys * kKv4Dim / 4) + lane;
 #pragma unroll
   for (int d = 0; d < 4; d++)
 #pragma unroll
-    for (int j = 0; j < 4; j++) {
-      const float4 o = make_float4(acc[d][4 * j], acc[d][4 * j + 1], acc[d][4 * j + 2], acc[d][4 * j + 3]);
-      const int dim = 32 * d + 8 * j + 4 * h;
-      if (p.ns == 1)
-        finish_row(p, kvh, row, dim, o, m, l);
-      else
-        *reinterpret_cast<float4*>(p.part_o + ((row0 + row) * p.ns + split) * kKv4Dim + dim) = o;
-    }
-  if (p.ns > 1 && h == 0)
-    *reinterpret_cast<float2*>(p.part_ml + ((row0 + row) * p.ns + split) * 2) = make_float2(m, l);
+    for (int j = 0; j < 4; j++)
+      po[64 * (4 * d + j)] = f32x4_t{acc[d][4 * j], acc[d][4 * j + 1], acc[d][4 * j + 2], acc[d][4 * j + 3]};
+  if (h == 0) *reinterpret_cast<float2*>(p.part_ml + (unit * kKeys + lr) * 2) = make_float2(m, l);
 }
 
-// Joins the splits of kv4_tile_kernel: 32 lanes per row, 4 dims each.
+// Joins the splits of kv4_tile_kernel: a wave per 4 dims of each half of a
+// 32-row tile, in the lane order of its partials.
 __global__ void __launch_bounds__(256) kv4_merge_kernel(const Kv4AttnParams p) {
-  const int R = p.Hq / p.c.n_kv_heads * p.M;
-  const int64_t rows = static_cast<int64_t>(p.c.n_kv_heads) * R;
-  const int64_t at = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
-  const int d = 4 * (threadIdx.x & 31);
-  if (at >= rows) return;
-  const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + at * p.ns;
-  const float* po = p.part_o + at * p.ns * kKv4Dim + d;
+  const int R = p.Hq / p.c.n_kv_heads * p.M, tiles = (R + kKeys - 1) / kKeys;
+  const int wave = wave_id(), lane = threadIdx.x & 63, lr = lane & 31, h = lane >> 5;
+  const int64_t tile = blockIdx.x >> 2;
+  const int k = (blockIdx.x & 3) * 4 + wave;  // 4 d + j of kv4_tile_kernel
+  const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + tile * p.ns * kKeys + lr;
+  const f32x4_t* po = reinterpret_cast<const f32x4_t*>(p.part_o) + tile * p.ns * (kKeys * kKv4Dim / 4) + 64 * k + lane;
+  const int kvh = static_cast<int>(tile / tiles), r = static_cast<int>(tile % tiles) * kKeys + lr;
   float m = -INFINITY, l = 0.0f;
-  for (int s = 0; s < p.ns; s++) m = fmaxf(m, ml[s].x);
-  float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 4
+  for (int s = 0; s < p.ns; s++) m = fmaxf(m, ml[s * kKeys].x);
+  f32x4_t o = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 8
   for (int s = 0; s < p.ns; s++) {
-    const float2 v = ml[s];
+    const float2 v = ml[s * kKeys];
     const float f = v.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((v.x - m) * p.c2);
-    const float4 u = *reinterpret_cast<const float4*>(po + static_cast<int64_t>(s) * kKv4Dim);
     l = __builtin_fmaf(f, v.y, l);
-    o.x = __builtin_fmaf(f, u.x, o.x);
-    o.y = __builtin_fmaf(f, u.y, o.y);
-    o.z = __builtin_fmaf(f, u.z, o.z);
-    o.w = __builtin_fmaf(f, u.w, o.w);
+    o += f * po[static_cast<int64_t>(s) * (kKeys * kKv4Dim / 4)];
   }
-  finish_row(p, static_cast<int>(at / R), static_cast<int>(at % R), d, o, m, l);
+  if (r < R) finish_row(p, kvh, r, 8 * k + 4 * h, make_float4(o[0], o[1], o[2], o[3]), m, l);
 }
 
 // weights[h][j] += sum over the query rows of exp2(S c2 - max c2 - log2 sum).
-// A wave holds 32 keys unpacked and walks the query rows 16 at a time, the
-// next rows' queries loaded ahead; rw waves of a workgroup share keys and
-// take every rw-th row tile.  The start of the accumulators, -16 Q_g, comes
-// from the matrix cores too: a product of the pieces with -16.
-constexpr int kWeighWaves = 8;
+// A wave holds 32 keys unpacked, a workgroup 256; all of them walk the rows of
+// the grid's row range 16 at a time, four such tiles to a stage of LDS (two
+// stages: the next is loaded while this one is multiplied).  Read by each wave
+// from the L2 instead, the queries were the bound: 140 MB for 32 tokens over
+// 16384 rows, 16 us.  The accumulators' start, -16 Q_g, comes from the matrix
+// cores too: a product of the pieces with -16.  With several row ranges the
+// sums go to p.sums [range][head][L], added up by kv4_add_kernel.
+constexpr int kWeighWaves = 8, kWeighKeys = kWeighWaves * kKeys, kWeighTiles = 4;
 __global__ void __launch_bounds__(64 * kWeighWaves) kv4_weigh_kernel(const Kv4AttnParams p) {
-  __shared__ float red[kWeighWaves][kKeys];
+  constexpr int kRowsStage = kWeighTiles * kRows, kWords = kRowsStage * kQueryWords;
+  constexpr int kPer = (kWords + 64 * kWeighWaves - 1) / (64 * kWeighWaves);
+  __shared__ u32x4_t qs[2][kWords];
+  __shared__ float2 ls[2][kRowsStage];
   const int tid = threadIdx.x, wave = wave_id(), lane = tid & 63, li = lane & 15, g = lane >> 4;
-  const int kvh = blockIdx.x, kg = kWeighWaves / p.rw;  // key blocks per workgroup
-  const int b = blockIdx.y * kg + wave / p.rw, rs = wave % p.rw;
+  const int kvh = blockIdx.x, b = blockIdx.y * kWeighWaves + wave;
   const int M = p.M, R = p.Hq / p.c.n_kv_heads * M, L = p.offset + M;
-  const int tiles = (R + kRows - 1) / kRows;
+  // this range's rows [ra, rb), a multiple of the stage but at the end
+  const int stages = (R + kRowsStage - 1) / kRowsStage, per = (stages + gridDim.z - 1) / gridDim.z;
+  const int ra = static_cast<int>(blockIdx.z) * per * kRowsStage, rb = min(R, ra + per * kRowsStage);
   const int64_t slot = static_cast<int64_t>(kvh) * p.c.capacity, row0 = static_cast<int64_t>(kvh) * R;
   const f32x4_t zero = {0.0f, 0.0f, 0.0f, 0.0f};
   const PairK nk;
-  float acc[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-  if (b * kKeys < L) {
-    const __amdgpu_buffer_rsrc_t kwr = rsrc(p.c.k, slot * kKv4Words, L * 64);
-    const __amdgpu_buffer_rsrc_t ksr = rsrc(reinterpret_cast<const uint32_t*>(p.c.k_scales), slot, L * 4);
-    const __amdgpu_buffer_rsrc_t kbr = rsrc(reinterpret_cast<const uint32_t*>(p.c.k_biases), slot, L * 4);
-    u32x4_t ka[2][2][2];  // [tile][group][word]
-    uint32_t kb[2];
-    float ks[2][8];
-    // the queries of row tile rt
-    u32x4_t qf[4], qp;
-    float2 st;
-    auto load_q = [&](int rt) {
-      const int64_t row = row0 + min(rt * kRows + li, R - 1);
-      const u32x4_t* src = reinterpret_cast<const u32x4_t*>(p.qp) + row * kQueryWords;
+
+  u32x4_t gq[kPer];
+  float2 gl;
+  const u32x4_t* src = reinterpret_cast<const u32x4_t*>(p.qp) + row0 * kQueryWords;
+  auto fetch = [&](int r) {  // rows r .. of the stage; past rb the last row again
 #pragma unroll
-      for (int k = 0; k < 4; k++) qf[k] = src[4 * g + k];
-      qp = src[16];
-      st = p.lse[row];
-    };
-    load_q(rs);
-#pragma unroll
-    for (int t = 0; t < 2; t++) {
-      const int key = b * kKeys + 16 * t;
-#pragma unroll
-      for (int y = 0; y < 2; y++) {
-        const u32x2_t w = load2(kwr, (key + li) * 64 + 8 * g + 32 * y);
-        ka[t][y][0] = word_pairs(w.x, nk);
-        ka[t][y][1] = word_pairs(w.y, nk);
-      }
-      kb[t] = load1(kbr, (key + li) * 4);
-      const u32x4_t s = load4(ksr, (key + 4 * g) * 4);
-#pragma unroll
-      for (int i = 0; i < 4; i++) {
-        ks[0][4 * t + i] = lo_f(s[i]);
-        ks[1][4 * t + i] = hi_f(s[i]);
-      }
+    for (int k = 0; k < kPer; k++) {
+      const int w = min(tid + 64 * kWeighWaves * k, kWords - 1), row = w / kQueryWords;
+      gq[k] = src[static_cast<int64_t>(min(r + row, rb - 1)) * kQueryWords + (w - row * kQueryWords)];
     }
-    for (int rt = rs; rt < tiles; rt += p.rw) {
-      const int r = rt * kRows + li;
-      const int t0 = rt * kRows % M, n = min(kRows, R - rt * kRows);
-      const int tmax = t0 + n > M ? M - 1 : t0 + n - 1, tmin = t0 + n > M ? 0 : t0;
-      const bool none = b * kKeys > p.offset + tmax;  // uniform: none of these rows sees any of these keys
-      const bool cut = n < kRows || b * kKeys + kKeys > p.offset + tmin + 1;
-      const int lim = r < R ? p.offset + r % M + 1 : 0;
-      const u32x4_t pieces = g ? u32x4_t{0u, 0u, 0u, 0u} : qp;
-      const float mc = st.x, lg = st.y;
-      f32x4_t d[2][3];
-      if (!none) {
-        // rows all alike: -16 Q_0, -16 Q_1
-        const f32x4_t s0 = mfma(u32x4_t{0xC180u, 0xC180u, 0xC180u, 0u}, pieces, zero);
-        const f32x4_t s1 = mfma(u32x4_t{0xC1800000u, 0xC1800000u, 0xC1800000u, 0u}, pieces, zero);
+    if (tid < kRowsStage) gl = p.lse[row0 + min(r + tid, rb - 1)];
+  };
+  auto stage = [&](int buf) {
 #pragma unroll
-        for (int t = 0; t < 2; t++) {
-          d[t][0] = mfma(ka[t][0][0], qf[0], s0);
-          d[t][1] = mfma(ka[t][1][0], qf[2], s1);
-          d[t][0] = mfma(ka[t][0][1], qf[1], d[t][0]);
-          d[t][1] = mfma(ka[t][1][1], qf[3], d[t][1]);
-          d[t][2] = mfma(u32x4_t{kb[t], kb[t], kb[t], kb[t]}, pieces, zero);
+    for (int k = 0; k < kPer; k++) {
+      const int w = tid + 64 * kWeighWaves * k;
+      if (w < kWords) qs[buf][w] = gq[k];
+    }
+    if (tid < kRowsStage) ls[buf][tid] = gl;
+  };
+  if (ra < rb) fetch(ra);
+
+  const __amdgpu_buffer_rsrc_t kwr = rsrc(p.c.k, slot * kKv4Words, L * 64);
+  const __amdgpu_buffer_rsrc_t ksr = rsrc(reinterpret_cast<const uint32_t*>(p.c.k_scales), slot, L * 4);
+  const __amdgpu_buffer_rsrc_t kbr = rsrc(reinterpret_cast<const uint32_t*>(p.c.k_biases), slot, L * 4);
+  u32x4_t ka[2][2][2];  // [tile][group][word]
+  uint32_t kb[2];
+  float ks[2][8], acc[8];
+#pragma unroll
+  for (int t = 0; t < 2; t++) {
+    const int key = b * kKeys + 16 * t;
+#pragma unroll
+    for (int y = 0; y < 2; y++) {
+      const u32x2_t w = load2(kwr, (key + li) * 64 + 8 * g + 32 * y);
+      ka[t][y][0] = word_pairs(w.x, nk);
+      ka[t][y][1] = word_pairs(w.y, nk);
+    }
+    kb[t] = load1(kbr, (key + li) * 4);
+    const u32x4_t s = load4(ksr, (key + 4 * g) * 4);
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      ks[0][4 * t + i] = lo_f(s[i]);
+      ks[1][4 * t + i] = hi_f(s[i]);
+      acc[4 * t + i] = 0.0f;
+    }
+  }
+
+  if (ra < rb) stage(0);
+  __syncthreads();
+  int buf = 0;
+  for (int r0 = ra; r0 < rb; r0 += kRowsStage, buf ^= 1) {
+    const bool more = r0 + kRowsStage < rb;
+    if (more) fetch(r0 + kRowsStage);
+    int t0 = r0 % M;  // token of the tile's first row
+    for (int tile = 0; tile < kWeighTiles; tile++) {
+      const int rt = r0 + tile * kRows, n = min(kRows, rb - rt);
+      if (n <= 0 || b * kKeys >= L) break;  // uniform
+      const bool wraps = t0 + n > M;
+      const int tmax = wraps ? M - 1 : t0 + n - 1, tmin = wraps ? 0 : t0;
+      t0 += kRows;
+      if (t0 >= M) t0 = (rt + kRows) % M;
+      if (b * kKeys > p.offset + tmax) continue;  // uniform: none of these rows sees any of these keys
+      const u32x4_t* q = &qs[buf][(tile * kRows + li) * kQueryWords];
+      const u32x4_t w = q[16], pieces = g ? u32x4_t{0u, 0u, 0u, 0u} : w;
+      const float2 st = ls[buf][tile * kRows + li];
+      // rows all alike: -16 Q_0, -16 Q_1
+      const f32x4_t s0 = mfma(u32x4_t{0xC180u, 0xC180u, 0xC180u, 0u}, pieces, zero);
+      const f32x4_t s1 = mfma(u32x4_t{0xC1800000u, 0xC1800000u, 0xC1800000u, 0u}, pieces, zero);
+      const u32x4_t q0 = q[4 * g], q1 = q[4 * g + 1], q2 = q[4 * g + 2], q3 = q[4 * g + 3];
+      float e[8];
+#pragma unroll
+      for (int t = 0; t < 2; t++) {
+        f32x4_t d0 = mfma(ka[t][0][0], q0, s0);
+        f32x4_t d1 = mfma(ka[t][1][0], q2, s1);
+        d0 = mfma(ka[t][0][1], q1, d0);
+        d1 = mfma(ka[t][1][1], q3, d1);
+        const f32x4_t db = mfma(u32x4_t{kb[t], kb[t], kb[t], kb[t]}, pieces, zero);
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          const float s = __builtin_fmaf(ks[0][4 * t + i], d0[i], __builtin_fmaf(ks[1][4 * t + i], d1[i], db[i]));
+          e[4 * t + i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s, p.c2, -st.x) - st.y);
         }
       }
-      load_q(min(rt + p.rw, tiles - 1));
-      if (none) continue;
-      float w[8];
+      if (n < kRows || b * kKeys + kKeys > p.offset + tmin + 1) {
+        const int lim = li < n ? p.offset + (rt + li) % M + 1 : 0;
 #pragma unroll
-      for (int e = 0; e < 8; e++) {
-        const int t = e >> 2, i = e & 3;
-        const float s = __builtin_fmaf(ks[0][e], d[t][0][i], __builtin_fmaf(ks[1][e], d[t][1][i], d[t][2][i]));
-        w[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s, p.c2, -mc) - lg);
-      }
-      if (cut) {
-#pragma unroll
-        for (int e = 0; e < 8; e++)
-          if (b * kKeys + 16 * (e >> 2) + 4 * g + (e & 3) >= lim) w[e] = 0.0f;
+        for (int i = 0; i < 8; i++)
+          if (b * kKeys + 16 * (i >> 2) + 4 * g + (i & 3) >= lim) e[i] = 0.0f;
       }
 #pragma unroll
-      for (int e = 0; e < 8; e++) acc[e] += w[e];
+      for (int i = 0; i < 8; i++) acc[i] += e[i];
     }
+    if (more) stage(buf ^ 1);
+    __syncthreads();
   }
-  // over the 16 queries of a lane row, then over the waves that share keys
+  // over the 16 queries of a lane row; lane (li, g) of li < 8 stores key 4 g +
+  // li % 4 of tile li / 4
+  float mine = 0.0f;
 #pragma unroll
-  for (int e = 0; e < 8; e++) {
-    acc[e] = row16_sum(acc[e]);
-    if (li == 0) red[wave][16 * (e >> 2) + 4 * g + (e & 3)] = acc[e];
+  for (int i = 0; i < 8; i++) {
+    const float v = row16_sum(acc[i]);
+    if (li == i) mine = v;
   }
-  __syncthreads();
-  const int k = tid >> 5;  // key block of the workgroup
-  if (k >= kg) return;
-  const int key = (blockIdx.y * kg + k) * kKeys + (tid & 31);
-  if (key >= L) return;
-  float s = red[k * p.rw][tid & 31];
-  for (int i = 1; i < p.rw; i++) s += red[k * p.rw + i][tid & 31];
-  p.weights[slot + key] += s;
+  const int key = b * kKeys + 16 * (li >> 2) + 4 * g + (li & 3);
+  if (li >= 8 || key >= L) return;
+  if (gridDim.z == 1)
+    p.weights[slot + key] += mine;
+  else
+    p.sums[(static_cast<int64_t>(blockIdx.z) * gridDim.x + kvh) * L + key] = mine;
+}
+
+// weights[h][j] += the row ranges' sums, in order
+__global__ void __launch_bounds__(256) kv4_add_kernel(const Kv4AttnParams p, int ranges) {
+  const int L = p.offset + p.M, j = blockIdx.x * 256 + threadIdx.x;
+  if (j >= L) return;
+  const float* s = p.sums + static_cast<int64_t>(blockIdx.y) * L + j;
+  float v = s[0];
+  for (int z = 1; z < ranges; z++) v += s[static_cast<int64_t>(z) * p.c.n_kv_heads * L];
+  p.weights[static_cast<int64_t>(blockIdx.y) * p.c.capacity + j] += v;
 }
 
 constexpr int64_t kMaxQueryRows = 1 << 28;  // Hq * M of a call
@@ -1318,7 +1355,8 @@ struct Kv4Plan {
   int rc;  // query rows of the kernel: 4, 8, 16, 64, 128, 256
   int nw;  // its waves
   int tiles, ns, bps, cnt_stride;
-  size_t lse, qp, part_o, part_ml, bytes;  // byte offsets; the counters come first
+  int wz;  // row ranges of the weights' grid
+  size_t lse, qp, part_o, part_ml, sums, bytes;  // byte offsets; the counters come first
 };
 
 Kv4Plan make_plan(int Hq, int Hkv, int M, int L, bool weigh) {
@@ -1337,6 +1375,11 @@ Kv4Plan make_plan(int Hq, int Hkv, int M, int L, bool weigh) {
   if (a.rc <= kRows && pairs * a.cnt_stride * 4 > BMX_KV4_COUNTER_BYTES) ns = 1;
   a.bps = (steps + ns - 1) / ns;
   a.ns = (steps + a.bps - 1) / a.bps;
+  // the weights: row ranges until there are as many workgroups as CUs, of at
+  // least two stages each
+  const int64_t key_groups = static_cast<int64_t>(Hkv) * ((L + kWeighKeys - 1) / kWeighKeys);
+  const int64_t stages = (R + kWeighTiles * kRows - 1) / (kWeighTiles * kRows);
+  a.wz = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>((stages + 1) / 2, 256 / key_groups)));
   const size_t rows = static_cast<size_t>(Hq) * M;
   size_t at = BMX_KV4_COUNTER_BYTES;
   a.lse = at;
@@ -1345,22 +1388,27 @@ Kv4Plan make_plan(int Hq, int Hkv, int M, int L, bool weigh) {
   a.qp = at;
   if (weigh) at += rows * kQueryWords * sizeof(uint4);
   a.part_o = at;
-  if (a.ns > 1) at += rows * a.ns * kKv4Dim * sizeof(float);
+  const size_t part_rows = a.rc > kRows ? Hkv * ((R + kKeys - 1) / kKeys) * kKeys : rows;
+  if (a.ns > 1) at += part_rows * a.ns * kKv4Dim * sizeof(float);
   a.part_ml = at;
-  if (a.ns > 1) at += rows * a.ns * 2 * sizeof(float);
+  if (a.ns > 1) at += part_rows * a.ns * 2 * sizeof(float);
+  a.sums = at;
+  if (weigh && a.wz > 1) at += static_cast<size_t>(a.wz) * Hkv * L * sizeof(float);
   a.bytes = at;
   return a;
 }
 
-// What any call of up to M queries that ends at up to row L needs: with at
-// most kSplitGrid workgroups of kRows rows where keys are split at all, the
-// partials have a bound that grows with M and L, as the rest does.
-size_t plan_bound(int Hq, int M, int L, bool weigh) {
+// What any call of up to M queries that ends at up to row L needs, so a bound
+// that grows with both: at most kSplitGrid workgroups of 256 rows where keys
+// are split at all, tiles filled up to 32 rows, and the weights' sums for at
+// most 256 workgroups of 256 keys.
+size_t plan_bound(int Hq, int Hkv, int M, int L, bool weigh) {
   const size_t rows = static_cast<size_t>(Hq) * M;
   const size_t steps = (static_cast<size_t>(L) + 63) / 64;  // the smallest a split may be
-  const size_t parts = std::min<size_t>(rows * std::min<size_t>(steps, kMaxSplits), static_cast<size_t>(kSplitGrid) * 256);
-  return BMX_KV4_COUNTER_BYTES + (weigh ? rows * (sizeof(float2) + kQueryWords * sizeof(uint4)) + 16 : 0) +
-         parts * (kKv4Dim + 2) * sizeof(float);
+  const size_t parts = std::min<size_t>((rows + static_cast<size_t>(Hkv) * kKeys) * std::min<size_t>(steps, kMaxSplits),
+                                        static_cast<size_t>(kSplitGrid) * 256);
+  return BMX_KV4_COUNTER_BYTES + parts * (kKv4Dim + 2) * sizeof(float) +
+         (weigh ? rows * (sizeof(float2) + kQueryWords * sizeof(uint4)) + 16 + 256 * kWeighKeys * sizeof(float) : 0);
 }
 
 }  // namespace
@@ -1369,7 +1417,7 @@ size_t plan_bound(int Hq, int M, int L, bool weigh) {
 using namespace bmx;
 
 extern "C" size_t bmx_attention_kv4_workspace_bytes(int n_heads, int n_kv_heads, int M, int L, int weigh) {
-  return attn_shape_ok(n_heads, n_kv_heads, M, L) ? plan_bound(n_heads, M, L, weigh != 0) : 0;
+  return attn_shape_ok(n_heads, n_kv_heads, M, L) ? plan_bound(n_heads, n_kv_heads, M, L, weigh != 0) : 0;
 }
 
 extern "C" int bmx_attention_gqa_kv4(const bmx_bf16* q, const bmx_kv4* cache, bmx_bf16* out, float* weights,
@@ -1387,7 +1435,7 @@ extern "C" int bmx_attention_gqa_kv4(const bmx_bf16* q, const bmx_kv4* cache, bm
   if (!attn_shape_ok(n_heads, Hkv, M, L))
     return set_error(BMX_E_SHAPE, "attention_kv4: %d heads, M=%d too large for one call", n_heads, M);
   const Kv4Plan a = make_plan(n_heads, Hkv, M, L, weights != nullptr);
-  const size_t need = plan_bound(n_heads, M, L, weights != nullptr);
+  const size_t need = plan_bound(n_heads, Hkv, M, L, weights != nullptr);
   if (workspace_bytes < need || need < a.bytes)
     return set_error(BMX_E_ARG, "attention_kv4: workspace of %zu bytes, %zu needed", workspace_bytes, need);
   char* ws = static_cast<char*>(workspace);
@@ -1421,19 +1469,16 @@ extern "C" int bmx_attention_gqa_kv4(const bmx_bf16* q, const bmx_kv4* cache, bm
   else hipLaunchKernelGGL(kv4_tile_kernel<8>, grid, block, 0, st, p);
   if (int rc = check_launch("attention_kv4")) return rc;
   if (a.rc > kRows && a.ns > 1) {
-    const int64_t rows = static_cast<int64_t>(n_heads) * M;
-    hipLaunchKernelGGL(kv4_merge_kernel, dim3(static_cast<unsigned>((rows + 7) / 8)), dim3(256), 0, st, p);
+    const int64_t units = Hkv * ((static_cast<int64_t>(n_heads / Hkv) * M + kKeys - 1) / kKeys);
+    hipLaunchKernelGGL(kv4_merge_kernel, dim3(static_cast<unsigned>(4 * units)), dim3(256), 0, st, p);
     if (int rc = check_launch("attention_kv4 merge")) return rc;
   }
   if (!weights) return BMX_OK;
-  // waves that share keys: as many as bring 2048 waves (two per SIMD) or have
-  // a row tile each
-  const int64_t rt = (static_cast<int64_t>(n_heads / Hkv) * M + kRows - 1) / kRows;
-  const int64_t key_waves = static_cast<int64_t>(Hkv) * ((L + kKeys - 1) / kKeys);
-  p.rw = 1;
-  while (p.rw < kWeighWaves && p.rw < rt && key_waves * p.rw < 2048) p.rw *= 2;
-  const int per = kKeys * (kWeighWaves / p.rw);
-  const int groups = (L + per - 1) / per;  // at most 65535: kKv4MaxCapacity
-  hipLaunchKernelGGL(kv4_weigh_kernel, dim3(Hkv, groups), dim3(64 * kWeighWaves), 0, as_stream(stream), p);
+  p.sums = reinterpret_cast<float*>(ws + a.sums);
+  hipLaunchKernelGGL(kv4_weigh_kernel, dim3(Hkv, (L + kWeighKeys - 1) / kWeighKeys, a.wz), dim3(64 * kWeighWaves), 0, st,
+                     p);
+  if (a.wz == 1) return check_launch("attention_kv4 weights");
+  if (int rc = check_launch("attention_kv4 weights")) return rc;
+  hipLaunchKernelGGL(kv4_add_kernel, dim3((L + 255) / 256, Hkv), dim3(256), 0, st, p, a.wz);
   return check_launch("attention_kv4 weights");
 }

@@ -28,11 +28,20 @@ __device__ __forceinline__ uint16_t kv4_scale(float lo, float hi, bool nan) {
   const float range = hi - lo;
   return nan || !(range <= 3.402823466e38f) ? 0x7fc0u : f2bf(range / 15.0f);
 }
-// Nibble of x under the stored scale (as a float) and the group's minimum.
-__device__ __forceinline__ uint32_t kv4_nibble(float x, float lo, float s) {
-  const float n = rintf((x - lo) / s);
+// Nibble of x under the stored scale s (as a float; r = 1 / s) and the group's
+// minimum: rne((x - lo) / s), at most 15.  The quotient is formed as (x - lo)
+// r, off by less than 2^-21 of at most 16 from the rounded quotient; only
+// within 2^-17 of a half step can that round to another number, and there (and
+// where r is infinite) the division itself decides.
+__device__ __forceinline__ uint32_t kv4_nibble(float x, float lo, float s, float r) {
+  const float d = x - lo;
+  float t = d * r, n = rintf(t);
+  if (!(fabsf(fabsf(t - n) - 0.5f) >= 7.62939453125e-6f)) n = rintf(d / s);
   // s = 0 gives NaN or inf, s = NaN gives NaN: both pack as 0 and read back as lo and NaN
   return s > 0.0f ? static_cast<uint32_t>(fminf(n, 15.0f)) : 0u;
 }
+// The smallest and largest of a value over 64 lanes
+__device__ __forceinline__ float kv4_max64(float v) { return max_xor32(max_xor16(row16_max(v))); }
+__device__ __forceinline__ float kv4_min64(float v) { return -kv4_max64(-v); }
 
 }  // namespace bmx

@@ -37,6 +37,12 @@ int check_kv4_rows(const char* what, const bmx_kv4* c, int M, int offset) {
 
 namespace {
 
+typedef __attribute__((ext_vector_type(2))) unsigned short u16x2_t;
+template <int CTRL>
+__device__ __forceinline__ u16x2_t dpp_u16x2(u16x2_t v) {
+  return __builtin_bit_cast(u16x2_t, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xF, 0xF, false));
+}
+
 struct Kv4Tensor {
   const uint16_t* x;  // bf16 rows (write: in, read: out)
   int64_t head_stride, row_stride;
@@ -47,22 +53,20 @@ struct Kv4Tensor {
 
 struct Kv4RowsParams {
   Kv4Tensor t[2];  // k, v
-  int64_t rows;    // n_kv_heads * M
   int M, cap, offset;
 };
 
 // 16 lanes per row, 8 values (one word) per lane: lanes 0-7 hold group 0,
-// lanes 8-15 group 1.  blockIdx.y: k or v.
+// lanes 8-15 group 1.  blockIdx.y: the kv head, blockIdx.z: k or v (and so no
+// division by M: 15.4 us with one, 8191 rows of 8 heads).
 __global__ void __launch_bounds__(256) kv4_write_kernel(const Kv4RowsParams p) {
-  const int64_t r = static_cast<int64_t>(blockIdx.x) * 16 + (threadIdx.x >> 4);
-  const int li = threadIdx.x & 15;
-  if (r >= p.rows) return;
-  const Kv4Tensor& t = p.t[blockIdx.y];
-  const int64_t h = r / p.M, m = r - h * p.M;
+  const int m = blockIdx.x * 16 + (threadIdx.x >> 4), li = threadIdx.x & 15;
+  if (m >= p.M) return;
+  const Kv4Tensor& t = p.t[blockIdx.z];
+  const int64_t h = blockIdx.y;
   const uint4 d = *reinterpret_cast<const uint4*>(t.x + h * t.head_stride + m * t.row_stride + 8 * li);
   const uint32_t v[4] = {d.x, d.y, d.z, d.w};
   float x[8];
-  bool nan = false;
 #pragma unroll
   for (int i = 0; i < 4; i++) {
     x[2 * i] = bf2f(v[i] & 0xffffu);
@@ -70,23 +74,29 @@ __global__ void __launch_bounds__(256) kv4_write_kernel(const Kv4RowsParams p) {
   }
   float lo = x[0], hi = x[0];
 #pragma unroll
-  for (int i = 0; i < 8; i++) {
-    nan |= x[i] != x[i];
+  for (int i = 1; i < 8; i++) {
     lo = fminf(lo, x[i]);
     hi = fmaxf(hi, x[i]);
   }
-  int bad = nan;
-#pragma unroll
-  for (int o = 1; o < 8; o <<= 1) {
-    lo = fminf(lo, __shfl_xor(lo, o, 64));
-    hi = fmaxf(hi, __shfl_xor(hi, o, 64));
-    bad |= __shfl_xor(bad, o, 64);
-  }
-  const uint16_t sb = kv4_scale(lo, hi, bad);
-  const float s = bf2f(sb);
+  // a NaN, which min and max pass over, by the largest magnitude's bits
+  auto mag = [](uint32_t w) { return __builtin_bit_cast(u16x2_t, w & 0x7fff7fffu); };
+  u16x2_t top = __builtin_elementwise_max(__builtin_elementwise_max(mag(v[0]), mag(v[1])),
+                                          __builtin_elementwise_max(mag(v[2]), mag(v[3])));
+  // over the group's 8 lanes: lane ^ 1, lane ^ 2, 7 - lane (quad_perm twice, row_half_mirror)
+  lo = fminf(lo, dpp_f32<0xB1>(lo));
+  hi = fmaxf(hi, dpp_f32<0xB1>(hi));
+  top = __builtin_elementwise_max(top, dpp_u16x2<0xB1>(top));
+  lo = fminf(lo, dpp_f32<0x4E>(lo));
+  hi = fmaxf(hi, dpp_f32<0x4E>(hi));
+  top = __builtin_elementwise_max(top, dpp_u16x2<0x4E>(top));
+  lo = fminf(lo, dpp_f32<0x141>(lo));
+  hi = fmaxf(hi, dpp_f32<0x141>(hi));
+  top = __builtin_elementwise_max(top, dpp_u16x2<0x141>(top));
+  const uint16_t sb = kv4_scale(lo, hi, max(top.x, top.y) > 0x7f80u);
+  const float s = bf2f(sb), rs = 1.0f / s;
   uint32_t word = 0;
 #pragma unroll
-  for (int i = 0; i < 8; i++) word |= kv4_nibble(x[i], lo, s) << (4 * i);
+  for (int i = 0; i < 8; i++) word |= kv4_nibble(x[i], lo, s, rs) << (4 * i);
   const int64_t slot = h * p.cap + p.offset + m;
   t.w[slot * kKv4Words + li] = word;
   const uint16_t bb = s != s ? 0x7fc0u : f2bf(lo);
@@ -100,11 +110,10 @@ __global__ void __launch_bounds__(256) kv4_write_kernel(const Kv4RowsParams p) {
 
 // The inverse: one word per thread, 16 bytes out.
 __global__ void __launch_bounds__(256) kv4_read_kernel(const Kv4RowsParams p) {
-  const int64_t r = static_cast<int64_t>(blockIdx.x) * 16 + (threadIdx.x >> 4);
-  const int li = threadIdx.x & 15;
-  if (r >= p.rows) return;
-  const Kv4Tensor& t = p.t[blockIdx.y];
-  const int64_t h = r / p.M, m = r - h * p.M;
+  const int m = blockIdx.x * 16 + (threadIdx.x >> 4), li = threadIdx.x & 15;
+  if (m >= p.M) return;
+  const Kv4Tensor& t = p.t[blockIdx.z];
+  const int64_t h = blockIdx.y;
   const int64_t slot = h * p.cap + p.offset + m;
   const uint32_t wd = t.w[slot * kKv4Words + li];
   const int sh = li < 8 ? 0 : 16;
@@ -117,7 +126,7 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const Kv4RowsParams p) {
     const float hi = __builtin_fmaf(s, static_cast<float>((wd >> (8 * i + 4)) & 0xfu), b);
     o[i] = static_cast<uint32_t>(f2bf(lo)) | (static_cast<uint32_t>(f2bf(hi)) << 16);
   }
-  *reinterpret_cast<uint4*>(const_cast<uint16_t*>(t.x) + r * kKv4Dim + 8 * li) = make_uint4(o[0], o[1], o[2], o[3]);
+  *reinterpret_cast<uint4*>(const_cast<uint16_t*>(t.x) + (h * p.M + m) * kKv4Dim + 8 * li) = make_uint4(o[0], o[1], o[2], o[3]);
 }
 
 struct QkKv4Params {
@@ -141,18 +150,13 @@ __device__ __forceinline__ void kv4_store_row(float a, float b, int lane, uint32
   uint32_t sw = 0, bw = 0;
 #pragma unroll
   for (int g = 0; g < 2; g++) {
-    float lo = x[g], hi = x[g];
-    const bool nan = __any(x[g] != x[g]);
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      lo = fminf(lo, __shfl_xor(lo, o, 64));
-      hi = fmaxf(hi, __shfl_xor(hi, o, 64));
-    }
-    const uint16_t sb = kv4_scale(lo, hi, nan);
+    const float lo = kv4_min64(x[g]), hi = kv4_max64(x[g]);
+    const uint16_t sb = kv4_scale(lo, hi, __any(x[g] != x[g]));
     const float sf = bf2f(sb);
-    uint32_t n = kv4_nibble(x[g], lo, sf) << (4 * (lane & 7));
-#pragma unroll
-    for (int o = 1; o < 8; o <<= 1) n |= __shfl_xor(n, o, 64);
+    uint32_t n = kv4_nibble(x[g], lo, sf, 1.0f / sf) << (4 * (lane & 7));
+    n |= static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(n), 0xB1, 0xF, 0xF, false));
+    n |= static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(n), 0x4E, 0xF, 0xF, false));
+    n |= static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(n), 0x141, 0xF, 0xF, false));
     if ((lane & 7) == 0) w[8 * g + (lane >> 3)] = n;
     sw |= static_cast<uint32_t>(sb) << (16 * g);
     bw |= static_cast<uint32_t>(sf != sf ? 0x7fc0u : f2bf(lo)) << (16 * g);
@@ -202,19 +206,15 @@ Kv4RowsParams rows_params(const bmx_kv4& c, int M, int offset) {
   p.t[1].w = c.v;
   p.t[1].s = reinterpret_cast<uint32_t*>(c.v_scales);
   p.t[1].b = reinterpret_cast<uint32_t*>(c.v_biases);
-  p.rows = static_cast<int64_t>(c.n_kv_heads) * M;
   p.M = M;
   p.cap = c.capacity;
   p.offset = offset;
   return p;
 }
 
-// 16 rows per workgroup; the grid's x axis takes 2^31 - 1
-int rows_grid(const char* what, int64_t rows, unsigned* n) {
-  const int64_t blocks = (rows + 15) / 16;
-  if (blocks > 0x7fffffff) return set_error(BMX_E_SHAPE, "%s: %lld rows", what, static_cast<long long>(rows));
-  *n = static_cast<unsigned>(blocks);
-  return BMX_OK;
+// 16 rows of a head and array per workgroup
+dim3 rows_grid(const bmx_kv4& c, int M) {
+  return dim3(static_cast<unsigned>((M + 15) / 16), static_cast<unsigned>(c.n_kv_heads), 2);
 }
 
 }  // namespace
@@ -223,9 +223,7 @@ int launch_kv4_read(const bmx_kv4& c, uint16_t* k, uint16_t* v, int M, int start
   Kv4RowsParams p = rows_params(c, M, start);
   p.t[0].x = k;
   p.t[1].x = v;
-  unsigned n = 0;
-  if (int rc = rows_grid("kv4_read", p.rows, &n)) return rc;
-  hipLaunchKernelGGL(kv4_read_kernel, dim3(n, 2), dim3(256), 0, stream, p);
+  hipLaunchKernelGGL(kv4_read_kernel, rows_grid(c, M), dim3(256), 0, stream, p);
   return check_launch("kv4_read");
 }
 
@@ -251,9 +249,7 @@ extern "C" int bmx_kv4_write(const bmx_bf16* k, int64_t k_head_stride, int64_t k
   p.t[1].x = v;
   p.t[1].head_stride = v_head_stride;
   p.t[1].row_stride = v_row_stride;
-  unsigned n = 0;
-  if (int rc = rows_grid("kv4_write", p.rows, &n)) return rc;
-  hipLaunchKernelGGL(kv4_write_kernel, dim3(n, 2), dim3(256), 0, as_stream(stream), p);
+  hipLaunchKernelGGL(kv4_write_kernel, rows_grid(*cache, M), dim3(256), 0, as_stream(stream), p);
   return check_launch("kv4_write");
 }
 

@@ -353,9 +353,15 @@ size_t bmx_attention_kv4_workspace_bytes(int n_heads, int n_kv_heads, int M, int
  * into may be the cache itself (the same struct or equal pointers), and
  * weights_into weights, both then in place; otherwise nothing of `into` may
  * overlap the cache.  Rows of `into` from `budget` on stay as they are.
- * sink, recent >= 0, sink + recent <= budget. */
+ * sink, recent >= 0, sink + recent <= budget.  weights, weights_into and
+ * kept: 16-byte aligned.  `workspace`: bmx_kv4_evict_workspace_bytes or more
+ * for this n_kv_heads and length (16-byte aligned, any contents; NULL where
+ * that is 0); calls that share one must not run concurrently. */
 int bmx_kv4_evict(const bmx_kv4 *cache, const float *weights, const bmx_kv4 *into, float *weights_into,
-                  int32_t *kept, int length, int budget, int sink, int recent, int head_dim, void *stream);
+                  int32_t *kept, int length, int budget, int sink, int recent, int head_dim, void *workspace,
+                  size_t workspace_bytes, void *stream);
+/* Bytes of workspace bmx_kv4_evict needs (0 up to 16384 rows).  Host only. */
+size_t bmx_kv4_evict_workspace_bytes(int n_kv_heads, int length);
 
 /* ------------------------------------------------------------------ */
 /* Qwen3 model, KV cache, generation                                   */

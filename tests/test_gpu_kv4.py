@@ -451,7 +451,8 @@ def check_evict(w, cache, length, budget, sink, recent, in_place):
 
 SIZES = [(1, 1, 0, 0), (2, 1, 0, 0), (2, 1, 0, 1), (5, 5, 2, 3), (5, 5, 0, 0), (9, 4, 4, 0), (9, 4, 0, 4), (65, 64, 4, 8),
          (300, 37, 4, 11), (1024, 1023, 0, 0), (1025, 512, 4, 256), (4352, 1024, 4, 256), (9000, 77, 0, 0), (5000, 4999, 1, 1),
-         (40961, 2048, 4, 64)]
+         (16384, 4000, 4, 100), (16385, 4000, 4, 100), (16385, 16385, 0, 0), (40961, 2048, 4, 64), (40961, 30000, 0, 20000),
+         (100003, 30001, 20000, 5), (131072, 4096, 0, 0)]
 
 
 @pytest.mark.parametrize("in_place", [True, False])
@@ -465,7 +466,7 @@ def test_evict(gpu, length, budget, sink, recent, in_place):
 
 
 @pytest.mark.parametrize("kind", ["equal", "zeros", "few", "signed", "special", "rising", "falling", "subnormal"])
-@pytest.mark.parametrize("length,budget", [(700, 300), (3000, 64), (20000, 9000)])
+@pytest.mark.parametrize("length,budget", [(700, 300), (3000, 64), (9000, 2000), (20000, 9000), (50001, 700)])
 def test_evict_ties_and_orders(gpu, kind, length, budget):
     heads = 2
     cache = random_cache(1, heads, length)

@@ -42,7 +42,7 @@ def entry_points(c):
         "evict": lambda **k: lib.bmx_kv4_evict(r, k.get("w", 7 * P), r if "into" not in k else k["into"],
                                                k.get("w_into", 7 * P), k.get("kept", 9 * P), k.get("length", 50),
                                                k.get("budget", 20), k.get("sink", 4), k.get("recent", 8),
-                                               k.get("D", 128), None),
+                                               k.get("D", 128), k.get("ws"), k.get("wsb", 0), None),
     }
 
 
@@ -156,6 +156,18 @@ def test_evict_refusals():
     assert f(into=ctypes.pointer(small), w_into=8 * P) == bmx.BMX_E_KV_CAPACITY
     heads = kv4(n_kv_heads=3, **far)
     assert f(into=ctypes.pointer(heads), w_into=8 * P) == bmx.BMX_E_SHAPE
+
+
+def test_evict_workspace():
+    q = bmx.load().bmx_kv4_evict_workspace_bytes
+    assert q(8, 16384) == 0 and q(8, 16385) > 0 and q(0, 20000) == 0 and q(8, 0) == 0 and q(8, 16776961) == 0
+    sizes = [q(8, n) for n in (16385, 40000, 131072, 1 << 20, 16776960)]
+    assert sizes == sorted(sizes)
+    f = entry_points(kv4(capacity=20000))["evict"]
+    need = q(2, 20000)
+    assert f(length=20000) == bmx.BMX_E_ARG and "workspace" in bmx.last_error()
+    assert f(length=20000, ws=P, wsb=need - 1) == bmx.BMX_E_ARG
+    assert f(length=20000, ws=P + 8, wsb=need) == bmx.BMX_E_ALIGN
 
 
 def test_python_refusals_need_no_gpu():
