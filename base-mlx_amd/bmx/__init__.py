@@ -405,10 +405,17 @@ def _same_device(t, *others):
             raise BmxError(BMX_E_ARG, f"tensors on {t.device} and {o.device}")
 
 
+_raw_device = None  # as _raw_stream, for the current device's number
+
+
 def _elsewhere(device):
     """Whether a call's tensors live on another GPU than the current one (it
     then runs again with theirs current, on that device's current stream)."""
-    return device.index != _torch().cuda.current_device()
+    global _raw_device
+    if _raw_device is None:
+        _torch().cuda.current_device()  # (initialises the device)
+        _raw_device = getattr(_T._C, "_cuda_getDevice", None) or _T.cuda.current_device
+    return device.index != _raw_device()
 
 
 def _on_stream(stream, device):
@@ -439,34 +446,42 @@ def kv4_write(k, v, cache, offset, stream=None):
     offset .. offset+M-1.  k and v may be strided views with contiguous rows:
     rows of a bf16 cache, or projection rows seen as
     x.view(M, n_kv_heads, 128).transpose(0, 1)."""
-    torch = _torch()
-    if _elsewhere(cache.device):
-        with torch.cuda.device(cache.device):
+    dev = cache.device
+    if _elsewhere(dev):
+        with _T.cuda.device(dev):
             return kv4_write(k, v, cache, offset, stream)
-    _same_device(cache.k, k, v)
-    _bf16(k, v)
-    st = []
-    for t in (k, v):
-        if t.dim() != 3 or t.shape != k.shape or t.shape[0] != cache.n_kv_heads:
-            raise BmxError(BMX_E_SHAPE, f"k and v must be [{cache.n_kv_heads}, M, 128], got {tuple(t.shape)}")
-        s0, s1, s2 = t.stride()
-        if s2 != 1:
-            raise BmxError(BMX_E_ARG, "the 128 values of a row must be contiguous")
-        st += [s0 if t.shape[0] > 1 else 0, s1 if t.shape[1] > 1 else 0]
-    call("bmx_kv4_write", k.data_ptr(), st[0], st[1], v.data_ptr(), st[2], st[3], cache._ref, k.shape[1], k.shape[2],
-         offset, _stream(stream))
+    ks, bf16 = k.shape, _T.bfloat16
+    if k.dtype != bf16 or v.dtype != bf16:
+        raise BmxError(BMX_E_ARG, "k and v must be bfloat16")
+    if k.device != dev or v.device != dev:
+        raise BmxError(BMX_E_ARG, f"k and v must be on {dev}, as the cache")
+    if len(ks) != 3 or v.shape != ks or ks[0] != cache.n_kv_heads:
+        raise BmxError(BMX_E_SHAPE, f"k and v must be [{cache.n_kv_heads}, M, 128], got {tuple(ks)}, {tuple(v.shape)}")
+    k0, k1, k2 = k.stride()
+    v0, v1, v2 = v.stride()
+    if k2 != 1 or v2 != 1:
+        raise BmxError(BMX_E_ARG, "the 128 values of a row must be contiguous")
+    H, M, D = ks
+    if H == 1:
+        k0 = v0 = 0  # (the stride of an axis of one entry says nothing)
+    if M == 1:
+        k1 = v1 = 0
+    call("bmx_kv4_write", k.data_ptr(), k0, k1, v.data_ptr(), v0, v1, cache._ref, M, D, offset, _stream(stream))
 
 
 def kv4_read(cache, start, stop, stream=None):
     """Cache rows [start, stop) as bf16 (k, v), each [n_kv_heads, stop - start, 128]."""
-    torch = _torch()
     if _elsewhere(cache.device):
-        with torch.cuda.device(cache.device):
+        with _T.cuda.device(cache.device):
             return kv4_read(cache, start, stop, stream)
     if not 0 <= start <= stop <= cache.capacity:
         raise BmxError(BMX_E_KV_CAPACITY, f"rows [{start}, {stop}) of capacity {cache.capacity}")
     M = stop - start
-    k, v = _empty(stream, cache.device, torch.bfloat16, 2, cache.n_kv_heads, M, 128).unbind(0)
+    shape = (cache.n_kv_heads, M, 128)
+    if stream is None:
+        k, v = cache.k_scales.new_empty(shape), cache.k_scales.new_empty(shape)
+    else:
+        k, v = (_empty(stream, cache.device, _T.bfloat16, *shape) for _ in "kv")
     if M:
         call("bmx_kv4_read", cache._ref, k.data_ptr(), v.data_ptr(), M, 128, start, _stream(stream))
     return k, v

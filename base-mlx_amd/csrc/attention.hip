@@ -1615,6 +1615,7 @@ int flash_split_blocks(int groups, int tiles, int tq, int Hq, int M, int offset,
 }  // namespace
 
 void attention_prepare(hipStream_t stream) { (void)xcd_local_ok(stream); }
+bool attention_xcd_local(hipStream_t stream) { return xcd_local_ok(stream); }
 
 int launch_attention(const uint16_t* q, const uint16_t* k, const uint16_t* v, uint16_t* out, float* ws,
                      size_t ws_floats, int Hq, int Hkv, int M, int D, int cap, int offset, const int* offset_dev,

@@ -58,6 +58,7 @@ struct Kv4AttnParams {
   int ns;             // key splits
   int bps;            // steps of all waves per split
   int cnt_stride;
+  int local;          // every workgroup of a kv head runs on one XCD (shares its L2)
   float* sums;        // [row ranges, Hkv, L] of the weights
 };
 
@@ -117,17 +118,17 @@ __device__ __forceinline__ uint32_t load1(__amdgpu_buffer_rsrc_t r, int off) {
   return __builtin_amdgcn_raw_buffer_load_b32(r, off, 0, 0);
 }
 
-// Partials travel between workgroups (and XCDs) through agent-scope
-// accesses: written through to memory, complete before the arrival, read
-// after it.
+// Partials travel between workgroups, in general on different XCDs: agent-scope
+// stores (written through to memory), complete before the arrival, and loads
+// with sc1 after it.  Where all workgroups of a kv head share an XCD, plain
+// stores and L2 increments, and loads with sc0 (past the L1) do; the counter
+// is another word then, 256 bytes on, so that a line is only ever updated in
+// one place.
+constexpr int kAgentCoherent = 16, kL2Coherent = 1;
+constexpr int kLocalCounter = 64;  // words into a counter's 512 bytes
 __device__ __forceinline__ void store_part(float* p, float x, float y) {
   const uint64_t v = static_cast<uint64_t>(__float_as_uint(x)) | (static_cast<uint64_t>(__float_as_uint(y)) << 32);
   __hip_atomic_store(reinterpret_cast<uint64_t*>(p), v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
-__device__ __forceinline__ float2 load_part(const float* p) {
-  const uint64_t v =
-      __hip_atomic_load(reinterpret_cast<const uint64_t*>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  return make_float2(__uint_as_float(static_cast<uint32_t>(v)), __uint_as_float(static_cast<uint32_t>(v >> 32)));
 }
 
 // Q_0 and Q_1 of a query row, each in three bf16 pieces that add up to it
@@ -156,75 +157,147 @@ __device__ __forceinline__ void finish_row(const Kv4AttnParams& p, int kvh, int 
   if (p.lse && d == 0) p.lse[static_cast<int64_t>(kvh) * rep * p.M + r] = make_float2(m * p.c2, log2f(l));
 }
 
-template <int NW, int ROWS, int NT>
+template <int NW, int ROWS>
 struct JoinLds {
   alignas(16) float os[NW][ROWS][kOs];
-  float ms[NW][NT * ROWS], ls[NW][NT * ROWS], wt[NT * ROWS][kMaxSplits], fin[NT * ROWS][2];
+  float ms[NW][ROWS], ls[NW][ROWS], wt[ROWS][kMaxSplits], fin[ROWS][2];
   int last;
 };
 
-// The end of a workgroup: each wave hands in, for rows n * ROWS + li of the
-// tile (lanes li < ROWS), its maximum m and sum l over its keys, and in lane
-// (li, g) the products acc[n][y][nibble][i] of the dims described at the
-// kernel, to which x[n][y] adds.
-template <int NW, int ROWS, int NT>
-__device__ __forceinline__ void join_and_finish(const Kv4AttnParams& p, JoinLds<NW, ROWS, NT>& sm, int kvh, int split,
-                                                int r0, int RT, const float (&ma)[NT], const float (&la)[NT],
-                                                const f32x4_t (&acc)[NT][2][4], const float (&x)[NT][2]) {
+// Rows r0 .. r0 + RT - 1 from their splits' partials, by one workgroup; AUX:
+// the cache policy of the loads.
+template <int NW, int ROWS, int AUX>
+__device__ __forceinline__ void merge_splits(const Kv4AttnParams& p, JoinLds<NW, ROWS>& sm, int kvh, int r0, int RT) {
+  constexpr int kThreads = 64 * NW, kAhead = 8;
+  const int tid = threadIdx.x, wave = wave_id(), lane = tid & 63;
+  const int64_t row0 = static_cast<int64_t>(kvh) * (p.Hq / p.c.n_kv_heads) * p.M + r0;
+  const __amdgpu_buffer_rsrc_t rml =
+      rsrc(reinterpret_cast<const uint32_t*>(p.part_ml), row0 * p.ns * 2, RT * p.ns * 8);
+  const __amdgpu_buffer_rsrc_t ro =
+      rsrc(reinterpret_cast<const uint32_t*>(p.part_o), row0 * p.ns * kKv4Dim, RT * p.ns * kKv4Dim * 4);
+  // (row, 4 dims) per thread, the splits n, n + groups, .. over as many threads
+  // as there are; this thread's first eight are on their way while the splits'
+  // weights are formed
+  const int items = RT * 32, groups = max(1, kThreads / items), n = tid / items;
+  auto load_o = [&](int it, int s) {
+    return __builtin_bit_cast(f32x4_t, __builtin_amdgcn_raw_buffer_load_b128(
+                                           ro, (((it >> 5) * p.ns + s) * kKv4Dim + 4 * (it & 31)) * 4, 0, AUX));
+  };
+  // a wave per row, a lane per split
+  f32x2_t ml = {-INFINITY, 0.0f};
+  int r = wave;
+  auto load_ml = [&]() {
+    return __builtin_bit_cast(f32x2_t, __builtin_amdgcn_raw_buffer_load_b64(rml, (r * p.ns + min(lane, p.ns - 1)) * 8, 0, AUX));
+  };
+  if (r < RT) ml = load_ml();
+  int it = tid - n * items;
+  f32x4_t ahead[kAhead];
+  if (it < items && n < groups) {
+#pragma unroll
+    for (int k = 0; k < kAhead; k++) ahead[k] = load_o(it, min(n + k * groups, p.ns - 1));
+  }
+  while (r < RT) {
+    const float m = lane < p.ns ? ml.x : -INFINITY;
+    const float mm = max_xor32(max_xor16(row16_max(m)));
+    const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - mm) * p.c2);
+    const float sum = lanes_sum(lane < p.ns ? f * ml.y : 0.0f, 64);
+    sm.wt[r][lane] = f;
+    if (lane == 0) {
+      sm.fin[r][0] = mm;
+      sm.fin[r][1] = sum;
+    }
+    r += NW;
+    if (r < RT) ml = load_ml();
+  }
+  __syncthreads();
+  float* red = &sm.os[0][0][0];
+  for (bool first = true; it < items && n < groups; it += kThreads, first = false) {
+    const int row = it >> 5, d = 4 * (it & 31);
+    f32x4_t o = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (!first) {
+#pragma unroll
+      for (int k = 0; k < kAhead; k++) ahead[k] = load_o(it, min(n + k * groups, p.ns - 1));
+    }
+    int s = n;
+#pragma unroll
+    for (int k = 0; k < kAhead; k++, s += groups)
+      if (s < p.ns) o += sm.wt[row][s] * ahead[k];
+#pragma unroll 8
+    for (; s < p.ns; s += groups) o += sm.wt[row][s] * load_o(it, s);
+    if (groups == 1)
+      finish_row(p, kvh, r0 + row, d, make_float4(o[0], o[1], o[2], o[3]), sm.fin[row][0], sm.fin[row][1]);
+    else
+      *reinterpret_cast<f32x4_t*>(&red[(n * items + it) * 4]) = o;
+  }
+  if (groups == 1) return;
+  __syncthreads();
+  for (int k = tid; k < items; k += kThreads) {
+    f32x4_t o = *reinterpret_cast<const f32x4_t*>(&red[k * 4]);
+    for (int i = 1; i < groups; i++) o += *reinterpret_cast<const f32x4_t*>(&red[(i * items + k) * 4]);
+    finish_row(p, kvh, r0 + (k >> 5), 4 * (k & 31), make_float4(o[0], o[1], o[2], o[3]), sm.fin[k >> 5][0],
+               sm.fin[k >> 5][1]);
+  }
+}
+
+// The end of a workgroup: each wave hands in, for row li of the tile (lanes
+// li < ROWS), its maximum m and sum l over its keys, and in lane (li, g) the
+// products acc[y][nibble][i] of the dims described at the kernel, to which
+// x[y] adds.
+template <int NW, int ROWS>
+__device__ __forceinline__ void join_and_finish(const Kv4AttnParams& p, JoinLds<NW, ROWS>& sm, int kvh, int split,
+                                                int r0, int RT, float m, float l, const f32x4_t (&acc)[2][4],
+                                                const float (&x)[2]) {
   const int tid = threadIdx.x, wave = wave_id(), lane = tid & 63, li = lane & 15, g = lane >> 4;
   const int64_t row0 = static_cast<int64_t>(kvh) * (p.Hq / p.c.n_kv_heads) * p.M + r0;
   // ---- the waves' sums joined: weights exp2((m_w - m) c2) ----
-  float m[NT];
-#pragma unroll
-  for (int n = 0; n < NT; n++) {
-    m[n] = la[n] != la[n] ? la[n] : ma[n];  // a NaN score: the row stays NaN
-    if (g == 0 && li < ROWS) {
-      sm.ms[wave][n * ROWS + li] = m[n];
-      sm.ls[wave][n * ROWS + li] = la[n];
-    }
+  if (l != l) m = l;  // a NaN score: the row stays NaN
+  if (g == 0 && li < ROWS) {
+    sm.ms[wave][li] = m;
+    sm.ls[wave][li] = l;
   }
   __syncthreads();
+  if (li < ROWS) {
+    float mm = sm.ms[0][li];
 #pragma unroll
-  for (int n = 0; n < NT; n++) {
-    if (n > 0) __syncthreads();  // the rows before have been read
-    if (li < ROWS) {
-      float mm = sm.ms[0][n * ROWS + li];
+    for (int w = 1; w < NW; w++) mm = fmaxf(mm, sm.ms[w][li]);
+    const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - mm) * p.c2);
 #pragma unroll
-      for (int w = 1; w < NW; w++) mm = fmaxf(mm, sm.ms[w][n * ROWS + li]);
-      const float f = m[n] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m[n] - mm) * p.c2);
+    for (int y = 0; y < 2; y++)
 #pragma unroll
-      for (int y = 0; y < 2; y++)
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-          const int a = 4 * g + i;  // row of A: word a % 8, half a / 8
-          *reinterpret_cast<float4*>(&sm.os[wave][li][64 * y + 8 * (a & 7) + 4 * (a >> 3)]) =
-              make_float4((acc[n][y][0][i] + x[n][y]) * f, (acc[n][y][1][i] + x[n][y]) * f,
-                          (acc[n][y][2][i] + x[n][y]) * f, (acc[n][y][3][i] + x[n][y]) * f);
-        }
-    }
-    __syncthreads();
-    for (int it = tid; it < min(ROWS, RT - n * ROWS) * 32; it += 64 * NW) {
-      const int rr = it >> 5, r = n * ROWS + rr, d = 4 * (it & 31);
-      float mm = sm.ms[0][r];
-#pragma unroll
-      for (int w = 1; w < NW; w++) mm = fmaxf(mm, sm.ms[w][r]);
-      float sum = 0.0f;
-      float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-      for (int w = 0; w < NW; w++) {
-        const float f = sm.ms[w][r] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((sm.ms[w][r] - mm) * p.c2);
-        sum = __builtin_fmaf(f, sm.ls[w][r], sum);
-        const float4 v = *reinterpret_cast<const float4*>(&sm.os[w][rr][d]);
-        o.x += v.x;
-        o.y += v.y;
-        o.z += v.z;
-        o.w += v.w;
+      for (int i = 0; i < 4; i++) {
+        const int a = 4 * g + i;  // row of A: word a % 8, half a / 8
+        *reinterpret_cast<float4*>(&sm.os[wave][li][64 * y + 8 * (a & 7) + 4 * (a >> 3)]) =
+            make_float4((acc[y][0][i] + x[y]) * f, (acc[y][1][i] + x[y]) * f, (acc[y][2][i] + x[y]) * f,
+                        (acc[y][3][i] + x[y]) * f);
       }
-      if (sum != sum) mm = sum;
-      if (p.ns == 1) {
-        finish_row(p, kvh, r0 + r, d, o, mm, sum);
+  }
+  __syncthreads();
+  for (int it = tid; it < RT * 32; it += 64 * NW) {
+    const int r = it >> 5, d = 4 * (it & 31);
+    float mm = sm.ms[0][r];
+#pragma unroll
+    for (int w = 1; w < NW; w++) mm = fmaxf(mm, sm.ms[w][r]);
+    float sum = 0.0f;
+    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+    for (int w = 0; w < NW; w++) {
+      const float f = sm.ms[w][r] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((sm.ms[w][r] - mm) * p.c2);
+      sum = __builtin_fmaf(f, sm.ls[w][r], sum);
+      const float4 v = *reinterpret_cast<const float4*>(&sm.os[w][r][d]);
+      o.x += v.x;
+      o.y += v.y;
+      o.z += v.z;
+      o.w += v.w;
+    }
+    if (sum != sum) mm = sum;
+    if (p.ns == 1) {
+      finish_row(p, kvh, r0 + r, d, o, mm, sum);
+    } else {
+      const int64_t at = (row0 + r) * p.ns + split;
+      if (p.local) {
+        *reinterpret_cast<float4*>(p.part_o + at * kKv4Dim + d) = o;
+        if (d == 0) *reinterpret_cast<float2*>(p.part_ml + at * 2) = make_float2(mm, sum);
       } else {
-        const int64_t at = (row0 + r) * p.ns + split;
         store_part(p.part_o + at * kKv4Dim + d, o.x, o.y);
         store_part(p.part_o + at * kKv4Dim + d + 2, o.z, o.w);
         if (d == 0) store_part(p.part_ml + at * 2, mm, sum);
@@ -238,66 +311,27 @@ __device__ __forceinline__ void join_and_finish(const Kv4AttnParams& p, JoinLds<
   __syncthreads();
   if (tid == 0) {
     unsigned* c = p.cnt + (static_cast<int64_t>(blockIdx.z) * gridDim.x + kvh) * p.cnt_stride;
-    const unsigned n = __hip_atomic_fetch_add(c, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    unsigned n;
+    if (p.local) {
+      c += kLocalCounter;
+      n = __hip_atomic_fetch_add(c, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+    } else {
+      n = __hip_atomic_fetch_add(c, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
     sm.last = n == static_cast<unsigned>(p.ns - 1);
-    if (sm.last) __hip_atomic_store(c, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (sm.last) {
+      // (subtracted rather than stored: performed where the additions are)
+      if (p.local) __hip_atomic_fetch_sub(c, static_cast<unsigned>(p.ns), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+      else __hip_atomic_store(c, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
   }
   __syncthreads();
   if (!sm.last) return;
-  // a wave per row, a lane per split: the splits' weights
-  for (int r = wave; r < RT; r += NW) {
-    float2 ml = make_float2(-INFINITY, 0.0f);
-    if (lane < p.ns) ml = load_part(p.part_ml + ((row0 + r) * p.ns + lane) * 2);
-    const float mm = max_xor32(max_xor16(row16_max(ml.x)));
-    const float f = ml.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((ml.x - mm) * p.c2);
-    const float sum = lanes_sum(f * ml.y, 64);
-    sm.wt[r][lane] = f;
-    if (lane == 0) {
-      sm.fin[r][0] = mm;
-      sm.fin[r][1] = sum;
-    }
-  }
-  __syncthreads();
-  // (row, 4 dims) per thread, and the splits over as many threads as there are
-  constexpr int kThreads = 64 * NW;
-  const int items = RT * 32, groups = max(1, kThreads / items);
-  const int n = tid / items;  // this thread's group; those past the last have none
-  float* red = &sm.os[0][0][0];
-  for (int it = tid - n * items; it < items && n < groups; it += kThreads) {
-    const int r = it >> 5, d = 4 * (it & 31);
-    const float* src = p.part_o + (row0 + r) * p.ns * kKv4Dim + d;
-    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 8
-    for (int s = n; s < p.ns; s += groups) {
-      const float2 u = load_part(src + static_cast<int64_t>(s) * kKv4Dim);
-      const float2 v = load_part(src + static_cast<int64_t>(s) * kKv4Dim + 2);
-      const float f = sm.wt[r][s];
-      o.x = __builtin_fmaf(f, u.x, o.x);
-      o.y = __builtin_fmaf(f, u.y, o.y);
-      o.z = __builtin_fmaf(f, v.x, o.z);
-      o.w = __builtin_fmaf(f, v.y, o.w);
-    }
-    if (groups == 1)
-      finish_row(p, kvh, r0 + r, d, o, sm.fin[r][0], sm.fin[r][1]);
-    else
-      *reinterpret_cast<float4*>(&red[(n * items + it) * 4]) = o;
-  }
-  if (groups == 1) return;
-  __syncthreads();
-  for (int it = tid; it < items; it += kThreads) {
-    float4 o = *reinterpret_cast<const float4*>(&red[it * 4]);
-    for (int k = 1; k < groups; k++) {
-      const float4 v = *reinterpret_cast<const float4*>(&red[(k * items + it) * 4]);
-      o.x += v.x;
-      o.y += v.y;
-      o.z += v.z;
-      o.w += v.w;
-    }
-    finish_row(p, kvh, r0 + (it >> 5), 4 * (it & 31), o, sm.fin[it >> 5][0], sm.fin[it >> 5][1]);
-  }
+  if (p.local) merge_splits<NW, ROWS, kL2Coherent>(p, sm, kvh, r0, RT);
+  else merge_splits<NW, ROWS, kAgentCoherent>(p, sm, kvh, r0, RT);
 }
 
-// A workgroup of NW waves: one kv head, 16 NT query rows (row r = j * M + t:
+// A workgroup of NW waves: one kv head, 16 query rows (row r = j * M + t:
 // head kvh * rep + j, token t), one split of the keys; a wave takes 32 keys
 // a step, with its own running maximum and sums.
 //   Lanes: li = lane % 16, g = lane / 16.
@@ -311,19 +345,19 @@ __device__ __forceinline__ void join_and_finish(const Kv4AttnParams& p, JoinLds<
 //     4 (li / 8) + i.  Lane li < 8 loads a word of the even key of a pair,
 //     lane li + 8 the same word of the odd key, and they swap halves.
 // The next step's K is loaded once the scores are done, its V once P V is.
-// Bound by the VALU: per step about 180 instructions for the nibbles and
-// scales, which NT row tiles share, and 110 per tile.
-template <int NW, int NT>
+// Bound by instruction issue: a step takes about 310 VALU instructions and 21
+// products, which hardly overlap (32 tokens over 16384 rows, 32 heads of 8: 32
+// us).  Two row tiles per wave, to share the 180 that nibbles and scales take,
+// spilled registers and were no faster.
+template <int NW>
 __global__ void __launch_bounds__(64 * NW) kv4_rows_kernel(const Kv4AttnParams p) {
-  __shared__ JoinLds<NW, kRows, NT> sm;
+  __shared__ JoinLds<NW, kRows> sm;
   const int tid = threadIdx.x, wave = wave_id(), lane = tid & 63, li = lane & 15, g = lane >> 4;
-  const int kvh = blockIdx.x, split = blockIdx.y, r0 = blockIdx.z * (NT * kRows);
-  const int M = p.M, R = p.Hq / p.c.n_kv_heads * M, RT = min(NT * kRows, R - r0), L = p.offset + M;
+  const int kvh = blockIdx.x, split = blockIdx.y, r0 = blockIdx.z * kRows;
+  const int M = p.M, R = p.Hq / p.c.n_kv_heads * M, RT = min(kRows, R - r0), L = p.offset + M;
   const int64_t row0 = static_cast<int64_t>(kvh) * R + r0;
   // rows' tokens: a query sees keys < lim; the tile's first and last token
-  int lim[NT];
-#pragma unroll
-  for (int n = 0; n < NT; n++) lim[n] = p.offset + (r0 + min(n * kRows + li, RT - 1)) % M + 1;
+  const int lim = p.offset + (r0 + min(li, RT - 1)) % M + 1;
   const int t0 = r0 % M, tmin = t0 + RT > M ? 0 : t0, tmax = t0 + RT > M ? M - 1 : t0 + RT - 1;
   const int all_see = p.offset + tmin + 1, kend = p.offset + tmax + 1;
   const PairK nk;
@@ -370,15 +404,12 @@ __global__ void __launch_bounds__(64 * NW) kv4_rows_kernel(const Kv4AttnParams p
   load_k(b);
   load_v(b);
 
-  // ---- the query fragments, in the pair order of a word, and their sums;
-  // two row tiles' fragments would not fit the registers next to the rest
-  // (94 spilled), so every wave reads them from LDS each step ----
-  __shared__ u32x4_t ql[NT][5][64];
-  float start[NT][2];  // -16 Q_y of the query
-#pragma unroll
-  for (int n = 0; n < NT; n++) {
-    const uint16_t* qr = p.q + (row0 + min(n * kRows + li, RT - 1)) * kKv4Dim + 16 * g;
-    u32x4_t qf[2][2];
+  // ---- the query fragments, in the pair order of a word, and their sums ----
+  u32x4_t qf[2][2];
+  float start[2];  // -16 Q_y of the query
+  u32x4_t qp;      // lanes g = 0: Q_0, Q_1 in three bf16 pieces each
+  {
+    const uint16_t* qr = p.q + (row0 + min(li, RT - 1)) * kKv4Dim + 16 * g;
     float qs[2];
 #pragma unroll
     for (int y = 0; y < 2; y++) {
@@ -395,34 +426,22 @@ __global__ void __launch_bounds__(64 * NW) kv4_rows_kernel(const Kv4AttnParams p
         qf[y][e] = u32x4_t{d.x, d.y, d.z, d.w};
       }
       qs[y] = add_xor32(add_xor16(qs[y]));
-      start[n][y] = -16.0f * qs[y];
+      start[y] = -16.0f * qs[y];
     }
-    if (p.qp && split == 0 && wave == 0 && n * kRows + li < RT) store_query(p, row0 + n * kRows + li, g, qf, qs);
-    if (wave == 0) {
-      u32x4_t pieces = q_pieces(qs);  // Q_0, Q_1 in three bf16 pieces each, for lanes g = 0
-      if (g != 0) pieces = u32x4_t{0u, 0u, 0u, 0u};
-#pragma unroll
-      for (int k = 0; k < 4; k++) ql[n][k][lane] = qf[k >> 1][k & 1];
-      ql[n][4][lane] = pieces;
-    }
+    if (p.qp && split == 0 && wave == 0 && li < RT) store_query(p, row0 + li, g, qf, qs);
+    qp = q_pieces(qs);
+    if (g != 0) qp = u32x4_t{0u, 0u, 0u, 0u};
   }
-  __syncthreads();
 
   const f32x4_t zero = {0.0f, 0.0f, 0.0f, 0.0f};
   // edge: rows 0, 1 sum p~ b, rows 2, 3 sum p~ s, rows 4, 5 -23.5 sum p', of
   // groups 0 and 1
-  f32x4_t acc[NT][2][4], edge[NT];
-  float m[NT], l[NT], slow[NT][2];
+  f32x4_t acc[2][4], edge = zero;
 #pragma unroll
-  for (int n = 0; n < NT; n++) {
-    edge[n] = zero;
-    m[n] = -INFINITY;
-    l[n] = slow[n][0] = slow[n][1] = 0.0f;
+  for (int y = 0; y < 2; y++)
 #pragma unroll
-    for (int y = 0; y < 2; y++)
-#pragma unroll
-      for (int i = 0; i < 4; i++) acc[n][y][i] = zero;
-  }
+    for (int i = 0; i < 4; i++) acc[y][i] = zero;
+  float m = -INFINITY, l = 0.0f, slow[2] = {0.0f, 0.0f};
   const uint32_t centre[2] = {li == 4 ? 0xC1BCC1BCu : 0u, li == 5 ? 0xC1BCC1BCu : 0u};  // bf16 -23.5 twice
   const uint32_t half_sel = li < 8 ? 0x01000504u : 0x07060302u;
   // (selector 0x0c gives a zero byte: rows from 4 on take nothing)
@@ -430,40 +449,25 @@ __global__ void __launch_bounds__(64 * NW) kv4_rows_kernel(const Kv4AttnParams p
 
   auto step = [&](auto cut_) {
     constexpr bool cut = decltype(cut_)::value;  // some row does not see some key
-    asm volatile("" ::: "memory");  // (the fragments stay in LDS: not moved out of the loop)
     // ---- scores ----
-    float sc[NT][8];
+    float sc[8];
 #pragma unroll
     for (int t = 0; t < 2; t++) {
-      f32x4_t d0[NT], d1[NT], db[NT];
-#pragma unroll
-      for (int n = 0; n < NT; n++) {
-        d0[n] = f32x4_t{start[n][0], start[n][0], start[n][0], start[n][0]};
-        d1[n] = f32x4_t{start[n][1], start[n][1], start[n][1], start[n][1]};
-      }
+      f32x4_t d0 = {start[0], start[0], start[0], start[0]}, d1 = {start[1], start[1], start[1], start[1]};
 #pragma unroll
       for (int e = 0; e < 2; e++) {
-        const u32x4_t a0 = word_pairs(kw[t][0][e], nk), a1 = word_pairs(kw[t][1][e], nk);
-#pragma unroll
-        for (int n = 0; n < NT; n++) {
-          d0[n] = mfma(a0, ql[n][e][lane], d0[n]);
-          d1[n] = mfma(a1, ql[n][2 + e][lane], d1[n]);
-        }
+        d0 = mfma(word_pairs(kw[t][0][e], nk), qf[0][e], d0);
+        d1 = mfma(word_pairs(kw[t][1][e], nk), qf[1][e], d1);
       }
+      const f32x4_t db = mfma(u32x4_t{kb[t], kb[t], kb[t], kb[t]}, qp, zero);
 #pragma unroll
-      for (int n = 0; n < NT; n++) db[n] = mfma(u32x4_t{kb[t], kb[t], kb[t], kb[t]}, ql[n][4][lane], zero);
-#pragma unroll
-      for (int i = 0; i < 4; i++) {
-        const float s0 = lo_f(ks[t][i]), s1 = hi_f(ks[t][i]);
-#pragma unroll
-        for (int n = 0; n < NT; n++)
-          sc[n][4 * t + i] = __builtin_fmaf(s0, d0[n][i], __builtin_fmaf(s1, d1[n][i], db[n][i]));
-      }
+      for (int i = 0; i < 4; i++)
+        sc[4 * t + i] = __builtin_fmaf(lo_f(ks[t][i]), d0[i], __builtin_fmaf(hi_f(ks[t][i]), d1[i], db[i]));
     }
     load_k(b + NW);
     // ---- running softmax: the maximum over all keys of a query ----
     const int key0 = b * kKeys + 4 * g;
-    u32x4_t pb[NT][2], pt[NT];
+    u32x4_t pb[2], pt;
     bool odd = false;
     u32x4_t bw[2];
     if constexpr (cut) {
@@ -482,53 +486,50 @@ __global__ void __launch_bounds__(64 * NW) kv4_rows_kernel(const Kv4AttnParams p
       }
       odd = __any(odd);
     }
+    if constexpr (cut) {
 #pragma unroll
-    for (int n = 0; n < NT; n++) {
+      for (int e = 0; e < 8; e++)
+        if (key0 + (e & 3) + 16 * (e >> 2) >= lim) sc[e] = -INFINITY;
+    }
+    float bm = sc[0];
+#pragma unroll
+    for (int e = 1; e < 8; e++) bm = fmaxf(bm, sc[e]);
+    bm = max_xor32(max_xor16(bm));
+    if (__any(moves(bm, m, p.c2))) {
+      const float mn = fmaxf(m, bm);
+      const float a = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - mn) * p.c2);
+      m = mn;
+      l *= a;
+      edge *= a;
+#pragma unroll
+      for (int y = 0; y < 2; y++) {
+        slow[y] *= a;
+#pragma unroll
+        for (int i = 0; i < 4; i++) acc[y][i] *= a;
+      }
+    }
+    const float mc = m == -INFINITY ? 0.0f : m * p.c2;
+    float pr[8], ps[2][8];
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+      pr[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[e], p.c2, -mc));
+      ps[0][e] = pr[e] * lo_f(vs[e >> 2][e & 3]);
+      ps[1][e] = pr[e] * hi_f(vs[e >> 2][e & 3]);
       if constexpr (cut) {
-#pragma unroll
-        for (int e = 0; e < 8; e++)
-          if (key0 + (e & 3) + 16 * (e >> 2) >= lim[n]) sc[n][e] = -INFINITY;
-      }
-      float bm = sc[n][0];
-#pragma unroll
-      for (int e = 1; e < 8; e++) bm = fmaxf(bm, sc[n][e]);
-      bm = max_xor32(max_xor16(bm));
-      if (__any(moves(bm, m[n], p.c2))) {
-        const float mn = fmaxf(m[n], bm);
-        const float a = m[n] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m[n] - mn) * p.c2);
-        m[n] = mn;
-        l[n] *= a;
-        edge[n] *= a;
-#pragma unroll
-        for (int y = 0; y < 2; y++) {
-          slow[n][y] *= a;
-#pragma unroll
-          for (int i = 0; i < 4; i++) acc[n][y][i] *= a;
+        const bool seen = key0 + (e & 3) + 16 * (e >> 2) < lim;
+        if (!seen) pr[e] = ps[0][e] = ps[1][e] = 0.0f;
+        if (odd && seen) {
+          slow[0] += lo_f(bw[e >> 2][e & 3]) * 0.0f;  // 0 or NaN
+          slow[1] += hi_f(bw[e >> 2][e & 3]) * 0.0f;
         }
       }
-      const float mc = m[n] == -INFINITY ? 0.0f : m[n] * p.c2;
-      float pr[8], ps[2][8];
+    }
+    l += ((pr[0] + pr[1]) + (pr[2] + pr[3])) + ((pr[4] + pr[5]) + (pr[6] + pr[7]));
 #pragma unroll
-      for (int e = 0; e < 8; e++) {
-        pr[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[n][e], p.c2, -mc));
-        ps[0][e] = pr[e] * lo_f(vs[e >> 2][e & 3]);
-        ps[1][e] = pr[e] * hi_f(vs[e >> 2][e & 3]);
-        if constexpr (cut) {
-          const bool seen = key0 + (e & 3) + 16 * (e >> 2) < lim[n];
-          if (!seen) pr[e] = ps[0][e] = ps[1][e] = 0.0f;
-          if (odd && seen) {
-            slow[n][0] += lo_f(bw[e >> 2][e & 3]) * 0.0f;  // 0 or NaN
-            slow[n][1] += hi_f(bw[e >> 2][e & 3]) * 0.0f;
-          }
-        }
-      }
-      l[n] += ((pr[0] + pr[1]) + (pr[2] + pr[3])) + ((pr[4] + pr[5]) + (pr[6] + pr[7]));
-#pragma unroll
-      for (int j = 0; j < 4; j++) {
-        pb[n][0][j] = pack_bf(ps[0][2 * j], ps[0][2 * j + 1]);
-        pb[n][1][j] = pack_bf(ps[1][2 * j], ps[1][2 * j + 1]);
-        pt[n][j] = pack_bf(pr[2 * j], pr[2 * j + 1]);
-      }
+    for (int j = 0; j < 4; j++) {
+      pb[0][j] = pack_bf(ps[0][2 * j], ps[0][2 * j + 1]);
+      pb[1][j] = pack_bf(ps[1][2 * j], ps[1][2 * j + 1]);
+      pt[j] = pack_bf(pr[2 * j], pr[2 * j + 1]);
     }
     // ---- P V ----
 #pragma unroll
@@ -542,11 +543,8 @@ __global__ void __launch_bounds__(64 * NW) kv4_rows_kernel(const Kv4AttnParams p
           {nibble_pair<2>(v[0], nk), nibble_pair<2>(v[1], nk), nibble_pair<2>(v[2], nk), nibble_pair<2>(v[3], nk)},
           {nibble_pair<3>(v[0], nk), nibble_pair<3>(v[1], nk), nibble_pair<3>(v[2], nk), nibble_pair<3>(v[3], nk)}};
 #pragma unroll
-      for (int n = 0; n < NT; n++) {
-#pragma unroll
-        for (int i = 0; i < 4; i++) acc[n][y][i] = mfma(a[i], pb[n][y], acc[n][y][i]);
-        edge[n] = mfma(u32x4_t{centre[y], centre[y], centre[y], centre[y]}, pb[n][y], edge[n]);
-      }
+      for (int i = 0; i < 4; i++) acc[y][i] = mfma(a[i], pb[y], acc[y][i]);
+      edge = mfma(u32x4_t{centre[y], centre[y], centre[y], centre[y]}, pb[y], edge);
     }
     {
       // rows 0..3 of A: b_0, b_1, s_0, s_1 of the step's keys
@@ -561,8 +559,7 @@ __global__ void __launch_bounds__(64 * NW) kv4_rows_kernel(const Kv4AttnParams p
           if ((a[j] & 0x7f800000u) == 0x7f800000u) a[j] &= 0xffffu;
         }
       }
-#pragma unroll
-      for (int n = 0; n < NT; n++) edge[n] = mfma(a, pt[n], edge[n]);
+      edge = mfma(a, pt, edge);
     }
     load_v(b + NW);
   };
@@ -571,17 +568,12 @@ __global__ void __launch_bounds__(64 * NW) kv4_rows_kernel(const Kv4AttnParams p
   for (; b < b_full; b += NW) step(std::false_type{});
   for (; b < b_end; b += NW) step(std::true_type{});
 
-  float x[NT][2];  // what every dim of a group gets besides its product
+  float x[2];  // what every dim of a group gets besides its product
 #pragma unroll
-  for (int n = 0; n < NT; n++) {
-    l[n] = add_xor32(add_xor16(l[n]));
-#pragma unroll
-    for (int y = 0; y < 2; y++)
-      x[n][y] = __shfl(edge[n][y], 16 + li, 64) +
-                __builtin_fmaf(7.5f, __shfl(edge[n][2 + y], li, 64), __shfl(edge[n][y], li, 64)) +
-                add_xor32(add_xor16(slow[n][y]));
-  }
-  join_and_finish<NW, kRows, NT>(p, sm, kvh, split, r0, RT, m, l, acc, x);
+  for (int y = 0; y < 2; y++)
+    x[y] = __shfl(edge[y], 16 + li, 64) + __builtin_fmaf(7.5f, __shfl(edge[2 + y], li, 64), __shfl(edge[y], li, 64)) +
+           add_xor32(add_xor16(slow[y]));
+  join_and_finish<NW, kRows>(p, sm, kvh, split, r0, RT, m, add_xor32(add_xor16(l)), acc, x);
 }
 
 // Up to RC = 4 or 8 query rows.  The scores of T = 16 / RC key tiles share one
@@ -597,7 +589,7 @@ __global__ void __launch_bounds__(64 * NW) kv4_rows_kernel(const Kv4AttnParams p
 template <int RC, int NW>
 __global__ void __launch_bounds__(64 * NW) kv4_few_kernel(const Kv4AttnParams p) {
   constexpr int T = 16 / RC, kStep = 16 * T;
-  __shared__ JoinLds<NW, RC, 1> sm;
+  __shared__ JoinLds<NW, RC> sm;
   const int tid = threadIdx.x, wave = wave_id(), lane = tid & 63, li = lane & 15, g = lane >> 4;
   const int qi = li % RC, blk = li / RC;
   const int kvh = blockIdx.x, split = blockIdx.y;
@@ -668,7 +660,7 @@ __global__ void __launch_bounds__(64 * NW) kv4_few_kernel(const Kv4AttnParams p)
   }
   const float st[2] = {-16.0f * qs[0], -16.0f * qs[1]};
 
-  f32x4_t accs[1][2][4], (&acc)[2][4] = accs[0];
+  f32x4_t acc[2][4];
 #pragma unroll
   for (int y = 0; y < 2; y++)
 #pragma unroll
@@ -781,7 +773,7 @@ __global__ void __launch_bounds__(64 * NW) kv4_few_kernel(const Kv4AttnParams p)
     if constexpr (RC == 4) v += dpp_f32<0x124>(v);
     return v + dpp_f32<0x128>(v);
   };
-  float xs[1][2], (&x)[2] = xs[0];
+  float x[2];
 #pragma unroll
   for (int y = 0; y < 2; y++) {
     x[y] = add_xor32(add_xor16(columns(add[y])));
@@ -790,8 +782,7 @@ __global__ void __launch_bounds__(64 * NW) kv4_few_kernel(const Kv4AttnParams p)
 #pragma unroll
       for (int e = 0; e < 4; e++) acc[y][i][e] = columns(acc[y][i][e]);
   }
-  const float ms[1] = {m}, ls[1] = {add_xor32(add_xor16(columns(l)))};
-  join_and_finish<NW, RC, 1>(p, sm, kvh, split, 0, R, ms, ls, accs, xs);
+  join_and_finish<NW, RC>(p, sm, kvh, split, 0, R, m, add_xor32(add_xor16(columns(l))), acc, x);
 }
 
 __device__ __forceinline__ u32x4_t lds_read(const uint16_t* p) { return *reinterpret_cast<const u32x4_t*>(p); }
@@ -1348,29 +1339,75 @@ bool attn_shape_ok(int Hq, int Hkv, int M, int64_t L) {
   return (static_cast<int64_t>(Hq / Hkv) * M + 255) / 256 <= 65535;  // row tiles: grid z
 }
 
-constexpr int kSplitGrid = 256;  // workgroups that a call's splits aim at (twice as many of 4 waves)
+constexpr int kSplitGrid = 256;  // workgroups that a call's splits aim at: one per CU
 
 // Where the keys of a call are split, and where its workspace's parts are.
 struct Kv4Plan {
-  int rc;  // query rows of the kernel: 4, 8, 16, 64, 128, 256
+  int rc;  // query rows of the kernel: 4, 8, 16, 64, 256
   int nw;  // its waves
   int tiles, ns, bps, cnt_stride;
   int wz;  // row ranges of the weights' grid
   size_t lse, qp, part_o, part_ml, sums, bytes;  // byte offsets; the counters come first
 };
 
+// The kernel and split count for R > 8 query rows per kv head, by estimated
+// time (us).  16 rows: 5 for the launch, and per round of 256 workgroups 5 and
+// 1.31 per step of a wave (32 keys; two waves share a SIMD).  64 and 256 rows:
+// 9.5 for the launch and the start, per iteration 2.4 (128 keys) and 0.6 + 1.75
+// per full tile (64 keys); splits cost a second launch, 3.5, and 0.45 per MB of
+// partials, which go through memory between the launches.
+// Measured (32 q heads over 8; 16 / 64 / 256 rows, us): 32 tokens over 30032
+// 49 / 52 / 51, over 120032 164 / 150 / 129; 128 over 4128 28 / 37 / 38, over
+// 16128 89 / 87 / 62; 512 over 512 30 / 18 / 29, over 2512 73 / 53 / 49.
+void choose_kernel(int Hkv, int64_t R, int M, int L, int* rc, int* ns_out) {
+  const double seen = L - 0.5 * (M - 1);  // keys of an average query
+  double least = 1e30;
+  for (int rows : {16, 64, 256}) {
+    const int keys = rows == 16 ? 256 : rows == 64 ? 128 : 64;  // of a workgroup's step
+    const int64_t pairs = Hkv * ((R + rows - 1) / rows);
+    const int steps = (L + keys - 1) / keys;
+    const int most = static_cast<int>(std::min<int64_t>({std::max<int64_t>(1, kSplitGrid / pairs), steps, kMaxSplits}));
+    for (int ns = 1; ns <= most; ns++) {
+      const int bps = (steps + ns - 1) / ns;
+      if (ns != (steps + bps - 1) / bps) continue;  // as another count
+      const double rounds = std::ceil(static_cast<double>(pairs) * ns / kSplitGrid);
+      // (the 64-row kernel's time is its last row tile's, the others' an average one's)
+      const double n = std::max(1.0, (rows == 64 ? L : seen) / (static_cast<double>(keys) * ns));
+      double t;
+      if (rows == 16) t = 5.0 + rounds * (5.0 + 1.31 * n) + (ns > 1 ? 2.0 : 0.0);
+      else
+        t = 9.5 + rounds * n * (rows == 64 ? 2.4 : 0.6 + 1.75 * std::min<double>(R, 256.0) / 256.0) +
+            (ns > 1 ? 3.5 + 0.45e-6 * 520.0 * pairs * rows * ns : 0.0);
+      if (t < least) {
+        least = t;
+        *rc = rows;
+        *ns_out = ns;
+      }
+    }
+  }
+}
+
 Kv4Plan make_plan(int Hq, int Hkv, int M, int L, bool weigh) {
   Kv4Plan a{};
   const int64_t R = static_cast<int64_t>(Hq / Hkv) * M;
-  a.rc = R <= 4 ? 4 : R <= 8 ? 8 : R <= 2 * kRows ? kRows : R <= 64 ? 64 : R <= 128 ? 128 : 256;
+  a.nw = 8;
+  int ns = 1, keys;  // keys of a workgroup's step
+  if (R <= 8) {
+    a.rc = R <= 4 ? 4 : 8;
+    // workgroups of 4 waves as long as one step of each covers the context
+    // with a workgroup per CU: they start and join sooner (32 heads over 8, us
+    // with 4 / 8 waves: 4097 rows 8.7 / 10.8, 8192 9.8 / 11.3, but 12001 14.0 / 12.2)
+    keys = a.rc == 4 ? 64 : 32;
+    a.nw = Hkv * ((L + 4 * keys - 1) / (4 * keys)) <= kSplitGrid ? 4 : 8;
+    keys *= a.nw;
+    ns = std::min<int64_t>({std::max<int64_t>(1, kSplitGrid / Hkv), (L + keys - 1) / keys, kMaxSplits});
+  } else {
+    choose_kernel(Hkv, R, M, L, &a.rc, &ns);
+    keys = a.rc == 16 ? 256 : a.rc == 64 ? 128 : 64;
+  }
+  const int steps = (L + keys - 1) / keys;
   a.tiles = static_cast<int>((R + a.rc - 1) / a.rc);
   const int64_t pairs = static_cast<int64_t>(Hkv) * a.tiles;
-  a.nw = a.rc < kRows && L <= 16384 ? 4 : 8;
-  // keys of a split's unit: a step of every wave, or an iteration
-  const int keys = a.rc == 4 ? 64 * a.nw : a.rc <= kRows ? 32 * a.nw : a.rc == 64 ? 128 : 64;
-  const int steps = (L + keys - 1) / keys;
-  const int64_t want = std::max<int64_t>(1, (a.rc < kRows && a.nw == 4 ? 2 * kSplitGrid : kSplitGrid) / pairs);
-  int ns = static_cast<int>(std::min<int64_t>({want, steps, kMaxSplits}));
   a.cnt_stride = pairs <= 128 ? 128 : 16;
   if (a.rc <= kRows && pairs * a.cnt_stride * 4 > BMX_KV4_COUNTER_BYTES) ns = 1;
   a.bps = (steps + ns - 1) / ns;
@@ -1457,15 +1494,16 @@ extern "C" int bmx_attention_gqa_kv4(const bmx_bf16* q, const bmx_kv4* cache, bm
   p.ns = a.ns;
   p.bps = a.bps;
   p.cnt_stride = a.cnt_stride;
+  // workgroups go to the XCDs in turn by their linear number, x first
+  p.local = a.rc <= kRows && a.ns > 1 && a.cnt_stride == 128 && Hkv % 8 == 0 && attention_xcd_local(as_stream(stream));
   const dim3 grid(Hkv, a.ns, a.tiles), block(64 * a.nw);
   const hipStream_t st = as_stream(stream);
   if (a.rc == 4 && a.nw == 4) hipLaunchKernelGGL((kv4_few_kernel<4, 4>), grid, block, 0, st, p);
   else if (a.rc == 4) hipLaunchKernelGGL((kv4_few_kernel<4, 8>), grid, block, 0, st, p);
   else if (a.rc == 8 && a.nw == 4) hipLaunchKernelGGL((kv4_few_kernel<8, 4>), grid, block, 0, st, p);
   else if (a.rc == 8) hipLaunchKernelGGL((kv4_few_kernel<8, 8>), grid, block, 0, st, p);
-  else if (a.rc == kRows) hipLaunchKernelGGL((kv4_rows_kernel<8, 1>), grid, block, 0, st, p);
+  else if (a.rc == kRows) hipLaunchKernelGGL((kv4_rows_kernel<8>), grid, block, 0, st, p);
   else if (a.rc == 64) hipLaunchKernelGGL(kv4_tile_kernel<2>, grid, block, 0, st, p);
-  else if (a.rc == 128) hipLaunchKernelGGL(kv4_tile_kernel<4>, grid, block, 0, st, p);
   else hipLaunchKernelGGL(kv4_tile_kernel<8>, grid, block, 0, st, p);
   if (int rc = check_launch("attention_kv4")) return rc;
   if (a.rc > kRows && a.ns > 1) {

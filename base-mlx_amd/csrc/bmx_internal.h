@@ -203,6 +203,9 @@ size_t attention_workspace_floats(int Hq, int M, int ns);
 // Runs the decode kernel's one-time device check (waits for the stream);
 // call before capturing a graph that holds decode attention.
 void attention_prepare(hipStream_t stream);
+// The result of that check: whether workgroups with equal linear numbers mod 8
+// share an XCD (false under capture until it has been made).
+bool attention_xcd_local(hipStream_t stream);
 // QK-norm + RoPE + KV write + decode attention in one kernel; kNoFit unless
 // M <= 16, M * (Hq / Hkv) <= 64 and ws holds one split per 256 keys of L_max.
 int launch_qkv_attention(const uint16_t* q, const uint16_t* k, const uint16_t* v, const uint16_t* q_norm,
