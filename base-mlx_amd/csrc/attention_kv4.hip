@@ -37,6 +37,8 @@ constexpr int kOs = kKv4Dim + 4;           // LDS stride of an output row
 
 typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8_t;
 typedef __attribute__((ext_vector_type(4))) float f32x4_t;
+typedef __attribute__((ext_vector_type(8))) _Float16 f16x8_t;
+typedef __attribute__((ext_vector_type(2))) _Float16 f16x2_t;
 typedef __attribute__((ext_vector_type(16))) float f32x16_t;
 typedef __attribute__((ext_vector_type(2))) float f32x2_t;
 typedef __attribute__((ext_vector_type(2))) unsigned u32x2_t;
@@ -67,6 +69,10 @@ __device__ __forceinline__ f32x4_t mfma(u32x4_t a, u32x4_t b, f32x4_t c) {
                                                  0, 0, 0);
 }
 
+__device__ __forceinline__ f32x16_t mfma32_f16(u32x4_t a, u32x4_t b, f32x16_t c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c, 0, 0,
+                                                0);
+}
 __device__ __forceinline__ f32x16_t mfma32(u32x4_t a, u32x4_t b, f32x16_t c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c,
                                                  0, 0, 0);
@@ -131,6 +137,10 @@ __device__ __forceinline__ void store_part(float* p, float x, float y) {
   __hip_atomic_store(reinterpret_cast<uint64_t*>(p), v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
+__device__ __forceinline__ uint32_t pack_f16(float a, float b) {  // round to nearest even
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2_t{a, b}, f16x2_t));
+}
+
 // Q_0 and Q_1 of a query row, each in three bf16 pieces that add up to it
 __device__ __forceinline__ u32x4_t q_pieces(const float (&qs)[2]) {
   const float h0 = round_bf(qs[0]), h1 = round_bf(qs[1]);
@@ -154,7 +164,7 @@ __device__ __forceinline__ void finish_row(const Kv4AttnParams& p, int kvh, int 
   const float inv = 1.0f / l;
   *reinterpret_cast<uint2*>(p.out + (static_cast<int64_t>(t) * p.Hq + h) * kKv4Dim + d) =
       make_uint2(pack_bf(o.x * inv, o.y * inv), pack_bf(o.z * inv, o.w * inv));
-  if (p.lse && d == 0) p.lse[static_cast<int64_t>(kvh) * rep * p.M + r] = make_float2(m * p.c2, log2f(l));
+  if (p.lse && d == 0) p.lse[static_cast<int64_t>(kvh) * rep * p.M + r] = make_float2(m, log2f(l));
 }
 
 template <int NW, int ROWS>
@@ -225,7 +235,8 @@ __device__ __forceinline__ void merge_splits(const Kv4AttnParams& p, JoinLds<NW,
 #pragma unroll 8
     for (; s < p.ns; s += groups) o += sm.wt[row][s] * load_o(it, s);
     if (groups == 1)
-      finish_row(p, kvh, r0 + row, d, make_float4(o[0], o[1], o[2], o[3]), sm.fin[row][0], sm.fin[row][1]);
+      finish_row(p, kvh, r0 + row, d, make_float4(o[0], o[1], o[2], o[3]), sm.fin[row][0] * p.c2,
+                 sm.fin[row][1]);
     else
       *reinterpret_cast<f32x4_t*>(&red[(n * items + it) * 4]) = o;
   }
@@ -234,8 +245,8 @@ __device__ __forceinline__ void merge_splits(const Kv4AttnParams& p, JoinLds<NW,
   for (int k = tid; k < items; k += kThreads) {
     f32x4_t o = *reinterpret_cast<const f32x4_t*>(&red[k * 4]);
     for (int i = 1; i < groups; i++) o += *reinterpret_cast<const f32x4_t*>(&red[(i * items + k) * 4]);
-    finish_row(p, kvh, r0 + (k >> 5), 4 * (k & 31), make_float4(o[0], o[1], o[2], o[3]), sm.fin[k >> 5][0],
-               sm.fin[k >> 5][1]);
+    finish_row(p, kvh, r0 + (k >> 5), 4 * (k & 31), make_float4(o[0], o[1], o[2], o[3]),
+               sm.fin[k >> 5][0] * p.c2, sm.fin[k >> 5][1]);
   }
 }
 
@@ -291,7 +302,7 @@ __device__ __forceinline__ void join_and_finish(const Kv4AttnParams& p, JoinLds<
     }
     if (sum != sum) mm = sum;
     if (p.ns == 1) {
-      finish_row(p, kvh, r0 + r, d, o, mm, sum);
+      finish_row(p, kvh, r0 + r, d, o, mm * p.c2, sum);
     } else {
       const int64_t at = (row0 + r) * p.ns + split;
       if (p.local) {
@@ -434,15 +445,16 @@ __global__ void __launch_bounds__(64 * NW) kv4_rows_kernel(const Kv4AttnParams p
   }
 
   const f32x4_t zero = {0.0f, 0.0f, 0.0f, 0.0f};
-  // edge: rows 0, 1 sum p~ b, rows 2, 3 sum p~ s, rows 4, 5 -23.5 sum p', of
-  // groups 0 and 1
-  f32x4_t acc[2][4], edge = zero;
+  // edge: rows 0, 1 sum p~ b, rows 2, 3 sum p~ s of groups 0, 1; mid: -23.5
+  // sum p', in every row (a register set per group: a zero row would carry one
+  // group's infinite scale to the other)
+  f32x4_t acc[2][4], edge = zero, mid[2] = {zero, zero};
 #pragma unroll
   for (int y = 0; y < 2; y++)
 #pragma unroll
     for (int i = 0; i < 4; i++) acc[y][i] = zero;
   float m = -INFINITY, l = 0.0f, slow[2] = {0.0f, 0.0f};
-  const uint32_t centre[2] = {li == 4 ? 0xC1BCC1BCu : 0u, li == 5 ? 0xC1BCC1BCu : 0u};  // bf16 -23.5 twice
+  const uint32_t centre = 0xC1BCC1BCu;  // bf16 -23.5 twice
   const uint32_t half_sel = li < 8 ? 0x01000504u : 0x07060302u;
   // (selector 0x0c gives a zero byte: rows from 4 on take nothing)
   const uint32_t odd_sel = li >= 4 ? 0x0c0c0c0cu : li & 1 ? 0x07060302u : 0x05040100u;
@@ -504,6 +516,7 @@ __global__ void __launch_bounds__(64 * NW) kv4_rows_kernel(const Kv4AttnParams p
 #pragma unroll
       for (int y = 0; y < 2; y++) {
         slow[y] *= a;
+        mid[y] *= a;
 #pragma unroll
         for (int i = 0; i < 4; i++) acc[y][i] *= a;
       }
@@ -544,7 +557,7 @@ __global__ void __launch_bounds__(64 * NW) kv4_rows_kernel(const Kv4AttnParams p
           {nibble_pair<3>(v[0], nk), nibble_pair<3>(v[1], nk), nibble_pair<3>(v[2], nk), nibble_pair<3>(v[3], nk)}};
 #pragma unroll
       for (int i = 0; i < 4; i++) acc[y][i] = mfma(a[i], pb[y], acc[y][i]);
-      edge = mfma(u32x4_t{centre[y], centre[y], centre[y], centre[y]}, pb[y], edge);
+      mid[y] = mfma(u32x4_t{centre, centre, centre, centre}, pb[y], mid[y]);
     }
     {
       // rows 0..3 of A: b_0, b_1, s_0, s_1 of the step's keys
@@ -571,7 +584,7 @@ __global__ void __launch_bounds__(64 * NW) kv4_rows_kernel(const Kv4AttnParams p
   float x[2];  // what every dim of a group gets besides its product
 #pragma unroll
   for (int y = 0; y < 2; y++)
-    x[y] = __shfl(edge[y], 16 + li, 64) + __builtin_fmaf(7.5f, __shfl(edge[2 + y], li, 64), __shfl(edge[y], li, 64)) +
+    x[y] = mid[y][0] + __builtin_fmaf(7.5f, __shfl(edge[2 + y], li, 64), __shfl(edge[y], li, 64)) +
            add_xor32(add_xor16(slow[y]));
   join_and_finish<NW, kRows>(p, sm, kvh, split, r0, RT, m, add_xor32(add_xor16(l)), acc, x);
 }
@@ -790,10 +803,13 @@ __device__ __forceinline__ u32x4_t lds_read(const uint16_t* p) { return *reinter
 __device__ __forceinline__ void reads_go_out() { asm volatile("" ::: "memory"); }
 
 constexpr float kFloatMax = 3.402823466e38f;
-// Whether every value of a group of scale s and bias b is a finite number
-__device__ __forceinline__ bool kv4_finite(float s, float b) {
-  return __builtin_fmaf(15.0f, fabsf(s), fabsf(b)) <= kFloatMax;
+// The largest magnitude that values of scale s and bias b may have (not a
+// finite number where the scale or bias is not)
+__device__ __forceinline__ float kv4_most(float s, float b) {
+  const float end = fabsf(__builtin_fmaf(15.0f, s, b));
+  return end <= kFloatMax ? fmaxf(end, fabsf(b)) : end;
 }
+__device__ __forceinline__ bool kv4_finite(float s, float b) { return kv4_most(s, b) <= kFloatMax; }
 
 // Many query rows: 32 RW of one kv head per workgroup of 8 waves, wave w with
 // rows 32 (w % RW) ..; the waves that share rows take different key tiles of
@@ -805,11 +821,16 @@ __device__ __forceinline__ bool kv4_finite(float s, float b) {
 //   l % 32, h = l / 32) holds keys 8 j + 4 h + i.  One more product adds
 //   b_g Q_g - 16 s_g Q_g: its k index runs over biases (lanes h = 0) and
 //   scales (h = 1), each against the three pieces of Q_0 and Q_1.
-//   V as bf16(s n + b), transposed: [dim][key], the keys of a half tile in
-//   the order the score lanes hold them (16 k + 4 h + i, 16 k + 8 + 4 h + i),
-//   so P is its own B operand; 16-byte pieces swizzled by the dim.  Rounding V
-//   (by 2^-8 at most, as a bf16 cache would) saves the two scaled copies of
-//   P and three products a tile.
+//   V as fp16 (s n + b) 2^(15 - e), 2^e the power of two above the key's
+//     values (found two iterations ahead), transposed: [dim][key], the keys of
+//     a half tile in the order the score lanes hold them (16 k + 4 h + i,
+//     16 k + 8 + 4 h + i), so P is its own B operand; 16-byte pieces swizzled
+//     by the dim.
+// The softmax runs over t = S c2 + e (the same product adds e), so P 2^(t - M)
+// V 2^-e needs no further scaling, and what a key's values weigh, not only its
+// score, decides what may round away.  With 11 bits in P and V the outputs are
+// off by little more than their own rounding: 0.0017 of the norm for 2048
+// tokens over 4096 rows, where bf16 for both gave 0.0028 (and 12 us of 162 less).
 // A value that is not finite (its scale or bias is not) goes to LDS as 0 and
 // marks the iteration; the rows that see it become NaN by themselves.
 template <int RW>
@@ -822,7 +843,7 @@ __global__ void __launch_bounds__(512) kv4_tile_kernel(const Kv4AttnParams p) {
     alignas(16) uint16_t kt[KPI][KS];
     alignas(16) uint16_t vt[kKv4Dim][KPI];
     alignas(16) uint32_t sb[2][KPI];  // K's biases, scales
-    alignas(16) float sf[2][KPI];     // the scales of group 0, group 1
+    alignas(16) float sf[2][KPI];     // the scales of group 0, group 1, times c2
   };
   struct Join {
     alignas(16) float os[4][kKeys][kOs];
@@ -830,7 +851,10 @@ __global__ void __launch_bounds__(512) kv4_tile_kernel(const Kv4AttnParams p) {
   };
   constexpr size_t kLds = sizeof(Stage) * 2 > sizeof(Join) ? sizeof(Stage) * 2 : sizeof(Join);
   __shared__ __align__(16) char lds[kLds];
-  __shared__ int mark[2];
+  // of four iterations in turn: whether some value is not finite, the keys' 2^(15 - e), e
+  __shared__ int mark[4];
+  __shared__ __align__(16) float vscale[4][KPI];
+  __shared__ uint32_t ve[4][KPI];
   Stage* const st = reinterpret_cast<Stage*>(lds);
   Join& jn = *reinterpret_cast<Join*>(lds);
   const int tid = threadIdx.x, wave = wave_id(), lane = tid & 63, lr = lane & 31, h = lane >> 5;
@@ -905,36 +929,38 @@ __global__ void __launch_bounds__(512) kv4_tile_kernel(const Kv4AttnParams p) {
   };
   auto stage = [&](int it, int buf) {
     Stage& s = st[buf];
+    const bool marked = __builtin_amdgcn_readfirstlane(mark[it & 3]) == it + 1;
 #pragma unroll
     for (int i = 0; i < W; i++)
       *reinterpret_cast<u32x4_t*>(&s.kt[k_key][8 * (k_word + i)]) = word_pairs(gk[i], nk);
     if (tid < 2 * KPI) {
       (&s.sb[0][0])[tid] = gsb;
       if (tid >= KPI) {
-        s.sf[0][tid - KPI] = lo_f(gsb);
-        s.sf[1][tid - KPI] = hi_f(gsb);
+        s.sf[0][tid - KPI] = lo_f(gsb) * p.c2;
+        s.sf[1][tid - KPI] = hi_f(gsb) * p.c2;
       }
     }
 #pragma unroll
     for (int v = 0; v < VJ; v++) {
       const int job = tid + 512 * v, hw = job & 31, quad = job >> 5;
-      const int r = quad & 7, pair = 4 * (quad >> 3) + 2 * (r >> 2) + (r & 1);
-      float sv[4], cv[4], most = 0.0f;
+      const int q8 = quad & 7, pair = 4 * (quad >> 3) + 2 * (q8 >> 2) + (q8 & 1);
+      float sv[4], cv[4];
+      const f32x4_t r = *reinterpret_cast<const f32x4_t*>(&vscale[it & 3][4 * quad]);
       const uint32_t half = hw < 16 ? 0x01000c0cu : 0x03020c0cu;  // the group's scale as a float
 #pragma unroll
       for (int i = 0; i < 4; i++) {
         sv[i] = __uint_as_float(__builtin_amdgcn_perm(0u, gs[v][i], half));
-        const float b = __uint_as_float(__builtin_amdgcn_perm(0u, gb[v][i], half));
-        cv[i] = __builtin_fmaf(-16.0f, sv[i], b);
-        most += __builtin_fmaf(15.0f, fabsf(sv[i]), fabsf(b));
+        cv[i] = __uint_as_float(__builtin_amdgcn_perm(0u, gb[v][i], half));
       }
-      if (!(most <= kFloatMax)) {  // one of them, or just their sum
+      if (marked) {
 #pragma unroll
         for (int i = 0; i < 4; i++)
-          if (!kv4_finite(sv[i], __uint_as_float(__builtin_amdgcn_perm(0u, gb[v][i], half)))) {
-            sv[i] = cv[i] = 0.0f;
-            atomicMax(&mark[buf], it + 1);
-          }
+          if (!kv4_finite(sv[i], cv[i])) sv[i] = cv[i] = 0.0f;
+      }
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        sv[i] *= r[i];
+        cv[i] = __builtin_fmaf(-16.0f, sv[i], cv[i] * r[i]);
       }
       const uint32_t p01 = gv[v][0] | (gv[v][1] << 16), p23 = gv[v][2] | (gv[v][3] << 16);
       const uint32_t a[4] = {nibble_pair<0>(p01, nk), nibble_pair<1>(p01, nk), nibble_pair<2>(p01, nk),
@@ -943,16 +969,41 @@ __global__ void __launch_bounds__(512) kv4_tile_kernel(const Kv4AttnParams p) {
                              nibble_pair<3>(p23, nk)};
 #pragma unroll
       for (int i = 0; i < 4; i++)
-        *reinterpret_cast<u32x2_t*>(&s.vt[4 * hw + i][((pair ^ (hw & 7)) * 2 + ((r >> 1) & 1)) * 4]) =
-            u32x2_t{pack_bf(__builtin_fmaf(sv[0], lo_f(a[i]), cv[0]), __builtin_fmaf(sv[1], hi_f(a[i]), cv[1])),
-                    pack_bf(__builtin_fmaf(sv[2], lo_f(b[i]), cv[2]), __builtin_fmaf(sv[3], hi_f(b[i]), cv[3]))};
+        *reinterpret_cast<u32x2_t*>(&s.vt[4 * hw + i][((pair ^ (hw & 7)) * 2 + ((q8 >> 1) & 1)) * 4]) =
+            u32x2_t{pack_f16(__builtin_fmaf(sv[0], lo_f(a[i]), cv[0]), __builtin_fmaf(sv[1], hi_f(a[i]), cv[1])),
+                    pack_f16(__builtin_fmaf(sv[2], lo_f(b[i]), cv[2]), __builtin_fmaf(sv[3], hi_f(b[i]), cv[3]))};
     }
+  };
+
+  // e of an iteration's keys, a lane each.  Not below -64, so that a sum of
+  // P 2^(15 - e) stays in range: values from 2^-93 on keep their 11 bits.
+  uint32_t bs = 0, bb = 0;
+  auto fetch_e = [&](int it) {
+    if (wave >= KPI / 64) return;
+    bs = load1(vsr, (it * KPI + tid) * 4);
+    bb = load1(vbr, (it * KPI + tid) * 4);
+  };
+  auto find_e = [&](int it) {
+    if (wave >= KPI / 64) return;
+    const float m0 = kv4_most(lo_f(bs), lo_f(bb)), m1 = kv4_most(hi_f(bs), hi_f(bb));
+    const bool ok0 = m0 <= kFloatMax, ok1 = m1 <= kFloatMax;
+    const float most = fmaxf(ok0 ? m0 : 0.0f, ok1 ? m1 : 0.0f);
+    const int e = max(static_cast<int>(__float_as_uint(most) >> 23) - 126, -64);
+    vscale[it & 3][tid] = __uint_as_float(static_cast<uint32_t>(127 + 15 - e) << 23);
+    ve[it & 3][tid] = __float_as_uint(static_cast<float>(e)) >> 16;
+    if (!__all(ok0 && ok1) && lane == 0) mark[it & 3] = it + 1;
   };
 
   const int iters = (kend_wg + KPI - 1) / KPI;
   const int it0 = split * p.bps, it1 = min(iters, it0 + p.bps);
-  if (tid < 2) mark[tid] = 0;
+  if (tid < 4) mark[tid] = 0;
   if (it0 < it1) fetch(it0);
+  __syncthreads();
+  for (int i = 0; i < 2; i++) {
+    fetch_e(it0 + i);
+    find_e(it0 + i);
+  }
+  fetch_e(it0 + 2);
 
   // ---- the query fragments: word 2 k + h of step k, in its pair order ----
   u32x4_t qf[8], pieces;
@@ -981,8 +1032,9 @@ __global__ void __launch_bounds__(512) kv4_tile_kernel(const Kv4AttnParams p) {
       for (int k = 0; k < 8; k++) dst[4 * (k & 3) + 2 * (k >> 2) + h] = qf[k];
       if (h == 0) dst[16] = q_pieces(qs);
     }
-    const float f = h ? -16.0f : 1.0f, qh[2] = {f * qs[0], f * qs[1]};
+    const float f = h ? -16.0f * p.c2 : p.c2, qh[2] = {f * qs[0], f * qs[1]};
     pieces = q_pieces(qh);
+    pieces.w = h ? 0u : 0x3f80u;  // e, once
   }
 
   f32x16_t acc[4];
@@ -1007,13 +1059,14 @@ __global__ void __launch_bounds__(512) kv4_tile_kernel(const Kv4AttnParams p) {
 #pragma unroll
     for (int i = 0; i < 16; i++) d0[i] = d1[i] = db[i] = 0.0f;
     const uint32_t w = s.sb[h][kl + lr];
-    const bool marked = __builtin_amdgcn_readfirstlane(mark[buf]) == it + 1;  // some value of the iteration is not finite
+    const uint32_t we = ve[it & 3][kl + lr];
+    const bool marked = __builtin_amdgcn_readfirstlane(mark[it & 3]) == it + 1;
 #pragma unroll
     for (int k = 0; k < 4; k++) {
       d0 = mfma32(kf[k], qf[k], d0);
       d1 = mfma32(kf[4 + k], qf[4 + k], d1);
     }
-    db = mfma32(u32x4_t{w, w, w, w}, pieces, db);
+    db = mfma32(u32x4_t{w, w, w, we}, pieces, db);
     float sc[16];
 #pragma unroll
     for (int j = 0; j < 4; j++) {
@@ -1039,34 +1092,30 @@ __global__ void __launch_bounds__(512) kv4_tile_kernel(const Kv4AttnParams p) {
 #pragma unroll
     for (int e = 1; e < 16; e++) bm = fmaxf(bm, sc[e]);
     bm = max_xor32(bm);
-    if (__any(moves(bm, m, p.c2))) {
-      const float mn = fmaxf(m, bm);
-      const float a = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - mn) * p.c2);
+    if (__any(moves(bm, m, 1.0f))) {
+      const float mn = ceilf(fmaxf(m, bm));  // whole, so that all steps from it are exact
+      const float a = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
       m = mn;
       l *= a;
 #pragma unroll
       for (int d = 0; d < 4; d++) acc[d] *= a;
     }
-    const float mc = m == -INFINITY ? 0.0f : m * p.c2;
+    // P up to 2^15 (its maximum is off by up to 2^8, see moves)
+    const float mc = (m == -INFINITY ? 0.0f : m) - 7.0f;
 #pragma unroll
-    for (int e = 0; e < 16; e++) sc[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[e], p.c2, -mc));
-    if (cut) {
-#pragma unroll
-      for (int e = 0; e < 16; e++)
-        if (key0 + 8 * (e >> 2) + 4 * h + (e & 3) >= lim) sc[e] = 0.0f;
-    }
-    float sum = 0.0f;
+    for (int e = 0; e < 16; e++) sc[e] = __builtin_amdgcn_exp2f(sc[e] - mc);
     u32x4_t pb[2];
 #pragma unroll
     for (int j = 0; j < 4; j++) {
-      sum += (sc[4 * j] + sc[4 * j + 1]) + (sc[4 * j + 2] + sc[4 * j + 3]);
-      pb[j >> 1][2 * (j & 1)] = pack_bf(sc[4 * j], sc[4 * j + 1]);
-      pb[j >> 1][2 * (j & 1) + 1] = pack_bf(sc[4 * j + 2], sc[4 * j + 3]);
+      const f32x4_t r = *reinterpret_cast<const f32x4_t*>(&vscale[it & 3][kl + 8 * j + 4 * h]);
+#pragma unroll
+      for (int i = 0; i < 4; i++) l = __builtin_fmaf(sc[4 * j + i], r[i], l);
+      pb[j >> 1][2 * (j & 1)] = pack_f16(sc[4 * j], sc[4 * j + 1]);
+      pb[j >> 1][2 * (j & 1) + 1] = pack_f16(sc[4 * j + 2], sc[4 * j + 3]);
     }
-    l += sum;
     if (more) read_k(buf, tile + 1);
 #pragma unroll
-    for (int k = 0; k < 8; k++) acc[k & 3] = mfma32(vf[k], pb[k >> 2], acc[k & 3]);
+    for (int k = 0; k < 8; k++) acc[k & 3] = mfma32_f16(vf[k], pb[k >> 2], acc[k & 3]);
     if (marked) {
       for (int e = 0; e < 16; e++) {
         const int key = key0 + 8 * (e >> 2) + 4 * h + (e & 3);
@@ -1079,7 +1128,7 @@ __global__ void __launch_bounds__(512) kv4_tile_kernel(const Kv4AttnParams p) {
     }
   };
 
-  __syncthreads();  // (the marks are cleared)
+  __syncthreads();  // (the marks are cleared, the first bounds found)
   if (it0 < it1) stage(it0, 0);
   if (it0 + 1 < it1) fetch(it0 + 1);
   __syncthreads();
@@ -1091,6 +1140,9 @@ __global__ void __launch_bounds__(512) kv4_tile_kernel(const Kv4AttnParams p) {
     if (wave >= 4) {
       if (it + 1 < it1) stage(it + 1, buf ^ 1);
       if (it + 2 < it1) fetch(it + 2);
+    } else {
+      find_e(it + 2);
+      fetch_e(it + 3);
     }
 #pragma unroll
     for (int t = 0; t < TPW; t++) multiply(it, buf, kwi * TPW + t, t + 1 < TPW);
@@ -1102,9 +1154,13 @@ __global__ void __launch_bounds__(512) kv4_tile_kernel(const Kv4AttnParams p) {
   }
 
   l = add_xor32(l);
-  if (l != l) m = l;  // a NaN score: the row stays NaN
+  m = l != l ? l : m - 22.0f;  // P had a factor 2^7, V 2^15; a NaN score: the row stays NaN
 #pragma unroll
-  for (int d = 0; d < 4; d++) acc[d] += add_xor32(poison[d >> 1]);
+  for (int d = 0; d < 4; d++) {
+    const float bad = add_xor32(poison[d >> 1]);
+#pragma unroll
+    for (int i = 0; i < 16; i++) acc[d][i] += bad;
+  }
   // ---- waves of the same rows, two by two ----
 #pragma unroll
   for (int half = KW / 2; half > 0; half >>= 1) {
@@ -1124,8 +1180,8 @@ __global__ void __launch_bounds__(512) kv4_tile_kernel(const Kv4AttnParams p) {
     __syncthreads();
     if (kwi < half) {
       const float mo = jn.ms[sl][lr], lo = jn.ls[sl][lr], mm = fmaxf(m, mo);
-      const float a = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - mm) * p.c2);
-      const float b = mo == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((mo - mm) * p.c2);
+      const float a = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mm);
+      const float b = mo == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mo - mm);
       l = __builtin_fmaf(l, a, lo * b);
       m = l != l ? l : mm;
 #pragma unroll
@@ -1179,7 +1235,7 @@ __global__ void __launch_bounds__(256) kv4_merge_kernel(const Kv4AttnParams p) {
 #pragma unroll 8
   for (int s = 0; s < p.ns; s++) {
     const float2 v = ml[s * kKeys];
-    const float f = v.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((v.x - m) * p.c2);
+    const float f = v.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(v.x - m);
     l = __builtin_fmaf(f, v.y, l);
     o += f * po[static_cast<int64_t>(s) * (kKeys * kKv4Dim / 4)];
   }

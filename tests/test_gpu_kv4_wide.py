@@ -1,0 +1,162 @@
+"""Attention over the 4-bit KV cache where its kernels for many rows, long
+contexts and unusual values run: against float64 on the same device, one kv
+head at a time."""
+import math
+
+import pytest
+import torch
+
+import bmx
+from test_gpu_kv4 import D, U24, U8, queries, random_cache
+
+pytestmark = pytest.mark.gpu
+
+
+def values(words, s, b):
+    n = (words.to(torch.int64)[..., None] >> (4 * torch.arange(8, device=words.device))) & 15
+    wide = lambda x: x.double().repeat_interleave(64, -1)
+    return n.reshape(*words.shape[:-1], D).double() * wide(s) + wide(b)
+
+
+def check(q, cache, past, scale=None, weigh=True):
+    """Outputs [M, Hq, 128] and weights of a call, each held to its bound:
+    U8 of the output for its rounding; P and V off by U8 each at most, against
+    the weighted magnitudes or against the centred nibbles and the middles
+    (U8 (2 mass + centred)); a score off by e moves its weight by a factor
+    within exp(2 e)."""
+    Hq, M, _ = q.shape
+    Hkv, L = cache.n_kv_heads, past + M
+    rep, scale = Hq // Hkv, 1 / math.sqrt(D) if scale is None else scale
+    w = torch.full((Hkv, cache.capacity), 0.5, device="cuda") if weigh else None
+    got = bmx.attention_kv4(q, cache, past, scale=scale, weights=w)
+    if weigh:  # the outputs are the same bits without
+        assert torch.equal(got, bmx.attention_kv4(q, cache, past, scale=scale))
+        assert (w[:, L:] == 0.5).all()
+    see = torch.arange(L, device="cuda") <= past + torch.arange(M, device="cuda")[:, None]
+    see = see.repeat(rep, 1)
+    diff = ref = 0.0
+    for h in range(Hkv):
+        k = values(cache.k[h, :L], cache.k_scales[h, :L], cache.k_biases[h, :L])
+        v = values(cache.v[h, :L], cache.v_scales[h, :L], cache.v_biases[h, :L])
+        qd = q[h * rep:(h + 1) * rep].double().reshape(rep * M, D)
+        s = torch.mm(qd, k.t().contiguous()) * scale
+        p = torch.softmax(s.masked_fill(~see, -math.inf), -1)
+        out = torch.mm(p, v)
+        mass = torch.mm(p, v.abs())
+        centred = 7.5 * torch.mm(p, cache.v_scales[h, :L].double().abs().repeat_interleave(64, -1))
+        e = 140 * U24 * abs(scale) * qd.abs().sum(-1, keepdim=True) * torch.maximum(
+            31 * cache.k_scales[h, :L].double().abs().amax(-1), cache.k_biases[h, :L].double().abs().amax(-1))
+        es = e.amax(-1, keepdim=True)
+        bound = U8 * out.abs() + 1.05 * (2 * es * mass + U8 * (2 * mass + centred)) + 2.0 ** -20 * (mass + centred) + 1e-30
+        g = got.view(M, Hq, D)[:, h * rep:(h + 1) * rep].transpose(0, 1).reshape(rep * M, D).double()
+        off = ((g - out).abs() / bound).max()
+        assert off < 1, f"kv head {h}: {float(off):.3g} of the bound"
+        diff, ref = diff + float((g - out).square().sum()), ref + float(out.square().sum())
+        if weigh:
+            want = 0.5 + p.sum(0)
+            tol = (p * (2 * es + 64 * U24)).sum(0) + 4 * U24 * (0.5 + want)
+            d = (w[h, :L].double() - want).abs()
+            assert (d <= tol).all(), f"kv head {h}: {float((d / tol).max()):.3g} of the weights' tolerance"
+    assert diff ** 0.5 < 3e-3 * ref ** 0.5, (diff / ref) ** 0.5
+    return got
+
+
+WIDE = [(32, 8, 512, 0), (32, 8, 511, 2001), (64, 8, 130, 70), (64, 8, 65, 3001), (16, 1, 777, 0), (64, 8, 40, 20000),
+        (16, 2, 700, 0), (64, 64, 30, 100), (6, 2, 1000, 0), (5, 5, 700, 33), (24, 3, 200, 1000), (12, 2, 333, 4100),
+        (16, 1, 64, 20001), (32, 8, 1, 12000), (64, 8, 1, 5001), (3, 3, 1, 300001), (8, 1, 1, 300001), (64, 8, 16, 9000)]
+
+
+@pytest.mark.parametrize("Hq,Hkv,M,past", WIDE)
+def test_wide(gpu, Hq, Hkv, M, past):
+    cache = random_cache(M + past, Hkv, past + M + 3, past + M)
+    check(queries(M, Hq, M), cache, past)
+
+
+# a call for each kernel: few rows, more, tiles of 64, of 256
+KERNELS = [(8, 2, 1, 700), (8, 2, 40, 70), (64, 8, 130, 70), (32, 8, 512, 0)]
+
+
+@pytest.mark.parametrize("Hq,Hkv,M,past", KERNELS)
+@pytest.mark.parametrize("scale", [-0.07, 1e-4, 0.6])
+def test_scales(gpu, Hq, Hkv, M, past, scale):
+    cache = random_cache(1, Hkv, past + M, past + M)
+    check(queries(M, Hq, M), cache, past, scale=scale)
+
+
+@pytest.mark.parametrize("Hq,Hkv,M,past", KERNELS)
+@pytest.mark.parametrize("kind", ["tiny", "huge", "ends", "rows", "rising", "groups", "negative"])
+def test_value_magnitudes(gpu, Hq, Hkv, M, past, kind):
+    """Values of 2^-60, 2^100 and 2^117 as a whole, of 2^-20 .. 2^20 from row to row,
+    rising along the context, of 2^12 between a row's groups, and negative scales."""
+    cache = random_cache(2, Hkv, past + M, past + M)
+    g = torch.Generator().manual_seed(5)
+    n = past + M
+    f = {"tiny": torch.full((n, 2), 2.0 ** -60), "huge": torch.full((n, 2), 2.0 ** 100),
+         "ends": torch.full((n, 2), 2.0 ** 117),
+         "rows": 2.0 ** torch.randint(-20, 21, (n, 1), generator=g).float().expand(n, 2),
+         "rising": 2.0 ** torch.linspace(-30, 30, n).round()[:, None].expand(n, 2),
+         "groups": torch.tensor([[2.0 ** -12, 1.0]]).expand(n, 2),
+         "negative": torch.where(torch.rand(n, 2, generator=g) < 0.5, -1.0, 1.0)}[kind].cuda()
+    cache.v_scales.mul_(f)
+    cache.v_biases.mul_(f)
+    check(queries(M, Hq, M), cache, past, weigh=False)
+
+
+@pytest.mark.parametrize("Hq,Hkv,M,past", KERNELS[1:])
+@pytest.mark.parametrize("kind", ["largest", "lowest", "nan"])
+def test_what_a_query_does_not_see(gpu, Hq, Hkv, M, past, kind):
+    """The last rows hold bf16's ends or NaN: the queries before keep their bits."""
+    cache = random_cache(3, Hkv, past + M + 9, past + M)
+    q = queries(M, Hq, M)
+    clean = bmx.attention_kv4(q, cache, past)
+    last = slice(past + M - 5, past + M)
+    most = torch.finfo(torch.bfloat16).max
+    value = {"largest": most, "lowest": -most, "nan": math.nan}[kind]
+    cache.v_biases[:, last] = value
+    cache.v_scales[:, last] = 0.0 if kind != "nan" else math.inf
+    cache.k_biases[:, last] = value
+    dirty = bmx.attention_kv4(q, cache, past)
+    assert torch.equal(dirty[:-5], clean[:-5])
+
+
+@pytest.mark.parametrize("Hq,Hkv,M,past", KERNELS)
+def test_bad_rows_stay_in_their_group(gpu, Hq, Hkv, M, past):
+    """A NaN key takes its kv head's rows that see it, an infinite value its group of 64."""
+    cache = random_cache(4, Hkv, past + M, past + M)
+    at = past + M // 2
+    cache.v[1, at, 8:] = 0x77777777  # (0 times infinity is no infinity)
+    cache.k_scales[0, at, 1] = math.nan
+    cache.v_scales[1, at, 1] = math.inf
+    w = torch.zeros(Hkv, past + M, device="cuda")
+    out = bmx.attention_kv4(queries(M, Hq, M), cache, past, weights=w).view(M, Hkv, Hq // Hkv, D)
+    sees = M // 2
+    assert out[sees:, 0].isnan().all() and torch.isfinite(out[:sees]).all()
+    assert not torch.isfinite(out[sees:, 1, :, 64:]).any() and torch.isfinite(out[:, 1, :, :64]).all()
+    assert torch.isfinite(out[:, 2:]).all()
+    assert w[0, :at + 1].isnan().all() and torch.isfinite(w[1:]).all()
+
+
+def test_steps_share_a_workspace_between_graphs(gpu):
+    """Two captured calls of different kernels, one workspace, replayed in turns."""
+    cache = random_cache(6, 8, 3000, 3000)
+    ws = bmx.attention_kv4_workspace(32, 8, 300, 3000, weigh=True)
+    calls = [(queries(1, 32, 1), 2999), (queries(2, 32, 300), 2500), (queries(3, 32, 5), 700)]
+    want, graphs = [], []
+    for q, past in calls:
+        w = torch.zeros(8, 3000, device="cuda")
+        want.append((bmx.attention_kv4(q, cache, past, weights=w, workspace=ws).clone(), w))
+    torch.cuda.synchronize()
+    for q, past in calls:
+        w, out = torch.zeros(8, 3000, device="cuda"), torch.empty(q.shape[1], 32 * D, dtype=torch.bfloat16, device="cuda")
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            w.zero_()
+            bmx.attention_kv4(q, cache, past, weights=w, workspace=ws, out=out)
+        graphs.append((graph, out, w))
+    for turn in range(3):
+        for i in (turn, (turn + 1) % 3, (turn + 2) % 3):
+            graphs[i][0].replay()
+        torch.cuda.synchronize()
+        for (graph, out, w), (o, ww) in zip(graphs, want):
+            assert torch.equal(out, o) and torch.equal(w, ww)
+            out.zero_()
