@@ -462,6 +462,8 @@ def kv4_write(k, v, cache, offset, stream=None):
     if k2 != 1 or v2 != 1:
         raise BmxError(BMX_E_ARG, "the 128 values of a row must be contiguous")
     H, M, D = ks
+    if M == 0 and 0 <= offset <= cache.capacity:
+        return  # (an empty tensor has no address)
     if H == 1:
         k0 = v0 = 0  # (the stride of an axis of one entry says nothing)
     if M == 1:
@@ -507,6 +509,8 @@ def qk_norm_rope_kv4(q, k, v, q_norm, k_norm, cache, offset, position=None, eps=
         raise BmxError(BMX_E_SHAPE, "q_norm and k_norm must hold 128 weights")
     Hq = q.shape[1] // 128
     out = _empty(stream, cache.device, torch.bfloat16, Hq, M, 128)
+    if M == 0 and 0 <= offset <= cache.capacity:
+        return out
     call("bmx_qk_norm_rope_kv4", q.data_ptr(), k.data_ptr(), v.data_ptr(), q_norm.data_ptr(), k_norm.data_ptr(),
          out.data_ptr(), cache._ref, M, Hq, 128, offset, offset if position is None else position, eps, theta,
          _stream(stream))

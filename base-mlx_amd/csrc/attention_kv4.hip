@@ -1518,10 +1518,11 @@ extern "C" int bmx_attention_gqa_kv4(const bmx_bf16* q, const bmx_kv4* cache, bm
                                      size_t workspace_bytes, void* stream) {
   if (int rc = check_kv4("attention_kv4", cache, head_dim)) return rc;
   if (!q || !out || !workspace) return set_error(BMX_E_ARG, "attention_kv4: null pointer");
-  const int Hkv = cache->n_kv_heads, L = offset + M;
+  const int Hkv = cache->n_kv_heads;
   if (M < 0 || n_heads <= 0 || n_heads % Hkv)
     return set_error(BMX_E_SHAPE, "attention_kv4: M=%d, %d heads over %d kv heads", M, n_heads, Hkv);
   if (int rc = check_kv4_rows("attention_kv4", cache, M, offset)) return rc;
+  const int L = offset + M;
   if (!aligned(q, 16) || !aligned(out, 16) || !aligned(workspace, 16) || !aligned(weights, 16))
     return set_error(BMX_E_ALIGN, "attention_kv4: q, out, weights and workspace must be 16-byte aligned");
   if (M == 0) return BMX_OK;
@@ -1531,6 +1532,8 @@ extern "C" int bmx_attention_gqa_kv4(const bmx_bf16* q, const bmx_kv4* cache, bm
   const size_t need = plan_bound(n_heads, Hkv, M, L, weights != nullptr);
   if (workspace_bytes < need || need < a.bytes)
     return set_error(BMX_E_ARG, "attention_kv4: workspace of %zu bytes, %zu needed", workspace_bytes, need);
+  const size_t bytes = static_cast<size_t>(n_heads) * M * kKv4Dim * sizeof(uint16_t);
+  if (kv4_overlap(q, bytes, out, bytes)) return set_error(BMX_E_ARG, "attention_kv4: out overlaps q");
   char* ws = static_cast<char*>(workspace);
   Kv4AttnParams p{};
   p.q = q;

@@ -19,6 +19,12 @@ int check_kv4(const char* what, const bmx_kv4* c, int head_dim);
 // ... and of rows [offset, offset + M) in it
 int check_kv4_rows(const char* what, const bmx_kv4* c, int M, int offset);
 
+// Whether a bytes from x and b bytes from y have any in common
+inline bool kv4_overlap(const void* x, size_t a, const void* y, size_t b) {
+  const uintptr_t i = reinterpret_cast<uintptr_t>(x), j = reinterpret_cast<uintptr_t>(y);
+  return i < j + b && j < i + a;
+}
+
 // bmx_kv4_read, checked arguments
 int launch_kv4_read(const bmx_kv4& c, uint16_t* k, uint16_t* v, int M, int start, hipStream_t stream);
 

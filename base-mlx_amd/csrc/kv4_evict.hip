@@ -512,6 +512,19 @@ bool same_pointers(const bmx_kv4& a, const bmx_kv4& b) {
          a.v_scales == b.v_scales && a.v_biases == b.v_biases;
 }
 
+// Whether any array of one cache (its weights among them) reaches into one of the other
+bool caches_overlap(const bmx_kv4& a, const float* aw, const bmx_kv4& b, const float* bw) {
+  const void* x[7] = {a.k, a.v, aw, a.k_scales, a.k_biases, a.v_scales, a.v_biases};
+  const void* y[7] = {b.k, b.v, bw, b.k_scales, b.k_biases, b.v_scales, b.v_biases};
+  const size_t rows_a = static_cast<size_t>(a.n_kv_heads) * a.capacity;
+  const size_t rows_b = static_cast<size_t>(b.n_kv_heads) * b.capacity;
+  auto bytes = [](int i, size_t rows) { return rows * (i < 2 ? kKv4Words * 4 : 4); };
+  for (int i = 0; i < 7; i++)
+    for (int j = 0; j < 7; j++)
+      if (kv4_overlap(x[i], bytes(i, rows_a), y[j], bytes(j, rows_b))) return true;
+  return false;
+}
+
 // Slices of a head and the rows of each (0: one workgroup holds the head)
 int select_slices(int length, int* rows) {
   if (length <= kOneWorkgroup) return 0;
@@ -550,6 +563,8 @@ extern "C" int bmx_kv4_evict(const bmx_kv4* cache, const float* weights, const b
   const bool in_place = same_pointers(*cache, *into);
   if (in_place != (weights == weights_into) || (in_place && into->capacity != cache->capacity))
     return set_error(BMX_E_ARG, "kv4_evict: cache and weights must both be in place, or neither");
+  if (!in_place && caches_overlap(*cache, weights, *into, weights_into))
+    return set_error(BMX_E_ARG, "kv4_evict: into overlaps the cache");
   const size_t need = bmx_kv4_evict_workspace_bytes(cache->n_kv_heads, length);
   if (need && (!workspace || workspace_bytes < need))
     return set_error(BMX_E_ARG, "kv4_evict: workspace of %zu bytes, %zu needed", workspace ? workspace_bytes : 0, need);

@@ -329,8 +329,12 @@ int bmx_qk_norm_rope_kv4(const bmx_bf16 *q, const bmx_bf16 *k, const bmx_bf16 *v
  * leaves them zero; 16-byte aligned; calls that share one must not run
  * concurrently) but not optional: bmx_attention_kv4_workspace_bytes for the
  * call's n_heads, n_kv_heads, M, L = offset + M and weights != NULL, or more
- * (BMX_E_ARG otherwise, nothing enqueued).  A call of many queries unpacks
- * the cache to bf16 there once: 512 bytes per row and kv head.
+ * (BMX_E_ARG otherwise, nothing enqueued).  out must not overlap q
+ * (BMX_E_ARG).  A row that a query does not see leaves it alone, whatever it
+ * holds; one that it sees, with a scale or bias that is not finite, makes
+ * that group's 64 outputs (V) or all of them and the kv head's weights (K)
+ * not finite.  Values up to 2^120 in magnitude keep their precision, with
+ * many queries those from 2^-93 on.
  * Replaces: mlx_rs::fast::scaled_dot_product_attention as
  *   bmx_attention_gqa does (crates/base-mlx-core/src/model/qwen3.rs:491-518);
  *   the reference has no quantized cache and no eviction. */
@@ -352,7 +356,7 @@ size_t bmx_attention_kv4_workspace_bytes(int n_heads, int n_kv_heads, int M, int
  * from `budget` on; kept [n_kv_heads, budget] their old row numbers.
  * into may be the cache itself (the same struct or equal pointers), and
  * weights_into weights, both then in place; otherwise nothing of `into` may
- * overlap the cache.  Rows of `into` from `budget` on stay as they are.
+ * overlap the cache (BMX_E_ARG).  Rows of `into` from `budget` on stay as they are.
  * sink, recent >= 0, sink + recent <= budget.  weights, weights_into and
  * kept: 16-byte aligned.  `workspace`: bmx_kv4_evict_workspace_bytes or more
  * for this n_kv_heads and length (16-byte aligned, any contents; NULL where

@@ -364,8 +364,9 @@ def test_workspace_needs_no_more_than_it_says(gpu):
         ws = torch.full((n + 4096,), 0xA5, dtype=torch.uint8, device="cuda")
         ws[:bmx.KV4_COUNTER_BYTES] = 0
         w = torch.zeros(Hkv, past + M, device="cuda") if weigh else None
-        rc = bmx.load().bmx_attention_gqa_kv4(queries(1, Hq, M).data_ptr(), cache._ref, torch.empty(M, Hq * D, dtype=torch.bfloat16, device="cuda").data_ptr(),
-                                              None if w is None else w.data_ptr(), Hq, M, D, past, 0.1, ws.data_ptr(), n, None)
+        q, out = queries(1, Hq, M), torch.empty(M, Hq * D, dtype=torch.bfloat16, device="cuda")
+        rc = bmx.load().bmx_attention_gqa_kv4(q.data_ptr(), cache._ref, out.data_ptr(), None if w is None else w.data_ptr(),
+                                              Hq, M, D, past, 0.1, ws.data_ptr(), n, None)
         torch.cuda.synchronize()
         assert rc == 0 and (ws[n:] == 0xA5).all()
 

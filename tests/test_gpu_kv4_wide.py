@@ -160,3 +160,19 @@ def test_steps_share_a_workspace_between_graphs(gpu):
         for (graph, out, w), (o, ww) in zip(graphs, want):
             assert torch.equal(out, o) and torch.equal(w, ww)
             out.zero_()
+
+
+def test_no_tokens(gpu):
+    """Calls of no tokens at all leave the cache as it is."""
+    cache = random_cache(7, 2, 20)
+    before = [t.clone() for t in (cache.k, cache.v, cache.k_scales.view(torch.int16))]
+    none = torch.empty(2, 0, D, dtype=torch.bfloat16, device="cuda")
+    bmx.kv4_write(none, none, cache, 20)
+    rows = [torch.empty(0, n * D, dtype=torch.bfloat16, device="cuda") for n in (4, 2, 2)]
+    unit = torch.ones(D, dtype=torch.bfloat16, device="cuda")
+    assert bmx.qk_norm_rope_kv4(*rows, unit, unit, cache, 20).shape == (4, 0, D)
+    assert bmx.attention_kv4(queries(1, 4, 1)[:, :0].contiguous(), cache, 20).shape == (0, 4 * D)
+    for f in (lambda: bmx.kv4_write(none, none, cache, 21), lambda: bmx.qk_norm_rope_kv4(*rows, unit, unit, cache, 21)):
+        with pytest.raises(bmx.BmxError):
+            f()
+    assert all(torch.equal(a, b) for a, b in zip(before, (cache.k, cache.v, cache.k_scales.view(torch.int16))))

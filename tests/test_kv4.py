@@ -180,3 +180,29 @@ def test_python_refusals_need_no_gpu():
     with pytest.raises(bmx.BmxError) as e:
         bmx.attention_kv4_workspace(4, 3, 1, 10)
     assert e.value.code == bmx.BMX_E_SHAPE
+
+
+def test_attention_refuses_out_over_q():
+    f = entry_points(kv4())["attention"]
+    assert f(q=P, out=P) == bmx.BMX_E_ARG and f(q=P, out=P + 4096 - 16) == bmx.BMX_E_ARG
+    assert "overlaps" in bmx.last_error()
+
+
+@pytest.mark.parametrize("shared", ["k", "k_scales", "k_biases", "v", "v_scales", "v_biases"])
+def test_evict_refuses_a_cache_over_itself(shared):
+    """`into` that shares one array, or the end of one, with the cache."""
+    far = dict(k=11 * P, k_scales=12 * P, k_biases=13 * P, v=14 * P, v_scales=15 * P, v_biases=16 * P)
+    c = kv4()
+    f = entry_points(c)["evict"]
+    for at in (getattr(c, shared), getattr(c, shared) + 784):
+        into = kv4(**{**far, shared: at})
+        assert f(into=ctypes.pointer(into), w_into=17 * P) == bmx.BMX_E_ARG
+        assert "overlaps" in bmx.last_error()
+    into = kv4(**far)
+    assert f(into=ctypes.pointer(into), w_into=7 * P + 784) == bmx.BMX_E_ARG
+
+
+def test_attention_row_range_does_not_wrap():
+    f = entry_points(kv4())["attention"]
+    assert f(M=2 ** 31 - 1, offset=100) == bmx.BMX_E_KV_CAPACITY
+    assert f(M=2, offset=2 ** 31 - 1) == bmx.BMX_E_KV_CAPACITY
