@@ -407,27 +407,37 @@ __global__ void __launch_bounds__(kThreads) kv4_emit_kernel(const SelectParams p
     __syncthreads();
     at += s.sel[0][0];
     const uint32_t all = s.first[kMaxSlices];
-    // every candidate of the head, 4 per thread at a time: f(key, slice, there is one)
+    // every candidate of the head, 4 per thread at a time: f(key, slice, or -1
+    // where there is none).  The first 4096 stay in registers.
+    auto fetch = [&](uint32_t g0, uint32_t (&key)[4], int (&from)[4]) {
+#pragma unroll
+      for (int k = 0; k < 4; k++) {
+        const uint32_t g = g0 + k * kThreads;
+        from[k] = -1;
+        key[k] = 0;
+        if (g < all) {
+          int lo = 0, hi = p.slices - 1;  // the last slice that starts at or before g
+          while (lo < hi) {
+            const int mid = (lo + hi + 1) >> 1;
+            if (s.first[mid] <= g) lo = mid;
+            else hi = mid - 1;
+          }
+          from[k] = lo;
+          key[k] = cand[static_cast<int64_t>(lo) * p.slice_rows + (g - s.first[lo])];
+        }
+      }
+    };
+    uint32_t held[4];
+    int held_from[4];
+    fetch(threadIdx.x, held, held_from);
     auto each = [&](auto f) {
-      for (uint32_t g0 = threadIdx.x; g0 - threadIdx.x < all; g0 += 4 * kThreads) {
+#pragma unroll
+      for (int k = 0; k < 4; k++)
+        if (static_cast<uint32_t>(k) * kThreads < all) f(held[k], held_from[k]);
+      for (uint32_t g0 = 4 * kThreads + threadIdx.x; g0 - threadIdx.x < all; g0 += 4 * kThreads) {
         uint32_t key[4];
         int from[4];
-#pragma unroll
-        for (int k = 0; k < 4; k++) {
-          const uint32_t g = g0 + k * kThreads;
-          from[k] = -1;
-          key[k] = 0;
-          if (g < all) {
-            int lo = 0, hi = p.slices - 1;  // the last slice that starts at or before g
-            while (lo < hi) {
-              const int mid = (lo + hi + 1) >> 1;
-              if (s.first[mid] <= g) lo = mid;
-              else hi = mid - 1;
-            }
-            from[k] = lo;
-            key[k] = cand[static_cast<int64_t>(lo) * p.slice_rows + (g - s.first[lo])];
-          }
-        }
+        fetch(g0, key, from);
 #pragma unroll
         for (int k = 0; k < 4; k++) f(key[k], from[k]);
       }
