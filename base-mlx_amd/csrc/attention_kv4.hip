@@ -92,6 +92,11 @@ struct PairK {
   uint32_t mask, one;
   __device__ __forceinline__ PairK() : mask(0x00780078u), one(0x41804180u) { asm volatile("" : "+v"(mask), "+v"(one)); }
 };
+struct PairH {  // ... of fp16 1024 + n
+  uint32_t mask, one;
+  __device__ __forceinline__ PairH() : mask(0x000f000fu), one(0x64006400u) { asm volatile("" : "+v"(mask), "+v"(one)); }
+};
+__device__ __forceinline__ f16x2_t half2(uint32_t x) { return __builtin_bit_cast(f16x2_t, x); }
 // Nibbles i and i + 4 of w as the bf16 pair (16 + n_i, 16 + n_(i+4))
 template <int I>
 __device__ __forceinline__ uint32_t nibble_pair(uint32_t w, const PairK& k) {
@@ -802,6 +807,10 @@ __device__ __forceinline__ u32x4_t lds_read(const uint16_t* p) { return *reinter
 // Reads before it stay before it, and so ahead of the branches that follow
 __device__ __forceinline__ void reads_go_out() { asm volatile("" ::: "memory"); }
 
+// Keeps what is done to x in a seldom taken branch there: without, the compiler
+// does it always and selects
+__device__ __forceinline__ void stay_here(float& x) { asm volatile("" : "+v"(x)); }
+
 constexpr float kFloatMax = 3.402823466e38f;
 // The largest magnitude that values of scale s and bias b may have (not a
 // finite number where the scale or bias is not)
@@ -822,13 +831,15 @@ __device__ __forceinline__ bool kv4_finite(float s, float b) { return kv4_most(s
 //   b_g Q_g - 16 s_g Q_g: its k index runs over biases (lanes h = 0) and
 //   scales (h = 1), each against the three pieces of Q_0 and Q_1.
 //   V as fp16 (s n + b) 2^(15 - e), 2^e the power of two above the key's
-//     values (found two iterations ahead), transposed: [dim][key], the keys of
+//     values (found two iterations ahead, with s and b times 2^(15 - e), which
+//     fp16 holds exactly), by packed fp16 arithmetic that rounds once; transposed: [dim][key], the keys of
 //     a half tile in the order the score lanes hold them (16 k + 4 h + i,
-//     16 k + 8 + 4 h + i), so P is its own B operand; 16-byte pieces swizzled
-//     by the dim.
-// The softmax runs over t = S c2 + e (the same product adds e), so P 2^(t - M)
-// V 2^-e needs no further scaling, and what a key's values weigh, not only its
-// score, decides what may round away.  With 11 bits in P and V the outputs are
+//     16 k + 8 + 4 h + i), so P is its own B operand.
+// The softmax runs over t = S c2 + e, so P = 2^(t - M) times V 2^-e needs no
+// further scaling, and what a key's values weigh, not only its score, decides
+// what may round away.  The product that adds the biases adds e and -M too, M
+// in three bf16 pieces; M moves only where P would pass 2^15, to make the
+// largest 2^7.  With 11 bits in P and V the outputs are
 // off by little more than their own rounding: 0.0017 of the norm for 2048
 // tokens over 4096 rows, where bf16 for both gave 0.0028 (and 12 us of 162 less).
 // A value that is not finite (its scale or bias is not) goes to LDS as 0 and
@@ -855,6 +866,7 @@ __global__ void __launch_bounds__(512) kv4_tile_kernel(const Kv4AttnParams p) {
   __shared__ int mark[4];
   __shared__ __align__(16) float vscale[4][KPI];
   __shared__ uint32_t ve[4][KPI];
+  __shared__ __align__(16) uint16_t vsb[4][2][2][KPI];  // ... scales, biases of group 0, 1, times 2^(15 - e), as fp16
   Stage* const st = reinterpret_cast<Stage*>(lds);
   Join& jn = *reinterpret_cast<Join*>(lds);
   const int tid = threadIdx.x, wave = wave_id(), lane = tid & 63, lr = lane & 31, h = lane >> 5;
@@ -891,6 +903,7 @@ __global__ void __launch_bounds__(512) kv4_tile_kernel(const Kv4AttnParams p) {
     if (first < R) kend_wg = max(kend_wg, end_of(first, min(kKeys, R - first)));
   }
   const PairK nk;
+  const PairH hk;
 
   const int64_t slot = static_cast<int64_t>(kvh) * p.c.capacity;
   const __amdgpu_buffer_rsrc_t kwr = rsrc(p.c.k, slot * kKv4Words, L * 64);
@@ -900,10 +913,14 @@ __global__ void __launch_bounds__(512) kv4_tile_kernel(const Kv4AttnParams p) {
   const __amdgpu_buffer_rsrc_t vsr = rsrc(reinterpret_cast<const uint32_t*>(p.c.v_scales), slot, L * 4);
   const __amdgpu_buffer_rsrc_t vbr = rsrc(reinterpret_cast<const uint32_t*>(p.c.v_biases), slot, L * 4);
 
+  // The 16-byte pieces of V's row d stand at their number xor this: different
+  // banks for the 16 rows that a read takes together (bits 0 .. 3 of d) and
+  // the rows 4 apart of a write (bits 2 .. 4)
+  auto swizzle = [](int d) { return (((d >> 1) & 7) ^ ((d >> 4) & 1)) | (KPI == 128 ? (d & 1) << 3 : 0); };
+
   // ---- staging: this thread's part of an iteration ----
   uint32_t gk[W], gsb = 0;
   uint32_t gv[VJ][4];
-  u32x4_t gs[VJ], gb[VJ];
   const int k_key = tid / (16 / W), k_word = W * (tid % (16 / W));
   auto fetch = [&](int it) {
     const int key0 = it * KPI;
@@ -923,13 +940,10 @@ __global__ void __launch_bounds__(512) kv4_tile_kernel(const Kv4AttnParams p) {
 #pragma unroll
       for (int i = 0; i < 4; i++)
         gv[v][i] = __builtin_amdgcn_raw_buffer_load_b16(vwr, (key0 + 4 * quad + i) * 64 + 2 * hw, 0, 0);
-      gs[v] = load4(vsr, (key0 + 4 * quad) * 4);
-      gb[v] = load4(vbr, (key0 + 4 * quad) * 4);
     }
   };
   auto stage = [&](int it, int buf) {
     Stage& s = st[buf];
-    const bool marked = __builtin_amdgcn_readfirstlane(mark[it & 3]) == it + 1;
 #pragma unroll
     for (int i = 0; i < W; i++)
       *reinterpret_cast<u32x4_t*>(&s.kt[k_key][8 * (k_word + i)]) = word_pairs(gk[i], nk);
@@ -944,34 +958,20 @@ __global__ void __launch_bounds__(512) kv4_tile_kernel(const Kv4AttnParams p) {
     for (int v = 0; v < VJ; v++) {
       const int job = tid + 512 * v, hw = job & 31, quad = job >> 5;
       const int q8 = quad & 7, pair = 4 * (quad >> 3) + 2 * (q8 >> 2) + (q8 & 1);
-      float sv[4], cv[4];
-      const f32x4_t r = *reinterpret_cast<const f32x4_t*>(&vscale[it & 3][4 * quad]);
-      const uint32_t half = hw < 16 ? 0x01000c0cu : 0x03020c0cu;  // the group's scale as a float
+      const uint32_t w[2] = {gv[v][0] | (gv[v][1] << 16), gv[v][2] | (gv[v][3] << 16)};
+      const u32x2_t sv = *reinterpret_cast<const u32x2_t*>(&vsb[it & 3][0][hw >> 4][4 * quad]);
+      const u32x2_t bv = *reinterpret_cast<const u32x2_t*>(&vsb[it & 3][1][hw >> 4][4 * quad]);
 #pragma unroll
       for (int i = 0; i < 4; i++) {
-        sv[i] = __uint_as_float(__builtin_amdgcn_perm(0u, gs[v][i], half));
-        cv[i] = __uint_as_float(__builtin_amdgcn_perm(0u, gb[v][i], half));
-      }
-      if (marked) {
+        u32x2_t x;
 #pragma unroll
-        for (int i = 0; i < 4; i++)
-          if (!kv4_finite(sv[i], cv[i])) sv[i] = cv[i] = 0.0f;
+        for (int y = 0; y < 2; y++) {
+          // 1024 + n as fp16, less 1024: n exactly; then one rounding
+          const f16x2_t n = half2((w[y] >> (4 * i) & hk.mask) | hk.one) - f16x2_t{1024.0f16, 1024.0f16};
+          x[y] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(n, half2(sv[y]), half2(bv[y])));
+        }
+        *reinterpret_cast<u32x2_t*>(&s.vt[4 * hw + i][((pair ^ swizzle(4 * hw + i)) * 2 + ((q8 >> 1) & 1)) * 4]) = x;
       }
-#pragma unroll
-      for (int i = 0; i < 4; i++) {
-        sv[i] *= r[i];
-        cv[i] = __builtin_fmaf(-16.0f, sv[i], cv[i] * r[i]);
-      }
-      const uint32_t p01 = gv[v][0] | (gv[v][1] << 16), p23 = gv[v][2] | (gv[v][3] << 16);
-      const uint32_t a[4] = {nibble_pair<0>(p01, nk), nibble_pair<1>(p01, nk), nibble_pair<2>(p01, nk),
-                             nibble_pair<3>(p01, nk)};
-      const uint32_t b[4] = {nibble_pair<0>(p23, nk), nibble_pair<1>(p23, nk), nibble_pair<2>(p23, nk),
-                             nibble_pair<3>(p23, nk)};
-#pragma unroll
-      for (int i = 0; i < 4; i++)
-        *reinterpret_cast<u32x2_t*>(&s.vt[4 * hw + i][((pair ^ (hw & 7)) * 2 + ((q8 >> 1) & 1)) * 4]) =
-            u32x2_t{pack_f16(__builtin_fmaf(sv[0], lo_f(a[i]), cv[0]), __builtin_fmaf(sv[1], hi_f(a[i]), cv[1])),
-                    pack_f16(__builtin_fmaf(sv[2], lo_f(b[i]), cv[2]), __builtin_fmaf(sv[3], hi_f(b[i]), cv[3]))};
     }
   };
 
@@ -989,8 +989,15 @@ __global__ void __launch_bounds__(512) kv4_tile_kernel(const Kv4AttnParams p) {
     const bool ok0 = m0 <= kFloatMax, ok1 = m1 <= kFloatMax;
     const float most = fmaxf(ok0 ? m0 : 0.0f, ok1 ? m1 : 0.0f);
     const int e = max(static_cast<int>(__float_as_uint(most) >> 23) - 126, -64);
-    vscale[it & 3][tid] = __uint_as_float(static_cast<uint32_t>(127 + 15 - e) << 23);
-    ve[it & 3][tid] = __float_as_uint(static_cast<float>(e)) >> 16;
+    const float r = __uint_as_float(static_cast<uint32_t>(127 + 15 - e) << 23);
+    const uint32_t x0 = ok0 ? pack_f16(lo_f(bs) * r, lo_f(bb) * r) : 0u;
+    const uint32_t x1 = ok1 ? pack_f16(hi_f(bs) * r, hi_f(bb) * r) : 0u;
+    vsb[it & 3][0][0][tid] = static_cast<uint16_t>(x0);
+    vsb[it & 3][1][0][tid] = static_cast<uint16_t>(x0 >> 16);
+    vsb[it & 3][0][1][tid] = static_cast<uint16_t>(x1);
+    vsb[it & 3][1][1][tid] = static_cast<uint16_t>(x1 >> 16);
+    vscale[it & 3][tid] = r;
+    ve[it & 3][tid] = 0x3f800000u | __float_as_uint(static_cast<float>(e)) >> 16;
     if (!__all(ok0 && ok1) && lane == 0) mark[it & 3] = it + 1;
   };
 
@@ -1034,7 +1041,7 @@ __global__ void __launch_bounds__(512) kv4_tile_kernel(const Kv4AttnParams p) {
     }
     const float f = h ? -16.0f * p.c2 : p.c2, qh[2] = {f * qs[0], f * qs[1]};
     pieces = q_pieces(qh);
-    pieces.w = h ? 0u : 0x3f80u;  // e, once
+    pieces.w = h ? 0u : 0x3f80u;  // the factor of e; the others take -M
   }
 
   f32x16_t acc[4];
@@ -1042,7 +1049,9 @@ __global__ void __launch_bounds__(512) kv4_tile_kernel(const Kv4AttnParams p) {
   for (int d = 0; d < 4; d++)
 #pragma unroll
     for (int i = 0; i < 16; i++) acc[d][i] = 0.0f;
-  float m = -INFINITY, l = 0.0f, poison[2] = {0.0f, 0.0f};
+  // M is whole, so that the steps from one to the next are exact; `most` is the
+  // largest t - M that leaves it as it is, -infinity before the first M
+  float m = 0.0f, most = -INFINITY, l = 0.0f, poison[2] = {0.0f, 0.0f};
 
   // K's fragments of the tile to come: read while P V of the one before runs
   u32x4_t kf[8];
@@ -1059,7 +1068,7 @@ __global__ void __launch_bounds__(512) kv4_tile_kernel(const Kv4AttnParams p) {
 #pragma unroll
     for (int i = 0; i < 16; i++) d0[i] = d1[i] = db[i] = 0.0f;
     const uint32_t w = s.sb[h][kl + lr];
-    const uint32_t we = ve[it & 3][kl + lr];
+    const uint32_t e1 = ve[it & 3][kl + lr], we = h ? 0x3f803f80u : e1;
     const bool marked = __builtin_amdgcn_readfirstlane(mark[it & 3]) == it + 1;
 #pragma unroll
     for (int k = 0; k < 4; k++) {
@@ -1080,30 +1089,36 @@ __global__ void __launch_bounds__(512) kv4_tile_kernel(const Kv4AttnParams p) {
     u32x4_t vf[8];
 #pragma unroll
     for (int k = 0; k < 8; k++)
-      vf[k] = lds_read(&s.vt[32 * (k & 3) + lr][((4 * tile + 2 * (k >> 2) + h) ^ ((lr >> 2) & 7)) * 8]);
+      vf[k] = lds_read(&s.vt[32 * (k & 3) + lr][((4 * tile + 2 * (k >> 2) + h) ^ swizzle(lr)) * 8]);
     reads_go_out();
     const bool cut = key0 + kKeys > all_see;
     if (cut) {
+      const int first = lim - key0 - 4 * h;  // hidden from here on
 #pragma unroll
-      for (int e = 0; e < 16; e++)
-        if (key0 + 8 * (e >> 2) + 4 * h + (e & 3) >= lim) sc[e] = -INFINITY;
+      for (int e = 0; e < 16; e++) {
+        stay_here(sc[e]);
+        if (8 * (e >> 2) + (e & 3) >= first) sc[e] = -INFINITY;
+      }
     }
     float bm = sc[0];
 #pragma unroll
     for (int e = 1; e < 16; e++) bm = fmaxf(bm, sc[e]);
     bm = max_xor32(bm);
-    if (__any(moves(bm, m, 1.0f))) {
-      const float mn = ceilf(fmaxf(m, bm));  // whole, so that all steps from it are exact
-      const float a = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
-      m = mn;
+    if (__any(bm > most)) {
+      const float up = bm > most ? ceilf(bm) - 7.0f : 0.0f;
+      const float a = most == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(-up);
+      if (bm > most) most = 15.0f;
+      m += up;
+      const float m0 = round_bf(-m), m1 = round_bf(-m - m0);
+      pieces.w = h ? pack_bf(m1, -m - m0 - m1) : pack_bf(1.0f, m0);
+#pragma unroll
+      for (int e = 0; e < 16; e++) sc[e] -= up;
       l *= a;
 #pragma unroll
       for (int d = 0; d < 4; d++) acc[d] *= a;
     }
-    // P up to 2^15 (its maximum is off by up to 2^8, see moves)
-    const float mc = (m == -INFINITY ? 0.0f : m) - 7.0f;
 #pragma unroll
-    for (int e = 0; e < 16; e++) sc[e] = __builtin_amdgcn_exp2f(sc[e] - mc);
+    for (int e = 0; e < 16; e++) sc[e] = __builtin_amdgcn_exp2f(sc[e]);
     u32x4_t pb[2];
 #pragma unroll
     for (int j = 0; j < 4; j++) {
@@ -1117,6 +1132,7 @@ __global__ void __launch_bounds__(512) kv4_tile_kernel(const Kv4AttnParams p) {
 #pragma unroll
     for (int k = 0; k < 8; k++) acc[k & 3] = mfma32_f16(vf[k], pb[k >> 2], acc[k & 3]);
     if (marked) {
+#pragma unroll 1
       for (int e = 0; e < 16; e++) {
         const int key = key0 + 8 * (e >> 2) + 4 * h + (e & 3);
         const uint32_t sw = load1(vsr, key * 4), bw = load1(vbr, key * 4);
@@ -1154,7 +1170,7 @@ __global__ void __launch_bounds__(512) kv4_tile_kernel(const Kv4AttnParams p) {
   }
 
   l = add_xor32(l);
-  m = l != l ? l : m - 22.0f;  // P had a factor 2^7, V 2^15; a NaN score: the row stays NaN
+  m = l != l ? l : most == -INFINITY ? most : m - 15.0f;  // V had a factor 2^15; a NaN score: the row stays NaN
 #pragma unroll
   for (int d = 0; d < 4; d++) {
     const float bad = add_xor32(poison[d >> 1]);
