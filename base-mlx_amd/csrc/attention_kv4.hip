@@ -1423,20 +1423,22 @@ struct Kv4Plan {
 };
 
 // The kernel and split count for R > 8 query rows per kv head, by estimated
-// time (us).  16 rows: 5 for the launch, and per round of 256 workgroups 5 and
-// 1.31 per step of a wave (32 keys; two waves share a SIMD).  64 and 256 rows:
-// 9.5 for the launch and the start, per iteration 2.4 (128 keys) and 0.6 + 1.75
-// per full tile (64 keys); splits cost a second launch, 3.5, and 0.45 per MB of
-// partials, which go through memory between the launches.
+// time (us) over rounds of 256 workgroups.  16 rows: 5 a round and 1.32 per
+// step of a wave (32 keys; two waves share a SIMD).  64 and 256 rows: 1.92 per
+// iteration (128 keys), 2.05 + 0.58 per full tile (64 keys).  Splits cost the
+// last workgroup's merge, or a second launch that reads all partials from
+// memory: by their number, where that walk is long, or by their size.
 // Measured (32 q heads over 8; 16 / 64 / 256 rows, us): 32 tokens over 30032
-// 49 / 52 / 51, over 120032 164 / 150 / 129; 128 over 4128 28 / 37 / 38, over
-// 16128 89 / 87 / 62; 512 over 512 30 / 18 / 29, over 2512 73 / 53 / 49.
+// 51 / 50 / 56; 128 over 4128 27 / 33 / 37, over 16128 86 / 75 / 62; 200 over
+// 200 12 / 12 / 17; 512 over 512 27 / 16 / 23, over 2512 68 / 44 / 48; 1024
+// over 1024 61 / 43 / 38.
 void choose_kernel(int Hkv, int64_t R, int M, int L, int* rc, int* ns_out) {
   const double seen = L - 0.5 * (M - 1);  // keys of an average query
   double least = 1e30;
   for (int rows : {16, 64, 256}) {
     const int keys = rows == 16 ? 256 : rows == 64 ? 128 : 64;  // of a workgroup's step
     const int64_t pairs = Hkv * ((R + rows - 1) / rows);
+    if ((R + rows - 1) / rows > 65535) continue;  // (grid z)
     const int steps = (L + keys - 1) / keys;
     const int most = static_cast<int>(std::min<int64_t>({std::max<int64_t>(1, kSplitGrid / pairs), steps, kMaxSplits}));
     for (int ns = 1; ns <= most; ns++) {
@@ -1446,10 +1448,11 @@ void choose_kernel(int Hkv, int64_t R, int M, int L, int* rc, int* ns_out) {
       // (the 64-row kernel's time is its last row tile's, the others' an average one's)
       const double n = std::max(1.0, (rows == 64 ? L : seen) / (static_cast<double>(keys) * ns));
       double t;
-      if (rows == 16) t = 5.0 + rounds * (5.0 + 1.31 * n) + (ns > 1 ? 2.0 : 0.0);
+      if (rows == 16) t = 1.0 + rounds * (5.0 + 1.32 * n) + (ns > 1 ? 3.0 : 0.0);
+      else if (rows == 64) t = 8.6 + rounds * n * 1.92 + (ns > 1 ? 5.3 + 0.42 * ns : 0.0);
       else
-        t = 9.5 + rounds * n * (rows == 64 ? 2.4 : 0.6 + 1.75 * std::min<double>(R, 256.0) / 256.0) +
-            (ns > 1 ? 3.5 + 0.45e-6 * 520.0 * pairs * rows * ns : 0.0);
+        t = 13.0 + rounds * n * (2.05 + 0.58 * std::min<double>(R, 256.0) / 256.0) +
+            (ns > 1 ? 0.5 + 0.38e-6 * 520.0 * kKeys * Hkv * ((R + kKeys - 1) / kKeys) * ns : 0.0);
       if (t < least) {
         least = t;
         *rc = rows;
