@@ -603,7 +603,8 @@ __global__ void __launch_bounds__(64 * NW) kv4_rows_kernel(const Kv4AttnParams p
 // column's tile is not the product's, two tiles to a product.  The columns of
 // a query are added at the end.  The sums over a lane's own keys that take
 // p', s and b (see the top) are fp32 here.
-// One token over 131072 rows, 32 heads of 8: 44 us with the kernel above.
+// One token over 131072 rows, 32 heads of 8: 33 us, 4.6 TB/s, where the kernel
+// above takes 44.
 template <int RC, int NW>
 __global__ void __launch_bounds__(64 * NW) kv4_few_kernel(const Kv4AttnParams p) {
   constexpr int T = 16 / RC, kStep = 16 * T;
@@ -831,17 +832,24 @@ __device__ __forceinline__ bool kv4_finite(float s, float b) { return kv4_most(s
 //   b_g Q_g - 16 s_g Q_g: its k index runs over biases (lanes h = 0) and
 //   scales (h = 1), each against the three pieces of Q_0 and Q_1.
 //   V as fp16 (s n + b) 2^(15 - e), 2^e the power of two above the key's
-//     values (found two iterations ahead, with s and b times 2^(15 - e), which
-//     fp16 holds exactly), by packed fp16 arithmetic that rounds once; transposed: [dim][key], the keys of
-//     a half tile in the order the score lanes hold them (16 k + 4 h + i,
-//     16 k + 8 + 4 h + i), so P is its own B operand.
+//     values, transposed: [dim][key], the keys of a half tile in the order the
+//     score lanes hold them (16 k + 4 h + i, 16 k + 8 + 4 h + i), so P is its
+//     own B operand.  Two iterations ahead a lane per key finds e and turns s
+//     and b into fp16 (exactly: 8 bits); a pair of values is then a packed
+//     subtraction and a packed multiply-add, which rounds once.
 // The softmax runs over t = S c2 + e, so P = 2^(t - M) times V 2^-e needs no
 // further scaling, and what a key's values weigh, not only its score, decides
 // what may round away.  The product that adds the biases adds e and -M too, M
 // in three bf16 pieces; M moves only where P would pass 2^15, to make the
-// largest 2^7.  With 11 bits in P and V the outputs are
-// off by little more than their own rounding: 0.0017 of the norm for 2048
-// tokens over 4096 rows, where bf16 for both gave 0.0028 (and 12 us of 162 less).
+// largest 2^7.  With 11 bits in P and V the outputs are off by little more
+// than their own rounding: 0.0017 of the norm for 2048 tokens over 4096 rows,
+// where bf16 for both gave 0.0028.
+// 2048 tokens over 4096 rows, 32 heads of 8: 145 us, 710 TFLOP/s, 56 % of what
+// a large matrix product reaches.  A tile of 32 x 32 takes 17 products of 32
+// cycles and about 120 VALU instructions of 4 with its share of the unpacking,
+// 16 of them exponentials of 16: the two hardly overlap, so the VALU work is
+// half the time.  Rates of the counters: matrix cores busy 36 %, VALU 49 %,
+// LDS 44 %, 1 / 9 of that in bank conflicts.
 // A value that is not finite (its scale or bias is not) goes to LDS as 0 and
 // marks the iteration; the rows that see it become NaN by themselves.
 template <int RW>
@@ -978,13 +986,12 @@ __global__ void __launch_bounds__(512) kv4_tile_kernel(const Kv4AttnParams p) {
   // e of an iteration's keys, a lane each.  Not below -64, so that a sum of
   // P 2^(15 - e) stays in range: values from 2^-93 on keep their 11 bits.
   uint32_t bs = 0, bb = 0;
+  const int ahead = wave / (KPI / 64), ke = tid - KPI * ahead;  // waves with `ahead` 0, and 1 at the start
   auto fetch_e = [&](int it) {
-    if (wave >= KPI / 64) return;
-    bs = load1(vsr, (it * KPI + tid) * 4);
-    bb = load1(vbr, (it * KPI + tid) * 4);
+    bs = load1(vsr, (it * KPI + ke) * 4);
+    bb = load1(vbr, (it * KPI + ke) * 4);
   };
   auto find_e = [&](int it) {
-    if (wave >= KPI / 64) return;
     const float m0 = kv4_most(lo_f(bs), lo_f(bb)), m1 = kv4_most(hi_f(bs), hi_f(bb));
     const bool ok0 = m0 <= kFloatMax, ok1 = m1 <= kFloatMax;
     const float most = fmaxf(ok0 ? m0 : 0.0f, ok1 ? m1 : 0.0f);
@@ -992,37 +999,41 @@ __global__ void __launch_bounds__(512) kv4_tile_kernel(const Kv4AttnParams p) {
     const float r = __uint_as_float(static_cast<uint32_t>(127 + 15 - e) << 23);
     const uint32_t x0 = ok0 ? pack_f16(lo_f(bs) * r, lo_f(bb) * r) : 0u;
     const uint32_t x1 = ok1 ? pack_f16(hi_f(bs) * r, hi_f(bb) * r) : 0u;
-    vsb[it & 3][0][0][tid] = static_cast<uint16_t>(x0);
-    vsb[it & 3][1][0][tid] = static_cast<uint16_t>(x0 >> 16);
-    vsb[it & 3][0][1][tid] = static_cast<uint16_t>(x1);
-    vsb[it & 3][1][1][tid] = static_cast<uint16_t>(x1 >> 16);
-    vscale[it & 3][tid] = r;
-    ve[it & 3][tid] = 0x3f800000u | __float_as_uint(static_cast<float>(e)) >> 16;
+    vsb[it & 3][0][0][ke] = static_cast<uint16_t>(x0);
+    vsb[it & 3][1][0][ke] = static_cast<uint16_t>(x0 >> 16);
+    vsb[it & 3][0][1][ke] = static_cast<uint16_t>(x1);
+    vsb[it & 3][1][1][ke] = static_cast<uint16_t>(x1 >> 16);
+    vscale[it & 3][ke] = r;
+    ve[it & 3][ke] = 0x3f800000u | __float_as_uint(static_cast<float>(e)) >> 16;
     if (!__all(ok0 && ok1) && lane == 0) mark[it & 3] = it + 1;
   };
 
   const int iters = (kend_wg + KPI - 1) / KPI;
   const int it0 = split * p.bps, it1 = min(iters, it0 + p.bps);
+  // everything that the start waits for, at once
   if (tid < 4) mark[tid] = 0;
+  if (ahead < 2) fetch_e(it0 + ahead);
   if (it0 < it1) fetch(it0);
-  __syncthreads();
-  for (int i = 0; i < 2; i++) {
-    fetch_e(it0 + i);
-    find_e(it0 + i);
+  uint4 qd[8];
+  {
+    const uint16_t* qr = p.q + (row0 + row) * kKv4Dim + 8 * h;
+#pragma unroll
+    for (int k = 0; k < 8; k++) qd[k] = *reinterpret_cast<const uint4*>(qr + 16 * k);
   }
-  fetch_e(it0 + 2);
+  __syncthreads();
+  if (ahead < 2) find_e(it0 + ahead);
+  if (ahead == 0) fetch_e(it0 + 2);
 
   // ---- the query fragments: word 2 k + h of step k, in its pair order ----
   u32x4_t qf[8], pieces;
   {
-    const uint16_t* qr = p.q + (row0 + row) * kKv4Dim + 8 * h;
     float qs[2];
 #pragma unroll
     for (int y = 0; y < 2; y++) {
       qs[y] = 0.0f;
 #pragma unroll
       for (int k = 0; k < 4; k++) {
-        uint4 d = *reinterpret_cast<const uint4*>(qr + 64 * y + 16 * k);
+        uint4 d = qd[4 * y + k];
         d.x ^= p.flip;
         d.y ^= p.flip;
         d.z ^= p.flip;
@@ -1156,7 +1167,7 @@ __global__ void __launch_bounds__(512) kv4_tile_kernel(const Kv4AttnParams p) {
     if (wave >= 4) {
       if (it + 1 < it1) stage(it + 1, buf ^ 1);
       if (it + 2 < it1) fetch(it + 2);
-    } else {
+    } else if (ahead == 0) {
       find_e(it + 2);
       fetch_e(it + 3);
     }
