@@ -177,3 +177,81 @@ def test_no_tokens(gpu):
         with pytest.raises(bmx.BmxError):
             f()
     assert all(torch.equal(a, b) for a, b in zip(before, (cache.k, cache.v, cache.k_scales.view(torch.int16))))
+
+
+@pytest.mark.parametrize("Hq,Hkv,M,past", KERNELS)
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+def test_a_bad_query_stays_alone(gpu, Hq, Hkv, M, past, bad):
+    """A NaN or infinity in one query: every other row keeps its bits."""
+    cache = random_cache(8, Hkv, past + M, past + M)
+    q = queries(M, Hq, M)
+    want = bmx.attention_kv4(q, cache, past).view(M, Hq, D)
+    h, t = Hq // 2, M // 2
+    q[h, t, 70] = bad
+    got = bmx.attention_kv4(q, cache, past).view(M, Hq, D)
+    same = torch.ones(M, Hq, dtype=torch.bool, device="cuda")
+    same[t, h] = False
+    assert torch.equal(got[same], want[same]) and not torch.isfinite(got[t, h]).all()
+
+
+def test_two_streams_at_once(gpu):
+    """Calls on two streams with a workspace each, queued without waiting."""
+    cache = random_cache(9, 8, 5000, 5000)
+    calls = [(queries(i, 32, M), past) for i, (M, past) in enumerate([(1, 4999), (5, 3000), (300, 100), (1, 10)])]
+    want = [bmx.attention_kv4(q, cache, past) for q, past in calls]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    spaces = [bmx.attention_kv4_workspace(32, 8, 300, 5000) for _ in streams]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for turn in range(10):
+        for i, (s, ws) in enumerate(zip(streams, spaces)):
+            q, past = calls[(turn + i) % 4]
+            got[i].append(bmx.attention_kv4(q, cache, past, workspace=ws, stream=s))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for turn in range(10):
+            assert torch.equal(got[i][turn], want[(turn + i) % 4]), (i, turn)
+
+
+def test_past_four_gib(gpu):
+    """Heads whose rows lie more than 2^32 bytes into the cache: written, read,
+    attended over, weighed and cut.  All rows but the last ten are zeros, which
+    score 0 and add nothing."""
+    Hkv, Hq, cap, new = 8, 16, 9_000_000, 10
+    past = cap - new
+    cache, w = bmx.Kv4Cache.empty(Hkv, cap), torch.zeros(Hkv, cap, device="cuda")
+    g = torch.Generator().manual_seed(1)
+    k, v = ((4 * torch.randn(Hkv, new, D, generator=g)).to(torch.bfloat16).cuda() for _ in "kv")
+    bmx.kv4_write(k, v, cache, past)
+    rk, rv = bmx.kv4_read(cache, past - 1, cap)
+    assert not rk[:, 0].any() and not rv[:, 0].any()
+    kd, vd = (values(*(getattr(cache, n + s)[:, past:] for s in ("", "_scales", "_biases"))) for n in "kv")
+    assert torch.equal(rk[:, 1:], kd.float().to(torch.bfloat16)) and torch.equal(rv[:, 1:], vd.float().to(torch.bfloat16))
+    for M in (1, new):  # few rows, more
+        lo = cap - M
+        q = queries(3 + M, Hq, M, std=4.0)
+        w.zero_()
+        got = bmx.attention_kv4(q, cache, lo, weights=w).view(M, Hkv, 2, D)
+        s = torch.matmul(q.double().view(Hkv, 2 * M, D), kd.transpose(1, 2).contiguous()) / math.sqrt(D)
+        see = (torch.arange(new, device="cuda") - (new - M) <= torch.arange(M, device="cuda")[:, None]).repeat(2, 1)
+        x = torch.where(see, s.exp(), 0.0)
+        p = x / (past + x.sum(-1, keepdim=True))
+        out = torch.matmul(p, vd).view(Hkv, 2, M, D).permute(2, 0, 1, 3)
+        # outputs as above: U8 for the rounding, U8 (2 mass + centred) for P and V
+        size = 3 * vd.abs() + 7.5 * cache.v_scales[:, past:].double().abs().repeat_interleave(64, -1)
+        size = torch.matmul(p, size).view(Hkv, 2, M, D).permute(2, 0, 1, 3)
+        assert ((got.double() - out).abs() <= 1.05 * U8 * size + 1e-12).all()
+        # weights: a sum of 9 million equal terms is off by far less than 1e-4
+        tol = 1e-4 * p.sum(1) + 1e-12
+        assert ((w[:, past:].double() - p.sum(1)).abs() <= tol).all()
+        zero = (1 / (past + x.sum(-1))).sum(-1, keepdim=True)
+        assert ((w[:, ::1000003].double() - zero).abs() <= 1e-4 * zero).all()
+    r = torch.rand(Hkv, cap, generator=g)
+    w.copy_(r)
+    into, wi = bmx.Kv4Cache.empty(Hkv, 1000), torch.empty(Hkv, 1000, device="cuda")
+    kept = bmx.kv4_evict(cache, w, cap, 1000, sink=4, recent=new, into=into, weights_into=wi)
+    order = torch.sort(w[:, 4:past], dim=1, descending=True, stable=True)[1][:, :1000 - 4 - new] + 4
+    assert torch.equal(kept[:, 4:-new].long(), order.sort(1)[0])
+    assert torch.equal(into.v[:, -new:], cache.v[:, past:]) and torch.equal(wi, torch.gather(w, 1, kept.long()))
+    assert bmx.kv4_evict(cache, w, cap, 1000, sink=4, recent=new).equal(kept)
+    assert torch.equal(cache.k[:, :1000], into.k) and torch.equal(cache.v_biases[:, :1000], into.v_biases)
