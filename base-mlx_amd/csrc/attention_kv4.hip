@@ -111,7 +111,7 @@ __device__ __forceinline__ uint32_t pack_bf(float a, float b) {  // one v_cvt_pk
   return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2_t{a, b}, bf16x2_t));
 }
 __device__ __forceinline__ uint32_t dpp_ror8(uint32_t v) {
-  return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0x128, 0xF, 0xF, false));
+  return static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(v), 0x128, 0xF, 0xF, true));
 }
 // A head's array as a buffer that ends after `bytes`: reads past it give
 // zeros without a memory access
