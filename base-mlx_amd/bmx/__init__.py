@@ -365,8 +365,14 @@ class Kv4Cache:
     """bmx_kv4: one layer's keys and values as MLX affine 4-bit rows of 128
     values, group size 64 -- k, v [n_kv_heads, capacity, 16] int32 (packed
     words), *_scales and *_biases [n_kv_heads, capacity, 2] bf16, contiguous,
-    on one GPU.  The object holds the tensors, in attributes of these names,
-    and describes them to the library as they are now."""
+    on one GPU.  The object holds the tensors, in attributes of these names:
+    change what they hold freely, but other tensors need another object."""
+
+    def __setattr__(self, name, value):
+        # the library has the tensors' addresses from the constructor
+        if self.__dict__.get(name, value) is not value:
+            raise BmxError(BMX_E_ARG, f"{name} of a Kv4Cache is fixed: make another")
+        self.__dict__[name] = value
 
     def __init__(self, k, k_scales, k_biases, v, v_scales, v_biases):
         torch = _torch()

@@ -12,7 +12,8 @@
 // where -16 Q_g is the accumulator's start and b_g Q_g one more product over
 // k = (group, piece) with Q_g in three bf16 pieces (24 bits); the scales
 // multiply fp32 results.  So a score is fp32 arithmetic on the stored values:
-// nothing of K is rounded.  For the values, with p' = bf16(p s_g),
+// nothing of K is rounded.  For the values (of many rows: at kv4_tile_kernel),
+// with p' = bf16(p s_g),
 //   sum_j p_j (s n + b)_j = sum_j p'_j (16 + n_j) - 23.5 sum_j p'_j
 //                         + 7.5 sum_j p~_j s_j + sum_j p~_j b_j,  p~ = bf16(p):
 // the roundings of p' then act on n - 7.5, the centred nibble, and so weigh
@@ -53,7 +54,7 @@ struct Kv4AttnParams {
   float2* lse;        // [Hq, M] (max * c2, log2 of the sum), or null
   uint4* qp;          // [Hq, M, 17] the queries as the weights' kernel takes them, with lse
   float* part_o;      // [Hq, M, ns, 128]
-  float* part_ml;     // [Hq, M, ns, 2]
+  float* part_ml;     // [Hq, M, ns, 2]; of kv4_tile_kernel by 32-row tiles, as part_o, its maxima times c2
   int Hq, M, offset;
   float c2;           // |scale| log2(e)
   uint32_t flip;      // sign bits of a bf16 pair where scale < 0

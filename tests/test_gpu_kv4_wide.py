@@ -255,3 +255,13 @@ def test_past_four_gib(gpu):
     assert torch.equal(into.v[:, -new:], cache.v[:, past:]) and torch.equal(wi, torch.gather(w, 1, kept.long()))
     assert bmx.kv4_evict(cache, w, cap, 1000, sink=4, recent=new).equal(kept)
     assert torch.equal(cache.k[:, :1000], into.k) and torch.equal(cache.v_biases[:, :1000], into.v_biases)
+
+
+def test_a_cache_keeps_its_tensors(gpu):
+    """Other tensors in a cache's place would leave the library with the old addresses."""
+    cache = random_cache(1, 2, 8)
+    cache.v_scales *= 2  # the same tensor
+    for name in ("k", "v_biases", "capacity"):
+        with pytest.raises(bmx.BmxError):
+            setattr(cache, name, torch.zeros(1))
+    assert cache.capacity == 8
