@@ -1277,13 +1277,17 @@ __global__ void __launch_bounds__(256) kv4_merge_kernel(const Kv4AttnParams p) {
 // from the L2 instead, the queries were the bound: 140 MB for 32 tokens over
 // 16384 rows, 16 us.  The accumulators' start, -16 Q_g, comes from the matrix
 // cores too: a product of the pieces with -16.  With several row ranges the
-// sums go to p.sums [range][head][L], added up by kv4_add_kernel.
+// sums go to p.sums [range][head][L], added up by the last workgroup of a
+// range of keys (a launch for it took 1 us more for 509 tokens over 1509 rows).
 constexpr int kWeighWaves = 8, kWeighKeys = kWeighWaves * kKeys, kWeighTiles = 4;
+constexpr int kWeighCounter = 128;  // words from one counter to the next: there are at most 128 (see Kv4Plan::wz)
+static_assert(128 * kWeighCounter * 4 <= BMX_KV4_COUNTER_BYTES);
 __global__ void __launch_bounds__(64 * kWeighWaves) kv4_weigh_kernel(const Kv4AttnParams p) {
   constexpr int kRowsStage = kWeighTiles * kRows, kWords = kRowsStage * kQueryWords;
   constexpr int kPer = (kWords + 64 * kWeighWaves - 1) / (64 * kWeighWaves);
   __shared__ u32x4_t qs[2][kWords];
   __shared__ float2 ls[2][kRowsStage];
+  __shared__ bool last;
   const int tid = threadIdx.x, wave = wave_id(), lane = tid & 63, li = lane & 15, g = lane >> 4;
   const int kvh = blockIdx.x, b = blockIdx.y * kWeighWaves + wave;
   const int M = p.M, R = p.Hq / p.c.n_kv_heads * M, L = p.offset + M;
@@ -1397,21 +1401,29 @@ __global__ void __launch_bounds__(64 * kWeighWaves) kv4_weigh_kernel(const Kv4At
     if (li == i) mine = v;
   }
   const int key = b * kKeys + 16 * (li >> 2) + 4 * g + (li & 3);
-  if (li >= 8 || key >= L) return;
-  if (gridDim.z == 1)
-    p.weights[slot + key] += mine;
-  else
-    p.sums[(static_cast<int64_t>(blockIdx.z) * gridDim.x + kvh) * L + key] = mine;
-}
-
-// weights[h][j] += the row ranges' sums, in order
-__global__ void __launch_bounds__(256) kv4_add_kernel(const Kv4AttnParams p, int ranges) {
-  const int L = p.offset + p.M, j = blockIdx.x * 256 + threadIdx.x;
-  if (j >= L) return;
-  const float* s = p.sums + static_cast<int64_t>(blockIdx.y) * L + j;
-  float v = s[0];
-  for (int z = 1; z < ranges; z++) v += s[static_cast<int64_t>(z) * p.c.n_kv_heads * L];
-  p.weights[static_cast<int64_t>(blockIdx.y) * p.c.capacity + j] += v;
+  const bool own = li < 8 && key < L;
+  if (gridDim.z == 1) {
+    if (own) p.weights[slot + key] += mine;
+    return;
+  }
+  // ---- the last workgroup of these keys adds the ranges' sums, in order ----
+  auto sums = [&](int z, int j) { return p.sums + (static_cast<int64_t>(z) * gridDim.x + kvh) * L + j; };
+  if (own) __hip_atomic_store(sums(blockIdx.z, key), mine, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  if (tid == 0) {
+    unsigned* c = p.cnt + (kvh * gridDim.y + blockIdx.y) * kWeighCounter;
+    last = __hip_atomic_fetch_add(c, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == gridDim.z - 1;
+    if (last) __hip_atomic_store(c, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  __syncthreads();
+  const int j = blockIdx.y * kWeighKeys + tid;
+  if (!last || tid >= kWeighKeys || j >= L) return;
+  float v = 0.0f;
+#pragma unroll 8
+  for (int z = 0; z < static_cast<int>(gridDim.z); z++)
+    v += __hip_atomic_load(sums(z, j), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  p.weights[slot + j] += v;
 }
 
 constexpr int64_t kMaxQueryRows = 1 << 28;  // Hq * M of a call
@@ -1430,7 +1442,7 @@ struct Kv4Plan {
   int rc;  // query rows of the kernel: 4, 8, 16, 64, 256
   int nw;  // its waves
   int tiles, ns, bps, cnt_stride;
-  int wz;  // row ranges of the weights' grid
+  int wz;  // row ranges of the weights' grid (1 where that has more than 128 workgroups)
   size_t lse, qp, part_o, part_ml, sums, bytes;  // byte offsets; the counters come first
 };
 
@@ -1605,8 +1617,5 @@ extern "C" int bmx_attention_gqa_kv4(const bmx_bf16* q, const bmx_kv4* cache, bm
   p.sums = reinterpret_cast<float*>(ws + a.sums);
   hipLaunchKernelGGL(kv4_weigh_kernel, dim3(Hkv, (L + kWeighKeys - 1) / kWeighKeys, a.wz), dim3(64 * kWeighWaves), 0, st,
                      p);
-  if (a.wz == 1) return check_launch("attention_kv4 weights");
-  if (int rc = check_launch("attention_kv4 weights")) return rc;
-  hipLaunchKernelGGL(kv4_add_kernel, dim3((L + 255) / 256, Hkv), dim3(256), 0, st, p, a.wz);
   return check_launch("attention_kv4 weights");
 }
