@@ -7,8 +7,8 @@
 // the keys in registers.  Longer ones: up to 64 slices of a head and three
 // launches.  The first leaves every slice's histogram of the first digit (the
 // next adds them up, so nothing has to be cleared and the order is fixed); the
-// second, knowing where that digit ends, each slice's keys of that digit and
-// how many lie above; the third finds the other digits among those few, in
+// second, knowing where that digit ends, each slice's keys of that digit, the
+// ends of their range and how many lie above; the third finds the other digits among those few, in
 // every slice again, and writes the numbers of its own rows.
 // Compaction: rows kept[i] to rows i, kept[i] >= i; into another cache by the
 // workgroup that found the numbers, in place by a launch of its own.
@@ -25,7 +25,6 @@ constexpr int kThreads = 1024, kWaves = kThreads / 64;
 constexpr int kBins = 2048;
 constexpr int kCopies = 2;  // of a histogram in LDS: equal digits of a wave collide less
 constexpr int kOneWorkgroup = 16 * kThreads;  // rows
-constexpr int kPerThread = 8, kSlice = kThreads * kPerThread;  // of longer heads
 constexpr int kMaxSlices = 64;
 constexpr int kShift[3] = {21, 10, 0};
 
@@ -50,10 +49,10 @@ struct SelectParams {
   MoveParams m;
   uint32_t* hist;   // [heads, slices, kBins] of the first digit
   uint32_t* found;  // [heads, 2]: the first digit's place in the key, the count left
-  uint32_t* count;  // [heads, slices, 2]: keys above the first digit, keys of it
+  uint32_t* count;  // [heads, slices, 4]: keys above the first digit, keys of it, the largest of these, of their complements
   uint32_t* cand;   // [heads, slices, slice_rows]: the keys of it
   int length, sink, recent;
-  int slices, slice_rows;  // rows per slice, a multiple of kPerThread
+  int slices, slice_rows;  // rows per slice, a multiple of 8
   int moves;               // rows are copied, too
 };
 
@@ -79,6 +78,19 @@ __device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
   v = dpp_add<0x118, 0xF>(v);
   v = dpp_add<0x142, 0xA>(v);
   return dpp_add<0x143, 0xC>(v);
+}
+// Lane 63: the largest of a wave's v, the same way.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t dpp_max(uint32_t v) {
+  return max(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), CTRL, ROWS, 0xF, false)));
+}
+__device__ __forceinline__ uint32_t wave_largest(uint32_t v) {
+  v = dpp_max<0x111, 0xF>(v);
+  v = dpp_max<0x112, 0xF>(v);
+  v = dpp_max<0x114, 0xF>(v);
+  v = dpp_max<0x118, 0xF>(v);
+  v = dpp_max<0x142, 0xA>(v);
+  return dpp_max<0x143, 0xC>(v);
 }
 // Sum of v over the workgroup's earlier threads; *total over all.  Calls take
 // the buffers `turn` = 0, 1, 0, 1, ..: the barrier of the one between keeps a
@@ -305,18 +317,19 @@ __global__ void __launch_bounds__(kThreads) kv4_select_kernel(const SelectParams
 }
 
 // Long heads, first launch: the histogram of a slice's first digit.
+template <int E>
 __global__ void __launch_bounds__(kThreads) kv4_hist_kernel(const SelectParams p) {
   __shared__ SelectLds s;
   const int h = blockIdx.x, slice = blockIdx.y, start = slice * p.slice_rows, end = min(p.length, start + p.slice_rows);
   const float* w = p.m.w + static_cast<int64_t>(h) * p.m.cap;
   for (int i = threadIdx.x; i < kCopies * kBins; i += kThreads) (&s.hist[0][0][0])[i] = 0;
   __syncthreads();
-  for (int j0 = start; j0 < end; j0 += kSlice) {
-    const int first = j0 + static_cast<int>(threadIdx.x) * kPerThread;
-    Rows<kPerThread> r;
-    load_rows<kPerThread>(p, w, first, r);
+  for (int j0 = start; j0 < end; j0 += kThreads * E) {
+    const int first = j0 + static_cast<int>(threadIdx.x) * E;
+    Rows<E> r;
+    load_rows<E>(p, w, first, r);
     if (first >= end) r.mid = 0;
-    count_digits<kPerThread>(r, 0, 0u, s);
+    count_digits<E>(r, 0, 0u, s);
   }
   __syncthreads();
   uint32_t* out = p.hist + (static_cast<int64_t>(h) * p.slices + slice) * kBins;
@@ -329,14 +342,16 @@ __global__ void __launch_bounds__(kThreads) kv4_hist_kernel(const SelectParams p
 }
 
 // Second launch: where the first digit ends, and a slice's keys of it.
+template <int E>
 __global__ void __launch_bounds__(kThreads) kv4_pick_kernel(const SelectParams p) {
   __shared__ SelectLds s;
   const int h = blockIdx.x, slice = blockIdx.y, start = slice * p.slice_rows, end = min(p.length, start + p.slice_rows);
   const float* w = p.m.w + static_cast<int64_t>(h) * p.m.cap;
   uint32_t left = static_cast<uint32_t>(p.m.budget - p.sink - p.recent), digit;
   if (left == 0) return;  // uniform: nothing to select
-  Rows<kPerThread> r;
-  load_rows<kPerThread>(p, w, start + static_cast<int>(threadIdx.x) * kPerThread, r);
+  if (threadIdx.x == 0) s.sel[1][0] = s.sel[1][1] = 0;
+  Rows<E> r;
+  load_rows<E>(p, w, start + static_cast<int>(threadIdx.x) * E, r);
   const uint32_t* hist = p.hist + static_cast<int64_t>(h) * p.slices * kBins + (kBins - 2 - 2 * static_cast<int>(threadIdx.x));
   uint32_t c0 = 0, c1 = 0;
 #pragma unroll 8
@@ -352,15 +367,16 @@ __global__ void __launch_bounds__(kThreads) kv4_pick_kernel(const SelectParams p
   }
   const int64_t at = static_cast<int64_t>(h) * p.slices + slice;
   uint32_t* cand = p.cand + at * p.slice_rows;
-  uint32_t above = 0, mine = 0;  // keys so far
+  uint32_t above = 0, mine = 0;        // keys so far
+  uint32_t largest = 0, smallest = 0;  // of this thread's, the smallest as its complement
   int turn = 1;
-  for (int j0 = start; j0 < end; j0 += kSlice, turn ^= 1) {
-    const int first = j0 + static_cast<int>(threadIdx.x) * kPerThread;
-    if (j0 > start) load_rows<kPerThread>(p, w, first, r);
+  for (int j0 = start; j0 < end; j0 += kThreads * E, turn ^= 1) {
+    const int first = j0 + static_cast<int>(threadIdx.x) * E;
+    if (j0 > start) load_rows<E>(p, w, first, r);
     if (first >= end) r.mid = 0;
     uint32_t over = 0, eq = 0;
 #pragma unroll
-    for (int i = 0; i < kPerThread; i++) {
+    for (int i = 0; i < E; i++) {
       const uint32_t d = digit_of(r.key[i], 0);
       if ((r.mid >> i & 1u) && d > digit) over++;
       if ((r.mid >> i & 1u) && d == digit) eq |= 1u << i;
@@ -368,24 +384,33 @@ __global__ void __launch_bounds__(kThreads) kv4_pick_kernel(const SelectParams p
     uint32_t total;
     uint32_t pos = mine + (block_scan(over << 16 | static_cast<uint32_t>(__popc(eq)), s, turn, &total) & 0xffffu);
 #pragma unroll
-    for (int i = 0; i < kPerThread; i++)
-      if (eq >> i & 1u) cand[pos++] = r.key[i];
+    for (int i = 0; i < E; i++)
+      if (eq >> i & 1u) {
+        cand[pos++] = r.key[i];
+        largest = max(largest, r.key[i]);
+        smallest = max(smallest, ~r.key[i]);
+      }
     above += total >> 16;
     mine += total & 0xffffu;
   }
-  if (threadIdx.x == 0) {
-    p.count[2 * at] = above;
-    p.count[2 * at + 1] = mine;
+  largest = wave_largest(largest);
+  smallest = wave_largest(smallest);
+  if ((threadIdx.x & 63) == 63) {
+    atomicMax(&s.sel[1][0], largest);
+    atomicMax(&s.sel[1][1], smallest);
   }
+  __syncthreads();
+  if (threadIdx.x == 0) *reinterpret_cast<u32x4_t*>(&p.count[4 * at]) = u32x4_t{above, mine, s.sel[1][0], s.sel[1][1]};
 }
 
 // Third launch: the smallest kept key, and the numbers of a slice's kept rows.
+template <int E>
 __global__ void __launch_bounds__(kThreads) kv4_emit_kernel(const SelectParams p) {
   __shared__ SelectLds s;
   const int h = blockIdx.x, slice = blockIdx.y, start = slice * p.slice_rows, end = min(p.length, start + p.slice_rows);
   const float* w = p.m.w + static_cast<int64_t>(h) * p.m.cap;
-  Rows<kPerThread> r;
-  load_rows<kPerThread>(p, w, start + static_cast<int>(threadIdx.x) * kPerThread, r);
+  Rows<E> r;
+  load_rows<E>(p, w, start + static_cast<int>(threadIdx.x) * E, r);
   const bool none = p.m.budget - p.sink - p.recent == 0;
   uint32_t T = 0, left = 0;
   // rows kept in the slices before: of the ends, above T, and equal to it
@@ -393,84 +418,96 @@ __global__ void __launch_bounds__(kThreads) kv4_emit_kernel(const SelectParams p
   if (!none) {
     T = p.found[2 * h];
     left = p.found[2 * h + 1];
-    const uint32_t* count = p.count + static_cast<int64_t>(h) * p.slices * 2;
+    const u32x4_t* count = reinterpret_cast<const u32x4_t*>(p.count) + static_cast<int64_t>(h) * p.slices;
     const uint32_t* cand = p.cand + static_cast<int64_t>(h) * p.slices * p.slice_rows;
     if (threadIdx.x < 64) {
       const int i = threadIdx.x;
-      const uint32_t n = i < p.slices ? count[2 * i + 1] : 0u, scan = wave_scan(n);
+      const u32x4_t c = i < p.slices ? count[i] : u32x4_t{0u, 0u, 0u, 0u};
+      const uint32_t n = c.y, scan = wave_scan(n);
       s.first[i] = scan - n;
       if (i == 63) s.first[64] = scan;
-      const uint32_t over = wave_scan(i < slice ? count[2 * i] : 0u);
-      if (i == 63) s.sel[0][0] = over;
+      const uint32_t over = wave_scan(i < slice ? c.x : 0u);
+      const uint32_t largest = wave_largest(c.z), smallest = ~wave_largest(c.w);
+      if (i == 63) {
+        s.sel[0][0] = over;
+        s.sel[0][1] = largest;
+        s.sel[1][1] = smallest;
+      }
     }
     clear_hists(s);
     __syncthreads();
     at += s.sel[0][0];
     const uint32_t all = s.first[kMaxSlices];
-    // every candidate of the head, 4 per thread at a time: f(key, slice, or -1
-    // where there is none).  The first 4096 stay in registers.
-    auto fetch = [&](uint32_t g0, uint32_t (&key)[4], int (&from)[4]) {
+    uint32_t equal = s.first[slice];  // keys T in the slices before
+    if (s.sel[0][1] == s.sel[1][1]) {  // all alike (a fresh cache's zeros): nothing left to find
+      T = s.sel[0][1];
+    } else {
+      // every candidate of the head, 4 per thread at a time: f(key, slice, or -1
+      // where there is none).  The first 4096 stay in registers.
+      auto fetch = [&](uint32_t g0, uint32_t (&key)[4], int (&from)[4]) {
 #pragma unroll
-      for (int k = 0; k < 4; k++) {
-        const uint32_t g = g0 + k * kThreads;
-        from[k] = -1;
-        key[k] = 0;
-        if (g < all) {
-          int lo = 0, hi = p.slices - 1;  // the last slice that starts at or before g
-          while (lo < hi) {
-            const int mid = (lo + hi + 1) >> 1;
-            if (s.first[mid] <= g) lo = mid;
-            else hi = mid - 1;
+        for (int k = 0; k < 4; k++) {
+          const uint32_t g = g0 + k * kThreads;
+          from[k] = -1;
+          key[k] = 0;
+          if (g < all) {
+            int lo = 0, hi = p.slices - 1;  // the last slice that starts at or before g
+            while (lo < hi) {
+              const int mid = (lo + hi + 1) >> 1;
+              if (s.first[mid] <= g) lo = mid;
+              else hi = mid - 1;
+            }
+            from[k] = lo;
+            key[k] = cand[static_cast<int64_t>(lo) * p.slice_rows + (g - s.first[lo])];
           }
-          from[k] = lo;
-          key[k] = cand[static_cast<int64_t>(lo) * p.slice_rows + (g - s.first[lo])];
         }
-      }
-    };
-    uint32_t held[4];
-    int held_from[4];
-    fetch(threadIdx.x, held, held_from);
-    auto each = [&](auto f) {
+      };
+      uint32_t held[4];
+      int held_from[4];
+      fetch(threadIdx.x, held, held_from);
+      auto each = [&](auto f) {
 #pragma unroll
-      for (int k = 0; k < 4; k++)
-        if (static_cast<uint32_t>(k) * kThreads < all) f(held[k], held_from[k]);
-      for (uint32_t g0 = 4 * kThreads + threadIdx.x; g0 - threadIdx.x < all; g0 += 4 * kThreads) {
-        uint32_t key[4];
-        int from[4];
-        fetch(g0, key, from);
+        for (int k = 0; k < 4; k++)
+          if (static_cast<uint32_t>(k) * kThreads < all) f(held[k], held_from[k]);
+        for (uint32_t g0 = 4 * kThreads + threadIdx.x; g0 - threadIdx.x < all; g0 += 4 * kThreads) {
+          uint32_t key[4];
+          int from[4];
+          fetch(g0, key, from);
 #pragma unroll
-        for (int k = 0; k < 4; k++) f(key[k], from[k]);
+          for (int k = 0; k < 4; k++) f(key[k], from[k]);
+        }
+      };
+      for (int d = 1; d < 3; d++) {
+        const uint32_t prefix = T;
+        each([&](uint32_t key, int from) {
+          Rows<1> one;
+          one.key[0] = key;
+          one.mid = from >= 0;
+          count_digits<1>(one, d, prefix, s);
+        });
+        __syncthreads();
+        find_own_digit(s, d, &T, &left);
       }
-    };
-    for (int d = 1; d < 3; d++) {
-      const uint32_t prefix = T;
+      uint32_t above = 0, total;
+      equal = 0;
       each([&](uint32_t key, int from) {
-        Rows<1> one;
-        one.key[0] = key;
-        one.mid = from >= 0;
-        count_digits<1>(one, d, prefix, s);
+        above += from >= 0 && from < slice && key > T;
+        equal += from >= 0 && from < slice && key == T;
       });
-      __syncthreads();
-      find_own_digit(s, d, &T, &left);
+      block_scan(above, s, 1, &total);
+      at += total;
+      block_scan(equal, s, 0, &equal);
     }
-    uint32_t above = 0, equal = 0, total;
-    each([&](uint32_t key, int from) {
-      above += from >= 0 && from < slice && key > T;
-      equal += from >= 0 && from < slice && key == T;
-    });
-    block_scan(above, s, 1, &total);
-    at += total;
-    block_scan(equal, s, 0, &total);
-    const uint32_t took = min(total, left);
+    const uint32_t took = min(equal, left);
     at += took;
     left -= took;
   }
   const uint32_t at0 = at;
   int turn = 1;
-  for (int j0 = start; j0 < end; j0 += kSlice, turn ^= 1) {
-    const int first = j0 + static_cast<int>(threadIdx.x) * kPerThread;
-    if (j0 > start) load_rows<kPerThread>(p, w, first, r);
-    emit_rows<kPerThread>(r, first, end, T, none, left, at, p.m.kept + static_cast<int64_t>(h) * p.m.budget, s, turn);
+  for (int j0 = start; j0 < end; j0 += kThreads * E, turn ^= 1) {
+    const int first = j0 + static_cast<int>(threadIdx.x) * E;
+    if (j0 > start) load_rows<E>(p, w, first, r);
+    emit_rows<E>(r, first, end, T, none, left, at, p.m.kept + static_cast<int64_t>(h) * p.m.budget, s, turn);
   }
   if (!p.moves) return;
   __syncthreads();  // (the numbers are written: the workgroup reads its own)
@@ -535,12 +572,23 @@ bool caches_overlap(const bmx_kv4& a, const float* aw, const bmx_kv4& b, const f
   return false;
 }
 
-// Slices of a head and the rows of each (0: one workgroup holds the head)
-int select_slices(int length, int* rows) {
+// Slices of a head (0: one workgroup holds the head), the rows of each and how
+// many a thread takes at a time.  4096 rows a slice while that is no more
+// workgroups than CUs, else 8192 and up (out of place, us, 4096 / 8192: 8
+// heads of 20001 rows to 4000 17.9 / 21.7, of 131001 to 4096 31.5 / 32.9; but
+// 32 heads 63 / 46).
+int select_slices(int heads, int length, int* rows, int* per_thread) {
   if (length <= kOneWorkgroup) return 0;
-  const int n = std::min(kMaxSlices, (length + kSlice - 1) / kSlice);
-  *rows = ((length + n - 1) / n + kPerThread - 1) / kPerThread * kPerThread;
+  auto slices = [&](int e) { return (length + kThreads * e - 1) / (kThreads * e); };
+  *per_thread = slices(4) <= kMaxSlices && static_cast<int64_t>(heads) * slices(4) <= 256 ? 4 : 8;
+  const int n = std::min(kMaxSlices, slices(*per_thread));
+  *rows = ((length + n - 1) / n + 7) / 8 * 8;
   return (length + *rows - 1) / *rows;
+}
+// Words of a head's workspace, as many as any shorter head's
+size_t select_words(int length) {
+  const size_t slices = std::min(kMaxSlices, (length + 4 * kThreads - 1) / (4 * kThreads));
+  return slices * (kBins + 4 + 8) + length + 2;
 }
 
 }  // namespace
@@ -550,9 +598,7 @@ using namespace bmx;
 
 extern "C" size_t bmx_kv4_evict_workspace_bytes(int n_kv_heads, int length) {
   if (n_kv_heads <= 0 || length <= 0 || length > kKv4MaxCapacity) return 0;
-  int rows = 0;
-  const size_t slices = static_cast<size_t>(select_slices(length, &rows));
-  return slices ? static_cast<size_t>(n_kv_heads) * (slices * (kBins + 2 + rows) + 2) * sizeof(uint32_t) : 0;
+  return length > kOneWorkgroup ? n_kv_heads * select_words(length) * sizeof(uint32_t) : 0;
 }
 
 extern "C" int bmx_kv4_evict(const bmx_kv4* cache, const float* weights, const bmx_kv4* into, float* weights_into,
@@ -603,20 +649,28 @@ extern "C" int bmx_kv4_evict(const bmx_kv4* cache, const float* weights, const b
   s.length = length;
   s.sink = sink;
   s.recent = recent;
-  s.slices = select_slices(length, &s.slice_rows);
+  int per_thread = 0;
+  s.slices = select_slices(heads, length, &s.slice_rows, &per_thread);
   s.hist = static_cast<uint32_t*>(workspace);
-  s.cand = s.hist + static_cast<size_t>(heads) * s.slices * kBins;
-  s.count = s.cand + static_cast<size_t>(heads) * s.slices * s.slice_rows;
-  s.found = s.count + static_cast<size_t>(heads) * s.slices * 2;
+  s.count = s.hist + static_cast<size_t>(heads) * s.slices * kBins;
+  s.cand = s.count + static_cast<size_t>(heads) * s.slices * 4;
+  s.found = s.cand + static_cast<size_t>(heads) * s.slices * s.slice_rows;
   s.moves = !in_place;
   if (s.slices == 0) {
     if (length <= 4 * kThreads) hipLaunchKernelGGL(kv4_select_kernel<4>, dim3(heads), dim3(kThreads), 0, st, s);
     else if (length <= 8 * kThreads) hipLaunchKernelGGL(kv4_select_kernel<8>, dim3(heads), dim3(kThreads), 0, st, s);
     else hipLaunchKernelGGL(kv4_select_kernel<16>, dim3(heads), dim3(kThreads), 0, st, s);
   } else {
-    hipLaunchKernelGGL(kv4_hist_kernel, dim3(heads, s.slices), dim3(kThreads), 0, st, s);
-    hipLaunchKernelGGL(kv4_pick_kernel, dim3(heads, s.slices), dim3(kThreads), 0, st, s);
-    hipLaunchKernelGGL(kv4_emit_kernel, dim3(heads, s.slices), dim3(kThreads), 0, st, s);
+    const dim3 grid(heads, s.slices), block(kThreads);
+    if (per_thread == 4) {
+      hipLaunchKernelGGL(kv4_hist_kernel<4>, grid, block, 0, st, s);
+      hipLaunchKernelGGL(kv4_pick_kernel<4>, grid, block, 0, st, s);
+      hipLaunchKernelGGL(kv4_emit_kernel<4>, grid, block, 0, st, s);
+    } else {
+      hipLaunchKernelGGL(kv4_hist_kernel<8>, grid, block, 0, st, s);
+      hipLaunchKernelGGL(kv4_pick_kernel<8>, grid, block, 0, st, s);
+      hipLaunchKernelGGL(kv4_emit_kernel<8>, grid, block, 0, st, s);
+    }
   }
   if (int rc = check_launch("kv4_evict select")) return rc;
   if (!in_place) return BMX_OK;

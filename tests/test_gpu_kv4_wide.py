@@ -7,7 +7,7 @@ import pytest
 import torch
 
 import bmx
-from test_gpu_kv4 import D, U24, U8, queries, random_cache
+from test_gpu_kv4 import D, U24, U8, check_evict, queries, random_cache
 
 pytestmark = pytest.mark.gpu
 
@@ -265,3 +265,20 @@ def test_a_cache_keeps_its_tensors(gpu):
         with pytest.raises(bmx.BmxError):
             setattr(cache, name, torch.zeros(1))
     assert cache.capacity == 8
+
+
+@pytest.mark.parametrize("kind", ["random", "equal", "few", "narrow"])
+@pytest.mark.parametrize("heads,length,budget", [(60, 17000, 500), (2, 33000, 9000)])
+def test_evict_slices(gpu, kind, heads, length, budget):
+    """Both sizes of a long head's slices; weights that agree in all their bits, or in the first eleven."""
+    g = torch.Generator().manual_seed(heads)
+    r = torch.rand(heads, length, generator=g)
+    w = {"random": r ** 5, "equal": torch.full_like(r, 0.5), "few": torch.round(2 * r), "narrow": 0.5 + 0.01 * r}[kind]
+    check_evict(w.cuda(), random_cache(2, heads, length), length, budget, 4, 100, False)
+
+
+def test_evict_workspace_serves_shorter_lengths():
+    q = bmx.load().bmx_kv4_evict_workspace_bytes
+    for heads in (1, 8, 16, 17, 64):
+        sizes = [q(heads, n) for n in range(16385, 600000, 991)]
+        assert sizes == sorted(sizes)
