@@ -3,7 +3,7 @@
 // Selection, per kv head: the n = budget - sink - recent largest weights of
 // rows [sink, length - recent), ties to the lower row, by radix selection over
 // order-preserving integer keys in digits of 11, 11 and 10 bits; then every
-// kept row's number in order.  Heads of up to 16384 rows: one workgroup each,
+// kept row's number in order.  Heads of up to 8192 rows: one workgroup each,
 // the keys in registers.  Longer ones: up to 64 slices of a head and three
 // launches.  The first leaves every slice's histogram of the first digit (the
 // next adds them up, so nothing has to be cleared and the order is fixed); the
@@ -11,7 +11,8 @@
 // ends of their range and how many lie above; the third finds the other digits among those few, in
 // every slice again, and writes the numbers of its own rows.
 // Compaction: rows kept[i] to rows i, kept[i] >= i; into another cache by the
-// workgroup that found the numbers, in place by a launch of its own.
+// workgroup that found the numbers, where it has few, else and in place by a
+// launch of its own.
 #include <math.h>
 
 #include <algorithm>
@@ -24,7 +25,10 @@ namespace {
 constexpr int kThreads = 1024, kWaves = kThreads / 64;
 constexpr int kBins = 2048;
 constexpr int kCopies = 2;  // of a histogram in LDS: equal digits of a wave collide less
-constexpr int kOneWorkgroup = 16 * kThreads;  // rows
+// Rows of a head that one workgroup selects from.  Above, slices are faster (8
+// heads out of place, us: 12000 rows to 2000 16.8 against 19.8 with 16 rows a
+// thread, 16000 to 4000 18.3 / 27.6).
+constexpr int kOneWorkgroup = 8 * kThreads;
 constexpr int kMaxSlices = 64;
 constexpr int kShift[3] = {21, 10, 0};
 
@@ -289,6 +293,13 @@ __device__ __forceinline__ void copy_rows(const MoveParams& m, int64_t h, int r0
   for (int64_t i = m.budget + static_cast<int64_t>(part) * kThreads + threadIdx.x; i < m.cap_into;
        i += static_cast<int64_t>(parts) * kThreads)
     m.w_out[h * m.cap_into + i] = 0.0f;
+}
+
+// The rows of a head by several workgroups (see own_copy).
+constexpr int kCopyRows = 256;
+__global__ void __launch_bounds__(kThreads) kv4_copy_kernel(const MoveParams m) {
+  const int r0 = blockIdx.y * kCopyRows;
+  copy_rows(m, blockIdx.x, r0, min(m.budget, r0 + kCopyRows), blockIdx.y, gridDim.y);
 }
 
 // A head in one workgroup: up to kThreads * E rows, in registers.
@@ -585,6 +596,15 @@ int select_slices(int heads, int length, int* rows, int* per_thread) {
   *rows = ((length + n - 1) / n + 7) / 8 * 8;
   return (length + *rows - 1) / *rows;
 }
+// Whether the kept rows are copied by a launch of its own, not by the
+// workgroups that find them: where one of these has many of them.  Out of
+// place, us, own launch / not: one workgroup a head, 8 heads of 4352 rows to
+// 512 10.7 / 10.4, to 1024 10.8 / 12.1, to 4000 11.4 / 21.3; slices, 16000 to
+// 1000 16.6 / 15.7, to 4000 17.0 / 18.3, to 12000 20.5 / 27.5, 131001 to 4096
+// 22.9 / 21.3.  The first and the last rows are all in one slice.
+bool own_copy(int slices, int budget, int end) {
+  return slices == 0 ? budget > 512 : end > 1024 || budget > 768 * slices;
+}
 // Words of a head's workspace, as many as any shorter head's
 size_t select_words(int length) {
   const size_t slices = std::min(kMaxSlices, (length + 4 * kThreads - 1) / (4 * kThreads));
@@ -655,11 +675,11 @@ extern "C" int bmx_kv4_evict(const bmx_kv4* cache, const float* weights, const b
   s.count = s.hist + static_cast<size_t>(heads) * s.slices * kBins;
   s.cand = s.count + static_cast<size_t>(heads) * s.slices * 4;
   s.found = s.cand + static_cast<size_t>(heads) * s.slices * s.slice_rows;
-  s.moves = !in_place;
+  const bool copies = !in_place && own_copy(s.slices, budget, std::max(sink, recent));
+  s.moves = !in_place && !copies;
   if (s.slices == 0) {
     if (length <= 4 * kThreads) hipLaunchKernelGGL(kv4_select_kernel<4>, dim3(heads), dim3(kThreads), 0, st, s);
-    else if (length <= 8 * kThreads) hipLaunchKernelGGL(kv4_select_kernel<8>, dim3(heads), dim3(kThreads), 0, st, s);
-    else hipLaunchKernelGGL(kv4_select_kernel<16>, dim3(heads), dim3(kThreads), 0, st, s);
+    else hipLaunchKernelGGL(kv4_select_kernel<8>, dim3(heads), dim3(kThreads), 0, st, s);
   } else {
     const dim3 grid(heads, s.slices), block(kThreads);
     if (per_thread == 4) {
@@ -673,6 +693,10 @@ extern "C" int bmx_kv4_evict(const bmx_kv4* cache, const float* weights, const b
     }
   }
   if (int rc = check_launch("kv4_evict select")) return rc;
+  if (copies) {
+    hipLaunchKernelGGL(kv4_copy_kernel, dim3(heads, (budget + kCopyRows - 1) / kCopyRows), dim3(kThreads), 0, st, s.m);
+    return check_launch("kv4_evict copy");
+  }
   if (!in_place) return BMX_OK;
   hipLaunchKernelGGL(kv4_move_kernel, dim3(heads, 13), dim3(kThreads), 0, st, s.m);
   return check_launch("kv4_evict move");

@@ -364,7 +364,7 @@ size_t bmx_attention_kv4_workspace_bytes(int n_heads, int n_kv_heads, int M, int
 int bmx_kv4_evict(const bmx_kv4 *cache, const float *weights, const bmx_kv4 *into, float *weights_into,
                   int32_t *kept, int length, int budget, int sink, int recent, int head_dim, void *workspace,
                   size_t workspace_bytes, void *stream);
-/* Bytes of workspace bmx_kv4_evict needs (0 up to 16384 rows).  Host only. */
+/* Bytes of workspace bmx_kv4_evict needs (0 up to 8192 rows).  Host only. */
 size_t bmx_kv4_evict_workspace_bytes(int n_kv_heads, int length);
 
 /* ------------------------------------------------------------------ */

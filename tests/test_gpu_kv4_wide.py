@@ -280,5 +280,5 @@ def test_evict_slices(gpu, kind, heads, length, budget):
 def test_evict_workspace_serves_shorter_lengths():
     q = bmx.load().bmx_kv4_evict_workspace_bytes
     for heads in (1, 8, 16, 17, 64):
-        sizes = [q(heads, n) for n in range(16385, 600000, 991)]
+        sizes = [q(heads, n) for n in range(8193, 600000, 991)]
         assert sizes == sorted(sizes)

@@ -160,8 +160,8 @@ def test_evict_refusals():
 
 def test_evict_workspace():
     q = bmx.load().bmx_kv4_evict_workspace_bytes
-    assert q(8, 16384) == 0 and q(8, 16385) > 0 and q(0, 20000) == 0 and q(8, 0) == 0 and q(8, 16776961) == 0
-    sizes = [q(8, n) for n in (16385, 40000, 131072, 1 << 20, 16776960)]
+    assert q(8, 8192) == 0 and q(8, 8193) > 0 and q(0, 20000) == 0 and q(8, 0) == 0 and q(8, 16776961) == 0
+    sizes = [q(8, n) for n in (8193, 40000, 131072, 1 << 20, 16776960)]
     assert sizes == sorted(sizes)
     f = entry_points(kv4(capacity=20000))["evict"]
     need = q(2, 20000)
