@@ -597,13 +597,14 @@ int select_slices(int heads, int length, int* rows, int* per_thread) {
   return (length + *rows - 1) / *rows;
 }
 // Whether the kept rows are copied by a launch of its own, not by the
-// workgroups that find them: where one of these has many of them.  Out of
-// place, us, own launch / not: one workgroup a head, 8 heads of 4352 rows to
-// 512 10.7 / 10.4, to 1024 10.8 / 12.1, to 4000 11.4 / 21.3; slices, 16000 to
-// 1000 16.6 / 15.7, to 4000 17.0 / 18.3, to 12000 20.5 / 27.5, 131001 to 4096
-// 22.9 / 21.3.  The first and the last rows are all in one slice.
+// workgroups that find them: where one of these has many of them, so that the
+// card gains the 2 us that another launch costs the host.  Out of place, us,
+// own launch / not: one workgroup a head, 8 heads of 4352 rows to 512 10.7 /
+// 10.4, to 1024 10.8 / 12.1, to 1536 10.8 / 13.6, to 4000 11.4 / 21.3; slices,
+// 16000 to 1000 16.6 / 15.7, to 4000 17.0 / 18.3, to 12000 20.5 / 27.5, 131001
+// to 4096 22.9 / 21.3.  The first and the last rows are all in one slice.
 bool own_copy(int slices, int budget, int end) {
-  return slices == 0 ? budget > 512 : end > 1024 || budget > 768 * slices;
+  return slices == 0 ? budget > 1536 : end > 1024 || budget > 768 * slices;
 }
 // Words of a head's workspace, as many as any shorter head's
 size_t select_words(int length) {
