@@ -1248,7 +1248,9 @@ __global__ void __launch_bounds__(512) kv4_tile_kernel(const Kv4AttnParams p) {
 }
 
 // Joins the splits of kv4_tile_kernel: a wave per 4 dims of each half of a
-// 32-row tile, in the lane order of its partials.
+// 32-row tile, in the lane order of its partials.  Bound by the latency of its
+// loads: with one split after another 32 tokens over 30032 rows (16 splits)
+// took 5 us more.
 __global__ void __launch_bounds__(256) kv4_merge_kernel(const Kv4AttnParams p) {
   const int R = p.Hq / p.c.n_kv_heads * p.M, tiles = (R + kKeys - 1) / kKeys;
   const int wave = wave_id(), lane = threadIdx.x & 63, lr = lane & 31, h = lane >> 5;
@@ -1257,15 +1259,36 @@ __global__ void __launch_bounds__(256) kv4_merge_kernel(const Kv4AttnParams p) {
   const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + tile * p.ns * kKeys + lr;
   const f32x4_t* po = reinterpret_cast<const f32x4_t*>(p.part_o) + tile * p.ns * (kKeys * kKv4Dim / 4) + 64 * k + lane;
   const int kvh = static_cast<int>(tile / tiles), r = static_cast<int>(tile % tiles) * kKeys + lr;
+  // 16 splits at a time, all loads of them under way at once
+  constexpr int N = 16;
   float m = -INFINITY, l = 0.0f;
-  for (int s = 0; s < p.ns; s++) m = fmaxf(m, ml[s * kKeys].x);
   f32x4_t o = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 8
-  for (int s = 0; s < p.ns; s++) {
-    const float2 v = ml[s * kKeys];
-    const float f = v.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(v.x - m);
-    l = __builtin_fmaf(f, v.y, l);
-    o += f * po[static_cast<int64_t>(s) * (kKeys * kKv4Dim / 4)];
+  for (int s0 = 0; s0 < p.ns; s0 += N) {
+    float2 v[N];
+    f32x4_t x[N];
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+      v[i] = make_float2(-INFINITY, 0.0f);
+      x[i] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+      if (s0 + i < p.ns) {
+        v[i] = ml[(s0 + i) * kKeys];
+        x[i] = po[static_cast<int64_t>(s0 + i) * (kKeys * kKv4Dim / 4)];
+      }
+    }
+    reads_go_out();
+    float mn = m;
+#pragma unroll
+    for (int i = 0; i < N; i++) mn = fmaxf(mn, v[i].x);
+    const float a = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
+    l *= a;
+    o *= a;
+    m = mn;
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+      const float f = v[i].x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(v[i].x - m);
+      l = __builtin_fmaf(f, v[i].y, l);
+      o += f * x[i];
+    }
   }
   if (r < R) finish_row(p, kvh, r, 8 * k + 4 * h, make_float4(o[0], o[1], o[2], o[3]), m, l);
 }
@@ -1448,14 +1471,14 @@ struct Kv4Plan {
 
 // The kernel and split count for R > 8 query rows per kv head, by estimated
 // time (us) over rounds of 256 workgroups.  16 rows: 5 a round and 1.32 per
-// step of a wave (32 keys; two waves share a SIMD).  64 and 256 rows: 1.92 per
-// iteration (128 keys), 2.05 + 0.58 per full tile (64 keys).  Splits cost the
+// step of a wave (32 keys; two waves share a SIMD).  64 and 256 rows: 1.93 per
+// iteration (128 keys), 2.05 + 0.4 per full tile (64 keys).  Splits cost the
 // last workgroup's merge, or a second launch that reads all partials from
-// memory: by their number, where that walk is long, or by their size.
-// Measured (32 q heads over 8; 16 / 64 / 256 rows, us): 32 tokens over 30032
-// 51 / 50 / 56; 128 over 4128 27 / 33 / 37, over 16128 86 / 75 / 62; 200 over
-// 200 12 / 12 / 17; 512 over 512 27 / 16 / 23, over 2512 68 / 44 / 48; 1024
-// over 1024 61 / 43 / 38.
+// memory.
+// Measured (32 q heads over 8; 16 / 64 / 256 rows, us): 32 tokens over 16384
+// 30 / 31 / 34, over 30032 50 / 44 / 48; 128 over 4128 26 / 32 / 34, over 16128
+// 84 / 74 / 59; 200 over 200 12 / 12 / 16; 512 over 512 27 / 16 / 23, over 2512
+// 67 / 44 / 48; 1024 over 1024 61 / 42 / 37.
 void choose_kernel(int Hkv, int64_t R, int M, int L, int* rc, int* ns_out) {
   const double seen = L - 0.5 * (M - 1);  // keys of an average query
   double least = 1e30;
@@ -1471,12 +1494,12 @@ void choose_kernel(int Hkv, int64_t R, int M, int L, int* rc, int* ns_out) {
       const double rounds = std::ceil(static_cast<double>(pairs) * ns / kSplitGrid);
       // (the 64-row kernel's time is its last row tile's, the others' an average one's)
       const double n = std::max(1.0, (rows == 64 ? L : seen) / (static_cast<double>(keys) * ns));
+      const double mb = 520e-6 * kKeys * Hkv * ((R + kKeys - 1) / kKeys) * ns;  // of partials
       double t;
       if (rows == 16) t = 1.0 + rounds * (5.0 + 1.32 * n) + (ns > 1 ? 3.0 : 0.0);
-      else if (rows == 64) t = 8.6 + rounds * n * 1.92 + (ns > 1 ? 5.3 + 0.42 * ns : 0.0);
       else
-        t = 13.0 + rounds * n * (2.05 + 0.58 * std::min<double>(R, 256.0) / 256.0) +
-            (ns > 1 ? 0.5 + 0.38e-6 * 520.0 * kKeys * Hkv * ((R + kKeys - 1) / kKeys) * ns : 0.0);
+        t = rows == 64 ? 8.2 + rounds * n * 1.93 + (ns > 1 ? 1.5 + 0.7 * mb : 0.0)
+                       : 13.1 + rounds * n * (2.05 + 0.4 * std::min<double>(R, 256.0) / 256.0) + (ns > 1 ? 0.35 * mb : 0.0);
       if (t < least) {
         least = t;
         *rc = rows;

@@ -64,7 +64,7 @@ def check(q, cache, past, scale=None, weigh=True):
 WIDE = [(32, 8, 512, 0), (32, 8, 511, 2001), (64, 8, 130, 70), (64, 8, 65, 3001), (16, 1, 777, 0), (64, 8, 40, 20000),
         (16, 2, 700, 0), (64, 64, 30, 100), (6, 2, 1000, 0), (5, 5, 700, 33), (24, 3, 200, 1000), (12, 2, 333, 4100),
         (16, 1, 64, 20001), (32, 8, 1024, 0),
-        (32, 8, 140, 16001), (64, 64, 200, 0), (8, 1, 1500, 700), (32, 8, 1, 12000), (64, 8, 1, 5001), (3, 3, 1, 300001), (8, 1, 1, 300001), (64, 8, 16, 9000)]
+        (32, 8, 140, 16001), (64, 8, 32, 16000), (64, 64, 200, 0), (8, 1, 1500, 700), (32, 8, 1, 12000), (64, 8, 1, 5001), (3, 3, 1, 300001), (8, 1, 1, 300001), (64, 8, 16, 9000)]
 
 
 @pytest.mark.parametrize("Hq,Hkv,M,past", WIDE)
