@@ -447,6 +447,12 @@ def _bf16(*ts):
             raise BmxError(BMX_E_ARG, f"bfloat16 tensors expected, got {t.dtype}")
 
 
+def _kv4_rows(cache, M, offset):
+    # (in Python: ctypes would pass the low 32 bits of a larger number)
+    if not 0 <= offset <= cache.capacity - M:
+        raise BmxError(BMX_E_KV_CAPACITY, f"rows {offset} .. {offset + M - 1}, capacity {cache.capacity}")
+
+
 def kv4_write(k, v, cache, offset, stream=None):
     """Quantizes keys and values [n_kv_heads, M, 128] bf16 into cache rows
     offset .. offset+M-1.  k and v may be strided views with contiguous rows:
@@ -468,7 +474,8 @@ def kv4_write(k, v, cache, offset, stream=None):
     if k2 != 1 or v2 != 1:
         raise BmxError(BMX_E_ARG, "the 128 values of a row must be contiguous")
     H, M, D = ks
-    if M == 0 and 0 <= offset <= cache.capacity:
+    _kv4_rows(cache, M, offset)
+    if M == 0:
         return  # (an empty tensor has no address)
     if H == 1:
         k0 = v0 = 0  # (the stride of an axis of one entry says nothing)
@@ -513,13 +520,17 @@ def qk_norm_rope_kv4(q, k, v, q_norm, k_norm, cache, offset, position=None, eps=
                                     f"[M, {cache.n_kv_heads}*128] expected")
     if q_norm.shape != (128,) or k_norm.shape != (128,):
         raise BmxError(BMX_E_SHAPE, "q_norm and k_norm must hold 128 weights")
+    _kv4_rows(cache, M, offset)
+    if position is None:
+        position = offset
+    if not 0 <= position < 1 << 63:
+        raise BmxError(BMX_E_ARG, f"position={position}")
     Hq = q.shape[1] // 128
     out = _empty(stream, cache.device, torch.bfloat16, Hq, M, 128)
-    if M == 0 and 0 <= offset <= cache.capacity:
+    if M == 0:
         return out
     call("bmx_qk_norm_rope_kv4", q.data_ptr(), k.data_ptr(), v.data_ptr(), q_norm.data_ptr(), k_norm.data_ptr(),
-         out.data_ptr(), cache._ref, M, Hq, 128, offset, offset if position is None else position, eps, theta,
-         _stream(stream))
+         out.data_ptr(), cache._ref, M, Hq, 128, offset, position, eps, theta, _stream(stream))
     return out
 
 
@@ -528,7 +539,9 @@ def attention_kv4_workspace(n_heads, n_kv_heads, M, L, weigh=False, device="cuda
     to row L (weigh: with weights), its counters zeroed.  It serves one call
     at a time."""
     torch = _torch()
-    nbytes = load().bmx_attention_kv4_workspace_bytes(n_heads, n_kv_heads, M, L, int(bool(weigh)))
+    nbytes = 0
+    if 0 < min(n_heads, n_kv_heads, M, L) and max(n_heads, n_kv_heads, M, L) < 1 << 31:
+        nbytes = load().bmx_attention_kv4_workspace_bytes(n_heads, n_kv_heads, M, L, int(bool(weigh)))
     if not nbytes:
         raise BmxError(BMX_E_SHAPE, f"{n_heads} heads over {n_kv_heads}, M={M}, L={L}")
     with _on_stream(stream, device):
@@ -564,10 +577,9 @@ def attention_kv4(q, cache, offset, scale=None, weights=None, workspace=None, ou
         _bf16(out)
         if out.numel() != M * Hq * D:
             raise BmxError(BMX_E_SHAPE, f"out must hold [{M}, {Hq * D}], got {tuple(out.shape)}")
+    _kv4_rows(cache, M, offset)
     if M == 0:
         return out
-    if not 0 <= offset <= cache.capacity - M:
-        raise BmxError(BMX_E_KV_CAPACITY, f"rows {offset} .. {offset + M - 1}, capacity {cache.capacity}")
     if workspace is None:
         workspace = attention_kv4_workspace(Hq, cache.n_kv_heads, M, offset + M, weights is not None, cache.device,
                                             stream)
@@ -607,8 +619,11 @@ def kv4_evict(cache, weights, length, budget, sink=4, recent=0, into=None, weigh
     _same_device(cache.k, into.k)
     _kv4_weights(weights, cache)
     _kv4_weights(weights_into, into)
-    if budget < 1:
-        raise BmxError(BMX_E_SHAPE, f"budget={budget}")
+    if length > cache.capacity or budget > into.capacity:
+        raise BmxError(BMX_E_KV_CAPACITY, f"length {length} of capacity {cache.capacity}, budget {budget} of capacity "
+                                          f"{into.capacity}")
+    if not 1 <= budget <= length or sink < 0 or recent < 0 or sink + recent > budget:
+        raise BmxError(BMX_E_SHAPE, f"length={length} budget={budget} sink={sink} recent={recent}")
     if kept is None:
         kept = _empty(stream, cache.device, torch.int32, cache.n_kv_heads, budget)
     else:
