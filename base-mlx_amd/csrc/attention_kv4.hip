@@ -114,6 +114,13 @@ __device__ __forceinline__ uint32_t pack_bf(float a, float b) {  // one v_cvt_pk
 __device__ __forceinline__ uint32_t dpp_ror8(uint32_t v) {
   return static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(v), 0x128, 0xF, 0xF, true));
 }
+// Whether one of a row's two scales (or biases) is infinite or NaN
+__device__ __forceinline__ bool not_finite(uint32_t w) {
+  return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u;
+}
+// Keeps what is done to x in a seldom taken branch there: without, the compiler
+// does it always and selects
+__device__ __forceinline__ void stay_here(float& x) { asm volatile("" : "+v"(x)); }
 // A head's array as a buffer that ends after `bytes`: reads past it give
 // zeros without a memory access
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc(const uint32_t* base, int64_t words, int bytes) {
@@ -482,6 +489,19 @@ __global__ void __launch_bounds__(64 * NW) kv4_rows_kernel(const Kv4AttnParams p
       for (int i = 0; i < 4; i++)
         sc[4 * t + i] = __builtin_fmaf(lo_f(ks[t][i]), d0[i], __builtin_fmaf(hi_f(ks[t][i]), d1[i], db[i]));
     }
+    // An infinite scale that meets a product of the other sign gives -infinity,
+    // as a hidden row's score; it is NaN instead.  (An infinite bias always is:
+    // it also meets the zeros of qp.)
+    float least = sc[0];
+#pragma unroll
+    for (int e = 1; e < 8; e++) least = fminf(least, sc[e]);
+    if (__any(least == -INFINITY)) {
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        stay_here(sc[e]);
+        if (not_finite(ks[e >> 2][e & 3])) sc[e] = NAN;
+      }
+    }
     load_k(b + NW);
     // ---- running softmax: the maximum over all keys of a query ----
     const int key0 = b * kKeys + 4 * g;
@@ -714,6 +734,15 @@ __global__ void __launch_bounds__(64 * NW) kv4_few_kernel(const Kv4AttnParams p)
       sc[i] = __builtin_fmaf(lo_f(kb[i]), qs[0], hi_f(kb[i]) * qs[1]);
       sc[i] = __builtin_fmaf(lo_f(ks[i]), d0[0][i], __builtin_fmaf(hi_f(ks[i]), d1[0][i], sc[i]));
     }
+    // an infinite scale or bias must not make its key's score -infinity, as a
+    // hidden row's
+    if (__any(fminf(fminf(sc[0], sc[1]), fminf(sc[2], sc[3])) == -INFINITY)) {
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        stay_here(sc[i]);
+        if (not_finite(ks[i]) || not_finite(kb[i])) sc[i] = NAN;
+      }
+    }
     load_k(b + NW);
     const int key0 = b * kStep + 16 * blk + 4 * g;
     if constexpr (cut) {
@@ -809,10 +838,6 @@ __device__ __forceinline__ u32x4_t lds_read(const uint16_t* p) { return *reinter
 // Reads before it stay before it, and so ahead of the branches that follow
 __device__ __forceinline__ void reads_go_out() { asm volatile("" ::: "memory"); }
 
-// Keeps what is done to x in a seldom taken branch there: without, the compiler
-// does it always and selects
-__device__ __forceinline__ void stay_here(float& x) { asm volatile("" : "+v"(x)); }
-
 constexpr float kFloatMax = 3.402823466e38f;
 // The largest magnitude that values of scale s and bias b may have (not a
 // finite number where the scale or bias is not)
@@ -852,7 +877,8 @@ __device__ __forceinline__ bool kv4_finite(float s, float b) { return kv4_most(s
 // half the time.  Rates of the counters: matrix cores busy 36 %, VALU 49 %,
 // LDS 44 %, 1 / 9 of that in bank conflicts.
 // A value that is not finite (its scale or bias is not) goes to LDS as 0 and
-// marks the iteration; the rows that see it become NaN by themselves.
+// marks the iteration, as a key's scale or bias that is not finite does; the
+// rows that see it become NaN by themselves.
 template <int RW>
 __global__ void __launch_bounds__(512) kv4_tile_kernel(const Kv4AttnParams p) {
   constexpr int KW = 8 / RW, TPW = RW == 8 ? 2 : 1, KPI = kKeys * KW * TPW;
@@ -871,7 +897,7 @@ __global__ void __launch_bounds__(512) kv4_tile_kernel(const Kv4AttnParams p) {
   };
   constexpr size_t kLds = sizeof(Stage) * 2 > sizeof(Join) ? sizeof(Stage) * 2 : sizeof(Join);
   __shared__ __align__(16) char lds[kLds];
-  // of four iterations in turn: whether some value is not finite, the keys' 2^(15 - e), e
+  // of four iterations in turn: whether some key or value is not finite, the keys' 2^(15 - e), e
   __shared__ int mark[4];
   __shared__ __align__(16) float vscale[4][KPI];
   __shared__ uint32_t ve[4][KPI];
@@ -956,8 +982,9 @@ __global__ void __launch_bounds__(512) kv4_tile_kernel(const Kv4AttnParams p) {
 #pragma unroll
     for (int i = 0; i < W; i++)
       *reinterpret_cast<u32x4_t*>(&s.kt[k_key][8 * (k_word + i)]) = word_pairs(gk[i], nk);
-    if (tid < 2 * KPI) {
+    if (tid < 2 * KPI) {  // (all of a wave or none)
       (&s.sb[0][0])[tid] = gsb;
+      if (__any(not_finite(gsb)) && lane == 0) mark[it & 3] = it + 1;
       if (tid >= KPI) {
         s.sf[0][tid - KPI] = lo_f(gsb) * p.c2;
         s.sf[1][tid - KPI] = hi_f(gsb) * p.c2;
@@ -1148,7 +1175,9 @@ __global__ void __launch_bounds__(512) kv4_tile_kernel(const Kv4AttnParams p) {
       for (int e = 0; e < 16; e++) {
         const int key = key0 + 8 * (e >> 2) + 4 * h + (e & 3);
         const uint32_t sw = load1(vsr, key * 4), bw = load1(vbr, key * 4);
+        const uint32_t sk = load1(ksr, key * 4), bk = load1(kbr, key * 4);
         if (key < lim) {
+          if (not_finite(sk) || not_finite(bk)) l = NAN;
           if (!kv4_finite(lo_f(sw), lo_f(bw))) poison[0] = NAN;
           if (!kv4_finite(hi_f(sw), hi_f(bw))) poison[1] = NAN;
         }
