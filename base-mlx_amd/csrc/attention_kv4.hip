@@ -82,6 +82,12 @@ __device__ __forceinline__ f32x16_t mfma32(u32x4_t a, u32x4_t b, f32x16_t c) {
 // The wave's number as a scalar, so branches on it cost no lane masks
 __device__ __forceinline__ int wave_id() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
 
+// The kernels for up to 16 rows a wave multiply all weights by 2^-28, which
+// the division by their sum takes out again: 2^24 rows of values of 2^120,
+// whose sums of p s (16 + n) are 2^122 each, at a weight of 2^8 (see moves) stay
+// below 2^127.  What a row draws below 2^-98 of the largest weight is 0.
+constexpr float kDown = 28.0f;
+
 // Whether a running maximum m moves to its step's maximum bm: only where the
 // weights exp2((bm - m) c2) would pass 2^8.  Until then m stays, P goes up to
 // 2^8, and the products so far need no rescaling.
@@ -171,13 +177,15 @@ __device__ __forceinline__ void store_query(const Kv4AttnParams& p, int64_t row,
   if (g == 0) dst[16] = q_pieces(qs);
 }
 
-// One output row's 4 dims, and the row's softmax statistics for the weights.
-__device__ __forceinline__ void finish_row(const Kv4AttnParams& p, int kvh, int r, int d, float4 o, float m, float l) {
+// One output row's 4 dims, and the row's softmax statistics for the weights;
+// o and l hold a factor 2^-down.
+__device__ __forceinline__ void finish_row(const Kv4AttnParams& p, int kvh, int r, int d, float4 o, float m, float l,
+                                           float down) {
   const int rep = p.Hq / p.c.n_kv_heads, t = r % p.M, h = kvh * rep + r / p.M;
   const float inv = 1.0f / l;
   *reinterpret_cast<uint2*>(p.out + (static_cast<int64_t>(t) * p.Hq + h) * kKv4Dim + d) =
       make_uint2(pack_bf(o.x * inv, o.y * inv), pack_bf(o.z * inv, o.w * inv));
-  if (p.lse && d == 0) p.lse[static_cast<int64_t>(kvh) * rep * p.M + r] = make_float2(m, log2f(l));
+  if (p.lse && d == 0) p.lse[static_cast<int64_t>(kvh) * rep * p.M + r] = make_float2(m, log2f(l) + down);
 }
 
 template <int NW, int ROWS>
@@ -249,7 +257,7 @@ __device__ __forceinline__ void merge_splits(const Kv4AttnParams& p, JoinLds<NW,
     for (; s < p.ns; s += groups) o += sm.wt[row][s] * load_o(it, s);
     if (groups == 1)
       finish_row(p, kvh, r0 + row, d, make_float4(o[0], o[1], o[2], o[3]), sm.fin[row][0] * p.c2,
-                 sm.fin[row][1]);
+                 sm.fin[row][1], kDown);
     else
       *reinterpret_cast<f32x4_t*>(&red[(n * items + it) * 4]) = o;
   }
@@ -259,7 +267,7 @@ __device__ __forceinline__ void merge_splits(const Kv4AttnParams& p, JoinLds<NW,
     f32x4_t o = *reinterpret_cast<const f32x4_t*>(&red[k * 4]);
     for (int i = 1; i < groups; i++) o += *reinterpret_cast<const f32x4_t*>(&red[(i * items + k) * 4]);
     finish_row(p, kvh, r0 + (k >> 5), 4 * (k & 31), make_float4(o[0], o[1], o[2], o[3]),
-               sm.fin[k >> 5][0] * p.c2, sm.fin[k >> 5][1]);
+               sm.fin[k >> 5][0] * p.c2, sm.fin[k >> 5][1], kDown);
   }
 }
 
@@ -315,7 +323,7 @@ __device__ __forceinline__ void join_and_finish(const Kv4AttnParams& p, JoinLds<
     }
     if (sum != sum) mm = sum;
     if (p.ns == 1) {
-      finish_row(p, kvh, r0 + r, d, o, mm * p.c2, sum);
+      finish_row(p, kvh, r0 + r, d, o, mm * p.c2, sum, kDown);
     } else {
       const int64_t at = (row0 + r) * p.ns + split;
       if (p.local) {
@@ -547,7 +555,7 @@ __global__ void __launch_bounds__(64 * NW) kv4_rows_kernel(const Kv4AttnParams p
         for (int i = 0; i < 4; i++) acc[y][i] *= a;
       }
     }
-    const float mc = m == -INFINITY ? 0.0f : m * p.c2;
+    const float mc = m == -INFINITY ? kDown : __builtin_fmaf(m, p.c2, kDown);
     float pr[8], ps[2][8];
 #pragma unroll
     for (int e = 0; e < 8; e++) {
@@ -766,7 +774,7 @@ __global__ void __launch_bounds__(64 * NW) kv4_few_kernel(const Kv4AttnParams p)
         for (int i = 0; i < 4; i++) acc[y][i] *= a;
       }
     }
-    const float mc = m == -INFINITY ? 0.0f : m * p.c2;
+    const float mc = m == -INFINITY ? kDown : __builtin_fmaf(m, p.c2, kDown);
 #pragma unroll
     for (int i = 0; i < 4; i++) {
       pr[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[i], p.c2, -mc));
@@ -1262,7 +1270,7 @@ __global__ void __launch_bounds__(512) kv4_tile_kernel(const Kv4AttnParams p) {
 #pragma unroll
       for (int j = 0; j < 4; j++)
         finish_row(p, kvh, row, 32 * d + 8 * j + 4 * h,
-                   make_float4(acc[d][4 * j], acc[d][4 * j + 1], acc[d][4 * j + 2], acc[d][4 * j + 3]), m, l);
+                   make_float4(acc[d][4 * j], acc[d][4 * j + 1], acc[d][4 * j + 2], acc[d][4 * j + 3]), m, l, 0.0f);
     return;
   }
   // partials in the lanes' order, so a store writes 1 KB in one piece
@@ -1319,7 +1327,7 @@ __global__ void __launch_bounds__(256) kv4_merge_kernel(const Kv4AttnParams p) {
       o += f * x[i];
     }
   }
-  if (r < R) finish_row(p, kvh, r, 8 * k + 4 * h, make_float4(o[0], o[1], o[2], o[3]), m, l);
+  if (r < R) finish_row(p, kvh, r, 8 * k + 4 * h, make_float4(o[0], o[1], o[2], o[3]), m, l, 0.0f);
 }
 
 // weights[h][j] += sum over the query rows of exp2(S c2 - max c2 - log2 sum).

@@ -333,8 +333,9 @@ int bmx_qk_norm_rope_kv4(const bmx_bf16 *q, const bmx_bf16 *k, const bmx_bf16 *v
  * (BMX_E_ARG).  A row that a query does not see leaves it alone, whatever it
  * holds; one that it sees, with a scale or bias that is not finite, makes
  * that group's 64 outputs (V) or all of them and the kv head's weights (K)
- * not finite.  Values up to 2^120 in magnitude keep their precision, with
- * many queries those from 2^-93 on.
+ * not finite.  Values (V) of 2^-60 to 2^120 in magnitude keep their precision
+ * over any number of rows; smaller ones are off by 2^-70 at most.  A row whose
+ * weight is below 2^-98 of the query's largest may count as one of weight 0.
  * Replaces: mlx_rs::fast::scaled_dot_product_attention as
  *   bmx_attention_gqa does (crates/base-mlx-core/src/model/qwen3.rs:491-518);
  *   the reference has no quantized cache and no eviction. */
