@@ -82,10 +82,10 @@ __device__ __forceinline__ f32x16_t mfma32(u32x4_t a, u32x4_t b, f32x16_t c) {
 // The wave's number as a scalar, so branches on it cost no lane masks
 __device__ __forceinline__ int wave_id() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
 
-// The kernels for up to 16 rows a wave multiply all weights by 2^-28, which
-// the division by their sum takes out again: 2^24 rows of values of 2^120,
-// whose sums of p s (16 + n) are 2^122 each, at a weight of 2^8 (see moves) stay
-// below 2^127.  What a row draws below 2^-98 of the largest weight is 0.
+// All weights hold a factor 2^-28 where they are summed up, which the division
+// by their sum takes out again: 2^24 rows of values of 2^120, whose sums of
+// p s (16 + n) are 2^122 each, at a weight of 2^8 (see moves) stay below 2^127.
+// What a row draws below 2^-98 of the largest weight is 0.
 constexpr float kDown = 28.0f;
 
 // Whether a running maximum m moves to its step's maximum bm: only where the
@@ -178,14 +178,13 @@ __device__ __forceinline__ void store_query(const Kv4AttnParams& p, int64_t row,
 }
 
 // One output row's 4 dims, and the row's softmax statistics for the weights;
-// o and l hold a factor 2^-down.
-__device__ __forceinline__ void finish_row(const Kv4AttnParams& p, int kvh, int r, int d, float4 o, float m, float l,
-                                           float down) {
+// o and l hold the factor 2^-28.
+__device__ __forceinline__ void finish_row(const Kv4AttnParams& p, int kvh, int r, int d, float4 o, float m, float l) {
   const int rep = p.Hq / p.c.n_kv_heads, t = r % p.M, h = kvh * rep + r / p.M;
   const float inv = 1.0f / l;
   *reinterpret_cast<uint2*>(p.out + (static_cast<int64_t>(t) * p.Hq + h) * kKv4Dim + d) =
       make_uint2(pack_bf(o.x * inv, o.y * inv), pack_bf(o.z * inv, o.w * inv));
-  if (p.lse && d == 0) p.lse[static_cast<int64_t>(kvh) * rep * p.M + r] = make_float2(m, log2f(l) + down);
+  if (p.lse && d == 0) p.lse[static_cast<int64_t>(kvh) * rep * p.M + r] = make_float2(m, log2f(l) + kDown);
 }
 
 template <int NW, int ROWS>
@@ -257,7 +256,7 @@ __device__ __forceinline__ void merge_splits(const Kv4AttnParams& p, JoinLds<NW,
     for (; s < p.ns; s += groups) o += sm.wt[row][s] * load_o(it, s);
     if (groups == 1)
       finish_row(p, kvh, r0 + row, d, make_float4(o[0], o[1], o[2], o[3]), sm.fin[row][0] * p.c2,
-                 sm.fin[row][1], kDown);
+                 sm.fin[row][1]);
     else
       *reinterpret_cast<f32x4_t*>(&red[(n * items + it) * 4]) = o;
   }
@@ -267,7 +266,7 @@ __device__ __forceinline__ void merge_splits(const Kv4AttnParams& p, JoinLds<NW,
     f32x4_t o = *reinterpret_cast<const f32x4_t*>(&red[k * 4]);
     for (int i = 1; i < groups; i++) o += *reinterpret_cast<const f32x4_t*>(&red[(i * items + k) * 4]);
     finish_row(p, kvh, r0 + (k >> 5), 4 * (k & 31), make_float4(o[0], o[1], o[2], o[3]),
-               sm.fin[k >> 5][0] * p.c2, sm.fin[k >> 5][1], kDown);
+               sm.fin[k >> 5][0] * p.c2, sm.fin[k >> 5][1]);
   }
 }
 
@@ -323,7 +322,7 @@ __device__ __forceinline__ void join_and_finish(const Kv4AttnParams& p, JoinLds<
     }
     if (sum != sum) mm = sum;
     if (p.ns == 1) {
-      finish_row(p, kvh, r0 + r, d, o, mm * p.c2, sum, kDown);
+      finish_row(p, kvh, r0 + r, d, o, mm * p.c2, sum);
     } else {
       const int64_t at = (row0 + r) * p.ns + split;
       if (p.local) {
@@ -875,7 +874,12 @@ __device__ __forceinline__ bool kv4_finite(float s, float b) { return kv4_most(s
 // further scaling, and what a key's values weigh, not only its score, decides
 // what may round away.  The product that adds the biases adds e and -M too, M
 // in three bf16 pieces; M moves only where P would pass 2^15, to make the
-// largest 2^7.  With 11 bits in P and V the outputs are off by little more
+// largest 2^7.  The sum of the weights is that of P 2^(15 - e), so e of the
+// keys that weigh anything must lie within 2^80 of each other: not below -48,
+// and where a key's is above 32 the rows that see it are computed again, by a
+// pass with a sum, and a maximum, of the scores alone (three exponentials per
+// score; no other row's bits change).  A row leaves with its weights' exponent
+// taken out, so that splits are joined by what they weigh.  With 11 bits in P and V the outputs are off by little more
 // than their own rounding: 0.0017 of the norm for 2048 tokens over 4096 rows,
 // where bf16 for both gave 0.0028.
 // 2048 tokens over 4096 rows, 32 heads of 8: 145 us, 710 TFLOP/s, 56 % of what
@@ -907,6 +911,7 @@ __global__ void __launch_bounds__(512) kv4_tile_kernel(const Kv4AttnParams p) {
   __shared__ __align__(16) char lds[kLds];
   // of four iterations in turn: whether some key or value is not finite, the keys' 2^(15 - e), e
   __shared__ int mark[4];
+  __shared__ int first_wide;  // the first key whose values' exponent is above kMostE
   __shared__ __align__(16) float vscale[4][KPI];
   __shared__ uint32_t ve[4][KPI];
   __shared__ __align__(16) uint16_t vsb[4][2][2][KPI];  // ... scales, biases of group 0, 1, times 2^(15 - e), as fp16
@@ -1019,19 +1024,21 @@ __global__ void __launch_bounds__(512) kv4_tile_kernel(const Kv4AttnParams p) {
     }
   };
 
-  // e of an iteration's keys, a lane each.  Not below -64, so that a sum of
-  // P 2^(15 - e) stays in range: values from 2^-93 on keep their 11 bits.
+  // e of an iteration's keys, a lane each.  Not below -48: values from 2^-77 on
+  // keep their 11 bits.
+  constexpr int kLeastE = -48, kMostE = 32;
   uint32_t bs = 0, bb = 0;
   const int ahead = wave / (KPI / 64), ke = tid - KPI * ahead;  // waves with `ahead` 0, and 1 at the start
   auto fetch_e = [&](int it) {
     bs = load1(vsr, (it * KPI + ke) * 4);
     bb = load1(vbr, (it * KPI + ke) * 4);
   };
-  auto find_e = [&](int it) {
+  auto find_e = [&](int it, auto wide_) {
+    constexpr bool wide = decltype(wide_)::value;
     const float m0 = kv4_most(lo_f(bs), lo_f(bb)), m1 = kv4_most(hi_f(bs), hi_f(bb));
     const bool ok0 = m0 <= kFloatMax, ok1 = m1 <= kFloatMax;
     const float most = fmaxf(ok0 ? m0 : 0.0f, ok1 ? m1 : 0.0f);
-    const int e = max(static_cast<int>(__float_as_uint(most) >> 23) - 126, -64);
+    const int e = max(static_cast<int>(__float_as_uint(most) >> 23) - 126, kLeastE);
     const float r = __uint_as_float(static_cast<uint32_t>(127 + 15 - e) << 23);
     const uint32_t x0 = ok0 ? pack_f16(lo_f(bs) * r, lo_f(bb) * r) : 0u;
     const uint32_t x1 = ok1 ? pack_f16(hi_f(bs) * r, hi_f(bb) * r) : 0u;
@@ -1039,8 +1046,15 @@ __global__ void __launch_bounds__(512) kv4_tile_kernel(const Kv4AttnParams p) {
     vsb[it & 3][1][0][ke] = static_cast<uint16_t>(x0 >> 16);
     vsb[it & 3][0][1][ke] = static_cast<uint16_t>(x1);
     vsb[it & 3][1][1][ke] = static_cast<uint16_t>(x1 >> 16);
-    vscale[it & 3][ke] = r;
-    ve[it & 3][ke] = 0x3f800000u | __float_as_uint(static_cast<float>(e)) >> 16;
+    if constexpr (wide) {
+      vscale[it & 3][ke] = static_cast<float>(e);
+    } else {
+      vscale[it & 3][ke] = r;
+      ve[it & 3][ke] = 0x3f800000u | __float_as_uint(static_cast<float>(e)) >> 16;
+      if (const uint64_t above = __ballot(e > kMostE)) {
+        if (lane == 0) atomicMin(&first_wide, it * KPI + ke + __builtin_ctzll(above));
+      }
+    }
     if (!__all(ok0 && ok1) && lane == 0) mark[it & 3] = it + 1;
   };
 
@@ -1048,6 +1062,7 @@ __global__ void __launch_bounds__(512) kv4_tile_kernel(const Kv4AttnParams p) {
   const int it0 = split * p.bps, it1 = min(iters, it0 + p.bps);
   // everything that the start waits for, at once
   if (tid < 4) mark[tid] = 0;
+  if (tid == 0) first_wide = INT32_MAX;
   if (ahead < 2) fetch_e(it0 + ahead);
   if (it0 < it1) fetch(it0);
   uint4 qd[8];
@@ -1057,7 +1072,7 @@ __global__ void __launch_bounds__(512) kv4_tile_kernel(const Kv4AttnParams p) {
     for (int k = 0; k < 8; k++) qd[k] = *reinterpret_cast<const uint4*>(qr + 16 * k);
   }
   __syncthreads();
-  if (ahead < 2) find_e(it0 + ahead);
+  if (ahead < 2) find_e(it0 + ahead, std::false_type{});
   if (ahead == 0) fetch_e(it0 + 2);
 
   // ---- the query fragments: word 2 k + h of step k, in its pair order ----
@@ -1092,13 +1107,10 @@ __global__ void __launch_bounds__(512) kv4_tile_kernel(const Kv4AttnParams p) {
   }
 
   f32x16_t acc[4];
-#pragma unroll
-  for (int d = 0; d < 4; d++)
-#pragma unroll
-    for (int i = 0; i < 16; i++) acc[d][i] = 0.0f;
   // M is whole, so that the steps from one to the next are exact; `most` is the
-  // largest t - M that leaves it as it is, -infinity before the first M
-  float m = 0.0f, most = -INFINITY, l = 0.0f, poison[2] = {0.0f, 0.0f};
+  // largest t - M that leaves it as it is, -infinity before the first M.  ml:
+  // the wide pass's maximum of the scores, as M above all of them
+  float m, most, ml, l, poison[2];
 
   // K's fragments of the tile to come: read while P V of the one before runs
   u32x4_t kf[8];
@@ -1107,7 +1119,8 @@ __global__ void __launch_bounds__(512) kv4_tile_kernel(const Kv4AttnParams p) {
     for (int k = 0; k < 8; k++) kf[k] = lds_read(&st[buf].kt[kKeys * tile + lr][8 * (2 * k + h)]);
     reads_go_out();
   };
-  auto multiply = [&](int it, int buf, int tile, bool more) {
+  auto multiply = [&](int it, int buf, int tile, bool more, auto wide_) {
+    constexpr bool wide = decltype(wide_)::value;
     const Stage& s = st[buf];
     const int key0 = it * KPI + kKeys * tile, kl = kKeys * tile;
     if (key0 >= kend) return;  // uniform in the wave
@@ -1115,7 +1128,7 @@ __global__ void __launch_bounds__(512) kv4_tile_kernel(const Kv4AttnParams p) {
 #pragma unroll
     for (int i = 0; i < 16; i++) d0[i] = d1[i] = db[i] = 0.0f;
     const uint32_t w = s.sb[h][kl + lr];
-    const uint32_t e1 = ve[it & 3][kl + lr], we = h ? 0x3f803f80u : e1;
+    const uint32_t e1 = wide ? 0u : ve[it & 3][kl + lr], we = h ? 0x3f803f80u : e1;
     const bool marked = __builtin_amdgcn_readfirstlane(mark[it & 3]) == it + 1;
 #pragma unroll
     for (int k = 0; k < 4; k++) {
@@ -1151,33 +1164,73 @@ __global__ void __launch_bounds__(512) kv4_tile_kernel(const Kv4AttnParams p) {
 #pragma unroll
     for (int e = 1; e < 16; e++) bm = fmaxf(bm, sc[e]);
     bm = max_xor32(bm);
-    if (__any(bm > most)) {
-      const float up = bm > most ? ceilf(bm) - 7.0f : 0.0f;
-      const float a = most == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(-up);
-      if (bm > most) most = 15.0f;
-      m += up;
-      const float m0 = round_bf(-m), m1 = round_bf(-m - m0);
-      pieces.w = h ? pack_bf(m1, -m - m0 - m1) : pack_bf(1.0f, m0);
+    if constexpr (wide) {
+      // the scores' own maximum and sum, then per group the products
+      const float top = fmaxf(ml, ceilf(bm));
+      if (__any(top > ml)) {
+        if (ml != -INFINITY) l *= __builtin_amdgcn_exp2f(ml - top);
+        ml = top;
+      }
+      const float base = ml == -INFINITY ? 0.0f : ml;
+      float t[16];
 #pragma unroll
-      for (int e = 0; e < 16; e++) sc[e] -= up;
-      l *= a;
+      for (int j = 0; j < 4; j++) {
+        const f32x4_t e = *reinterpret_cast<const f32x4_t*>(&vscale[it & 3][kl + 8 * j + 4 * h]);
 #pragma unroll
-      for (int d = 0; d < 4; d++) acc[d] *= a;
+        for (int i = 0; i < 4; i++) {
+          l += __builtin_amdgcn_exp2f(sc[4 * j + i] - base);
+          t[4 * j + i] = e[i];
+        }
+      }
+      float bt = sc[0] + t[0];
+#pragma unroll
+      for (int e = 1; e < 16; e++) bt = fmaxf(bt, sc[e] + t[e]);
+      bt = max_xor32(bt);
+      if (__any(bt - m > most)) {
+        const bool up = bt - m > most;
+        const float to = up ? ceilf(bt) - 7.0f : m, a = most == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - to);
+        if (up) most = 15.0f;
+        m = to;
+#pragma unroll
+        for (int d = 0; d < 4; d++) acc[d] *= a;
+      }
+      u32x4_t pb[2];
+#pragma unroll
+      for (int e = 0; e < 16; e++) t[e] = __builtin_amdgcn_exp2f(sc[e] + (t[e] - m));
+#pragma unroll
+      for (int j = 0; j < 8; j++) pb[j >> 2][j & 3] = pack_f16(t[2 * j], t[2 * j + 1]);
+      if (more) read_k(buf, tile + 1);
+#pragma unroll
+      for (int k = 0; k < 8; k++) acc[k & 3] = mfma32_f16(vf[k], pb[k >> 2], acc[k & 3]);
+    } else {
+      if (__any(bm > most)) {
+        const float up = bm > most ? ceilf(bm) - 7.0f : 0.0f;
+        const float a = most == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(-up);
+        if (bm > most) most = 15.0f;
+        m += up;
+        const float m0 = round_bf(-m), m1 = round_bf(-m - m0);
+        pieces.w = h ? pack_bf(m1, -m - m0 - m1) : pack_bf(1.0f, m0);
+#pragma unroll
+        for (int e = 0; e < 16; e++) sc[e] -= up;
+        l *= a;
+#pragma unroll
+        for (int d = 0; d < 4; d++) acc[d] *= a;
+      }
+#pragma unroll
+      for (int e = 0; e < 16; e++) sc[e] = __builtin_amdgcn_exp2f(sc[e]);
+      u32x4_t pb[2];
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        const f32x4_t r = *reinterpret_cast<const f32x4_t*>(&vscale[it & 3][kl + 8 * j + 4 * h]);
+#pragma unroll
+        for (int i = 0; i < 4; i++) l = __builtin_fmaf(sc[4 * j + i], r[i], l);
+        pb[j >> 1][2 * (j & 1)] = pack_f16(sc[4 * j], sc[4 * j + 1]);
+        pb[j >> 1][2 * (j & 1) + 1] = pack_f16(sc[4 * j + 2], sc[4 * j + 3]);
+      }
+      if (more) read_k(buf, tile + 1);
+#pragma unroll
+      for (int k = 0; k < 8; k++) acc[k & 3] = mfma32_f16(vf[k], pb[k >> 2], acc[k & 3]);
     }
-#pragma unroll
-    for (int e = 0; e < 16; e++) sc[e] = __builtin_amdgcn_exp2f(sc[e]);
-    u32x4_t pb[2];
-#pragma unroll
-    for (int j = 0; j < 4; j++) {
-      const f32x4_t r = *reinterpret_cast<const f32x4_t*>(&vscale[it & 3][kl + 8 * j + 4 * h]);
-#pragma unroll
-      for (int i = 0; i < 4; i++) l = __builtin_fmaf(sc[4 * j + i], r[i], l);
-      pb[j >> 1][2 * (j & 1)] = pack_f16(sc[4 * j], sc[4 * j + 1]);
-      pb[j >> 1][2 * (j & 1) + 1] = pack_f16(sc[4 * j + 2], sc[4 * j + 3]);
-    }
-    if (more) read_k(buf, tile + 1);
-#pragma unroll
-    for (int k = 0; k < 8; k++) acc[k & 3] = mfma32_f16(vf[k], pb[k >> 2], acc[k & 3]);
     if (marked) {
 #pragma unroll 1
       for (int e = 0; e < 16; e++) {
@@ -1193,95 +1246,126 @@ __global__ void __launch_bounds__(512) kv4_tile_kernel(const Kv4AttnParams p) {
     }
   };
 
-  __syncthreads();  // (the marks are cleared, the first bounds found)
-  if (it0 < it1) stage(it0, 0);
-  if (it0 + 1 < it1) fetch(it0 + 1);
-  __syncthreads();
-  for (int it = it0; it < it1; it++) {
-    const int buf = (it - it0) & 1;
-    // the two waves of a SIMD (w and w + 4) unpack at different ends of the
-    // iteration: between barriers one's VALU work falls on the other's products
-    read_k(buf, kwi * TPW);
-    if (wave >= 4) {
-      if (it + 1 < it1) stage(it + 1, buf ^ 1);
-      if (it + 2 < it1) fetch(it + 2);
-    } else if (ahead == 0) {
-      find_e(it + 2);
-      fetch_e(it + 3);
-    }
+  // One run over the split's keys, and its rows' results; the wide one's only
+  // for the rows that see key `from`
+  auto pass = [&](int from, auto wide_) {
+    constexpr bool wide = decltype(wide_)::value;
 #pragma unroll
-    for (int t = 0; t < TPW; t++) multiply(it, buf, kwi * TPW + t, t + 1 < TPW);
-    if (wave < 4) {
-      if (it + 1 < it1) stage(it + 1, buf ^ 1);
-      if (it + 2 < it1) fetch(it + 2);
-    }
+    for (int d = 0; d < 4; d++)
+#pragma unroll
+      for (int i = 0; i < 16; i++) acc[d][i] = 0.0f;
+    m = l = poison[0] = poison[1] = 0.0f;
+    most = ml = -INFINITY;
+    __syncthreads();  // (the marks are cleared, the first bounds found)
+    if (it0 < it1) stage(it0, 0);
+    if (it0 + 1 < it1) fetch(it0 + 1);
     __syncthreads();
-  }
+    for (int it = it0; it < it1; it++) {
+      const int buf = (it - it0) & 1;
+      // the two waves of a SIMD (w and w + 4) unpack at different ends of the
+      // iteration: between barriers one's VALU work falls on the other's products
+      read_k(buf, kwi * TPW);
+      if (wave >= 4) {
+        if (it + 1 < it1) stage(it + 1, buf ^ 1);
+        if (it + 2 < it1) fetch(it + 2);
+      } else if (ahead == 0) {
+        find_e(it + 2, wide_);
+        fetch_e(it + 3);
+      }
+#pragma unroll
+      for (int t = 0; t < TPW; t++) multiply(it, buf, kwi * TPW + t, t + 1 < TPW, wide_);
+      if (wave < 4) {
+        if (it + 1 < it1) stage(it + 1, buf ^ 1);
+        if (it + 2 < it1) fetch(it + 2);
+      }
+      __syncthreads();
+    }
 
-  l = add_xor32(l);
-  m = l != l ? l : most == -INFINITY ? most : m - 15.0f;  // V had a factor 2^15; a NaN score: the row stays NaN
+    // ---- relative to the weights' sum: l in [1, 2) 2^-28, exactly ----
+    l = add_xor32(l);
+    // V had a factor 2^15; acc is relative to 2^(m - 15), and so is l, but for the wide pass
+    const float ref = wide ? ml : m - 15.0f;
+    const int k = static_cast<int>(__float_as_uint(l) >> 23 & 255u) - 127;
+    const int down = -k - static_cast<int>(kDown);
+    const int shift = wide ? down + static_cast<int>(fmaxf(-1000.0f, fminf(1000.0f, m - 15.0f - ml))) : down;
+    m = l != l ? l : l > 0.0f ? ref + static_cast<float>(k) : -INFINITY;  // a NaN score: the row stays NaN
+    l = __builtin_amdgcn_ldexpf(l, down);
 #pragma unroll
-  for (int d = 0; d < 4; d++) {
-    const float bad = add_xor32(poison[d >> 1]);
+    for (int d = 0; d < 4; d++) {
+      const float bad = add_xor32(poison[d >> 1]);
 #pragma unroll
-    for (int i = 0; i < 16; i++) acc[d][i] += bad;
-  }
-  // ---- waves of the same rows, two by two ----
+      for (int i = 0; i < 16; i++) acc[d][i] = __builtin_amdgcn_ldexpf(acc[d][i], shift) + bad;
+    }
+    // ---- waves of the same rows, two by two ----
 #pragma unroll
-  for (int half = KW / 2; half > 0; half >>= 1) {
-    const int sl = (kwi & (half - 1)) * RW + rwi;
-    if (kwi >= half && kwi < 2 * half) {
+    for (int half = KW / 2; half > 0; half >>= 1) {
+      const int sl = (kwi & (half - 1)) * RW + rwi;
+      if (kwi >= half && kwi < 2 * half) {
+#pragma unroll
+        for (int d = 0; d < 4; d++)
+#pragma unroll
+          for (int j = 0; j < 4; j++)
+            *reinterpret_cast<float4*>(&jn.os[sl][lr][32 * d + 8 * j + 4 * h]) =
+                make_float4(acc[d][4 * j], acc[d][4 * j + 1], acc[d][4 * j + 2], acc[d][4 * j + 3]);
+        if (h == 0) {
+          jn.ms[sl][lr] = m;
+          jn.ls[sl][lr] = l;
+        }
+      }
+      __syncthreads();
+      if (kwi < half) {
+        const float mo = jn.ms[sl][lr], lo = jn.ls[sl][lr], mm = fmaxf(m, mo);
+        const float a = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mm);
+        const float b = mo == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mo - mm);
+        l = __builtin_fmaf(l, a, lo * b);
+        m = l != l ? l : mm;
+#pragma unroll
+        for (int d = 0; d < 4; d++)
+#pragma unroll
+          for (int j = 0; j < 4; j++) {
+            const float4 v = *reinterpret_cast<const float4*>(&jn.os[sl][lr][32 * d + 8 * j + 4 * h]);
+            acc[d][4 * j] = __builtin_fmaf(acc[d][4 * j], a, v.x * b);
+            acc[d][4 * j + 1] = __builtin_fmaf(acc[d][4 * j + 1], a, v.y * b);
+            acc[d][4 * j + 2] = __builtin_fmaf(acc[d][4 * j + 2], a, v.z * b);
+            acc[d][4 * j + 3] = __builtin_fmaf(acc[d][4 * j + 3], a, v.w * b);
+          }
+      }
+      __syncthreads();
+    }
+    if (kwi > 0 || n <= 0 || (wide && lim <= from)) return;
+    if (p.ns == 1) {
+      if (lr >= n) return;
 #pragma unroll
       for (int d = 0; d < 4; d++)
 #pragma unroll
         for (int j = 0; j < 4; j++)
-          *reinterpret_cast<float4*>(&jn.os[sl][lr][32 * d + 8 * j + 4 * h]) =
-              make_float4(acc[d][4 * j], acc[d][4 * j + 1], acc[d][4 * j + 2], acc[d][4 * j + 3]);
-      if (h == 0) {
-        jn.ms[sl][lr] = m;
-        jn.ls[sl][lr] = l;
-      }
+          finish_row(p, kvh, row, 32 * d + 8 * j + 4 * h,
+                     make_float4(acc[d][4 * j], acc[d][4 * j + 1], acc[d][4 * j + 2], acc[d][4 * j + 3]), m, l);
+      return;
     }
-    __syncthreads();
-    if (kwi < half) {
-      const float mo = jn.ms[sl][lr], lo = jn.ls[sl][lr], mm = fmaxf(m, mo);
-      const float a = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mm);
-      const float b = mo == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mo - mm);
-      l = __builtin_fmaf(l, a, lo * b);
-      m = l != l ? l : mm;
-#pragma unroll
-      for (int d = 0; d < 4; d++)
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-          const float4 v = *reinterpret_cast<const float4*>(&jn.os[sl][lr][32 * d + 8 * j + 4 * h]);
-          acc[d][4 * j] = __builtin_fmaf(acc[d][4 * j], a, v.x * b);
-          acc[d][4 * j + 1] = __builtin_fmaf(acc[d][4 * j + 1], a, v.y * b);
-          acc[d][4 * j + 2] = __builtin_fmaf(acc[d][4 * j + 2], a, v.z * b);
-          acc[d][4 * j + 3] = __builtin_fmaf(acc[d][4 * j + 3], a, v.w * b);
-        }
-    }
-    __syncthreads();
-  }
-  if (kwi > 0 || n <= 0) return;
-  if (p.ns == 1) {
-    if (lr >= n) return;
+    // partials in the lanes' order, so a store writes 1 KB in one piece
+    const int64_t unit = (static_cast<int64_t>(kvh) * ((R + kKeys - 1) / kKeys) + tile_of(rwi)) * p.ns + split;
+    f32x4_t* po = reinterpret_cast<f32x4_t*>(p.part_o) + unit * (kKeys * kKv4Dim / 4) + lane;
 #pragma unroll
     for (int d = 0; d < 4; d++)
 #pragma unroll
       for (int j = 0; j < 4; j++)
-        finish_row(p, kvh, row, 32 * d + 8 * j + 4 * h,
-                   make_float4(acc[d][4 * j], acc[d][4 * j + 1], acc[d][4 * j + 2], acc[d][4 * j + 3]), m, l, 0.0f);
-    return;
-  }
-  // partials in the lanes' order, so a store writes 1 KB in one piece
-  const int64_t unit = (static_cast<int64_t>(kvh) * ((R + kKeys - 1) / kKeys) + tile_of(rwi)) * p.ns + split;
-  f32x4_t* po = reinterpret_cast<f32x4_t*>(p.part_o) + unit * (kKeys * kKv4Dim / 4) + lane;
-#pragma unroll
-  for (int d = 0; d < 4; d++)
-#pragma unroll
-    for (int j = 0; j < 4; j++)
-      po[64 * (4 * d + j)] = f32x4_t{acc[d][4 * j], acc[d][4 * j + 1], acc[d][4 * j + 2], acc[d][4 * j + 3]};
-  if (h == 0) *reinterpret_cast<float2*>(p.part_ml + (unit * kKeys + lr) * 2) = make_float2(m, l);
+        po[64 * (4 * d + j)] = f32x4_t{acc[d][4 * j], acc[d][4 * j + 1], acc[d][4 * j + 2], acc[d][4 * j + 3]};
+    if (h == 0) *reinterpret_cast<float2*>(p.part_ml + (unit * kKeys + lr) * 2) = make_float2(m, l);
+  };
+  pass(0, std::false_type{});
+
+  // ---- rows that see values beyond the plain pass, again ----
+  const int from = first_wide;  // (the last barrier is past: all keys have been looked at)
+  if (from >= min(kend_wg, it1 * KPI)) return;  // uniform
+  if (tid < 4) mark[tid] = 0;
+  if (ahead < 2) fetch_e(it0 + ahead);
+  if (it0 < it1) fetch(it0);
+  __syncthreads();
+  if (ahead < 2) find_e(it0 + ahead, std::true_type{});
+  if (ahead == 0) fetch_e(it0 + 2);
+  pieces.w = 0u;
+  pass(from, std::true_type{});
 }
 
 // Joins the splits of kv4_tile_kernel: a wave per 4 dims of each half of a
@@ -1327,7 +1411,7 @@ __global__ void __launch_bounds__(256) kv4_merge_kernel(const Kv4AttnParams p) {
       o += f * x[i];
     }
   }
-  if (r < R) finish_row(p, kvh, r, 8 * k + 4 * h, make_float4(o[0], o[1], o[2], o[3]), m, l, 0.0f);
+  if (r < R) finish_row(p, kvh, r, 8 * k + 4 * h, make_float4(o[0], o[1], o[2], o[3]), m, l);
 }
 
 // weights[h][j] += sum over the query rows of exp2(S c2 - max c2 - log2 sum).

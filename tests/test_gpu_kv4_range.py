@@ -60,3 +60,45 @@ def test_largest_values_over_many_rows(gpu, Hq, Hkv, M, past, kind):
     cache.k_biases.copy_((60 * math.log(2) * torch.arange(past + M) / (past + M))[:, None].expand(Hkv, -1, 2))
     q = torch.full((Hq, M, D), 1 / D, dtype=torch.bfloat16, device="cuda")  # scores: the keys' biases
     check(bmx.attention_kv4, q, cache, past, scale=1.0)
+
+
+def scaled_cache(Hkv, rows, f):
+    """Random rows whose values are multiplied by f, [rows, 2] per group."""
+    cache = random_cache(2, Hkv, rows, rows)
+    cache.v_scales.mul_(f.cuda())
+    cache.v_biases.mul_(f.cuda())
+    return cache
+
+
+# ... and keys split over the grid next to few rows, short contexts
+SPANS = KERNELS + [(32, 8, 512, 2000), (16, 1, 64, 20001), (64, 64, 200, 0), (32, 8, 70, 0)]
+
+
+@pytest.mark.parametrize("Hq,Hkv,M,past", SPANS)
+@pytest.mark.parametrize("kind", ["ends", "zeros", "late", "early", "steps", "once", "edge"])
+def test_values_of_one_context_far_apart(gpu, Hq, Hkv, M, past, kind):
+    """Rows of 2^-60 next to rows of 2^100, zero rows next to 2^71, one after
+    the other, and at the end of what the tile kernel does in one pass: what a
+    row weighs does not depend on its values."""
+    n = past + M
+    g = torch.Generator().manual_seed(M)
+    half = torch.rand(n, 1, generator=g) < 0.5
+    at = torch.arange(n)[:, None]
+    f = {"ends": torch.where(half, 2.0 ** -60, 2.0 ** 100), "zeros": torch.where(half, 0.0, 2.0 ** 71),
+         "late": torch.where(at < n // 2, 2.0 ** -60, 2.0 ** 100), "early": torch.where(at < n // 2, 2.0 ** 100, 2.0 ** -60),
+         "steps": 2.0 ** (-60 + 160 * at / n).floor(), "once": torch.where(at == n - M // 2 - 1, 2.0 ** 100, 1.0),
+         "edge": torch.where(half, 0.0, 2.0 ** (30 + 2 * torch.rand(n, 1, generator=g)).round())}[kind]
+    check(bmx.attention_kv4, queries(M, Hq, M), scaled_cache(Hkv, n, f.expand(n, 2)), past)
+
+
+@pytest.mark.parametrize("Hq,Hkv,M,past", [k for k in SPANS if k[2] > 30])
+def test_rows_before_a_large_value_keep_their_bits(gpu, Hq, Hkv, M, past):
+    """One row of 2^100 in the middle of the new tokens: the queries before it
+    are computed as without it, the others to their bounds."""
+    n, at = past + M, past + M // 2
+    f = torch.ones(n, 2)
+    q = queries(M, Hq, M)
+    clean = bmx.attention_kv4(q, scaled_cache(Hkv, n, f), past)
+    f[at] = 2.0 ** 100
+    got = check(bmx.attention_kv4, q, scaled_cache(Hkv, n, f), past)
+    assert torch.equal(got[:M // 2], clean[:M // 2])
