@@ -877,8 +877,11 @@ __device__ __forceinline__ bool kv4_finite(float s, float b) { return kv4_most(s
 // largest 2^7.  The sum of the weights is that of P 2^(15 - e), so e of the
 // keys that weigh anything must lie within 2^80 of each other: not below -48,
 // and where a key's is above 32 the rows that see it are computed again, by a
-// pass with a sum, and a maximum, of the scores alone (three exponentials per
-// score; no other row's bits change).  A row leaves with its weights' exponent
+// wide pass with a sum, and a maximum, of the scores alone, and P and V of each
+// group by the group's own e.  So are rows that see a key whose groups are more
+// than 2^6 apart: in the smaller one P 2^-25 of the largest, which is 2^7 at
+// least and belongs to the other, would vanish, a part of N 2^-26 at most with
+// N keys.  (Three exponentials per score; no other row's bits change.)  A row leaves with its weights' exponent
 // taken out, so that splits are joined by what they weigh.  With 11 bits in P and V the outputs are off by little more
 // than their own rounding: 0.0017 of the norm for 2048 tokens over 4096 rows,
 // where bf16 for both gave 0.0028.
@@ -909,9 +912,10 @@ __global__ void __launch_bounds__(512) kv4_tile_kernel(const Kv4AttnParams p) {
   };
   constexpr size_t kLds = sizeof(Stage) * 2 > sizeof(Join) ? sizeof(Stage) * 2 : sizeof(Join);
   __shared__ __align__(16) char lds[kLds];
-  // of four iterations in turn: whether some key or value is not finite, the keys' 2^(15 - e), e
+  // of four iterations in turn: whether some key or value is not finite, the
+  // keys' 2^(15 - e), e (wide pass: e of group 0, of group 1)
   __shared__ int mark[4];
-  __shared__ int first_wide;  // the first key whose values' exponent is above kMostE
+  __shared__ int first_wide;  // the first key whose values the plain pass does not serve
   __shared__ __align__(16) float vscale[4][KPI];
   __shared__ uint32_t ve[4][KPI];
   __shared__ __align__(16) uint16_t vsb[4][2][2][KPI];  // ... scales, biases of group 0, 1, times 2^(15 - e), as fp16
@@ -1026,7 +1030,8 @@ __global__ void __launch_bounds__(512) kv4_tile_kernel(const Kv4AttnParams p) {
 
   // e of an iteration's keys, a lane each.  Not below -48: values from 2^-77 on
   // keep their 11 bits.
-  constexpr int kLeastE = -48, kMostE = 32;
+  constexpr int kLeastE = -48, kMostE = 32, kApart = 6;
+  auto exponent = [&](float most) { return max(static_cast<int>(__float_as_uint(most) >> 23) - 126, kLeastE); };
   uint32_t bs = 0, bb = 0;
   const int ahead = wave / (KPI / 64), ke = tid - KPI * ahead;  // waves with `ahead` 0, and 1 at the start
   auto fetch_e = [&](int it) {
@@ -1037,22 +1042,26 @@ __global__ void __launch_bounds__(512) kv4_tile_kernel(const Kv4AttnParams p) {
     constexpr bool wide = decltype(wide_)::value;
     const float m0 = kv4_most(lo_f(bs), lo_f(bb)), m1 = kv4_most(hi_f(bs), hi_f(bb));
     const bool ok0 = m0 <= kFloatMax, ok1 = m1 <= kFloatMax;
-    const float most = fmaxf(ok0 ? m0 : 0.0f, ok1 ? m1 : 0.0f);
-    const int e = max(static_cast<int>(__float_as_uint(most) >> 23) - 126, kLeastE);
-    const float r = __uint_as_float(static_cast<uint32_t>(127 + 15 - e) << 23);
-    const uint32_t x0 = ok0 ? pack_f16(lo_f(bs) * r, lo_f(bb) * r) : 0u;
-    const uint32_t x1 = ok1 ? pack_f16(hi_f(bs) * r, hi_f(bb) * r) : 0u;
+    const int a0 = exponent(m0), a1 = exponent(m1);  // (of a group that is not finite: as the other)
+    int e0 = ok0 || !ok1 ? a0 : a1, e1 = ok1 ? a1 : e0;
+    const bool apart = max(e0, e1) - min(e0, e1) > kApart;
+    if constexpr (!wide) e0 = e1 = max(e0, e1);
+    const float r0 = __uint_as_float(static_cast<uint32_t>(127 + 15 - e0) << 23);
+    const float r1 = __uint_as_float(static_cast<uint32_t>(127 + 15 - e1) << 23);
+    const uint32_t x0 = ok0 ? pack_f16(lo_f(bs) * r0, lo_f(bb) * r0) : 0u;
+    const uint32_t x1 = ok1 ? pack_f16(hi_f(bs) * r1, hi_f(bb) * r1) : 0u;
     vsb[it & 3][0][0][ke] = static_cast<uint16_t>(x0);
     vsb[it & 3][1][0][ke] = static_cast<uint16_t>(x0 >> 16);
     vsb[it & 3][0][1][ke] = static_cast<uint16_t>(x1);
     vsb[it & 3][1][1][ke] = static_cast<uint16_t>(x1 >> 16);
     if constexpr (wide) {
-      vscale[it & 3][ke] = static_cast<float>(e);
+      vscale[it & 3][ke] = static_cast<float>(e0);
+      ve[it & 3][ke] = __float_as_uint(static_cast<float>(e1));
     } else {
-      vscale[it & 3][ke] = r;
-      ve[it & 3][ke] = 0x3f800000u | __float_as_uint(static_cast<float>(e)) >> 16;
-      if (const uint64_t above = __ballot(e > kMostE)) {
-        if (lane == 0) atomicMin(&first_wide, it * KPI + ke + __builtin_ctzll(above));
+      vscale[it & 3][ke] = r0;
+      ve[it & 3][ke] = 0x3f800000u | __float_as_uint(static_cast<float>(e0)) >> 16;
+      if (const uint64_t beyond = __ballot(apart || e0 > kMostE)) {
+        if (lane == 0) atomicMin(&first_wide, it * KPI + ke + __builtin_ctzll(beyond));
       }
     }
     if (!__all(ok0 && ok1) && lane == 0) mark[it & 3] = it + 1;
@@ -1108,9 +1117,9 @@ __global__ void __launch_bounds__(512) kv4_tile_kernel(const Kv4AttnParams p) {
 
   f32x16_t acc[4];
   // M is whole, so that the steps from one to the next are exact; `most` is the
-  // largest t - M that leaves it as it is, -infinity before the first M.  ml:
-  // the wide pass's maximum of the scores, as M above all of them
-  float m, most, ml, l, poison[2];
+  // largest t - M that leaves it as it is, -infinity before the first M.  Of
+  // the wide pass: one for each group, and ml, at or above all scores
+  float m, most, mg[2], most_g[2], ml, l, poison[2];
 
   // K's fragments of the tile to come: read while P V of the one before runs
   u32x4_t kf[8];
@@ -1172,36 +1181,43 @@ __global__ void __launch_bounds__(512) kv4_tile_kernel(const Kv4AttnParams p) {
         ml = top;
       }
       const float base = ml == -INFINITY ? 0.0f : ml;
-      float t[16];
 #pragma unroll
-      for (int j = 0; j < 4; j++) {
-        const f32x4_t e = *reinterpret_cast<const f32x4_t*>(&vscale[it & 3][kl + 8 * j + 4 * h]);
+      for (int e = 0; e < 16; e++) l += __builtin_amdgcn_exp2f(sc[e] - base);
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-          l += __builtin_amdgcn_exp2f(sc[4 * j + i] - base);
-          t[4 * j + i] = e[i];
+      for (int y = 0; y < 2; y++) {
+        const float* ey = y ? reinterpret_cast<const float*>(ve[it & 3]) : vscale[it & 3];
+        float t[16];
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          const f32x4_t e = *reinterpret_cast<const f32x4_t*>(&ey[kl + 8 * j + 4 * h]);
+#pragma unroll
+          for (int i = 0; i < 4; i++) t[4 * j + i] = e[i];
+        }
+        float bt = sc[0] + t[0];
+#pragma unroll
+        for (int e = 1; e < 16; e++) bt = fmaxf(bt, sc[e] + t[e]);
+        bt = max_xor32(bt);
+        if (__any(bt - mg[y] > most_g[y])) {
+          const bool up = bt - mg[y] > most_g[y];
+          const float to = up ? ceilf(bt) - 7.0f : mg[y];
+          const float a = most_g[y] == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(mg[y] - to);
+          if (up) most_g[y] = 15.0f;
+          mg[y] = to;
+          acc[2 * y] *= a;
+          acc[2 * y + 1] *= a;
+        }
+        u32x4_t pb[2];
+#pragma unroll
+        for (int e = 0; e < 16; e++) t[e] = __builtin_amdgcn_exp2f(sc[e] + (t[e] - mg[y]));
+#pragma unroll
+        for (int j = 0; j < 8; j++) pb[j >> 2][j & 3] = pack_f16(t[2 * j], t[2 * j + 1]);
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+          acc[2 * y] = mfma32_f16(vf[4 * k + 2 * y], pb[k], acc[2 * y]);
+          acc[2 * y + 1] = mfma32_f16(vf[4 * k + 2 * y + 1], pb[k], acc[2 * y + 1]);
         }
       }
-      float bt = sc[0] + t[0];
-#pragma unroll
-      for (int e = 1; e < 16; e++) bt = fmaxf(bt, sc[e] + t[e]);
-      bt = max_xor32(bt);
-      if (__any(bt - m > most)) {
-        const bool up = bt - m > most;
-        const float to = up ? ceilf(bt) - 7.0f : m, a = most == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - to);
-        if (up) most = 15.0f;
-        m = to;
-#pragma unroll
-        for (int d = 0; d < 4; d++) acc[d] *= a;
-      }
-      u32x4_t pb[2];
-#pragma unroll
-      for (int e = 0; e < 16; e++) t[e] = __builtin_amdgcn_exp2f(sc[e] + (t[e] - m));
-#pragma unroll
-      for (int j = 0; j < 8; j++) pb[j >> 2][j & 3] = pack_f16(t[2 * j], t[2 * j + 1]);
       if (more) read_k(buf, tile + 1);
-#pragma unroll
-      for (int k = 0; k < 8; k++) acc[k & 3] = mfma32_f16(vf[k], pb[k >> 2], acc[k & 3]);
     } else {
       if (__any(bm > most)) {
         const float up = bm > most ? ceilf(bm) - 7.0f : 0.0f;
@@ -1254,8 +1270,8 @@ __global__ void __launch_bounds__(512) kv4_tile_kernel(const Kv4AttnParams p) {
     for (int d = 0; d < 4; d++)
 #pragma unroll
       for (int i = 0; i < 16; i++) acc[d][i] = 0.0f;
-    m = l = poison[0] = poison[1] = 0.0f;
-    most = ml = -INFINITY;
+    m = mg[0] = mg[1] = l = poison[0] = poison[1] = 0.0f;
+    most = most_g[0] = most_g[1] = ml = -INFINITY;
     __syncthreads();  // (the marks are cleared, the first bounds found)
     if (it0 < it1) stage(it0, 0);
     if (it0 + 1 < it1) fetch(it0 + 1);
@@ -1287,14 +1303,19 @@ __global__ void __launch_bounds__(512) kv4_tile_kernel(const Kv4AttnParams p) {
     const float ref = wide ? ml : m - 15.0f;
     const int k = static_cast<int>(__float_as_uint(l) >> 23 & 255u) - 127;
     const int down = -k - static_cast<int>(kDown);
-    const int shift = wide ? down + static_cast<int>(fmaxf(-1000.0f, fminf(1000.0f, m - 15.0f - ml))) : down;
+    int shift[2] = {down, down};
+    if constexpr (wide) {
+#pragma unroll
+      for (int y = 0; y < 2; y++)
+        shift[y] += static_cast<int>(fmaxf(-1000.0f, fminf(1000.0f, mg[y] - 15.0f - ml)));
+    }
     m = l != l ? l : l > 0.0f ? ref + static_cast<float>(k) : -INFINITY;  // a NaN score: the row stays NaN
     l = __builtin_amdgcn_ldexpf(l, down);
 #pragma unroll
     for (int d = 0; d < 4; d++) {
       const float bad = add_xor32(poison[d >> 1]);
 #pragma unroll
-      for (int i = 0; i < 16; i++) acc[d][i] = __builtin_amdgcn_ldexpf(acc[d][i], shift) + bad;
+      for (int i = 0; i < 16; i++) acc[d][i] = __builtin_amdgcn_ldexpf(acc[d][i], shift[d >> 1]) + bad;
     }
     // ---- waves of the same rows, two by two ----
 #pragma unroll

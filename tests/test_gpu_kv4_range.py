@@ -102,3 +102,21 @@ def test_rows_before_a_large_value_keep_their_bits(gpu, Hq, Hkv, M, past):
     f[at] = 2.0 ** 100
     got = check(bmx.attention_kv4, q, scaled_cache(Hkv, n, f), past)
     assert torch.equal(got[:M // 2], clean[:M // 2])
+
+
+@pytest.mark.parametrize("Hq,Hkv,M,past", SPANS)
+@pytest.mark.parametrize("kind", ["2^-7", "2^-28", "2^-40", "2^60", "zero", "swapped", "outliers", "both"])
+def test_groups_far_apart(gpu, Hq, Hkv, M, past, kind):
+    """A group much smaller than the other of its row, everywhere, from row to
+    row in turns, or next to a few rows whose other group is large: each
+    group is judged by itself, and keeps its precision."""
+    n = past + M
+    g = torch.Generator().manual_seed(M + 1)
+    some = torch.rand(n, 1, generator=g)
+    pair = lambda a, b: torch.tensor([[a, b]])
+    f = {"2^-7": pair(2.0 ** -7, 1.0), "2^-28": pair(2.0 ** -28, 1.0), "2^-40": pair(1.0, 2.0 ** -40),
+         "2^60": pair(1.0, 2.0 ** 60), "zero": pair(0.0, 1.0),
+         "swapped": torch.where(some < 0.5, pair(2.0 ** -30, 1.0), pair(1.0, 2.0 ** -30)),
+         "outliers": torch.where(some < 0.05, pair(2.0 ** 35, 1.0), pair(1.0, 1.0)),
+         "both": torch.where(some < 0.5, pair(2.0 ** 100, 2.0 ** 20), pair(2.0 ** -20, 2.0 ** 60))}[kind]
+    check(bmx.attention_kv4, queries(M, Hq, M), scaled_cache(Hkv, n, f.expand(n, 2)), past)
