@@ -50,7 +50,7 @@ struct Kv4AttnParams {
   bmx_kv4 c;
   uint16_t* out;      // [M, Hq*128]
   float* weights;     // [Hkv, cap], or null
-  unsigned* cnt;      // arrival counters, cnt_stride words apart, zero between calls
+  unsigned* cnt;      // arrival counters, kCounterWords apart, zero between calls
   float2* lse;        // [Hq, M] (max * c2, log2 of the sum), or null
   uint4* qp;          // [Hq, M, 17] the queries as the weights' kernel takes them, with lse
   float* part_o;      // [Hq, M, ns, 128]
@@ -60,7 +60,6 @@ struct Kv4AttnParams {
   uint32_t flip;      // sign bits of a bf16 pair where scale < 0
   int ns;             // key splits
   int bps;            // steps of all waves per split
-  int cnt_stride;
   int local;          // every workgroup of a kv head runs on one XCD (shares its L2)
   float* sums;        // [row ranges, Hkv, L] of the weights
 };
@@ -151,6 +150,7 @@ __device__ __forceinline__ uint32_t load1(__amdgpu_buffer_rsrc_t r, int off) {
 // one place.
 constexpr int kAgentCoherent = 16, kL2Coherent = 1;
 constexpr int kLocalCounter = 64;  // words into a counter's 512 bytes
+constexpr int kCounterWords = 128, kMaxCounters = BMX_KV4_COUNTER_BYTES / (4 * kCounterWords);
 __device__ __forceinline__ void store_part(float* p, float x, float y) {
   const uint64_t v = static_cast<uint64_t>(__float_as_uint(x)) | (static_cast<uint64_t>(__float_as_uint(y)) << 32);
   __hip_atomic_store(reinterpret_cast<uint64_t*>(p), v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -341,7 +341,7 @@ __device__ __forceinline__ void join_and_finish(const Kv4AttnParams& p, JoinLds<
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
   if (tid == 0) {
-    unsigned* c = p.cnt + (static_cast<int64_t>(blockIdx.z) * gridDim.x + kvh) * p.cnt_stride;
+    unsigned* c = p.cnt + (static_cast<int64_t>(blockIdx.z) * gridDim.x + kvh) * kCounterWords;
     unsigned n;
     if (p.local) {
       c += kLocalCounter;
@@ -1445,8 +1445,6 @@ __global__ void __launch_bounds__(256) kv4_merge_kernel(const Kv4AttnParams p) {
 // sums go to p.sums [range][head][L], added up by the last workgroup of a
 // range of keys (a launch for it took 1 us more for 509 tokens over 1509 rows).
 constexpr int kWeighWaves = 8, kWeighKeys = kWeighWaves * kKeys, kWeighTiles = 4;
-constexpr int kWeighCounter = 128;  // words from one counter to the next: there are at most 128 (see Kv4Plan::wz)
-static_assert(128 * kWeighCounter * 4 <= BMX_KV4_COUNTER_BYTES);
 __global__ void __launch_bounds__(64 * kWeighWaves) kv4_weigh_kernel(const Kv4AttnParams p) {
   constexpr int kRowsStage = kWeighTiles * kRows, kWords = kRowsStage * kQueryWords;
   constexpr int kPer = (kWords + 64 * kWeighWaves - 1) / (64 * kWeighWaves);
@@ -1577,7 +1575,7 @@ __global__ void __launch_bounds__(64 * kWeighWaves) kv4_weigh_kernel(const Kv4At
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
   if (tid == 0) {
-    unsigned* c = p.cnt + (kvh * gridDim.y + blockIdx.y) * kWeighCounter;
+    unsigned* c = p.cnt + (kvh * gridDim.y + blockIdx.y) * kCounterWords;
     last = __hip_atomic_fetch_add(c, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == gridDim.z - 1;
     if (last) __hip_atomic_store(c, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   }
@@ -1600,14 +1598,18 @@ bool attn_shape_ok(int Hq, int Hkv, int M, int64_t L) {
   return (static_cast<int64_t>(Hq / Hkv) * M + 255) / 256 <= 65535;  // row tiles: grid z
 }
 
-constexpr int kSplitGrid = 256;  // workgroups that a call's splits aim at: one per CU
+// Workgroups that a call's splits aim at: one per CU.  So keys are split over
+// at most half as many (kv head, row tile) pairs, and the weights' rows over as
+// many (kv head, key range) pairs: a counter each.
+constexpr int kSplitGrid = 256;
+static_assert(kSplitGrid / 2 <= kMaxCounters);
 
 // Where the keys of a call are split, and where its workspace's parts are.
 struct Kv4Plan {
   int rc;  // query rows of the kernel: 4, 8, 16, 64, 256
   int nw;  // its waves
-  int tiles, ns, bps, cnt_stride;
-  int wz;  // row ranges of the weights' grid (1 where that has more than 128 workgroups)
+  int tiles, ns, bps;
+  int wz;  // row ranges of the weights' grid (1 where that has more than kSplitGrid / 2 workgroups)
   size_t lse, qp, part_o, part_ml, sums, bytes;  // byte offsets; the counters come first
 };
 
@@ -1671,16 +1673,13 @@ Kv4Plan make_plan(int Hq, int Hkv, int M, int L, bool weigh) {
   }
   const int steps = (L + keys - 1) / keys;
   a.tiles = static_cast<int>((R + a.rc - 1) / a.rc);
-  const int64_t pairs = static_cast<int64_t>(Hkv) * a.tiles;
-  a.cnt_stride = pairs <= 128 ? 128 : 16;
-  if (a.rc <= kRows && pairs * a.cnt_stride * 4 > BMX_KV4_COUNTER_BYTES) ns = 1;
   a.bps = (steps + ns - 1) / ns;
   a.ns = (steps + a.bps - 1) / a.bps;
   // the weights: row ranges until there are as many workgroups as CUs, of at
   // least two stages each
   const int64_t key_groups = static_cast<int64_t>(Hkv) * ((L + kWeighKeys - 1) / kWeighKeys);
   const int64_t stages = (R + kWeighTiles * kRows - 1) / (kWeighTiles * kRows);
-  a.wz = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>((stages + 1) / 2, 256 / key_groups)));
+  a.wz = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>((stages + 1) / 2, kSplitGrid / key_groups)));
   const size_t rows = static_cast<size_t>(Hq) * M;
   size_t at = BMX_KV4_COUNTER_BYTES;
   a.lse = at;
@@ -1760,9 +1759,8 @@ extern "C" int bmx_attention_gqa_kv4(const bmx_bf16* q, const bmx_kv4* cache, bm
   p.flip = scale < 0.0f ? 0x80008000u : 0u;
   p.ns = a.ns;
   p.bps = a.bps;
-  p.cnt_stride = a.cnt_stride;
   // workgroups go to the XCDs in turn by their linear number, x first
-  p.local = a.rc <= kRows && a.ns > 1 && a.cnt_stride == 128 && Hkv % 8 == 0 && attention_xcd_local(as_stream(stream));
+  p.local = a.rc <= kRows && a.ns > 1 && Hkv % 8 == 0 && attention_xcd_local(as_stream(stream));
   const dim3 grid(Hkv, a.ns, a.tiles), block(64 * a.nw);
   const hipStream_t st = as_stream(stream);
   if (a.rc == 4 && a.nw == 4) hipLaunchKernelGGL((kv4_few_kernel<4, 4>), grid, block, 0, st, p);
