@@ -506,7 +506,7 @@ def qk_norm_rope_kv4(q, k, v, q_norm, k_norm, cache, offset, position=None, eps=
     """qk_norm_rope_kv into a 4-bit cache: raw projection rows q [M, Hq*128],
     k, v [M, Hkv*128]; the new rows go to cache rows offset .. offset+M-1,
     rotated for text positions position .. position+M-1 (None: offset; rows
-    and positions differ once rows were evicted).  Returns q_out [Hq, M, 128]."""
+    and positions differ once rows were evicted; at most 2^24).  Returns q_out [Hq, M, 128]."""
     torch = _torch()
     if _elsewhere(cache.device):
         with torch.cuda.device(cache.device):

@@ -37,6 +37,8 @@ int check_kv4_rows(const char* what, const bmx_kv4* c, int M, int offset) {
 
 namespace {
 
+constexpr int kMaxPosition = 1 << 24;  // the largest up to which every position is an fp32 number
+
 typedef __attribute__((ext_vector_type(2))) unsigned short u16x2_t;
 template <int CTRL>
 __device__ __forceinline__ u16x2_t dpp_u16x2(u16x2_t v) {
@@ -271,7 +273,9 @@ extern "C" int bmx_qk_norm_rope_kv4(const bmx_bf16* q, const bmx_bf16* k, const 
   if (!q || !k || !v || !q_norm || !k_norm || !q_out) return set_error(BMX_E_ARG, "qk_norm_rope_kv4: null pointer");
   if (n_heads <= 0) return set_error(BMX_E_SHAPE, "qk_norm_rope_kv4: n_heads=%d", n_heads);
   if (int rc = check_kv4_rows("qk_norm_rope_kv4", cache, M, offset)) return rc;
-  if (position < 0) return set_error(BMX_E_ARG, "qk_norm_rope_kv4: position=%lld", static_cast<long long>(position));
+  if (position < 0 || position > kMaxPosition - (M - 1))
+    return set_error(BMX_E_ARG, "qk_norm_rope_kv4: position=%lld, M=%d (up to position %d)",
+                     static_cast<long long>(position), M, kMaxPosition);
   if (M == 0) return BMX_OK;
   const int64_t waves = static_cast<int64_t>(M) * (n_heads + cache->n_kv_heads);
   if (waves > INT32_MAX) return set_error(BMX_E_SHAPE, "qk_norm_rope_kv4: M=%d too large for one launch", M);

@@ -311,6 +311,8 @@ int bmx_kv4_read(const bmx_kv4 *cache, bmx_bf16 *k, bmx_bf16 *v, int M, int head
  * as bmx_kv4_write does it (the same bits as the two calls), the queries to
  * q_out [n_heads, M, 128].  `position` is the first token's position in the
  * text: it sets the rotation and is not the row once rows have been evicted.
+ * 0 <= position, position + M - 1 <= 2^24 (BMX_E_ARG): the angle takes it as an
+ * fp32 number.
  * Replaces: the same sequence of Qwen3::forward_internal as
  *   bmx_qk_norm_rope_kv (crates/base-mlx-core/src/model/qwen3.rs:392-489). */
 int bmx_qk_norm_rope_kv4(const bmx_bf16 *q, const bmx_bf16 *k, const bmx_bf16 *v, const bmx_bf16 *q_norm,

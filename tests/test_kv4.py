@@ -202,6 +202,13 @@ def test_evict_refuses_a_cache_over_itself(shared):
     assert f(into=ctypes.pointer(into), w_into=7 * P + 784) == bmx.BMX_E_ARG
 
 
+def test_rope_refuses_positions_past_fp32():
+    """The rotation's angle takes the position as an fp32 number: beyond 2^24 neighbours would share one."""
+    f = entry_points(kv4())["rope"]
+    for position in (2 ** 24 - 2, 2 ** 24 + 1, 2 ** 31, 2 ** 40, 2 ** 63 - 1):
+        assert f(position=position) == bmx.BMX_E_ARG and "position" in bmx.last_error()
+
+
 def test_attention_row_range_does_not_wrap():
     f = entry_points(kv4())["attention"]
     assert f(M=2 ** 31 - 1, offset=100) == bmx.BMX_E_KV_CAPACITY
