@@ -12,8 +12,8 @@
 // where -16 Q_g is the accumulator's start and b_g Q_g one more product over
 // k = (group, piece) with Q_g in three bf16 pieces (24 bits); the scales
 // multiply fp32 results.  So a score is fp32 arithmetic on the stored values:
-// nothing of K is rounded.  For the values (of many rows: at kv4_tile_kernel),
-// with p' = bf16(p s_g),
+// nothing of K is rounded.  For the values (of few rows: at kv4_few_kernel, of
+// many: at kv4_tile_kernel), with p' = bf16(p s_g),
 //   sum_j p_j (s n + b)_j = sum_j p'_j (16 + n_j) - 23.5 sum_j p'_j
 //                         + 7.5 sum_j p~_j s_j + sum_j p~_j b_j,  p~ = bf16(p):
 // the roundings of p' then act on n - 7.5, the centred nibble, and so weigh
@@ -629,8 +629,11 @@ __global__ void __launch_bounds__(64 * NW) kv4_rows_kernel(const Kv4AttnParams p
 // multiplied with all 16 columns (the queries RC by RC again) and each lane
 // takes the result of its tile; P goes back as a B operand with zeros where a
 // column's tile is not the product's, two tiles to a product.  The columns of
-// a query are added at the end.  The sums over a lane's own keys that take
-// p', s and b (see the top) are fp32 here.
+// a query are added at the end.  p s goes to the products in two bf16 pieces, 16
+// bits, and what 16 + n has too much, -16 sum p s, and the biases' sum p b are
+// fp32 sums over a lane's own keys: the outputs are off by their own rounding
+// alone (one piece: 0.0018 of the norm for one token over 4097 rows, 0.0024 over
+// 131072, where the rounding is 0.0017; it saved 1 and 3 % of the time).
 // One token over 131072 rows, 32 heads of 8: 33 us, 4.6 TB/s, where the kernel
 // above takes 44.
 template <int RC, int NW>
@@ -785,38 +788,42 @@ __global__ void __launch_bounds__(64 * NW) kv4_few_kernel(const Kv4AttnParams p)
     float mid[2][4];
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-      mid[0][i] = __builtin_fmaf(7.5f, ps[0][i], pr[i] * lo_f(vb[i]));
-      mid[1][i] = __builtin_fmaf(7.5f, ps[1][i], pr[i] * hi_f(vb[i]));
+      mid[0][i] = __builtin_fmaf(-16.0f, ps[0][i], pr[i] * lo_f(vb[i]));
+      mid[1][i] = __builtin_fmaf(-16.0f, ps[1][i], pr[i] * hi_f(vb[i]));
       if constexpr (cut) {
         if (key0 + i >= lim) pr[i] = ps[0][i] = ps[1][i] = mid[0][i] = mid[1][i] = 0.0f;
       }
     }
     l += (pr[0] + pr[1]) + (pr[2] + pr[3]);
-    uint32_t pb[2][2];
+    uint32_t pb[2][2][2];  // [group][piece]
 #pragma unroll
     for (int y = 0; y < 2; y++) {
-      pb[y][0] = pack_bf(ps[y][0], ps[y][1]);
-      pb[y][1] = pack_bf(ps[y][2], ps[y][3]);
-      const float sum = (lo_f(pb[y][0]) + hi_f(pb[y][0])) + (lo_f(pb[y][1]) + hi_f(pb[y][1]));
-      add[y] += __builtin_fmaf(-23.5f, sum, (mid[y][0] + mid[y][1]) + (mid[y][2] + mid[y][3]));
+#pragma unroll
+      for (int j = 0; j < 2; j++) {
+        pb[y][0][j] = pack_bf(ps[y][2 * j], ps[y][2 * j + 1]);
+        pb[y][1][j] = pack_bf(ps[y][2 * j] - lo_f(pb[y][0][j]), ps[y][2 * j + 1] - hi_f(pb[y][0][j]));
+      }
+      add[y] += (mid[y][0] + mid[y][1]) + (mid[y][2] + mid[y][3]);
     }
 #pragma unroll
     for (int u = 0; u < T / 2; u++)
 #pragma unroll
       for (int y = 0; y < 2; y++) {
-        const u32x4_t pv = {blk == 2 * u ? pb[y][0] : 0u, blk == 2 * u ? pb[y][1] : 0u,
-                            blk == 2 * u + 1 ? pb[y][0] : 0u, blk == 2 * u + 1 ? pb[y][1] : 0u};
         uint32_t v[4];
 #pragma unroll
         for (int j = 0; j < 4; j++) v[j] = __builtin_amdgcn_perm(vw[u][y][j], dpp_ror8(vw[u][y][j]), half_sel);
-        acc[y][0] = mfma(u32x4_t{nibble_pair<0>(v[0], nk), nibble_pair<0>(v[1], nk), nibble_pair<0>(v[2], nk),
-                                 nibble_pair<0>(v[3], nk)}, pv, acc[y][0]);
-        acc[y][1] = mfma(u32x4_t{nibble_pair<1>(v[0], nk), nibble_pair<1>(v[1], nk), nibble_pair<1>(v[2], nk),
-                                 nibble_pair<1>(v[3], nk)}, pv, acc[y][1]);
-        acc[y][2] = mfma(u32x4_t{nibble_pair<2>(v[0], nk), nibble_pair<2>(v[1], nk), nibble_pair<2>(v[2], nk),
-                                 nibble_pair<2>(v[3], nk)}, pv, acc[y][2]);
-        acc[y][3] = mfma(u32x4_t{nibble_pair<3>(v[0], nk), nibble_pair<3>(v[1], nk), nibble_pair<3>(v[2], nk),
-                                 nibble_pair<3>(v[3], nk)}, pv, acc[y][3]);
+        const u32x4_t a[4] = {
+            {nibble_pair<0>(v[0], nk), nibble_pair<0>(v[1], nk), nibble_pair<0>(v[2], nk), nibble_pair<0>(v[3], nk)},
+            {nibble_pair<1>(v[0], nk), nibble_pair<1>(v[1], nk), nibble_pair<1>(v[2], nk), nibble_pair<1>(v[3], nk)},
+            {nibble_pair<2>(v[0], nk), nibble_pair<2>(v[1], nk), nibble_pair<2>(v[2], nk), nibble_pair<2>(v[3], nk)},
+            {nibble_pair<3>(v[0], nk), nibble_pair<3>(v[1], nk), nibble_pair<3>(v[2], nk), nibble_pair<3>(v[3], nk)}};
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+          const u32x4_t pv = {blk == 2 * u ? pb[y][k][0] : 0u, blk == 2 * u ? pb[y][k][1] : 0u,
+                              blk == 2 * u + 1 ? pb[y][k][0] : 0u, blk == 2 * u + 1 ? pb[y][k][1] : 0u};
+#pragma unroll
+          for (int i = 0; i < 4; i++) acc[y][i] = mfma(a[i], pv, acc[y][i]);
+        }
       }
     load_v(b + NW);
   };
