@@ -12,13 +12,12 @@
 // where -16 Q_g is the accumulator's start and b_g Q_g one more product over
 // k = (group, piece) with Q_g in three bf16 pieces (24 bits); the scales
 // multiply fp32 results.  So a score is fp32 arithmetic on the stored values:
-// nothing of K is rounded.  For the values (of few rows: at kv4_few_kernel, of
-// many: at kv4_tile_kernel), with p' = bf16(p s_g),
-//   sum_j p_j (s n + b)_j = sum_j p'_j (16 + n_j) - 23.5 sum_j p'_j
-//                         + 7.5 sum_j p~_j s_j + sum_j p~_j b_j,  p~ = bf16(p):
-// the roundings of p' then act on n - 7.5, the centred nibble, and so weigh
-// no more than rounding P does in a bf16 attention.  The last three sums are
-// products with constant or raw scale / bias rows.
+// nothing of K is rounded.  For the values (of many rows: at kv4_tile_kernel),
+//   sum_j p_j (s n + b)_j = sum_j (p s)_j (16 + n_j) - 16 sum_j p_j s_j + sum_j p_j b_j
+// with p s_g, and p where the last two sums are products with rows of scales
+// and biases, in two bf16 pieces each: 16 bits, so that the outputs are off by
+// their own rounding alone.  (One piece: 0.0018 to 0.0024 of the norm, long
+// contexts worst, where the rounding is 0.0017.)
 #include <math.h>
 
 #include <algorithm>
@@ -376,10 +375,11 @@ __device__ __forceinline__ void join_and_finish(const Kv4AttnParams& p, JoinLds<
 //     4 (li / 8) + i.  Lane li < 8 loads a word of the even key of a pair,
 //     lane li + 8 the same word of the odd key, and they swap halves.
 // The next step's K is loaded once the scores are done, its V once P V is.
-// Bound by instruction issue: a step takes about 310 VALU instructions and 21
-// products, which hardly overlap (32 tokens over 16384 rows, 32 heads of 8: 32
-// us).  Two row tiles per wave, to share the 180 that nibbles and scales take,
-// spilled registers and were no faster.
+// Bound by instruction issue: a step takes about 370 VALU instructions and 28
+// products, which hardly overlap (64 tokens over 4064 rows, 32 heads of 8: 21
+// us; with one piece of p s and p, 60 instructions and 7 products less, 19).
+// Two row tiles per wave, to share the 180 that nibbles and scales take, spilled
+// registers and were no faster.
 template <int NW>
 __global__ void __launch_bounds__(64 * NW) kv4_rows_kernel(const Kv4AttnParams p) {
   __shared__ JoinLds<NW, kRows> sm;
@@ -465,16 +465,13 @@ __global__ void __launch_bounds__(64 * NW) kv4_rows_kernel(const Kv4AttnParams p
   }
 
   const f32x4_t zero = {0.0f, 0.0f, 0.0f, 0.0f};
-  // edge: rows 0, 1 sum p~ b, rows 2, 3 sum p~ s of groups 0, 1; mid: -23.5
-  // sum p', in every row (a register set per group: a zero row would carry one
-  // group's infinite scale to the other)
-  f32x4_t acc[2][4], edge = zero, mid[2] = {zero, zero};
+  // edge: rows 0, 1 sum p b, rows 2, 3 sum p s of groups 0, 1
+  f32x4_t acc[2][4], edge = zero;
 #pragma unroll
   for (int y = 0; y < 2; y++)
 #pragma unroll
     for (int i = 0; i < 4; i++) acc[y][i] = zero;
   float m = -INFINITY, l = 0.0f, slow[2] = {0.0f, 0.0f};
-  const uint32_t centre = 0xC1BCC1BCu;  // bf16 -23.5 twice
   const uint32_t half_sel = li < 8 ? 0x01000504u : 0x07060302u;
   // (selector 0x0c gives a zero byte: rows from 4 on take nothing)
   const uint32_t odd_sel = li >= 4 ? 0x0c0c0c0cu : li & 1 ? 0x07060302u : 0x05040100u;
@@ -512,7 +509,7 @@ __global__ void __launch_bounds__(64 * NW) kv4_rows_kernel(const Kv4AttnParams p
     load_k(b + NW);
     // ---- running softmax: the maximum over all keys of a query ----
     const int key0 = b * kKeys + 4 * g;
-    u32x4_t pb[2], pt;
+    u32x4_t pb[2][2], pt[2];  // [group][piece], [piece]
     bool odd = false;
     u32x4_t bw[2];
     if constexpr (cut) {
@@ -549,7 +546,6 @@ __global__ void __launch_bounds__(64 * NW) kv4_rows_kernel(const Kv4AttnParams p
 #pragma unroll
       for (int y = 0; y < 2; y++) {
         slow[y] *= a;
-        mid[y] *= a;
 #pragma unroll
         for (int i = 0; i < 4; i++) acc[y][i] *= a;
       }
@@ -573,9 +569,20 @@ __global__ void __launch_bounds__(64 * NW) kv4_rows_kernel(const Kv4AttnParams p
     l += ((pr[0] + pr[1]) + (pr[2] + pr[3])) + ((pr[4] + pr[5]) + (pr[6] + pr[7]));
 #pragma unroll
     for (int j = 0; j < 4; j++) {
-      pb[0][j] = pack_bf(ps[0][2 * j], ps[0][2 * j + 1]);
-      pb[1][j] = pack_bf(ps[1][2 * j], ps[1][2 * j + 1]);
-      pt[j] = pack_bf(pr[2 * j], pr[2 * j + 1]);
+      auto pieces = [](float a, float b, uint32_t& hi, uint32_t& lo) {
+        hi = pack_bf(a, b);
+        lo = pack_bf(a - lo_f(hi), b - hi_f(hi));
+      };
+      uint32_t hi, lo;
+#pragma unroll
+      for (int y = 0; y < 2; y++) {
+        pieces(ps[y][2 * j], ps[y][2 * j + 1], hi, lo);
+        pb[y][0][j] = hi;
+        pb[y][1][j] = lo;
+      }
+      pieces(pr[2 * j], pr[2 * j + 1], hi, lo);
+      pt[0][j] = hi;
+      pt[1][j] = lo;
     }
     // ---- P V ----
 #pragma unroll
@@ -589,8 +596,9 @@ __global__ void __launch_bounds__(64 * NW) kv4_rows_kernel(const Kv4AttnParams p
           {nibble_pair<2>(v[0], nk), nibble_pair<2>(v[1], nk), nibble_pair<2>(v[2], nk), nibble_pair<2>(v[3], nk)},
           {nibble_pair<3>(v[0], nk), nibble_pair<3>(v[1], nk), nibble_pair<3>(v[2], nk), nibble_pair<3>(v[3], nk)}};
 #pragma unroll
-      for (int i = 0; i < 4; i++) acc[y][i] = mfma(a[i], pb[y], acc[y][i]);
-      mid[y] = mfma(u32x4_t{centre, centre, centre, centre}, pb[y], mid[y]);
+      for (int k = 0; k < 2; k++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) acc[y][i] = mfma(a[i], pb[y][k], acc[y][i]);
     }
     {
       // rows 0..3 of A: b_0, b_1, s_0, s_1 of the step's keys
@@ -605,7 +613,8 @@ __global__ void __launch_bounds__(64 * NW) kv4_rows_kernel(const Kv4AttnParams p
           if ((a[j] & 0x7f800000u) == 0x7f800000u) a[j] &= 0xffffu;
         }
       }
-      edge = mfma(a, pt, edge);
+#pragma unroll
+      for (int k = 0; k < 2; k++) edge = mfma(a, pt[k], edge);
     }
     load_v(b + NW);
   };
@@ -617,8 +626,7 @@ __global__ void __launch_bounds__(64 * NW) kv4_rows_kernel(const Kv4AttnParams p
   float x[2];  // what every dim of a group gets besides its product
 #pragma unroll
   for (int y = 0; y < 2; y++)
-    x[y] = mid[y][0] + __builtin_fmaf(7.5f, __shfl(edge[2 + y], li, 64), __shfl(edge[y], li, 64)) +
-           add_xor32(add_xor16(slow[y]));
+    x[y] = __builtin_fmaf(-16.0f, __shfl(edge[2 + y], li, 64), __shfl(edge[y], li, 64)) + add_xor32(add_xor16(slow[y]));
   join_and_finish<NW, kRows>(p, sm, kvh, split, r0, RT, m, add_xor32(add_xor16(l)), acc, x);
 }
 
@@ -629,11 +637,9 @@ __global__ void __launch_bounds__(64 * NW) kv4_rows_kernel(const Kv4AttnParams p
 // multiplied with all 16 columns (the queries RC by RC again) and each lane
 // takes the result of its tile; P goes back as a B operand with zeros where a
 // column's tile is not the product's, two tiles to a product.  The columns of
-// a query are added at the end.  p s goes to the products in two bf16 pieces, 16
-// bits, and what 16 + n has too much, -16 sum p s, and the biases' sum p b are
-// fp32 sums over a lane's own keys: the outputs are off by their own rounding
-// alone (one piece: 0.0018 of the norm for one token over 4097 rows, 0.0024 over
-// 131072, where the rounding is 0.0017; it saved 1 and 3 % of the time).
+// a query are added at the end.  The sums over a lane's own keys that take s
+// and b (see the top) are fp32 here.  The second piece of p s takes 1 % of the
+// time over 4097 rows, 3 % over 131072.
 // One token over 131072 rows, 32 heads of 8: 33 us, 4.6 TB/s, where the kernel
 // above takes 44.
 template <int RC, int NW>
@@ -1621,15 +1627,16 @@ struct Kv4Plan {
 };
 
 // The kernel and split count for R > 8 query rows per kv head, by estimated
-// time (us) over rounds of 256 workgroups.  16 rows: 5 a round and 1.32 per
+// time (us) over rounds of 256 workgroups.  16 rows: 5.8 a round and 1.53 per
 // step of a wave (32 keys; two waves share a SIMD).  64 and 256 rows: 1.93 per
 // iteration (128 keys), 2.05 + 0.4 per full tile (64 keys).  Splits cost the
 // last workgroup's merge, or a second launch that reads all partials from
 // memory.
-// Measured (32 q heads over 8; 16 / 64 / 256 rows, us): 32 tokens over 16384
-// 30 / 31 / 34, over 30032 50 / 44 / 48; 128 over 4128 26 / 32 / 34, over 16128
-// 84 / 74 / 59; 200 over 200 12 / 12 / 16; 512 over 512 27 / 16 / 23, over 2512
-// 67 / 44 / 48; 1024 over 1024 61 / 42 / 37.
+// Measured (32 q heads over 8; 16 / 64 / 256 rows, us): 32 tokens over 4032
+// 14.8 / 19.1 / 22.4, over 16384 35 / 32 / 35, over 30032 60 / 45 / 49; 64 over
+// 4064 21 / 23 / 29; 128 over 4128 31 / 32 / 34, over 16128 102 / 76 / 59; 200
+// over 200 12.6 / 12.1 / 16; 512 over 512 28 / 16 / 23, over 2512 78 / 45 / 48;
+// 1024 over 1024 66 / 43 / 38.
 void choose_kernel(int Hkv, int64_t R, int M, int L, int* rc, int* ns_out) {
   const double seen = L - 0.5 * (M - 1);  // keys of an average query
   double least = 1e30;
@@ -1647,7 +1654,7 @@ void choose_kernel(int Hkv, int64_t R, int M, int L, int* rc, int* ns_out) {
       const double n = std::max(1.0, (rows == 64 ? L : seen) / (static_cast<double>(keys) * ns));
       const double mb = 520e-6 * kKeys * Hkv * ((R + kKeys - 1) / kKeys) * ns;  // of partials
       double t;
-      if (rows == 16) t = 1.0 + rounds * (5.0 + 1.32 * n) + (ns > 1 ? 3.0 : 0.0);
+      if (rows == 16) t = 1.0 + rounds * (5.8 + 1.53 * n) + (ns > 1 ? 3.0 : 0.0);
       else
         t = rows == 64 ? 8.2 + rounds * n * 1.93 + (ns > 1 ? 1.5 + 0.7 * mb : 0.0)
                        : 13.1 + rounds * n * (2.05 + 0.4 * std::min<double>(R, 256.0) / 256.0) + (ns > 1 ? 0.35 * mb : 0.0);
