@@ -83,7 +83,8 @@ __device__ __forceinline__ int wave_id() { return __builtin_amdgcn_readfirstlane
 // All weights hold a factor 2^-28 where they are summed up, which the division
 // by their sum takes out again: 2^24 rows of values of 2^120, whose sums of
 // p s (16 + n) are 2^122 each, at a weight of 2^8 (see moves) stay below 2^127.
-// What a row draws below 2^-98 of the largest weight is 0.
+// A weight below 2^-88 of the largest loses the second of its bf16 pieces, one
+// below 2^-98 is 0.
 constexpr float kDown = 28.0f;
 
 // Whether a running maximum m moves to its step's maximum bm: only where the
@@ -641,7 +642,7 @@ __global__ void __launch_bounds__(64 * NW) kv4_rows_kernel(const Kv4AttnParams p
 // and b (see the top) are fp32 here.  The second piece of p s takes 1 % of the
 // time over 4097 rows, 3 % over 131072.
 // One token over 131072 rows, 32 heads of 8: 33 us, 4.6 TB/s, where the kernel
-// above takes 44.
+// above took 44 with one piece.
 template <int RC, int NW>
 __global__ void __launch_bounds__(64 * NW) kv4_few_kernel(const Kv4AttnParams p) {
   constexpr int T = 16 / RC, kStep = 16 * T;
@@ -898,12 +899,13 @@ __device__ __forceinline__ bool kv4_finite(float s, float b) { return kv4_most(s
 // taken out, so that splits are joined by what they weigh.  With 11 bits in P and V the outputs are off by little more
 // than their own rounding: 0.0017 of the norm for 2048 tokens over 4096 rows,
 // where bf16 for both gave 0.0028.
-// 2048 tokens over 4096 rows, 32 heads of 8: 145 us, 710 TFLOP/s, 56 % of what
-// a large matrix product reaches.  A tile of 32 x 32 takes 17 products of 32
-// cycles and about 120 VALU instructions of 4 with its share of the unpacking,
-// 16 of them exponentials of 16: the two hardly overlap, so the VALU work is
-// half the time.  Rates of the counters: matrix cores busy 36 %, VALU 49 %,
-// LDS 44 %, 1 / 9 of that in bank conflicts.
+// 2048 tokens over 4096 rows, 32 heads of 8: 149 us, 692 TFLOP/s, 54 % of what
+// a large matrix product reaches (347 us where every row takes the wide pass,
+// too).  A tile of 32 x 32 takes 17 products of 32 cycles and about 150 VALU
+// instructions of 4 with its share of the unpacking, 16 of them exponentials of
+// 16: the two hardly overlap, so the VALU work is half the time.  Rates of the
+// counters: matrix cores busy 35 %, VALU 44 %, LDS 43 %, 1 / 9 of that in bank
+// conflicts.
 // A value that is not finite (its scale or bias is not) goes to LDS as 0 and
 // marks the iteration, as a key's scale or bias that is not finite does; the
 // rows that see it become NaN by themselves.
@@ -1676,7 +1678,8 @@ Kv4Plan make_plan(int Hq, int Hkv, int M, int L, bool weigh) {
     a.rc = R <= 4 ? 4 : 8;
     // workgroups of 4 waves as long as one step of each covers the context
     // with a workgroup per CU: they start and join sooner (32 heads over 8, us
-    // with 4 / 8 waves: 4097 rows 8.7 / 10.8, 8192 9.8 / 11.3, but 12001 14.0 / 12.2)
+    // with 4 / 8 waves: 4097 rows 8.6 / 10.6, 8192 9.2 / 10.5, 12001 10.4 / 10.9,
+    // 20001 12.2 / 13.1, but 131072 37 / 34)
     keys = a.rc == 4 ? 64 : 32;
     a.nw = Hkv * ((L + 4 * keys - 1) / (4 * keys)) <= kSplitGrid ? 4 : 8;
     keys *= a.nw;

@@ -296,6 +296,8 @@ typedef struct {
  * overflows fp32, gets NaN for scale and bias.  Rows outside the range stay
  * as they are; offset + M > capacity returns BMX_E_KV_CAPACITY and writes
  * nothing; M = 0 is a no-op.
+ * (The layout is MLX's, the choice of bias and scale is not: its quantizer
+ * anchors the end of larger magnitude and gives other nibbles.)
  * The 4-bit form of the write mlx_ext::slice_update makes
  * (crates/base-mlx-core/src/model/qwen3.rs:431-489). */
 int bmx_kv4_write(const bmx_bf16 *k, int64_t k_head_stride, int64_t k_row_stride, const bmx_bf16 *v,
@@ -335,9 +337,10 @@ int bmx_qk_norm_rope_kv4(const bmx_bf16 *q, const bmx_bf16 *k, const bmx_bf16 *v
  * (BMX_E_ARG).  A row that a query does not see leaves it alone, whatever it
  * holds; one that it sees, with a scale or bias that is not finite, makes
  * that group's 64 outputs (V) or all of them and the kv head's weights (K)
- * not finite.  Values (V) of 2^-60 to 2^120 in magnitude keep their precision
- * over any number of rows; smaller ones are off by 2^-70 at most.  A row whose
- * weight is below 2^-98 of the query's largest may count as one of weight 0.
+ * not finite.  With values (V) up to 2^120 in magnitude and any number of rows
+ * outputs keep their precision from 2^-60 on; smaller ones are off by 2^-70 at
+ * most.  What a row adds at a weight below 2^-88 of the query's largest may be
+ * lost.
  * Replaces: mlx_rs::fast::scaled_dot_product_attention as
  *   bmx_attention_gqa does (crates/base-mlx-core/src/model/qwen3.rs:491-518);
  *   the reference has no quantized cache and no eviction. */
