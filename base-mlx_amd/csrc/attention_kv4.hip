@@ -53,7 +53,7 @@ struct Kv4AttnParams {
   float2* lse;        // [Hq, M] (max * c2, log2 of the sum), or null
   uint4* qp;          // [Hq, M, 17] the queries as the weights' kernel takes them, with lse
   float* part_o;      // [Hq, M, ns, 128]
-  float* part_ml;     // [Hq, M, ns, 2]; of kv4_tile_kernel by 32-row tiles, as part_o, its maxima times c2
+  float* part_ml;     // [Hq, M, ns, 2]; of kv4_tile_kernel by 32-row tiles, as part_o, and relative to powers of two (log2)
   int Hq, M, offset;
   float c2;           // |scale| log2(e)
   uint32_t flip;      // sign bits of a bf16 pair where scale < 0
@@ -895,10 +895,11 @@ __device__ __forceinline__ bool kv4_finite(float s, float b) { return kv4_most(s
 // group by the group's own e.  So are rows that see a key whose groups are more
 // than 2^6 apart: in the smaller one P 2^-25 of the largest, which is 2^7 at
 // least and belongs to the other, would vanish, a part of N 2^-26 at most with
-// N keys.  (Three exponentials per score; no other row's bits change.)  A row leaves with its weights' exponent
-// taken out, so that splits are joined by what they weigh.  With 11 bits in P and V the outputs are off by little more
-// than their own rounding: 0.0017 of the norm for 2048 tokens over 4096 rows,
-// where bf16 for both gave 0.0028.
+// N keys.  (Three exponentials per score; no other row's bits change.)  A row
+// leaves with its weights' exponent taken out, so that splits are joined by what
+// they weigh.  With 11 bits in P and V the outputs are off by little more than
+// their own rounding: 0.0017 of the norm for 2048 tokens over 4096 rows, where
+// bf16 for both gave 0.0028.
 // 2048 tokens over 4096 rows, 32 heads of 8: 149 us, 692 TFLOP/s, 54 % of what
 // a large matrix product reaches (347 us where every row takes the wide pass,
 // too).  A tile of 32 x 32 takes 17 products of 32 cycles and about 150 VALU
@@ -932,7 +933,7 @@ __global__ void __launch_bounds__(512) kv4_tile_kernel(const Kv4AttnParams p) {
   __shared__ int mark[4];
   __shared__ int first_wide;  // the first key whose values the plain pass does not serve
   __shared__ __align__(16) float vscale[4][KPI];
-  __shared__ uint32_t ve[4][KPI];
+  __shared__ __align__(16) uint32_t ve[4][KPI];
   __shared__ __align__(16) uint16_t vsb[4][2][2][KPI];  // ... scales, biases of group 0, 1, times 2^(15 - e), as fp16
   Stage* const st = reinterpret_cast<Stage*>(lds);
   Join& jn = *reinterpret_cast<Join*>(lds);

@@ -66,7 +66,7 @@ def head_reference(q, cache, h, past, scale):
     return out, p, bound, weigh, big
 
 
-def judge(got, out, bound, what=""):
+def hold(got, out, bound, what=""):
     """Every element within its bound, and every row's half (a group of 64) close as a whole."""
     off = (got - out).abs() / bound
     assert bool(torch.isfinite(got).all()), f"{what}: not finite"
@@ -88,7 +88,7 @@ def check(call, q, cache, past, scale=None, weigh=True):
     for h in range(Hkv):
         out, p, bound, tol, big = head_reference(q, cache, h, past, scale)
         g = got.view(M, Hq, D)[:, h * rep:(h + 1) * rep].transpose(0, 1).reshape(rep * M, D).double()
-        judge(g, out, bound, f"kv head {h}")
+        hold(g, out, bound, f"kv head {h}")
         if weigh:
             want = 0.5 + p.sum(0)
             d = (w[h, :L].double() - want).abs() / (tol + 4 * U24 * (0.5 + want))

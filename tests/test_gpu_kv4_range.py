@@ -109,7 +109,7 @@ def test_rows_before_a_large_value_keep_their_bits(gpu, Hq, Hkv, M, past):
 def test_groups_far_apart(gpu, Hq, Hkv, M, past, kind):
     """A group much smaller than the other of its row, everywhere, from row to
     row in turns, or next to a few rows whose other group is large: each
-    group is judged by itself, and keeps its precision."""
+    group counts by itself, and keeps its precision."""
     n = past + M
     g = torch.Generator().manual_seed(M + 1)
     some = torch.rand(n, 1, generator=g)
