@@ -1058,8 +1058,8 @@ __global__ void __launch_bounds__(512) kv4_tile_kernel(const Kv4AttnParams p) {
     constexpr bool wide = decltype(wide_)::value;
     const float m0 = kv4_most(lo_f(bs), lo_f(bb)), m1 = kv4_most(hi_f(bs), hi_f(bb));
     const bool ok0 = m0 <= kFloatMax, ok1 = m1 <= kFloatMax;
-    const int a0 = exponent(m0), a1 = exponent(m1);  // (of a group that is not finite: as the other)
-    int e0 = ok0 || !ok1 ? a0 : a1, e1 = ok1 ? a1 : e0;
+    // (a group that is not finite: as the other)
+    int e0 = exponent(ok0 ? m0 : ok1 ? m1 : 0.0f), e1 = exponent(ok1 ? m1 : ok0 ? m0 : 0.0f);
     const bool apart = max(e0, e1) - min(e0, e1) > kApart;
     if constexpr (!wide) e0 = e1 = max(e0, e1);
     const float r0 = __uint_as_float(static_cast<uint32_t>(127 + 15 - e0) << 23);

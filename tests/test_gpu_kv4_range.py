@@ -120,3 +120,24 @@ def test_groups_far_apart(gpu, Hq, Hkv, M, past, kind):
          "outliers": torch.where(some < 0.05, pair(2.0 ** 35, 1.0), pair(1.0, 1.0)),
          "both": torch.where(some < 0.5, pair(2.0 ** 100, 2.0 ** 20), pair(2.0 ** -20, 2.0 ** 60))}[kind]
     check(bmx.attention_kv4, queries(M, Hq, M), scaled_cache(Hkv, n, f.expand(n, 2)), past)
+
+
+@pytest.mark.parametrize("Hq,Hkv,M,past", KERNELS)
+@pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan])
+@pytest.mark.parametrize("name", ["v_scales", "v_biases"])
+def test_a_row_of_bad_values_leaves_the_weights_alone(gpu, Hq, Hkv, M, past, name, bad):
+    """Both groups of a row's values not finite: the outputs of the queries that
+    see it are not, the weights do not change, nor do the other queries' bits."""
+    at, q = past + M // 2, queries(M, Hq, M)
+    out, w = [], []
+    for spoil in (False, True):
+        cache = random_cache(4, Hkv, past + M, past + M)
+        cache.v[0, at] = 0x77777777
+        if spoil:
+            getattr(cache, name)[0, at] = bad
+        w.append(torch.zeros(Hkv, past + M, device="cuda"))
+        out.append(bmx.attention_kv4(q, cache, past, weights=w[-1]).view(M, Hkv, Hq // Hkv, D))
+    assert not torch.isfinite(out[1][M // 2:, 0]).any()
+    assert torch.equal(out[1][:M // 2], out[0][:M // 2]) and torch.equal(out[1][:, 1:], out[0][:, 1:])
+    # (the weights' sum is added up with another exponent for that row: a few roundings)
+    assert ((w[1] - w[0]).abs() <= 16 * 2.0 ** -24 * w[0]).all()
