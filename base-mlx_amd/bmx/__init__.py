@@ -639,6 +639,196 @@ def kv4_evict(cache, weights, length, budget, sink=4, recent=0, into=None, weigh
 
 
 # ---------------------------------------------------------------------------
+# a paged KV cache for a batch of sequences
+# ---------------------------------------------------------------------------
+class _PagedKvStruct(ctypes.Structure):
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p)] + [
+        (n, ctypes.c_int) for n in ("n_pages", "n_kv_heads", "page_size")]
+
+
+class _BatchStruct(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("starts", "lens", "pages")] + [
+        (n, ctypes.c_int) for n in ("n_seqs", "max_pages", "tokens", "max_new")]
+
+
+class _Fixed:
+    """Attributes that stay once set: the library keeps their addresses."""
+
+    def __setattr__(self, name, value):
+        if self.__dict__.get(name, value) is not value:
+            raise BmxError(BMX_E_ARG, f"{name} of a {type(self).__name__} is fixed: make another")
+        self.__dict__[name] = value
+
+
+class PagedKvCache(_Fixed):
+    """bmx_paged_kv: one layer's keys and values in pages, k and v [n_pages,
+    n_kv_heads, page_size, 128] bf16, contiguous, on one GPU; page_size a power
+    of two from 16 to 4096.  The object holds the tensors: change what they hold
+    freely, but other tensors need another object."""
+
+    def __init__(self, k, v):
+        _torch()
+        _require_cuda(k, v)
+        _bf16(k, v)
+        if k.dim() != 4 or k.shape[3] != 128 or v.shape != k.shape:
+            raise BmxError(BMX_E_SHAPE, f"k and v must be [n_pages, n_kv_heads, page_size, 128], got {tuple(k.shape)}, "
+                                        f"{tuple(v.shape)}")
+        _same_device(k, v)
+        self.k, self.v, self.device = k, v, k.device
+        self.n_pages, self.n_kv_heads, self.page_size = k.shape[:3]
+        if max(k.shape) >= 1 << 31:
+            raise BmxError(BMX_E_SHAPE, f"too large: {tuple(k.shape)}")
+        self._struct = _PagedKvStruct(k.data_ptr(), v.data_ptr(), *k.shape[:3])
+        self._ref = ctypes.addressof(self._struct)
+
+    @classmethod
+    def empty(cls, n_pages, n_kv_heads, page_size, device="cuda"):
+        """A zero-filled cache."""
+        torch = _torch()
+        return cls(*(torch.zeros(n_pages, n_kv_heads, page_size, 128, dtype=torch.bfloat16, device=device) for _ in "kv"))
+
+
+class PagedBatch(_Fixed):
+    """bmx_batch: a step's sequences, the same for every layer -- starts
+    [n_seqs + 1], lens [n_seqs] and pages [n_seqs, max_pages] int32, contiguous,
+    on one GPU.  The new tokens of sequence b are packed rows starts[b] ..
+    starts[b + 1] - 1 and the last of its lens[b] cached rows; row j of a
+    sequence lies on page pages[b, j // page_size].  tokens: the packed rows
+    there are (>= starts[-1]); max_new: at least every sequence's new tokens
+    (None: tokens).  The arrays are read when the work runs: change what they
+    hold between steps, or between replays of a graph."""
+
+    def __init__(self, starts, lens, pages, tokens, max_new=None):
+        torch = _torch()
+        _require_cuda(starts, lens, pages)
+        _same_device(starts, lens, pages)
+        if any(t.dtype != torch.int32 for t in (starts, lens, pages)):
+            raise BmxError(BMX_E_ARG, "starts, lens and pages must be int32")
+        B = lens.shape[0] if lens.dim() == 1 else -1
+        if starts.shape != (B + 1,) or pages.dim() != 2 or pages.shape[0] != B:
+            raise BmxError(BMX_E_SHAPE, f"starts [n_seqs + 1], lens [n_seqs], pages [n_seqs, max_pages] expected, got "
+                                        f"{tuple(starts.shape)}, {tuple(lens.shape)}, {tuple(pages.shape)}")
+        max_new = tokens if max_new is None else max_new
+        if not 0 <= tokens < 1 << 31 or not min(tokens, 1) <= max_new <= tokens or max(pages.shape) >= 1 << 31:
+            raise BmxError(BMX_E_SHAPE, f"tokens={tokens}, max_new={max_new}")
+        self.starts, self.lens, self.pages, self.device = starts, lens, pages, lens.device
+        self.n_seqs, self.max_pages, self.tokens, self.max_new = B, pages.shape[1], tokens, max_new
+        self._struct = _BatchStruct(starts.data_ptr(), lens.data_ptr(), pages.data_ptr(), B, pages.shape[1], tokens,
+                                    max_new)
+        self._ref = ctypes.addressof(self._struct)
+
+    @classmethod
+    def of(cls, new, lens, pages, device="cuda"):
+        """From lists: per sequence its new tokens, its cached rows with them,
+        and its pages."""
+        torch = _torch()
+        if not len(new) == len(lens) == len(pages):
+            raise BmxError(BMX_E_SHAPE, f"{len(new)} counts of new tokens, {len(lens)} lengths, {len(pages)} page lists")
+        starts = [0]
+        for n in new:
+            starts.append(starts[-1] + n)
+        width = max([1, *map(len, pages)])
+        table = [[*p, *[-1] * (width - len(p))] for p in pages]
+        i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=device)
+        return cls(i32(starts), i32(list(lens)), i32(table).reshape(len(pages), width), starts[-1], max([0, *new]))
+
+
+def _paged_args(cache, batch, *ts):
+    for t in ts:
+        if not t.is_cuda or not t.is_contiguous():
+            _require_cuda(t)
+        if t.device != cache.device:
+            raise BmxError(BMX_E_ARG, f"tensors on {cache.device} and {t.device}")
+    if batch.device != cache.device:
+        raise BmxError(BMX_E_ARG, f"the cache on {cache.device}, the batch on {batch.device}")
+    _bf16(*ts)
+
+
+def qk_norm_rope_paged(q, k, v, q_norm, k_norm, cache, batch, eps=1e-6, theta=1e6, out=None, stream=None):
+    """Fused QK-norm + RoPE of a batch's packed projection rows q [tokens,
+    Hq*128], k, v [tokens, Hkv*128], keys and values appended to their
+    sequences' pages; returns q_out [Hq, tokens, 128] (rows that belong to no
+    sequence are left unwritten: `out`'s stay as they were)."""
+    if _elsewhere(cache.device):
+        with _T.cuda.device(cache.device):
+            return qk_norm_rope_paged(q, k, v, q_norm, k_norm, cache, batch, eps, theta, out, stream)
+    _paged_args(cache, batch, q, k, v, q_norm, k_norm)
+    T = batch.tokens
+    if q.dim() != 2 or q.shape[0] != T or q.shape[1] % 128 or k.shape != (T, cache.n_kv_heads * 128) or v.shape != k.shape:
+        raise BmxError(BMX_E_SHAPE, f"q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}: [{T}, Hq*128] and "
+                                    f"[{T}, {cache.n_kv_heads}*128] expected")
+    if q_norm.shape != (128,) or k_norm.shape != (128,):
+        raise BmxError(BMX_E_SHAPE, "q_norm and k_norm must hold 128 weights")
+    Hq = q.shape[1] // 128
+    if out is None:
+        out = _empty(stream, cache.device, _T.bfloat16, Hq, T, 128)
+    else:
+        _paged_args(cache, batch, out)
+        if out.shape != (Hq, T, 128):
+            raise BmxError(BMX_E_SHAPE, f"out must be {(Hq, T, 128)}, got {tuple(out.shape)}")
+    if T == 0:
+        return out  # (an empty tensor has no address)
+    call("bmx_qk_norm_rope_paged", q.data_ptr(), k.data_ptr(), v.data_ptr(), q_norm.data_ptr(), k_norm.data_ptr(),
+         out.data_ptr(), cache._ref, batch._ref, Hq, 128, eps, theta, _stream(stream))
+    return out
+
+
+def attention_paged_workspace(n_heads, n_kv_heads, batch, shared=0, device=None, stream=None):
+    """A workspace for attention_paged calls of batches with up to as many
+    tokens, sequences and new tokens of one as `batch` (a PagedBatch, or the
+    three as a tuple) has; shared: whether any has shared rows.  It serves one
+    call at a time."""
+    torch = _torch()
+    sizes = (batch.tokens, batch.n_seqs, batch.max_new) if isinstance(batch, PagedBatch) else tuple(batch)
+    if device is None:
+        device = batch.device if isinstance(batch, PagedBatch) else "cuda"
+    nbytes = 0
+    if 0 < min(n_heads, n_kv_heads, *sizes) and max(n_heads, n_kv_heads, *sizes) < 1 << 31:
+        nbytes = load().bmx_attention_paged_workspace_bytes(n_heads, n_kv_heads, *sizes, int(bool(shared)))
+    if not nbytes:
+        raise BmxError(BMX_E_SHAPE, f"{n_heads} heads over {n_kv_heads}, (tokens, n_seqs, max_new) = {sizes}")
+    with _on_stream(stream, device):
+        return torch.empty(nbytes, dtype=torch.uint8, device=device)
+
+
+def attention_paged(q, cache, batch, scale=None, shared=0, workspace=None, out=None, stream=None):
+    """Causal GQA attention of a batch's packed queries q [Hq, tokens, 128] over
+    their sequences' pages, a token seeing its sequence's rows up to its own;
+    returns [tokens, Hq*128] bf16 (rows that belong to no sequence are left
+    unwritten: `out`'s stay as they were).  shared: rows (whole pages) that all
+    sequences have in common, read once from the pages of sequence 0.
+    workspace: from attention_paged_workspace (None: one for this call)."""
+    if _elsewhere(cache.device):
+        with _T.cuda.device(cache.device):
+            return attention_paged(q, cache, batch, scale, shared, workspace, out, stream)
+    _paged_args(cache, batch, q)
+    T = batch.tokens
+    if q.dim() != 3 or q.shape[1:] != (T, 128) or q.shape[0] == 0 or q.shape[0] % cache.n_kv_heads:
+        raise BmxError(BMX_E_SHAPE, f"q must be [Hq, {T}, 128] with Hq a multiple of {cache.n_kv_heads}, got "
+                                    f"{tuple(q.shape)}")
+    Hq = q.shape[0]
+    if not 0 <= shared <= batch.max_pages * cache.page_size:
+        raise BmxError(BMX_E_ARG, f"shared={shared}")
+    if out is None:
+        out = _empty(stream, cache.device, _T.bfloat16, T, Hq * 128)
+    else:
+        _paged_args(cache, batch, out)
+        if out.numel() != T * Hq * 128:
+            raise BmxError(BMX_E_SHAPE, f"out must hold {(T, Hq * 128)}, got {tuple(out.shape)}")
+    if T == 0 or batch.n_seqs == 0:
+        return out
+    if workspace is None:
+        workspace = attention_paged_workspace(Hq, cache.n_kv_heads, batch, shared, stream=stream)
+    else:
+        _require_cuda(workspace)
+        _same_device(cache.k, workspace)
+    call("bmx_attention_paged", q.data_ptr(), cache._ref, batch._ref, out.data_ptr(), Hq, 128, shared,
+         1.0 / 128 ** 0.5 if scale is None else scale, workspace.data_ptr(),
+         workspace.numel() * workspace.element_size(), _stream(stream))
+    return out
+
+
+# ---------------------------------------------------------------------------
 # Qwen3 model / KV cache / generation (host mirror of the reference's
 # Qwen3, KvCache, LoadedModel::generate_text and speculative::generate)
 # ---------------------------------------------------------------------------

@@ -1,0 +1,1110 @@
+// Causal GQA attention of a batch's packed queries over a paged KV cache
+// (gfx950).
+//
+//   out[i, h] = softmax(scale q[h, i] k^T) v over rows 0 .. p of the token's
+//   sequence, p its position
+//
+// Of a kv head and a sequence the query rows are r = token * rep + (q head
+// within the kv head's rep), so that any number of heads fills a tile.
+//
+// Two kernels by the rows a sequence can have (max_new * rep):
+//   up to 64 (decode, verified drafts): paged_few_kernel, memory-bound.  The
+//     key blocks of all (sequence, kv head) pairs in a row are cut into equal
+//     shares, one per workgroup, so lengths need not be alike; a pair that
+//     several workgroups share is joined by paged_few_merge_kernel.
+//   more (prompts, chunks, and decode steps beside them): paged_tile_kernel,
+//     compute-bound, by 128-row tiles that paged_plan_kernel lists longest
+//     first and cuts where they are few.
+// Rows common to all sequences (`shared`) are one more "sequence" of all the
+// batch's query rows, taken by the tile kernel before the rest; what it leaves
+// is folded in by the merges.
+//
+// Scores are in base 2: p = 2^(s c - m), c = |scale| log2 e (a negative scale
+// flips q's signs).  The running maximum m follows a row's largest score only
+// once that is 2^8 ahead: sums and outputs are fp32 either way, and the
+// rescaling of the outputs all but vanishes.  p enters the second product in
+// two bf16 pieces (16 bits): with one, outputs were off by 0.0024 of their
+// norm where their own rounding is 0.0017.
+#include <math.h>
+
+#include <algorithm>
+
+#include "paged.h"
+
+namespace bmx {
+namespace {
+
+constexpr int kD = kPagedDim;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLazy = 8.0f;  // log2 by which a maximum may lag
+constexpr float kLeast = 1.17549435e-38f;  // of c: a scale of 0 leaves a hidden key's -inf what it is
+
+typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8_t;
+typedef __attribute__((ext_vector_type(4))) float f32x4_t;
+typedef __attribute__((ext_vector_type(16))) float f32x16_t;
+typedef __attribute__((ext_vector_type(4))) short s16x4_t;
+
+struct PagedAttn {
+  const uint16_t* q;  // [Hq, T, 128]
+  const uint16_t* k;  // [n_pages, Hkv, page_size, 128]
+  const uint16_t* v;
+  uint16_t* out;      // [T, Hq*128]
+  const int* starts;
+  const int* lens;
+  const int* pages;
+  int B, max_pages, T, max_new;
+  int Hq, Hkv, rep, n_pages, shift;
+  int shared;
+  float c2;           // |scale| log2(e)
+  uint32_t flip;      // sign bits of a bf16 pair where scale < 0
+  // ---- workspace ----
+  int* plan;          // few: share, blocks before each sequence; tiles: PlanHead and its lists
+  float* row_o;       // few: [T, Hq, 128] parts that start a pair's blocks
+  float* row_ml;      // [T, Hq, 2]
+  float* wg_o;        // few: [workgroups, rows, 128] parts that continue a pair's; tiles: [slots, Hkv, 128, 128]
+  float* wg_ml;
+  float* pre_o;       // [np, T, Hq, 128] parts over the shared rows
+  float* pre_ml;
+  int np;             // key splits of the shared rows
+  int pre_bps;        // 64-key blocks of such a split
+  int most_items, most_cuts;  // of the plan's lists
+};
+
+// 2^x; maxima of -inf (no key seen) count as 0
+__device__ __forceinline__ float finite_max(float m) { return m == -INFINITY ? 0.0f : m; }
+// The maximum that a partial result is stored with.  -inf tells the merge that
+// nothing was seen; scores that are all NaN leave it there too, with a sum that
+// is NaN, and must not be skipped.
+__device__ __forceinline__ float part_max(float m, float l) { return l == l ? m : 0.0f; }
+
+// The bf16 pairs (-1, 0) and (0, -1) held in registers: as constants in the
+// instruction they came out as other numbers (the products as 0).
+struct MinusOne {
+  uint32_t low, high;
+};
+__device__ __forceinline__ MinusOne minus_one() {
+  MinusOne c{0x0000bf80u, 0xbf800000u};
+  asm volatile("" : "+v"(c.low), "+v"(c.high));
+  return c;
+}
+// Eight probabilities as two bf16 operands, hi + lo
+__device__ __forceinline__ void split8(const float (&p)[8], const MinusOne& one, bf16x8_t& hi, bf16x8_t& lo) {
+  uint32_t h[4], l[4];
+#pragma unroll
+  for (int u = 0; u < 4; u++) {
+    h[u] = static_cast<uint32_t>(f2bf(p[2 * u])) | (static_cast<uint32_t>(f2bf(p[2 * u + 1])) << 16);
+    // p - hi, exact: products with -1 and 0
+    const float a = dot2_bf16(h[u], one.low, p[2 * u]), b = dot2_bf16(h[u], one.high, p[2 * u + 1]);
+    l[u] = static_cast<uint32_t>(f2bf(a)) | (static_cast<uint32_t>(f2bf(b)) << 16);
+  }
+  hi = __builtin_bit_cast(bf16x8_t, make_uint4(h[0], h[1], h[2], h[3]));
+  lo = __builtin_bit_cast(bf16x8_t, make_uint4(l[0], l[1], l[2], l[3]));
+}
+
+// ---- values that are not finite, in rows that only some queries see ----
+// A product over keys would carry 0 x inf of a hidden row into a query.  Where
+// a block holds such a row (rare), its operands get zeros in place of values
+// that are not finite, and what these do to the queries that see them is
+// counted by two more products: of 1 where a query sees a key with 1 where a
+// value is +inf or NaN, and where it is -inf or NaN.
+__device__ __forceinline__ uint32_t not_finite(uint32_t w) {  // bits 15, 31: halves whose exponent is all ones
+  return ((w & 0x7f807f80u) + 0x00800080u) & 0x80008000u;
+}
+__device__ __forceinline__ uint32_t half_mask(uint32_t top) { return (top >> 15) * 0xffffu; }  // bits 15, 31 -> halves
+__device__ __forceinline__ uint32_t finite_part(uint32_t w) { return w & ~half_mask(not_finite(w)); }
+// bf16 1 in halves that are +inf or NaN (sign 0), -inf or NaN (sign 1)
+__device__ __forceinline__ uint32_t ones_where(uint32_t w, int sign) {
+  const uint32_t nf = not_finite(w);
+  const uint32_t nan = nf & (((w & 0x007f007fu) + 0x007f007fu) << 8);  // a mantissa bit: bits 7, 23 of the sum
+  const uint32_t neg = w & 0x80008000u;
+  const uint32_t pick = nf & (nan | (sign ? neg : ~neg));
+  return half_mask(pick) & 0x3f803f80u;
+}
+__device__ __forceinline__ float poison(float o, float plus, float minus) {
+  if (plus > 0.0f) o += INFINITY;
+  if (minus > 0.0f) o -= INFINITY;
+  return o;
+}
+
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
+// ===========================================================================
+// few query rows
+// ===========================================================================
+constexpr int kFewKeys = 128;  // of a block: 32 per wave
+constexpr int kFewOs = kD + 4;  // LDS stride of an output row
+
+// Exclusive prefix over the workgroup's 256 threads, and the total
+__device__ __forceinline__ int scan256(int v, int* tmp, int* total) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int x = v;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int y = __shfl_up(x, o, 64);
+    if (lane >= o) x += y;
+  }
+  if (lane == 63) tmp[wave] = x;
+  __syncthreads();
+  int before = 0, all = 0;
+#pragma unroll
+  for (int w = 0; w < 4; w++) {
+    const int s = tmp[w];
+    if (w < wave) before += s;
+    all += s;
+  }
+  *total = all;
+  return before + x - v;
+}
+
+// Key blocks of a sequence (past the shared rows): 0 where it has no new token
+__device__ __forceinline__ int few_blocks(const PagedAttn& p, const PagedSeq& s) {
+  if (s.tokens == 0) return 0;
+  const int end = min(s.pos + min(s.tokens, p.max_new), p.max_pages << p.shift);
+  return max(end - p.shared + kFewKeys - 1, 0) / kFewKeys;
+}
+
+// A share of the blocks: segments of (sequence, kv head) pairs, heads inner.
+// Per wave and step of 32 keys, in two 16-key tiles:
+//   S^T = K Q^T (v_mfma_f32_16x16x32_bf16): lane l holds query row l % 16 and
+//     keys 4 (l / 16) + i of each tile;
+//   O^T += V^T P^T: the eight keys of a lane's scores are its k slice as they
+//     lie; lane l loads values 8 (l % 16) .. + 7 of just these keys and turns
+//     them by byte permutes, so neither K, V nor P goes through LDS.  Product
+//     j's row l % 16 is value 8 (l % 16) + j: a lane ends with the outputs
+//     32 (l / 16) .. + 31 of its query.
+// The next step's K is requested when this step's scores are done, its V when
+// the values are turned.
+template <int NT>
+__global__ void __launch_bounds__(256, NT == 1 ? 3 : NT == 2 ? 2 : 1) paged_few_kernel(const PagedAttn p) {
+  __shared__ int tmp[4];
+  __shared__ int found[2];
+  __shared__ __align__(16) float os[4][16][kFewOs];
+  __shared__ float ms[4][16 * NT], ls[4][16 * NT];
+  const int tid = threadIdx.x, wave = uniform(tid >> 6), lane = tid & 63, li = lane & 15, g = lane >> 4;
+  const MinusOne one = minus_one();
+  // ---- this workgroup's share: blocks [t0, t1) of all pairs' ----
+  const int per = (p.B + 255) >> 8, b0 = tid * per;
+  int mine = 0;
+  for (int i = 0; i < per && b0 + i < p.B; i++)
+    mine += few_blocks(p, paged_seq(p.starts[b0 + i], p.starts[b0 + i + 1], p.lens[b0 + i], p.T));
+  int all;
+  const int before = scan256(mine, tmp, &all);
+  const int share = max(1, (p.Hkv * all + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x));
+  const int t0 = blockIdx.x * share, t1 = min(t0 + share, p.Hkv * all);
+  if (blockIdx.x == 0 || (t0 < t1 && p.Hkv * before <= t0 && t0 < p.Hkv * (before + mine))) {
+    int at = before;
+    for (int i = 0; i < per && b0 + i < p.B; i++) {
+      const int n = few_blocks(p, paged_seq(p.starts[b0 + i], p.starts[b0 + i + 1], p.lens[b0 + i], p.T));
+      if (blockIdx.x == 0) p.plan[1 + b0 + i] = at;
+      if (p.Hkv * at <= t0 && t0 < p.Hkv * (at + n)) {
+        found[0] = b0 + i;
+        found[1] = at;
+      }
+      at += n;
+    }
+    if (blockIdx.x == 0 && tid == 0) p.plan[0] = share;
+  }
+  __syncthreads();
+  if (t0 >= t1) return;
+  int b = uniform(found[0]);
+  const int rel = t0 - p.Hkv * uniform(found[1]);
+  PagedSeq sq = paged_seq(p.starts[b], p.starts[b + 1], p.lens[b], p.T);
+  int nb = few_blocks(p, sq);
+  if (nb == 0) return;  // (not reached: the scan found blocks here)
+  int h = min(rel / nb, p.Hkv - 1), j = min(rel - h * nb, nb - 1);
+  for (int t = t0; t < t1;) {
+    const int n = min(t1 - t, nb - j);
+    // ---- the segment: blocks j .. j + n - 1 of (b, h) ----
+    const int R = min(sq.tokens, p.max_new) * p.rep;
+    const int cap = p.max_pages << p.shift;
+    const int end = min(sq.pos + min(sq.tokens, p.max_new), cap);  // rows < end are seen by some query
+    const int first = min(sq.pos + 1, cap);                         // rows < first by every query
+    const int* table = p.pages + static_cast<int64_t>(b) * p.max_pages;
+    int lim[NT];   // rows < lim are seen by the lane's query
+    uint4 qf[NT][4];
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++) {
+      const int r = min(16 * nt + li, R - 1), tok = r / p.rep, hd = h * p.rep + r - tok * p.rep;
+      lim[nt] = min(sq.pos + tok + 1, cap);
+      const uint16_t* src = p.q + (static_cast<int64_t>(hd) * p.T + sq.row0 + tok) * kD + 8 * g;
+#pragma unroll
+      for (int ks = 0; ks < 4; ks++) {
+        qf[nt][ks] = *reinterpret_cast<const uint4*>(src + 32 * ks);
+        qf[nt][ks].x ^= p.flip;
+        qf[nt][ks].y ^= p.flip;
+        qf[nt][ks].z ^= p.flip;
+        qf[nt][ks].w ^= p.flip;
+      }
+    }
+    f32x4_t o[NT][8];
+    float m[NT], l[NT];
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++) {
+      m[nt] = -INFINITY;
+      l[nt] = 0.0f;
+#pragma unroll
+      for (int d = 0; d < 8; d++) o[nt][d] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    uint4 kb[2][4], vw[8];
+    int64_t base[2];  // elements to the 16-key tiles' rows; -1: no such page
+    auto locate = [&](int c0) {
+#pragma unroll
+      for (int u = 0; u < 2; u++) {
+        const int key = c0 + 16 * u;
+        base[u] = -1;
+        if (key < end) {
+          const int pg = uniform(table[key >> p.shift]);
+          if (static_cast<unsigned>(pg) < static_cast<unsigned>(p.n_pages))
+            base[u] = (((static_cast<int64_t>(pg) * p.Hkv + h) << p.shift) + (key & ((1 << p.shift) - 1))) * kD;
+        }
+      }
+    };
+    auto load_k = [&]() {
+#pragma unroll
+      for (int u = 0; u < 2; u++) {
+        const uint16_t* src = p.k + max(base[u], static_cast<int64_t>(0)) + li * kD + 8 * g;
+#pragma unroll
+        for (int ks = 0; ks < 4; ks++) kb[u][ks] = *reinterpret_cast<const uint4*>(src + 32 * ks);
+      }
+    };
+    auto load_v = [&]() {
+#pragma unroll
+      for (int e = 0; e < 8; e++)
+        vw[e] = *reinterpret_cast<const uint4*>(p.v + max(base[e >> 2], static_cast<int64_t>(0)) +
+                                                (4 * g + (e & 3)) * kD + 8 * li);
+    };
+    int c0 = p.shared + j * kFewKeys + wave * 32;
+    locate(c0);
+    load_k();
+    load_v();
+    for (int s = 0; s < n; s++, c0 += kFewKeys) {
+      const bool ok0 = base[0] >= 0, ok1 = base[1] >= 0;
+      const bool whole = ok0 && ok1 && c0 + 32 <= first;  // every query sees every key
+      // ---- scores ----
+      f32x4_t sc[NT][2];
+#pragma unroll
+      for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+          sc[nt][u] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+          for (int ks = 0; ks < 4; ks++)
+            sc[nt][u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, kb[u][ks]),
+                                                                __builtin_bit_cast(bf16x8_t, qf[nt][ks]), sc[nt][u], 0,
+                                                                0, 0);
+        }
+      const bool more = s + 1 < n;
+      if (more) {
+        locate(c0 + kFewKeys);
+        load_k();
+      }
+      bf16x8_t hi[NT], lo[NT];
+#pragma unroll
+      for (int nt = 0; nt < NT; nt++) {
+        if (!whole) {
+#pragma unroll
+          for (int u = 0; u < 2; u++)
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+              if (!((u ? ok1 : ok0) && c0 + 16 * u + 4 * g + i < lim[nt])) sc[nt][u][i] = -INFINITY;
+        }
+        float mx = sc[nt][0][0];
+#pragma unroll
+        for (int e = 1; e < 8; e++) mx = fmaxf(mx, sc[nt][e >> 2][e & 3]);
+        mx = max_xor32(max_xor16(mx)) * p.c2;
+        if (__any(mx > m[nt] + kLazy)) {
+          const float m1 = fmaxf(m[nt], mx), alpha = __builtin_amdgcn_exp2f(m[nt] - finite_max(m1));
+          m[nt] = m1;
+          l[nt] *= alpha;
+#pragma unroll
+          for (int d = 0; d < 8; d++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) o[nt][d][i] *= alpha;
+        }
+        const float mu = finite_max(m[nt]);
+        float e8[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+          e8[e] = __builtin_amdgcn_exp2f(fmaf(sc[nt][e >> 2][e & 3], p.c2, -mu));
+          l[nt] += e8[e];
+        }
+        split8(e8, one, hi[nt], lo[nt]);
+      }
+      // ---- rows that no query sees count as zeros ----
+      if (!(ok0 && ok1 && c0 + 32 <= end)) {
+#pragma unroll
+        for (int e = 0; e < 8; e++)
+          if (!((e < 4 ? ok0 : ok1) && c0 + 16 * (e >> 2) + 4 * g + (e & 3) < end)) vw[e] = make_uint4(0, 0, 0, 0);
+      }
+      bool odd = false;  // values that are not finite, in rows that some queries see
+      if (first < end && c0 + 32 > first) {
+        uint32_t nf = 0;
+#pragma unroll
+        for (int e = 0; e < 8; e++) nf |= not_finite(vw[e].x) | not_finite(vw[e].y) | not_finite(vw[e].z) | not_finite(vw[e].w);
+        odd = __any(nf != 0);
+      }
+#pragma unroll
+      for (int d2 = 0; d2 < 4; d2++) {
+        auto word = [&](int e) { return d2 == 0 ? vw[e].x : d2 == 1 ? vw[e].y : d2 == 2 ? vw[e].z : vw[e].w; };
+        uint32_t a[2][4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          a[0][e] = __builtin_amdgcn_perm(word(2 * e + 1), word(2 * e), 0x05040100u);
+          a[1][e] = __builtin_amdgcn_perm(word(2 * e + 1), word(2 * e), 0x07060302u);
+        }
+#pragma unroll
+        for (int z = 0; z < 2; z++) {
+          const int d = 2 * d2 + z;
+          uint4 av = make_uint4(a[z][0], a[z][1], a[z][2], a[z][3]);
+          if (odd) {  // uniform
+            const uint4 plus = make_uint4(ones_where(av.x, 0), ones_where(av.y, 0), ones_where(av.z, 0), ones_where(av.w, 0));
+            const uint4 minus = make_uint4(ones_where(av.x, 1), ones_where(av.y, 1), ones_where(av.z, 1), ones_where(av.w, 1));
+            av = make_uint4(finite_part(av.x), finite_part(av.y), finite_part(av.z), finite_part(av.w));
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++) {
+              uint32_t see[4];
+#pragma unroll
+              for (int e = 0; e < 4; e++) {
+                const int key = c0 + 16 * (e >> 1) + 4 * g + 2 * (e & 1);
+                see[e] = (key < lim[nt] ? 0x3f80u : 0u) | (key + 1 < lim[nt] ? 0x3f800000u : 0u);
+              }
+              const bf16x8_t sv = __builtin_bit_cast(bf16x8_t, make_uint4(see[0], see[1], see[2], see[3]));
+              f32x4_t cp = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f}, cn = cp;
+              cp = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, plus), sv, cp, 0, 0, 0);
+              cn = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, minus), sv, cn, 0, 0, 0);
+#pragma unroll
+              for (int i = 0; i < 4; i++) o[nt][d][i] = poison(o[nt][d][i], cp[i], cn[i]);
+            }
+          }
+          const bf16x8_t vb = __builtin_bit_cast(bf16x8_t, av);
+#pragma unroll
+          for (int nt = 0; nt < NT; nt++) {
+            o[nt][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vb, hi[nt], o[nt][d], 0, 0, 0);
+            o[nt][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vb, lo[nt], o[nt][d], 0, 0, 0);
+          }
+        }
+      }
+      if (more) load_v();
+    }
+    // ---- the four waves' parts joined, 16 rows at a time ----
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++) {
+      const float sum = add_xor32(add_xor16(l[nt]));
+      if (g == 0) {
+        ms[wave][16 * nt + li] = part_max(m[nt], sum);
+        ls[wave][16 * nt + li] = sum;
+      }
+    }
+    const bool direct = n == nb && !p.shared;
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++) {
+      if (16 * nt >= R) break;  // uniform
+      if (nt > 0) __syncthreads();
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        float* dst = &os[wave][li][32 * g + 8 * i];
+        *reinterpret_cast<float4*>(dst) = make_float4(o[nt][0][i], o[nt][1][i], o[nt][2][i], o[nt][3][i]);
+        *reinterpret_cast<float4*>(dst + 4) = make_float4(o[nt][4][i], o[nt][5][i], o[nt][6][i], o[nt][7][i]);
+      }
+      __syncthreads();
+      const int row = tid >> 4, d0 = 8 * (tid & 15), r = 16 * nt + row;
+      if (r < R) {
+        float mm = -INFINITY, ll = 0.0f, a[8] = {};
+#pragma unroll
+        for (int w = 0; w < 4; w++) mm = fmaxf(mm, ms[w][r]);
+#pragma unroll
+        for (int w = 0; w < 4; w++) {
+          const float x = ms[w][r] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ms[w][r] - mm);
+          if (ms[w][r] == -INFINITY) continue;  // (its outputs are zeros)
+          ll += x * ls[w][r];
+#pragma unroll
+          for (int d = 0; d < 8; d++) a[d] += x * os[w][row][d0 + d];
+        }
+        const int tok = r / p.rep, hd = h * p.rep + r - tok * p.rep;
+        const int64_t at = static_cast<int64_t>(sq.row0 + tok) * p.Hq + hd;
+        if (direct) {
+          const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;
+          uint32_t w4[4];
+#pragma unroll
+          for (int d = 0; d < 4; d++)
+            w4[d] = static_cast<uint32_t>(f2bf(a[2 * d] * inv)) | (static_cast<uint32_t>(f2bf(a[2 * d + 1] * inv)) << 16);
+          *reinterpret_cast<uint4*>(p.out + at * kD + d0) = make_uint4(w4[0], w4[1], w4[2], w4[3]);
+        } else {
+          const int64_t slot = j == 0 ? at : static_cast<int64_t>(blockIdx.x) * (16 * NT) + r;
+          float* po = (j == 0 ? p.row_o : p.wg_o) + slot * kD + d0;
+          *reinterpret_cast<float4*>(po) = make_float4(a[0], a[1], a[2], a[3]);
+          *reinterpret_cast<float4*>(po + 4) = make_float4(a[4], a[5], a[6], a[7]);
+          if (d0 == 0) *reinterpret_cast<float2*>((j == 0 ? p.row_ml : p.wg_ml) + slot * 2) = make_float2(part_max(mm, ll), ll);
+        }
+      }
+    }
+    __syncthreads();  // (os, ms and ls are the next segment's)
+    // ---- the next pair ----
+    t += n;
+    j = 0;
+    if (t < t1 && ++h == p.Hkv) {
+      h = 0;
+      do {
+        if (++b == p.B) return;  // (not reached: blocks remain, so a sequence with some does)
+        sq = paged_seq(p.starts[b], p.starts[b + 1], p.lens[b], p.T);
+        nb = few_blocks(p, sq);
+      } while (nb == 0);
+    }
+  }
+}
+
+// A row's parts, folded one after another: 32 lanes per row, 4 values each.
+struct Fold {
+  float m = -INFINITY, l = 0.0f;
+  float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  __device__ __forceinline__ void add(const float2& ml, const float4& v) {
+    if (ml.x == -INFINITY) return;  // nothing seen
+    const float mn = fmaxf(m, ml.x);
+    const float wa = __builtin_amdgcn_exp2f(m - mn), wb = __builtin_amdgcn_exp2f(ml.x - mn);
+    l = l * wa + ml.y * wb;
+    a.x = a.x * wa + v.x * wb;
+    a.y = a.y * wa + v.y * wb;
+    a.z = a.z * wa + v.z * wb;
+    a.w = a.w * wa + v.w * wb;
+    m = mn;
+  }
+  // parts at o + i * ostep, ml + i * mstep (in rows), i < n
+  __device__ __forceinline__ void add_all(const float* o, const float* ml, int64_t step, int n, int d) {
+    constexpr int kB = 8;  // in flight
+    for (int i0 = 0; i0 < n; i0 += kB) {
+      float2 mv[kB];
+      float4 ov[kB];
+#pragma unroll
+      for (int u = 0; u < kB; u++) {
+        const int64_t r = min(i0 + u, n - 1) * step;
+        mv[u] = *reinterpret_cast<const float2*>(ml + r * 2);
+        ov[u] = *reinterpret_cast<const float4*>(o + r * kD + d);
+      }
+#pragma unroll
+      for (int u = 0; u < kB; u++)
+        if (i0 + u < n) add(mv[u], ov[u]);
+    }
+  }
+  __device__ __forceinline__ void store(uint16_t* dst) const {
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    *reinterpret_cast<uint2*>(dst) =
+        make_uint2(static_cast<uint32_t>(f2bf(a.x * inv)) | (static_cast<uint32_t>(f2bf(a.y * inv)) << 16),
+                   static_cast<uint32_t>(f2bf(a.z * inv)) | (static_cast<uint32_t>(f2bf(a.w * inv)) << 16));
+  }
+};
+
+// The rows of (sequence z, kv head y) that paged_few_kernel did not finish:
+// parts over the shared rows, the part that starts the pair's blocks, and one
+// of each further workgroup they go through.
+template <int NT>
+__global__ void __launch_bounds__(256) paged_few_merge_kernel(const PagedAttn p) {
+  const int b = blockIdx.z, h = blockIdx.y, r = blockIdx.x * 8 + (threadIdx.x >> 5), d = 4 * (threadIdx.x & 31);
+  const PagedSeq sq = paged_seq(p.starts[b], p.starts[b + 1], p.lens[b], p.T);
+  if (r >= min(sq.tokens, p.max_new) * p.rep) return;
+  const int nb = few_blocks(p, sq), share = p.plan[0], u0 = p.Hkv * p.plan[1 + b] + h * nb;
+  const int w0 = u0 / share, w1 = (u0 + nb - 1) / share;
+  if (!p.shared && nb > 0 && w0 == w1) return;  // done
+  const int tok = r / p.rep;
+  const int64_t at = static_cast<int64_t>(sq.row0 + tok) * p.Hq + h * p.rep + r - tok * p.rep;
+  Fold f;
+  if (p.shared) f.add_all(p.pre_o + at * kD, p.pre_ml + at * 2, static_cast<int64_t>(p.T) * p.Hq, p.np, d);
+  if (nb > 0) {
+    f.add_all(p.row_o + at * kD, p.row_ml + at * 2, 0, 1, d);
+    const int64_t first = static_cast<int64_t>(w0 + 1) * (16 * NT) + r;
+    if (w1 > w0) f.add_all(p.wg_o + first * kD, p.wg_ml + first * 2, 16 * NT, w1 - w0, d);
+  }
+  f.store(p.out + at * kD + d);
+}
+
+// ===========================================================================
+// many query rows
+// ===========================================================================
+constexpr int kTileRows = 128, kTileKeys = 64;
+constexpr int kTileBytes = kTileKeys * kD * 2;  // of a K or V tile
+// K and V, two of each, and which 16-row quarters of the two blocks exist
+constexpr size_t kTileLds = 4 * kTileBytes + 2 * 4 * sizeof(int);
+
+// A piece of work: rows r0 .. of sequence b, 64-key blocks [j0, j1), and the
+// slot that takes its result (-1: it is the whole of it).
+struct Item {
+  int b, r0, j0, j1, slot, pad[3];
+};
+// Rows r0 .. of sequence b whose keys were cut into n pieces, in slots slot ..
+struct Cut {
+  int b, r0, slot, n;
+};
+struct PlanHead {
+  int items, cuts, pad[2];
+};
+__device__ __forceinline__ Item* plan_items(const PagedAttn& p) { return reinterpret_cast<Item*>(p.plan + 4); }
+__device__ __forceinline__ Cut* plan_cuts(const PagedAttn& p) {
+  return reinterpret_cast<Cut*>(plan_items(p) + p.most_items);
+}
+
+__device__ __align__(256) uint32_t g_zeros[64];  // a row that is read in the place of one that no query sees
+
+// Rows r0 .. r0 + 127 of (sequence, kv head) -- of all the batch's rows, over
+// the shared ones, where PRE -- against 64-key blocks, 32 rows to a wave.
+//   S^T = K Q^T (v_mfma_f32_32x32x16_bf16): lane l holds query row l % 32 and
+//     keys 8 (r / 4) + 4 (l / 32) + r % 4 of its 16 registers r per 32 keys;
+//   O^T += V^T P^T: the eight keys of a step are eight neighbouring score
+//     registers; V^T comes out of LDS by transposed reads (ds_read_b64_tr_b16:
+//     16 lanes read 4 keys x 16 values and each gets one value of the 4 keys).
+// K and V tiles go from memory straight to LDS, a block ahead; a row's 16-byte
+// chunk c lies at c ^ (4 (row % 4) + row / 4 % 4), which keeps both kinds of
+// read off each other's banks.  64 KB of LDS and up to 256 registers: two
+// workgroups share a CU, one's exponentials beside the other's products.
+template <bool PRE>
+__device__ __forceinline__ void tile_run(const PagedAttn& p, char* lds, int b, int h, int r0, int j0, int j1, int slot) {
+  const int tid = threadIdx.x, wave = uniform(tid >> 6), lane = tid & 63, j = lane & 31, hf = lane >> 5;
+  int* exist = reinterpret_cast<int*>(lds + 4 * kTileBytes);  // [2][4]
+  const MinusOne one = minus_one();
+  const int cap = p.max_pages << p.shift;
+  PagedSeq sq{0, p.T, 0};
+  if constexpr (!PRE) sq = paged_seq(p.starts[b], p.starts[b + 1], p.lens[b], p.T);
+  const int tokens = PRE ? p.T : min(sq.tokens, p.max_new);
+  const int R = tokens * p.rep;
+  const int key0 = PRE ? 0 : p.shared;
+  auto limit = [&](int r) {  // rows seen by query row r
+    return PRE ? p.shared : min(sq.pos + r / p.rep + 1, cap);
+  };
+  const int end = limit(min(r0 + kTileRows, R) - 1);             // by some row of the tile
+  const int rw = r0 + 32 * wave;
+  const bool live = rw < R;                                        // (uniform) the wave has rows
+  const int end_w = live ? limit(min(rw + 32, R) - 1) : 0, first_w = live ? limit(rw) : 0;  // by some, by every row of the wave
+  const int rr = min(rw + j, R - 1), tok = rr / p.rep, hd = h * p.rep + rr - tok * p.rep;
+  const int lim = limit(rr);
+  const int* table = p.pages + static_cast<int64_t>(b) * p.max_pages;
+  uint4 qf[8];
+  {
+    const uint16_t* src = p.q + (static_cast<int64_t>(hd) * p.T + sq.row0 + tok) * kD + 8 * hf;
+#pragma unroll
+    for (int ks = 0; ks < 8; ks++) {
+      qf[ks] = *reinterpret_cast<const uint4*>(src + 16 * ks);
+      qf[ks].x ^= p.flip;
+      qf[ks].y ^= p.flip;
+      qf[ks].z ^= p.flip;
+      qf[ks].w ^= p.flip;
+    }
+  }
+  f32x16_t o[4];
+#pragma unroll
+  for (int dt = 0; dt < 4; dt++)
+#pragma unroll
+    for (int r = 0; r < 16; r++) o[dt][r] = 0.0f;
+  float m = -INFINITY, l = 0.0f;
+  // ---- staging: the wave's 16 rows of each tile, 4 rows to an instruction ----
+  const int lrow = lane >> 4;  // row of the four
+  auto stage = [&](int jb, int buf) {
+    const int k0 = key0 + jb * kTileKeys + 16 * wave;
+    int pg = -1;
+    if (k0 < end) pg = uniform(table[k0 >> p.shift]);
+    const bool ok = static_cast<unsigned>(pg) < static_cast<unsigned>(p.n_pages);
+    if (lane == 0) exist[4 * buf + wave] = ok;
+    const int64_t at = ok ? (((static_cast<int64_t>(pg) * p.Hkv + h) << p.shift) + (k0 & ((1 << p.shift) - 1))) * kD : 0;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const int row = 4 * i + lrow;
+      // chunk (lane % 16) of LDS holds the row's chunk ^ swizzle
+      const int ch = (lane & 15) ^ (4 * lrow + i);
+      const bool in = ok && k0 + row < end;
+      const uint16_t* zero = reinterpret_cast<const uint16_t*>(g_zeros) + 8 * (lane & 15);
+      const uint16_t* ks = in ? p.k + at + row * kD + 8 * ch : zero;
+      const uint16_t* vs = in ? p.v + at + row * kD + 8 * ch : zero;
+      const uint32_t dst = lds_offset(lds) + buf * 2 * kTileBytes + (16 * wave + 4 * i) * 256;
+      lds_load16(ks, uniform(dst));
+      lds_load16(vs, uniform(dst + kTileBytes));
+    }
+  };
+  // ---- LDS addresses ----
+  const int swk = 4 * (j & 3) + ((j >> 2) & 3);
+  const char* kat[8];
+#pragma unroll
+  for (int ks = 0; ks < 8; ks++) kat[ks] = lds + j * 256 + (((2 * ks + hf) ^ swk) << 4);
+  const int i16 = lane & 15, grp = (lane >> 4) & 1;
+  const char* vat[2][4];  // [half of the 8 keys][dim tile], of key step 0
+#pragma unroll
+  for (int u = 0; u < 2; u++)
+#pragma unroll
+    for (int dt = 0; dt < 4; dt++) {
+      const int row = 8 * u + 4 * hf + (i16 >> 2);
+      const int ch = (4 * dt + 2 * grp + ((i16 & 3) >> 1)) ^ (4 * (row & 3) + ((row >> 2) & 3));
+      vat[u][dt] = lds + kTileBytes + row * 256 + ch * 16 + 8 * (i16 & 1);
+    }
+  __syncthreads();  // (an earlier piece's reads of LDS are over)
+  if (j0 < j1) stage(j0, 0);
+  for (int jb = j0; jb < j1; jb++) {
+    const int buf = (jb - j0) & 1, bo = buf * 2 * kTileBytes;
+    vm_wait<0>();
+    __syncthreads();
+    if (jb + 1 < j1) stage(jb + 1, buf ^ 1);
+    const int k0 = key0 + jb * kTileKeys;
+    if (k0 >= end_w) continue;  // uniform: hidden from all of the wave's rows
+    // ---- scores ----
+    f32x16_t sc[2];
+#pragma unroll
+    for (int kt = 0; kt < 2; kt++)
+#pragma unroll
+      for (int r = 0; r < 16; r++) sc[kt][r] = 0.0f;
+#pragma unroll
+    for (int ks = 0; ks < 8; ks++)
+#pragma unroll
+      for (int kt = 0; kt < 2; kt++) {
+        const uint4 a = *reinterpret_cast<const uint4*>(kat[ks] + bo + kt * 32 * 256);
+        sc[kt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a),
+                                                         __builtin_bit_cast(bf16x8_t, qf[ks]), sc[kt], 0, 0, 0);
+      }
+    const int4 ex = *reinterpret_cast<const int4*>(exist + 4 * buf);
+    const bool all = uniform(ex.x & ex.y & ex.z & ex.w) != 0;
+    bool odd = false;
+    if (!all || k0 + kTileKeys > first_w) {  // uniform
+      const int e4[4] = {ex.x, ex.y, ex.z, ex.w};
+#pragma unroll
+      for (int kt = 0; kt < 2; kt++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) {
+          const int key = 32 * kt + 8 * (r >> 2) + 4 * hf + (r & 3);
+          const bool see = k0 + key < lim && e4[2 * kt + (r >> 3)];
+          sc[kt][r] = see ? sc[kt][r] : -INFINITY;
+        }
+      uint32_t nf = 0;
+#pragma unroll 4
+      for (int i = 0; i < 16; i++) {
+        const uint4 w = *reinterpret_cast<const uint4*>(lds + bo + kTileBytes + i * 1024 + lane * 16);
+        nf |= not_finite(w.x) | not_finite(w.y) | not_finite(w.z) | not_finite(w.w);
+      }
+      odd = __any(nf != 0);
+    }
+    // ---- softmax ----
+    float mx = sc[0][0];
+#pragma unroll
+    for (int r = 1; r < 32; r++) mx = fmaxf(mx, sc[r >> 4][r & 15]);
+    mx = max_xor32(mx) * p.c2;
+    if (__any(mx > m + kLazy)) {
+      const float m1 = fmaxf(m, mx), alpha = __builtin_amdgcn_exp2f(m - finite_max(m1));
+      m = m1;
+      l *= alpha;
+#pragma unroll
+      for (int dt = 0; dt < 4; dt++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) o[dt][r] *= alpha;
+    }
+    const float mu = finite_max(m);
+    float sum = 0.0f;
+    bf16x8_t hi[4], lo[4];
+#pragma unroll
+    for (int s = 0; s < 4; s++) {
+      float e8[8];
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        e8[e] = __builtin_amdgcn_exp2f(fmaf(sc[s >> 1][8 * (s & 1) + e], p.c2, -mu));
+        sum += e8[e];
+      }
+      split8(e8, one, hi[s], lo[s]);
+    }
+    l += sum;
+    // ---- O^T += V^T P^T ----
+    auto values = [&](int dt, int s) {
+      const s16x4_t a = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+          (__attribute__((address_space(3))) s16x4_t*)(vat[0][dt] + bo + s * 16 * 256));
+      const s16x4_t c = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+          (__attribute__((address_space(3))) s16x4_t*)(vat[1][dt] + bo + s * 16 * 256));
+      const uint2 x = __builtin_bit_cast(uint2, a), y = __builtin_bit_cast(uint2, c);
+      return make_uint4(x.x, x.y, y.x, y.y);
+    };
+    if (odd) {  // uniform
+#pragma unroll 1
+      for (int s = 0; s < 4; s++) {
+        uint32_t see[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          const int key = k0 + 16 * s + 8 * (e >> 1) + 4 * hf + 2 * (e & 1);
+          see[e] = (key < lim ? 0x3f80u : 0u) | (key + 1 < lim ? 0x3f800000u : 0u);
+        }
+        const bf16x8_t sv = __builtin_bit_cast(bf16x8_t, make_uint4(see[0], see[1], see[2], see[3]));
+        const bf16x8_t ph = s == 0 ? hi[0] : s == 1 ? hi[1] : s == 2 ? hi[2] : hi[3];
+        const bf16x8_t pl = s == 0 ? lo[0] : s == 1 ? lo[1] : s == 2 ? lo[2] : lo[3];
+#pragma unroll
+        for (int dt = 0; dt < 4; dt++) {
+          uint4 a = values(dt, s);
+          const uint4 plus = make_uint4(ones_where(a.x, 0), ones_where(a.y, 0), ones_where(a.z, 0), ones_where(a.w, 0));
+          const uint4 minus = make_uint4(ones_where(a.x, 1), ones_where(a.y, 1), ones_where(a.z, 1), ones_where(a.w, 1));
+          f32x16_t c;
+#pragma unroll
+          for (int r = 0; r < 16; r++) c[r] = 0.0f;
+          c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, plus), sv, c, 0, 0, 0);
+#pragma unroll
+          for (int r = 0; r < 16; r++) o[dt][r] = poison(o[dt][r], c[r], 0.0f);
+#pragma unroll
+          for (int r = 0; r < 16; r++) c[r] = 0.0f;
+          c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, minus), sv, c, 0, 0, 0);
+#pragma unroll
+          for (int r = 0; r < 16; r++) o[dt][r] = poison(o[dt][r], 0.0f, c[r]);
+          a = make_uint4(finite_part(a.x), finite_part(a.y), finite_part(a.z), finite_part(a.w));
+          o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a), ph, o[dt], 0, 0, 0);
+          o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a), pl, o[dt], 0, 0, 0);
+        }
+      }
+      continue;
+    }
+#pragma unroll
+    for (int dt = 0; dt < 4; dt++) {
+#pragma unroll
+      for (int s = 0; s < 4; s++) {
+        const bf16x8_t a = __builtin_bit_cast(bf16x8_t, values(dt, s));
+        o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, hi[s], o[dt], 0, 0, 0);
+        o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, lo[s], o[dt], 0, 0, 0);
+      }
+    }
+  }
+  l = add_xor32(l);
+  if (rw + j >= R) return;
+  const int64_t row = static_cast<int64_t>(sq.row0 + tok) * p.Hq + hd;
+  if (slot < 0) {
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    uint16_t* dst = p.out + row * kD + 4 * hf;
+#pragma unroll
+    for (int dt = 0; dt < 4; dt++)
+#pragma unroll
+      for (int r4 = 0; r4 < 4; r4++) {
+        const f32x16_t& a = o[dt];
+        *reinterpret_cast<uint2*>(dst + 32 * dt + 8 * r4) = make_uint2(
+            static_cast<uint32_t>(f2bf(a[4 * r4] * inv)) | (static_cast<uint32_t>(f2bf(a[4 * r4 + 1] * inv)) << 16),
+            static_cast<uint32_t>(f2bf(a[4 * r4 + 2] * inv)) | (static_cast<uint32_t>(f2bf(a[4 * r4 + 3] * inv)) << 16));
+      }
+    return;
+  }
+  const int64_t part = PRE ? static_cast<int64_t>(slot) * p.T * p.Hq + row
+                           : (static_cast<int64_t>(slot) * p.Hkv + h) * kTileRows + 32 * wave + j;
+  if (hf == 0) *reinterpret_cast<float2*>((PRE ? p.pre_ml : p.wg_ml) + part * 2) = make_float2(part_max(m, l), l);
+  float* dst = (PRE ? p.pre_o : p.wg_o) + part * kD + 4 * hf;
+#pragma unroll
+  for (int dt = 0; dt < 4; dt++)
+#pragma unroll
+    for (int r4 = 0; r4 < 4; r4++)
+      *reinterpret_cast<float4*>(dst + 32 * dt + 8 * r4) =
+          make_float4(o[dt][4 * r4], o[dt][4 * r4 + 1], o[dt][4 * r4 + 2], o[dt][4 * r4 + 3]);
+}
+
+// The shared rows: grid (kv heads, row tiles, key splits).
+__global__ void __launch_bounds__(256, 2) paged_prefix_kernel(const PagedAttn p) {
+  extern __shared__ __align__(16) char lds[];
+  const int nb = (p.shared + kTileKeys - 1) / kTileKeys, j0 = blockIdx.z * p.pre_bps;
+  tile_run<true>(p, lds, 0, blockIdx.x, blockIdx.y * kTileRows, j0, min(j0 + p.pre_bps, nb), blockIdx.z);
+}
+
+// The plan's items, longest first: kv head blockIdx % Hkv, items a, 2A-1-a,
+// 2A+a, ... of the A workgroups of a head, so that who had a longer one has a
+// shorter one next.
+__global__ void __launch_bounds__(256, 2) paged_tile_kernel(const PagedAttn p) {
+  extern __shared__ __align__(16) char lds[];
+  const int h = blockIdx.x % p.Hkv, a = blockIdx.x / p.Hkv, A = gridDim.x / p.Hkv;
+  const int items = p.plan[0];
+  for (int r = 0; r * A < items; r++) {
+    const int at = r * A + ((r & 1) ? A - 1 - a : a);
+    if (at >= items) continue;
+    const Item it = plan_items(p)[at];
+    tile_run<false>(p, lds, uniform(it.b), h, uniform(it.r0), uniform(it.j0), uniform(it.j1), uniform(it.slot));
+  }
+}
+
+// One workgroup lists the tiles of all sequences, cut where there are too few
+// to fill the `per_head` workgroups of a kv head.
+constexpr int kPlanThreads = 1024, kPlanBins = 1024;
+__global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const PagedAttn p, int per_head) {
+  __shared__ int tiles_before[kPagedMaxSeqs + 1];
+  __shared__ int bins[kPlanBins];
+  __shared__ int wsum[16], wmax[16], counts[3];  // items, cuts, slots
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  if (tid < 3) counts[tid] = 0;
+  for (int i = tid; i < kPlanBins; i += kPlanThreads) bins[i] = 0;
+  // ---- tiles before each sequence ----
+  const int per = (p.B + kPlanThreads - 1) / kPlanThreads, b0 = tid * per;
+  auto tiles_of = [&](int b) {
+    const PagedSeq s = paged_seq(p.starts[b], p.starts[b + 1], p.lens[b], p.T);
+    return (min(s.tokens, p.max_new) * p.rep + kTileRows - 1) / kTileRows;
+  };
+  int mine = 0;
+  for (int i = 0; i < per && b0 + i < p.B; i++) mine += tiles_of(b0 + i);
+  int x = mine;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int y = __shfl_up(x, o, 64);
+    if (lane >= o) x += y;
+  }
+  if (lane == 63) wsum[wave] = x;
+  __syncthreads();
+  int at = x - mine, n = 0;
+  for (int w = 0; w < 16; w++) {
+    if (w < wave) at += wsum[w];
+    n += wsum[w];
+  }
+  for (int i = 0; i < per && b0 + i < p.B; i++) {
+    tiles_before[b0 + i] = at;
+    at += tiles_of(b0 + i);
+  }
+  if (tid == 0) tiles_before[p.B] = n;
+  __syncthreads();
+  n = min(n, p.most_items - 2 * per_head);  // (starts out of order could count more)
+  // ---- a tile's sequence, first row and blocks ----
+  auto tile = [&](int i, int& b, int& r0) {
+    int lo = 0, hi = p.B;  // the last sequence with tiles_before <= i
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (tiles_before[mid] <= i) lo = mid;
+      else hi = mid;
+    }
+    b = lo;
+    r0 = (i - tiles_before[lo]) * kTileRows;
+    const PagedSeq s = paged_seq(p.starts[b], p.starts[b + 1], p.lens[b], p.T);
+    const int R = min(s.tokens, p.max_new) * p.rep;
+    const int end = min(s.pos + (min(r0 + kTileRows, R) - 1) / p.rep + 1, p.max_pages << p.shift);
+    return max(end - p.shared + kTileKeys - 1, 0) / kTileKeys;
+  };
+  int sum = 0, most = 0;
+  for (int i = tid; i < n; i += kPlanThreads) {
+    int b, r0;
+    const int nb = tile(i, b, r0);
+    sum += nb;
+    most = max(most, nb);
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    sum += __shfl_xor(sum, o, 64);
+    most = max(most, __shfl_xor(most, o, 64));
+  }
+  __syncthreads();
+  if (lane == 0) {
+    wsum[wave] = sum;
+    wmax[wave] = most;
+  }
+  __syncthreads();
+  sum = 0;
+  most = 1;
+  for (int w = 0; w < 16; w++) {
+    sum += wsum[w];
+    most = max(most, wmax[w]);
+  }
+  // ---- pieces of at most `size` blocks: what each workgroup has to do on
+  // average, where that is less than the longest tile ----
+  int size = max((sum + per_head - 1) / per_head, 4);
+  // (tiles longer than that number at most per_head, and so do their further pieces)
+  size = min(size, most);
+  auto pieces = [&](int nb) { return max((nb + size - 1) / size, 1); };
+  const float to_bin = static_cast<float>(kPlanBins - 1) / static_cast<float>(size);
+  auto bin_of = [&](int len) { return kPlanBins - 1 - min(static_cast<int>(len * to_bin), kPlanBins - 1); };
+  for (int i = tid; i < n; i += kPlanThreads) {
+    int b, r0;
+    const int nb = tile(i, b, r0), np = pieces(nb), len = (nb + np - 1) / np;
+    atomicAdd(&bins[bin_of(len)], (nb + max(len, 1) - 1) / max(len, 1) + (nb == 0));
+  }
+  __syncthreads();
+  // exclusive prefix of the bins (one per thread)
+  {
+    const int v = bins[tid];
+    int y = v;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int z = __shfl_up(y, o, 64);
+      if (lane >= o) y += z;
+    }
+    __syncthreads();
+    if (lane == 63) wsum[wave] = y;
+    __syncthreads();
+    int first = y - v;
+    for (int w = 0; w < wave; w++) first += wsum[w];
+    bins[tid] = first;
+  }
+  __syncthreads();
+  Item* items = plan_items(p);
+  Cut* cuts = plan_cuts(p);
+  for (int i = tid; i < n; i += kPlanThreads) {
+    int b, r0;
+    const int nb = tile(i, b, r0), np = pieces(nb), len = (nb + np - 1) / np;
+    const int parts = max((nb + max(len, 1) - 1) / max(len, 1), 1);
+    int slot = -1;
+    if (parts > 1 || p.shared) {
+      slot = atomicAdd(&counts[2], parts);
+      const int c = atomicAdd(&counts[1], 1);
+      if (c < p.most_cuts) cuts[c] = Cut{b, r0, slot, parts};
+    }
+    const int to = atomicAdd(&bins[bin_of(len)], parts);
+    atomicAdd(&counts[0], parts);
+    for (int k = 0; k < parts; k++)
+      if (to + k < p.most_items)
+        items[to + k] = Item{b, r0, k * len, min((k + 1) * len, nb), slot < 0 ? -1 : slot + k, {0, 0, 0}};
+  }
+  __syncthreads();
+  if (tid == 0) {
+    p.plan[0] = min(counts[0], p.most_items);
+    p.plan[1] = min(counts[1], p.most_cuts);
+  }
+}
+
+// The cut tiles' rows: parts over the shared rows, then the pieces'.
+__global__ void __launch_bounds__(256) paged_tile_merge_kernel(const PagedAttn p) {
+  const int n = p.plan[1] * p.Hkv * (kTileRows / 8), d = 4 * (threadIdx.x & 31);
+  for (int w = blockIdx.x; w < n; w += gridDim.x) {
+    const int g = w % (kTileRows / 8), h = w / (kTileRows / 8) % p.Hkv;
+    const Cut c = plan_cuts(p)[w / (kTileRows / 8) / p.Hkv];
+    const PagedSeq sq = paged_seq(p.starts[c.b], p.starts[c.b + 1], p.lens[c.b], p.T);
+    const int k = 8 * g + (threadIdx.x >> 5), r = c.r0 + k;
+    if (r >= min(sq.tokens, p.max_new) * p.rep) continue;
+    const int tok = r / p.rep;
+    const int64_t at = static_cast<int64_t>(sq.row0 + tok) * p.Hq + h * p.rep + r - tok * p.rep;
+    Fold f;
+    if (p.shared) f.add_all(p.pre_o + at * kD, p.pre_ml + at * 2, static_cast<int64_t>(p.T) * p.Hq, p.np, d);
+    const int64_t first = (static_cast<int64_t>(c.slot) * p.Hkv + h) * kTileRows + k;
+    f.add_all(p.wg_o + first * kD, p.wg_ml + first * 2, static_cast<int64_t>(p.Hkv) * kTileRows, c.n, d);
+    f.store(p.out + at * kD + d);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// host
+// ---------------------------------------------------------------------------
+constexpr int kFewRows = 64;       // rows of a (sequence, kv head) pair up to which paged_few_kernel serves
+constexpr int kFewGrid = 768;      // its workgroups: three to a CU
+constexpr int kTileGrid = 512;     // of the tile kernel: two to a CU
+constexpr int kMaxPre = 64;        // key splits of the shared rows
+
+struct PagedPlan {
+  int few, nt;        // few: row tiles of 16
+  int per_head;       // tile workgroups of a kv head
+  int np;             // most key splits of the shared rows
+  int most_items, most_cuts;
+  size_t plan, row_ml, row_o, wg_ml, wg_o, pre_ml, pre_o;  // byte offsets
+  size_t bytes;       // enough for every batch that is no larger
+};
+
+// Where a call's workspace has its parts.  The same offsets would do for any
+// smaller batch only if it took the same kernel, so `bytes` counts the larger of
+// both kernels' needs, each of which grows with the batch.
+PagedPlan make_plan(int Hq, int Hkv, int T, int B, int max_new, bool shared) {
+  PagedPlan a{};
+  const int rep = Hq / Hkv;
+  const size_t rows = static_cast<size_t>(T) * Hq;
+  const int64_t R = static_cast<int64_t>(max_new) * rep;
+  a.few = R <= kFewRows;
+  a.per_head = std::max(1, kTileGrid / Hkv);
+  const int64_t all = (static_cast<int64_t>(T) * rep + kTileRows - 1) / kTileRows;
+  // whole tiles, and as many pieces more as there are workgroups
+  const int64_t tiles = all + std::min(B, T);
+  a.most_items = static_cast<int>(tiles) + 2 * a.per_head;
+  a.most_cuts = static_cast<int>(shared ? tiles : std::min<int64_t>(tiles, 2 * a.per_head));
+  size_t at = 0;
+  auto take = [&](size_t bytes) {
+    const size_t was = at;
+    at += (bytes + 255) & ~static_cast<size_t>(255);
+    return was;
+  };
+  size_t most = 0;
+  auto parts = [&](bool few) {
+    const int64_t r = few ? std::min<int64_t>(R, kFewRows) : R;
+    a.nt = r <= 16 ? 1 : r <= 32 ? 2 : 4;
+    at = 0;
+    a.plan = take(few ? (1 + static_cast<size_t>(B)) * sizeof(int)
+                      : sizeof(PlanHead) + a.most_items * sizeof(Item) + a.most_cuts * sizeof(Cut));
+    const size_t firsts = few ? rows : 0;
+    const size_t others = few ? static_cast<size_t>(kFewGrid) * 16 * a.nt
+                              : static_cast<size_t>(shared ? a.most_items : 2 * a.per_head) * Hkv * kTileRows;
+    a.row_ml = take(firsts * 2 * sizeof(float));
+    a.row_o = take(firsts * kD * sizeof(float));
+    a.wg_ml = take(others * 2 * sizeof(float));
+    a.wg_o = take(others * kD * sizeof(float));
+    most = std::max(most, at);
+  };
+  if (a.few) {
+    parts(true);
+  } else {
+    if (rep <= kFewRows) parts(true);
+    parts(false);
+  }
+  if (shared) {
+    a.np = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(kMaxPre, a.per_head / all)));
+    // (np splits of T rep rows each: at most per_head tiles, or one split of them all)
+    const size_t slots = Hkv * std::min<size_t>(kMaxPre * static_cast<size_t>(T) * rep,
+                                                std::max<size_t>(static_cast<size_t>(a.per_head) * kTileRows,
+                                                                 static_cast<size_t>(T) * rep));
+    at = most;
+    a.pre_ml = take(slots * 2 * sizeof(float));
+    a.pre_o = take(slots * kD * sizeof(float));
+    most = at;
+  }
+  a.bytes = most;
+  return a;
+}
+
+}  // namespace
+}  // namespace bmx
+
+using namespace bmx;
+
+extern "C" size_t bmx_attention_paged_workspace_bytes(int n_heads, int n_kv_heads, int tokens, int n_seqs,
+                                                      int max_new, int shared) {
+  if (n_kv_heads <= 0 || n_kv_heads > 1024 || n_heads <= 0 || n_heads > 65535 || n_heads % n_kv_heads ||
+      tokens <= 0 || n_seqs <= 0 || n_seqs > kPagedMaxSeqs || max_new < 1 || max_new > tokens ||
+      static_cast<int64_t>(tokens) * n_heads > (1 << 28))
+    return 0;
+  return make_plan(n_heads, n_kv_heads, tokens, n_seqs, max_new, shared != 0).bytes;
+}
+
+extern "C" int bmx_attention_paged(const bmx_bf16* q, const bmx_paged_kv* cache, const bmx_batch* batch, bmx_bf16* out,
+                                   int n_heads, int head_dim, int shared, float scale, void* workspace,
+                                   size_t workspace_bytes, void* stream) {
+  if (int rc = check_paged("attention_paged", cache, batch, n_heads, head_dim)) return rc;
+  if (!q || !out || !workspace) return set_error(BMX_E_ARG, "attention_paged: null pointer");
+  const int T = batch->tokens, B = batch->n_seqs, Hkv = cache->n_kv_heads;
+  if (shared < 0 || shared % cache->page_size || shared > batch->max_pages * cache->page_size)
+    return set_error(BMX_E_ARG, "attention_paged: shared=%d must be whole pages of %d, at most %d", shared,
+                     cache->page_size, batch->max_pages);
+  if (!aligned(q, 16) || !aligned(out, 16) || !aligned(workspace, 16))
+    return set_error(BMX_E_ALIGN, "attention_paged: q, out and workspace must be 16-byte aligned");
+  if (T == 0 || B == 0) return BMX_OK;
+  const size_t bytes = static_cast<size_t>(T) * n_heads * kD * sizeof(uint16_t);
+  if (paged_overlap(q, bytes, out, bytes)) return set_error(BMX_E_ARG, "attention_paged: out overlaps q");
+  // (blocks of all pairs are counted in an int)
+  if (static_cast<int64_t>(B) * Hkv * ((static_cast<int64_t>(batch->max_pages) * cache->page_size + 63) / 64) > (1 << 30))
+    return set_error(BMX_E_SHAPE, "attention_paged: %d sequences of up to %d pages, %d kv heads: too many", B,
+                     batch->max_pages, Hkv);
+  const PagedPlan a = make_plan(n_heads, Hkv, T, B, batch->max_new, shared > 0);
+  if (workspace_bytes < a.bytes)
+    return set_error(BMX_E_ARG, "attention_paged: workspace of %zu bytes, %zu needed", workspace_bytes, a.bytes);
+  char* ws = static_cast<char*>(workspace);
+  auto part = [&](size_t off) { return reinterpret_cast<float*>(ws + off); };
+  const int nb = (shared + kTileKeys - 1) / kTileKeys;
+  const int bps = a.np ? (nb + a.np - 1) / a.np : 0, np = bps ? (nb + bps - 1) / bps : 0;
+  PagedAttn p{q, cache->k, cache->v, out, batch->starts, batch->lens, batch->pages, B, batch->max_pages, T,
+                    batch->max_new, n_heads, Hkv, n_heads / Hkv, cache->n_pages, log2_of(cache->page_size), shared,
+                    fabsf(scale) * kLog2e, scale < 0.0f ? 0x80008000u : 0u, reinterpret_cast<int*>(ws + a.plan),
+                    part(a.row_o), part(a.row_ml), part(a.wg_o), part(a.wg_ml), part(a.pre_o), part(a.pre_ml), np, bps,
+                    a.most_items, a.most_cuts};
+  p.c2 = p.c2 < kLeast ? kLeast : p.c2;
+  const hipStream_t st = as_stream(stream);
+  if (shared) {
+    if (int rc = allow_lds(paged_prefix_kernel, kTileLds)) return rc;
+    const int tiles = (T * p.rep + kTileRows - 1) / kTileRows;
+    if (tiles > 65535) return set_error(BMX_E_SHAPE, "attention_paged: tokens=%d too many for shared rows", T);
+    hipLaunchKernelGGL(paged_prefix_kernel, dim3(Hkv, tiles, np), dim3(256), kTileLds, st, p);
+    if (int rc = check_launch("attention_paged shared rows")) return rc;
+  }
+  if (a.few) {
+    const dim3 grid(kFewGrid), merge((batch->max_new * p.rep + 7) / 8, Hkv, B);
+    if (a.nt == 1) {
+      hipLaunchKernelGGL(paged_few_kernel<1>, grid, dim3(256), 0, st, p);
+      hipLaunchKernelGGL(paged_few_merge_kernel<1>, merge, dim3(256), 0, st, p);
+    } else if (a.nt == 2) {
+      hipLaunchKernelGGL(paged_few_kernel<2>, grid, dim3(256), 0, st, p);
+      hipLaunchKernelGGL(paged_few_merge_kernel<2>, merge, dim3(256), 0, st, p);
+    } else {
+      hipLaunchKernelGGL(paged_few_kernel<4>, grid, dim3(256), 0, st, p);
+      hipLaunchKernelGGL(paged_few_merge_kernel<4>, merge, dim3(256), 0, st, p);
+    }
+    return check_launch("attention_paged");
+  }
+  if (int rc = allow_lds(paged_tile_kernel, kTileLds)) return rc;
+  hipLaunchKernelGGL(paged_plan_kernel, dim3(1), dim3(kPlanThreads), 0, st, p, a.per_head);
+  hipLaunchKernelGGL(paged_tile_kernel, dim3(a.per_head * Hkv), dim3(256), kTileLds, st, p);
+  hipLaunchKernelGGL(paged_tile_merge_kernel, dim3(1024), dim3(256), 0, st, p);
+  return check_launch("attention_paged");
+}

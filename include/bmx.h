@@ -374,6 +374,90 @@ int bmx_kv4_evict(const bmx_kv4 *cache, const float *weights, const bmx_kv4 *int
 size_t bmx_kv4_evict_workspace_bytes(int n_kv_heads, int length);
 
 /* ------------------------------------------------------------------ */
+/* A paged KV cache for a batch of sequences                            */
+/* ------------------------------------------------------------------ */
+
+/* One layer's keys and values in pages that sequences take as they grow: k
+ * and v [n_pages, n_kv_heads, page_size, 128] bf16 (16-byte aligned device
+ * pointers; the struct itself is host memory, read during the call).
+ * page_size is a power of two, 16 .. 4096 (BMX_E_UNSUPPORTED).
+ * No counterpart in the reference, whose KvCache holds one sequence
+ * (crates/base-mlx-core/src/model/qwen3.rs:109-162) and whose server runs one
+ * request at a time (crates/base-mlx-server/src/state.rs:1-19). */
+typedef struct {
+  bmx_bf16 *k, *v;
+  int n_pages, n_kv_heads, page_size;
+} bmx_paged_kv;
+
+/* The batch of a step, the same for every layer: `tokens` rows of packed
+ * tokens, of which rows starts[b] .. starts[b+1]-1 are the new tokens of
+ * sequence b.  lens[b] counts the sequence's cached rows with them, so its
+ * token i (from 0) is at position lens[b] - (starts[b+1] - starts[b]) + i of
+ * the text, and position j lies in row j % page_size of page
+ * pages[b * max_pages + j / page_size].  starts [n_seqs + 1] (not descending),
+ * lens [n_seqs] and pages [n_seqs, max_pages] are DEVICE arrays, read when the
+ * work runs, so a captured graph may be replayed with other contents; the
+ * struct is host memory.  A sequence may have no new tokens, and rows from
+ * starts[n_seqs] on belong to none: what a call writes per row stays there as
+ * it was.  max_new: no sequence has more new tokens (1 <= max_new <= tokens;
+ * attention leaves out, unwritten, what a sequence has past its first max_new).
+ * n_seqs <= 4096, max_pages * page_size <= 2^24 (BMX_E_SHAPE).
+ * Whatever the device arrays hold, no call leaves its buffers: a page number
+ * outside 0 .. n_pages-1 and a position outside 0 .. max_pages*page_size-1
+ * mean rows that are neither written nor seen.  Two sequences may share pages
+ * that neither writes in this step. */
+typedef struct {
+  const int32_t *starts, *lens, *pages;
+  int n_seqs, max_pages, tokens, max_new;
+} bmx_batch;
+
+/* QK-norm + RoPE of a batch's packed rows, and their keys and values appended
+ * to the sequences' pages: q [tokens, n_heads*128], k, v [tokens,
+ * n_kv_heads*128] (projection outputs) -> q_out [n_heads, tokens, 128] and the
+ * cache rows of the tokens' positions.  In fp32 from the bf16 inputs to the
+ * one rounding of each result, with the angle position * theta^(-i/64) reduced
+ * in double, so that far positions keep their precision.  (bmx_qk_norm_rope_kv
+ * rounds the norm to bf16 twice on the way, as MLX does, and takes the angle in
+ * fp32: results differ by those roundings.)  All pointers 16-byte aligned;
+ * q_out overlaps none of q, k, v (BMX_E_ARG).  tokens = 0 or n_seqs = 0 is a
+ * no-op.
+ * Replaces: the per-layer sequence of Qwen3::forward_internal q_norm/k_norm ->
+ *   transpose -> fast::rope -> mlx_ext::slice_update
+ *   (crates/base-mlx-core/src/model/qwen3.rs:392-489), for a batch. */
+int bmx_qk_norm_rope_paged(const bmx_bf16 *q, const bmx_bf16 *k, const bmx_bf16 *v, const bmx_bf16 *q_norm,
+                           const bmx_bf16 *k_norm, bmx_bf16 *q_out, const bmx_paged_kv *cache, const bmx_batch *batch,
+                           int n_heads, int head_dim, float eps, float theta, void *stream);
+
+/* Causal GQA attention of a batch's packed queries q [n_heads, tokens, 128]
+ * over their sequences' pages: out [tokens, n_heads*128] =
+ * softmax(scale q k^T) v, a token at position p seeing rows 0 .. p of its
+ * sequence (cached before the call, its own included).  Prompts, chunks of
+ * prompts, verified drafts and single tokens may be one batch.
+ * shared: the first `shared` rows (a multiple of page_size, else BMX_E_ARG; 0:
+ * none) are common to all sequences and lie on the pages that sequence 0's
+ * table names; they are read once for the whole batch.  Every sequence with
+ * new tokens has at least that many rows before them.
+ * A token that sees no row gets zeros.  A row that a query does not see leaves
+ * it alone, whatever it holds; one that it sees with a value that is not
+ * finite makes that dimension of its output not finite.  The order of every sum
+ * is fixed by the shapes and the batch's arrays: equal calls give equal bits.
+ * `workspace` (16-byte aligned device memory of
+ * bmx_attention_paged_workspace_bytes or more, else BMX_E_ARG; any contents):
+ * calls that share one must not run concurrently.  q, out: 16-byte aligned,
+ * without overlap (BMX_E_ARG).  tokens = 0 or n_seqs = 0 is a no-op.
+ * Replaces: mlx_rs::fast::scaled_dot_product_attention as bmx_attention_gqa
+ *   does (crates/base-mlx-core/src/model/qwen3.rs:491-518, 629-653), for a
+ *   batch. */
+int bmx_attention_paged(const bmx_bf16 *q, const bmx_paged_kv *cache, const bmx_batch *batch, bmx_bf16 *out,
+                        int n_heads, int head_dim, int shared, float scale, void *workspace, size_t workspace_bytes,
+                        void *stream);
+/* Bytes of workspace bmx_attention_paged needs for batches of up to `tokens`
+ * rows, n_seqs sequences and max_new new tokens each, with shared rows if
+ * `shared` (0 for arguments it would refuse).  Host only. */
+size_t bmx_attention_paged_workspace_bytes(int n_heads, int n_kv_heads, int tokens, int n_seqs, int max_new,
+                                           int shared);
+
+/* ------------------------------------------------------------------ */
 /* Qwen3 model, KV cache, generation                                   */
 /* ------------------------------------------------------------------ */
 
