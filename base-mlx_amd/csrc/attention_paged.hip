@@ -37,9 +37,13 @@ namespace {
 constexpr int kD = kPagedDim;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLazy = 8.0f;  // log2 by which a maximum may lag
+constexpr float kUp = 7.0f;    // log2 by which fp16 probabilities are scaled up: the largest, with kLazy, are 2^15
 constexpr float kLeast = 1.17549435e-38f;  // of c: a scale of 0 leaves a hidden key's -inf what it is
 
 typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8_t;
+typedef __attribute__((ext_vector_type(8))) _Float16 f16x8_t;
+typedef __attribute__((ext_vector_type(2))) _Float16 f16x2_t;
+typedef __attribute__((ext_vector_type(2))) unsigned short u16x2_t;
 typedef __attribute__((ext_vector_type(4))) float f32x4_t;
 typedef __attribute__((ext_vector_type(16))) float f32x16_t;
 typedef __attribute__((ext_vector_type(4))) short s16x4_t;
@@ -77,6 +81,14 @@ __device__ __forceinline__ float finite_max(float m) { return m == -INFINITY ? 0
 // is NaN, and must not be skipped.
 __device__ __forceinline__ float part_max(float m, float l) { return l == l ? m : 0.0f; }
 
+typedef __attribute__((ext_vector_type(2))) float f32x2_t;
+__device__ __forceinline__ uint32_t pack2h(float lo, float hi) {
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2_t{lo, hi}, f16x2_t));
+}
+// Two bf16 values in a word: one v_cvt_pk_bf16_f32
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2_t{lo, hi}, bf16x2_t));
+}
 // The bf16 pairs (-1, 0) and (0, -1) held in registers: as constants in the
 // instruction they came out as other numbers (the products as 0).
 struct MinusOne {
@@ -92,38 +104,34 @@ __device__ __forceinline__ void split8(const float (&p)[8], const MinusOne& one,
   uint32_t h[4], l[4];
 #pragma unroll
   for (int u = 0; u < 4; u++) {
-    h[u] = static_cast<uint32_t>(f2bf(p[2 * u])) | (static_cast<uint32_t>(f2bf(p[2 * u + 1])) << 16);
+    h[u] = pack2(p[2 * u], p[2 * u + 1]);
     // p - hi, exact: products with -1 and 0
     const float a = dot2_bf16(h[u], one.low, p[2 * u]), b = dot2_bf16(h[u], one.high, p[2 * u + 1]);
-    l[u] = static_cast<uint32_t>(f2bf(a)) | (static_cast<uint32_t>(f2bf(b)) << 16);
+    l[u] = pack2(a, b);
   }
   hi = __builtin_bit_cast(bf16x8_t, make_uint4(h[0], h[1], h[2], h[3]));
   lo = __builtin_bit_cast(bf16x8_t, make_uint4(l[0], l[1], l[2], l[3]));
 }
 
 // ---- values that are not finite, in rows that only some queries see ----
-// A product over keys would carry 0 x inf of a hidden row into a query.  Where
-// a block holds such a row (rare), its operands get zeros in place of values
-// that are not finite, and what these do to the queries that see them is
-// counted by two more products: of 1 where a query sees a key with 1 where a
-// value is +inf or NaN, and where it is -inf or NaN.
+// A product over keys would carry 0 x inf of a hidden row into a query.  So in
+// the blocks that only some queries see whole, values that are not finite enter
+// the product as zeros, and where there were any (rare), the queries that see
+// them get them added at the end.
 __device__ __forceinline__ uint32_t not_finite(uint32_t w) {  // bits 15, 31: halves whose exponent is all ones
   return ((w & 0x7f807f80u) + 0x00800080u) & 0x80008000u;
 }
-__device__ __forceinline__ uint32_t half_mask(uint32_t top) { return (top >> 15) * 0xffffu; }  // bits 15, 31 -> halves
-__device__ __forceinline__ uint32_t finite_part(uint32_t w) { return w & ~half_mask(not_finite(w)); }
-// bf16 1 in halves that are +inf or NaN (sign 0), -inf or NaN (sign 1)
-__device__ __forceinline__ uint32_t ones_where(uint32_t w, int sign) {
-  const uint32_t nf = not_finite(w);
-  const uint32_t nan = nf & (((w & 0x007f007fu) + 0x007f007fu) << 8);  // a mantissa bit: bits 7, 23 of the sum
-  const uint32_t neg = w & 0x80008000u;
-  const uint32_t pick = nf & (nan | (sign ? neg : ~neg));
-  return half_mask(pick) & 0x3f803f80u;
+__device__ __forceinline__ uint32_t finite_part(uint32_t w) { return w & ~((not_finite(w) >> 15) * 0xffffu); }
+// o plus a pair of values where these are not finite
+__device__ __forceinline__ void add_not_finite(float& o0, float& o1, uint32_t w) {
+  if (not_finite(w) & 0x8000u) o0 += bf2f(w & 0xffffu);
+  if (not_finite(w) & 0x80000000u) o1 += bf2f(w >> 16);
 }
-__device__ __forceinline__ float poison(float o, float plus, float minus) {
-  if (plus > 0.0f) o += INFINITY;
-  if (minus > 0.0f) o -= INFINITY;
-  return o;
+// Where row `key` of a sequence's page table lies (in values, of kv head h); -1: nowhere
+__device__ __forceinline__ int64_t row_at(const PagedAttn& p, const int* table, int h, int key) {
+  const int pg = table[key >> p.shift];
+  if (static_cast<unsigned>(pg) >= static_cast<unsigned>(p.n_pages)) return -1;
+  return (((static_cast<int64_t>(pg) * p.Hkv + h) << p.shift) + (key & ((1 << p.shift) - 1))) * kD;
 }
 
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
@@ -273,6 +281,7 @@ __global__ void __launch_bounds__(256, NT == 1 ? 3 : NT == 2 ? 2 : 1) paged_few_
         vw[e] = *reinterpret_cast<const uint4*>(p.v + max(base[e >> 2], static_cast<int64_t>(0)) +
                                                 (4 * g + (e & 3)) * kD + 8 * li);
     };
+    bool odd = false;  // some value that is not finite was left out
     int c0 = p.shared + j * kFewKeys + wave * 32;
     locate(c0);
     load_k();
@@ -336,12 +345,14 @@ __global__ void __launch_bounds__(256, NT == 1 ? 3 : NT == 2 ? 2 : 1) paged_few_
         for (int e = 0; e < 8; e++)
           if (!((e < 4 ? ok0 : ok1) && c0 + 16 * (e >> 2) + 4 * g + (e & 3) < end)) vw[e] = make_uint4(0, 0, 0, 0);
       }
-      bool odd = false;  // values that are not finite, in rows that some queries see
-      if (first < end && c0 + 32 > first) {
+      if (first < end && c0 + 32 > first) {  // (uniform) rows that only some queries see
         uint32_t nf = 0;
 #pragma unroll
-        for (int e = 0; e < 8; e++) nf |= not_finite(vw[e].x) | not_finite(vw[e].y) | not_finite(vw[e].z) | not_finite(vw[e].w);
-        odd = __any(nf != 0);
+        for (int e = 0; e < 8; e++) {
+          nf |= not_finite(vw[e].x) | not_finite(vw[e].y) | not_finite(vw[e].z) | not_finite(vw[e].w);
+          vw[e] = make_uint4(finite_part(vw[e].x), finite_part(vw[e].y), finite_part(vw[e].z), finite_part(vw[e].w));
+        }
+        odd = odd || __any(nf != 0);
       }
 #pragma unroll
       for (int d2 = 0; d2 < 4; d2++) {
@@ -355,27 +366,7 @@ __global__ void __launch_bounds__(256, NT == 1 ? 3 : NT == 2 ? 2 : 1) paged_few_
 #pragma unroll
         for (int z = 0; z < 2; z++) {
           const int d = 2 * d2 + z;
-          uint4 av = make_uint4(a[z][0], a[z][1], a[z][2], a[z][3]);
-          if (odd) {  // uniform
-            const uint4 plus = make_uint4(ones_where(av.x, 0), ones_where(av.y, 0), ones_where(av.z, 0), ones_where(av.w, 0));
-            const uint4 minus = make_uint4(ones_where(av.x, 1), ones_where(av.y, 1), ones_where(av.z, 1), ones_where(av.w, 1));
-            av = make_uint4(finite_part(av.x), finite_part(av.y), finite_part(av.z), finite_part(av.w));
-#pragma unroll
-            for (int nt = 0; nt < NT; nt++) {
-              uint32_t see[4];
-#pragma unroll
-              for (int e = 0; e < 4; e++) {
-                const int key = c0 + 16 * (e >> 1) + 4 * g + 2 * (e & 1);
-                see[e] = (key < lim[nt] ? 0x3f80u : 0u) | (key + 1 < lim[nt] ? 0x3f800000u : 0u);
-              }
-              const bf16x8_t sv = __builtin_bit_cast(bf16x8_t, make_uint4(see[0], see[1], see[2], see[3]));
-              f32x4_t cp = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f}, cn = cp;
-              cp = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, plus), sv, cp, 0, 0, 0);
-              cn = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, minus), sv, cn, 0, 0, 0);
-#pragma unroll
-              for (int i = 0; i < 4; i++) o[nt][d][i] = poison(o[nt][d][i], cp[i], cn[i]);
-            }
-          }
+          const uint4 av = make_uint4(a[z][0], a[z][1], a[z][2], a[z][3]);
           const bf16x8_t vb = __builtin_bit_cast(bf16x8_t, av);
 #pragma unroll
           for (int nt = 0; nt < NT; nt++) {
@@ -385,6 +376,26 @@ __global__ void __launch_bounds__(256, NT == 1 ? 3 : NT == 2 ? 2 : 1) paged_few_
         }
       }
       if (more) load_v();
+    }
+    if (odd) {  // uniform
+      const int k0 = p.shared + j * kFewKeys;
+      for (int key = max(k0, p.shared + ((first - p.shared) & ~31)); key < min(k0 + n * kFewKeys, end); key++) {
+        const int64_t at = row_at(p, table, h, key);
+        if (at < 0) continue;
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+#pragma unroll
+          for (int d = 0; d < 8; d += 2) {
+            const uint32_t w = *reinterpret_cast<const uint32_t*>(p.v + at + 32 * g + 8 * i + d);
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++) {
+              float x = o[nt][d][i], y = o[nt][d + 1][i];
+              if (key < lim[nt]) add_not_finite(x, y, w);
+              o[nt][d][i] = x;
+              o[nt][d + 1][i] = y;
+            }
+          }
+      }
     }
     // ---- the four waves' parts joined, 16 rows at a time ----
 #pragma unroll
@@ -427,7 +438,7 @@ __global__ void __launch_bounds__(256, NT == 1 ? 3 : NT == 2 ? 2 : 1) paged_few_
           uint32_t w4[4];
 #pragma unroll
           for (int d = 0; d < 4; d++)
-            w4[d] = static_cast<uint32_t>(f2bf(a[2 * d] * inv)) | (static_cast<uint32_t>(f2bf(a[2 * d + 1] * inv)) << 16);
+            w4[d] = pack2(a[2 * d] * inv, a[2 * d + 1] * inv);
           *reinterpret_cast<uint4*>(p.out + at * kD + d0) = make_uint4(w4[0], w4[1], w4[2], w4[3]);
         } else {
           const int64_t slot = j == 0 ? at : static_cast<int64_t>(blockIdx.x) * (16 * NT) + r;
@@ -488,8 +499,7 @@ struct Fold {
   __device__ __forceinline__ void store(uint16_t* dst) const {
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     *reinterpret_cast<uint2*>(dst) =
-        make_uint2(static_cast<uint32_t>(f2bf(a.x * inv)) | (static_cast<uint32_t>(f2bf(a.y * inv)) << 16),
-                   static_cast<uint32_t>(f2bf(a.z * inv)) | (static_cast<uint32_t>(f2bf(a.w * inv)) << 16));
+        make_uint2(pack2(a.x * inv, a.y * inv), pack2(a.z * inv, a.w * inv));
   }
 };
 
@@ -521,8 +531,8 @@ __global__ void __launch_bounds__(256) paged_few_merge_kernel(const PagedAttn p)
 // ===========================================================================
 constexpr int kTileRows = 128, kTileKeys = 64;
 constexpr int kTileBytes = kTileKeys * kD * 2;  // of a K or V tile
-// K and V, two of each, and which 16-row quarters of the two blocks exist
-constexpr size_t kTileLds = 4 * kTileBytes + 2 * 4 * sizeof(int);
+// K and V, two of each; which 16-row quarters of the two blocks exist; a flag
+constexpr size_t kTileLds = 4 * kTileBytes + (2 * 4 + 1) * sizeof(int);
 
 // A piece of work: rows r0 .. of sequence b, 64-key blocks [j0, j1), and the
 // slot that takes its result (-1: it is the whole of it).
@@ -541,7 +551,18 @@ __device__ __forceinline__ Cut* plan_cuts(const PagedAttn& p) {
   return reinterpret_cast<Cut*>(plan_items(p) + p.most_items);
 }
 
+// lane l's 16 bytes at base + off go to LDS byte `dst` + 16 l; base and dst are
+// wave-uniform (lds_load16 with the base in scalar registers)
+__device__ __forceinline__ void lds_load16_at(const void* base, uint32_t off, uint32_t dst) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(dst) : "memory");
+}
+
 __device__ __align__(256) uint32_t g_zeros[64];  // a row that is read in the place of one that no query sees
+
+// The order of a loop's instructions: groups of n products, LDS reads, or vector
+// arithmetic (exponentials included) as listed.
+#define SCHED(kind, n) __builtin_amdgcn_sched_group_barrier(kind, n, 0)
+constexpr int kSchedMfma = 0x8, kSchedRead = 0x100, kSchedValu = 0x402;
 
 // Rows r0 .. r0 + 127 of (sequence, kv head) -- of all the batch's rows, over
 // the shared ones, where PRE -- against 64-key blocks, 32 rows to a wave.
@@ -554,10 +575,11 @@ __device__ __align__(256) uint32_t g_zeros[64];  // a row that is read in the pl
 // chunk c lies at c ^ (4 (row % 4) + row / 4 % 4), which keeps both kinds of
 // read off each other's banks.  64 KB of LDS and up to 256 registers: two
 // workgroups share a CU, one's exponentials beside the other's products.
-template <bool PRE>
-__device__ __forceinline__ void tile_run(const PagedAttn& p, char* lds, int b, int h, int r0, int j0, int j1, int slot) {
+template <bool PRE, bool HALF>
+__device__ __forceinline__ bool tile_try(const PagedAttn& p, char* lds, int b, int h, int r0, int j0, int j1, int slot) {
   const int tid = threadIdx.x, wave = uniform(tid >> 6), lane = tid & 63, j = lane & 31, hf = lane >> 5;
   int* exist = reinterpret_cast<int*>(lds + 4 * kTileBytes);  // [2][4]
+  int* left_out = exist + 8;  // some value that is not finite was left out
   const MinusOne one = minus_one();
   const int cap = p.max_pages << p.shift;
   PagedSeq sq{0, p.T, 0};
@@ -568,7 +590,7 @@ __device__ __forceinline__ void tile_run(const PagedAttn& p, char* lds, int b, i
   auto limit = [&](int r) {  // rows seen by query row r
     return PRE ? p.shared : min(sq.pos + r / p.rep + 1, cap);
   };
-  const int end = limit(min(r0 + kTileRows, R) - 1);             // by some row of the tile
+  const int end = limit(min(r0 + kTileRows, R) - 1), first = limit(r0);  // by some, by every row of the tile
   const int rw = r0 + 32 * wave;
   const bool live = rw < R;                                        // (uniform) the wave has rows
   const int end_w = live ? limit(min(rw + 32, R) - 1) : 0, first_w = live ? limit(rw) : 0;  // by some, by every row of the wave
@@ -595,6 +617,10 @@ __device__ __forceinline__ void tile_run(const PagedAttn& p, char* lds, int b, i
   float m = -INFINITY, l = 0.0f;
   // ---- staging: the wave's 16 rows of each tile, 4 rows to an instruction ----
   const int lrow = lane >> 4;  // row of the four
+  // chunk (lane % 16) of LDS holds the row's chunk ^ swizzle
+  uint32_t voff[4];
+#pragma unroll
+  for (int i = 0; i < 4; i++) voff[i] = (4 * i + lrow) * 256 + (((lane & 15) ^ (4 * lrow + i)) << 4);
   auto stage = [&](int jb, int buf) {
     const int k0 = key0 + jb * kTileKeys + 16 * wave;
     int pg = -1;
@@ -602,18 +628,73 @@ __device__ __forceinline__ void tile_run(const PagedAttn& p, char* lds, int b, i
     const bool ok = static_cast<unsigned>(pg) < static_cast<unsigned>(p.n_pages);
     if (lane == 0) exist[4 * buf + wave] = ok;
     const int64_t at = ok ? (((static_cast<int64_t>(pg) * p.Hkv + h) << p.shift) + (k0 & ((1 << p.shift) - 1))) * kD : 0;
+    const uint32_t dst = uniform(lds_offset(lds) + buf * 2 * kTileBytes + wave * 4096);
+    if (ok && k0 + 16 <= end) {  // uniform
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        lds_load16_at(p.k + at, voff[i], dst + 1024 * i);
+        lds_load16_at(p.v + at, voff[i], dst + kTileBytes + 1024 * i);
+      }
+      return;
+    }
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-      const int row = 4 * i + lrow;
-      // chunk (lane % 16) of LDS holds the row's chunk ^ swizzle
-      const int ch = (lane & 15) ^ (4 * lrow + i);
-      const bool in = ok && k0 + row < end;
-      const uint16_t* zero = reinterpret_cast<const uint16_t*>(g_zeros) + 8 * (lane & 15);
-      const uint16_t* ks = in ? p.k + at + row * kD + 8 * ch : zero;
-      const uint16_t* vs = in ? p.v + at + row * kD + 8 * ch : zero;
-      const uint32_t dst = lds_offset(lds) + buf * 2 * kTileBytes + (16 * wave + 4 * i) * 256;
-      lds_load16(ks, uniform(dst));
-      lds_load16(vs, uniform(dst + kTileBytes));
+      const bool in = ok && k0 + 4 * i + lrow < end;
+      const char* zero = reinterpret_cast<const char*>(g_zeros) + 16 * (lane & 15);
+      lds_load16(in ? reinterpret_cast<const char*>(p.k + at) + voff[i] : zero, dst + 1024 * i);
+      lds_load16(in ? reinterpret_cast<const char*>(p.v + at) + voff[i] : zero, dst + kTileBytes + 1024 * i);
+    }
+  };
+  // ... and what is done to the wave's 16 rows of V once they are there: values
+  // to fp16 where that loses nothing (quarter 1), else left as bf16 (quarter 2);
+  // in blocks that only some queries see whole, values that are not finite to 0
+  auto settle = [&](int jb, int buf) {
+    const int k0 = key0 + jb * kTileKeys;
+    const bool mixed = !PRE && k0 + kTileKeys > first && first < end;  // (uniform)
+    if (!HALF && !mixed) return;
+    char* at = lds + buf * 2 * kTileBytes + kTileBytes + wave * 4096 + lane * 16;
+    uint4 w[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) w[i] = *reinterpret_cast<const uint4*>(at + i * 1024);
+    bool changed = false;
+    if (mixed) {
+      uint32_t nf = 0;
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        nf |= not_finite(w[i].x) | not_finite(w[i].y) | not_finite(w[i].z) | not_finite(w[i].w);
+        w[i] = make_uint4(finite_part(w[i].x), finite_part(w[i].y), finite_part(w[i].z), finite_part(w[i].w));
+      }
+      changed = __any(nf != 0);
+      if (changed && lane == 0) *left_out = 1;
+    }
+    if constexpr (HALF) {
+      // of the lane's 8 values of a row the largest magnitude, as bits: 0, or
+      // from 2^-12 to below 2^16
+      uint32_t top = 0, low = ~0u;
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        auto mag = [](uint32_t x) { return __builtin_bit_cast(u16x2_t, x & 0x7fff7fffu); };
+        const u16x2_t a = __builtin_elementwise_max(__builtin_elementwise_max(mag(w[i].x), mag(w[i].y)),
+                                                    __builtin_elementwise_max(mag(w[i].z), mag(w[i].w)));
+        const uint32_t t = max(static_cast<uint32_t>(a.x), static_cast<uint32_t>(a.y));
+        top = max(top, t);
+        low = min(low, t - 1u);  // (0 wraps to the largest)
+      }
+      if (__any(top >= 0x4780u || low < 0x3980u - 1u)) {
+        if (lane == 0) exist[4 * buf + wave] = 2;
+        return;
+      }
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        auto h2 = [](uint32_t x) {
+          return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(__uint_as_float(x << 16),
+                                                                         __uint_as_float(x & 0xffff0000u)));
+        };
+        *reinterpret_cast<uint4*>(at + i * 1024) = make_uint4(h2(w[i].x), h2(w[i].y), h2(w[i].z), h2(w[i].w));
+      }
+    } else if (changed) {
+#pragma unroll
+      for (int i = 0; i < 4; i++) *reinterpret_cast<uint4*>(at + i * 1024) = w[i];
     }
   };
   // ---- LDS addresses ----
@@ -631,15 +712,7 @@ __device__ __forceinline__ void tile_run(const PagedAttn& p, char* lds, int b, i
       const int ch = (4 * dt + 2 * grp + ((i16 & 3) >> 1)) ^ (4 * (row & 3) + ((row >> 2) & 3));
       vat[u][dt] = lds + kTileBytes + row * 256 + ch * 16 + 8 * (i16 & 1);
     }
-  __syncthreads();  // (an earlier piece's reads of LDS are over)
-  if (j0 < j1) stage(j0, 0);
-  for (int jb = j0; jb < j1; jb++) {
-    const int buf = (jb - j0) & 1, bo = buf * 2 * kTileBytes;
-    vm_wait<0>();
-    __syncthreads();
-    if (jb + 1 < j1) stage(jb + 1, buf ^ 1);
-    const int k0 = key0 + jb * kTileKeys;
-    if (k0 >= end_w) continue;  // uniform: hidden from all of the wave's rows
+  auto block = [&](int bo, int k0, const int4& ex, bool all) {
     // ---- scores ----
     f32x16_t sc[2];
 #pragma unroll
@@ -654,9 +727,14 @@ __device__ __forceinline__ void tile_run(const PagedAttn& p, char* lds, int b, i
         sc[kt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a),
                                                          __builtin_bit_cast(bf16x8_t, qf[ks]), sc[kt], 0, 0, 0);
       }
-    const int4 ex = *reinterpret_cast<const int4*>(exist + 4 * buf);
-    const bool all = uniform(ex.x & ex.y & ex.z & ex.w) != 0;
-    bool odd = false;
+    // (reads of K two steps ahead of the products that take them)
+    SCHED(kSchedRead, 4);
+#pragma unroll
+    for (int i = 0; i < 6; i++) {
+      SCHED(kSchedMfma, 2);
+      SCHED(kSchedRead, 2);
+    }
+    SCHED(kSchedMfma, 4);
     if (!all || k0 + kTileKeys > first_w) {  // uniform
       const int e4[4] = {ex.x, ex.y, ex.z, ex.w};
 #pragma unroll
@@ -667,13 +745,6 @@ __device__ __forceinline__ void tile_run(const PagedAttn& p, char* lds, int b, i
           const bool see = k0 + key < lim && e4[2 * kt + (r >> 3)];
           sc[kt][r] = see ? sc[kt][r] : -INFINITY;
         }
-      uint32_t nf = 0;
-#pragma unroll 4
-      for (int i = 0; i < 16; i++) {
-        const uint4 w = *reinterpret_cast<const uint4*>(lds + bo + kTileBytes + i * 1024 + lane * 16);
-        nf |= not_finite(w.x) | not_finite(w.y) | not_finite(w.z) | not_finite(w.w);
-      }
-      odd = __any(nf != 0);
     }
     // ---- softmax ----
     float mx = sc[0][0];
@@ -689,21 +760,8 @@ __device__ __forceinline__ void tile_run(const PagedAttn& p, char* lds, int b, i
 #pragma unroll
         for (int r = 0; r < 16; r++) o[dt][r] *= alpha;
     }
-    const float mu = finite_max(m);
-    float sum = 0.0f;
-    bf16x8_t hi[4], lo[4];
-#pragma unroll
-    for (int s = 0; s < 4; s++) {
-      float e8[8];
-#pragma unroll
-      for (int e = 0; e < 8; e++) {
-        e8[e] = __builtin_amdgcn_exp2f(fmaf(sc[s >> 1][8 * (s & 1) + e], p.c2, -mu));
-        sum += e8[e];
-      }
-      split8(e8, one, hi[s], lo[s]);
-    }
-    l += sum;
-    // ---- O^T += V^T P^T ----
+    // ---- O^T += V^T P^T, 16 keys a step; a step's exponentials beside the
+    // products of the one before ----
     auto values = [&](int dt, int s) {
       const s16x4_t a = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
           (__attribute__((address_space(3))) s16x4_t*)(vat[0][dt] + bo + s * 16 * 256));
@@ -712,53 +770,134 @@ __device__ __forceinline__ void tile_run(const PagedAttn& p, char* lds, int b, i
       const uint2 x = __builtin_bit_cast(uint2, a), y = __builtin_bit_cast(uint2, c);
       return make_uint4(x.x, x.y, y.x, y.y);
     };
-    if (odd) {  // uniform
-#pragma unroll 1
-      for (int s = 0; s < 4; s++) {
-        uint32_t see[4];
+    const float mu = finite_max(m) - (HALF ? kUp : 0.0f);
+    float sum = 0.0f;
+    auto weigh = [&](int s, float (&e8)[8]) {
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-          const int key = k0 + 16 * s + 8 * (e >> 1) + 4 * hf + 2 * (e & 1);
-          see[e] = (key < lim ? 0x3f80u : 0u) | (key + 1 < lim ? 0x3f800000u : 0u);
-        }
-        const bf16x8_t sv = __builtin_bit_cast(bf16x8_t, make_uint4(see[0], see[1], see[2], see[3]));
-        const bf16x8_t ph = s == 0 ? hi[0] : s == 1 ? hi[1] : s == 2 ? hi[2] : hi[3];
-        const bf16x8_t pl = s == 0 ? lo[0] : s == 1 ? lo[1] : s == 2 ? lo[2] : lo[3];
-#pragma unroll
-        for (int dt = 0; dt < 4; dt++) {
-          uint4 a = values(dt, s);
-          const uint4 plus = make_uint4(ones_where(a.x, 0), ones_where(a.y, 0), ones_where(a.z, 0), ones_where(a.w, 0));
-          const uint4 minus = make_uint4(ones_where(a.x, 1), ones_where(a.y, 1), ones_where(a.z, 1), ones_where(a.w, 1));
-          f32x16_t c;
-#pragma unroll
-          for (int r = 0; r < 16; r++) c[r] = 0.0f;
-          c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, plus), sv, c, 0, 0, 0);
-#pragma unroll
-          for (int r = 0; r < 16; r++) o[dt][r] = poison(o[dt][r], c[r], 0.0f);
-#pragma unroll
-          for (int r = 0; r < 16; r++) c[r] = 0.0f;
-          c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, minus), sv, c, 0, 0, 0);
-#pragma unroll
-          for (int r = 0; r < 16; r++) o[dt][r] = poison(o[dt][r], 0.0f, c[r]);
-          a = make_uint4(finite_part(a.x), finite_part(a.y), finite_part(a.z), finite_part(a.w));
-          o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a), ph, o[dt], 0, 0, 0);
-          o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a), pl, o[dt], 0, 0, 0);
-        }
+      for (int e = 0; e < 8; e++) {
+        e8[e] = __builtin_amdgcn_exp2f(fmaf(sc[s >> 1][8 * (s & 1) + e], p.c2, -mu));
+        sum += e8[e];
       }
-      continue;
+    };
+    if constexpr (HALF) {
+      auto weigh16 = [&](int s) {
+        float e8[8];
+        weigh(s, e8);
+        return __builtin_bit_cast(f16x8_t, make_uint4(pack2h(e8[0], e8[1]), pack2h(e8[2], e8[3]), pack2h(e8[4], e8[5]),
+                                                      pack2h(e8[6], e8[7])));
+      };
+      uint4 va[4];
+#pragma unroll
+      for (int dt = 0; dt < 4; dt++) va[dt] = values(dt, 0);
+      f16x8_t pw = weigh16(0);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int s = 0; s < 4; s++) {
+        const f16x8_t w = pw;
+        uint4 vc[4];
+#pragma unroll
+        for (int dt = 0; dt < 4; dt++) vc[dt] = va[dt];
+        if (s < 3) {
+#pragma unroll
+          for (int dt = 0; dt < 4; dt++) va[dt] = values(dt, s + 1);
+          pw = weigh16(s + 1);
+        }
+#pragma unroll
+        for (int dt = 0; dt < 4; dt++)
+          o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, vc[dt]), w, o[dt], 0, 0, 0);
+        if (s < 3) {
+          SCHED(kSchedRead, 8);
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            SCHED(kSchedMfma, 1);
+            SCHED(kSchedValu, 7);
+          }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    } else {
+      uint4 va[4];
+#pragma unroll
+      for (int dt = 0; dt < 4; dt++) va[dt] = values(dt, 0);
+      bf16x8_t hi, lo;
+      auto weigh2 = [&](int s) {
+        float e8[8];
+        weigh(s, e8);
+        split8(e8, one, hi, lo);
+      };
+      weigh2(0);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int s = 0; s < 4; s++) {
+        const bf16x8_t h1 = hi, h2 = lo;
+        uint4 vc[4];
+#pragma unroll
+        for (int dt = 0; dt < 4; dt++) vc[dt] = va[dt];
+        if (s < 3) {
+#pragma unroll
+          for (int dt = 0; dt < 4; dt++) va[dt] = values(dt, s + 1);
+          weigh2(s + 1);
+        }
+#pragma unroll
+        for (int dt = 0; dt < 4; dt++)
+          o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, vc[dt]), h1, o[dt], 0, 0, 0);
+#pragma unroll
+        for (int dt = 0; dt < 4; dt++)
+          o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, vc[dt]), h2, o[dt], 0, 0, 0);
+        if (s < 3) {
+          SCHED(kSchedRead, 8);
+#pragma unroll
+          for (int i = 0; i < 8; i++) {
+            SCHED(kSchedMfma, 1);
+            SCHED(kSchedValu, 6);
+          }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
     }
-#pragma unroll
-    for (int dt = 0; dt < 4; dt++) {
-#pragma unroll
-      for (int s = 0; s < 4; s++) {
-        const bf16x8_t a = __builtin_bit_cast(bf16x8_t, values(dt, s));
-        o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, hi[s], o[dt], 0, 0, 0);
-        o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, lo[s], o[dt], 0, 0, 0);
-      }
+    l += sum;
+  };
+  __syncthreads();  // (an earlier piece's reads of LDS are over)
+  if (tid == 0) *left_out = 0;
+  if (j0 < j1) {
+    stage(j0, 0);
+    vm_wait<0>();
+    settle(j0, 0);
+  }
+  for (int jb = j0; jb < j1; jb++) {
+    const int buf = (jb - j0) & 1, bo = buf * 2 * kTileBytes;
+    __syncthreads();
+    const int4 ex = *reinterpret_cast<const int4*>(exist + 4 * buf);
+    const bool all = uniform(min(min(ex.x, ex.y), min(ex.z, ex.w))) != 0;
+    if (HALF && uniform(max(max(ex.x, ex.y), max(ex.z, ex.w))) > 1) return false;  // (in every wave)
+    if (jb + 1 < j1) stage(jb + 1, buf ^ 1);
+    const int k0 = key0 + jb * kTileKeys;
+    // (uniform: a block hidden from all of the wave's rows is only settled)
+    if (k0 < end_w) block(bo, k0, ex, all);
+    if (jb + 1 < j1) {
+      vm_wait<0>();
+      settle(jb + 1, buf ^ 1);
     }
   }
   l = add_xor32(l);
-  if (rw + j >= R) return;
+  if constexpr (!PRE) {
+    if (j0 < j1 && uniform(*left_out)) {  // (the last block's barriers lie behind)
+      for (int key = key0 + max(j0 * kTileKeys, (first - key0) & ~(kTileKeys - 1)); key < min(key0 + j1 * kTileKeys, end); key++) {
+        const int64_t at = row_at(p, table, h, key);
+        if (at < 0 || key >= lim) continue;
+#pragma unroll
+        for (int dt = 0; dt < 4; dt++)
+#pragma unroll
+          for (int r = 0; r < 16; r += 2) {
+            float x = o[dt][r], y = o[dt][r + 1];
+            add_not_finite(x, y, *reinterpret_cast<const uint32_t*>(p.v + at + 32 * dt + 8 * (r >> 2) + 4 * hf + (r & 3)));
+            o[dt][r] = x;
+            o[dt][r + 1] = y;
+          }
+      }
+    }
+  }
+  auto finish = [&]() {
   const int64_t row = static_cast<int64_t>(sq.row0 + tok) * p.Hq + hd;
   if (slot < 0) {
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
@@ -768,15 +907,14 @@ __device__ __forceinline__ void tile_run(const PagedAttn& p, char* lds, int b, i
 #pragma unroll
       for (int r4 = 0; r4 < 4; r4++) {
         const f32x16_t& a = o[dt];
-        *reinterpret_cast<uint2*>(dst + 32 * dt + 8 * r4) = make_uint2(
-            static_cast<uint32_t>(f2bf(a[4 * r4] * inv)) | (static_cast<uint32_t>(f2bf(a[4 * r4 + 1] * inv)) << 16),
-            static_cast<uint32_t>(f2bf(a[4 * r4 + 2] * inv)) | (static_cast<uint32_t>(f2bf(a[4 * r4 + 3] * inv)) << 16));
+        *reinterpret_cast<uint2*>(dst + 32 * dt + 8 * r4) =
+            make_uint2(pack2(a[4 * r4] * inv, a[4 * r4 + 1] * inv), pack2(a[4 * r4 + 2] * inv, a[4 * r4 + 3] * inv));
       }
     return;
   }
   const int64_t part = PRE ? static_cast<int64_t>(slot) * p.T * p.Hq + row
                            : (static_cast<int64_t>(slot) * p.Hkv + h) * kTileRows + 32 * wave + j;
-  if (hf == 0) *reinterpret_cast<float2*>((PRE ? p.pre_ml : p.wg_ml) + part * 2) = make_float2(part_max(m, l), l);
+  if (hf == 0) *reinterpret_cast<float2*>((PRE ? p.pre_ml : p.wg_ml) + part * 2) = make_float2(part_max(m, l) - (HALF ? kUp : 0.0f), l);
   float* dst = (PRE ? p.pre_o : p.wg_o) + part * kD + 4 * hf;
 #pragma unroll
   for (int dt = 0; dt < 4; dt++)
@@ -784,6 +922,14 @@ __device__ __forceinline__ void tile_run(const PagedAttn& p, char* lds, int b, i
     for (int r4 = 0; r4 < 4; r4++)
       *reinterpret_cast<float4*>(dst + 32 * dt + 8 * r4) =
           make_float4(o[dt][4 * r4], o[dt][4 * r4 + 1], o[dt][4 * r4 + 2], o[dt][4 * r4 + 3]);
+  };
+  if (rw + j < R) finish();
+  return true;
+}
+template <bool PRE>
+__device__ __forceinline__ void tile_run(const PagedAttn& p, char* lds, int b, int h, int r0, int j0, int j1, int slot) {
+  if (!uniform(tile_try<PRE, true>(p, lds, b, h, r0, j0, j1, slot)))
+    tile_try<PRE, false>(p, lds, b, h, r0, j0, j1, slot);
 }
 
 // The shared rows: grid (kv heads, row tiles, key splits).
