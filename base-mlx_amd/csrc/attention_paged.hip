@@ -47,6 +47,7 @@ typedef __attribute__((ext_vector_type(2))) unsigned short u16x2_t;
 typedef __attribute__((ext_vector_type(4))) float f32x4_t;
 typedef __attribute__((ext_vector_type(16))) float f32x16_t;
 typedef __attribute__((ext_vector_type(4))) short s16x4_t;
+typedef __attribute__((ext_vector_type(4))) unsigned u32x4_t;
 
 struct PagedAttn {
   const uint16_t* q;  // [Hq, T, 128]
@@ -142,7 +143,7 @@ __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirs
 constexpr int kFewKeys = 128;  // of a block: 32 per wave
 constexpr int kFewOs = kD + 4;  // LDS stride of an output row
 
-// Exclusive prefix over the workgroup's 256 threads, and the total
+// Exclusive prefix over 256 threads (further ones hold the same again), and the total
 __device__ __forceinline__ int scan256(int v, int* tmp, int* total) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   int x = v;
@@ -157,7 +158,7 @@ __device__ __forceinline__ int scan256(int v, int* tmp, int* total) {
 #pragma unroll
   for (int w = 0; w < 4; w++) {
     const int s = tmp[w];
-    if (w < wave) before += s;
+    if (w < (wave & 3)) before += s;
     all += s;
   }
   *total = all;
@@ -182,19 +183,25 @@ __device__ __forceinline__ int few_blocks(const PagedAttn& p, const PagedSeq& s)
 //     32 (l / 16) .. + 31 of its query.
 // The next step's K is requested when this step's scores are done, its V when
 // the values are turned.
-template <int NT>
-__global__ void __launch_bounds__(256, NT == 1 ? 3 : NT == 2 ? 2 : 1) paged_few_kernel(const PagedAttn p) {
-  __shared__ int tmp[4];
-  __shared__ int found[2];
+// RG groups of 4 waves take 16 NT rows each over the same keys (64 rows by one
+// group needed more than 256 registers a wave: 36 us for 16 sequences of 5
+// tokens, against @@).
+template <int NT, int RG>
+__global__ void __launch_bounds__(256 * RG, 2) paged_few_kernel(const PagedAttn p) {
+  __shared__ int tmp[8];
+  __shared__ int found[5];
   __shared__ __align__(16) float os[4][16][kFewOs];
-  __shared__ float ms[4][16 * NT], ls[4][16 * NT];
-  const int tid = threadIdx.x, wave = uniform(tid >> 6), lane = tid & 63, li = lane & 15, g = lane >> 4;
+  __shared__ float ms[4][16 * NT * RG], ls[4][16 * NT * RG];
+  const int tid = threadIdx.x, wave = uniform(tid >> 6) & 3, rg = uniform(tid >> 8), lane = tid & 63, li = lane & 15, g = lane >> 4;
   const MinusOne one = minus_one();
   // ---- this workgroup's share: blocks [t0, t1) of all pairs' ----
-  const int per = (p.B + 255) >> 8, b0 = tid * per;
+  const int per = (p.B + 255) >> 8, b0 = (tid & 255) * per;
   int mine = 0;
-  for (int i = 0; i < per && b0 + i < p.B; i++)
-    mine += few_blocks(p, paged_seq(p.starts[b0 + i], p.starts[b0 + i + 1], p.lens[b0 + i], p.T));
+  PagedSeq only{0, 0, 0};
+  for (int i = 0; i < per && b0 + i < p.B; i++) {
+    only = paged_seq(p.starts[b0 + i], p.starts[b0 + i + 1], p.lens[b0 + i], p.T);
+    mine += few_blocks(p, only);
+  }
   int all;
   const int before = scan256(mine, tmp, &all);
   const int share = max(1, (p.Hkv * all + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x));
@@ -202,11 +209,15 @@ __global__ void __launch_bounds__(256, NT == 1 ? 3 : NT == 2 ? 2 : 1) paged_few_
   if (blockIdx.x == 0 || (t0 < t1 && p.Hkv * before <= t0 && t0 < p.Hkv * (before + mine))) {
     int at = before;
     for (int i = 0; i < per && b0 + i < p.B; i++) {
-      const int n = few_blocks(p, paged_seq(p.starts[b0 + i], p.starts[b0 + i + 1], p.lens[b0 + i], p.T));
+      const PagedSeq s = per == 1 ? only : paged_seq(p.starts[b0 + i], p.starts[b0 + i + 1], p.lens[b0 + i], p.T);
+      const int n = few_blocks(p, s);
       if (blockIdx.x == 0) p.plan[1 + b0 + i] = at;
       if (p.Hkv * at <= t0 && t0 < p.Hkv * (at + n)) {
         found[0] = b0 + i;
         found[1] = at;
+        found[2] = s.row0;
+        found[3] = s.tokens;
+        found[4] = s.pos;
       }
       at += n;
     }
@@ -216,7 +227,7 @@ __global__ void __launch_bounds__(256, NT == 1 ? 3 : NT == 2 ? 2 : 1) paged_few_
   if (t0 >= t1) return;
   int b = uniform(found[0]);
   const int rel = t0 - p.Hkv * uniform(found[1]);
-  PagedSeq sq = paged_seq(p.starts[b], p.starts[b + 1], p.lens[b], p.T);
+  PagedSeq sq{uniform(found[2]), uniform(found[3]), uniform(found[4])};
   int nb = few_blocks(p, sq);
   if (nb == 0) return;  // (not reached: the scan found blocks here)
   int h = min(rel / nb, p.Hkv - 1), j = min(rel - h * nb, nb - 1);
@@ -232,7 +243,7 @@ __global__ void __launch_bounds__(256, NT == 1 ? 3 : NT == 2 ? 2 : 1) paged_few_
     uint4 qf[NT][4];
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
-      const int r = min(16 * nt + li, R - 1), tok = r / p.rep, hd = h * p.rep + r - tok * p.rep;
+      const int r = min(16 * (NT * rg + nt) + li, R - 1), tok = r / p.rep, hd = h * p.rep + r - tok * p.rep;
       lim[nt] = min(sq.pos + tok + 1, cap);
       const uint16_t* src = p.q + (static_cast<int64_t>(hd) * p.T + sq.row0 + tok) * kD + 8 * g;
 #pragma unroll
@@ -255,16 +266,19 @@ __global__ void __launch_bounds__(256, NT == 1 ? 3 : NT == 2 ? 2 : 1) paged_few_
     }
     uint4 kb[2][4], vw[8];
     int64_t base[2];  // elements to the 16-key tiles' rows; -1: no such page
+    // page numbers are asked for a step before the rows they lead to
+    int pg[2];
+    auto ask = [&](int c0) {
+#pragma unroll
+      for (int u = 0; u < 2; u++) pg[u] = c0 + 16 * u < end ? table[(c0 + 16 * u) >> p.shift] : -1;
+    };
     auto locate = [&](int c0) {
 #pragma unroll
       for (int u = 0; u < 2; u++) {
-        const int key = c0 + 16 * u;
-        base[u] = -1;
-        if (key < end) {
-          const int pg = uniform(table[key >> p.shift]);
-          if (static_cast<unsigned>(pg) < static_cast<unsigned>(p.n_pages))
-            base[u] = (((static_cast<int64_t>(pg) * p.Hkv + h) << p.shift) + (key & ((1 << p.shift) - 1))) * kD;
-        }
+        const int at = uniform(pg[u]), key = c0 + 16 * u;
+        base[u] = static_cast<unsigned>(at) < static_cast<unsigned>(p.n_pages)
+                      ? (((static_cast<int64_t>(at) * p.Hkv + h) << p.shift) + (key & ((1 << p.shift) - 1))) * kD
+                      : -1;
       }
     };
     auto load_k = [&]() {
@@ -283,7 +297,9 @@ __global__ void __launch_bounds__(256, NT == 1 ? 3 : NT == 2 ? 2 : 1) paged_few_
     };
     bool odd = false;  // some value that is not finite was left out
     int c0 = p.shared + j * kFewKeys + wave * 32;
+    ask(c0);
     locate(c0);
+    ask(c0 + kFewKeys);
     load_k();
     load_v();
     for (int s = 0; s < n; s++, c0 += kFewKeys) {
@@ -306,6 +322,7 @@ __global__ void __launch_bounds__(256, NT == 1 ? 3 : NT == 2 ? 2 : 1) paged_few_
       if (more) {
         locate(c0 + kFewKeys);
         load_k();
+        ask(c0 + 2 * kFewKeys);
       }
       bf16x8_t hi[NT], lo[NT];
 #pragma unroll
@@ -397,54 +414,58 @@ __global__ void __launch_bounds__(256, NT == 1 ? 3 : NT == 2 ? 2 : 1) paged_few_
           }
       }
     }
-    // ---- the four waves' parts joined, 16 rows at a time ----
+    // ---- the parts of four waves joined, 16 rows at a time ----
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
       const float sum = add_xor32(add_xor16(l[nt]));
       if (g == 0) {
-        ms[wave][16 * nt + li] = part_max(m[nt], sum);
-        ls[wave][16 * nt + li] = sum;
+        ms[wave][16 * (NT * rg + nt) + li] = part_max(m[nt], sum);
+        ls[wave][16 * (NT * rg + nt) + li] = sum;
       }
     }
     const bool direct = n == nb && !p.shared;
 #pragma unroll
-    for (int nt = 0; nt < NT; nt++) {
-      if (16 * nt >= R) break;  // uniform
-      if (nt > 0) __syncthreads();
+    for (int pass = 0; pass < NT * RG; pass++) {
+      if (16 * pass >= R) break;  // uniform
+      if (pass > 0) __syncthreads();
+      if (rg == pass / NT) {
+        constexpr int kN = NT;
+        const int nt = pass % kN;
 #pragma unroll
-      for (int i = 0; i < 4; i++) {
-        float* dst = &os[wave][li][32 * g + 8 * i];
-        *reinterpret_cast<float4*>(dst) = make_float4(o[nt][0][i], o[nt][1][i], o[nt][2][i], o[nt][3][i]);
-        *reinterpret_cast<float4*>(dst + 4) = make_float4(o[nt][4][i], o[nt][5][i], o[nt][6][i], o[nt][7][i]);
+        for (int i = 0; i < 4; i++) {
+          float* dst = &os[wave][li][32 * g + 8 * i];
+          *reinterpret_cast<float4*>(dst) = make_float4(o[nt][0][i], o[nt][1][i], o[nt][2][i], o[nt][3][i]);
+          *reinterpret_cast<float4*>(dst + 4) = make_float4(o[nt][4][i], o[nt][5][i], o[nt][6][i], o[nt][7][i]);
+        }
       }
       __syncthreads();
-      const int row = tid >> 4, d0 = 8 * (tid & 15), r = 16 * nt + row;
+      constexpr int kE = 8 / RG, kPer = kD / kE;  // values of a thread, threads of a row
+      const int row = tid / kPer, d0 = kE * (tid % kPer), r = 16 * pass + row;
       if (r < R) {
-        float mm = -INFINITY, ll = 0.0f, a[8] = {};
+        float mm = -INFINITY, ll = 0.0f, a[kE] = {};
 #pragma unroll
         for (int w = 0; w < 4; w++) mm = fmaxf(mm, ms[w][r]);
 #pragma unroll
         for (int w = 0; w < 4; w++) {
-          const float x = ms[w][r] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ms[w][r] - mm);
           if (ms[w][r] == -INFINITY) continue;  // (its outputs are zeros)
+          const float x = __builtin_amdgcn_exp2f(ms[w][r] - mm);
           ll += x * ls[w][r];
 #pragma unroll
-          for (int d = 0; d < 8; d++) a[d] += x * os[w][row][d0 + d];
+          for (int d = 0; d < kE; d++) a[d] += x * os[w][row][d0 + d];
         }
         const int tok = r / p.rep, hd = h * p.rep + r - tok * p.rep;
         const int64_t at = static_cast<int64_t>(sq.row0 + tok) * p.Hq + hd;
         if (direct) {
           const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;
-          uint32_t w4[4];
 #pragma unroll
-          for (int d = 0; d < 4; d++)
-            w4[d] = pack2(a[2 * d] * inv, a[2 * d + 1] * inv);
-          *reinterpret_cast<uint4*>(p.out + at * kD + d0) = make_uint4(w4[0], w4[1], w4[2], w4[3]);
+          for (int d = 0; d < kE; d += 4)
+            *reinterpret_cast<uint2*>(p.out + at * kD + d0 + d) =
+                make_uint2(pack2(a[d] * inv, a[d + 1] * inv), pack2(a[d + 2] * inv, a[d + 3] * inv));
         } else {
-          const int64_t slot = j == 0 ? at : static_cast<int64_t>(blockIdx.x) * (16 * NT) + r;
+          const int64_t slot = j == 0 ? at : static_cast<int64_t>(blockIdx.x) * (16 * NT * RG) + r;
           float* po = (j == 0 ? p.row_o : p.wg_o) + slot * kD + d0;
-          *reinterpret_cast<float4*>(po) = make_float4(a[0], a[1], a[2], a[3]);
-          *reinterpret_cast<float4*>(po + 4) = make_float4(a[4], a[5], a[6], a[7]);
+#pragma unroll
+          for (int d = 0; d < kE; d += 4) *reinterpret_cast<float4*>(po + d) = make_float4(a[d], a[d + 1], a[d + 2], a[d + 3]);
           if (d0 == 0) *reinterpret_cast<float2*>((j == 0 ? p.row_ml : p.wg_ml) + slot * 2) = make_float2(part_max(mm, ll), ll);
         }
       }
@@ -479,21 +500,21 @@ struct Fold {
     a.w = a.w * wa + v.w * wb;
     m = mn;
   }
-  // parts at o + i * ostep, ml + i * mstep (in rows), i < n
-  __device__ __forceinline__ void add_all(const float* o, const float* ml, int64_t step, int n, int d) {
+  // parts i0, i0 + by, ... < n, `step` rows apart, lane's values from d on
+  __device__ __forceinline__ void add_all(const float* o, const float* ml, int64_t step, int i0, int by, int n, int d) {
     constexpr int kB = 8;  // in flight
-    for (int i0 = 0; i0 < n; i0 += kB) {
+    for (; i0 < n; i0 += kB * by) {
       float2 mv[kB];
       float4 ov[kB];
 #pragma unroll
       for (int u = 0; u < kB; u++) {
-        const int64_t r = min(i0 + u, n - 1) * step;
+        const int64_t r = min(i0 + u * by, n - 1) * step;
         mv[u] = *reinterpret_cast<const float2*>(ml + r * 2);
         ov[u] = *reinterpret_cast<const float4*>(o + r * kD + d);
       }
 #pragma unroll
       for (int u = 0; u < kB; u++)
-        if (i0 + u < n) add(mv[u], ov[u]);
+        if (i0 + u * by < n) add(mv[u], ov[u]);
     }
   }
   __device__ __forceinline__ void store(uint16_t* dst) const {
@@ -505,10 +526,15 @@ struct Fold {
 
 // The rows of (sequence z, kv head y) that paged_few_kernel did not finish:
 // parts over the shared rows, the part that starts the pair's blocks, and one
-// of each further workgroup they go through.
-template <int NT>
+// of each further workgroup they go through.  8 rows to a workgroup, or (WIDE)
+// one, whose parts its eight 32-lane groups share out: the 32 rows of one
+// sequence of 4097, 32 parts each, take 5.2 us instead of 7.4.
+template <int NT, bool WIDE>
 __global__ void __launch_bounds__(256) paged_few_merge_kernel(const PagedAttn p) {
-  const int b = blockIdx.z, h = blockIdx.y, r = blockIdx.x * 8 + (threadIdx.x >> 5), d = 4 * (threadIdx.x & 31);
+  __shared__ __align__(16) float4 as[8][32];
+  __shared__ float2 mls[8];
+  const int b = blockIdx.z, h = blockIdx.y, sub = threadIdx.x >> 5, ln = threadIdx.x & 31, d = 4 * ln;
+  const int r = WIDE ? blockIdx.x : blockIdx.x * 8 + sub;
   const PagedSeq sq = paged_seq(p.starts[b], p.starts[b + 1], p.lens[b], p.T);
   if (r >= min(sq.tokens, p.max_new) * p.rep) return;
   const int nb = few_blocks(p, sq), share = p.plan[0], u0 = p.Hkv * p.plan[1 + b] + h * nb;
@@ -516,12 +542,22 @@ __global__ void __launch_bounds__(256) paged_few_merge_kernel(const PagedAttn p)
   if (!p.shared && nb > 0 && w0 == w1) return;  // done
   const int tok = r / p.rep;
   const int64_t at = static_cast<int64_t>(sq.row0 + tok) * p.Hq + h * p.rep + r - tok * p.rep;
+  const int i0 = WIDE ? sub : 0, by = WIDE ? 8 : 1;
   Fold f;
-  if (p.shared) f.add_all(p.pre_o + at * kD, p.pre_ml + at * 2, static_cast<int64_t>(p.T) * p.Hq, p.np, d);
+  if (p.shared) f.add_all(p.pre_o + at * kD, p.pre_ml + at * 2, static_cast<int64_t>(p.T) * p.Hq, i0, by, p.np, d);
   if (nb > 0) {
-    f.add_all(p.row_o + at * kD, p.row_ml + at * 2, 0, 1, d);
+    if (i0 == 0) f.add(*reinterpret_cast<const float2*>(p.row_ml + at * 2), *reinterpret_cast<const float4*>(p.row_o + at * kD + d));
     const int64_t first = static_cast<int64_t>(w0 + 1) * (16 * NT) + r;
-    if (w1 > w0) f.add_all(p.wg_o + first * kD, p.wg_ml + first * 2, 16 * NT, w1 - w0, d);
+    if (w1 > w0) f.add_all(p.wg_o + first * kD, p.wg_ml + first * 2, 16 * NT, i0, by, w1 - w0, d);
+  }
+  if constexpr (WIDE) {
+    as[sub][ln] = f.a;
+    if (ln == 0) mls[sub] = make_float2(part_max(f.m, f.l), f.l);
+    __syncthreads();
+    if (sub != 0) return;
+    f = Fold();
+#pragma unroll
+    for (int u = 0; u < 8; u++) f.add(mls[u], as[u][ln]);
   }
   f.store(p.out + at * kD + d);
 }
@@ -551,6 +587,10 @@ __device__ __forceinline__ Cut* plan_cuts(const PagedAttn& p) {
   return reinterpret_cast<Cut*>(plan_items(p) + p.most_items);
 }
 
+template <class T>
+__device__ __forceinline__ __attribute__((address_space(3))) T* lds_ptr(uint32_t off) {
+  return reinterpret_cast<__attribute__((address_space(3))) T*>(off);
+}
 // lane l's 16 bytes at base + off go to LDS byte `dst` + 16 l; base and dst are
 // wave-uniform (lds_load16 with the base in scalar registers)
 __device__ __forceinline__ void lds_load16_at(const void* base, uint32_t off, uint32_t dst) {
@@ -558,6 +598,14 @@ __device__ __forceinline__ void lds_load16_at(const void* base, uint32_t off, ui
 }
 
 __device__ __align__(256) uint32_t g_zeros[64];  // a row that is read in the place of one that no query sees
+
+// Where a tile's rows go: to `out`, or as partial results, at the rows' places
+// [T, Hq] or at the tile's own.
+struct Result {
+  float* o;
+  float* ml;
+  bool by_row;
+};
 
 // The order of a loop's instructions: groups of n products, LDS reads, or vector
 // arithmetic (exponentials included) as listed.
@@ -575,9 +623,11 @@ constexpr int kSchedMfma = 0x8, kSchedRead = 0x100, kSchedValu = 0x402;
 // chunk c lies at c ^ (4 (row % 4) + row / 4 % 4), which keeps both kinds of
 // read off each other's banks.  64 KB of LDS and up to 256 registers: two
 // workgroups share a CU, one's exponentials beside the other's products.
-template <bool PRE, bool HALF>
-__device__ __forceinline__ bool tile_try(const PagedAttn& p, char* lds, int b, int h, int r0, int j0, int j1, int slot) {
+template <bool PRE, bool HALF, int WK>
+__device__ __forceinline__ bool tile_try(const PagedAttn& p, char* lds, int b, int h, int r0, int j0, int j1, const Result& to) {
+  constexpr int WR = 4 / WK, NK = 2 / WK;  // row groups of waves; 32-key tiles of a wave
   const int tid = threadIdx.x, wave = uniform(tid >> 6), lane = tid & 63, j = lane & 31, hf = lane >> 5;
+  const int wr = wave % WR, wk = wave / WR;
   int* exist = reinterpret_cast<int*>(lds + 4 * kTileBytes);  // [2][4]
   int* left_out = exist + 8;  // some value that is not finite was left out
   const MinusOne one = minus_one();
@@ -590,8 +640,8 @@ __device__ __forceinline__ bool tile_try(const PagedAttn& p, char* lds, int b, i
   auto limit = [&](int r) {  // rows seen by query row r
     return PRE ? p.shared : min(sq.pos + r / p.rep + 1, cap);
   };
-  const int end = limit(min(r0 + kTileRows, R) - 1), first = limit(r0);  // by some, by every row of the tile
-  const int rw = r0 + 32 * wave;
+  const int end = limit(min(r0 + 32 * WR, R) - 1), first = limit(r0);  // by some, by every row of the tile
+  const int rw = r0 + 32 * wr;
   const bool live = rw < R;                                        // (uniform) the wave has rows
   const int end_w = live ? limit(min(rw + 32, R) - 1) : 0, first_w = live ? limit(rw) : 0;  // by some, by every row of the wave
   const int rr = min(rw + j, R - 1), tok = rr / p.rep, hd = h * p.rep + rr - tok * p.rep;
@@ -618,17 +668,24 @@ __device__ __forceinline__ bool tile_try(const PagedAttn& p, char* lds, int b, i
   // ---- staging: the wave's 16 rows of each tile, 4 rows to an instruction ----
   const int lrow = lane >> 4;  // row of the four
   // chunk (lane % 16) of LDS holds the row's chunk ^ swizzle
-  uint32_t voff[4];
-#pragma unroll
-  for (int i = 0; i < 4; i++) voff[i] = (4 * i + lrow) * 256 + (((lane & 15) ^ (4 * lrow + i)) << 4);
+  const uint32_t voff0 = lrow * 256 + (((lane & 15) ^ (4 * lrow)) << 4);
+  // (the page is asked for a block before its rows)
+  int asked = -1;
+  auto ask = [&](int jb) {
+    const int k0 = key0 + jb * kTileKeys + 16 * wave;
+    asked = k0 < end ? table[k0 >> p.shift] : -1;
+  };
   auto stage = [&](int jb, int buf) {
     const int k0 = key0 + jb * kTileKeys + 16 * wave;
-    int pg = -1;
-    if (k0 < end) pg = uniform(table[k0 >> p.shift]);
+    const int pg = uniform(asked);
+    ask(jb + 1);
     const bool ok = static_cast<unsigned>(pg) < static_cast<unsigned>(p.n_pages);
     if (lane == 0) exist[4 * buf + wave] = ok;
     const int64_t at = ok ? (((static_cast<int64_t>(pg) * p.Hkv + h) << p.shift) + (k0 & ((1 << p.shift) - 1))) * kD : 0;
     const uint32_t dst = uniform(lds_offset(lds) + buf * 2 * kTileBytes + wave * 4096);
+    uint32_t v0 = voff0;
+    asm volatile("" : "+v"(v0));
+    const uint32_t voff[4] = {v0, v0 ^ (1024 | 16), v0 ^ (2048 | 32), v0 ^ (3072 | 48)};  // + 4 i rows
     if (ok && k0 + 16 <= end) {  // uniform
 #pragma unroll
       for (int i = 0; i < 4; i++) {
@@ -697,59 +754,58 @@ __device__ __forceinline__ bool tile_try(const PagedAttn& p, char* lds, int b, i
       for (int i = 0; i < 4; i++) *reinterpret_cast<uint4*>(at + i * 1024) = w[i];
     }
   };
-  // ---- LDS addresses ----
+  // ---- LDS addresses: of a row's chunk, the others' follow by exclusive or
+  // (made anew in every block: 16 registers otherwise) ----
   const int swk = 4 * (j & 3) + ((j >> 2) & 3);
-  const char* kat[8];
-#pragma unroll
-  for (int ks = 0; ks < 8; ks++) kat[ks] = lds + j * 256 + (((2 * ks + hf) ^ swk) << 4);
+  const uint32_t kat0 = lds_offset(lds) + wk * NK * 32 * 256 + j * 256 + ((hf ^ swk) << 4);
   const int i16 = lane & 15, grp = (lane >> 4) & 1;
-  const char* vat[2][4];  // [half of the 8 keys][dim tile], of key step 0
+  uint32_t vat0[2];  // [half of the 8 keys], of key step 0 and dim tile 0
 #pragma unroll
-  for (int u = 0; u < 2; u++)
-#pragma unroll
-    for (int dt = 0; dt < 4; dt++) {
-      const int row = 8 * u + 4 * hf + (i16 >> 2);
-      const int ch = (4 * dt + 2 * grp + ((i16 & 3) >> 1)) ^ (4 * (row & 3) + ((row >> 2) & 3));
-      vat[u][dt] = lds + kTileBytes + row * 256 + ch * 16 + 8 * (i16 & 1);
-    }
+  for (int u = 0; u < 2; u++) {
+    const int row = 8 * u + 4 * hf + (i16 >> 2);
+    const int ch = (2 * grp + ((i16 & 3) >> 1)) ^ (4 * (row & 3) + ((row >> 2) & 3));
+    vat0[u] = lds_offset(lds) + kTileBytes + wk * NK * 32 * 256 + row * 256 + ch * 16 + 8 * (i16 & 1);
+  }
   auto block = [&](int bo, int k0, const int4& ex, bool all) {
+    uint32_t kat = kat0 + bo, vat[2] = {vat0[0] + bo, vat0[1] + bo};
+    asm volatile("" : "+v"(kat), "+v"(vat[0]), "+v"(vat[1]));
     // ---- scores ----
-    f32x16_t sc[2];
+    f32x16_t sc[NK];
 #pragma unroll
-    for (int kt = 0; kt < 2; kt++)
+    for (int kt = 0; kt < NK; kt++)
 #pragma unroll
       for (int r = 0; r < 16; r++) sc[kt][r] = 0.0f;
 #pragma unroll
     for (int ks = 0; ks < 8; ks++)
 #pragma unroll
-      for (int kt = 0; kt < 2; kt++) {
-        const uint4 a = *reinterpret_cast<const uint4*>(kat[ks] + bo + kt * 32 * 256);
+      for (int kt = 0; kt < NK; kt++) {
+        const u32x4_t a = *lds_ptr<u32x4_t>((kat ^ (ks << 5)) + kt * 32 * 256);
         sc[kt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a),
                                                          __builtin_bit_cast(bf16x8_t, qf[ks]), sc[kt], 0, 0, 0);
       }
     // (reads of K two steps ahead of the products that take them)
-    SCHED(kSchedRead, 4);
+    SCHED(kSchedRead, 2 * NK);
 #pragma unroll
     for (int i = 0; i < 6; i++) {
-      SCHED(kSchedMfma, 2);
-      SCHED(kSchedRead, 2);
+      SCHED(kSchedMfma, NK);
+      SCHED(kSchedRead, NK);
     }
-    SCHED(kSchedMfma, 4);
-    if (!all || k0 + kTileKeys > first_w) {  // uniform
+    SCHED(kSchedMfma, 2 * NK);
+    if (!all || k0 + 32 * NK > first_w) {  // uniform
       const int e4[4] = {ex.x, ex.y, ex.z, ex.w};
 #pragma unroll
-      for (int kt = 0; kt < 2; kt++)
+      for (int kt = 0; kt < NK; kt++)
 #pragma unroll
         for (int r = 0; r < 16; r++) {
           const int key = 32 * kt + 8 * (r >> 2) + 4 * hf + (r & 3);
-          const bool see = k0 + key < lim && e4[2 * kt + (r >> 3)];
+          const bool see = k0 + key < lim && (WK == 1 || wk == 0 ? e4[2 * kt + (r >> 3)] : e4[2 + (r >> 3)]);
           sc[kt][r] = see ? sc[kt][r] : -INFINITY;
         }
     }
     // ---- softmax ----
     float mx = sc[0][0];
 #pragma unroll
-    for (int r = 1; r < 32; r++) mx = fmaxf(mx, sc[r >> 4][r & 15]);
+    for (int r = 1; r < 16 * NK; r++) mx = fmaxf(mx, sc[r >> 4][r & 15]);
     mx = max_xor32(mx) * p.c2;
     if (__any(mx > m + kLazy)) {
       const float m1 = fmaxf(m, mx), alpha = __builtin_amdgcn_exp2f(m - finite_max(m1));
@@ -763,10 +819,8 @@ __device__ __forceinline__ bool tile_try(const PagedAttn& p, char* lds, int b, i
     // ---- O^T += V^T P^T, 16 keys a step; a step's exponentials beside the
     // products of the one before ----
     auto values = [&](int dt, int s) {
-      const s16x4_t a = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-          (__attribute__((address_space(3))) s16x4_t*)(vat[0][dt] + bo + s * 16 * 256));
-      const s16x4_t c = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-          (__attribute__((address_space(3))) s16x4_t*)(vat[1][dt] + bo + s * 16 * 256));
+      const s16x4_t a = __builtin_amdgcn_ds_read_tr16_b64_v4i16(lds_ptr<s16x4_t>((vat[0] ^ (dt << 6)) + s * 16 * 256));
+      const s16x4_t c = __builtin_amdgcn_ds_read_tr16_b64_v4i16(lds_ptr<s16x4_t>((vat[1] ^ (dt << 6)) + s * 16 * 256));
       const uint2 x = __builtin_bit_cast(uint2, a), y = __builtin_bit_cast(uint2, c);
       return make_uint4(x.x, x.y, y.x, y.y);
     };
@@ -792,12 +846,12 @@ __device__ __forceinline__ bool tile_try(const PagedAttn& p, char* lds, int b, i
       f16x8_t pw = weigh16(0);
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int s = 0; s < 4; s++) {
+      for (int s = 0; s < 2 * NK; s++) {
         const f16x8_t w = pw;
         uint4 vc[4];
 #pragma unroll
         for (int dt = 0; dt < 4; dt++) vc[dt] = va[dt];
-        if (s < 3) {
+        if (s < 2 * NK - 1) {
 #pragma unroll
           for (int dt = 0; dt < 4; dt++) va[dt] = values(dt, s + 1);
           pw = weigh16(s + 1);
@@ -805,7 +859,7 @@ __device__ __forceinline__ bool tile_try(const PagedAttn& p, char* lds, int b, i
 #pragma unroll
         for (int dt = 0; dt < 4; dt++)
           o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, vc[dt]), w, o[dt], 0, 0, 0);
-        if (s < 3) {
+        if (s < 2 * NK - 1) {
           SCHED(kSchedRead, 8);
 #pragma unroll
           for (int i = 0; i < 4; i++) {
@@ -828,12 +882,12 @@ __device__ __forceinline__ bool tile_try(const PagedAttn& p, char* lds, int b, i
       weigh2(0);
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int s = 0; s < 4; s++) {
+      for (int s = 0; s < 2 * NK; s++) {
         const bf16x8_t h1 = hi, h2 = lo;
         uint4 vc[4];
 #pragma unroll
         for (int dt = 0; dt < 4; dt++) vc[dt] = va[dt];
-        if (s < 3) {
+        if (s < 2 * NK - 1) {
 #pragma unroll
           for (int dt = 0; dt < 4; dt++) va[dt] = values(dt, s + 1);
           weigh2(s + 1);
@@ -844,7 +898,7 @@ __device__ __forceinline__ bool tile_try(const PagedAttn& p, char* lds, int b, i
 #pragma unroll
         for (int dt = 0; dt < 4; dt++)
           o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, vc[dt]), h2, o[dt], 0, 0, 0);
-        if (s < 3) {
+        if (s < 2 * NK - 1) {
           SCHED(kSchedRead, 8);
 #pragma unroll
           for (int i = 0; i < 8; i++) {
@@ -860,6 +914,7 @@ __device__ __forceinline__ bool tile_try(const PagedAttn& p, char* lds, int b, i
   __syncthreads();  // (an earlier piece's reads of LDS are over)
   if (tid == 0) *left_out = 0;
   if (j0 < j1) {
+    ask(j0);
     stage(j0, 0);
     vm_wait<0>();
     settle(j0, 0);
@@ -871,8 +926,8 @@ __device__ __forceinline__ bool tile_try(const PagedAttn& p, char* lds, int b, i
     const bool all = uniform(min(min(ex.x, ex.y), min(ex.z, ex.w))) != 0;
     if (HALF && uniform(max(max(ex.x, ex.y), max(ex.z, ex.w))) > 1) return false;  // (in every wave)
     if (jb + 1 < j1) stage(jb + 1, buf ^ 1);
-    const int k0 = key0 + jb * kTileKeys;
-    // (uniform: a block hidden from all of the wave's rows is only settled)
+    const int k0 = key0 + jb * kTileKeys + wk * NK * 32;
+    // (uniform: keys hidden from all of the wave's rows are only settled)
     if (k0 < end_w) block(bo, k0, ex, all);
     if (jb + 1 < j1) {
       vm_wait<0>();
@@ -897,9 +952,37 @@ __device__ __forceinline__ bool tile_try(const PagedAttn& p, char* lds, int b, i
       }
     }
   }
+  if constexpr (WK > 1) {
+    // ---- the key halves of a row group joined: the second wave's state through LDS ----
+    static_assert(WK == 2);
+    __syncthreads();  // (reads of K and V are over)
+    float4* st = reinterpret_cast<float4*>(lds + wr * (64 * 64 * 4 + 1024));
+    float2* sml = reinterpret_cast<float2*>(st + 16 * 64);
+    if (wk == 1) {
+#pragma unroll
+      for (int i = 0; i < 16; i++)
+        st[i * 64 + lane] = make_float4(o[i >> 2][4 * (i & 3)], o[i >> 2][4 * (i & 3) + 1], o[i >> 2][4 * (i & 3) + 2], o[i >> 2][4 * (i & 3) + 3]);
+      sml[lane] = make_float2(part_max(m, l), l);
+    }
+    __syncthreads();
+    if (wk == 1) return true;
+    const float2 ml = sml[lane];
+    if (!(l == l)) m = 0.0f;
+    const float mn = fmaxf(m, ml.x);
+    const float wa = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn), wb = ml.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml.x - mn);
+    l = l * wa + ml.y * wb;
+    m = mn;
+#pragma unroll
+    for (int i = 0; i < 16; i++) {
+      const float4 x = st[i * 64 + lane];
+      const float v[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+      for (int r = 0; r < 4; r++) o[i >> 2][4 * (i & 3) + r] = o[i >> 2][4 * (i & 3) + r] * wa + v[r] * wb;
+    }
+  }
   auto finish = [&]() {
   const int64_t row = static_cast<int64_t>(sq.row0 + tok) * p.Hq + hd;
-  if (slot < 0) {
+  if (!to.o) {
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     uint16_t* dst = p.out + row * kD + 4 * hf;
 #pragma unroll
@@ -912,10 +995,9 @@ __device__ __forceinline__ bool tile_try(const PagedAttn& p, char* lds, int b, i
       }
     return;
   }
-  const int64_t part = PRE ? static_cast<int64_t>(slot) * p.T * p.Hq + row
-                           : (static_cast<int64_t>(slot) * p.Hkv + h) * kTileRows + 32 * wave + j;
-  if (hf == 0) *reinterpret_cast<float2*>((PRE ? p.pre_ml : p.wg_ml) + part * 2) = make_float2(part_max(m, l) - (HALF ? kUp : 0.0f), l);
-  float* dst = (PRE ? p.pre_o : p.wg_o) + part * kD + 4 * hf;
+  const int64_t part = to.by_row ? row : 32 * wr + j;
+  if (hf == 0) *reinterpret_cast<float2*>(to.ml + part * 2) = make_float2(part_max(m, l) - (HALF ? kUp : 0.0f), l);
+  float* dst = to.o + part * kD + 4 * hf;
 #pragma unroll
   for (int dt = 0; dt < 4; dt++)
 #pragma unroll
@@ -926,31 +1008,35 @@ __device__ __forceinline__ bool tile_try(const PagedAttn& p, char* lds, int b, i
   if (rw + j < R) finish();
   return true;
 }
-template <bool PRE>
-__device__ __forceinline__ void tile_run(const PagedAttn& p, char* lds, int b, int h, int r0, int j0, int j1, int slot) {
-  if (!uniform(tile_try<PRE, true>(p, lds, b, h, r0, j0, j1, slot)))
-    tile_try<PRE, false>(p, lds, b, h, r0, j0, j1, slot);
+template <bool PRE, int WK>
+__device__ __forceinline__ void tile_run(const PagedAttn& p, char* lds, int b, int h, int r0, int j0, int j1, const Result& to) {
+  if (!uniform(tile_try<PRE, true, WK>(p, lds, b, h, r0, j0, j1, to)))
+    tile_try<PRE, false, WK>(p, lds, b, h, r0, j0, j1, to);
 }
 
 // The shared rows: grid (kv heads, row tiles, key splits).
 __global__ void __launch_bounds__(256, 2) paged_prefix_kernel(const PagedAttn p) {
-  extern __shared__ __align__(16) char lds[];
+  extern __shared__ __align__(256) char lds[];  // (a row's 256 bytes: the addresses are made by exclusive or)
   const int nb = (p.shared + kTileKeys - 1) / kTileKeys, j0 = blockIdx.z * p.pre_bps;
-  tile_run<true>(p, lds, 0, blockIdx.x, blockIdx.y * kTileRows, j0, min(j0 + p.pre_bps, nb), blockIdx.z);
+  const int64_t slot = static_cast<int64_t>(blockIdx.z) * p.T * p.Hq;
+  tile_run<true, 1>(p, lds, 0, blockIdx.x, blockIdx.y * kTileRows, j0, min(j0 + p.pre_bps, nb),
+                    Result{p.pre_o + slot * kD, p.pre_ml + slot * 2, true});
 }
 
 // The plan's items, longest first: kv head blockIdx % Hkv, items a, 2A-1-a,
 // 2A+a, ... of the A workgroups of a head, so that who had a longer one has a
 // shorter one next.
 __global__ void __launch_bounds__(256, 2) paged_tile_kernel(const PagedAttn p) {
-  extern __shared__ __align__(16) char lds[];
+  extern __shared__ __align__(256) char lds[];  // (a row's 256 bytes: the addresses are made by exclusive or)
   const int h = blockIdx.x % p.Hkv, a = blockIdx.x / p.Hkv, A = gridDim.x / p.Hkv;
   const int items = p.plan[0];
   for (int r = 0; r * A < items; r++) {
     const int at = r * A + ((r & 1) ? A - 1 - a : a);
     if (at >= items) continue;
     const Item it = plan_items(p)[at];
-    tile_run<false>(p, lds, uniform(it.b), h, uniform(it.r0), uniform(it.j0), uniform(it.j1), uniform(it.slot));
+    const int64_t slot = (static_cast<int64_t>(uniform(it.slot)) * p.Hkv + h) * kTileRows;
+    tile_run<false, 1>(p, lds, uniform(it.b), h, uniform(it.r0), uniform(it.j0), uniform(it.j1),
+                       slot < 0 ? Result{nullptr, nullptr, false} : Result{p.wg_o + slot * kD, p.wg_ml + slot * 2, false});
   }
 }
 
@@ -1099,9 +1185,9 @@ __global__ void __launch_bounds__(256) paged_tile_merge_kernel(const PagedAttn p
     const int tok = r / p.rep;
     const int64_t at = static_cast<int64_t>(sq.row0 + tok) * p.Hq + h * p.rep + r - tok * p.rep;
     Fold f;
-    if (p.shared) f.add_all(p.pre_o + at * kD, p.pre_ml + at * 2, static_cast<int64_t>(p.T) * p.Hq, p.np, d);
+    if (p.shared) f.add_all(p.pre_o + at * kD, p.pre_ml + at * 2, static_cast<int64_t>(p.T) * p.Hq, 0, 1, p.np, d);
     const int64_t first = (static_cast<int64_t>(c.slot) * p.Hkv + h) * kTileRows + k;
-    f.add_all(p.wg_o + first * kD, p.wg_ml + first * 2, static_cast<int64_t>(p.Hkv) * kTileRows, c.n, d);
+    f.add_all(p.wg_o + first * kD, p.wg_ml + first * 2, static_cast<int64_t>(p.Hkv) * kTileRows, 0, 1, c.n, d);
     f.store(p.out + at * kD + d);
   }
 }
@@ -1110,7 +1196,9 @@ __global__ void __launch_bounds__(256) paged_tile_merge_kernel(const PagedAttn p
 // host
 // ---------------------------------------------------------------------------
 constexpr int kFewRows = 64;       // rows of a (sequence, kv head) pair up to which paged_few_kernel serves
-constexpr int kFewGrid = 768;      // its workgroups: three to a CU
+// its workgroups: as many as fit the CUs at once
+constexpr int kFewGrid = 512;
+constexpr int few_grid(int nt) { return nt == 4 ? kFewGrid / 2 : kFewGrid; }
 constexpr int kTileGrid = 512;     // of the tile kernel: two to a CU
 constexpr int kMaxPre = 64;        // key splits of the shared rows
 
@@ -1152,7 +1240,7 @@ PagedPlan make_plan(int Hq, int Hkv, int T, int B, int max_new, bool shared) {
     a.plan = take(few ? (1 + static_cast<size_t>(B)) * sizeof(int)
                       : sizeof(PlanHead) + a.most_items * sizeof(Item) + a.most_cuts * sizeof(Cut));
     const size_t firsts = few ? rows : 0;
-    const size_t others = few ? static_cast<size_t>(kFewGrid) * 16 * a.nt
+    const size_t others = few ? static_cast<size_t>(few_grid(a.nt)) * 16 * a.nt
                               : static_cast<size_t>(shared ? a.most_items : 2 * a.per_head) * Hkv * kTileRows;
     a.row_ml = take(firsts * 2 * sizeof(float));
     a.row_o = take(firsts * kD * sizeof(float));
@@ -1235,18 +1323,20 @@ extern "C" int bmx_attention_paged(const bmx_bf16* q, const bmx_paged_kv* cache,
     if (int rc = check_launch("attention_paged shared rows")) return rc;
   }
   if (a.few) {
-    const dim3 grid(kFewGrid), merge((batch->max_new * p.rep + 7) / 8, Hkv, B);
-    if (a.nt == 1) {
-      hipLaunchKernelGGL(paged_few_kernel<1>, grid, dim3(256), 0, st, p);
-      hipLaunchKernelGGL(paged_few_merge_kernel<1>, merge, dim3(256), 0, st, p);
-    } else if (a.nt == 2) {
-      hipLaunchKernelGGL(paged_few_kernel<2>, grid, dim3(256), 0, st, p);
-      hipLaunchKernelGGL(paged_few_merge_kernel<2>, merge, dim3(256), 0, st, p);
-    } else {
-      hipLaunchKernelGGL(paged_few_kernel<4>, grid, dim3(256), 0, st, p);
-      hipLaunchKernelGGL(paged_few_merge_kernel<4>, merge, dim3(256), 0, st, p);
-    }
-    return check_launch("attention_paged");
+    // few rows have many parts each
+    const bool wide = shared > 0 || static_cast<int64_t>(T) * n_heads <= 1024;
+    const int rows = batch->max_new * p.rep;
+    const dim3 merge(wide ? rows : (rows + 7) / 8, Hkv, B);
+    auto launch = [&](auto few, auto joint, auto joint_wide) {
+      hipLaunchKernelGGL(few, dim3(few_grid(a.nt)), dim3(a.nt == 4 ? 512 : 256), 0, st, p);
+      if (int rc = check_launch("attention_paged")) return rc;
+      if (wide) hipLaunchKernelGGL(joint_wide, merge, dim3(256), 0, st, p);
+      else hipLaunchKernelGGL(joint, merge, dim3(256), 0, st, p);
+      return check_launch("attention_paged merge");
+    };
+    if (a.nt == 1) return launch(paged_few_kernel<1, 1>, paged_few_merge_kernel<1, false>, paged_few_merge_kernel<1, true>);
+    if (a.nt == 2) return launch(paged_few_kernel<2, 1>, paged_few_merge_kernel<2, false>, paged_few_merge_kernel<2, true>);
+    return launch(paged_few_kernel<2, 2>, paged_few_merge_kernel<4, false>, paged_few_merge_kernel<4, true>);
   }
   if (int rc = allow_lds(paged_tile_kernel, kTileLds)) return rc;
   hipLaunchKernelGGL(paged_plan_kernel, dim3(1), dim3(kPlanThreads), 0, st, p, a.per_head);
