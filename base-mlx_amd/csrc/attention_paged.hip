@@ -73,6 +73,7 @@ struct PagedAttn {
   int np;             // key splits of the shared rows
   int pre_bps;        // 64-key blocks of such a split
   int most_items, most_cuts;  // of the plan's lists
+  int tile_rows;      // 128 or 256
 };
 
 // 2^x; maxima of -inf (no key seen) count as 0
@@ -565,19 +566,20 @@ __global__ void __launch_bounds__(256) paged_few_merge_kernel(const PagedAttn p)
 // ===========================================================================
 // many query rows
 // ===========================================================================
-constexpr int kTileRows = 128, kTileKeys = 64;
+constexpr int kTileKeys = 64;  // of a block
 constexpr int kTileBytes = kTileKeys * kD * 2;  // of a K or V tile
-// K and V, two of each; which 16-row quarters of the two blocks exist; a flag
-constexpr size_t kTileLds = 4 * kTileBytes + (2 * 4 + 1) * sizeof(int);
+// K and V, two of each; which waves' rows of the two blocks exist; a flag
+constexpr size_t kTileLds = 4 * kTileBytes + (2 * 8 + 1) * sizeof(int);
 
 // A piece of work: rows r0 .. of sequence b, 64-key blocks [j0, j1), and the
 // slot that takes its result (-1: it is the whole of it).
 struct Item {
   int b, r0, j0, j1, slot, pad[3];
 };
-// Rows r0 .. of sequence b whose keys were cut into n pieces, in slots slot ..
+// A tile whose keys were cut into n pieces, in slots slot ..: rows r0 .. R - 1
+// (at most a tile's) of the sequence whose packed rows begin at row0
 struct Cut {
-  int b, r0, slot, n;
+  int row0, R, r0, slot, n, pad[3];
 };
 struct PlanHead {
   int items, cuts, pad[2];
@@ -623,13 +625,14 @@ constexpr int kSchedMfma = 0x8, kSchedRead = 0x100, kSchedValu = 0x402;
 // chunk c lies at c ^ (4 (row % 4) + row / 4 % 4), which keeps both kinds of
 // read off each other's banks.  64 KB of LDS and up to 256 registers: two
 // workgroups share a CU, one's exponentials beside the other's products.
-template <bool PRE, bool HALF, int WK>
+template <bool PRE, bool HALF, int NW, int WK>
 __device__ __forceinline__ bool tile_try(const PagedAttn& p, char* lds, int b, int h, int r0, int j0, int j1, const Result& to) {
-  constexpr int WR = 4 / WK, NK = 2 / WK;  // row groups of waves; 32-key tiles of a wave
+  constexpr int WR = NW / WK, NK = 2 / WK;  // row groups of waves; 32-key tiles of a wave
+  constexpr int kOwn = kTileKeys / NW;      // rows of K and V that a wave stages
   const int tid = threadIdx.x, wave = uniform(tid >> 6), lane = tid & 63, j = lane & 31, hf = lane >> 5;
   const int wr = wave % WR, wk = wave / WR;
-  int* exist = reinterpret_cast<int*>(lds + 4 * kTileBytes);  // [2][4]
-  int* left_out = exist + 8;  // some value that is not finite was left out
+  int* exist = reinterpret_cast<int*>(lds + 4 * kTileBytes);  // [2][NW]
+  int* left_out = exist + 2 * NW;  // some value that is not finite was left out
   const MinusOne one = minus_one();
   const int cap = p.max_pages << p.shift;
   PagedSeq sq{0, p.T, 0};
@@ -665,37 +668,37 @@ __device__ __forceinline__ bool tile_try(const PagedAttn& p, char* lds, int b, i
 #pragma unroll
     for (int r = 0; r < 16; r++) o[dt][r] = 0.0f;
   float m = -INFINITY, l = 0.0f;
-  // ---- staging: the wave's 16 rows of each tile, 4 rows to an instruction ----
+  // ---- staging: the wave's rows of each tile, 4 rows to an instruction ----
   const int lrow = lane >> 4;  // row of the four
   // chunk (lane % 16) of LDS holds the row's chunk ^ swizzle
-  const uint32_t voff0 = lrow * 256 + (((lane & 15) ^ (4 * lrow)) << 4);
+  const uint32_t voff0 = lrow * 256 + (((lane & 15) ^ (4 * lrow) ^ (kOwn / 4 * wave & 3)) << 4);
   // (the page is asked for a block before its rows)
   int asked = -1;
   auto ask = [&](int jb) {
-    const int k0 = key0 + jb * kTileKeys + 16 * wave;
+    const int k0 = key0 + jb * kTileKeys + kOwn * wave;
     asked = k0 < end ? table[k0 >> p.shift] : -1;
   };
   auto stage = [&](int jb, int buf) {
-    const int k0 = key0 + jb * kTileKeys + 16 * wave;
+    const int k0 = key0 + jb * kTileKeys + kOwn * wave;
     const int pg = uniform(asked);
     ask(jb + 1);
     const bool ok = static_cast<unsigned>(pg) < static_cast<unsigned>(p.n_pages);
-    if (lane == 0) exist[4 * buf + wave] = ok;
+    if (lane == 0) exist[NW * buf + wave] = ok;
     const int64_t at = ok ? (((static_cast<int64_t>(pg) * p.Hkv + h) << p.shift) + (k0 & ((1 << p.shift) - 1))) * kD : 0;
-    const uint32_t dst = uniform(lds_offset(lds) + buf * 2 * kTileBytes + wave * 4096);
+    const uint32_t dst = uniform(lds_offset(lds) + buf * 2 * kTileBytes + wave * kOwn * 256);
     uint32_t v0 = voff0;
     asm volatile("" : "+v"(v0));
     const uint32_t voff[4] = {v0, v0 ^ (1024 | 16), v0 ^ (2048 | 32), v0 ^ (3072 | 48)};  // + 4 i rows
-    if (ok && k0 + 16 <= end) {  // uniform
+    if (ok && k0 + kOwn <= end) {  // uniform
 #pragma unroll
-      for (int i = 0; i < 4; i++) {
+      for (int i = 0; i < kOwn / 4; i++) {
         lds_load16_at(p.k + at, voff[i], dst + 1024 * i);
         lds_load16_at(p.v + at, voff[i], dst + kTileBytes + 1024 * i);
       }
       return;
     }
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
+    for (int i = 0; i < kOwn / 4; i++) {
       const bool in = ok && k0 + 4 * i + lrow < end;
       const char* zero = reinterpret_cast<const char*>(g_zeros) + 16 * (lane & 15);
       lds_load16(in ? reinterpret_cast<const char*>(p.k + at) + voff[i] : zero, dst + 1024 * i);
@@ -709,15 +712,15 @@ __device__ __forceinline__ bool tile_try(const PagedAttn& p, char* lds, int b, i
     const int k0 = key0 + jb * kTileKeys;
     const bool mixed = !PRE && k0 + kTileKeys > first && first < end;  // (uniform)
     if (!HALF && !mixed) return;
-    char* at = lds + buf * 2 * kTileBytes + kTileBytes + wave * 4096 + lane * 16;
-    uint4 w[4];
+    char* at = lds + buf * 2 * kTileBytes + kTileBytes + wave * kOwn * 256 + lane * 16;
+    uint4 w[kOwn / 4];
 #pragma unroll
-    for (int i = 0; i < 4; i++) w[i] = *reinterpret_cast<const uint4*>(at + i * 1024);
+    for (int i = 0; i < kOwn / 4; i++) w[i] = *reinterpret_cast<const uint4*>(at + i * 1024);
     bool changed = false;
     if (mixed) {
       uint32_t nf = 0;
 #pragma unroll
-      for (int i = 0; i < 4; i++) {
+      for (int i = 0; i < kOwn / 4; i++) {
         nf |= not_finite(w[i].x) | not_finite(w[i].y) | not_finite(w[i].z) | not_finite(w[i].w);
         w[i] = make_uint4(finite_part(w[i].x), finite_part(w[i].y), finite_part(w[i].z), finite_part(w[i].w));
       }
@@ -729,7 +732,7 @@ __device__ __forceinline__ bool tile_try(const PagedAttn& p, char* lds, int b, i
       // from 2^-12 to below 2^16
       uint32_t top = 0, low = ~0u;
 #pragma unroll
-      for (int i = 0; i < 4; i++) {
+      for (int i = 0; i < kOwn / 4; i++) {
         auto mag = [](uint32_t x) { return __builtin_bit_cast(u16x2_t, x & 0x7fff7fffu); };
         const u16x2_t a = __builtin_elementwise_max(__builtin_elementwise_max(mag(w[i].x), mag(w[i].y)),
                                                     __builtin_elementwise_max(mag(w[i].z), mag(w[i].w)));
@@ -738,11 +741,11 @@ __device__ __forceinline__ bool tile_try(const PagedAttn& p, char* lds, int b, i
         low = min(low, t - 1u);  // (0 wraps to the largest)
       }
       if (__any(top >= 0x4780u || low < 0x3980u - 1u)) {
-        if (lane == 0) exist[4 * buf + wave] = 2;
+        if (lane == 0) exist[NW * buf + wave] = 2;
         return;
       }
 #pragma unroll
-      for (int i = 0; i < 4; i++) {
+      for (int i = 0; i < kOwn / 4; i++) {
         auto h2 = [](uint32_t x) {
           return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(__uint_as_float(x << 16),
                                                                          __uint_as_float(x & 0xffff0000u)));
@@ -751,7 +754,7 @@ __device__ __forceinline__ bool tile_try(const PagedAttn& p, char* lds, int b, i
       }
     } else if (changed) {
 #pragma unroll
-      for (int i = 0; i < 4; i++) *reinterpret_cast<uint4*>(at + i * 1024) = w[i];
+      for (int i = 0; i < kOwn / 4; i++) *reinterpret_cast<uint4*>(at + i * 1024) = w[i];
     }
   };
   // ---- LDS addresses: of a row's chunk, the others' follow by exclusive or
@@ -766,7 +769,7 @@ __device__ __forceinline__ bool tile_try(const PagedAttn& p, char* lds, int b, i
     const int ch = (2 * grp + ((i16 & 3) >> 1)) ^ (4 * (row & 3) + ((row >> 2) & 3));
     vat0[u] = lds_offset(lds) + kTileBytes + wk * NK * 32 * 256 + row * 256 + ch * 16 + 8 * (i16 & 1);
   }
-  auto block = [&](int bo, int k0, const int4& ex, bool all) {
+  auto block = [&](int bo, int k0, const int (&e4)[4], bool all) {
     uint32_t kat = kat0 + bo, vat[2] = {vat0[0] + bo, vat0[1] + bo};
     asm volatile("" : "+v"(kat), "+v"(vat[0]), "+v"(vat[1]));
     // ---- scores ----
@@ -792,8 +795,7 @@ __device__ __forceinline__ bool tile_try(const PagedAttn& p, char* lds, int b, i
     }
     SCHED(kSchedMfma, 2 * NK);
     if (!all || k0 + 32 * NK > first_w) {  // uniform
-      const int e4[4] = {ex.x, ex.y, ex.z, ex.w};
-#pragma unroll
+      #pragma unroll
       for (int kt = 0; kt < NK; kt++)
 #pragma unroll
         for (int r = 0; r < 16; r++) {
@@ -922,13 +924,24 @@ __device__ __forceinline__ bool tile_try(const PagedAttn& p, char* lds, int b, i
   for (int jb = j0; jb < j1; jb++) {
     const int buf = (jb - j0) & 1, bo = buf * 2 * kTileBytes;
     __syncthreads();
-    const int4 ex = *reinterpret_cast<const int4*>(exist + 4 * buf);
-    const bool all = uniform(min(min(ex.x, ex.y), min(ex.z, ex.w))) != 0;
-    if (HALF && uniform(max(max(ex.x, ex.y), max(ex.z, ex.w))) > 1) return false;  // (in every wave)
+    int e4[4], most = 0, least = 2;
+#pragma unroll
+    for (int i = 0; i < NW; i += 4) {
+      const int4 e = *reinterpret_cast<const int4*>(exist + NW * buf + i);
+      least = min(least, min(min(e.x, e.y), min(e.z, e.w)));
+      most = max(most, max(max(e.x, e.y), max(e.z, e.w)));
+      if constexpr (NW == 4) {
+        e4[0] = e.x, e4[1] = e.y, e4[2] = e.z, e4[3] = e.w;
+      } else {
+        e4[i / 2] = e.x, e4[i / 2 + 1] = e.z;  // (two waves to 16 rows)
+      }
+    }
+    const bool all = uniform(least) != 0;
+    if (HALF && uniform(most) > 1) return false;  // (in every wave)
     if (jb + 1 < j1) stage(jb + 1, buf ^ 1);
     const int k0 = key0 + jb * kTileKeys + wk * NK * 32;
     // (uniform: keys hidden from all of the wave's rows are only settled)
-    if (k0 < end_w) block(bo, k0, ex, all);
+    if (k0 < end_w) block(bo, k0, e4, all);
     if (jb + 1 < j1) {
       vm_wait<0>();
       settle(jb + 1, buf ^ 1);
@@ -1008,25 +1021,27 @@ __device__ __forceinline__ bool tile_try(const PagedAttn& p, char* lds, int b, i
   if (rw + j < R) finish();
   return true;
 }
-template <bool PRE, int WK>
+template <bool PRE, int NW, int WK>
 __device__ __forceinline__ void tile_run(const PagedAttn& p, char* lds, int b, int h, int r0, int j0, int j1, const Result& to) {
-  if (!uniform(tile_try<PRE, true, WK>(p, lds, b, h, r0, j0, j1, to)))
-    tile_try<PRE, false, WK>(p, lds, b, h, r0, j0, j1, to);
+  if (!uniform(tile_try<PRE, true, NW, WK>(p, lds, b, h, r0, j0, j1, to)))
+    tile_try<PRE, false, NW, WK>(p, lds, b, h, r0, j0, j1, to);
 }
 
 // The shared rows: grid (kv heads, row tiles, key splits).
-__global__ void __launch_bounds__(256, 2) paged_prefix_kernel(const PagedAttn p) {
+template <int NW>
+__global__ void __launch_bounds__(64 * NW, 2) paged_prefix_kernel(const PagedAttn p) {
   extern __shared__ __align__(256) char lds[];  // (a row's 256 bytes: the addresses are made by exclusive or)
   const int nb = (p.shared + kTileKeys - 1) / kTileKeys, j0 = blockIdx.z * p.pre_bps;
   const int64_t slot = static_cast<int64_t>(blockIdx.z) * p.T * p.Hq;
-  tile_run<true, 1>(p, lds, 0, blockIdx.x, blockIdx.y * kTileRows, j0, min(j0 + p.pre_bps, nb),
+  tile_run<true, NW, 1>(p, lds, 0, blockIdx.x, blockIdx.y * (32 * NW), j0, min(j0 + p.pre_bps, nb),
                     Result{p.pre_o + slot * kD, p.pre_ml + slot * 2, true});
 }
 
 // The plan's items, longest first: kv head blockIdx % Hkv, items a, 2A-1-a,
 // 2A+a, ... of the A workgroups of a head, so that who had a longer one has a
 // shorter one next.
-__global__ void __launch_bounds__(256, 2) paged_tile_kernel(const PagedAttn p) {
+template <int NW>
+__global__ void __launch_bounds__(64 * NW, 2) paged_tile_kernel(const PagedAttn p) {
   extern __shared__ __align__(256) char lds[];  // (a row's 256 bytes: the addresses are made by exclusive or)
   const int h = blockIdx.x % p.Hkv, a = blockIdx.x / p.Hkv, A = gridDim.x / p.Hkv;
   const int items = p.plan[0];
@@ -1034,52 +1049,66 @@ __global__ void __launch_bounds__(256, 2) paged_tile_kernel(const PagedAttn p) {
     const int at = r * A + ((r & 1) ? A - 1 - a : a);
     if (at >= items) continue;
     const Item it = plan_items(p)[at];
-    const int64_t slot = (static_cast<int64_t>(uniform(it.slot)) * p.Hkv + h) * kTileRows;
-    tile_run<false, 1>(p, lds, uniform(it.b), h, uniform(it.r0), uniform(it.j0), uniform(it.j1),
+    const int64_t slot = (static_cast<int64_t>(uniform(it.slot)) * p.Hkv + h) * (32 * NW);
+    tile_run<false, NW, 1>(p, lds, uniform(it.b), h, uniform(it.r0), uniform(it.j0), uniform(it.j1),
                        slot < 0 ? Result{nullptr, nullptr, false} : Result{p.wg_o + slot * kD, p.wg_ml + slot * 2, false});
   }
 }
 
 // One workgroup lists the tiles of all sequences, cut where there are too few
-// to fill the `per_head` workgroups of a kv head.
+// to fill the `per_head` workgroups of a kv head: longest piece first, by a
+// counting sort of the pieces' lengths.  Pieces of one length come in any
+// order, which moves work about and no result.
 constexpr int kPlanThreads = 1024, kPlanBins = 1024;
-__global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const PagedAttn p, int per_head) {
-  __shared__ int tiles_before[kPagedMaxSeqs + 1];
-  __shared__ int bins[kPlanBins];
-  __shared__ int wsum[16], wmax[16], counts[3];  // items, cuts, slots
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  if (tid < 3) counts[tid] = 0;
-  for (int i = tid; i < kPlanBins; i += kPlanThreads) bins[i] = 0;
-  // ---- tiles before each sequence ----
-  const int per = (p.B + kPlanThreads - 1) / kPlanThreads, b0 = tid * per;
-  auto tiles_of = [&](int b) {
-    const PagedSeq s = paged_seq(p.starts[b], p.starts[b + 1], p.lens[b], p.T);
-    return (min(s.tokens, p.max_new) * p.rep + kTileRows - 1) / kTileRows;
-  };
-  int mine = 0;
-  for (int i = 0; i < per && b0 + i < p.B; i++) mine += tiles_of(b0 + i);
-  int x = mine;
+
+// Exclusive prefix of v over the workgroup, and the total; tmp: 17 ints
+__device__ __forceinline__ int plan_scan(int v, int* tmp, int* total) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int x = v;
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
     const int y = __shfl_up(x, o, 64);
     if (lane >= o) x += y;
   }
-  if (lane == 63) wsum[wave] = x;
+  if (lane == 63) tmp[wave] = x;
   __syncthreads();
-  int at = x - mine, n = 0;
-  for (int w = 0; w < 16; w++) {
-    if (w < wave) at += wsum[w];
-    n += wsum[w];
+  int y = tmp[lane & 15];
+#pragma unroll
+  for (int o = 1; o < 16; o <<= 1) {
+    const int z = __shfl_up(y, o, 16);
+    if ((lane & 15) >= o) y += z;
   }
-  for (int i = 0; i < per && b0 + i < p.B; i++) {
-    tiles_before[b0 + i] = at;
-    at += tiles_of(b0 + i);
+  *total = __shfl(y, 15, 64);
+  return x - v + (wave ? __shfl(y, wave - 1, 64) : 0);
+}
+
+__global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const PagedAttn p, int per_head) {
+  __shared__ int tiles_before[kPagedMaxSeqs], rows_of[kPagedMaxSeqs], pos_of[kPagedMaxSeqs];
+  __shared__ int bins[kPlanBins];
+  __shared__ int tmp[2][16], top[16], sums[16], counts[3];  // items, cuts, slots
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  if (tid < 3) counts[tid] = 0;
+  bins[tid] = 0;
+  // ---- sequences, and the tiles before each ----
+  const int per = (p.B + kPlanThreads - 1) / kPlanThreads, b0 = tid * per;
+  int mine = 0;
+  for (int b = b0; b < min(b0 + per, p.B); b++) {
+    const PagedSeq s = paged_seq(p.starts[b], p.starts[b + 1], p.lens[b], p.T);
+    const int R = min(s.tokens, p.max_new) * p.rep;
+    rows_of[b] = R;
+    pos_of[b] = s.pos;
+    mine += (R + p.tile_rows - 1) / p.tile_rows;
   }
-  if (tid == 0) tiles_before[p.B] = n;
+  int n;
+  int at = plan_scan(mine, tmp[0], &n);
+  for (int b = b0; b < min(b0 + per, p.B); b++) {
+    tiles_before[b] = at;
+    at += (rows_of[b] + p.tile_rows - 1) / p.tile_rows;
+  }
   __syncthreads();
   n = min(n, p.most_items - 2 * per_head);  // (starts out of order could count more)
-  // ---- a tile's sequence, first row and blocks ----
-  auto tile = [&](int i, int& b, int& r0) {
+  // ---- a tile's sequence, first row and blocks; a thread's first is kept ----
+  auto find = [&](int i, int& b, int& r0) {
     int lo = 0, hi = p.B;  // the last sequence with tiles_before <= i
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
@@ -1087,13 +1116,19 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const PagedAtt
       else hi = mid;
     }
     b = lo;
-    r0 = (i - tiles_before[lo]) * kTileRows;
-    const PagedSeq s = paged_seq(p.starts[b], p.starts[b + 1], p.lens[b], p.T);
-    const int R = min(s.tokens, p.max_new) * p.rep;
-    const int end = min(s.pos + (min(r0 + kTileRows, R) - 1) / p.rep + 1, p.max_pages << p.shift);
+    r0 = (i - tiles_before[lo]) * p.tile_rows;
+    const int end = min(pos_of[lo] + (min(r0 + p.tile_rows, rows_of[lo]) - 1) / p.rep + 1, p.max_pages << p.shift);
     return max(end - p.shared + kTileKeys - 1, 0) / kTileKeys;
   };
-  int sum = 0, most = 0;
+  int kb = 0, kr0 = 0;
+  const int knb = tid < n ? find(tid, kb, kr0) : 0;
+  auto tile = [&](int i, int& b, int& r0) {
+    if (i != tid) return find(i, b, r0);
+    b = kb;
+    r0 = kr0;
+    return knb;
+  };
+  int sum = 0, most = 1;
   for (int i = tid; i < n; i += kPlanThreads) {
     int b, r0;
     const int nb = tile(i, b, r0);
@@ -1105,63 +1140,55 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const PagedAtt
     sum += __shfl_xor(sum, o, 64);
     most = max(most, __shfl_xor(most, o, 64));
   }
-  __syncthreads();
   if (lane == 0) {
-    wsum[wave] = sum;
-    wmax[wave] = most;
+    sums[wave] = sum;
+    top[wave] = most;
   }
   __syncthreads();
-  sum = 0;
-  most = 1;
-  for (int w = 0; w < 16; w++) {
-    sum += wsum[w];
-    most = max(most, wmax[w]);
+  sum = sums[lane & 15];
+  most = top[lane & 15];
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) {
+    sum += __shfl_xor(sum, o, 16);
+    most = max(most, __shfl_xor(most, o, 16));
   }
   // ---- pieces of at most `size` blocks: what each workgroup has to do on
   // average, where that is less than the longest tile ----
-  int size = max((sum + per_head - 1) / per_head, 4);
   // (tiles longer than that number at most per_head, and so do their further pieces)
-  size = min(size, most);
-  auto pieces = [&](int nb) { return max((nb + size - 1) / size, 1); };
+  const int size = min(max((sum + per_head - 1) / per_head, 4), most);
   const float to_bin = static_cast<float>(kPlanBins - 1) / static_cast<float>(size);
   auto bin_of = [&](int len) { return kPlanBins - 1 - min(static_cast<int>(len * to_bin), kPlanBins - 1); };
+  auto cut = [&](int nb, int& len) {  // into pieces of len blocks (the last the rest)
+    const int np = max((nb + size - 1) / size, 1);
+    len = (nb + np - 1) / np;
+    return max((nb + max(len, 1) - 1) / max(len, 1), 1);
+  };
   for (int i = tid; i < n; i += kPlanThreads) {
-    int b, r0;
-    const int nb = tile(i, b, r0), np = pieces(nb), len = (nb + np - 1) / np;
-    atomicAdd(&bins[bin_of(len)], (nb + max(len, 1) - 1) / max(len, 1) + (nb == 0));
+    int b, r0, len;
+    const int parts = cut(tile(i, b, r0), len);
+    atomicAdd(&bins[bin_of(len)], parts);
   }
   __syncthreads();
-  // exclusive prefix of the bins (one per thread)
   {
-    const int v = bins[tid];
-    int y = v;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int z = __shfl_up(y, o, 64);
-      if (lane >= o) y += z;
-    }
-    __syncthreads();
-    if (lane == 63) wsum[wave] = y;
-    __syncthreads();
-    int first = y - v;
-    for (int w = 0; w < wave; w++) first += wsum[w];
-    bins[tid] = first;
+    int total;
+    const int first = plan_scan(bins[tid], tmp[1], &total);
+    bins[tid] = first;  // (each thread its own)
+    if (tid == 0) counts[0] = total;
   }
   __syncthreads();
   Item* items = plan_items(p);
   Cut* cuts = plan_cuts(p);
   for (int i = tid; i < n; i += kPlanThreads) {
-    int b, r0;
-    const int nb = tile(i, b, r0), np = pieces(nb), len = (nb + np - 1) / np;
-    const int parts = max((nb + max(len, 1) - 1) / max(len, 1), 1);
+    int b, r0, len;
+    const int nb = tile(i, b, r0), parts = cut(nb, len);
     int slot = -1;
     if (parts > 1 || p.shared) {
       slot = atomicAdd(&counts[2], parts);
       const int c = atomicAdd(&counts[1], 1);
-      if (c < p.most_cuts) cuts[c] = Cut{b, r0, slot, parts};
+      const int row0 = min(max(p.starts[b], 0), p.T);
+      if (c < p.most_cuts) cuts[c] = Cut{row0, rows_of[b], r0, slot, parts, {0, 0, 0}};
     }
     const int to = atomicAdd(&bins[bin_of(len)], parts);
-    atomicAdd(&counts[0], parts);
     for (int k = 0; k < parts; k++)
       if (to + k < p.most_items)
         items[to + k] = Item{b, r0, k * len, min((k + 1) * len, nb), slot < 0 ? -1 : slot + k, {0, 0, 0}};
@@ -1173,21 +1200,22 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const PagedAtt
   }
 }
 
-// The cut tiles' rows: parts over the shared rows, then the pieces'.
+// The cut tiles' rows, 8 to a workgroup: parts over the shared rows, then the
+// pieces'.
+constexpr int kTileMergeGrid = 2048;
 __global__ void __launch_bounds__(256) paged_tile_merge_kernel(const PagedAttn p) {
-  const int n = p.plan[1] * p.Hkv * (kTileRows / 8), d = 4 * (threadIdx.x & 31);
+  const int groups = p.tile_rows / 8, n = p.plan[1] * p.Hkv * groups, d = 4 * (threadIdx.x & 31);
   for (int w = blockIdx.x; w < n; w += gridDim.x) {
-    const int g = w % (kTileRows / 8), h = w / (kTileRows / 8) % p.Hkv;
-    const Cut c = plan_cuts(p)[w / (kTileRows / 8) / p.Hkv];
-    const PagedSeq sq = paged_seq(p.starts[c.b], p.starts[c.b + 1], p.lens[c.b], p.T);
+    const int g = w % groups, h = w / groups % p.Hkv;
+    const Cut c = plan_cuts(p)[w / groups / p.Hkv];
     const int k = 8 * g + (threadIdx.x >> 5), r = c.r0 + k;
-    if (r >= min(sq.tokens, p.max_new) * p.rep) continue;
+    if (r >= c.R) continue;
     const int tok = r / p.rep;
-    const int64_t at = static_cast<int64_t>(sq.row0 + tok) * p.Hq + h * p.rep + r - tok * p.rep;
+    const int64_t at = static_cast<int64_t>(c.row0 + tok) * p.Hq + h * p.rep + r - tok * p.rep;
     Fold f;
     if (p.shared) f.add_all(p.pre_o + at * kD, p.pre_ml + at * 2, static_cast<int64_t>(p.T) * p.Hq, 0, 1, p.np, d);
-    const int64_t first = (static_cast<int64_t>(c.slot) * p.Hkv + h) * kTileRows + k;
-    f.add_all(p.wg_o + first * kD, p.wg_ml + first * 2, static_cast<int64_t>(p.Hkv) * kTileRows, 0, 1, c.n, d);
+    const int64_t first = (static_cast<int64_t>(c.slot) * p.Hkv + h) * p.tile_rows + k;
+    f.add_all(p.wg_o + first * kD, p.wg_ml + first * 2, static_cast<int64_t>(p.Hkv) * p.tile_rows, 0, 1, c.n, d);
     f.store(p.out + at * kD + d);
   }
 }
@@ -1202,9 +1230,17 @@ constexpr int few_grid(int nt) { return nt == 4 ? kFewGrid / 2 : kFewGrid; }
 constexpr int kTileGrid = 512;     // of the tile kernel: two to a CU
 constexpr int kMaxPre = 64;        // key splits of the shared rows
 
+// Rows of a tile.  256 stage and convert a block of keys once for twice the rows,
+// but leave a workgroup alone on its CU, with more of them idle in short
+// sequences (us with 128 / 256 rows: one prompt of 4096 tokens 187 / 173, six of
+// 1 to 2049 90 / 88; a chunk of 509 beside 31 single tokens 77 / 90; 160 and 64
+// single tokens over shared rows 161 / 164 and 41.4 / 43.1).
+int tile_rows(int rep, int T, int B) { return static_cast<int64_t>(T) * rep >= static_cast<int64_t>(B) * 1536 ? 256 : 128; }
+
 struct PagedPlan {
   int few, nt;        // few: row tiles of 16
-  int per_head;       // tile workgroups of a kv head
+  int rows, per_head; // of a tile; tile workgroups of a kv head
+  int64_t all;        // tiles of all the batch's rows
   int np;             // most key splits of the shared rows
   int most_items, most_cuts;
   size_t plan, row_ml, row_o, wg_ml, wg_o, pre_ml, pre_o;  // byte offsets
@@ -1212,53 +1248,61 @@ struct PagedPlan {
 };
 
 // Where a call's workspace has its parts.  The same offsets would do for any
-// smaller batch only if it took the same kernel, so `bytes` counts the larger of
-// both kernels' needs, each of which grows with the batch.
+// smaller batch only if it took the same kernel and tiles, so `bytes` counts the
+// largest of all their needs, each of which grows with the batch.
 PagedPlan make_plan(int Hq, int Hkv, int T, int B, int max_new, bool shared) {
   PagedPlan a{};
   const int rep = Hq / Hkv;
   const size_t rows = static_cast<size_t>(T) * Hq;
   const int64_t R = static_cast<int64_t>(max_new) * rep;
-  a.few = R <= kFewRows;
-  a.per_head = std::max(1, kTileGrid / Hkv);
-  const int64_t all = (static_cast<int64_t>(T) * rep + kTileRows - 1) / kTileRows;
-  // whole tiles, and as many pieces more as there are workgroups
-  const int64_t tiles = all + std::min(B, T);
-  a.most_items = static_cast<int>(tiles) + 2 * a.per_head;
-  a.most_cuts = static_cast<int>(shared ? tiles : std::min<int64_t>(tiles, 2 * a.per_head));
-  size_t at = 0;
+  size_t at = 0, most = 0;
   auto take = [&](size_t bytes) {
     const size_t was = at;
     at += (bytes + 255) & ~static_cast<size_t>(255);
     return was;
   };
-  size_t most = 0;
-  auto parts = [&](bool few) {
-    const int64_t r = few ? std::min<int64_t>(R, kFewRows) : R;
-    a.nt = r <= 16 ? 1 : r <= 32 ? 2 : 4;
+  auto parts = [&](size_t plan, size_t firsts, size_t others) {
     at = 0;
-    a.plan = take(few ? (1 + static_cast<size_t>(B)) * sizeof(int)
-                      : sizeof(PlanHead) + a.most_items * sizeof(Item) + a.most_cuts * sizeof(Cut));
-    const size_t firsts = few ? rows : 0;
-    const size_t others = few ? static_cast<size_t>(few_grid(a.nt)) * 16 * a.nt
-                              : static_cast<size_t>(shared ? a.most_items : 2 * a.per_head) * Hkv * kTileRows;
+    a.plan = take(plan);
     a.row_ml = take(firsts * 2 * sizeof(float));
     a.row_o = take(firsts * kD * sizeof(float));
     a.wg_ml = take(others * 2 * sizeof(float));
     a.wg_o = take(others * kD * sizeof(float));
     most = std::max(most, at);
   };
+  auto few = [&]() {
+    const int64_t r = std::min<int64_t>(R, kFewRows);
+    a.nt = r <= 16 ? 1 : r <= 32 ? 2 : 4;
+    parts((1 + static_cast<size_t>(B)) * sizeof(int), rows, static_cast<size_t>(few_grid(a.nt)) * 16 * a.nt);
+  };
+  auto tile = [&](int tile_rows) {
+    a.rows = tile_rows;
+    a.per_head = std::max(1, kTileGrid * 128 / tile_rows / Hkv);
+    a.all = (static_cast<int64_t>(T) * rep + tile_rows - 1) / tile_rows;
+    // whole tiles, and as many pieces more as there are workgroups
+    const int64_t tiles = a.all + std::min(B, T);
+    a.most_items = static_cast<int>(tiles) + 2 * a.per_head;
+    a.most_cuts = static_cast<int>(shared ? tiles : std::min<int64_t>(tiles, 2 * a.per_head));
+    parts(sizeof(PlanHead) + a.most_items * sizeof(Item) + a.most_cuts * sizeof(Cut), 0,
+          static_cast<size_t>(shared ? a.most_items : 2 * a.per_head) * Hkv * tile_rows);
+  };
+  a.few = R <= kFewRows;
+  const int mine = tile_rows(rep, T, B);
+  if (!a.few) {
+    if (rep <= kFewRows) few();
+    tile(128 + 256 - mine);
+  }
+  const size_t others = most;
+  tile(mine);  // (the shared rows', and the call's own where it is not of few rows)
   if (a.few) {
-    parts(true);
-  } else {
-    if (rep <= kFewRows) parts(true);
-    parts(false);
+    most = others;
+    few();
   }
   if (shared) {
-    a.np = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(kMaxPre, a.per_head / all)));
+    a.np = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(kMaxPre, a.per_head / a.all)));
     // (np splits of T rep rows each: at most per_head tiles, or one split of them all)
     const size_t slots = Hkv * std::min<size_t>(kMaxPre * static_cast<size_t>(T) * rep,
-                                                std::max<size_t>(static_cast<size_t>(a.per_head) * kTileRows,
+                                                std::max<size_t>(static_cast<size_t>(a.per_head) * a.rows,
                                                                  static_cast<size_t>(T) * rep));
     at = most;
     a.pre_ml = take(slots * 2 * sizeof(float));
@@ -1312,14 +1356,15 @@ extern "C" int bmx_attention_paged(const bmx_bf16* q, const bmx_paged_kv* cache,
                     batch->max_new, n_heads, Hkv, n_heads / Hkv, cache->n_pages, log2_of(cache->page_size), shared,
                     fabsf(scale) * kLog2e, scale < 0.0f ? 0x80008000u : 0u, reinterpret_cast<int*>(ws + a.plan),
                     part(a.row_o), part(a.row_ml), part(a.wg_o), part(a.wg_ml), part(a.pre_o), part(a.pre_ml), np, bps,
-                    a.most_items, a.most_cuts};
+                    a.most_items, a.most_cuts, a.rows};
   p.c2 = p.c2 < kLeast ? kLeast : p.c2;
   const hipStream_t st = as_stream(stream);
   if (shared) {
-    if (int rc = allow_lds(paged_prefix_kernel, kTileLds)) return rc;
-    const int tiles = (T * p.rep + kTileRows - 1) / kTileRows;
-    if (tiles > 65535) return set_error(BMX_E_SHAPE, "attention_paged: tokens=%d too many for shared rows", T);
-    hipLaunchKernelGGL(paged_prefix_kernel, dim3(Hkv, tiles, np), dim3(256), kTileLds, st, p);
+        const int tiles = static_cast<int>(a.all);
+    const auto kernel = a.rows == 256 ? paged_prefix_kernel<8> : paged_prefix_kernel<4>;
+    if (a.all > 65535) return set_error(BMX_E_SHAPE, "attention_paged: tokens=%d too many for shared rows", T);
+    if (int rc = allow_lds(kernel, kTileLds)) return rc;
+    hipLaunchKernelGGL(kernel, dim3(Hkv, tiles, np), dim3(2 * a.rows), kTileLds, st, p);
     if (int rc = check_launch("attention_paged shared rows")) return rc;
   }
   if (a.few) {
@@ -1338,9 +1383,10 @@ extern "C" int bmx_attention_paged(const bmx_bf16* q, const bmx_paged_kv* cache,
     if (a.nt == 2) return launch(paged_few_kernel<2, 1>, paged_few_merge_kernel<2, false>, paged_few_merge_kernel<2, true>);
     return launch(paged_few_kernel<2, 2>, paged_few_merge_kernel<4, false>, paged_few_merge_kernel<4, true>);
   }
-  if (int rc = allow_lds(paged_tile_kernel, kTileLds)) return rc;
+  const auto kernel = a.rows == 256 ? paged_tile_kernel<8> : paged_tile_kernel<4>;
+  if (int rc = allow_lds(kernel, kTileLds)) return rc;
   hipLaunchKernelGGL(paged_plan_kernel, dim3(1), dim3(kPlanThreads), 0, st, p, a.per_head);
-  hipLaunchKernelGGL(paged_tile_kernel, dim3(a.per_head * Hkv), dim3(256), kTileLds, st, p);
-  hipLaunchKernelGGL(paged_tile_merge_kernel, dim3(1024), dim3(256), 0, st, p);
+  hipLaunchKernelGGL(kernel, dim3(a.per_head * Hkv), dim3(2 * a.rows), kTileLds, st, p);
+  hipLaunchKernelGGL(paged_tile_merge_kernel, dim3(kTileMergeGrid), dim3(256), 0, st, p);
   return check_launch("attention_paged");
 }

@@ -115,6 +115,25 @@ def test_workspace_grows_with_the_batch():
                                 assert q(hq, hkv, tokens, seqs, new, 0) <= most
 
 
+def test_workspace_never_shrinks():
+    """More tokens, sequences or new tokens of one, and shared rows, need no less."""
+    q = bmx.load().bmx_attention_paged_workspace_bytes
+    sizes = [1, 2, 7, 60, 95, 96, 97, 190, 191, 192, 193, 384, 385, 1000, 1535, 1536, 1537, 3000]
+    for hq, hkv in ((32, 8), (8, 8), (64, 1)):
+        for shared in (0, 1):
+            for tokens in sizes:
+                for seqs in (1, 2, 3, 4, 7, 8, 9, 60, 400):
+                    for new in sizes:
+                        if new > tokens:
+                            continue
+                        n = q(hq, hkv, tokens, seqs, new, shared)
+                        at = (hq, hkv, tokens, seqs, new, shared)
+                        assert q(hq, hkv, tokens + 1, seqs, new, shared) >= n, at
+                        assert q(hq, hkv, tokens, seqs + 1, new, shared) >= n, at
+                        assert new == tokens or q(hq, hkv, tokens, seqs, new + 1, shared) >= n, at
+                        assert q(hq, hkv, tokens, seqs, new, 1) >= n, at
+
+
 def test_python_refusals_need_no_gpu():
     import torch
 
