@@ -74,6 +74,7 @@ struct PagedAttn {
   int pre_bps;        // 64-key blocks of such a split
   int most_items, most_cuts;  // of the plan's lists
   int tile_rows;      // 128 or 256
+  int few_shift;      // of few rows: log2 of a block's keys
 };
 
 // 2^x; maxima of -inf (no key seen) count as 0
@@ -170,11 +171,74 @@ __device__ __forceinline__ int scan256(int v, int* tmp, int* total) {
 __device__ __forceinline__ int few_blocks(const PagedAttn& p, const PagedSeq& s) {
   if (s.tokens == 0) return 0;
   const int end = min(s.pos + min(s.tokens, p.max_new), p.max_pages << p.shift);
-  return max(end - p.shared + kFewKeys - 1, 0) / kFewKeys;
+  return max(end - p.shared + (1 << p.few_shift) - 1, 0) >> p.few_shift;
 }
 
-// A share of the blocks: segments of (sequence, kv head) pairs, heads inner.
-// Per wave and step of 32 keys, in two 16-key tiles:
+// A workgroup's share of all pairs' blocks, [t, t1): a pair (sequence, kv head;
+// heads inner) and a block of it at a time.
+struct Share {
+  int t, t1, b, h, j, nb;
+  PagedSeq sq;
+};
+// False where the share is empty.  tmp: 8 ints, found: 5.
+__device__ __forceinline__ bool first_share(const PagedAttn& p, int* tmp, int* found, Share& s) {
+  const int tid = threadIdx.x;
+  const int per = (p.B + 255) >> 8, b0 = (tid & 255) * per;
+  int mine = 0;
+  PagedSeq only{0, 0, 0};
+  for (int i = 0; i < per && b0 + i < p.B; i++) {
+    only = paged_seq(p.starts[b0 + i], p.starts[b0 + i + 1], p.lens[b0 + i], p.T);
+    mine += few_blocks(p, only);
+  }
+  int all;
+  const int before = scan256(mine, tmp, &all);
+  const int share = max(1, (p.Hkv * all + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x));
+  s.t = blockIdx.x * share;
+  s.t1 = min(s.t + share, p.Hkv * all);
+  if (blockIdx.x == 0 || (s.t < s.t1 && p.Hkv * before <= s.t && s.t < p.Hkv * (before + mine))) {
+    int at = before;
+    for (int i = 0; i < per && b0 + i < p.B; i++) {
+      const PagedSeq q = per == 1 ? only : paged_seq(p.starts[b0 + i], p.starts[b0 + i + 1], p.lens[b0 + i], p.T);
+      const int n = few_blocks(p, q);
+      if (blockIdx.x == 0) p.plan[1 + b0 + i] = at;
+      if (p.Hkv * at <= s.t && s.t < p.Hkv * (at + n)) {
+        found[0] = b0 + i;
+        found[1] = at;
+        found[2] = q.row0;
+        found[3] = q.tokens;
+        found[4] = q.pos;
+      }
+      at += n;
+    }
+    if (blockIdx.x == 0 && tid == 0) p.plan[0] = share;
+  }
+  __syncthreads();
+  if (s.t >= s.t1) return false;
+  s.b = uniform(found[0]);
+  const int rel = s.t - p.Hkv * uniform(found[1]);
+  s.sq = PagedSeq{uniform(found[2]), uniform(found[3]), uniform(found[4])};
+  s.nb = few_blocks(p, s.sq);
+  if (s.nb == 0) return false;  // (not reached: the scan found blocks here)
+  s.h = min(rel / s.nb, p.Hkv - 1);
+  s.j = min(rel - s.h * s.nb, s.nb - 1);
+  return true;
+}
+// n blocks on, to the start of the next pair; false at the end
+__device__ __forceinline__ bool next_share(const PagedAttn& p, int n, Share& s) {
+  s.t += n;
+  s.j = 0;
+  if (s.t >= s.t1) return false;
+  if (++s.h < p.Hkv) return true;
+  s.h = 0;
+  do {
+    if (++s.b == p.B) return false;  // (not reached: blocks remain, so a sequence with some does)
+    s.sq = paged_seq(p.starts[s.b], p.starts[s.b + 1], p.lens[s.b], p.T);
+    s.nb = few_blocks(p, s.sq);
+  } while (s.nb == 0);
+  return true;
+}
+
+// Up to 16 query rows of a pair (NT = 1), in blocks of 128 keys.  Per wave and step of 32 keys, in two 16-key tiles:
 //   S^T = K Q^T (v_mfma_f32_16x16x32_bf16): lane l holds query row l % 16 and
 //     keys 4 (l / 16) + i of each tile;
 //   O^T += V^T P^T: the eight keys of a lane's scores are its k slice as they
@@ -187,53 +251,20 @@ __device__ __forceinline__ int few_blocks(const PagedAttn& p, const PagedSeq& s)
 // RG groups of 4 waves take 16 NT rows each over the same keys (64 rows by one
 // group needed more than 256 registers a wave: 36 us for 16 sequences of 5
 // tokens, against @@).
-template <int NT, int RG>
-__global__ void __launch_bounds__(256 * RG, 2) paged_few_kernel(const PagedAttn p) {
+template <int NT>
+__global__ void __launch_bounds__(256, 2) paged_few_kernel(const PagedAttn p) {
   __shared__ int tmp[8];
   __shared__ int found[5];
   __shared__ __align__(16) float os[4][16][kFewOs];
-  __shared__ float ms[4][16 * NT * RG], ls[4][16 * NT * RG];
-  const int tid = threadIdx.x, wave = uniform(tid >> 6) & 3, rg = uniform(tid >> 8), lane = tid & 63, li = lane & 15, g = lane >> 4;
+  __shared__ float ms[4][16 * NT], ls[4][16 * NT];
+  const int tid = threadIdx.x, wave = uniform(tid >> 6), lane = tid & 63, li = lane & 15, g = lane >> 4;
   const MinusOne one = minus_one();
-  // ---- this workgroup's share: blocks [t0, t1) of all pairs' ----
-  const int per = (p.B + 255) >> 8, b0 = (tid & 255) * per;
-  int mine = 0;
-  PagedSeq only{0, 0, 0};
-  for (int i = 0; i < per && b0 + i < p.B; i++) {
-    only = paged_seq(p.starts[b0 + i], p.starts[b0 + i + 1], p.lens[b0 + i], p.T);
-    mine += few_blocks(p, only);
-  }
-  int all;
-  const int before = scan256(mine, tmp, &all);
-  const int share = max(1, (p.Hkv * all + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x));
-  const int t0 = blockIdx.x * share, t1 = min(t0 + share, p.Hkv * all);
-  if (blockIdx.x == 0 || (t0 < t1 && p.Hkv * before <= t0 && t0 < p.Hkv * (before + mine))) {
-    int at = before;
-    for (int i = 0; i < per && b0 + i < p.B; i++) {
-      const PagedSeq s = per == 1 ? only : paged_seq(p.starts[b0 + i], p.starts[b0 + i + 1], p.lens[b0 + i], p.T);
-      const int n = few_blocks(p, s);
-      if (blockIdx.x == 0) p.plan[1 + b0 + i] = at;
-      if (p.Hkv * at <= t0 && t0 < p.Hkv * (at + n)) {
-        found[0] = b0 + i;
-        found[1] = at;
-        found[2] = s.row0;
-        found[3] = s.tokens;
-        found[4] = s.pos;
-      }
-      at += n;
-    }
-    if (blockIdx.x == 0 && tid == 0) p.plan[0] = share;
-  }
-  __syncthreads();
-  if (t0 >= t1) return;
-  int b = uniform(found[0]);
-  const int rel = t0 - p.Hkv * uniform(found[1]);
-  PagedSeq sq{uniform(found[2]), uniform(found[3]), uniform(found[4])};
-  int nb = few_blocks(p, sq);
-  if (nb == 0) return;  // (not reached: the scan found blocks here)
-  int h = min(rel / nb, p.Hkv - 1), j = min(rel - h * nb, nb - 1);
-  for (int t = t0; t < t1;) {
-    const int n = min(t1 - t, nb - j);
+  Share at;
+  if (!first_share(p, tmp, found, at)) return;
+  bool more_shares;
+  do {
+    const PagedSeq sq = at.sq;
+    const int b = at.b, h = at.h, j = at.j, nb = at.nb, n = min(at.t1 - at.t, nb - j);
     // ---- the segment: blocks j .. j + n - 1 of (b, h) ----
     const int R = min(sq.tokens, p.max_new) * p.rep;
     const int cap = p.max_pages << p.shift;
@@ -244,7 +275,7 @@ __global__ void __launch_bounds__(256 * RG, 2) paged_few_kernel(const PagedAttn 
     uint4 qf[NT][4];
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
-      const int r = min(16 * (NT * rg + nt) + li, R - 1), tok = r / p.rep, hd = h * p.rep + r - tok * p.rep;
+      const int r = min(16 * nt + li, R - 1), tok = r / p.rep, hd = h * p.rep + r - tok * p.rep;
       lim[nt] = min(sq.pos + tok + 1, cap);
       const uint16_t* src = p.q + (static_cast<int64_t>(hd) * p.T + sq.row0 + tok) * kD + 8 * g;
 #pragma unroll
@@ -420,28 +451,24 @@ __global__ void __launch_bounds__(256 * RG, 2) paged_few_kernel(const PagedAttn 
     for (int nt = 0; nt < NT; nt++) {
       const float sum = add_xor32(add_xor16(l[nt]));
       if (g == 0) {
-        ms[wave][16 * (NT * rg + nt) + li] = part_max(m[nt], sum);
-        ls[wave][16 * (NT * rg + nt) + li] = sum;
+        ms[wave][16 * nt + li] = part_max(m[nt], sum);
+        ls[wave][16 * nt + li] = sum;
       }
     }
     const bool direct = n == nb && !p.shared;
 #pragma unroll
-    for (int pass = 0; pass < NT * RG; pass++) {
-      if (16 * pass >= R) break;  // uniform
-      if (pass > 0) __syncthreads();
-      if (rg == pass / NT) {
-        constexpr int kN = NT;
-        const int nt = pass % kN;
+    for (int nt = 0; nt < NT; nt++) {
+      if (16 * nt >= R) break;  // uniform
+      if (nt > 0) __syncthreads();
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-          float* dst = &os[wave][li][32 * g + 8 * i];
-          *reinterpret_cast<float4*>(dst) = make_float4(o[nt][0][i], o[nt][1][i], o[nt][2][i], o[nt][3][i]);
-          *reinterpret_cast<float4*>(dst + 4) = make_float4(o[nt][4][i], o[nt][5][i], o[nt][6][i], o[nt][7][i]);
-        }
+      for (int i = 0; i < 4; i++) {
+        float* dst = &os[wave][li][32 * g + 8 * i];
+        *reinterpret_cast<float4*>(dst) = make_float4(o[nt][0][i], o[nt][1][i], o[nt][2][i], o[nt][3][i]);
+        *reinterpret_cast<float4*>(dst + 4) = make_float4(o[nt][4][i], o[nt][5][i], o[nt][6][i], o[nt][7][i]);
       }
       __syncthreads();
-      constexpr int kE = 8 / RG, kPer = kD / kE;  // values of a thread, threads of a row
-      const int row = tid / kPer, d0 = kE * (tid % kPer), r = 16 * pass + row;
+      constexpr int kE = 8;  // values of a thread
+      const int row = tid >> 4, d0 = kE * (tid & 15), r = 16 * nt + row;
       if (r < R) {
         float mm = -INFINITY, ll = 0.0f, a[kE] = {};
 #pragma unroll
@@ -455,15 +482,15 @@ __global__ void __launch_bounds__(256 * RG, 2) paged_few_kernel(const PagedAttn 
           for (int d = 0; d < kE; d++) a[d] += x * os[w][row][d0 + d];
         }
         const int tok = r / p.rep, hd = h * p.rep + r - tok * p.rep;
-        const int64_t at = static_cast<int64_t>(sq.row0 + tok) * p.Hq + hd;
+        const int64_t dst = static_cast<int64_t>(sq.row0 + tok) * p.Hq + hd;
         if (direct) {
           const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;
 #pragma unroll
           for (int d = 0; d < kE; d += 4)
-            *reinterpret_cast<uint2*>(p.out + at * kD + d0 + d) =
+            *reinterpret_cast<uint2*>(p.out + dst * kD + d0 + d) =
                 make_uint2(pack2(a[d] * inv, a[d + 1] * inv), pack2(a[d + 2] * inv, a[d + 3] * inv));
         } else {
-          const int64_t slot = j == 0 ? at : static_cast<int64_t>(blockIdx.x) * (16 * NT * RG) + r;
+          const int64_t slot = j == 0 ? dst : static_cast<int64_t>(blockIdx.x) * (16 * NT) + r;
           float* po = (j == 0 ? p.row_o : p.wg_o) + slot * kD + d0;
 #pragma unroll
           for (int d = 0; d < kE; d += 4) *reinterpret_cast<float4*>(po + d) = make_float4(a[d], a[d + 1], a[d + 2], a[d + 3]);
@@ -472,18 +499,8 @@ __global__ void __launch_bounds__(256 * RG, 2) paged_few_kernel(const PagedAttn 
       }
     }
     __syncthreads();  // (os, ms and ls are the next segment's)
-    // ---- the next pair ----
-    t += n;
-    j = 0;
-    if (t < t1 && ++h == p.Hkv) {
-      h = 0;
-      do {
-        if (++b == p.B) return;  // (not reached: blocks remain, so a sequence with some does)
-        sq = paged_seq(p.starts[b], p.starts[b + 1], p.lens[b], p.T);
-        nb = few_blocks(p, sq);
-      } while (nb == 0);
-    }
-  }
+    more_shares = next_share(p, n, at);
+  } while (more_shares);
 }
 
 // A row's parts, folded one after another: 32 lanes per row, 4 values each.
@@ -626,7 +643,7 @@ constexpr int kSchedMfma = 0x8, kSchedRead = 0x100, kSchedValu = 0x402;
 // read off each other's banks.  64 KB of LDS and up to 256 registers: two
 // workgroups share a CU, one's exponentials beside the other's products.
 template <bool PRE, bool HALF, int NW, int WK>
-__device__ __forceinline__ bool tile_try(const PagedAttn& p, char* lds, int b, int h, int r0, int j0, int j1, const Result& to) {
+__device__ __forceinline__ bool tile_try(const PagedAttn& p, char* lds, const PagedSeq& sq, int b, int h, int r0, int j0, int j1, const Result& to) {
   constexpr int WR = NW / WK, NK = 2 / WK;  // row groups of waves; 32-key tiles of a wave
   constexpr int kOwn = kTileKeys / NW;      // rows of K and V that a wave stages
   const int tid = threadIdx.x, wave = uniform(tid >> 6), lane = tid & 63, j = lane & 31, hf = lane >> 5;
@@ -635,8 +652,6 @@ __device__ __forceinline__ bool tile_try(const PagedAttn& p, char* lds, int b, i
   int* left_out = exist + 2 * NW;  // some value that is not finite was left out
   const MinusOne one = minus_one();
   const int cap = p.max_pages << p.shift;
-  PagedSeq sq{0, p.T, 0};
-  if constexpr (!PRE) sq = paged_seq(p.starts[b], p.starts[b + 1], p.lens[b], p.T);
   const int tokens = PRE ? p.T : min(sq.tokens, p.max_new);
   const int R = tokens * p.rep;
   const int key0 = PRE ? 0 : p.shared;
@@ -1022,9 +1037,9 @@ __device__ __forceinline__ bool tile_try(const PagedAttn& p, char* lds, int b, i
   return true;
 }
 template <bool PRE, int NW, int WK>
-__device__ __forceinline__ void tile_run(const PagedAttn& p, char* lds, int b, int h, int r0, int j0, int j1, const Result& to) {
-  if (!uniform(tile_try<PRE, true, NW, WK>(p, lds, b, h, r0, j0, j1, to)))
-    tile_try<PRE, false, NW, WK>(p, lds, b, h, r0, j0, j1, to);
+__device__ __forceinline__ void tile_run(const PagedAttn& p, char* lds, const PagedSeq& sq, int b, int h, int r0, int j0, int j1, const Result& to) {
+  if (!uniform(tile_try<PRE, true, NW, WK>(p, lds, sq, b, h, r0, j0, j1, to)))
+    tile_try<PRE, false, NW, WK>(p, lds, sq, b, h, r0, j0, j1, to);
 }
 
 // The shared rows: grid (kv heads, row tiles, key splits).
@@ -1033,7 +1048,7 @@ __global__ void __launch_bounds__(64 * NW, 2) paged_prefix_kernel(const PagedAtt
   extern __shared__ __align__(256) char lds[];  // (a row's 256 bytes: the addresses are made by exclusive or)
   const int nb = (p.shared + kTileKeys - 1) / kTileKeys, j0 = blockIdx.z * p.pre_bps;
   const int64_t slot = static_cast<int64_t>(blockIdx.z) * p.T * p.Hq;
-  tile_run<true, NW, 1>(p, lds, 0, blockIdx.x, blockIdx.y * (32 * NW), j0, min(j0 + p.pre_bps, nb),
+  tile_run<true, NW, 1>(p, lds, PagedSeq{0, p.T, 0}, 0, blockIdx.x, blockIdx.y * (32 * NW), j0, min(j0 + p.pre_bps, nb),
                     Result{p.pre_o + slot * kD, p.pre_ml + slot * 2, true});
 }
 
@@ -1050,9 +1065,30 @@ __global__ void __launch_bounds__(64 * NW, 2) paged_tile_kernel(const PagedAttn 
     if (at >= items) continue;
     const Item it = plan_items(p)[at];
     const int64_t slot = (static_cast<int64_t>(uniform(it.slot)) * p.Hkv + h) * (32 * NW);
-    tile_run<false, NW, 1>(p, lds, uniform(it.b), h, uniform(it.r0), uniform(it.j0), uniform(it.j1),
+    const int b = uniform(it.b);
+    tile_run<false, NW, 1>(p, lds, paged_seq(p.starts[b], p.starts[b + 1], p.lens[b], p.T), b, h, uniform(it.r0), uniform(it.j0), uniform(it.j1),
                        slot < 0 ? Result{nullptr, nullptr, false} : Result{p.wg_o + slot * kD, p.wg_ml + slot * 2, false});
   }
+}
+
+// Up to 64 query rows of a pair, in blocks of 64 keys by shares as
+// paged_few_kernel: two row groups of waves, each by two waves that take half of
+// a block's keys.
+__global__ void __launch_bounds__(256, 2) paged_mid_kernel(const PagedAttn p) {
+  extern __shared__ __align__(256) char lds[];  // (a row's 256 bytes: the addresses are made by exclusive or)
+  __shared__ int tmp[8];
+  __shared__ int found[5];
+  Share at;
+  if (!first_share(p, tmp, found, at)) return;
+  bool more;
+  do {
+    const int n = min(at.t1 - at.t, at.nb - at.j);
+    const int64_t slot = static_cast<int64_t>(blockIdx.x) * 64;
+    Result to{nullptr, nullptr, false};
+    if (n < at.nb || p.shared) to = at.j == 0 ? Result{p.row_o, p.row_ml, true} : Result{p.wg_o + slot * kD, p.wg_ml + slot * 2, false};
+    tile_run<false, 4, 2>(p, lds, at.sq, at.b, at.h, 0, at.j, at.j + n, to);
+    more = next_share(p, n, at);
+  } while (more);
 }
 
 // One workgroup lists the tiles of all sequences, cut where there are too few
@@ -1226,7 +1262,6 @@ __global__ void __launch_bounds__(256) paged_tile_merge_kernel(const PagedAttn p
 constexpr int kFewRows = 64;       // rows of a (sequence, kv head) pair up to which paged_few_kernel serves
 // its workgroups: as many as fit the CUs at once
 constexpr int kFewGrid = 512;
-constexpr int few_grid(int nt) { return nt == 4 ? kFewGrid / 2 : kFewGrid; }
 constexpr int kTileGrid = 512;     // of the tile kernel: two to a CU
 constexpr int kMaxPre = 64;        // key splits of the shared rows
 
@@ -1273,7 +1308,7 @@ PagedPlan make_plan(int Hq, int Hkv, int T, int B, int max_new, bool shared) {
   auto few = [&]() {
     const int64_t r = std::min<int64_t>(R, kFewRows);
     a.nt = r <= 16 ? 1 : r <= 32 ? 2 : 4;
-    parts((1 + static_cast<size_t>(B)) * sizeof(int), rows, static_cast<size_t>(few_grid(a.nt)) * 16 * a.nt);
+    parts((1 + static_cast<size_t>(B)) * sizeof(int), rows, static_cast<size_t>(kFewGrid) * 16 * a.nt);
   };
   auto tile = [&](int tile_rows) {
     a.rows = tile_rows;
@@ -1356,7 +1391,7 @@ extern "C" int bmx_attention_paged(const bmx_bf16* q, const bmx_paged_kv* cache,
                     batch->max_new, n_heads, Hkv, n_heads / Hkv, cache->n_pages, log2_of(cache->page_size), shared,
                     fabsf(scale) * kLog2e, scale < 0.0f ? 0x80008000u : 0u, reinterpret_cast<int*>(ws + a.plan),
                     part(a.row_o), part(a.row_ml), part(a.wg_o), part(a.wg_ml), part(a.pre_o), part(a.pre_ml), np, bps,
-                    a.most_items, a.most_cuts, a.rows};
+                    a.most_items, a.most_cuts, a.rows, a.nt == 4 ? 6 : 7};
   p.c2 = p.c2 < kLeast ? kLeast : p.c2;
   const hipStream_t st = as_stream(stream);
   if (shared) {
@@ -1373,15 +1408,16 @@ extern "C" int bmx_attention_paged(const bmx_bf16* q, const bmx_paged_kv* cache,
     const int rows = batch->max_new * p.rep;
     const dim3 merge(wide ? rows : (rows + 7) / 8, Hkv, B);
     auto launch = [&](auto few, auto joint, auto joint_wide) {
-      hipLaunchKernelGGL(few, dim3(few_grid(a.nt)), dim3(a.nt == 4 ? 512 : 256), 0, st, p);
+      hipLaunchKernelGGL(few, dim3(kFewGrid), dim3(256), a.nt == 4 ? kTileLds : 0, st, p);
       if (int rc = check_launch("attention_paged")) return rc;
       if (wide) hipLaunchKernelGGL(joint_wide, merge, dim3(256), 0, st, p);
       else hipLaunchKernelGGL(joint, merge, dim3(256), 0, st, p);
       return check_launch("attention_paged merge");
     };
-    if (a.nt == 1) return launch(paged_few_kernel<1, 1>, paged_few_merge_kernel<1, false>, paged_few_merge_kernel<1, true>);
-    if (a.nt == 2) return launch(paged_few_kernel<2, 1>, paged_few_merge_kernel<2, false>, paged_few_merge_kernel<2, true>);
-    return launch(paged_few_kernel<2, 2>, paged_few_merge_kernel<4, false>, paged_few_merge_kernel<4, true>);
+    if (a.nt == 1) return launch(paged_few_kernel<1>, paged_few_merge_kernel<1, false>, paged_few_merge_kernel<1, true>);
+    if (a.nt == 2) return launch(paged_few_kernel<2>, paged_few_merge_kernel<2, false>, paged_few_merge_kernel<2, true>);
+    if (int rc = allow_lds(paged_mid_kernel, kTileLds)) return rc;
+    return launch(paged_mid_kernel, paged_few_merge_kernel<4, false>, paged_few_merge_kernel<4, true>);
   }
   const auto kernel = a.rows == 256 ? paged_tile_kernel<8> : paged_tile_kernel<4>;
   if (int rc = allow_lds(kernel, kTileLds)) return rc;
