@@ -247,7 +247,8 @@ __device__ __forceinline__ bool next_share(const PagedAttn& p, int n, Share& s) 
 //     j's row l % 16 is value 8 (l % 16) + j: a lane ends with the outputs
 //     32 (l / 16) .. + 31 of its query.
 // The next step's K is requested when this step's scores are done, its V when
-// the values are turned.
+// the values are turned, also where the next step is another pair's: short
+// sequences wait for no first load but the workgroup's.
 // RG groups of 4 waves take 16 NT rows each over the same keys (64 rows by one
 // group needed more than 256 registers a wave: 36 us for 16 sequences of 5
 // tokens, against @@).
@@ -261,26 +262,93 @@ __global__ void __launch_bounds__(256, 2) paged_few_kernel(const PagedAttn p) {
   const MinusOne one = minus_one();
   Share at;
   if (!first_share(p, tmp, found, at)) return;
-  bool more_shares;
-  do {
-    const PagedSeq sq = at.sq;
-    const int b = at.b, h = at.h, j = at.j, nb = at.nb, n = min(at.t1 - at.t, nb - j);
-    // ---- the segment: blocks j .. j + n - 1 of (b, h) ----
-    const int R = min(sq.tokens, p.max_new) * p.rep;
-    const int cap = p.max_pages << p.shift;
-    const int end = min(sq.pos + min(sq.tokens, p.max_new), cap);  // rows < end are seen by some query
-    const int first = min(sq.pos + 1, cap);                         // rows < first by every query
-    const int* table = p.pages + static_cast<int64_t>(b) * p.max_pages;
-    int lim[NT];   // rows < lim are seen by the lane's query
-    uint4 qf[NT][4];
+  // What the loads of a pair's rows need
+  struct Where {
+    const int* table;
+    int h, c0, end;  // its kv head; the wave's keys of its first block; rows < end are seen by some query
+  };
+  auto where = [&](const Share& s) {
+    return Where{p.pages + static_cast<int64_t>(s.b) * p.max_pages, s.h, p.shared + s.j * kFewKeys + wave * 32,
+                 min(s.sq.pos + min(s.sq.tokens, p.max_new), p.max_pages << p.shift)};
+  };
+  uint4 kb[2][4], vw[8], qf[NT][4];
+  int64_t base[2];  // elements to the 16-key tiles' rows; -1: no such page
+  int pg[2];        // page numbers, asked for a step before the rows they lead to
+  auto ask = [&](const Where& w, int c0, int (&to)[2]) {
+#pragma unroll
+    for (int u = 0; u < 2; u++) to[u] = c0 + 16 * u < w.end ? w.table[(c0 + 16 * u) >> p.shift] : -1;
+  };
+  auto locate = [&](const Where& w, int c0, const int (&from)[2]) {
+#pragma unroll
+    for (int u = 0; u < 2; u++) {
+      const int at = uniform(from[u]), key = c0 + 16 * u;
+      base[u] = static_cast<unsigned>(at) < static_cast<unsigned>(p.n_pages)
+                    ? (((static_cast<int64_t>(at) * p.Hkv + w.h) << p.shift) + (key & ((1 << p.shift) - 1))) * kD
+                    : -1;
+    }
+  };
+  auto load_k = [&]() {
+#pragma unroll
+    for (int u = 0; u < 2; u++) {
+      const uint16_t* src = p.k + max(base[u], static_cast<int64_t>(0)) + li * kD + 8 * g;
+#pragma unroll
+      for (int ks = 0; ks < 4; ks++) kb[u][ks] = *reinterpret_cast<const uint4*>(src + 32 * ks);
+    }
+  };
+  auto load_v = [&]() {
+#pragma unroll
+    for (int e = 0; e < 8; e++)
+      vw[e] = *reinterpret_cast<const uint4*>(p.v + max(base[e >> 2], static_cast<int64_t>(0)) +
+                                              (4 * g + (e & 3)) * kD + 8 * li);
+  };
+  auto row_of = [&](const Share& s, int nt, int& tok, int& hd) {  // the lane's query row (past the last: that)
+    const int r = min(16 * nt + li, min(s.sq.tokens, p.max_new) * p.rep - 1);
+    tok = r / p.rep;
+    hd = s.h * p.rep + r - tok * p.rep;
+  };
+  auto load_q = [&](const Share& s) {
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
-      const int r = min(16 * nt + li, R - 1), tok = r / p.rep, hd = h * p.rep + r - tok * p.rep;
+      int tok, hd;
+      row_of(s, nt, tok, hd);
+      const uint16_t* src = p.q + (static_cast<int64_t>(hd) * p.T + s.sq.row0 + tok) * kD + 8 * g;
+#pragma unroll
+      for (int ks = 0; ks < 4; ks++) qf[nt][ks] = *reinterpret_cast<const uint4*>(src + 32 * ks);
+    }
+  };
+  Where now = where(at);
+  ask(now, now.c0, pg);
+  load_q(at);
+  locate(now, now.c0, pg);
+  ask(now, now.c0 + kFewKeys, pg);
+  load_k();
+  load_v();
+  bool more_shares;
+  do {
+    // ---- the segment: blocks j .. j + n - 1 of a pair ----
+    const PagedSeq sq = at.sq;
+    const int h = at.h, j = at.j, nb = at.nb, n = min(at.t1 - at.t, nb - j);
+    // the next one: its first rows are asked for in this one's last step
+    Share next = at;
+    more_shares = next_share(p, n, next);
+    Where then = now;
+    int first_pg[2] = {-1, -1};
+    if (more_shares) {
+      then = where(next);
+      ask(then, then.c0, first_pg);
+    }
+    const int R = min(sq.tokens, p.max_new) * p.rep;
+    const int cap = p.max_pages << p.shift, end = now.end;
+    const int first = min(sq.pos + 1, cap);  // rows < first are seen by every query
+    const int* table = now.table;
+    int lim[NT];   // rows < lim are seen by the lane's query
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++) {
+      int tok, hd;
+      row_of(at, nt, tok, hd);
       lim[nt] = min(sq.pos + tok + 1, cap);
-      const uint16_t* src = p.q + (static_cast<int64_t>(hd) * p.T + sq.row0 + tok) * kD + 8 * g;
 #pragma unroll
       for (int ks = 0; ks < 4; ks++) {
-        qf[nt][ks] = *reinterpret_cast<const uint4*>(src + 32 * ks);
         qf[nt][ks].x ^= p.flip;
         qf[nt][ks].y ^= p.flip;
         qf[nt][ks].z ^= p.flip;
@@ -296,44 +364,8 @@ __global__ void __launch_bounds__(256, 2) paged_few_kernel(const PagedAttn p) {
 #pragma unroll
       for (int d = 0; d < 8; d++) o[nt][d] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
     }
-    uint4 kb[2][4], vw[8];
-    int64_t base[2];  // elements to the 16-key tiles' rows; -1: no such page
-    // page numbers are asked for a step before the rows they lead to
-    int pg[2];
-    auto ask = [&](int c0) {
-#pragma unroll
-      for (int u = 0; u < 2; u++) pg[u] = c0 + 16 * u < end ? table[(c0 + 16 * u) >> p.shift] : -1;
-    };
-    auto locate = [&](int c0) {
-#pragma unroll
-      for (int u = 0; u < 2; u++) {
-        const int at = uniform(pg[u]), key = c0 + 16 * u;
-        base[u] = static_cast<unsigned>(at) < static_cast<unsigned>(p.n_pages)
-                      ? (((static_cast<int64_t>(at) * p.Hkv + h) << p.shift) + (key & ((1 << p.shift) - 1))) * kD
-                      : -1;
-      }
-    };
-    auto load_k = [&]() {
-#pragma unroll
-      for (int u = 0; u < 2; u++) {
-        const uint16_t* src = p.k + max(base[u], static_cast<int64_t>(0)) + li * kD + 8 * g;
-#pragma unroll
-        for (int ks = 0; ks < 4; ks++) kb[u][ks] = *reinterpret_cast<const uint4*>(src + 32 * ks);
-      }
-    };
-    auto load_v = [&]() {
-#pragma unroll
-      for (int e = 0; e < 8; e++)
-        vw[e] = *reinterpret_cast<const uint4*>(p.v + max(base[e >> 2], static_cast<int64_t>(0)) +
-                                                (4 * g + (e & 3)) * kD + 8 * li);
-    };
     bool odd = false;  // some value that is not finite was left out
-    int c0 = p.shared + j * kFewKeys + wave * 32;
-    ask(c0);
-    locate(c0);
-    ask(c0 + kFewKeys);
-    load_k();
-    load_v();
+    int c0 = now.c0;
     for (int s = 0; s < n; s++, c0 += kFewKeys) {
       const bool ok0 = base[0] >= 0, ok1 = base[1] >= 0;
       const bool whole = ok0 && ok1 && c0 + 32 <= first;  // every query sees every key
@@ -350,11 +382,15 @@ __global__ void __launch_bounds__(256, 2) paged_few_kernel(const PagedAttn p) {
                                                                 __builtin_bit_cast(bf16x8_t, qf[nt][ks]), sc[nt][u], 0,
                                                                 0, 0);
         }
-      const bool more = s + 1 < n;
-      if (more) {
-        locate(c0 + kFewKeys);
+      if (s + 1 < n) {
+        locate(now, c0 + kFewKeys, pg);
         load_k();
-        ask(c0 + 2 * kFewKeys);
+        ask(now, c0 + 2 * kFewKeys, pg);
+      } else if (more_shares) {
+        locate(then, then.c0, first_pg);
+        load_k();
+        load_q(next);
+        ask(then, then.c0 + kFewKeys, pg);
       }
       bf16x8_t hi[NT], lo[NT];
 #pragma unroll
@@ -424,7 +460,7 @@ __global__ void __launch_bounds__(256, 2) paged_few_kernel(const PagedAttn p) {
           }
         }
       }
-      if (more) load_v();
+      if (s + 1 < n || more_shares) load_v();
     }
     if (odd) {  // uniform
       const int k0 = p.shared + j * kFewKeys;
@@ -499,7 +535,8 @@ __global__ void __launch_bounds__(256, 2) paged_few_kernel(const PagedAttn p) {
       }
     }
     __syncthreads();  // (os, ms and ls are the next segment's)
-    more_shares = next_share(p, n, at);
+    at = next;
+    now = then;
   } while (more_shares);
 }
 
