@@ -674,7 +674,7 @@ class PagedKvCache(_Fixed):
             raise BmxError(BMX_E_SHAPE, f"k and v must be [n_pages, n_kv_heads, page_size, 128], got {tuple(k.shape)}, "
                                         f"{tuple(v.shape)}")
         _same_device(k, v)
-        self.k, self.v, self.device = k, v, k.device
+        self.k, self.v, self.device, self._index = k, v, k.device, k.get_device()
         self.n_pages, self.n_kv_heads, self.page_size = k.shape[:3]
         if max(k.shape) >= 1 << 31:
             raise BmxError(BMX_E_SHAPE, f"too large: {tuple(k.shape)}")
@@ -711,7 +711,7 @@ class PagedBatch(_Fixed):
         max_new = tokens if max_new is None else max_new
         if not 0 <= tokens < 1 << 31 or not min(tokens, 1) <= max_new <= tokens or max(pages.shape) >= 1 << 31:
             raise BmxError(BMX_E_SHAPE, f"tokens={tokens}, max_new={max_new}")
-        self.starts, self.lens, self.pages, self.device = starts, lens, pages, lens.device
+        self.starts, self.lens, self.pages, self.device, self._index = starts, lens, pages, lens.device, lens.get_device()
         self.n_seqs, self.max_pages, self.tokens, self.max_new = B, pages.shape[1], tokens, max_new
         self._struct = _BatchStruct(starts.data_ptr(), lens.data_ptr(), pages.data_ptr(), B, pages.shape[1], tokens,
                                     max_new)
@@ -734,14 +734,15 @@ class PagedBatch(_Fixed):
 
 
 def _paged_args(cache, batch, *ts):
+    # (a small call's time is the host's: three short questions to a tensor)
+    dev, bf16 = cache._index, _T.bfloat16
     for t in ts:
-        if not t.is_cuda or not t.is_contiguous():
+        if t.get_device() != dev or t.dtype is not bf16 or not t.is_contiguous():
             _require_cuda(t)
-        if t.device != cache.device:
-            raise BmxError(BMX_E_ARG, f"tensors on {cache.device} and {t.device}")
-    if batch.device != cache.device:
+            _same_device(cache.k, t)
+            _bf16(t)
+    if batch._index != dev:
         raise BmxError(BMX_E_ARG, f"the cache on {cache.device}, the batch on {batch.device}")
-    _bf16(*ts)
 
 
 def qk_norm_rope_paged(q, k, v, q_norm, k_norm, cache, batch, eps=1e-6, theta=1e6, out=None, stream=None):
@@ -753,15 +754,15 @@ def qk_norm_rope_paged(q, k, v, q_norm, k_norm, cache, batch, eps=1e-6, theta=1e
         with _T.cuda.device(cache.device):
             return qk_norm_rope_paged(q, k, v, q_norm, k_norm, cache, batch, eps, theta, out, stream)
     _paged_args(cache, batch, q, k, v, q_norm, k_norm)
-    T = batch.tokens
-    if q.dim() != 2 or q.shape[0] != T or q.shape[1] % 128 or k.shape != (T, cache.n_kv_heads * 128) or v.shape != k.shape:
-        raise BmxError(BMX_E_SHAPE, f"q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}: [{T}, Hq*128] and "
+    T, qs, ks = batch.tokens, q.shape, k.shape
+    if len(qs) != 2 or qs[0] != T or qs[1] % 128 or ks != (T, cache.n_kv_heads * 128) or v.shape != ks:
+        raise BmxError(BMX_E_SHAPE, f"q {tuple(qs)}, k {tuple(ks)}, v {tuple(v.shape)}: [{T}, Hq*128] and "
                                     f"[{T}, {cache.n_kv_heads}*128] expected")
     if q_norm.shape != (128,) or k_norm.shape != (128,):
         raise BmxError(BMX_E_SHAPE, "q_norm and k_norm must hold 128 weights")
-    Hq = q.shape[1] // 128
+    Hq = qs[1] // 128
     if out is None:
-        out = _empty(stream, cache.device, _T.bfloat16, Hq, T, 128)
+        out = q.new_empty((Hq, T, 128)) if stream is None else _empty(stream, cache.device, _T.bfloat16, Hq, T, 128)
     else:
         _paged_args(cache, batch, out)
         if out.shape != (Hq, T, 128):
@@ -802,15 +803,15 @@ def attention_paged(q, cache, batch, scale=None, shared=0, workspace=None, out=N
         with _T.cuda.device(cache.device):
             return attention_paged(q, cache, batch, scale, shared, workspace, out, stream)
     _paged_args(cache, batch, q)
-    T = batch.tokens
-    if q.dim() != 3 or q.shape[1:] != (T, 128) or q.shape[0] == 0 or q.shape[0] % cache.n_kv_heads:
+    T, qs = batch.tokens, q.shape
+    Hq = qs[0] if len(qs) == 3 else 0
+    if Hq == 0 or qs[1] != T or qs[2] != 128 or Hq % cache.n_kv_heads:
         raise BmxError(BMX_E_SHAPE, f"q must be [Hq, {T}, 128] with Hq a multiple of {cache.n_kv_heads}, got "
-                                    f"{tuple(q.shape)}")
-    Hq = q.shape[0]
+                                    f"{tuple(qs)}")
     if not 0 <= shared <= batch.max_pages * cache.page_size:
         raise BmxError(BMX_E_ARG, f"shared={shared}")
     if out is None:
-        out = _empty(stream, cache.device, _T.bfloat16, T, Hq * 128)
+        out = q.new_empty((T, Hq * 128)) if stream is None else _empty(stream, cache.device, _T.bfloat16, T, Hq * 128)
     else:
         _paged_args(cache, batch, out)
         if out.numel() != T * Hq * 128:
@@ -819,7 +820,7 @@ def attention_paged(q, cache, batch, scale=None, shared=0, workspace=None, out=N
         return out
     if workspace is None:
         workspace = attention_paged_workspace(Hq, cache.n_kv_heads, batch, shared, stream=stream)
-    else:
+    elif workspace.get_device() != cache._index or not workspace.is_contiguous():
         _require_cuda(workspace)
         _same_device(cache.k, workspace)
     call("bmx_attention_paged", q.data_ptr(), cache._ref, batch._ref, out.data_ptr(), Hq, 128, shared,
