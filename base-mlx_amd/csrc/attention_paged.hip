@@ -1225,10 +1225,13 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const PagedAtt
     sum += __shfl_xor(sum, o, 16);
     most = max(most, __shfl_xor(most, o, 16));
   }
-  // ---- pieces of at most `size` blocks: what each workgroup has to do on
-  // average, where that is less than the longest tile ----
-  // (tiles longer than that number at most per_head, and so do their further pieces)
-  const int size = min(max((sum + per_head - 1) / per_head, 4), most);
+  // ---- pieces of at most `size` blocks, half as many again as each workgroup
+  // has to do on average: each piece more is results to be written and joined (us
+  // with 1 / 1.25 / 1.5 / 2 times the average, or uncut: 1000 tokens over 3000 rows 120
+  // / 101 / 100 / 130 / 135; a chunk of 509 beside 31 single tokens 76 / 74 / 70 / 70 / 103;
+  // 64 over 30000 73 / 72 / 75 / 69 / 682) ----
+  // (tiles longer than the average number at most per_head, and so do their further pieces)
+  const int size = min(max((sum + per_head - 1) / per_head * 3 / 2, 4), most);
   const float to_bin = static_cast<float>(kPlanBins - 1) / static_cast<float>(size);
   auto bin_of = [&](int len) { return kPlanBins - 1 - min(static_cast<int>(len * to_bin), kPlanBins - 1); };
   auto cut = [&](int nb, int& len) {  // into pieces of len blocks (the last the rest)
