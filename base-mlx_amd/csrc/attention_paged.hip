@@ -1306,11 +1306,11 @@ constexpr int kTileGrid = 512;     // of the tile kernel: two to a CU
 constexpr int kMaxPre = 64;        // key splits of the shared rows
 
 // Rows of a tile.  256 stage and convert a block of keys once for twice the rows,
-// but leave a workgroup alone on its CU, with more of them idle in short
-// sequences (us with 128 / 256 rows: one prompt of 4096 tokens 187 / 173, six of
-// 1 to 2049 90 / 88; a chunk of 509 beside 31 single tokens 77 / 90; 160 and 64
-// single tokens over shared rows 161 / 164 and 41.4 / 43.1).
-int tile_rows(int rep, int T, int B) { return static_cast<int64_t>(T) * rep >= static_cast<int64_t>(B) * 1536 ? 256 : 128; }
+// but leave a workgroup alone on its CU, half as many tiles to balance, and more
+// of them idle in short sequences (us with 128 / 256 rows, 32 q heads over 8: one
+// prompt of 4096 tokens 190 / 176, 2048 over 2048 151 / 155, 512 26 / 30, six of 1 to
+// 2049 79 / 84; a chunk of 509 beside 31 single tokens 77 / 90).
+int tile_rows(int rep, int T, int B) { return static_cast<int64_t>(T) * rep >= static_cast<int64_t>(B) * 12288 ? 256 : 128; }
 
 struct PagedPlan {
   int few, nt;        // few: row tiles of 16

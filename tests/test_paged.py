@@ -118,7 +118,7 @@ def test_workspace_grows_with_the_batch():
 def test_workspace_never_shrinks():
     """More tokens, sequences or new tokens of one, and shared rows, need no less."""
     q = bmx.load().bmx_attention_paged_workspace_bytes
-    sizes = [1, 2, 7, 60, 95, 96, 97, 190, 191, 192, 193, 384, 385, 1000, 1535, 1536, 1537, 3000]
+    sizes = [1, 2, 7, 60, 96, 97, 191, 192, 193, 384, 385, 1000, 1536, 2900, 6143, 6144, 6145, 12287, 12289]
     for hq, hkv in ((32, 8), (8, 8), (64, 1)):
         for shared in (0, 1):
             for tokens in sizes:
