@@ -641,6 +641,9 @@ def kv4_evict(cache, weights, length, budget, sink=4, recent=0, into=None, weigh
 # ---------------------------------------------------------------------------
 # a paged KV cache for a batch of sequences
 # ---------------------------------------------------------------------------
+PAGED_COUNTER_BYTES = 524288  # BMX_PAGED_COUNTER_BYTES
+
+
 class _PagedKvStruct(ctypes.Structure):
     _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p)] + [
         (n, ctypes.c_int) for n in ("n_pages", "n_kv_heads", "page_size")]
@@ -777,8 +780,8 @@ def qk_norm_rope_paged(q, k, v, q_norm, k_norm, cache, batch, eps=1e-6, theta=1e
 def attention_paged_workspace(n_heads, n_kv_heads, batch, shared=0, device=None, stream=None):
     """A workspace for attention_paged calls of batches with up to as many
     tokens, sequences and new tokens of one as `batch` (a PagedBatch, or the
-    three as a tuple) has; shared: whether any has shared rows.  It serves one
-    call at a time."""
+    three as a tuple) has, its counters zeroed; shared: whether any has shared
+    rows.  It serves one call at a time."""
     torch = _torch()
     sizes = (batch.tokens, batch.n_seqs, batch.max_new) if isinstance(batch, PagedBatch) else tuple(batch)
     if device is None:
@@ -789,7 +792,9 @@ def attention_paged_workspace(n_heads, n_kv_heads, batch, shared=0, device=None,
     if not nbytes:
         raise BmxError(BMX_E_SHAPE, f"{n_heads} heads over {n_kv_heads}, (tokens, n_seqs, max_new) = {sizes}")
     with _on_stream(stream, device):
-        return torch.empty(nbytes, dtype=torch.uint8, device=device)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        ws[:PAGED_COUNTER_BYTES].zero_()
+    return ws
 
 
 def attention_paged(q, cache, batch, scale=None, shared=0, workspace=None, out=None, stream=None):

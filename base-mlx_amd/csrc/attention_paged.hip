@@ -75,7 +75,25 @@ struct PagedAttn {
   int most_items, most_cuts;  // of the plan's lists
   int tile_rows;      // 128 or 256
   int few_shift;      // of few rows: log2 of a block's keys
+  unsigned* cnt;      // arrivals of a pair's parts, kCounterStride apart, zero between calls; null: a launch joins them
 };
+
+// ---- parts that workgroups of one launch hand to one another ----
+// A pair's parts are written through to memory (agent-scope stores), which a
+// workgroup waits for before it counts its arrival; the last to arrive reads
+// them with agent-scope loads.  Nothing that an XCD's L2 holds from earlier is
+// read, and no L2 is flushed.  The counter wraps to zero with the last arrival.
+constexpr int kCounterStride = 16;  // words: a counter to a 64-byte piece of memory
+constexpr int kMaxCounters = BMX_PAGED_COUNTER_BYTES / (4 * kCounterStride);
+__device__ __forceinline__ void put2(float* to, float x, float y) {
+  __hip_atomic_store(reinterpret_cast<uint64_t*>(to),
+                     static_cast<uint64_t>(__float_as_uint(x)) | (static_cast<uint64_t>(__float_as_uint(y)) << 32),
+                     __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float2 get2(const float* from) {
+  const uint64_t v = __hip_atomic_load(reinterpret_cast<const uint64_t*>(from), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  return make_float2(__uint_as_float(static_cast<uint32_t>(v)), __uint_as_float(static_cast<uint32_t>(v >> 32)));
+}
 
 // 2^x; maxima of -inf (no key seen) count as 0
 __device__ __forceinline__ float finite_max(float m) { return m == -INFINITY ? 0.0f : m; }
@@ -177,22 +195,30 @@ __device__ __forceinline__ int few_blocks(const PagedAttn& p, const PagedSeq& s)
 // A workgroup's share of all pairs' blocks, [t, t1): a pair (sequence, kv head;
 // heads inner) and a block of it at a time.
 struct Share {
-  int t, t1, b, h, j, nb;
+  int t, t1, share, b, h, j, nb;
   PagedSeq sq;
 };
-// False where the share is empty.  tmp: 8 ints, found: 5.
-__device__ __forceinline__ bool first_share(const PagedAttn& p, int* tmp, int* found, Share& s) {
+// False where the share is empty.  *lone: whether any sequence has new tokens and
+// no block.  tmp: 8 ints, found: 5.
+__device__ __forceinline__ bool first_share(const PagedAttn& p, int* tmp, int* found, Share& s, bool* lone) {
   const int tid = threadIdx.x;
   const int per = (p.B + 255) >> 8, b0 = (tid & 255) * per;
   int mine = 0;
+  bool none = false;
   PagedSeq only{0, 0, 0};
   for (int i = 0; i < per && b0 + i < p.B; i++) {
     only = paged_seq(p.starts[b0 + i], p.starts[b0 + i + 1], p.lens[b0 + i], p.T);
-    mine += few_blocks(p, only);
+    const int n = few_blocks(p, only);
+    mine += n;
+    none = none || (only.tokens > 0 && n == 0);
   }
+  if ((tid & 63) == 0) tmp[4 + (tid >> 6 & 3)] = 0;
+  if (__any(none) && (tid & 63) == 0) tmp[4 + (tid >> 6 & 3)] = 1;
   int all;
   const int before = scan256(mine, tmp, &all);
+  *lone = (tmp[4] | tmp[5] | tmp[6] | tmp[7]) != 0;
   const int share = max(1, (p.Hkv * all + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x));
+  s.share = share;
   s.t = blockIdx.x * share;
   s.t1 = min(s.t + share, p.Hkv * all);
   if (blockIdx.x == 0 || (s.t < s.t1 && p.Hkv * before <= s.t && s.t < p.Hkv * (before + mine))) {
@@ -238,6 +264,66 @@ __device__ __forceinline__ bool next_share(const PagedAttn& p, int n, Share& s) 
   return true;
 }
 
+// A row's parts, folded one after another: 32 lanes per row, 4 values each.
+struct Fold {
+  float m = -INFINITY, l = 0.0f;
+  float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  __device__ __forceinline__ void add(const float2& ml, const float4& v) {
+    if (ml.x == -INFINITY) return;  // nothing seen
+    const float mn = fmaxf(m, ml.x);
+    const float wa = __builtin_amdgcn_exp2f(m - mn), wb = __builtin_amdgcn_exp2f(ml.x - mn);
+    l = l * wa + ml.y * wb;
+    a.x = a.x * wa + v.x * wb;
+    a.y = a.y * wa + v.y * wb;
+    a.z = a.z * wa + v.z * wb;
+    a.w = a.w * wa + v.w * wb;
+    m = mn;
+  }
+  // parts i0, i0 + by, ... < n, `step` rows apart, lane's values from d on, kB of
+  // them in flight; HANDED: written in this launch
+  template <bool HANDED, int kB>
+  __device__ __forceinline__ void add_batch(const float* o, const float* ml, int64_t step, int i0, int by, int n, int d) {
+    float2 mv[kB];
+    float4 ov[kB];
+#pragma unroll
+    for (int u = 0; u < kB; u++) {
+      const int64_t r = min(i0 + u * by, n - 1) * step;
+      if constexpr (HANDED) {
+        mv[u] = get2(ml + r * 2);
+        const float2 x = get2(o + r * kD + d), y = get2(o + r * kD + d + 2);
+        ov[u] = make_float4(x.x, x.y, y.x, y.y);
+      } else {
+        mv[u] = *reinterpret_cast<const float2*>(ml + r * 2);
+        ov[u] = *reinterpret_cast<const float4*>(o + r * kD + d);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kB; u++)
+      if (i0 + u * by < n) add(mv[u], ov[u]);
+  }
+  template <bool HANDED = false>
+  __device__ __forceinline__ void add_all(const float* o, const float* ml, int64_t step, int i0, int by, int n, int d) {
+    for (; i0 + 3 * by < n; i0 += 8 * by) add_batch<HANDED, 8>(o, ml, step, i0, by, n, d);
+    for (; i0 < n; i0 += 2 * by) add_batch<HANDED, 2>(o, ml, step, i0, by, n, d);
+  }
+  __device__ __forceinline__ void store(uint16_t* dst) const {
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    *reinterpret_cast<uint2*>(dst) =
+        make_uint2(pack2(a.x * inv, a.y * inv), pack2(a.z * inv, a.w * inv));
+  }
+};
+
+// Tokens of sequences without a block, which see nothing: zeros.  The workgroups
+// take sequences in turn.
+__device__ __forceinline__ void few_lone(const PagedAttn& p) {
+  for (int b = blockIdx.x; b < p.B; b += gridDim.x) {
+    const PagedSeq sq = paged_seq(p.starts[b], p.starts[b + 1], p.lens[b], p.T);
+    if (sq.tokens == 0 || few_blocks(p, sq) > 0) continue;
+    uint4* to = reinterpret_cast<uint4*>(p.out + static_cast<int64_t>(sq.row0) * p.Hq * kD);
+    for (int i = threadIdx.x; i < min(sq.tokens, p.max_new) * p.Hq * kD / 8; i += 256) to[i] = make_uint4(0, 0, 0, 0);
+  }
+}
+
 // Up to 16 query rows of a pair (NT = 1), in blocks of 128 keys.  Per wave and step of 32 keys, in two 16-key tiles:
 //   S^T = K Q^T (v_mfma_f32_16x16x32_bf16): lane l holds query row l % 16 and
 //     keys 4 (l / 16) + i of each tile;
@@ -261,7 +347,10 @@ __global__ void __launch_bounds__(256, 2) paged_few_kernel(const PagedAttn p) {
   const int tid = threadIdx.x, wave = uniform(tid >> 6), lane = tid & 63, li = lane & 15, g = lane >> 4;
   const MinusOne one = minus_one();
   Share at;
-  if (!first_share(p, tmp, found, at)) return;
+  bool lone;
+  const bool some = first_share(p, tmp, found, at, &lone);
+  if (NT == 1 && lone && p.cnt) few_lone(p);
+  if (!some) return;
   // What the loads of a pair's rows need
   struct Where {
     const int* table;
@@ -528,9 +617,50 @@ __global__ void __launch_bounds__(256, 2) paged_few_kernel(const PagedAttn p) {
         } else {
           const int64_t slot = j == 0 ? dst : static_cast<int64_t>(blockIdx.x) * (16 * NT) + r;
           float* po = (j == 0 ? p.row_o : p.wg_o) + slot * kD + d0;
+          float* pml = (j == 0 ? p.row_ml : p.wg_ml) + slot * 2;
+          if (NT == 1 && p.cnt) {
 #pragma unroll
-          for (int d = 0; d < kE; d += 4) *reinterpret_cast<float4*>(po + d) = make_float4(a[d], a[d + 1], a[d + 2], a[d + 3]);
-          if (d0 == 0) *reinterpret_cast<float2*>((j == 0 ? p.row_ml : p.wg_ml) + slot * 2) = make_float2(part_max(mm, ll), ll);
+            for (int d = 0; d < kE; d += 2) put2(po + d, a[d], a[d + 1]);
+            if (d0 == 0) put2(pml, part_max(mm, ll), ll);
+          } else {
+#pragma unroll
+            for (int d = 0; d < kE; d += 4) *reinterpret_cast<float4*>(po + d) = make_float4(a[d], a[d + 1], a[d + 2], a[d + 3]);
+            if (d0 == 0) *reinterpret_cast<float2*>(pml) = make_float2(part_max(mm, ll), ll);
+          }
+        }
+      }
+    }
+    if (NT == 1 && !direct && p.cnt) {
+      // ---- the last of the pair's workgroups to arrive folds its parts ----
+      const int u0 = at.t - j, w0 = u0 / at.share, parts = (u0 + nb - 1) / at.share - w0 + 1;
+      vm_wait<0>();  // this thread's part is in memory
+      __syncthreads();
+      if (tid == 0) {
+        unsigned* const c = p.cnt + (static_cast<int64_t>(at.b) * p.Hkv + h) * kCounterStride;
+        found[0] = __builtin_amdgcn_atomic_inc32(c, parts - 1, __ATOMIC_RELAXED, "agent") == static_cast<unsigned>(parts - 1);
+      }
+      __syncthreads();
+      if (uniform(found[0])) {
+        // 32 lanes to a row, or several times 32 where there are fewer rows than eight
+        const int by = R > 4 ? 1 : R > 2 ? 2 : R > 1 ? 4 : 8, sub = tid >> 5, ln = tid & 31, d = 4 * ln, i0 = sub % by;
+        for (int r = sub / by; r < (R + 7) / 8 * 8; r += 8 / by) {
+          Fold f;
+          const int rr = min(r, R - 1), tok = rr / p.rep;
+          const int64_t dst = static_cast<int64_t>(sq.row0 + tok) * p.Hq + h * p.rep + rr - tok * p.rep;
+          if (i0 == 0) f.add_batch<true, 1>(p.row_o + dst * kD, p.row_ml + dst * 2, 0, 0, 1, 1, d);
+          const int64_t first = static_cast<int64_t>(w0 + 1) * (16 * NT) + rr;
+          f.add_all<true>(p.wg_o + first * kD, p.wg_ml + first * 2, 16 * NT, i0, by, parts - 1, d);
+          if (by > 1) {  // (uniform: one turn)
+            float4* as = reinterpret_cast<float4*>(&os[0][0][0]);
+            float2* mls = reinterpret_cast<float2*>(&os[2][0][0]);
+            as[sub * 32 + ln] = f.a;
+            if (ln == 0) mls[sub] = make_float2(part_max(f.m, f.l), f.l);
+            __syncthreads();
+            f = Fold();
+            for (int u = 0; u < by; u++) f.add(mls[sub - i0 + u], as[(sub - i0 + u) * 32 + ln]);
+          }
+          if (i0 == 0 && r < R) f.store(p.out + dst * kD + d);
+          if (by > 1) break;
         }
       }
     }
@@ -539,45 +669,6 @@ __global__ void __launch_bounds__(256, 2) paged_few_kernel(const PagedAttn p) {
     now = then;
   } while (more_shares);
 }
-
-// A row's parts, folded one after another: 32 lanes per row, 4 values each.
-struct Fold {
-  float m = -INFINITY, l = 0.0f;
-  float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  __device__ __forceinline__ void add(const float2& ml, const float4& v) {
-    if (ml.x == -INFINITY) return;  // nothing seen
-    const float mn = fmaxf(m, ml.x);
-    const float wa = __builtin_amdgcn_exp2f(m - mn), wb = __builtin_amdgcn_exp2f(ml.x - mn);
-    l = l * wa + ml.y * wb;
-    a.x = a.x * wa + v.x * wb;
-    a.y = a.y * wa + v.y * wb;
-    a.z = a.z * wa + v.z * wb;
-    a.w = a.w * wa + v.w * wb;
-    m = mn;
-  }
-  // parts i0, i0 + by, ... < n, `step` rows apart, lane's values from d on
-  __device__ __forceinline__ void add_all(const float* o, const float* ml, int64_t step, int i0, int by, int n, int d) {
-    constexpr int kB = 8;  // in flight
-    for (; i0 < n; i0 += kB * by) {
-      float2 mv[kB];
-      float4 ov[kB];
-#pragma unroll
-      for (int u = 0; u < kB; u++) {
-        const int64_t r = min(i0 + u * by, n - 1) * step;
-        mv[u] = *reinterpret_cast<const float2*>(ml + r * 2);
-        ov[u] = *reinterpret_cast<const float4*>(o + r * kD + d);
-      }
-#pragma unroll
-      for (int u = 0; u < kB; u++)
-        if (i0 + u * by < n) add(mv[u], ov[u]);
-    }
-  }
-  __device__ __forceinline__ void store(uint16_t* dst) const {
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    *reinterpret_cast<uint2*>(dst) =
-        make_uint2(pack2(a.x * inv, a.y * inv), pack2(a.z * inv, a.w * inv));
-  }
-};
 
 // The rows of (sequence z, kv head y) that paged_few_kernel did not finish:
 // parts over the shared rows, the part that starts the pair's blocks, and one
@@ -1116,7 +1207,8 @@ __global__ void __launch_bounds__(256, 2) paged_mid_kernel(const PagedAttn p) {
   __shared__ int tmp[8];
   __shared__ int found[5];
   Share at;
-  if (!first_share(p, tmp, found, at)) return;
+  bool lone;
+  if (!first_share(p, tmp, found, at, &lone)) return;
   bool more;
   do {
     const int n = min(at.t1 - at.t, at.nb - at.j);
@@ -1337,7 +1429,7 @@ PagedPlan make_plan(int Hq, int Hkv, int T, int B, int max_new, bool shared) {
     return was;
   };
   auto parts = [&](size_t plan, size_t firsts, size_t others) {
-    at = 0;
+    at = BMX_PAGED_COUNTER_BYTES;
     a.plan = take(plan);
     a.row_ml = take(firsts * 2 * sizeof(float));
     a.row_o = take(firsts * kD * sizeof(float));
@@ -1436,7 +1528,7 @@ extern "C" int bmx_attention_paged(const bmx_bf16* q, const bmx_paged_kv* cache,
                     batch->max_new, n_heads, Hkv, n_heads / Hkv, cache->n_pages, log2_of(cache->page_size), shared,
                     fabsf(scale) * kLog2e, scale < 0.0f ? 0x80008000u : 0u, reinterpret_cast<int*>(ws + a.plan),
                     part(a.row_o), part(a.row_ml), part(a.wg_o), part(a.wg_ml), part(a.pre_o), part(a.pre_ml), np, bps,
-                    a.most_items, a.most_cuts, a.rows, a.nt == 4 ? 6 : 7};
+                    a.most_items, a.most_cuts, a.rows, a.nt == 4 ? 6 : 7, nullptr};
   p.c2 = p.c2 < kLeast ? kLeast : p.c2;
   const hipStream_t st = as_stream(stream);
   if (shared) {
@@ -1448,14 +1540,25 @@ extern "C" int bmx_attention_paged(const bmx_bf16* q, const bmx_paged_kv* cache,
     if (int rc = check_launch("attention_paged shared rows")) return rc;
   }
   if (a.few) {
+    // Where a pair's workgroups have few parts between them, they hand these to
+    // the last of them; a launch that spreads the rows over the card joins many.
+    // (Us, handed / launch: 160 sequences of 20 to 300 rows, 4 query rows a pair
+    // 20.9 / 24.7, 4 of 200 to 900 9.5 / 11.2, 64 of 500 to 8191 134 / 136; 1 of 4097,
+    // 33 parts a row 14.4 / 13.0; 4 with 28 query rows a pair 20.5 / 14.3; with
+    // parts over shared rows as well, 64 sequences 50 / 34.)
+    const int64_t pairs = static_cast<int64_t>(B) * Hkv;
+    const int64_t pieces = std::min<int64_t>(kFewGrid / pairs, (batch->max_pages * cache->page_size + kFewKeys - 1) / kFewKeys) + 1;
+    if (a.nt == 1 && !shared && pairs <= kMaxCounters && static_cast<int64_t>(batch->max_new) * p.rep * pieces <= 96)
+      p.cnt = reinterpret_cast<unsigned*>(ws);
     // (few rows have many parts each; us with 8 rows / 1 row to a workgroup: 64
-    // sequences of 32 rows over 4096 shared keys 35.1 / 41.2, 1 of 32 15.7 / 13.4)
+    // sequences, 32 rows each, over 4096 shared keys 35.1 / 41.2, 1 of 4097 15.7 / 13.4)
     const bool wide = static_cast<int64_t>(T) * n_heads <= 1024;
     const int rows = batch->max_new * p.rep;
     const dim3 merge(wide ? rows : (rows + 7) / 8, Hkv, B);
     auto launch = [&](auto few, auto joint, auto joint_wide) {
       hipLaunchKernelGGL(few, dim3(kFewGrid), dim3(256), a.nt == 4 ? kTileLds : 0, st, p);
       if (int rc = check_launch("attention_paged")) return rc;
+      if (p.cnt) return 0;
       if (wide) hipLaunchKernelGGL(joint_wide, merge, dim3(256), 0, st, p);
       else hipLaunchKernelGGL(joint, merge, dim3(256), 0, st, p);
       return check_launch("attention_paged merge");

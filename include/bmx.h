@@ -441,13 +441,15 @@ int bmx_qk_norm_rope_paged(const bmx_bf16 *q, const bmx_bf16 *k, const bmx_bf16 
  * it alone, whatever it holds; one that it sees with a value that is not
  * finite makes that dimension of its output not finite.  The order of every sum
  * is fixed by the shapes and the batch's arrays: equal calls give equal bits.
- * `workspace` (16-byte aligned device memory of
- * bmx_attention_paged_workspace_bytes or more, else BMX_E_ARG; any contents):
- * calls that share one must not run concurrently.  q, out: 16-byte aligned,
- * without overlap (BMX_E_ARG).  tokens = 0 or n_seqs = 0 is a no-op.
+ * `workspace`: 16-byte aligned device memory of
+ * bmx_attention_paged_workspace_bytes or more, else BMX_E_ARG; its first
+ * BMX_PAGED_COUNTER_BYTES zero-filled before its first use (every call leaves
+ * them zero); calls that share one must not run concurrently.  q, out: 16-byte
+ * aligned, without overlap (BMX_E_ARG).  tokens = 0 or n_seqs = 0 is a no-op.
  * Replaces: mlx_rs::fast::scaled_dot_product_attention as bmx_attention_gqa
  *   does (crates/base-mlx-core/src/model/qwen3.rs:491-518, 629-653), for a
  *   batch. */
+#define BMX_PAGED_COUNTER_BYTES 524288
 int bmx_attention_paged(const bmx_bf16 *q, const bmx_paged_kv *cache, const bmx_batch *batch, bmx_bf16 *out,
                         int n_heads, int head_dim, int shared, float scale, void *workspace, size_t workspace_bytes,
                         void *stream);

@@ -329,6 +329,23 @@ def test_rows_of_no_sequence_stay(gpu, new):
         hold(got[2:2 + T], want, bound)
 
 
+@pytest.mark.parametrize("hkv,seqs", [(4, 2048), (4, 2049), (2, 4096), (3, 4096)])
+@pytest.mark.parametrize("n", [1, 5])
+def test_many_sequences(gpu, hkv, seqs, n):
+    """As many pairs of sequences and kv heads as there are counters, and more; some
+    sequences empty, some long."""
+    new = [n if b % 7 else 0 for b in range(seqs)]
+    past = [(37 * b) % 50 + (3000 if b % 500 == 1 else 0) for b in range(seqs)]
+    q, cache, batch, lens, lists = case(21, (4 * hkv, hkv), 64, new, past)
+    got = bmx.attention_paged(q, cache, batch)
+    for b in (1, 2, 3, 499, 501, 1001, 1501, seqs - 2):
+        if new[b]:
+            at = sum(new[:b])
+            want, bound = attention_reference(q[:, at:at + n].contiguous(), cache.k, cache.v, [n], [lens[b]], [lists[b]],
+                                              1 / math.sqrt(D), half=False)
+            hold(got[at:at + n], want, bound, f"sequence {b}")
+
+
 @pytest.mark.parametrize("new,max_new", [([6, 2, 9], 4), ([60, 2, 90], 50)])
 def test_tokens_past_max_new_stay(gpu, new, max_new):
     q, cache, one, lens, lists = case(19, (8, 2), 16, new, [20, 3, 40])
@@ -370,8 +387,9 @@ def test_equal_calls_give_equal_bits(gpu, new, past, shared):
     ws = bmx.attention_paged_workspace(8, 2, batch, shared=shared)
     first = check(q, cache, batch, new, lens, lists, shared=shared, workspace=ws)
     for fill in (0, 255, 127):
-        ws.fill_(fill)  # any contents
+        ws[bmx.PAGED_COUNTER_BYTES:].fill_(fill)  # any contents
         assert torch.equal(bmx.attention_paged(q, cache, batch, shared=shared, workspace=ws), first)
+        assert not ws[:bmx.PAGED_COUNTER_BYTES].any()
 
 
 @pytest.mark.parametrize("new,shared", [([1, 1, 1, 0], 0), ([1, 1, 1, 0], 32), ([3, 2, 0, 60], 0), ([3, 2, 0, 60], 32)])
