@@ -198,9 +198,9 @@ struct Share {
   int t, t1, share, b, h, j, nb;
   PagedSeq sq;
 };
-// False where the share is empty.  *lone: whether any sequence has new tokens and
+// The share of workgroup wg of wgs; false where it is empty.  *lone: whether any sequence has new tokens and
 // no block.  tmp: 8 ints, found: 5.
-__device__ __forceinline__ bool first_share(const PagedAttn& p, int* tmp, int* found, Share& s, bool* lone) {
+__device__ __forceinline__ bool first_share(const PagedAttn& p, int wg, int wgs, int* tmp, int* found, Share& s, bool* lone) {
   const int tid = threadIdx.x;
   const int per = (p.B + 255) >> 8, b0 = (tid & 255) * per;
   int mine = 0;
@@ -217,16 +217,16 @@ __device__ __forceinline__ bool first_share(const PagedAttn& p, int* tmp, int* f
   int all;
   const int before = scan256(mine, tmp, &all);
   *lone = (tmp[4] | tmp[5] | tmp[6] | tmp[7]) != 0;
-  const int share = max(1, (p.Hkv * all + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x));
+  const int share = max(1, (p.Hkv * all + wgs - 1) / wgs);
   s.share = share;
-  s.t = blockIdx.x * share;
+  s.t = wg * share;
   s.t1 = min(s.t + share, p.Hkv * all);
-  if (blockIdx.x == 0 || (s.t < s.t1 && p.Hkv * before <= s.t && s.t < p.Hkv * (before + mine))) {
+  if (wg == 0 || (s.t < s.t1 && p.Hkv * before <= s.t && s.t < p.Hkv * (before + mine))) {
     int at = before;
     for (int i = 0; i < per && b0 + i < p.B; i++) {
       const PagedSeq q = per == 1 ? only : paged_seq(p.starts[b0 + i], p.starts[b0 + i + 1], p.lens[b0 + i], p.T);
       const int n = few_blocks(p, q);
-      if (blockIdx.x == 0) p.plan[1 + b0 + i] = at;
+      if (wg == 0) p.plan[1 + b0 + i] = at;
       if (p.Hkv * at <= s.t && s.t < p.Hkv * (at + n)) {
         found[0] = b0 + i;
         found[1] = at;
@@ -236,7 +236,7 @@ __device__ __forceinline__ bool first_share(const PagedAttn& p, int* tmp, int* f
       }
       at += n;
     }
-    if (blockIdx.x == 0 && tid == 0) p.plan[0] = share;
+    if (wg == 0 && tid == 0) p.plan[0] = share;
   }
   __syncthreads();
   if (s.t >= s.t1) return false;
@@ -338,17 +338,23 @@ __device__ __forceinline__ void few_lone(const PagedAttn& p) {
 // RG groups of 4 waves take 16 NT rows each over the same keys (64 rows by one
 // group needed more than 256 registers a wave: 36 us for 16 sequences of 5
 // tokens, against @@).
+struct FewLds {
+  float os[4][16][kFewOs];
+  float ms[4][32], ls[4][32];
+  int tmp[8], found[5];
+};
 template <int NT>
-__global__ void __launch_bounds__(256, 2) paged_few_kernel(const PagedAttn p) {
-  __shared__ int tmp[8];
-  __shared__ int found[5];
-  __shared__ __align__(16) float os[4][16][kFewOs];
-  __shared__ float ms[4][16 * NT], ls[4][16 * NT];
+__device__ __forceinline__ void few_run(const PagedAttn& p, FewLds& lds, int wg, int wgs) {
+  static_assert(NT <= 2);
+  auto& os = lds.os;
+  auto& ms = lds.ms;
+  auto& ls = lds.ls;
+  int* const found = lds.found;
   const int tid = threadIdx.x, wave = uniform(tid >> 6), lane = tid & 63, li = lane & 15, g = lane >> 4;
   const MinusOne one = minus_one();
   Share at;
   bool lone;
-  const bool some = first_share(p, tmp, found, at, &lone);
+  const bool some = first_share(p, wg, wgs, lds.tmp, found, at, &lone);
   if (NT == 1 && lone && p.cnt) few_lone(p);
   if (!some) return;
   // What the loads of a pair's rows need
@@ -615,7 +621,7 @@ __global__ void __launch_bounds__(256, 2) paged_few_kernel(const PagedAttn p) {
             *reinterpret_cast<uint2*>(p.out + dst * kD + d0 + d) =
                 make_uint2(pack2(a[d] * inv, a[d + 1] * inv), pack2(a[d + 2] * inv, a[d + 3] * inv));
         } else {
-          const int64_t slot = j == 0 ? dst : static_cast<int64_t>(blockIdx.x) * (16 * NT) + r;
+          const int64_t slot = j == 0 ? dst : static_cast<int64_t>(wg) * (16 * NT) + r;
           float* po = (j == 0 ? p.row_o : p.wg_o) + slot * kD + d0;
           float* pml = (j == 0 ? p.row_ml : p.wg_ml) + slot * 2;
           if (NT == 1 && p.cnt) {
@@ -668,6 +674,12 @@ __global__ void __launch_bounds__(256, 2) paged_few_kernel(const PagedAttn p) {
     at = next;
     now = then;
   } while (more_shares);
+}
+
+template <int NT>
+__global__ void __launch_bounds__(256, 2) paged_few_kernel(const PagedAttn p) {
+  __shared__ __align__(16) FewLds lds;
+  few_run<NT>(p, lds, blockIdx.x, gridDim.x);
 }
 
 // The rows of (sequence z, kv head y) that paged_few_kernel did not finish:
@@ -1170,14 +1182,21 @@ __device__ __forceinline__ void tile_run(const PagedAttn& p, char* lds, const Pa
     tile_try<PRE, false, NW, WK>(p, lds, sq, b, h, r0, j0, j1, to);
 }
 
-// The shared rows: grid (kv heads, row tiles, key splits).
+// Key split z of 128- (NW = 8: 256-) row tile i of all the batch's rows, over the
+// shared rows
+template <int NW>
+__device__ __forceinline__ void prefix_run(const PagedAttn& p, char* lds, int h, int i, int z) {
+  const int nb = (p.shared + kTileKeys - 1) / kTileKeys, j0 = z * p.pre_bps;
+  const int64_t slot = static_cast<int64_t>(z) * p.T * p.Hq;
+  tile_run<true, NW, 1>(p, lds, PagedSeq{0, p.T, 0}, 0, h, i * (32 * NW), j0, min(j0 + p.pre_bps, nb),
+                        Result{p.pre_o + slot * kD, p.pre_ml + slot * 2, true});
+}
+
+// Grid (kv heads, row tiles, key splits).
 template <int NW>
 __global__ void __launch_bounds__(64 * NW, 2) paged_prefix_kernel(const PagedAttn p) {
   extern __shared__ __align__(256) char lds[];  // (a row's 256 bytes: the addresses are made by exclusive or)
-  const int nb = (p.shared + kTileKeys - 1) / kTileKeys, j0 = blockIdx.z * p.pre_bps;
-  const int64_t slot = static_cast<int64_t>(blockIdx.z) * p.T * p.Hq;
-  tile_run<true, NW, 1>(p, lds, PagedSeq{0, p.T, 0}, 0, blockIdx.x, blockIdx.y * (32 * NW), j0, min(j0 + p.pre_bps, nb),
-                    Result{p.pre_o + slot * kD, p.pre_ml + slot * 2, true});
+  prefix_run<NW>(p, lds, blockIdx.x, blockIdx.y, blockIdx.z);
 }
 
 // The plan's items, longest first: kv head blockIdx % Hkv, items a, 2A-1-a,
@@ -1199,25 +1218,45 @@ __global__ void __launch_bounds__(64 * NW, 2) paged_tile_kernel(const PagedAttn 
   }
 }
 
-// Up to 64 query rows of a pair, in blocks of 64 keys by shares as
-// paged_few_kernel: two row groups of waves, each by two waves that take half of
-// a block's keys.
-__global__ void __launch_bounds__(256, 2) paged_mid_kernel(const PagedAttn p) {
-  extern __shared__ __align__(256) char lds[];  // (a row's 256 bytes: the addresses are made by exclusive or)
-  __shared__ int tmp[8];
-  __shared__ int found[5];
+// Up to 64 query rows of a pair, in blocks of 64 keys by shares as few_run: two
+// row groups of waves, each by two waves that take half of a block's keys.
+__device__ __forceinline__ void mid_run(const PagedAttn& p, char* lds, int wg, int wgs) {
+  int* const tmp = reinterpret_cast<int*>(lds + kTileLds);
   Share at;
   bool lone;
-  if (!first_share(p, tmp, found, at, &lone)) return;
+  if (!first_share(p, wg, wgs, tmp, tmp + 8, at, &lone)) return;
   bool more;
   do {
     const int n = min(at.t1 - at.t, at.nb - at.j);
-    const int64_t slot = static_cast<int64_t>(blockIdx.x) * 64;
+    const int64_t slot = static_cast<int64_t>(wg) * 64;
     Result to{nullptr, nullptr, false};
     if (n < at.nb || p.shared) to = at.j == 0 ? Result{p.row_o, p.row_ml, true} : Result{p.wg_o + slot * kD, p.wg_ml + slot * 2, false};
     tile_run<false, 4, 2>(p, lds, at.sq, at.b, at.h, 0, at.j, at.j + n, to);
     more = next_share(p, n, at);
   } while (more);
+}
+constexpr size_t kMidLds = kTileLds + 16 * sizeof(int);
+
+__global__ void __launch_bounds__(256, 2) paged_mid_kernel(const PagedAttn p) {
+  extern __shared__ __align__(256) char lds[];
+  mid_run(p, lds, blockIdx.x, gridDim.x);
+}
+
+// The shared rows (the first `pre` workgroups: kv heads x row tiles x key splits)
+// and the sequences' own by shares (NT = 4: mid_run) in one launch: neither waits
+// for the other's last workgroups.
+template <int NT>
+__global__ void __launch_bounds__(256, 2) paged_shared_kernel(const PagedAttn p, int pre) {
+  extern __shared__ __align__(256) char lds[];
+  const int wg = static_cast<int>(blockIdx.x) - pre, wgs = static_cast<int>(gridDim.x) - pre;
+  if (wg < 0) {
+    const int i = blockIdx.x / p.Hkv;
+    prefix_run<4>(p, lds, blockIdx.x % p.Hkv, i / p.np, i % p.np);
+  } else if constexpr (NT == 4) {
+    mid_run(p, lds, wg, wgs);
+  } else {
+    few_run<NT>(p, *reinterpret_cast<FewLds*>(lds), wg, wgs);
+  }
 }
 
 // One workgroup lists the tiles of all sequences, cut where there are too few
@@ -1531,14 +1570,7 @@ extern "C" int bmx_attention_paged(const bmx_bf16* q, const bmx_paged_kv* cache,
                     a.most_items, a.most_cuts, a.rows, a.nt == 4 ? 6 : 7, nullptr};
   p.c2 = p.c2 < kLeast ? kLeast : p.c2;
   const hipStream_t st = as_stream(stream);
-  if (shared) {
-        const int tiles = static_cast<int>(a.all);
-    const auto kernel = a.rows == 256 ? paged_prefix_kernel<8> : paged_prefix_kernel<4>;
-    if (a.all > 65535) return set_error(BMX_E_SHAPE, "attention_paged: tokens=%d too many for shared rows", T);
-    if (int rc = allow_lds(kernel, kTileLds)) return rc;
-    hipLaunchKernelGGL(kernel, dim3(Hkv, tiles, np), dim3(2 * a.rows), kTileLds, st, p);
-    if (int rc = check_launch("attention_paged shared rows")) return rc;
-  }
+  if (shared && a.all > 65535) return set_error(BMX_E_SHAPE, "attention_paged: tokens=%d too many for shared rows", T);
   if (a.few) {
     // Where a pair's workgroups have few parts between them, they hand these to
     // the last of them; a launch that spreads the rows over the card joins many.
@@ -1555,18 +1587,27 @@ extern "C" int bmx_attention_paged(const bmx_bf16* q, const bmx_paged_kv* cache,
     const bool wide = static_cast<int64_t>(T) * n_heads <= 1024;
     const int rows = batch->max_new * p.rep;
     const dim3 merge(wide ? rows : (rows + 7) / 8, Hkv, B);
-    auto launch = [&](auto few, auto joint, auto joint_wide) {
-      hipLaunchKernelGGL(few, dim3(kFewGrid), dim3(256), a.nt == 4 ? kTileLds : 0, st, p);
+    auto launch = [&](auto few, auto with_shared, auto joint, auto joint_wide) {
+      const size_t lds = shared || a.nt == 4 ? kMidLds : 0;
+      if (int rc = shared ? allow_lds(with_shared, lds) : allow_lds(few, lds)) return rc;
+      const int pre = shared ? Hkv * static_cast<int>(a.all) * np : 0;
+      if (shared) hipLaunchKernelGGL(with_shared, dim3(pre + kFewGrid), dim3(256), lds, st, p, pre);
+      else hipLaunchKernelGGL(few, dim3(kFewGrid), dim3(256), lds, st, p);
       if (int rc = check_launch("attention_paged")) return rc;
       if (p.cnt) return 0;
       if (wide) hipLaunchKernelGGL(joint_wide, merge, dim3(256), 0, st, p);
       else hipLaunchKernelGGL(joint, merge, dim3(256), 0, st, p);
       return check_launch("attention_paged merge");
     };
-    if (a.nt == 1) return launch(paged_few_kernel<1>, paged_few_merge_kernel<1, false>, paged_few_merge_kernel<1, true>);
-    if (a.nt == 2) return launch(paged_few_kernel<2>, paged_few_merge_kernel<2, false>, paged_few_merge_kernel<2, true>);
-    if (int rc = allow_lds(paged_mid_kernel, kTileLds)) return rc;
-    return launch(paged_mid_kernel, paged_few_merge_kernel<4, false>, paged_few_merge_kernel<4, true>);
+    if (a.nt == 1) return launch(paged_few_kernel<1>, paged_shared_kernel<1>, paged_few_merge_kernel<1, false>, paged_few_merge_kernel<1, true>);
+    if (a.nt == 2) return launch(paged_few_kernel<2>, paged_shared_kernel<2>, paged_few_merge_kernel<2, false>, paged_few_merge_kernel<2, true>);
+    return launch(paged_mid_kernel, paged_shared_kernel<4>, paged_few_merge_kernel<4, false>, paged_few_merge_kernel<4, true>);
+  }
+  if (shared) {
+    const auto kernel = a.rows == 256 ? paged_prefix_kernel<8> : paged_prefix_kernel<4>;
+    if (int rc = allow_lds(kernel, kTileLds)) return rc;
+    hipLaunchKernelGGL(kernel, dim3(Hkv, static_cast<unsigned>(a.all), np), dim3(2 * a.rows), kTileLds, st, p);
+    if (int rc = check_launch("attention_paged shared rows")) return rc;
   }
   const auto kernel = a.rows == 256 ? paged_tile_kernel<8> : paged_tile_kernel<4>;
   if (int rc = allow_lds(kernel, kTileLds)) return rc;
