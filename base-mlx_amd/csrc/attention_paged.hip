@@ -725,8 +725,8 @@ __global__ void __launch_bounds__(256) paged_few_merge_kernel(const PagedAttn p)
 // ===========================================================================
 constexpr int kTileKeys = 64;  // of a block
 constexpr int kTileBytes = kTileKeys * kD * 2;  // of a K or V tile
-// K and V, two of each; which waves' rows of the two blocks exist; a flag
-constexpr size_t kTileLds = 4 * kTileBytes + (2 * 8 + 1) * sizeof(int);
+// K and V, two of each; which waves' rows of the two blocks exist; a flag of each wave
+constexpr size_t kTileLds = 4 * kTileBytes + 3 * 8 * sizeof(int);
 
 // A piece of work: rows r0 .. of sequence b, 64-key blocks [j0, j1), and the
 // slot that takes its result (-1: it is the whole of it).
@@ -789,7 +789,7 @@ __device__ __forceinline__ bool tile_try(const PagedAttn& p, char* lds, const Pa
   const int tid = threadIdx.x, wave = uniform(tid >> 6), lane = tid & 63, j = lane & 31, hf = lane >> 5;
   const int wr = wave % WR, wk = wave / WR;
   int* exist = reinterpret_cast<int*>(lds + 4 * kTileBytes);  // [2][NW]
-  int* left_out = exist + 2 * NW;  // some value that is not finite was left out
+  int* left_out = exist + 2 * NW;  // [NW]: of a wave's rows, some value that is not finite was left out
   const MinusOne one = minus_one();
   const int cap = p.max_pages << p.shift;
   const int tokens = PRE ? p.T : min(sq.tokens, p.max_new);
@@ -843,7 +843,7 @@ __device__ __forceinline__ bool tile_try(const PagedAttn& p, char* lds, const Pa
     const uint32_t dst = uniform(lds_offset(lds) + buf * 2 * kTileBytes + wave * kOwn * 256);
     uint32_t v0 = voff0;
     asm volatile("" : "+v"(v0));
-    const uint32_t voff[4] = {v0, v0 ^ (1024 | 16), v0 ^ (2048 | 32), v0 ^ (3072 | 48)};  // + 4 i rows
+    const uint32_t voff[4] = {v0, v0 ^ (1024 | 16), v0 ^ (2048 | 32), v0 ^ (3 * 1024 | 48)};  // + 4 i rows
     if (ok && k0 + kOwn <= end) {  // uniform
 #pragma unroll
       for (int i = 0; i < kOwn / 4; i++) {
@@ -880,7 +880,7 @@ __device__ __forceinline__ bool tile_try(const PagedAttn& p, char* lds, const Pa
         w[i] = make_uint4(finite_part(w[i].x), finite_part(w[i].y), finite_part(w[i].z), finite_part(w[i].w));
       }
       changed = __any(nf != 0);
-      if (changed && lane == 0) *left_out = 1;
+      if (changed && lane == 0) left_out[wave] = 1;
     }
     if constexpr (HALF) {
       // of the lane's 8 values of a row the largest magnitude, as bits: 0, or
@@ -1069,7 +1069,7 @@ __device__ __forceinline__ bool tile_try(const PagedAttn& p, char* lds, const Pa
     l += sum;
   };
   __syncthreads();  // (an earlier piece's reads of LDS are over)
-  if (tid == 0) *left_out = 0;
+  if (lane == 0) left_out[wave] = 0;  // (each wave its own, which it alone sets)
   if (j0 < j1) {
     ask(j0);
     stage(j0, 0);
@@ -1104,7 +1104,10 @@ __device__ __forceinline__ bool tile_try(const PagedAttn& p, char* lds, const Pa
   }
   l = add_xor32(l);
   if constexpr (!PRE) {
-    if (j0 < j1 && uniform(*left_out)) {  // (the last block's barriers lie behind)
+    int odd = 0;  // (the last block was settled before its barrier)
+#pragma unroll
+    for (int w = 0; w < NW; w++) odd |= left_out[w];
+    if (j0 < j1 && uniform(odd)) {
       for (int key = key0 + max(j0 * kTileKeys, (first - key0) & ~(kTileKeys - 1)); key < min(key0 + j1 * kTileKeys, end); key++) {
         const int64_t at = row_at(p, table, h, key);
         if (at < 0 || key >= lim) continue;
