@@ -1552,10 +1552,14 @@ extern "C" int bmx_attention_paged(const bmx_bf16* q, const bmx_paged_kv* cache,
   if (paged_overlap(q, bytes, out, bytes)) return set_error(BMX_E_ARG, "attention_paged: out overlaps q");
   if (B == 1) shared = 0;  // (one sequence shares with nobody)
   // (blocks of all pairs are counted in an int)
-  if (static_cast<int64_t>(B) * Hkv * ((static_cast<int64_t>(batch->max_pages) * cache->page_size + 63) / 64) > (1 << 30))
+  const int64_t blocks = (static_cast<int64_t>(batch->max_pages) * cache->page_size + 63) / 64;
+  if (B * Hkv * blocks > (1 << 30))
     return set_error(BMX_E_SHAPE, "attention_paged: %d sequences of up to %d pages, %d kv heads: too many", B,
                      batch->max_pages, Hkv);
   const PagedPlan a = make_plan(n_heads, Hkv, T, B, batch->max_new, shared > 0);
+  // (and so are those of all tiles)
+  if (!a.few && (a.all + std::min(B, T)) * blocks > (1 << 30))
+    return set_error(BMX_E_SHAPE, "attention_paged: %d tokens over up to %d pages: too many", T, batch->max_pages);
   if (workspace_bytes < a.bytes)
     return set_error(BMX_E_ARG, "attention_paged: workspace of %zu bytes, %zu needed", workspace_bytes, a.bytes);
   char* ws = static_cast<char*>(workspace);

@@ -90,6 +90,9 @@ def test_attention_refusals():
     # more blocks of keys than an int counts
     assert attend(kv(n_kv_heads=1024), batch(n_seqs=4096, max_pages=1 << 20, tokens=4096, max_new=1), Hq=1024,
                   q=20 * P, out=40 * P) == bmx.BMX_E_SHAPE
+    # ... and of prompts, by all their tiles: 2^20 of 256 rows, 2^18 blocks each
+    assert attend(kv(n_kv_heads=1), batch(n_seqs=1, max_pages=1 << 20, tokens=1 << 23, max_new=1 << 23), Hq=32, q=1 << 40,
+                  out=1 << 42, wsb=1 << 45) == bmx.BMX_E_SHAPE and "too many" in bmx.last_error()
 
 
 def test_workspace_query_refuses_what_the_call_refuses():
