@@ -29,8 +29,8 @@ struct PagedSeq {
 __device__ __forceinline__ PagedSeq paged_seq(int s0, int s1, int len, int T) {
   s0 = min(max(s0, 0), T);
   s1 = min(max(s1, s0), T);
-  // (positions below -T or above the table are all the same: of no row)
-  return PagedSeq{s0, s1 - s0, min(max(len, 0), kPagedMaxRows) - (s1 - s0)};
+  // (positions below -T, and from the largest table's end on, are all the same: of no row)
+  return PagedSeq{s0, s1 - s0, min(max(len, 0), kPagedMaxRows + T) - (s1 - s0)};
 }
 
 }  // namespace bmx

@@ -119,6 +119,29 @@ def test_append_far_positions(gpu, theta):
     check_append((4, 2), cache, bmx.PagedBatch.of(new, lens, lists), new, lens, lists, *projections(9, (4, 2), 7), theta=theta)
 
 
+@pytest.mark.parametrize("len0", [(1 << 24) + 2, (1 << 24) + 300, 2 ** 31 - 1])
+@pytest.mark.parametrize("new", [[5, 1], [60, 1], [300, 1]])
+def test_lengths_past_the_largest_table(gpu, len0, new):
+    """Of a table of 2^24 rows: what lies past it is not written, and sees all that is there."""
+    heads, lens = (4, 2), [len0, 40]
+    lists = [[-1] * 4095 + [1], [0] + [-1] * 4095]
+    cache = cache_of(33, 2, 2, 4096)
+    x = projections(34, heads, sum(new))
+    batch = bmx.PagedBatch.of(new, lens, lists)
+    before = cache.k.clone(), cache.v.clone()
+    q = bmx.qk_norm_rope_paged(*x, cache, batch)
+    inside = max(0, (1 << 24) - (len0 - new[0]))  # tokens with a row
+    assert torch.equal(cache.v[1, :, 4096 - inside:], x[2][:inside].view(inside, 2, D).transpose(0, 1))
+    cache.k[1, :, 4096 - inside:], cache.v[1, :, 4096 - inside:] = (y[1, :, 4096 - inside:] for y in before)
+    assert torch.equal(cache.k[1], before[0][1]) and torch.equal(cache.v[1], before[1][1])
+    got = bmx.attention_paged(q, cache, batch)
+    # the same rows as a short sequence's
+    cut = [4096 + max(0, len0 - (1 << 24)), 40]
+    short = [[1], [0]]
+    want, bound = attention_reference(q, cache.k, cache.v, new, cut, short, 1 / math.sqrt(D), cap=4096)
+    hold(got, want, bound)
+
+
 def test_append_without_a_page(gpu):
     """Page numbers that do not exist, positions outside the table: no cache row, the queries all the same."""
     heads, new = (4, 2), [3, 2, 2, 1]
