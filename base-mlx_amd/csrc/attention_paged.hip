@@ -38,6 +38,7 @@ constexpr int kD = kPagedDim;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLazy = 8.0f;  // log2 by which a maximum may lag
 constexpr float kUp = 7.0f;    // log2 by which fp16 probabilities are scaled up: the largest, with kLazy, are 2^15
+constexpr int kValueUp = 8;     // log2 by which values are scaled up on their way to fp16
 constexpr float kLeast = 1.17549435e-38f;  // of c: a scale of 0 leaves a hidden key's -inf what it is
 
 typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8_t;
@@ -861,8 +862,10 @@ __device__ __forceinline__ bool tile_try(const PagedAttn& p, char* lds, const Pa
     }
   };
   // ... and what is done to the wave's 16 rows of V once they are there: values
-  // to fp16 where that loses nothing (quarter 1), else left as bf16 (quarter 2);
-  // in blocks that only some queries see whole, values that are not finite to 0
+  // to fp16, times 2^kValueUp; in blocks that only some queries see whole, values
+  // that are not finite to 0.  fp16 holds a bf16 value from 2^-25 up as it is and a
+  // smaller one to 2^-32: where some value is 2^8 or more, or eight neighbours are
+  // all below 2^-20, the rows are left for the tile's second try, in bf16.
   auto settle = [&](int jb, int buf) {
     const int k0 = key0 + jb * kTileKeys;
     const bool mixed = !PRE && k0 + kTileKeys > first && first < end;  // (uniform)
@@ -884,7 +887,7 @@ __device__ __forceinline__ bool tile_try(const PagedAttn& p, char* lds, const Pa
     }
     if constexpr (HALF) {
       // of the lane's 8 values of a row the largest magnitude, as bits: 0, or
-      // from 2^-12 to below 2^16
+      // from 2^-20 to below 2^8
       uint32_t top = 0, low = ~0u;
 #pragma unroll
       for (int i = 0; i < kOwn / 4; i++) {
@@ -895,13 +898,14 @@ __device__ __forceinline__ bool tile_try(const PagedAttn& p, char* lds, const Pa
         top = max(top, t);
         low = min(low, t - 1u);  // (0 wraps to the largest)
       }
-      if (__any(top >= 0x4780u || low < 0x3980u - 1u)) {
+      if (__any(top >= ((127u + 16u - kValueUp) << 7) || low < ((127u - 12u - kValueUp) << 7) - 1u)) {
         if (lane == 0) exist[NW * buf + wave] = 2;
         return;
       }
 #pragma unroll
       for (int i = 0; i < kOwn / 4; i++) {
         auto h2 = [](uint32_t x) {
+          x += kValueUp * 0x00800080u;  // (a pair's exponents; 0 stays below fp16's smallest)
           return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(__uint_as_float(x << 16),
                                                                          __uint_as_float(x & 0xffff0000u)));
         };
@@ -1151,10 +1155,11 @@ __device__ __forceinline__ bool tile_try(const PagedAttn& p, char* lds, const Pa
       for (int r = 0; r < 4; r++) o[i >> 2][4 * (i & 3) + r] = o[i >> 2][4 * (i & 3) + r] * wa + v[r] * wb;
     }
   }
+  constexpr float kDown = HALF ? 1.0f / (1 << kValueUp) : 1.0f;
   auto finish = [&]() {
   const int64_t row = static_cast<int64_t>(sq.row0 + tok) * p.Hq + hd;
   if (!to.o) {
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    const float inv = l == 0.0f ? 0.0f : kDown / l;
     uint16_t* dst = p.out + row * kD + 4 * hf;
 #pragma unroll
     for (int dt = 0; dt < 4; dt++)
@@ -1174,7 +1179,7 @@ __device__ __forceinline__ bool tile_try(const PagedAttn& p, char* lds, const Pa
 #pragma unroll
     for (int r4 = 0; r4 < 4; r4++)
       *reinterpret_cast<float4*>(dst + 32 * dt + 8 * r4) =
-          make_float4(o[dt][4 * r4], o[dt][4 * r4 + 1], o[dt][4 * r4 + 2], o[dt][4 * r4 + 3]);
+          make_float4(o[dt][4 * r4] * kDown, o[dt][4 * r4 + 1] * kDown, o[dt][4 * r4 + 2] * kDown, o[dt][4 * r4 + 3] * kDown);
   };
   if (rw + j < R) finish();
   return true;

@@ -50,8 +50,8 @@ def attention_reference(q, k, v, new, lens, tables, scale, shared=0, cap=None, h
     Weights are held in two bf16 pieces, each off by U8 of itself: U8^2 in all;
     or (half: prompts, shared rows) in fp16, off by 2^-11 at most, 2^-32 below
     the largest weight (2^7 of 2^-25 fp16's smallest step, halved), and with them
-    the values: exactly, but for what lies below 2^-14, which is off by less than
-    2^-24, where the 8 values about it reach 2^-12.
+    the values: exactly from 2^-25 on, below that off by less than 2^-32, where the 8
+    values about it reach 2^-20.
     The exponential (2 units), sums over keys and the parts' joining: fp32,
     fewer than 2^5 roundings on a chain at a weight's size for the lengths here
     beyond the random walk of the sum, which 2^-18 of the mass covers."""
@@ -94,7 +94,7 @@ def attention_reference(q, k, v, new, lens, tables, scale, shared=0, cap=None, h
             err = torch.where(see & torch.isfinite(err), err, 0.0).amax(1, keepdim=True)
             w = U8 * o.abs() + (torch.expm1(2 * err) + (2.0 ** -11 if half else U8 * U8) + 2.0 ** -18) * mass + 1e-37
             if half:
-                w = w + 2.0 ** -24 + 2.0 ** -32 * torch.mm(see.double(), clean.abs())
+                w = w + 2.0 ** -32 + 2.0 ** -32 * torch.mm(see.double(), clean.abs())
             out[row:row + n, h * rep:(h + 1) * rep] = o.reshape(n, rep, D)
             bound[row:row + n, h * rep:(h + 1) * rep] = w.reshape(n, rep, D)
         row += n

@@ -232,7 +232,7 @@ def test_scales(gpu, new, past, scale):
 
 @pytest.mark.parametrize("new,past", [([1, 1, 1], [50, 3, 2000]), ([3, 1, 4], [50, 3, 200]), ([90, 1, 400], [50, 3, 70])])
 @pytest.mark.parametrize("shared", [0, 160])
-@pytest.mark.parametrize("size", [2.0 ** -20, 2.0 ** 20, 2.0 ** 100, 2.0 ** -100])
+@pytest.mark.parametrize("size", [2.0 ** -30, 2.0 ** 20, 2.0 ** 100, 2.0 ** -100])
 def test_values_of_any_size(gpu, new, past, shared, size):
     """All values small or large; then one row, or 8 values of one, among others of size 1."""
     past = [p + shared for p in past]
@@ -248,6 +248,16 @@ def test_values_of_any_size(gpu, new, past, shared, size):
         check(q, cache, batch, new, lens, lists, shared=shared, half=size < 1 or None)
         cache.v[pg, :, r] = 0
         check(q, cache, batch, new, lens, lists, shared=shared)
+
+
+@pytest.mark.parametrize("new,past", [([3, 1, 4], [500, 3, 200]), ([10, 1, 9], [500, 3, 200]), ([90, 1, 400], [50, 3, 70])])
+@pytest.mark.parametrize("shared", [0, 160])
+@pytest.mark.parametrize("size", [2.0 ** -10, 2.0 ** -17, 2.0 ** -24])
+def test_small_dimensions(gpu, new, past, shared, size):
+    """Dimensions whose values are far smaller than their neighbours' keep their precision."""
+    q, cache, batch, lens, lists = case(8, (8, 2), 16, new, [p + shared for p in past], common=shared // 16)
+    cache.v[..., 3::5].mul_(size)
+    check(q, cache, batch, new, lens, lists, shared=shared)
 
 
 @pytest.mark.parametrize("new,past", [([1, 1, 1, 1], [50, 3, 200, 0]), ([3, 1, 4, 2], [50, 3, 200, 0]), ([90, 1, 40, 70], [50, 3, 70, 0])])
