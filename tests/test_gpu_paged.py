@@ -544,3 +544,94 @@ def test_empty_calls(gpu):
         idle = bmx.PagedBatch(i32(3), i32(2) + 5, i32(2, 1), 3, max_new=max_new)
         assert (bmx.attention_paged(bf(64, 3, D), cache, idle, out=bf(3, 64 * D) + 7) == 7).all()
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("new", [[1, 1, 1], [9, 2, 1], [120, 1, 33]])
+@pytest.mark.parametrize("page,past", [(4096, [4090, 9000, 100]), (2048, [4090, 3, 2047])])
+def test_large_pages(gpu, new, page, past):
+    q, cache, batch, lens, lists = case(100, (8, 2), page, new, past)
+    check(q, cache, batch, new, lens, lists)
+
+
+@pytest.mark.parametrize("new", [[1, 1, 1], [6, 2, 1], [9, 1, 12], [90, 1, 40]])
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+def test_values_not_finite_in_shared_rows(gpu, new, bad):
+    """Every query sees them: that dimension is lost, the others stay right."""
+    q, cache, batch, lens, lists = case(101, (8, 2), 16, new, [300, 260, 500], common=10)
+    want = check(q, cache, batch, new, lens, lists, shared=160)
+    pg = lists[0][4]
+    cache.v[pg, 1, 7, 9] = bad
+    got = check(q, cache, batch, new, lens, lists, shared=160).view(-1, 2, 4, D)
+    assert (torch.isnan(got[:, 1, :, 9]) | (got[:, 1, :, 9] == bad)).all()
+    assert torch.equal(got[:, 0], want.view(-1, 2, 4, D)[:, 0])
+
+
+@pytest.mark.parametrize("new,past", [([1, 1, 1], [50, 100, 2000]), ([3, 1, 4], [50, 100, 2000]), ([11, 1, 9], [50, 100, 2000]),
+                                      ([90, 1, 400], [50, 100, 70])])
+@pytest.mark.parametrize("shared", [0, 32])
+def test_scores_of_minus_infinity(gpu, new, past, shared):
+    """Keys whose product with a query is -inf have no weight; all of them: zeros."""
+    q, cache, batch, lens, lists = case(102, (8, 2), 16, new, past, common=shared // 16)
+    q[..., 0] = 1.0
+    seen = cache.k.clone()
+    cache.k[..., 0, 0] = -math.inf   # the first row of every page
+    got = bmx.attention_paged(q, cache, batch, shared=shared)
+    row = 0
+    for b, n in enumerate(new):
+        for i in {0, n - 1}:
+            L = lens[b] - n + i + 1
+            pages = lists[0][:shared // 16] + lists[b][shared // 16:]
+            k, v = (rows_of(x, pages, L)[0].double() for x in (seen, cache.v))
+            s = (q[:, row + i].double().view(2, 4, D) @ k.transpose(1, 2).contiguous()) / math.sqrt(D)
+            s[..., ::16] = -math.inf
+            want = s.softmax(-1) @ v
+            # (an output's rounding and 2^-11 of a weight's, with the values' largest)
+            assert (got[row + i].view(2, 4, D).double() - want).abs().max() <= 2.0 ** -8 * float(want.abs().max()) + 2.0 ** -11 * 6
+        row += n
+    cache.k[..., 0] = -math.inf
+    assert (bmx.attention_paged(q, cache, batch, shared=shared) == 0).all()
+
+
+def test_python_refusals(gpu):
+    q, cache, batch, lens, lists = case(103, (8, 2), 16, [2, 3], [20, 30])
+    x = projections(104, (8, 2), 5)
+
+    def refused(code, f, *a, **k):
+        with pytest.raises(bmx.BmxError) as e:
+            f(*a, **k)
+        assert e.value.code == code, e.value
+
+    att, app = bmx.attention_paged, bmx.qk_norm_rope_paged
+    for bad in (q.float(), q.cpu(), q.transpose(0, 1)):
+        refused(bmx.BMX_E_ARG, att, bad, cache, batch)
+    for bad in (q[:, :4].contiguous(), q[:5].contiguous(), q[..., :64].contiguous(), q.view(-1)):
+        refused(bmx.BMX_E_SHAPE, att, bad, cache, batch)
+    refused(bmx.BMX_E_ARG, att, q, cache, batch, shared=8)
+    refused(bmx.BMX_E_ARG, att, q, cache, batch, shared=-16)
+    refused(bmx.BMX_E_ARG, att, q, cache, batch, shared=1 << 20)
+    refused(bmx.BMX_E_ARG, att, q, cache, batch, out=q)
+    refused(bmx.BMX_E_ARG, att, q, cache, batch, out=q.float())
+    refused(bmx.BMX_E_SHAPE, att, q, cache, batch, out=q.new_empty(5, 7 * D))
+    ws = bmx.attention_paged_workspace(8, 2, batch)
+    refused(bmx.BMX_E_ARG, att, q, cache, batch, workspace=ws[:-1])
+    refused(bmx.BMX_E_ARG, att, q, cache, batch, workspace=ws.cpu())
+    refused(bmx.BMX_E_ARG, att, q, cache, batch, workspace=ws[::2])
+    for i in range(5):
+        for bad, code in ((x[i].float(), bmx.BMX_E_ARG), (x[i].cpu(), bmx.BMX_E_ARG),
+                          (x[i][..., :-1].contiguous(), bmx.BMX_E_SHAPE), (x[i][:4].contiguous(), bmx.BMX_E_SHAPE)):
+            refused(code, app, *x[:i], bad, *x[i + 1:], cache, batch)
+    refused(bmx.BMX_E_SHAPE, app, *x, cache, batch, out=q[:4].contiguous())
+    refused(bmx.BMX_E_ARG, app, *x, cache, batch, out=x[0].view(8, 5, D))
+    k = cache.k
+    for bad, code in (((k, k[:-1]), bmx.BMX_E_SHAPE), ((k, k.float()), bmx.BMX_E_ARG), ((k[0], k[0]), bmx.BMX_E_SHAPE),
+                      ((k.transpose(0, 1), k), bmx.BMX_E_ARG)):
+        refused(code, bmx.PagedKvCache, *bad)
+    for bad, code in (((batch.starts, batch.starts, batch.pages, 5), bmx.BMX_E_SHAPE), ((batch.starts.long(), batch.lens, batch.pages, 5), bmx.BMX_E_ARG),
+                      ((batch.starts, batch.lens, batch.pages, -1), bmx.BMX_E_SHAPE), ((batch.starts, batch.lens, batch.pages, 5, 6), bmx.BMX_E_SHAPE),
+                      ((batch.starts, batch.lens, batch.pages, 5, 0), bmx.BMX_E_SHAPE), ((batch.starts, batch.lens, batch.lens, 5), bmx.BMX_E_SHAPE)):
+        refused(code, bmx.PagedBatch, *bad)
+    with pytest.raises(bmx.BmxError):
+        batch.lens = batch.lens.clone()
+    refused(bmx.BMX_E_SHAPE, bmx.attention_paged_workspace, 7, 2, batch)
+    refused(bmx.BMX_E_SHAPE, bmx.attention_paged_workspace, 8, 2, (5, 2, 6))
+    check(q, cache, batch, [2, 3], lens, lists, workspace=ws)
