@@ -7,24 +7,32 @@
 // Of a kv head and a sequence the query rows are r = token * rep + (q head
 // within the kv head's rep), so that any number of heads fills a tile.
 //
-// Two kernels by the rows a sequence can have (max_new * rep):
-//   up to 64 (decode, verified drafts): paged_few_kernel, memory-bound.  The
-//     key blocks of all (sequence, kv head) pairs in a row are cut into equal
-//     shares, one per workgroup, so lengths need not be alike; a pair that
-//     several workgroups share is joined by paged_few_merge_kernel.
+// By the rows a sequence can have (max_new * rep):
+//   up to 32 (decode, verified drafts): paged_few_kernel, bound by memory.  K and
+//     V go from memory to registers and from there into the products.
+//   up to 64: paged_mid_kernel, by 64-key blocks through LDS.
+//     Either way the key blocks of all (sequence, kv head) pairs in a row are cut
+//     into equal shares, one per workgroup, so lengths need not be alike; what
+//     several workgroups did of a pair is joined by the last of them or by
+//     paged_few_merge_kernel.
 //   more (prompts, chunks, and decode steps beside them): paged_tile_kernel,
-//     compute-bound, by 128-row tiles that paged_plan_kernel lists longest
-//     first and cuts where they are few.
+//     bound by the products and the softmax between them, by tiles of 128 or 256
+//     rows that paged_plan_kernel lists longest first and cuts where they are
+//     few, paged_tile_merge_kernel joining the pieces.
 // Rows common to all sequences (`shared`) are one more "sequence" of all the
-// batch's query rows, taken by the tile kernel before the rest; what it leaves
-// is folded in by the merges.
+// batch's query rows, taken by tiles: in the launch of the rest where a sequence
+// has few rows (paged_shared_kernel), before it otherwise (paged_prefix_kernel).
+// The merges fold in what comes of them.
 //
 // Scores are in base 2: p = 2^(s c - m), c = |scale| log2 e (a negative scale
 // flips q's signs).  The running maximum m follows a row's largest score only
 // once that is 2^8 ahead: sums and outputs are fp32 either way, and the
-// rescaling of the outputs all but vanishes.  p enters the second product in
-// two bf16 pieces (16 bits): with one, outputs were off by 0.0024 of their
-// norm where their own rounding is 0.0017.
+// rescaling of the outputs all but vanishes.  With one bf16 piece of p, outputs
+// were off by 0.0024 of their norm where their own rounding is 0.0017, so p has
+// more bits: two bf16 pieces (16 bits) where memory bounds; fp16 (11 bits, off by
+// 2^-11) in the tiles, where a second product costs (a 4096-token prompt 215 us
+// with two, 184 then), with V in fp16 as well, which holds all but the far
+// ends of bf16's range as they are.
 #include <math.h>
 
 #include <algorithm>
@@ -64,10 +72,10 @@ struct PagedAttn {
   float c2;           // |scale| log2(e)
   uint32_t flip;      // sign bits of a bf16 pair where scale < 0
   // ---- workspace ----
-  int* plan;          // few: share, blocks before each sequence; tiles: PlanHead and its lists
-  float* row_o;       // few: [T, Hq, 128] parts that start a pair's blocks
+  int* plan;          // few rows: share, blocks before each sequence; tiles: PlanHead and its lists
+  float* row_o;       // few rows: [T, Hq, 128] parts that start a pair's blocks
   float* row_ml;      // [T, Hq, 2]
-  float* wg_o;        // few: [workgroups, rows, 128] parts that continue a pair's; tiles: [slots, Hkv, 128, 128]
+  float* wg_o;        // few rows: [workgroups, rows, 128] parts that continue a pair's; tiles: [slots, Hkv, tile_rows, 128]
   float* wg_ml;
   float* pre_o;       // [np, T, Hq, 128] parts over the shared rows
   float* pre_ml;
@@ -96,7 +104,7 @@ __device__ __forceinline__ float2 get2(const float* from) {
   return make_float2(__uint_as_float(static_cast<uint32_t>(v)), __uint_as_float(static_cast<uint32_t>(v >> 32)));
 }
 
-// 2^x; maxima of -inf (no key seen) count as 0
+// A maximum of -inf (no key seen) counts as 0
 __device__ __forceinline__ float finite_max(float m) { return m == -INFINITY ? 0.0f : m; }
 // The maximum that a partial result is stored with.  -inf tells the merge that
 // nothing was seen; scores that are all NaN leave it there too, with a sum that
@@ -161,10 +169,10 @@ __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirs
 // ===========================================================================
 // few query rows
 // ===========================================================================
-constexpr int kFewKeys = 128;  // of a block: 32 per wave
+constexpr int kFewKeys = 128;   // of a block: 32 per wave
 constexpr int kFewOs = kD + 4;  // LDS stride of an output row
 
-// Exclusive prefix over 256 threads (further ones hold the same again), and the total
+// Exclusive prefix over 256 threads, and the total; tmp: 4 ints
 __device__ __forceinline__ int scan256(int v, int* tmp, int* total) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   int x = v;
@@ -179,7 +187,7 @@ __device__ __forceinline__ int scan256(int v, int* tmp, int* total) {
 #pragma unroll
   for (int w = 0; w < 4; w++) {
     const int s = tmp[w];
-    if (w < (wave & 3)) before += s;
+    if (w < wave) before += s;
     all += s;
   }
   *total = all;
@@ -199,11 +207,11 @@ struct Share {
   int t, t1, share, b, h, j, nb;
   PagedSeq sq;
 };
-// The share of workgroup wg of wgs; false where it is empty.  *lone: whether any sequence has new tokens and
-// no block.  tmp: 8 ints, found: 5.
+// The share of workgroup wg of wgs; false where it is empty.  *lone: whether any
+// sequence has new tokens and no block.  tmp: 8 ints, found: 5.
 __device__ __forceinline__ bool first_share(const PagedAttn& p, int wg, int wgs, int* tmp, int* found, Share& s, bool* lone) {
   const int tid = threadIdx.x;
-  const int per = (p.B + 255) >> 8, b0 = (tid & 255) * per;
+  const int per = (p.B + 255) >> 8, b0 = tid * per;
   int mine = 0;
   bool none = false;
   PagedSeq only{0, 0, 0};
@@ -213,8 +221,8 @@ __device__ __forceinline__ bool first_share(const PagedAttn& p, int wg, int wgs,
     mine += n;
     none = none || (only.tokens > 0 && n == 0);
   }
-  if ((tid & 63) == 0) tmp[4 + (tid >> 6 & 3)] = 0;
-  if (__any(none) && (tid & 63) == 0) tmp[4 + (tid >> 6 & 3)] = 1;
+  const bool some = __any(none);
+  if ((tid & 63) == 0) tmp[4 + (tid >> 6)] = some;
   int all;
   const int before = scan256(mine, tmp, &all);
   *lone = (tmp[4] | tmp[5] | tmp[6] | tmp[7]) != 0;
@@ -325,7 +333,8 @@ __device__ __forceinline__ void few_lone(const PagedAttn& p) {
   }
 }
 
-// Up to 16 query rows of a pair (NT = 1), in blocks of 128 keys.  Per wave and step of 32 keys, in two 16-key tiles:
+// Up to 16 NT query rows of a pair, in blocks of 128 keys.  Per wave and step of
+// 32 keys, in two 16-key tiles:
 //   S^T = K Q^T (v_mfma_f32_16x16x32_bf16): lane l holds query row l % 16 and
 //     keys 4 (l / 16) + i of each tile;
 //   O^T += V^T P^T: the eight keys of a lane's scores are its k slice as they
@@ -336,9 +345,11 @@ __device__ __forceinline__ void few_lone(const PagedAttn& p) {
 // The next step's K is requested when this step's scores are done, its V when
 // the values are turned, also where the next step is another pair's: short
 // sequences wait for no first load but the workgroup's.
-// RG groups of 4 waves take 16 NT rows each over the same keys (64 rows by one
-// group needed more than 256 registers a wave: 36 us for 16 sequences of 5
-// tokens, against @@).
+// Bound by memory: two workgroups to a CU keep 2 x 4 waves x 16 KB on their way.
+// 64 single tokens over 500 to 8191 rows, 8 kv heads: 135 us, 711 MB at 5.3 TB/s (a
+// large copy moves 4.9); one over 131000 beside 7 short ones
+// 106 us, 5.1 TB/s.  One over 4096: 13 us, of which the join's launch is 4.5, and the rest is the latency
+// of the table, its rows and the sum through LDS.
 struct FewLds {
   float os[4][16][kFewOs];
   float ms[4][32], ls[4][32];
@@ -705,7 +716,8 @@ __global__ void __launch_bounds__(256) paged_few_merge_kernel(const PagedAttn p)
   Fold f;
   if (p.shared) f.add_all(p.pre_o + at * kD, p.pre_ml + at * 2, static_cast<int64_t>(p.T) * p.Hq, i0, by, p.np, d);
   if (nb > 0) {
-    if (i0 == 0) f.add(*reinterpret_cast<const float2*>(p.row_ml + at * 2), *reinterpret_cast<const float4*>(p.row_o + at * kD + d));
+    if (i0 == 0)
+      f.add(*reinterpret_cast<const float2*>(p.row_ml + at * 2), *reinterpret_cast<const float4*>(p.row_o + at * kD + d));
     const int64_t first = static_cast<int64_t>(w0 + 1) * (16 * NT) + r;
     if (w1 > w0) f.add_all(p.wg_o + first * kD, p.wg_ml + first * 2, 16 * NT, i0, by, w1 - w0, d);
   }
@@ -772,8 +784,10 @@ struct Result {
 #define SCHED(kind, n) __builtin_amdgcn_sched_group_barrier(kind, n, 0)
 constexpr int kSchedMfma = 0x8, kSchedRead = 0x100, kSchedValu = 0x402;
 
-// Rows r0 .. r0 + 127 of (sequence, kv head) -- of all the batch's rows, over
-// the shared ones, where PRE -- against 64-key blocks, 32 rows to a wave.
+// The 32 NW / WK rows from r0 on of (sequence, kv head) -- of all the batch's rows,
+// over the shared ones, where PRE -- against 64-key blocks, 32 rows to a wave (WK = 2:
+// to two, half of each block's keys each).  False, with nothing written, where HALF
+// met values that fp16 does not hold (see settle); every wave says the same.
 //   S^T = K Q^T (v_mfma_f32_32x32x16_bf16): lane l holds query row l % 32 and
 //     keys 8 (r / 4) + 4 (l / 32) + r % 4 of its 16 registers r per 32 keys;
 //   O^T += V^T P^T: the eight keys of a step are eight neighbouring score
@@ -783,8 +797,17 @@ constexpr int kSchedMfma = 0x8, kSchedRead = 0x100, kSchedValu = 0x402;
 // chunk c lies at c ^ (4 (row % 4) + row / 4 % 4), which keeps both kinds of
 // read off each other's banks.  64 KB of LDS and up to 256 registers: two
 // workgroups share a CU, one's exponentials beside the other's products.
+// One prompt of 4096 tokens, 32 heads: 165 us, 137 GFLOP at 0.83 PFLOP/s (a large
+// matrix product reaches 1.12).  The matrix cores are busy 38 % of the cycles and
+// the vector units 52 %, and two waves of a SIMD overlap them only in part (32
+// products and 232 vector instructions each: 1.5 us where either alone takes
+// 1.0).  What was tried against it and did not help: the next block's scores
+// beside this block's softmax (186 us then to 212, for the registers), row sums by a
+// product with ones (186 to 195), 32-key blocks with three waves to a SIMD (177 to
+// 230: spills), wave priorities, K read further ahead.
 template <bool PRE, bool HALF, int NW, int WK>
-__device__ __forceinline__ bool tile_try(const PagedAttn& p, char* lds, const PagedSeq& sq, int b, int h, int r0, int j0, int j1, const Result& to) {
+__device__ __forceinline__ bool tile_try(const PagedAttn& p, char* lds, const PagedSeq& sq, int b, int h, int r0, int j0,
+                                         int j1, const Result& to) {
   constexpr int WR = NW / WK, NK = 2 / WK;  // row groups of waves; 32-key tiles of a wave
   constexpr int kOwn = kTileKeys / NW;      // rows of K and V that a wave stages
   const int tid = threadIdx.x, wave = uniform(tid >> 6), lane = tid & 63, j = lane & 31, hf = lane >> 5;
@@ -1112,7 +1135,8 @@ __device__ __forceinline__ bool tile_try(const PagedAttn& p, char* lds, const Pa
 #pragma unroll
     for (int w = 0; w < NW; w++) odd |= left_out[w];
     if (j0 < j1 && uniform(odd)) {
-      for (int key = key0 + max(j0 * kTileKeys, (first - key0) & ~(kTileKeys - 1)); key < min(key0 + j1 * kTileKeys, end); key++) {
+      const int from = key0 + max(j0 * kTileKeys, (first - key0) & ~(kTileKeys - 1));
+      for (int key = from; key < min(key0 + j1 * kTileKeys, end); key++) {
         const int64_t at = row_at(p, table, h, key);
         if (at < 0 || key >= lim) continue;
 #pragma unroll
@@ -1136,7 +1160,8 @@ __device__ __forceinline__ bool tile_try(const PagedAttn& p, char* lds, const Pa
     if (wk == 1) {
 #pragma unroll
       for (int i = 0; i < 16; i++)
-        st[i * 64 + lane] = make_float4(o[i >> 2][4 * (i & 3)], o[i >> 2][4 * (i & 3) + 1], o[i >> 2][4 * (i & 3) + 2], o[i >> 2][4 * (i & 3) + 3]);
+        st[i * 64 + lane] = make_float4(o[i >> 2][4 * (i & 3)], o[i >> 2][4 * (i & 3) + 1], o[i >> 2][4 * (i & 3) + 2],
+                                        o[i >> 2][4 * (i & 3) + 3]);
       sml[lane] = make_float2(part_max(m, l), l);
     }
     __syncthreads();
@@ -1144,7 +1169,8 @@ __device__ __forceinline__ bool tile_try(const PagedAttn& p, char* lds, const Pa
     const float2 ml = sml[lane];
     if (!(l == l)) m = 0.0f;
     const float mn = fmaxf(m, ml.x);
-    const float wa = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn), wb = ml.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml.x - mn);
+    const float wa = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
+    const float wb = ml.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml.x - mn);
     l = l * wa + ml.y * wb;
     m = mn;
 #pragma unroll
@@ -1157,35 +1183,36 @@ __device__ __forceinline__ bool tile_try(const PagedAttn& p, char* lds, const Pa
   }
   constexpr float kDown = HALF ? 1.0f / (1 << kValueUp) : 1.0f;
   auto finish = [&]() {
-  const int64_t row = static_cast<int64_t>(sq.row0 + tok) * p.Hq + hd;
-  if (!to.o) {
-    const float inv = l == 0.0f ? 0.0f : kDown / l;
-    uint16_t* dst = p.out + row * kD + 4 * hf;
+    const int64_t row = static_cast<int64_t>(sq.row0 + tok) * p.Hq + hd;
+    if (!to.o) {
+      const float inv = l == 0.0f ? 0.0f : kDown / l;
+      uint16_t* dst = p.out + row * kD + 4 * hf;
+#pragma unroll
+      for (int dt = 0; dt < 4; dt++)
+#pragma unroll
+        for (int r4 = 0; r4 < 4; r4++) {
+          const f32x16_t& a = o[dt];
+          *reinterpret_cast<uint2*>(dst + 32 * dt + 8 * r4) =
+              make_uint2(pack2(a[4 * r4] * inv, a[4 * r4 + 1] * inv), pack2(a[4 * r4 + 2] * inv, a[4 * r4 + 3] * inv));
+        }
+      return;
+    }
+    const int64_t part = to.by_row ? row : 32 * wr + j;
+    if (hf == 0) *reinterpret_cast<float2*>(to.ml + part * 2) = make_float2(part_max(m, l) - (HALF ? kUp : 0.0f), l);
+    float* dst = to.o + part * kD + 4 * hf;
 #pragma unroll
     for (int dt = 0; dt < 4; dt++)
 #pragma unroll
-      for (int r4 = 0; r4 < 4; r4++) {
-        const f32x16_t& a = o[dt];
-        *reinterpret_cast<uint2*>(dst + 32 * dt + 8 * r4) =
-            make_uint2(pack2(a[4 * r4] * inv, a[4 * r4 + 1] * inv), pack2(a[4 * r4 + 2] * inv, a[4 * r4 + 3] * inv));
-      }
-    return;
-  }
-  const int64_t part = to.by_row ? row : 32 * wr + j;
-  if (hf == 0) *reinterpret_cast<float2*>(to.ml + part * 2) = make_float2(part_max(m, l) - (HALF ? kUp : 0.0f), l);
-  float* dst = to.o + part * kD + 4 * hf;
-#pragma unroll
-  for (int dt = 0; dt < 4; dt++)
-#pragma unroll
-    for (int r4 = 0; r4 < 4; r4++)
-      *reinterpret_cast<float4*>(dst + 32 * dt + 8 * r4) =
-          make_float4(o[dt][4 * r4] * kDown, o[dt][4 * r4 + 1] * kDown, o[dt][4 * r4 + 2] * kDown, o[dt][4 * r4 + 3] * kDown);
+      for (int r4 = 0; r4 < 4; r4++)
+        *reinterpret_cast<float4*>(dst + 32 * dt + 8 * r4) =
+            make_float4(o[dt][4 * r4] * kDown, o[dt][4 * r4 + 1] * kDown, o[dt][4 * r4 + 2] * kDown, o[dt][4 * r4 + 3] * kDown);
   };
   if (rw + j < R) finish();
   return true;
 }
 template <bool PRE, int NW, int WK>
-__device__ __forceinline__ void tile_run(const PagedAttn& p, char* lds, const PagedSeq& sq, int b, int h, int r0, int j0, int j1, const Result& to) {
+__device__ __forceinline__ void tile_run(const PagedAttn& p, char* lds, const PagedSeq& sq, int b, int h, int r0, int j0,
+                                         int j1, const Result& to) {
   if (!uniform(tile_try<PRE, true, NW, WK>(p, lds, sq, b, h, r0, j0, j1, to)))
     tile_try<PRE, false, NW, WK>(p, lds, sq, b, h, r0, j0, j1, to);
 }
@@ -1221,13 +1248,16 @@ __global__ void __launch_bounds__(64 * NW, 2) paged_tile_kernel(const PagedAttn 
     const Item it = plan_items(p)[at];
     const int64_t slot = (static_cast<int64_t>(uniform(it.slot)) * p.Hkv + h) * (32 * NW);
     const int b = uniform(it.b);
-    tile_run<false, NW, 1>(p, lds, paged_seq(p.starts[b], p.starts[b + 1], p.lens[b], p.T), b, h, uniform(it.r0), uniform(it.j0), uniform(it.j1),
+    const PagedSeq sq = paged_seq(p.starts[b], p.starts[b + 1], p.lens[b], p.T);
+    tile_run<false, NW, 1>(p, lds, sq, b, h, uniform(it.r0), uniform(it.j0), uniform(it.j1),
                        slot < 0 ? Result{nullptr, nullptr, false} : Result{p.wg_o + slot * kD, p.wg_ml + slot * 2, false});
   }
 }
 
 // Up to 64 query rows of a pair, in blocks of 64 keys by shares as few_run: two
-// row groups of waves, each by two waves that take half of a block's keys.
+// row groups of waves, each by two waves that take half of a block's keys.  16
+// sequences of 5 tokens, 40 rows each, over 300 to 3000 rows: 30 us (the kernel 24.6), 79 MB at
+// 3.2 TB/s: bound by the softmax between loads that LDS holds one block ahead.
 __device__ __forceinline__ void mid_run(const PagedAttn& p, char* lds, int wg, int wgs) {
   int* const tmp = reinterpret_cast<int*>(lds + kTileLds);
   Share at;
@@ -1238,7 +1268,8 @@ __device__ __forceinline__ void mid_run(const PagedAttn& p, char* lds, int wg, i
     const int n = min(at.t1 - at.t, at.nb - at.j);
     const int64_t slot = static_cast<int64_t>(wg) * 64;
     Result to{nullptr, nullptr, false};
-    if (n < at.nb || p.shared) to = at.j == 0 ? Result{p.row_o, p.row_ml, true} : Result{p.wg_o + slot * kD, p.wg_ml + slot * 2, false};
+    if (n < at.nb || p.shared)
+      to = at.j == 0 ? Result{p.row_o, p.row_ml, true} : Result{p.wg_o + slot * kD, p.wg_ml + slot * 2, false};
     tile_run<false, 4, 2>(p, lds, at.sq, at.b, at.h, 0, at.j, at.j + n, to);
     more = next_share(p, n, at);
   } while (more);
@@ -1252,7 +1283,8 @@ __global__ void __launch_bounds__(256, 2) paged_mid_kernel(const PagedAttn p) {
 
 // The shared rows (the first `pre` workgroups: kv heads x row tiles x key splits)
 // and the sequences' own by shares (NT = 4: mid_run) in one launch: neither waits
-// for the other's last workgroups.
+// for the other's last workgroups (8 tokens over 2048 shared rows 21 us in two launches,
+// 15 in one; 64 over 4096 35 and 33).
 template <int NT>
 __global__ void __launch_bounds__(256, 2) paged_shared_kernel(const PagedAttn p, int pre) {
   extern __shared__ __align__(256) char lds[];
@@ -1416,7 +1448,8 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const PagedAtt
 }
 
 // The cut tiles' rows, 8 to a workgroup: parts over the shared rows, then the
-// pieces'.
+// pieces'.  (6 to 8 us, most of it the launch and the latency of the plan, a part's
+// maximum and its values.)
 constexpr int kTileMergeGrid = 2048;
 __global__ void __launch_bounds__(256) paged_tile_merge_kernel(const PagedAttn p) {
   const int groups = p.tile_rows / 8, n = p.plan[1] * p.Hkv * groups, d = 4 * (threadIdx.x & 31);
@@ -1438,10 +1471,19 @@ __global__ void __launch_bounds__(256) paged_tile_merge_kernel(const PagedAttn p
 // ---------------------------------------------------------------------------
 // host
 // ---------------------------------------------------------------------------
-constexpr int kFewRows = 64;       // rows of a (sequence, kv head) pair up to which paged_few_kernel serves
-// its workgroups: as many as fit the CUs at once
-constexpr int kFewGrid = 512;
-constexpr int kTileGrid = 512;     // of the tile kernel: two to a CU
+// Rows of a (sequence, kv head) pair up to which shares serve: no launches for a
+// plan, and lengths balanced to a block.  (Us, shares / tiles, 48 rows a pair, 8 kv
+// heads: 16 sequences of 20 to 300 rows 14.6 / 19.5, of 2000 to 3000 48.8 / 53.3, 4 of
+// 7000 to 8000 36.7 / 44.8, 16 behind 2048 shared rows 33 / 50; 64 of 500 to 4000 with up
+// to 60 rows, where the products weigh, 115 / 112.)
+constexpr int kFewRows = 64;
+// Of these up to 32 go straight from memory to registers, more through LDS: 20 rows
+// 17.0 / 19.0 and 22.0 / 26.0 us that way / this, 28 and 32 rows even (26.5 / 24.8, 107.5 /
+// 109.2); 64 rows that way need more than 256 registers (36 us for 16 sequences of 5
+// tokens, where the other takes 30).
+constexpr int kFewDirect = 32;
+constexpr int kFewGrid = 512;      // workgroups of shares: two to a CU
+constexpr int kTileGrid = 512;     // 128-row tiles at once: two workgroups to a CU
 constexpr int kMaxPre = 64;        // key splits of the shared rows
 
 // Rows of a tile.  256 stage and convert a block of keys once for twice the rows,
@@ -1452,7 +1494,7 @@ constexpr int kMaxPre = 64;        // key splits of the shared rows
 int tile_rows(int rep, int T, int B) { return static_cast<int64_t>(T) * rep >= static_cast<int64_t>(B) * 12288 ? 256 : 128; }
 
 struct PagedPlan {
-  int few, nt;        // few: row tiles of 16
+  int few, nt;        // few rows: 16-row tiles of a pair, 1, 2 or (by mid_run) 4
   int rows, per_head; // of a tile; tile workgroups of a kv head
   int64_t all;        // tiles of all the batch's rows
   int np;             // most key splits of the shared rows
@@ -1486,7 +1528,7 @@ PagedPlan make_plan(int Hq, int Hkv, int T, int B, int max_new, bool shared) {
   };
   auto few = [&]() {
     const int64_t r = std::min<int64_t>(R, kFewRows);
-    a.nt = r <= 16 ? 1 : r <= 32 ? 2 : 4;
+    a.nt = r <= 16 ? 1 : r <= kFewDirect ? 2 : 4;
     parts((1 + static_cast<size_t>(B)) * sizeof(int), rows, static_cast<size_t>(kFewGrid) * 16 * a.nt);
   };
   auto tile = [&](int tile_rows) {
@@ -1591,7 +1633,8 @@ extern "C" int bmx_attention_paged(const bmx_bf16* q, const bmx_paged_kv* cache,
     // 33 parts a row 14.4 / 13.0; 4 with 28 query rows a pair 20.5 / 14.3; with
     // parts over shared rows as well, 64 sequences 50 / 34.)
     const int64_t pairs = static_cast<int64_t>(B) * Hkv;
-    const int64_t pieces = std::min<int64_t>(kFewGrid / pairs, (batch->max_pages * cache->page_size + kFewKeys - 1) / kFewKeys) + 1;
+    const int most_blocks = (batch->max_pages * cache->page_size + kFewKeys - 1) / kFewKeys;
+    const int64_t pieces = std::min<int64_t>(kFewGrid / pairs, most_blocks) + 1;
     if (a.nt == 1 && !shared && pairs <= kMaxCounters && static_cast<int64_t>(batch->max_new) * p.rep * pieces <= 96)
       p.cnt = reinterpret_cast<unsigned*>(ws);
     // (few rows have many parts each; us with 8 rows / 1 row to a workgroup: 64
@@ -1611,8 +1654,10 @@ extern "C" int bmx_attention_paged(const bmx_bf16* q, const bmx_paged_kv* cache,
       else hipLaunchKernelGGL(joint, merge, dim3(256), 0, st, p);
       return check_launch("attention_paged merge");
     };
-    if (a.nt == 1) return launch(paged_few_kernel<1>, paged_shared_kernel<1>, paged_few_merge_kernel<1, false>, paged_few_merge_kernel<1, true>);
-    if (a.nt == 2) return launch(paged_few_kernel<2>, paged_shared_kernel<2>, paged_few_merge_kernel<2, false>, paged_few_merge_kernel<2, true>);
+    if (a.nt == 1) return launch(paged_few_kernel<1>, paged_shared_kernel<1>, paged_few_merge_kernel<1, false>,
+                                  paged_few_merge_kernel<1, true>);
+    if (a.nt == 2) return launch(paged_few_kernel<2>, paged_shared_kernel<2>, paged_few_merge_kernel<2, false>,
+                                  paged_few_merge_kernel<2, true>);
     return launch(paged_mid_kernel, paged_shared_kernel<4>, paged_few_merge_kernel<4, false>, paged_few_merge_kernel<4, true>);
   }
   if (shared) {

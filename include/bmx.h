@@ -437,7 +437,7 @@ int bmx_qk_norm_rope_paged(const bmx_bf16 *q, const bmx_bf16 *k, const bmx_bf16 
  * none) are common to all sequences and lie on the pages that sequence 0's
  * table names; they are read once for the whole batch.  Every sequence with
  * new tokens has at least that many rows before them.
- * A token that sees no row gets zeros.  A row that a query does not see leaves
+ * A token that sees no row, or whose every score is -inf, gets zeros.  A row that a query does not see leaves
  * it alone, whatever it holds; one that it sees with a value that is not
  * finite makes that dimension of its output not finite.  The order of every sum
  * is fixed by the shapes and the batch's arrays: equal calls give equal bits.
@@ -445,7 +445,8 @@ int bmx_qk_norm_rope_paged(const bmx_bf16 *q, const bmx_bf16 *k, const bmx_bf16 
  * bmx_attention_paged_workspace_bytes or more, else BMX_E_ARG; its first
  * BMX_PAGED_COUNTER_BYTES zero-filled before its first use (every call leaves
  * them zero); calls that share one must not run concurrently.  q, out: 16-byte
- * aligned, without overlap (BMX_E_ARG).  tokens = 0 or n_seqs = 0 is a no-op.
+ * aligned, without overlap (BMX_E_ARG).  tokens = 0 or n_seqs = 0 is a no-op;
+ * more than 2^30 blocks of 64 keys in all is BMX_E_SHAPE.
  * Replaces: mlx_rs::fast::scaled_dot_product_attention as bmx_attention_gqa
  *   does (crates/base-mlx-core/src/model/qwen3.rs:491-518, 629-653), for a
  *   batch. */
