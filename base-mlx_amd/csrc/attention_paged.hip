@@ -1284,7 +1284,7 @@ __global__ void __launch_bounds__(256, 2) paged_mid_kernel(const PagedAttn p) {
 // The shared rows (the first `pre` workgroups: kv heads x row tiles x key splits)
 // and the sequences' own by shares (NT = 4: mid_run) in one launch: neither waits
 // for the other's last workgroups (8 tokens over 2048 shared rows 21 us in two launches,
-// 15 in one; 64 over 4096 35 and 33).
+// 15 in one; 64 over 4096 35 and 31).
 template <int NT>
 __global__ void __launch_bounds__(256, 2) paged_shared_kernel(const PagedAttn p, int pre) {
   extern __shared__ __align__(256) char lds[];
@@ -1615,7 +1615,19 @@ extern "C" int bmx_attention_paged(const bmx_bf16* q, const bmx_paged_kv* cache,
   // at least 4 blocks to a split of the shared rows (32 and 160 single tokens
   // over 8192 and 512 shared rows, as many splits as fill the CUs / that: 38.7 /
   // 31.5, 54.2 / 46.6 us)
-  const int splits = std::min(a.np, (nb + 3) / 4), bps = splits ? (nb + splits - 1) / splits : 0;
+  // -- nor more than the shared rows' part of the places, where the sequences' own
+  // are few: a pair's, whose lengths are not known here, for three blocks of a tile
+  // (us, so / without: 64 single tokens over 4096 shared rows 28.3 / 30.8, 160 over 2048
+  // 34.8 / 39.9, 30 of one q head a kv head over 16384 23.1 / 26.5, 200 over 4096
+  // 56.1 / 59.9; 32 over 8192, 64 over 1024, 160 over 32768 alike; with two blocks
+  // 30.8, 34.3, 25.9, 59.8, with five 27.5, 38.5, 23.6, 54.3 and 160 over 32768 150 for 145)
+  int splits = std::min(a.np, (nb + 3) / 4);
+  const int64_t pairs = static_cast<int64_t>(B) * Hkv, pre_tiles = Hkv * a.all;
+  if (a.few && splits > 1) {
+    const int64_t places = kFewGrid * pre_tiles * nb / (pre_tiles * nb + 3 * pairs);
+    splits = static_cast<int>(std::min<int64_t>(splits, std::max<int64_t>(1, (places + pre_tiles / 2) / pre_tiles)));
+  }
+  const int bps = splits ? (nb + splits - 1) / splits : 0;
   const int np = bps ? (nb + bps - 1) / bps : 0;
   PagedAttn p{q, cache->k, cache->v, out, batch->starts, batch->lens, batch->pages, B, batch->max_pages, T,
                     batch->max_new, n_heads, Hkv, n_heads / Hkv, cache->n_pages, log2_of(cache->page_size), shared,
@@ -1632,7 +1644,6 @@ extern "C" int bmx_attention_paged(const bmx_bf16* q, const bmx_paged_kv* cache,
     // 20.9 / 24.7, 4 of 200 to 900 9.5 / 11.2, 64 of 500 to 8191 134 / 136; 1 of 4097,
     // 33 parts a row 14.4 / 13.0; 4 with 28 query rows a pair 20.5 / 14.3; with
     // parts over shared rows as well, 64 sequences 50 / 34.)
-    const int64_t pairs = static_cast<int64_t>(B) * Hkv;
     const int most_blocks = (batch->max_pages * cache->page_size + kFewKeys - 1) / kFewKeys;
     const int64_t pieces = std::min<int64_t>(kFewGrid / pairs, most_blocks) + 1;
     if (a.nt == 1 && !shared && pairs <= kMaxCounters && static_cast<int64_t>(batch->max_new) * p.rep * pieces <= 96)
@@ -1646,7 +1657,14 @@ extern "C" int bmx_attention_paged(const bmx_bf16* q, const bmx_paged_kv* cache,
       const size_t lds = shared || a.nt == 4 ? kMidLds : 0;
       if (int rc = shared ? allow_lds(with_shared, lds) : allow_lds(few, lds)) return rc;
       const int pre = shared ? Hkv * static_cast<int>(a.all) * np : 0;
-      if (shared) hipLaunchKernelGGL(with_shared, dim3(pre + kFewGrid), dim3(256), lds, st, p, pre);
+      // Shares for the places that the shared rows' tiles leave of a round, so that
+      // none waits for a place -- if that is a quarter of them and they get four
+      // pairs each at most.  (Us, so / always kFewGrid: 64 tokens over 4096 shared rows
+      // 30.6 / 32.9, 32 over 8192 25.6 / 28.5, 160 over 512 29.6 / 33.5; 160 over 2048, 6.7
+      // pairs each, 48.0 / 39.7; 64 over 2048 with 500 to 3000 of their own 85.7 / 84.4.)
+      const int left = kFewGrid - pre % kFewGrid;
+      const int few_grid = 4 * left >= kFewGrid && pairs <= 4 * left ? left : kFewGrid;
+      if (shared) hipLaunchKernelGGL(with_shared, dim3(pre + few_grid), dim3(256), lds, st, p, pre);
       else hipLaunchKernelGGL(few, dim3(kFewGrid), dim3(256), lds, st, p);
       if (int rc = check_launch("attention_paged")) return rc;
       if (p.cnt) return 0;
