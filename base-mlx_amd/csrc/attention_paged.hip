@@ -800,11 +800,14 @@ constexpr int kSchedMfma = 0x8, kSchedRead = 0x100, kSchedValu = 0x402;
 // One prompt of 4096 tokens, 32 heads: 165 us, 137 GFLOP at 0.83 PFLOP/s (a large
 // matrix product reaches 1.12).  The matrix cores are busy 38 % of the cycles and
 // the vector units 52 %, and two waves of a SIMD overlap them only in part (32
-// products and 232 vector instructions each: 1.5 us where either alone takes
-// 1.0).  What was tried against it and did not help: the next block's scores
-// beside this block's softmax (186 us then to 212, for the registers), row sums by a
-// product with ones (186 to 195), 32-key blocks with three waves to a SIMD (177 to
-// 230: spills), wave priorities, K read further ahead.
+// products and 232 vector instructions each: 1.6 us, made to alternate 1.5, where
+// either alone takes 1.0).  V's way to fp16 is 8 to 12 % of it.  What was tried and
+// did not help: the next block's scores beside this block's softmax (186 us then to
+// 212, for the registers), one half of a block's weights beside the other's scores
+// (163 to 171), V turned beside the scores, with one more barrier (165 to 172), row
+// sums by a product with ones (186 to 195) or by dot products (alike), 32-key blocks
+// with three waves to a SIMD (177 to 230: spills), wave priorities, K read further
+// ahead.
 template <bool PRE, bool HALF, int NW, int WK>
 __device__ __forceinline__ bool tile_try(const PagedAttn& p, char* lds, const PagedSeq& sq, int b, int h, int r0, int j0,
                                          int j1, const Result& to) {
