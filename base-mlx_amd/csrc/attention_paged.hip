@@ -29,10 +29,10 @@
 // once that is 2^8 ahead: sums and outputs are fp32 either way, and the
 // rescaling of the outputs all but vanishes.  With one bf16 piece of p, outputs
 // were off by 0.0024 of their norm where their own rounding is 0.0017, so p has
-// more bits: two bf16 pieces (16 bits) where memory bounds; fp16 (11 bits, off by
-// 2^-11) in the tiles, where a second product costs (a 4096-token prompt 215 us
-// with two, 184 then), with V in fp16 as well, which holds all but the far
-// ends of bf16's range as they are.
+// more bits: two bf16 pieces (16 bits) up to 64 rows, where memory bounds; fp16
+// (11 bits, off by 2^-11) in the tiles, where a second product costs (a 4096-token
+// prompt 215 us with two, 184 then), with V in fp16 as well, which holds all but
+// the far ends of bf16's range as they are.
 #include <math.h>
 
 #include <algorithm>
@@ -1213,11 +1213,11 @@ __device__ __forceinline__ bool tile_try(const PagedAttn& p, char* lds, const Pa
   if (rw + j < R) finish();
   return true;
 }
-template <bool PRE, int NW, int WK>
+template <bool PRE, int NW>
 __device__ __forceinline__ void tile_run(const PagedAttn& p, char* lds, const PagedSeq& sq, int b, int h, int r0, int j0,
                                          int j1, const Result& to) {
-  if (!uniform(tile_try<PRE, true, NW, WK>(p, lds, sq, b, h, r0, j0, j1, to)))
-    tile_try<PRE, false, NW, WK>(p, lds, sq, b, h, r0, j0, j1, to);
+  if (!uniform(tile_try<PRE, true, NW, 1>(p, lds, sq, b, h, r0, j0, j1, to)))
+    tile_try<PRE, false, NW, 1>(p, lds, sq, b, h, r0, j0, j1, to);
 }
 
 // Key split z of 128- (NW = 8: 256-) row tile i of all the batch's rows, over the
@@ -1226,7 +1226,7 @@ template <int NW>
 __device__ __forceinline__ void prefix_run(const PagedAttn& p, char* lds, int h, int i, int z) {
   const int nb = (p.shared + kTileKeys - 1) / kTileKeys, j0 = z * p.pre_bps;
   const int64_t slot = static_cast<int64_t>(z) * p.T * p.Hq;
-  tile_run<true, NW, 1>(p, lds, PagedSeq{0, p.T, 0}, 0, h, i * (32 * NW), j0, min(j0 + p.pre_bps, nb),
+  tile_run<true, NW>(p, lds, PagedSeq{0, p.T, 0}, 0, h, i * (32 * NW), j0, min(j0 + p.pre_bps, nb),
                         Result{p.pre_o + slot * kD, p.pre_ml + slot * 2, true});
 }
 
@@ -1252,15 +1252,17 @@ __global__ void __launch_bounds__(64 * NW, 2) paged_tile_kernel(const PagedAttn 
     const int64_t slot = (static_cast<int64_t>(uniform(it.slot)) * p.Hkv + h) * (32 * NW);
     const int b = uniform(it.b);
     const PagedSeq sq = paged_seq(p.starts[b], p.starts[b + 1], p.lens[b], p.T);
-    tile_run<false, NW, 1>(p, lds, sq, b, h, uniform(it.r0), uniform(it.j0), uniform(it.j1),
+    tile_run<false, NW>(p, lds, sq, b, h, uniform(it.r0), uniform(it.j0), uniform(it.j1),
                        slot < 0 ? Result{nullptr, nullptr, false} : Result{p.wg_o + slot * kD, p.wg_ml + slot * 2, false});
   }
 }
 
 // Up to 64 query rows of a pair, in blocks of 64 keys by shares as few_run: two
-// row groups of waves, each by two waves that take half of a block's keys.  16
-// sequences of 5 tokens, 40 rows each, over 300 to 3000 rows: 30 us (the kernel 24.6), 79 MB at
-// 3.2 TB/s: bound by the softmax between loads that LDS holds one block ahead.
+// row groups of waves, each by two waves that take half of a block's keys.  Two
+// bf16 pieces of the weights here: V's way to fp16 takes longer than the second
+// product (29.2 us for 30.2 of the following).  16 sequences of 5 tokens, 40 rows
+// each, over 300 to 3000 rows: 29 us (the kernel 23.1), 79 MB at 3.4 TB/s: bound by
+// the softmax between loads that LDS holds one block ahead.
 __device__ __forceinline__ void mid_run(const PagedAttn& p, char* lds, int wg, int wgs) {
   int* const tmp = reinterpret_cast<int*>(lds + kTileLds);
   Share at;
@@ -1273,7 +1275,7 @@ __device__ __forceinline__ void mid_run(const PagedAttn& p, char* lds, int wg, i
     Result to{nullptr, nullptr, false};
     if (n < at.nb || p.shared)
       to = at.j == 0 ? Result{p.row_o, p.row_ml, true} : Result{p.wg_o + slot * kD, p.wg_ml + slot * 2, false};
-    tile_run<false, 4, 2>(p, lds, at.sq, at.b, at.h, 0, at.j, at.j + n, to);
+    tile_try<false, false, 4, 2>(p, lds, at.sq, at.b, at.h, 0, at.j, at.j + n, to);
     more = next_share(p, n, at);
   } while (more);
 }

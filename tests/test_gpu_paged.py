@@ -31,8 +31,8 @@ def case(seed, heads, page, new, past, common=0, std=1.5):
 
 def check(q, cache, batch, new, lens, lists, shared=0, scale=None, what="", half=None, **kw):
     got = bmx.attention_paged(q, cache, batch, scale=scale, shared=shared, **kw)
-    if half is None:  # more query rows per kv head than 32, or shared ones: weights in fp16
-        half = shared > 0 or batch.max_new * (q.shape[0] // cache.n_kv_heads) > 32
+    if half is None:  # more query rows per kv head than 64, or shared ones: weights in fp16
+        half = shared > 0 or batch.max_new * (q.shape[0] // cache.n_kv_heads) > 64
     out, bound = attention_reference(q, cache.k, cache.v, new, lens, lists, 1 / math.sqrt(D) if scale is None else scale,
                                      shared, half=half)
     T = sum(new)
