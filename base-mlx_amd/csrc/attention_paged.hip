@@ -29,10 +29,11 @@
 // once that is 2^8 ahead: sums and outputs are fp32 either way, and the
 // rescaling of the outputs all but vanishes.  With one bf16 piece of p, outputs
 // were off by 0.0024 of their norm where their own rounding is 0.0017, so p has
-// more bits: two bf16 pieces (16 bits) up to 64 rows, where memory bounds; fp16
-// (11 bits, off by 2^-11) in the tiles, where a second product costs (a 4096-token
-// prompt 215 us with two, 184 then), with V in fp16 as well, which holds all but
-// the far ends of bf16's range as they are.
+// more bits: two bf16 pieces (16 bits), in every kernel, so that a token's
+// precision does not depend on what else is in its batch, and V stays the bf16
+// that it is, of any size.  (Tiles with p and V in fp16 save the second product,
+// a 4096-token prompt 166 us for 204, for 5 bits of p, for values below 2^-25
+// beside larger ones, and for a second run of tiles whose values lie far apart.)
 #include <math.h>
 
 #include <algorithm>
@@ -45,14 +46,9 @@ namespace {
 constexpr int kD = kPagedDim;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLazy = 8.0f;  // log2 by which a maximum may lag
-constexpr float kUp = 7.0f;    // log2 by which fp16 probabilities are scaled up: the largest, with kLazy, are 2^15
-constexpr int kValueUp = 8;     // log2 by which values are scaled up on their way to fp16
 constexpr float kLeast = 1.17549435e-38f;  // of c: a scale of 0 leaves a hidden key's -inf what it is
 
 typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8_t;
-typedef __attribute__((ext_vector_type(8))) _Float16 f16x8_t;
-typedef __attribute__((ext_vector_type(2))) _Float16 f16x2_t;
-typedef __attribute__((ext_vector_type(2))) unsigned short u16x2_t;
 typedef __attribute__((ext_vector_type(4))) float f32x4_t;
 typedef __attribute__((ext_vector_type(16))) float f32x16_t;
 typedef __attribute__((ext_vector_type(4))) short s16x4_t;
@@ -112,9 +108,6 @@ __device__ __forceinline__ float finite_max(float m) { return m == -INFINITY ? 0
 __device__ __forceinline__ float part_max(float m, float l) { return l == l ? m : 0.0f; }
 
 typedef __attribute__((ext_vector_type(2))) float f32x2_t;
-__device__ __forceinline__ uint32_t pack2h(float lo, float hi) {
-  return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2_t{lo, hi}, f16x2_t));
-}
 // Two bf16 values in a word: one v_cvt_pk_bf16_f32
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2_t{lo, hi}, bf16x2_t));
@@ -786,8 +779,7 @@ constexpr int kSchedMfma = 0x8, kSchedRead = 0x100, kSchedValu = 0x402;
 
 // The 32 NW / WK rows from r0 on of (sequence, kv head) -- of all the batch's rows,
 // over the shared ones, where PRE -- against 64-key blocks, 32 rows to a wave (WK = 2:
-// to two, half of each block's keys each).  False, with nothing written, where HALF
-// met values that fp16 does not hold (see settle); every wave says the same.
+// to two, half of each block's keys each).
 //   S^T = K Q^T (v_mfma_f32_32x32x16_bf16): lane l holds query row l % 32 and
 //     keys 8 (r / 4) + 4 (l / 32) + r % 4 of its 16 registers r per 32 keys;
 //   O^T += V^T P^T: the eight keys of a step are eight neighbouring score
@@ -797,19 +789,11 @@ constexpr int kSchedMfma = 0x8, kSchedRead = 0x100, kSchedValu = 0x402;
 // chunk c lies at c ^ (4 (row % 4) + row / 4 % 4), which keeps both kinds of
 // read off each other's banks.  64 KB of LDS and up to 256 registers: two
 // workgroups share a CU, one's exponentials beside the other's products.
-// One prompt of 4096 tokens, 32 heads: 165 us, 137 GFLOP at 0.83 PFLOP/s (a large
-// matrix product reaches 1.12).  The matrix cores are busy 38 % of the cycles and
-// the vector units 52 %, and two waves of a SIMD overlap them only in part (32
-// products and 232 vector instructions each: 1.6 us, made to alternate 1.5, where
-// either alone takes 1.0).  V's way to fp16 is 8 to 12 % of it.  What was tried and
-// did not help: the next block's scores beside this block's softmax (186 us then to
-// 212, for the registers), one half of a block's weights beside the other's scores
-// (163 to 171), V turned beside the scores, with one more barrier (165 to 172), row
-// sums by a product with ones (186 to 195) or by dot products (alike), 32-key blocks
-// with three waves to a SIMD (177 to 230: spills), wave priorities, K read further
-// ahead.
-template <bool PRE, bool HALF, int NW, int WK>
-__device__ __forceinline__ bool tile_try(const PagedAttn& p, char* lds, const PagedSeq& sq, int b, int h, int r0, int j0,
+// One prompt of 4096 tokens, 32 heads: 204 us, 137 GFLOP at 0.67 PFLOP/s (a large
+// matrix product reaches 1.12); the two pieces of the weights make 206 GFLOP of
+// products, 1.01.
+template <bool PRE, int NW, int WK>
+__device__ __forceinline__ void tile_run(const PagedAttn& p, char* lds, const PagedSeq& sq, int b, int h, int r0, int j0,
                                          int j1, const Result& to) {
   constexpr int WR = NW / WK, NK = 2 / WK;  // row groups of waves; 32-key tiles of a wave
   constexpr int kOwn = kTileKeys / NW;      // rows of K and V that a wave stages
@@ -887,60 +871,24 @@ __device__ __forceinline__ bool tile_try(const PagedAttn& p, char* lds, const Pa
       lds_load16(in ? reinterpret_cast<const char*>(p.v + at) + voff[i] : zero, dst + kTileBytes + 1024 * i);
     }
   };
-  // ... and what is done to the wave's 16 rows of V once they are there: values
-  // to fp16, times 2^kValueUp; in blocks that only some queries see whole, values
-  // that are not finite to 0.  fp16 holds a bf16 value from 2^-25 up as it is and a
-  // smaller one to 2^-32: where some value is 2^8 or more, or eight neighbours are
-  // all below 2^-20, the rows are left for the tile's second try, in bf16.
+  // ... and what is done to the wave's rows of V once they are there: in blocks
+  // that only some queries see whole, values that are not finite become 0
   auto settle = [&](int jb, int buf) {
     const int k0 = key0 + jb * kTileKeys;
-    const bool mixed = !PRE && k0 + kTileKeys > first && first < end;  // (uniform)
-    if (!HALF && !mixed) return;
+    if (PRE || k0 + kTileKeys <= first || first >= end) return;  // uniform
     char* at = lds + buf * 2 * kTileBytes + kTileBytes + wave * kOwn * 256 + lane * 16;
     uint4 w[kOwn / 4];
+    uint32_t nf = 0;
 #pragma unroll
-    for (int i = 0; i < kOwn / 4; i++) w[i] = *reinterpret_cast<const uint4*>(at + i * 1024);
-    bool changed = false;
-    if (mixed) {
-      uint32_t nf = 0;
-#pragma unroll
-      for (int i = 0; i < kOwn / 4; i++) {
-        nf |= not_finite(w[i].x) | not_finite(w[i].y) | not_finite(w[i].z) | not_finite(w[i].w);
-        w[i] = make_uint4(finite_part(w[i].x), finite_part(w[i].y), finite_part(w[i].z), finite_part(w[i].w));
-      }
-      changed = __any(nf != 0);
-      if (changed && lane == 0) left_out[wave] = 1;
+    for (int i = 0; i < kOwn / 4; i++) {
+      w[i] = *reinterpret_cast<const uint4*>(at + i * 1024);
+      nf |= not_finite(w[i].x) | not_finite(w[i].y) | not_finite(w[i].z) | not_finite(w[i].w);
+      w[i] = make_uint4(finite_part(w[i].x), finite_part(w[i].y), finite_part(w[i].z), finite_part(w[i].w));
     }
-    if constexpr (HALF) {
-      // of the lane's 8 values of a row the largest magnitude, as bits: 0, or
-      // from 2^-20 to below 2^8
-      uint32_t top = 0, low = ~0u;
+    if (!__any(nf != 0)) return;
+    if (lane == 0) left_out[wave] = 1;
 #pragma unroll
-      for (int i = 0; i < kOwn / 4; i++) {
-        auto mag = [](uint32_t x) { return __builtin_bit_cast(u16x2_t, x & 0x7fff7fffu); };
-        const u16x2_t a = __builtin_elementwise_max(__builtin_elementwise_max(mag(w[i].x), mag(w[i].y)),
-                                                    __builtin_elementwise_max(mag(w[i].z), mag(w[i].w)));
-        const uint32_t t = max(static_cast<uint32_t>(a.x), static_cast<uint32_t>(a.y));
-        top = max(top, t);
-        low = min(low, t - 1u);  // (0 wraps to the largest)
-      }
-      if (__any(top >= ((127u + 16u - kValueUp) << 7) || low < ((127u - 12u - kValueUp) << 7) - 1u)) {
-        if (lane == 0) exist[NW * buf + wave] = 2;
-        return;
-      }
-#pragma unroll
-      for (int i = 0; i < kOwn / 4; i++) {
-        auto h2 = [](uint32_t x) {
-          x += kValueUp * 0x00800080u;  // (a pair's exponents; 0 stays below fp16's smallest)
-          return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(__uint_as_float(x << 16),
-                                                                         __uint_as_float(x & 0xffff0000u)));
-        };
-        *reinterpret_cast<uint4*>(at + i * 1024) = make_uint4(h2(w[i].x), h2(w[i].y), h2(w[i].z), h2(w[i].w));
-      }
-    } else if (changed) {
-#pragma unroll
-      for (int i = 0; i < kOwn / 4; i++) *reinterpret_cast<uint4*>(at + i * 1024) = w[i];
-    }
+    for (int i = 0; i < kOwn / 4; i++) *reinterpret_cast<uint4*>(at + i * 1024) = w[i];
   };
   // ---- LDS addresses: of a row's chunk, the others' follow by exclusive or
   // (made anew in every block: 16 registers otherwise) ----
@@ -1011,7 +959,7 @@ __device__ __forceinline__ bool tile_try(const PagedAttn& p, char* lds, const Pa
       const uint2 x = __builtin_bit_cast(uint2, a), y = __builtin_bit_cast(uint2, c);
       return make_uint4(x.x, x.y, y.x, y.y);
     };
-    const float mu = finite_max(m) - (HALF ? kUp : 0.0f);
+    const float mu = finite_max(m);
     float sum = 0.0f;
     auto weigh = [&](int s, float (&e8)[8]) {
 #pragma unroll
@@ -1020,81 +968,43 @@ __device__ __forceinline__ bool tile_try(const PagedAttn& p, char* lds, const Pa
         sum += e8[e];
       }
     };
-    if constexpr (HALF) {
-      auto weigh16 = [&](int s) {
-        float e8[8];
-        weigh(s, e8);
-        return __builtin_bit_cast(f16x8_t, make_uint4(pack2h(e8[0], e8[1]), pack2h(e8[2], e8[3]), pack2h(e8[4], e8[5]),
-                                                      pack2h(e8[6], e8[7])));
-      };
-      uint4 va[4];
+    uint4 va[4];
 #pragma unroll
-      for (int dt = 0; dt < 4; dt++) va[dt] = values(dt, 0);
-      f16x8_t pw = weigh16(0);
-      __builtin_amdgcn_sched_barrier(0);
+    for (int dt = 0; dt < 4; dt++) va[dt] = values(dt, 0);
+    bf16x8_t hi, lo;
+    auto weigh2 = [&](int s) {
+      float e8[8];
+      weigh(s, e8);
+      split8(e8, one, hi, lo);
+    };
+    weigh2(0);
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int s = 0; s < 2 * NK; s++) {
-        const f16x8_t w = pw;
-        uint4 vc[4];
+    for (int s = 0; s < 2 * NK; s++) {
+      const bf16x8_t h1 = hi, h2 = lo;
+      uint4 vc[4];
 #pragma unroll
-        for (int dt = 0; dt < 4; dt++) vc[dt] = va[dt];
-        if (s < 2 * NK - 1) {
+      for (int dt = 0; dt < 4; dt++) vc[dt] = va[dt];
+      if (s < 2 * NK - 1) {
 #pragma unroll
-          for (int dt = 0; dt < 4; dt++) va[dt] = values(dt, s + 1);
-          pw = weigh16(s + 1);
-        }
-#pragma unroll
-        for (int dt = 0; dt < 4; dt++)
-          o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, vc[dt]), w, o[dt], 0, 0, 0);
-        if (s < 2 * NK - 1) {
-          SCHED(kSchedRead, 8);
-#pragma unroll
-          for (int i = 0; i < 4; i++) {
-            SCHED(kSchedMfma, 1);
-            SCHED(kSchedValu, 7);
-          }
-        }
-        __builtin_amdgcn_sched_barrier(0);
+        for (int dt = 0; dt < 4; dt++) va[dt] = values(dt, s + 1);
+        weigh2(s + 1);
       }
-    } else {
-      uint4 va[4];
 #pragma unroll
-      for (int dt = 0; dt < 4; dt++) va[dt] = values(dt, 0);
-      bf16x8_t hi, lo;
-      auto weigh2 = [&](int s) {
-        float e8[8];
-        weigh(s, e8);
-        split8(e8, one, hi, lo);
-      };
-      weigh2(0);
-      __builtin_amdgcn_sched_barrier(0);
+      for (int dt = 0; dt < 4; dt++)
+        o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, vc[dt]), h1, o[dt], 0, 0, 0);
 #pragma unroll
-      for (int s = 0; s < 2 * NK; s++) {
-        const bf16x8_t h1 = hi, h2 = lo;
-        uint4 vc[4];
+      for (int dt = 0; dt < 4; dt++)
+        o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, vc[dt]), h2, o[dt], 0, 0, 0);
+      if (s < 2 * NK - 1) {
+        SCHED(kSchedRead, 8);
 #pragma unroll
-        for (int dt = 0; dt < 4; dt++) vc[dt] = va[dt];
-        if (s < 2 * NK - 1) {
-#pragma unroll
-          for (int dt = 0; dt < 4; dt++) va[dt] = values(dt, s + 1);
-          weigh2(s + 1);
+        for (int i = 0; i < 8; i++) {
+          SCHED(kSchedMfma, 1);
+          SCHED(kSchedValu, 6);
         }
-#pragma unroll
-        for (int dt = 0; dt < 4; dt++)
-          o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, vc[dt]), h1, o[dt], 0, 0, 0);
-#pragma unroll
-        for (int dt = 0; dt < 4; dt++)
-          o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, vc[dt]), h2, o[dt], 0, 0, 0);
-        if (s < 2 * NK - 1) {
-          SCHED(kSchedRead, 8);
-#pragma unroll
-          for (int i = 0; i < 8; i++) {
-            SCHED(kSchedMfma, 1);
-            SCHED(kSchedValu, 6);
-          }
-        }
-        __builtin_amdgcn_sched_barrier(0);
       }
+      __builtin_amdgcn_sched_barrier(0);
     }
     l += sum;
   };
@@ -1109,12 +1019,11 @@ __device__ __forceinline__ bool tile_try(const PagedAttn& p, char* lds, const Pa
   for (int jb = j0; jb < j1; jb++) {
     const int buf = (jb - j0) & 1, bo = buf * 2 * kTileBytes;
     __syncthreads();
-    int e4[4], most = 0, least = 2;
+    int e4[4], least = 1;
 #pragma unroll
     for (int i = 0; i < NW; i += 4) {
       const int4 e = *reinterpret_cast<const int4*>(exist + NW * buf + i);
       least = min(least, min(min(e.x, e.y), min(e.z, e.w)));
-      most = max(most, max(max(e.x, e.y), max(e.z, e.w)));
       if constexpr (NW == 4) {
         e4[0] = e.x, e4[1] = e.y, e4[2] = e.z, e4[3] = e.w;
       } else {
@@ -1122,7 +1031,6 @@ __device__ __forceinline__ bool tile_try(const PagedAttn& p, char* lds, const Pa
       }
     }
     const bool all = uniform(least) != 0;
-    if (HALF && uniform(most) > 1) return false;  // (in every wave)
     if (jb + 1 < j1) stage(jb + 1, buf ^ 1);
     const int k0 = key0 + jb * kTileKeys + wk * NK * 32;
     // (uniform: keys hidden from all of the wave's rows are only settled)
@@ -1168,7 +1076,7 @@ __device__ __forceinline__ bool tile_try(const PagedAttn& p, char* lds, const Pa
       sml[lane] = make_float2(part_max(m, l), l);
     }
     __syncthreads();
-    if (wk == 1) return true;
+    if (wk == 1) return;
     const float2 ml = sml[lane];
     if (!(l == l)) m = 0.0f;
     const float mn = fmaxf(m, ml.x);
@@ -1184,11 +1092,10 @@ __device__ __forceinline__ bool tile_try(const PagedAttn& p, char* lds, const Pa
       for (int r = 0; r < 4; r++) o[i >> 2][4 * (i & 3) + r] = o[i >> 2][4 * (i & 3) + r] * wa + v[r] * wb;
     }
   }
-  constexpr float kDown = HALF ? 1.0f / (1 << kValueUp) : 1.0f;
   auto finish = [&]() {
     const int64_t row = static_cast<int64_t>(sq.row0 + tok) * p.Hq + hd;
     if (!to.o) {
-      const float inv = l == 0.0f ? 0.0f : kDown / l;
+      const float inv = l == 0.0f ? 0.0f : 1.0f / l;
       uint16_t* dst = p.out + row * kD + 4 * hf;
 #pragma unroll
       for (int dt = 0; dt < 4; dt++)
@@ -1201,23 +1108,16 @@ __device__ __forceinline__ bool tile_try(const PagedAttn& p, char* lds, const Pa
       return;
     }
     const int64_t part = to.by_row ? row : 32 * wr + j;
-    if (hf == 0) *reinterpret_cast<float2*>(to.ml + part * 2) = make_float2(part_max(m, l) - (HALF ? kUp : 0.0f), l);
+    if (hf == 0) *reinterpret_cast<float2*>(to.ml + part * 2) = make_float2(part_max(m, l), l);
     float* dst = to.o + part * kD + 4 * hf;
 #pragma unroll
     for (int dt = 0; dt < 4; dt++)
 #pragma unroll
       for (int r4 = 0; r4 < 4; r4++)
         *reinterpret_cast<float4*>(dst + 32 * dt + 8 * r4) =
-            make_float4(o[dt][4 * r4] * kDown, o[dt][4 * r4 + 1] * kDown, o[dt][4 * r4 + 2] * kDown, o[dt][4 * r4 + 3] * kDown);
+            make_float4(o[dt][4 * r4], o[dt][4 * r4 + 1], o[dt][4 * r4 + 2], o[dt][4 * r4 + 3]);
   };
   if (rw + j < R) finish();
-  return true;
-}
-template <bool PRE, int NW>
-__device__ __forceinline__ void tile_run(const PagedAttn& p, char* lds, const PagedSeq& sq, int b, int h, int r0, int j0,
-                                         int j1, const Result& to) {
-  if (!uniform(tile_try<PRE, true, NW, 1>(p, lds, sq, b, h, r0, j0, j1, to)))
-    tile_try<PRE, false, NW, 1>(p, lds, sq, b, h, r0, j0, j1, to);
 }
 
 // Key split z of 128- (NW = 8: 256-) row tile i of all the batch's rows, over the
@@ -1226,7 +1126,7 @@ template <int NW>
 __device__ __forceinline__ void prefix_run(const PagedAttn& p, char* lds, int h, int i, int z) {
   const int nb = (p.shared + kTileKeys - 1) / kTileKeys, j0 = z * p.pre_bps;
   const int64_t slot = static_cast<int64_t>(z) * p.T * p.Hq;
-  tile_run<true, NW>(p, lds, PagedSeq{0, p.T, 0}, 0, h, i * (32 * NW), j0, min(j0 + p.pre_bps, nb),
+  tile_run<true, NW, 1>(p, lds, PagedSeq{0, p.T, 0}, 0, h, i * (32 * NW), j0, min(j0 + p.pre_bps, nb),
                         Result{p.pre_o + slot * kD, p.pre_ml + slot * 2, true});
 }
 
@@ -1252,15 +1152,13 @@ __global__ void __launch_bounds__(64 * NW, 2) paged_tile_kernel(const PagedAttn 
     const int64_t slot = (static_cast<int64_t>(uniform(it.slot)) * p.Hkv + h) * (32 * NW);
     const int b = uniform(it.b);
     const PagedSeq sq = paged_seq(p.starts[b], p.starts[b + 1], p.lens[b], p.T);
-    tile_run<false, NW>(p, lds, sq, b, h, uniform(it.r0), uniform(it.j0), uniform(it.j1),
+    tile_run<false, NW, 1>(p, lds, sq, b, h, uniform(it.r0), uniform(it.j0), uniform(it.j1),
                        slot < 0 ? Result{nullptr, nullptr, false} : Result{p.wg_o + slot * kD, p.wg_ml + slot * 2, false});
   }
 }
 
 // Up to 64 query rows of a pair, in blocks of 64 keys by shares as few_run: two
-// row groups of waves, each by two waves that take half of a block's keys.  Two
-// bf16 pieces of the weights here: V's way to fp16 takes longer than the second
-// product (29.2 us for 30.2 of the following).  16 sequences of 5 tokens, 40 rows
+// row groups of waves, each by two waves that take half of a block's keys.  16 sequences of 5 tokens, 40 rows
 // each, over 300 to 3000 rows: 29 us (the kernel 23.1), 79 MB at 3.4 TB/s: bound by
 // the softmax between loads that LDS holds one block ahead.
 __device__ __forceinline__ void mid_run(const PagedAttn& p, char* lds, int wg, int wgs) {
@@ -1275,7 +1173,7 @@ __device__ __forceinline__ void mid_run(const PagedAttn& p, char* lds, int wg, i
     Result to{nullptr, nullptr, false};
     if (n < at.nb || p.shared)
       to = at.j == 0 ? Result{p.row_o, p.row_ml, true} : Result{p.wg_o + slot * kD, p.wg_ml + slot * 2, false};
-    tile_try<false, false, 4, 2>(p, lds, at.sq, at.b, at.h, 0, at.j, at.j + n, to);
+    tile_run<false, 4, 2>(p, lds, at.sq, at.b, at.h, 0, at.j, at.j + n, to);
     more = next_share(p, n, at);
   } while (more);
 }

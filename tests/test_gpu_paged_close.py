@@ -1,0 +1,60 @@
+"""Attention over the paged cache where the precision of its parts shows: the
+weights' own bits, and values far smaller than their neighbours.  All kernels
+alike, whatever else is in the batch."""
+import pytest
+import torch
+
+import bmx
+from _paged_check import D, U8, attention_reference
+from test_gpu_paged import case, check
+
+pytestmark = pytest.mark.gpu
+
+# A kernel each: single tokens, up to 32 and up to 64 query rows per kv head,
+# tiles of 128 and of 256 rows; a chunk beside single tokens; shared rows before
+# single tokens, before drafts and before prompts
+BATCHES = [
+    ((8, 2), [1, 1, 1, 1], [0, 3, 11, 40], 0), ((8, 2), [6, 1, 3], [0, 5, 9], 0), ((8, 2), [14, 1, 9], [0, 5, 9], 0),
+    ((8, 2), [48, 20], [0, 3], 0), ((64, 1), [200], [0], 0), ((8, 2), [40, 1, 1, 1], [0, 2, 5, 12], 0),
+    ((8, 2), [1] * 8, [0, 1, 2, 3, 5, 7, 9, 20], 16), ((8, 2), [6, 1], [0, 4], 16), ((8, 2), [14, 1], [0, 4], 16),
+    ((8, 2), [40, 1], [0, 4], 16),
+]
+
+
+@pytest.mark.parametrize("heads,new,past,shared", BATCHES)
+@pytest.mark.parametrize("scale", [0.25, -0.6, 1.0])
+def test_weights_have_16_bits(gpu, heads, new, past, shared, scale):
+    """Scores of one dimension are exact before the scale; values are positive, so
+    that nothing cancels.  A weight is then off by the two roundings of its score
+    in base 2 (below 2^5: 2^-18 together), the exponential's (2^-22) and its two bf16
+    pieces (U8 each: 2^-16); the fp32 sums of L terms and the parts' joining by at
+    most 2^-23 a term and as much for 32 more steps; scores and sums together below
+    (L + 64) 2^-23.  An output is that, then rounded to bf16 by at most half a
+    step of its binade.  With weights of 11 bits a few outputs in a hundred lie
+    outside."""
+    q, cache, batch, lens, lists = case(21, heads, 16, new, [p + shared for p in past], common=shared // 16)
+    q[..., 1:] = 0
+    q[..., 0] = q[..., 0].clamp(-4, 4)
+    cache.k[..., 1:] = 0
+    cache.k[..., 0] = cache.k[..., 0].clamp(-4, 4)
+    cache.v.copy_(0.5 + cache.v.float().abs().clamp(max=1.5))
+    got = bmx.attention_paged(q, cache, batch, scale=scale, shared=shared).double().view(sum(new), heads[0], D)
+    want, _ = attention_reference(q, cache.k, cache.v, new, lens, lists, scale, shared, half=False)
+    rel = U8 * U8 + (max(lens) + 64) * 2.0 ** -23
+    step = torch.exp2(torch.floor(torch.log2(want * (1 + rel))) - 7)
+    off = (got - want).abs() - step / 2 - rel * want
+    assert not (off > 0).any(), f"{int((off > 0).sum())} of {off.numel()} off, worst by {float((off / want).max()):.3g}"
+
+
+@pytest.mark.parametrize("heads,new,past,shared", BATCHES)
+@pytest.mark.parametrize("size", [2.0 ** -20, 2.0 ** -28, 2.0 ** -34, 2.0 ** -100])
+def test_small_values_beside_others(gpu, heads, new, past, shared, size):
+    """A dimension far smaller than those around it, one that holds a single value,
+    and single small values: as precise as any other."""
+    q, cache, batch, lens, lists = case(22, heads, 16, new, [p + shared for p in past], common=shared // 16)
+    cache.v[..., 9] *= size
+    cache.v[..., 26] = 1.9921875 * size
+    cache.v[:, :, 3::4, 41] *= size
+    got = check(q, cache, batch, new, lens, lists, shared=shared, half=False).view(-1, D)
+    # the mean of equal values: their one rounding, and that of the weights' sum (2^-16)
+    assert ((got[:, 26].double() / (1.9921875 * size) - 1).abs() <= U8 + 2.0 ** -15).all()
