@@ -25,9 +25,12 @@
 // The merges fold in what comes of them.
 //
 // Scores are in base 2: p = 2^(s c - m), c = |scale| log2 e (a negative scale
-// flips q's signs).  The running maximum m follows a row's largest score only
-// once that is 2^8 ahead: sums and outputs are fp32 either way, and the
-// rescaling of the outputs all but vanishes.  With one bf16 piece of p, outputs
+// flips q's signs).  The running m is 2^16 above a row's largest score, and follows
+// it only once that is 2^8 ahead: sums and outputs are fp32 either way, and the
+// rescaling of the outputs all but vanishes.  Weights of at most 2^-8, and 2^-16
+// where m has followed, keep the sums of 2^15 rows of values of 2^120 in range (of
+// 256 next to bf16's largest); values of 2^-100 still have 2^-116, above the
+// smallest normal.  With one bf16 piece of p, outputs
 // were off by 0.0024 of their norm where their own rounding is 0.0017, so p has
 // more bits: two bf16 pieces (16 bits), in every kernel, so that a token's
 // precision does not depend on what else is in its batch, and V stays the bf16
@@ -45,7 +48,8 @@ namespace {
 
 constexpr int kD = kPagedDim;
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLazy = 8.0f;  // log2 by which a maximum may lag
+constexpr float kAbove = 16.0f;  // log2 by which m is set above the largest score
+constexpr float kLazy = 8.0f;    // log2 by which it may lag behind that
 constexpr float kLeast = 1.17549435e-38f;  // of c: a scale of 0 leaves a hidden key's -inf what it is
 
 typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8_t;
@@ -506,8 +510,8 @@ __device__ __forceinline__ void few_run(const PagedAttn& p, FewLds& lds, int wg,
 #pragma unroll
         for (int e = 1; e < 8; e++) mx = fmaxf(mx, sc[nt][e >> 2][e & 3]);
         mx = max_xor32(max_xor16(mx)) * p.c2;
-        if (__any(mx > m[nt] + kLazy)) {
-          const float m1 = fmaxf(m[nt], mx), alpha = __builtin_amdgcn_exp2f(m[nt] - finite_max(m1));
+        if (__any(mx > m[nt] + (kLazy - kAbove))) {
+          const float m1 = fmaxf(m[nt], mx + kAbove), alpha = __builtin_amdgcn_exp2f(m[nt] - finite_max(m1));
           m[nt] = m1;
           l[nt] *= alpha;
 #pragma unroll
@@ -942,8 +946,8 @@ __device__ __forceinline__ void tile_run(const PagedAttn& p, char* lds, const Pa
 #pragma unroll
     for (int r = 1; r < 16 * NK; r++) mx = fmaxf(mx, sc[r >> 4][r & 15]);
     mx = max_xor32(mx) * p.c2;
-    if (__any(mx > m + kLazy)) {
-      const float m1 = fmaxf(m, mx), alpha = __builtin_amdgcn_exp2f(m - finite_max(m1));
+    if (__any(mx > m + (kLazy - kAbove))) {
+      const float m1 = fmaxf(m, mx + kAbove), alpha = __builtin_amdgcn_exp2f(m - finite_max(m1));
       m = m1;
       l *= alpha;
 #pragma unroll

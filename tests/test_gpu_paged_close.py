@@ -1,11 +1,11 @@
 """Attention over the paged cache where the precision of its parts shows: the
-weights' own bits, and values far smaller than their neighbours.  All kernels
-alike, whatever else is in the batch."""
+weights' own bits, values far smaller than their neighbours, and values as large
+as bf16 holds.  All kernels alike, whatever else is in the batch."""
 import pytest
 import torch
 
 import bmx
-from _paged_check import D, U8, attention_reference
+from _paged_check import D, U8, attention_reference, normal
 from test_gpu_paged import case, check
 
 pytestmark = pytest.mark.gpu
@@ -58,3 +58,36 @@ def test_small_values_beside_others(gpu, heads, new, past, shared, size):
     got = check(q, cache, batch, new, lens, lists, shared=shared, half=False).view(-1, D)
     # the mean of equal values: their one rounding, and that of the weights' sum (2^-16)
     assert ((got[:, 26].double() / (1.9921875 * size) - 1).abs() <= U8 + 2.0 ** -15).all()
+
+
+LARGE = [  # (heads, new tokens, their sequences' other rows, shared rows)
+    ((8, 2), [1, 1, 1], [300, 9000, 70000], 0), ((8, 2), [6, 1], [9000, 3], 0), ((8, 2), [14, 1], [9000, 3], 0),
+    ((8, 2), [40, 1], [9000, 3], 0), ((64, 1), [200], [3000], 0), ((8, 2), [1] * 3, [30, 4000, 0], 8000), ((8, 2), [40, 1], [4, 4000], 8000),
+]
+
+
+@pytest.mark.parametrize("heads,new,past,shared", LARGE)
+def test_values_of_2_to_the_120_over_many_rows(gpu, heads, new, past, shared):
+    """A mean of large values is no larger than they are: their weighted sum must
+    not leave fp32 before it is divided."""
+    q, cache, batch, lens, lists = case(24, heads, 16, new, [p + shared for p in past], common=shared // 16, std=0.0)
+    cache.v.copy_((1 + 0.9 * normal(25, *cache.v.shape).abs().clamp(max=1)) * 2.0 ** 120)
+    check(q, cache, batch, new, lens, lists, shared=shared, half=False)  # every key alike
+    q.copy_(normal(26, *q.shape).to(torch.bfloat16))
+    check(q, cache, batch, new, lens, lists, shared=shared, half=False)
+
+
+@pytest.mark.parametrize("heads,new,past,shared", BATCHES)
+def test_values_next_to_the_largest(gpu, heads, new, past, shared):
+    q, cache, batch, lens, lists = case(26, heads, 16, new, [p + shared for p in past], common=shared // 16)
+    cache.v.copy_((1 + 0.9 * normal(27, *cache.v.shape).abs().clamp(max=1)) * 2.0 ** 126 * normal(28, *cache.v.shape).sign())
+    check(q, cache, batch, new, lens, lists, shared=shared, half=False)
+    # keys whose scores rise slowly, so that the maximum lags behind them
+    q[..., 1:] = 0
+    q[..., 0] = 1
+    cache.k[..., 1:] = 0
+    for pages in lists:
+        for j, pg in enumerate(pages):
+            cache.k[pg, :, :, 0] = (16 * j + torch.arange(16, device="cuda", dtype=torch.float32)) / 8
+    cache.v.abs_()
+    check(q, cache, batch, new, lens, lists, shared=shared, scale=1.0, half=False)
