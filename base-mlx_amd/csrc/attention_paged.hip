@@ -1438,10 +1438,13 @@ PagedPlan make_plan(int Hq, int Hkv, int T, int B, int max_new, bool shared) {
     a.nt = r <= 16 ? 1 : r <= kFewDirect ? 2 : 4;
     parts((1 + static_cast<size_t>(B)) * sizeof(int), rows, static_cast<size_t>(kFewGrid) * 16 * a.nt);
   };
-  auto tile = [&](int tile_rows) {
+  auto rows_of_tile = [&](int tile_rows) {
     a.rows = tile_rows;
     a.per_head = std::max(1, kTileGrid * 128 / tile_rows / Hkv);
     a.all = (static_cast<int64_t>(T) * rep + tile_rows - 1) / tile_rows;
+  };
+  auto tile = [&](int tile_rows) {
+    rows_of_tile(tile_rows);
     // whole tiles, and as many pieces more as there are workgroups
     const int64_t tiles = a.all + std::min(B, T);
     a.most_items = static_cast<int>(tiles) + 2 * a.per_head;
@@ -1450,16 +1453,14 @@ PagedPlan make_plan(int Hq, int Hkv, int T, int B, int max_new, bool shared) {
           static_cast<size_t>(shared ? a.most_items : 2 * a.per_head) * Hkv * tile_rows);
   };
   a.few = R <= kFewRows;
-  const int mine = tile_rows(rep, T, B);
-  if (!a.few) {
-    if (rep <= kFewRows) few();
-    tile(128 + 256 - mine);
-  }
-  const size_t others = most;
-  tile(mine);  // (the shared rows', and the call's own where it is not of few rows)
   if (a.few) {
-    most = others;
+    rows_of_tile(128);  // (the shared rows': of paged_shared_kernel)
     few();
+  } else {
+    if (rep <= kFewRows) few();
+    const int mine = tile_rows(rep, T, B);
+    tile(128 + 256 - mine);
+    tile(mine);
   }
   if (shared) {
     a.np = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(kMaxPre, a.per_head / a.all)));
@@ -1543,7 +1544,6 @@ extern "C" int bmx_attention_paged(const bmx_bf16* q, const bmx_paged_kv* cache,
                     a.most_items, a.most_cuts, a.rows, a.nt == 4 ? 6 : 7, nullptr};
   p.c2 = p.c2 < kLeast ? kLeast : p.c2;
   const hipStream_t st = as_stream(stream);
-  if (shared && a.all > 65535) return set_error(BMX_E_SHAPE, "attention_paged: tokens=%d too many for shared rows", T);
   if (a.few) {
     // Where a pair's workgroups have few parts between them, they hand these to
     // the last of them; a launch that spreads the rows over the card joins many.
@@ -1586,6 +1586,7 @@ extern "C" int bmx_attention_paged(const bmx_bf16* q, const bmx_paged_kv* cache,
     return launch(paged_mid_kernel, paged_shared_kernel<4>, paged_few_merge_kernel<4, false>, paged_few_merge_kernel<4, true>);
   }
   if (shared) {
+    if (a.all > 65535) return set_error(BMX_E_SHAPE, "attention_paged: tokens=%d too many for shared rows", T);
     const auto kernel = a.rows == 256 ? paged_prefix_kernel<8> : paged_prefix_kernel<4>;
     if (int rc = allow_lds(kernel, kTileLds)) return rc;
     hipLaunchKernelGGL(kernel, dim3(Hkv, static_cast<unsigned>(a.all), np), dim3(2 * a.rows), kTileLds, st, p);

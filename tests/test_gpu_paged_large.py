@@ -1,0 +1,59 @@
+"""Attention over the paged cache of batches with many packed rows: few of them
+in use, and enough for tiles of 256 query rows."""
+import math
+
+import pytest
+import torch
+
+import bmx
+from _paged_check import D, attention_reference, hold, layout, normal
+from test_gpu_paged import cache_of
+
+pytestmark = pytest.mark.gpu
+
+PAGE = 16
+
+
+def dirty(n_heads, n_kv_heads, batch, shared):
+    """A workspace with its counters zero and the rest NaN."""
+    ws = bmx.attention_paged_workspace(n_heads, n_kv_heads, batch, shared=shared)
+    ws[bmx.PAGED_COUNTER_BYTES:].fill_(255)
+    return ws
+
+
+@pytest.mark.parametrize("n", [1, 6, 14])
+@pytest.mark.parametrize("tokens,first", [(6144, 6100), (6144, 3072), (6144, 0), (6200, 5), (20000, 19900)])
+def test_few_rows_of_many_behind_shared_ones(gpu, n, tokens, first):
+    """Two sequences of n tokens somewhere among many packed rows."""
+    hq, hkv, shared, new = 8, 2, 32, [n, n]
+    lens = [shared + n + 9, shared + n + 40]
+    lists, n_pages = layout(1, new, lens, PAGE, common=shared // PAGE)
+    cache = cache_of(2, n_pages, hkv, PAGE)
+    q = normal(3, hq, tokens, D).to(torch.bfloat16)
+    one = bmx.PagedBatch.of(new, lens, lists)
+    batch = bmx.PagedBatch(one.starts + first, one.lens, one.pages, tokens, max_new=n)
+    out = torch.full((tokens, hq * D), 7.0, dtype=torch.bfloat16, device="cuda")
+    bmx.attention_paged(q, cache, batch, shared=shared, workspace=dirty(hq, hkv, batch, shared), out=out)
+    want, bound = attention_reference(q[:, first:first + 2 * n].contiguous(), cache.k, cache.v, new, lens, lists,
+                                      1 / math.sqrt(D), shared, half=False)
+    hold(out[first:first + 2 * n], want, bound)
+    assert (out[:first] == 7).all() and (out[first + 2 * n:] == 7).all()
+
+
+def test_a_long_sequence_before_a_short_one_behind_shared_rows(gpu):
+    """Of a sequence with more than max_new new tokens the first max_new are
+    answered, and those of the sequences behind it."""
+    hq, hkv, shared, new = 8, 2, 32, [6100, 2]
+    lens = [shared + 6100, shared + 30]
+    lists, n_pages = layout(4, new, lens, PAGE, common=shared // PAGE)
+    cache = cache_of(5, n_pages, hkv, PAGE)
+    q = normal(6, hq, 6144, D).to(torch.bfloat16)
+    one = bmx.PagedBatch.of(new, lens, lists)
+    batch = bmx.PagedBatch(one.starts, one.lens, one.pages, 6144, max_new=2)
+    out = torch.full((6144, hq * D), 7.0, dtype=torch.bfloat16, device="cuda")
+    bmx.attention_paged(q, cache, batch, shared=shared, workspace=dirty(hq, hkv, batch, shared), out=out)
+    rows = [0, 1, 6100, 6101]
+    want, bound = attention_reference(q[:, rows].contiguous(), cache.k, cache.v, [2, 2], [shared + 2, lens[1]], lists,
+                                      1 / math.sqrt(D), shared, half=False)
+    hold(out[rows], want, bound)
+    assert (out[2:6100] == 7).all() and (out[6102:] == 7).all()
