@@ -42,6 +42,7 @@
 #include <algorithm>
 
 #include "paged.h"
+#include "paged_pieces.h"
 
 namespace bmx {
 namespace {
@@ -1303,23 +1304,16 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const PagedAtt
     sum += __shfl_xor(sum, o, 16);
     most = max(most, __shfl_xor(most, o, 16));
   }
-  // ---- pieces of at most `size` blocks, half as many again as each workgroup
-  // has to do on average: each piece more is results to be written and joined (us
-  // with 1 / 1.25 / 1.5 / 2 times the average, or uncut: 1000 tokens over 3000 rows 120
-  // / 101 / 100 / 130 / 135; a chunk of 509 beside 31 single tokens 76 / 74 / 70 / 70 / 103;
-  // 64 over 30000 73 / 72 / 75 / 69 / 682) ----
-  // (tiles longer than the average number at most per_head, and so do their further pieces)
-  const int size = min(max((sum + per_head - 1) / per_head * 3 / 2, 4), most);
+  // ---- pieces of at most `size` blocks: each piece more is results to be written
+  // and joined (us with 1 / 1.25 / 1.5 / 2 times the average, or uncut: 1000 tokens
+  // over 3000 rows 120 / 101 / 100 / 130 / 135; a chunk of 509 beside 31 single tokens
+  // 76 / 74 / 70 / 70 / 103; 64 over 30000 73 / 72 / 75 / 69 / 682) ----
+  const int size = piece_size(sum, per_head, most);
   const float to_bin = static_cast<float>(kPlanBins - 1) / static_cast<float>(size);
   auto bin_of = [&](int len) { return kPlanBins - 1 - min(static_cast<int>(len * to_bin), kPlanBins - 1); };
-  auto cut = [&](int nb, int& len) {  // into pieces of len blocks (the last the rest)
-    const int np = max((nb + size - 1) / size, 1);
-    len = (nb + np - 1) / np;
-    return max((nb + max(len, 1) - 1) / max(len, 1), 1);
-  };
   for (int i = tid; i < n; i += kPlanThreads) {
     int b, r0, len;
-    const int parts = cut(tile(i, b, r0), len);
+    const int parts = piece_count(tile(i, b, r0), size, &len);
     atomicAdd(&bins[bin_of(len)], parts);
   }
   __syncthreads();
@@ -1334,7 +1328,7 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const PagedAtt
   Cut* cuts = plan_cuts(p);
   for (int i = tid; i < n; i += kPlanThreads) {
     int b, r0, len;
-    const int nb = tile(i, b, r0), parts = cut(nb, len);
+    const int nb = tile(i, b, r0), parts = piece_count(nb, size, &len);
     int slot = -1;
     if (parts > 1 || p.shared) {
       slot = atomicAdd(&counts[2], parts);
