@@ -26,8 +26,8 @@
 //
 // Scores are in base 2: p = 2^(s c - m), c = |scale| log2 e (a negative scale
 // flips q's signs).  The running m is 2^16 above a row's largest score, and follows
-// it only once that is 2^8 ahead: sums and outputs are fp32 either way, and the
-// rescaling of the outputs all but vanishes.  Weights of at most 2^-8, and 2^-16
+// it only once that is 2^8 ahead, each row by itself: sums and outputs are fp32
+// either way, and the rescaling of the outputs all but vanishes.  Weights of at most 2^-8, and 2^-16
 // where m has followed, keep the sums of 2^15 rows of values of 2^120 in range (of
 // 256 next to bf16's largest); values of 2^-100 still have 2^-116, above the
 // smallest normal.  With one bf16 piece of p, outputs
@@ -512,7 +512,7 @@ __device__ __forceinline__ void few_run(const PagedAttn& p, FewLds& lds, int wg,
         for (int e = 1; e < 8; e++) mx = fmaxf(mx, sc[nt][e >> 2][e & 3]);
         mx = max_xor32(max_xor16(mx)) * p.c2;
         if (__any(mx > m[nt] + (kLazy - kAbove))) {
-          const float m1 = fmaxf(m[nt], mx + kAbove), alpha = __builtin_amdgcn_exp2f(m[nt] - finite_max(m1));
+          const float m1 = mx > m[nt] + (kLazy - kAbove) ? mx + kAbove : m[nt], alpha = __builtin_amdgcn_exp2f(m[nt] - finite_max(m1));
           m[nt] = m1;
           l[nt] *= alpha;
 #pragma unroll
@@ -948,7 +948,7 @@ __device__ __forceinline__ void tile_run(const PagedAttn& p, char* lds, const Pa
     for (int r = 1; r < 16 * NK; r++) mx = fmaxf(mx, sc[r >> 4][r & 15]);
     mx = max_xor32(mx) * p.c2;
     if (__any(mx > m + (kLazy - kAbove))) {
-      const float m1 = fmaxf(m, mx + kAbove), alpha = __builtin_amdgcn_exp2f(m - finite_max(m1));
+      const float m1 = mx > m + (kLazy - kAbove) ? mx + kAbove : m, alpha = __builtin_amdgcn_exp2f(m - finite_max(m1));
       m = m1;
       l *= alpha;
 #pragma unroll

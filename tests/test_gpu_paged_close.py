@@ -1,6 +1,7 @@
 """Attention over the paged cache where the precision of its parts shows: the
-weights' own bits, values far smaller than their neighbours, and values as large
-as bf16 holds.  All kernels alike, whatever else is in the batch."""
+weights' own bits, values far smaller than their neighbours, values as large as
+bf16 holds, and rows that a query does not see.  All kernels alike, whatever else
+is in the batch."""
 import pytest
 import torch
 
@@ -91,3 +92,49 @@ def test_values_next_to_the_largest(gpu, heads, new, past, shared):
             cache.k[pg, :, :, 0] = (16 * j + torch.arange(16, device="cuda", dtype=torch.float32)) / 8
     cache.v.abs_()
     check(q, cache, batch, new, lens, lists, shared=shared, scale=1.0, half=False)
+
+
+@pytest.mark.parametrize("heads,new", [((8, 2), [4, 2]), ((16, 2), [4, 2]), ((32, 2), [4, 2]), ((8, 2), [100, 40]), ((6, 2), [257, 33]),
+                                       ((64, 1), [200, 190])])
+@pytest.mark.parametrize("value", [2.0 ** 20, -2.0 ** 127, 2.0 ** -40])
+def test_hidden_values_change_no_bit(gpu, heads, new, value):
+    """A finite value of a later token's row, of whatever size, leaves the tokens
+    before it as they were, bit by bit."""
+    hkv = heads[1]
+    q, cache, batch, lens, lists = case(23, heads, 16, new, [30, 61])
+    want = check(q, cache, batch, new, lens, lists, half=False)
+    at = lens[0] - new[0] // 2
+    pg, r = lists[0][at // 16], at % 16
+    cache.v[pg, 0, r] = value
+    got = check(q, cache, batch, new, lens, lists, half=False)
+    first = new[0] - new[0] // 2
+    g, w = (x.view(sum(new), hkv, -1) for x in (got, want))
+    assert torch.equal(g[:first], w[:first]) and torch.equal(g[new[0]:], w[new[0]:]) and torch.equal(g[:, 1:], w[:, 1:])
+
+
+@pytest.mark.parametrize("heads,new", [((8, 2), [4, 2]), ((16, 2), [4, 2]), ((32, 2), [4, 2]), ((8, 2), [100, 40]), ((6, 2), [257, 33]),
+                                       ((64, 1), [200, 190])])
+@pytest.mark.parametrize("size", [3.0, 50.0])
+def test_hidden_keys_change_no_bit(gpu, heads, new, size):
+    """So does a key of a later token's row that scores far above all others: the
+    rows of a wave keep their maxima by themselves."""
+    hkv = heads[1]
+    q, cache, batch, lens, lists = case(29, heads, 16, new, [30, 61])
+    want = check(q, cache, batch, new, lens, lists, half=False)
+    first = new[0] - new[0] // 2
+    at = lens[0] - new[0] // 2  # a row that the later half of the first sequence's tokens see
+    pg, r = lists[0][at // 16], at % 16
+    cache.k[pg, 0, r] = (size * q[0, first].float()).to(torch.bfloat16)  # (as one of these asks)
+    got = check(q, cache, batch, new, lens, lists, half=False)
+    g, w = (x.view(sum(new), hkv, -1) for x in (got, want))
+    assert torch.equal(g[:first], w[:first]) and torch.equal(g[new[0]:], w[new[0]:]) and torch.equal(g[:, 1:], w[:, 1:])
+
+
+@pytest.mark.parametrize("heads,new,past,shared", BATCHES)
+def test_other_queries_change_no_bit(gpu, heads, new, past, shared):
+    """Nor does a query that scores far higher than the others."""
+    q, cache, batch, lens, lists = case(30, heads, 16, new, [p + shared for p in past], common=shared // 16)
+    want = check(q, cache, batch, new, lens, lists, shared=shared, half=False).view(sum(new), heads[0], D)
+    q[0, 0] = cache.k[lists[0][0], 0, 0] * 4
+    got = check(q, cache, batch, new, lens, lists, shared=shared, half=False).view(sum(new), heads[0], D)
+    assert torch.equal(got[1:], want[1:]) and torch.equal(got[0, 1:], want[0, 1:])
