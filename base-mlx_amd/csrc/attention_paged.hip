@@ -1498,7 +1498,6 @@ extern "C" int bmx_attention_paged(const bmx_bf16* q, const bmx_paged_kv* cache,
     return set_error(BMX_E_ALIGN, "attention_paged: q, out and workspace must be 16-byte aligned");
   if (T == 0 || B == 0) return BMX_OK;
   const size_t bytes = static_cast<size_t>(T) * n_heads * kD * sizeof(uint16_t);
-  if (paged_overlap(q, bytes, out, bytes)) return set_error(BMX_E_ARG, "attention_paged: out overlaps q");
   if (B == 1) shared = 0;  // (one sequence shares with nobody)
   // (blocks of all pairs are counted in an int)
   const int64_t blocks = (static_cast<int64_t>(batch->max_pages) * cache->page_size + 63) / 64;
@@ -1511,6 +1510,12 @@ extern "C" int bmx_attention_paged(const bmx_bf16* q, const bmx_paged_kv* cache,
     return set_error(BMX_E_SHAPE, "attention_paged: %d tokens over up to %d pages: too many", T, batch->max_pages);
   if (workspace_bytes < a.bytes)
     return set_error(BMX_E_ARG, "attention_paged: workspace of %zu bytes, %zu needed", workspace_bytes, a.bytes);
+  // (of the workspace, what the call uses)
+  const Span from{q, bytes}, to{out, bytes}, space{workspace, a.bytes};
+  if (overlaps(to, {from}) || over_cache(to, *cache) || over_batch(to, *batch))
+    return set_error(BMX_E_ARG, "attention_paged: out overlaps q, the cache or the batch's arrays");
+  if (overlaps(space, {from, to}) || over_cache(space, *cache) || over_batch(space, *batch))
+    return set_error(BMX_E_ARG, "attention_paged: the workspace overlaps q, out, the cache or the batch's arrays");
   char* ws = static_cast<char*>(workspace);
   auto part = [&](size_t off) { return reinterpret_cast<float*>(ws + off); };
   const int nb = (shared + kTileKeys - 1) / kTileKeys;

@@ -2,6 +2,8 @@
 // the kernels that append to it and attend over it.
 #pragma once
 
+#include <initializer_list>
+
 #include "bmx_device.h"
 
 namespace bmx {
@@ -13,10 +15,30 @@ constexpr int kPagedMaxRows = 1 << 24;  // of a sequence
 // Checks of the structs themselves; `what` names the entry point.
 int check_paged(const char* what, const bmx_paged_kv* c, const bmx_batch* b, int n_heads, int head_dim);
 
-// Whether a bytes from x and b bytes from y have any in common
-inline bool paged_overlap(const void* x, size_t a, const void* y, size_t b) {
-  const uintptr_t i = reinterpret_cast<uintptr_t>(x), j = reinterpret_cast<uintptr_t>(y);
-  return i < j + b && j < i + a;
+// Some bytes of memory
+struct Span {
+  const void* at;
+  size_t bytes;
+};
+// Whether `s` has a byte in common with any of the others
+inline bool overlaps(const Span& s, std::initializer_list<Span> others) {
+  const uintptr_t i = reinterpret_cast<uintptr_t>(s.at);
+  for (const Span& o : others) {
+    const uintptr_t j = reinterpret_cast<uintptr_t>(o.at);
+    if (i < j + o.bytes && j < i + s.bytes) return true;
+  }
+  return false;
+}
+inline Span span_of_pages(const bmx_paged_kv& c, const void* at) {
+  return {at, static_cast<size_t>(c.n_pages) * c.n_kv_heads * c.page_size * kPagedDim * sizeof(uint16_t)};
+}
+// Whether `s` lies over the cache, or over the batch's arrays
+inline bool over_cache(const Span& s, const bmx_paged_kv& c) {
+  return overlaps(s, {span_of_pages(c, c.k), span_of_pages(c, c.v)});
+}
+inline bool over_batch(const Span& s, const bmx_batch& b) {
+  const size_t n = b.n_seqs;
+  return overlaps(s, {{b.starts, (n + 1) * 4}, {b.lens, n * 4}, {b.pages, n * b.max_pages * 4}});
 }
 
 inline int log2_of(int n) { return 31 - __builtin_clz(static_cast<unsigned>(n)); }

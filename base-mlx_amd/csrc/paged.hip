@@ -32,6 +32,8 @@ int check_paged(const char* what, const bmx_paged_kv* c, const bmx_batch* b, int
   if (!aligned(c->k, 16) || !aligned(c->v, 16) || !aligned(b->starts, 4) || !aligned(b->lens, 4) ||
       !aligned(b->pages, 4))
     return set_error(BMX_E_ALIGN, "%s: k and v must be 16-byte aligned, the batch's arrays 4-byte", what);
+  if (overlaps(span_of_pages(*c, c->k), {span_of_pages(*c, c->v)}))
+    return set_error(BMX_E_ARG, "%s: k and v of the cache overlap", what);
   return BMX_OK;
 }
 
@@ -156,8 +158,16 @@ extern "C" int bmx_qk_norm_rope_paged(const bmx_bf16* q, const bmx_bf16* k, cons
   const int T = batch->tokens;
   if (T == 0 || batch->n_seqs == 0) return BMX_OK;
   const size_t qb = static_cast<size_t>(T) * n_heads * 256, kb = static_cast<size_t>(T) * cache->n_kv_heads * 256;
-  if (paged_overlap(q_out, qb, q, qb) || paged_overlap(q_out, qb, k, kb) || paged_overlap(q_out, qb, v, kb))
-    return set_error(BMX_E_ARG, "qk_norm_rope_paged: q_out overlaps an input");
+  const Span to{q_out, qb}, from[] = {{q, qb}, {k, kb}, {v, kb}, {q_norm, 256}, {k_norm, 256}};
+  if (over_batch(to, *batch)) return set_error(BMX_E_ARG, "qk_norm_rope_paged: q_out overlaps the batch's arrays");
+  if (over_cache(to, *cache)) return set_error(BMX_E_ARG, "qk_norm_rope_paged: q_out overlaps the cache");
+  for (const Span& s : from) {
+    if (overlaps(to, {s})) return set_error(BMX_E_ARG, "qk_norm_rope_paged: q_out overlaps an input");
+    if (over_cache(s, *cache)) return set_error(BMX_E_ARG, "qk_norm_rope_paged: an input overlaps the cache");
+  }
+  for (const void* pages : {cache->k, cache->v})
+    if (over_batch(span_of_pages(*cache, pages), *batch))
+      return set_error(BMX_E_ARG, "qk_norm_rope_paged: the batch's arrays overlap the cache");
   AppendParams p{q, k, v, q_norm, k_norm, q_out, *cache, *batch, n_heads, log2_of(cache->page_size), eps, {}};
   // (64 pow calls are most of a small call's host time: a thread keeps the last)
   thread_local float last = NAN;  // (unequal to anything)

@@ -380,7 +380,8 @@ size_t bmx_kv4_evict_workspace_bytes(int n_kv_heads, int length);
 /* One layer's keys and values in pages that sequences take as they grow: k
  * and v [n_pages, n_kv_heads, page_size, 128] bf16 (16-byte aligned device
  * pointers; the struct itself is host memory, read during the call).
- * page_size is a power of two, 16 .. 4096 (BMX_E_UNSUPPORTED).
+ * page_size is a power of two, 16 .. 4096 (BMX_E_UNSUPPORTED); k and v do not
+ * overlap (BMX_E_ARG).
  * No counterpart in the reference, whose KvCache holds one sequence
  * (crates/base-mlx-core/src/model/qwen3.rs:109-162) and whose server runs one
  * request at a time (crates/base-mlx-server/src/state.rs:1-19). */
@@ -419,8 +420,8 @@ typedef struct {
  * in double, so that far positions keep their precision.  (bmx_qk_norm_rope_kv
  * rounds the norm to bf16 twice on the way, as MLX does, and takes the angle in
  * fp32: results differ by those roundings.)  All pointers 16-byte aligned;
- * q_out overlaps none of q, k, v (BMX_E_ARG).  tokens = 0 or n_seqs = 0 is a
- * no-op.
+ * q_out and the cache overlap none of the inputs, the batch's arrays or each
+ * other (BMX_E_ARG).  tokens = 0 or n_seqs = 0 is a no-op.
  * Replaces: the per-layer sequence of Qwen3::forward_internal q_norm/k_norm ->
  *   transpose -> fast::rope -> mlx_ext::slice_update
  *   (crates/base-mlx-core/src/model/qwen3.rs:392-489), for a batch. */
@@ -448,7 +449,8 @@ int bmx_qk_norm_rope_paged(const bmx_bf16 *q, const bmx_bf16 *k, const bmx_bf16 
  * bmx_attention_paged_workspace_bytes or more, else BMX_E_ARG; its first
  * BMX_PAGED_COUNTER_BYTES zero-filled before its first use (every call leaves
  * them zero); calls that share one must not run concurrently.  q, out: 16-byte
- * aligned, without overlap (BMX_E_ARG).  tokens = 0 or n_seqs = 0 is a no-op;
+ * aligned.  out and the workspace overlap neither each other nor q, the cache or
+ * the batch's arrays (BMX_E_ARG).  tokens = 0 or n_seqs = 0 is a no-op;
  * more than 2^30 blocks of 64 keys in all is BMX_E_SHAPE.
  * Replaces: mlx_rs::fast::scaled_dot_product_attention as bmx_attention_gqa
  *   does (crates/base-mlx-core/src/model/qwen3.rs:491-518, 629-653), for a
