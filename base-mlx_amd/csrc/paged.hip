@@ -7,6 +7,8 @@
 //   a = p theta^(-i/64)
 #include <math.h>
 
+#include <algorithm>
+
 #include "paged.h"
 
 namespace bmx {
@@ -53,6 +55,8 @@ struct AppendParams {
   double turns[64];  // theta^(-i/64) / 2 pi: turns per position
 };
 
+constexpr int kGridRow = 1 << 20;  // workgroups: a grid's row holds fewer than 2^32 threads, 2^24 tokens of this kernel
+
 // A workgroup of 4 waves takes a token.  Its rows -- the q heads, the k heads,
 // the v heads -- go 16 lanes to a row, lane li holding values 4 li .. + 3 and
 // 64 + 4 li .. + 3, the two halves of four rotated pairs.  The sequence's search
@@ -62,9 +66,10 @@ struct AppendParams {
 // after another.
 __global__ void __launch_bounds__(256) qk_norm_rope_paged_kernel(const AppendParams p) {
   __shared__ __align__(16) float cs[2][64];
-  const int t = blockIdx.x;
+  const int t = blockIdx.y * kGridRow + blockIdx.x;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int T = p.b.tokens, B = p.b.n_seqs, Hkv = p.c.n_kv_heads;
+  if (t >= T) return;  // uniform, as every return up to the barrier
   // ---- the token's sequence: the last whose rows start at t or before.  64
   // samples of the starts, then the 64 (or fewer) from the last sample on ----
   const int step = (B + 63) >> 6;
@@ -72,7 +77,7 @@ __global__ void __launch_bounds__(256) qk_norm_rope_paged_kernel(const AppendPar
   if (step > 1) {
     const int at = lane * step;
     const uint64_t m = __ballot(at < B && p.b.starts[min(at, B - 1)] <= t);
-    if (m == 0) return;  // uniform, as every return up to the barrier
+    if (m == 0) return;
     seg = (__popcll(m) - 1) * step;
   }
   const int at = min(seg + lane, B - 1);
@@ -177,6 +182,6 @@ extern "C" int bmx_qk_norm_rope_paged(const bmx_bf16* q, const bmx_bf16* k, cons
     last = theta;
   }
   for (int i = 0; i < 64; i++) p.turns[i] = turns[i];
-  hipLaunchKernelGGL(qk_norm_rope_paged_kernel, dim3(static_cast<unsigned>(T)), dim3(256), 0, as_stream(stream), p);
+  hipLaunchKernelGGL(qk_norm_rope_paged_kernel, dim3(std::min(T, kGridRow), (T + kGridRow - 1) / kGridRow), dim3(256), 0, as_stream(stream), p);
   return check_launch("qk_norm_rope_paged");
 }

@@ -6,7 +6,7 @@ import pytest
 import torch
 
 import bmx
-from _paged_check import D, attention_reference, hold, layout, normal
+from _paged_check import D, attention_reference, hold, layout, normal, rotated
 from test_gpu_paged import cache_of
 
 pytestmark = pytest.mark.gpu
@@ -57,3 +57,27 @@ def test_a_long_sequence_before_a_short_one_behind_shared_rows(gpu):
                                       1 / math.sqrt(D), shared, half=False)
     hold(out[rows], want, bound)
     assert (out[2:6100] == 7).all() and (out[6102:] == 7).all()
+
+
+def test_append_of_more_tokens_than_a_grid_row(gpu):
+    """2^24 tokens and some, of which the first and the last few belong to sequences."""
+    T, new = (1 << 24) + 5, [3, 4]
+    lens = [3, 20]
+    lists, n_pages = layout(7, new, lens, PAGE)
+    cache = cache_of(8, n_pages, 1, PAGE)
+    x = [torch.zeros(T, D, dtype=torch.bfloat16, device="cuda") for _ in "qkv"]
+    rows = [0, 1, 2, T - 4, T - 3, T - 2, T - 1]
+    for i, t in enumerate(x):
+        t[rows] = normal(9 + i, 7, D).to(torch.bfloat16)
+    w = [(1 + 0.3 * normal(12 + i, D)).to(torch.bfloat16) for i in range(2)]
+    one = bmx.PagedBatch.of(new, lens, lists)
+    starts = torch.tensor([0, 3, T - 4, T], dtype=torch.int32, device="cuda")
+    # (the sequence between them has no pages, so its tokens no rows)
+    three = bmx.PagedBatch(starts, torch.tensor([3, 0, 20], dtype=torch.int32, device="cuda"),
+                           torch.stack([one.pages[0], torch.full_like(one.pages[0], -1), one.pages[1]]), T)
+    got = bmx.qk_norm_rope_paged(*x, *w, cache, three)
+    pos = torch.tensor([0, 1, 2, 16, 17, 18, 19], device="cuda")
+    for y, w1, g in ((x[0], w[0], got[0, rows]), (x[1], w[1], torch.cat([cache.k[lists[0][0], 0, :3], cache.k[lists[1][1], 0, :4]]))):
+        want, bound = rotated(y[rows].view(7, 1, D), w1, pos, 1e-6, 1e6)
+        assert ((g.double() - want[:, 0]).abs() <= bound[:, 0]).all()
+    assert torch.equal(torch.cat([cache.v[lists[0][0], 0, :3], cache.v[lists[1][1], 0, :4]]), x[2][rows])
