@@ -81,3 +81,75 @@ def test_append_of_more_tokens_than_a_grid_row(gpu):
         want, bound = rotated(y[rows].view(7, 1, D), w1, pos, 1e-6, 1e6)
         assert ((g.double() - want[:, 0]).abs() <= bound[:, 0]).all()
     assert torch.equal(torch.cat([cache.v[lists[0][0], 0, :3], cache.v[lists[1][1], 0, :4]]), x[2][rows])
+
+
+# ---------------------------------------------------------------------------
+# tiles of 256 query rows: 12288 a sequence
+# ---------------------------------------------------------------------------
+WIDE = [  # heads, new tokens, cached rows before them (own ones), shared rows
+    ((64, 1), [200], [0], 0), ((64, 1), [193], [7], 0),     # one tile after another, the last ragged
+    ((64, 1), [200], [5000], 0), ((64, 8), [1600], [3000], 0),  # cut along the keys, and joined
+    ((40, 1), [620, 1], [33, 900], 0),                      # 40 rows to a token: tiles that end inside one
+    ((64, 1), [390, 3], [0, 100], 48), ((64, 1), [200, 190], [3000, 0], 1008), ((48, 1), [500, 1, 300], [5, 700, 40], 16),
+]
+
+
+def wide(seed, heads, new, past, shared):
+    lens = [n + p + shared for n, p in zip(new, past)]
+    assert sum(new) * heads[0] // heads[1] >= 12288 * len(new)
+    lists, n_pages = layout(seed, new, lens, PAGE, common=shared // PAGE)
+    cache = cache_of(seed, n_pages, heads[1], PAGE)
+    q = (1.5 * normal(seed + 9, heads[0], sum(new), D)).to(torch.bfloat16)
+    return q, cache, lens, lists
+
+
+def attend(q, cache, new, lens, lists, shared):
+    batch = bmx.PagedBatch.of(new, lens, lists)
+    got = bmx.attention_paged(q, cache, batch, shared=shared, workspace=dirty(q.shape[0], cache.n_kv_heads, batch, shared))
+    want, bound = attention_reference(q, cache.k, cache.v, new, lens, lists, 1 / math.sqrt(D), shared, half=False)
+    hold(got, want, bound)
+    return got
+
+
+@pytest.mark.parametrize("heads,new,past,shared", WIDE)
+def test_wide_tiles(gpu, heads, new, past, shared):
+    q, cache, lens, lists = wide(20, heads, new, past, shared)
+    want = attend(q, cache, new, lens, lists, shared)
+    # rows of nobody
+    used = torch.zeros(cache.n_pages, PAGE, dtype=torch.bool, device="cuda")
+    for pages, n in zip(lists, lens):
+        for j in range(n):
+            used[pages[j // PAGE], j % PAGE] = True
+    for x in (cache.k, cache.v):
+        x[(~used)[:, None, :, None].expand_as(x)] = math.nan
+    assert torch.equal(attend(q, cache, new, lens, lists, shared), want)
+    # pages that do not exist, among the first sequence's own
+    lists[0][shared // PAGE + 1], lists[0][-1] = -3, cache.n_pages
+    attend(q, cache, new, lens, lists, shared)
+
+
+@pytest.mark.parametrize("heads,new,past,shared", WIDE)
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+def test_wide_tiles_values_not_finite(gpu, heads, new, past, shared, bad):
+    """One that the later half of the first sequence's tokens see, and one that all see."""
+    q, cache, lens, lists = wide(21, heads, new, past, shared)
+    hkv, rep = heads[1], heads[0] // heads[1]
+    want = attend(q, cache, new, lens, lists, shared)
+    first = new[0] // 2
+    at = lens[0] - new[0] + first
+    cache.v[lists[0][at // PAGE], 0, at % PAGE, 77] = bad
+    got = attend(q, cache, new, lens, lists, shared)
+    g, w = (x.view(sum(new), hkv, rep, D) for x in (got, want))
+    assert torch.equal(g[:first], w[:first]) and torch.equal(g[new[0]:], w[new[0]:])
+    assert not torch.isfinite(g[first:new[0], 0, :, 77]).any()
+    cache.v[lists[0][0], 0, 0, 5] = bad
+    g = attend(q, cache, new, lens, lists, shared).view(sum(new), hkv, rep, D)
+    assert not torch.isfinite(g[:sum(new) if shared else new[0], 0, :, 5]).any()
+
+
+@pytest.mark.parametrize("heads,new,past,shared", WIDE)
+def test_wide_tiles_of_large_and_small_values(gpu, heads, new, past, shared):
+    q, cache, lens, lists = wide(22, heads, new, past, shared)
+    cache.v[..., 3::5] *= 2.0 ** -40
+    cache.v[:, :, 2::7] *= 2.0 ** 100
+    attend(q, cache, new, lens, lists, shared)
