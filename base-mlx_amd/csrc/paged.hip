@@ -34,8 +34,6 @@ int check_paged(const char* what, const bmx_paged_kv* c, const bmx_batch* b, int
   if (!aligned(c->k, 16) || !aligned(c->v, 16) || !aligned(b->starts, 4) || !aligned(b->lens, 4) ||
       !aligned(b->pages, 4))
     return set_error(BMX_E_ALIGN, "%s: k and v must be 16-byte aligned, the batch's arrays 4-byte", what);
-  if (overlaps(span_of_pages(*c, c->k), {span_of_pages(*c, c->v)}))
-    return set_error(BMX_E_ARG, "%s: k and v of the cache overlap", what);
   return BMX_OK;
 }
 
@@ -162,6 +160,8 @@ extern "C" int bmx_qk_norm_rope_paged(const bmx_bf16* q, const bmx_bf16* k, cons
     return set_error(BMX_E_ALIGN, "qk_norm_rope_paged: pointers must be 16-byte aligned");
   const int T = batch->tokens;
   if (T == 0 || batch->n_seqs == 0) return BMX_OK;
+  if (overlaps(span_of_pages(*cache, cache->k), {span_of_pages(*cache, cache->v)}))
+    return set_error(BMX_E_ARG, "qk_norm_rope_paged: k and v of the cache overlap");
   const size_t qb = static_cast<size_t>(T) * n_heads * 256, kb = static_cast<size_t>(T) * cache->n_kv_heads * 256;
   const Span to{q_out, qb}, from[] = {{q, qb}, {k, kb}, {v, kb}, {q_norm, 256}, {k_norm, 256}};
   if (over_batch(to, *batch)) return set_error(BMX_E_ARG, "qk_norm_rope_paged: q_out overlaps the batch's arrays");

@@ -380,8 +380,7 @@ size_t bmx_kv4_evict_workspace_bytes(int n_kv_heads, int length);
 /* One layer's keys and values in pages that sequences take as they grow: k
  * and v [n_pages, n_kv_heads, page_size, 128] bf16 (16-byte aligned device
  * pointers; the struct itself is host memory, read during the call).
- * page_size is a power of two, 16 .. 4096 (BMX_E_UNSUPPORTED); k and v do not
- * overlap (BMX_E_ARG).
+ * page_size is a power of two, 16 .. 4096 (BMX_E_UNSUPPORTED).
  * No counterpart in the reference, whose KvCache holds one sequence
  * (crates/base-mlx-core/src/model/qwen3.rs:109-162) and whose server runs one
  * request at a time (crates/base-mlx-server/src/state.rs:1-19). */
@@ -420,8 +419,8 @@ typedef struct {
  * in double, so that far positions keep their precision.  (bmx_qk_norm_rope_kv
  * rounds the norm to bf16 twice on the way, as MLX does, and takes the angle in
  * fp32: results differ by those roundings.)  All pointers 16-byte aligned;
- * q_out and the cache overlap none of the inputs, the batch's arrays or each
- * other (BMX_E_ARG).  tokens = 0 or n_seqs = 0 is a no-op.
+ * q_out, cache->k and cache->v overlap neither each other nor the inputs or the
+ * batch's arrays (BMX_E_ARG).  tokens = 0 or n_seqs = 0 is a no-op.
  * Replaces: the per-layer sequence of Qwen3::forward_internal q_norm/k_norm ->
  *   transpose -> fast::rope -> mlx_ext::slice_update
  *   (crates/base-mlx-core/src/model/qwen3.rs:392-489), for a batch. */
