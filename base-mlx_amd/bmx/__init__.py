@@ -698,8 +698,9 @@ class PagedBatch(_Fixed):
     starts[b + 1] - 1 and the last of its lens[b] cached rows; row j of a
     sequence lies on page pages[b, j // page_size].  tokens: the packed rows
     there are (>= starts[-1]); max_new: at least every sequence's new tokens
-    (None: tokens).  The arrays are read when the work runs: change what they
-    hold between steps, or between replays of a graph."""
+    (None: tokens).  It chooses the kernels of attention_paged: pass the true
+    maximum, 1 for a decode step.  The arrays are read when the work runs: change
+    what they hold between steps, or between replays of a graph."""
 
     def __init__(self, starts, lens, pages, tokens, max_new=None):
         torch = _torch()

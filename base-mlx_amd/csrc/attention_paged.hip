@@ -794,9 +794,10 @@ constexpr int kSchedMfma = 0x8, kSchedRead = 0x100, kSchedValu = 0x402;
 // chunk c lies at c ^ (4 (row % 4) + row / 4 % 4), which keeps both kinds of
 // read off each other's banks.  64 KB of LDS and up to 256 registers: two
 // workgroups share a CU, one's exponentials beside the other's products.
-// One prompt of 4096 tokens, 32 heads: 204 us, 137 GFLOP at 0.67 PFLOP/s (a large
-// matrix product reaches 1.12); the two pieces of the weights make 206 GFLOP of
-// products, 1.01.
+// One prompt of 4096 tokens, 32 heads: 200 to 217 us (boxes differ; the kernel 208),
+// 137 GFLOP at 0.66 PFLOP/s, where a large matrix product reaches 1.12; the two
+// pieces of the weights make it 206 GFLOP of products, 0.99.  The matrix cores are
+// busy 51 % of the cycles and the vector units 46 %: the two overlap only in part.
 template <bool PRE, int NW, int WK>
 __device__ __forceinline__ void tile_run(const PagedAttn& p, char* lds, const PagedSeq& sq, int b, int h, int r0, int j0,
                                          int j1, const Result& to) {
@@ -1306,8 +1307,9 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const PagedAtt
   }
   // ---- pieces of at most `size` blocks: each piece more is results to be written
   // and joined (us with 1 / 1.25 / 1.5 / 2 times the average, or uncut: 1000 tokens
-  // over 3000 rows 120 / 101 / 100 / 130 / 135; a chunk of 509 beside 31 single tokens
-  // 76 / 74 / 70 / 70 / 103; 64 over 30000 73 / 72 / 75 / 69 / 682) ----
+  // over 3000 rows 130 / 115 / 115 / 135 / 125; a chunk of 509 beside 31 single tokens
+  // 77 / 76 / 75 / 80 / 107; 64 over 30000 76 / 78 / 81 / 73 / 758; six prompts of 1 to
+  // 2049 90 / 89 / 83 / 83 / 86; 509 over 3000 81 / 66 / 69 / 75 / 102) ----
   const int size = piece_size(sum, per_head, most);
   const float to_bin = static_cast<float>(kPlanBins - 1) / static_cast<float>(size);
   auto bin_of = [&](int len) { return kPlanBins - 1 - min(static_cast<int>(len * to_bin), kPlanBins - 1); };
@@ -1374,24 +1376,27 @@ __global__ void __launch_bounds__(256) paged_tile_merge_kernel(const PagedAttn p
 // ---------------------------------------------------------------------------
 // Rows of a (sequence, kv head) pair up to which shares serve: no launches for a
 // plan, and lengths balanced to a block.  (Us, shares / tiles, 48 rows a pair, 8 kv
-// heads: 16 sequences of 20 to 300 rows 14.6 / 19.5, of 2000 to 3000 48.8 / 53.3, 4 of
-// 7000 to 8000 36.7 / 44.8, 16 behind 2048 shared rows 33 / 50; 64 of 500 to 4000 with up
-// to 60 rows, where the products weigh, 115 / 112.)
+// heads: 16 sequences of 20 to 300 rows 14.6 / 19.8, of 2000 to 3000 48 / 57, 4 of
+// 7000 to 8000 37 / 47, 16 behind 2048 shared rows 30 / 50; 64 of 500 to 4000 with up
+// to 60 rows 100 / 111.)
 constexpr int kFewRows = 64;
-// Of these up to 32 go straight from memory to registers, more through LDS: 20 rows
-// 17.0 / 19.0 and 22.0 / 26.0 us that way / this, 28 and 32 rows even (26.5 / 24.8, 107.5 /
-// 109.2); 64 rows that way need more than 256 registers (36 us for 16 sequences of 5
-// tokens, where the other takes 30).
+// Of these up to 32 go straight from memory to registers, more through LDS: 64 rows
+// that way need more than 256 registers (36 us for 16 sequences of 5 tokens of 64
+// heads over 8, where the other takes 29).  Up to 16 rows that way is the faster
+// one; from 17 to 32 the two are within 15 % (us, that way / this, 8 kv heads, 64-row
+// pages: 16 sequences of 300 to 3000 rows, 20 query rows a pair 27.4 / 23.9, 32 of them
+// 28.7 / 25.0; 64 of 500 to 4000, 32 108 / 107; one over 4096, 20 16.9 / 16.2, over 131000,
+// 32 110 / 107; 16 behind 2048 shared rows, 20 24.6 / 24.2).
 constexpr int kFewDirect = 32;
 constexpr int kFewGrid = 512;      // workgroups of shares: two to a CU
 constexpr int kTileGrid = 512;     // 128-row tiles at once: two workgroups to a CU
 constexpr int kMaxPre = 64;        // key splits of the shared rows
 
-// Rows of a tile.  256 stage and convert a block of keys once for twice the rows,
-// but leave a workgroup alone on its CU, half as many tiles to balance, and more
-// of them idle in short sequences (us with 128 / 256 rows, 32 q heads over 8: one
-// prompt of 4096 tokens 190 / 176, 2048 over 2048 151 / 155, 512 26 / 30, six of 1 to
-// 2049 79 / 84; a chunk of 509 beside 31 single tokens 77 / 90).
+// Rows of a tile.  256 stage a block of keys once for twice the rows, but leave a
+// workgroup alone on its CU, half as many tiles to balance, and more of them idle
+// in short sequences (us with 128 / 256 rows, 32 q heads over 8: one prompt of 4096
+// tokens 221 / 216, 2048 over 2048 174 / 186, 512 26 / 31, six of 1 to 2049 83 / 91; a
+// chunk of 509 beside 31 single tokens 75 / 91).
 int tile_rows(int rep, int T, int B) { return static_cast<int64_t>(T) * rep >= static_cast<int64_t>(B) * 12288 ? 256 : 128; }
 
 struct PagedPlan {
@@ -1519,15 +1524,16 @@ extern "C" int bmx_attention_paged(const bmx_bf16* q, const bmx_paged_kv* cache,
   char* ws = static_cast<char*>(workspace);
   auto part = [&](size_t off) { return reinterpret_cast<float*>(ws + off); };
   const int nb = (shared + kTileKeys - 1) / kTileKeys;
-  // at least 4 blocks to a split of the shared rows (32 and 160 single tokens
-  // over 8192 and 512 shared rows, as many splits as fill the CUs / that: 38.7 /
-  // 31.5, 54.2 / 46.6 us)
+  // at least 4 blocks to a split of the shared rows, whose parts have to be joined
+  // (us, so / as many splits as fill the CUs, 20 tokens each: 2 sequences behind 2048
+  // shared rows 37 / 44, 4 behind 1024 37 / 42, 16 behind 512 45.8 / 47.6, 2 behind 512
+  // 33.9 / 31.4; 2 single tokens behind 512 14.5 / 11.8)
   // -- nor more than the shared rows' part of the places, where the sequences' own
   // are few: a pair's, whose lengths are not known here, for three blocks of a tile
-  // (us, so / without: 64 single tokens over 4096 shared rows 28.3 / 30.8, 160 over 2048
-  // 34.8 / 39.9, 30 of one q head a kv head over 16384 23.1 / 26.5, 200 over 4096
-  // 56.1 / 59.9; 32 over 8192, 64 over 1024, 160 over 32768 alike; with two blocks
-  // 30.8, 34.3, 25.9, 59.8, with five 27.5, 38.5, 23.6, 54.3 and 160 over 32768 150 for 145)
+  // (us, so / without: 64 single tokens over 4096 shared rows 28.1 / 31.0, 160 over 2048
+  // 36.3 / 40.9, 30 of one q head a kv head over 16384 25.2 / 28.2, 200 over 4096
+  // 55.8 / 60.1; 32 over 8192, 64 over 1024, 160 over 32768 alike; with two blocks
+  // 31.0, 35.1, 27.9, 56.4, with five 29.5, 43.1, 25.5, 57.4 and 160 over 32768 170 for 164)
   int splits = std::min(a.np, (nb + 3) / 4);
   const int64_t pairs = static_cast<int64_t>(B) * Hkv, pre_tiles = Hkv * a.all;
   if (a.few && splits > 1) {
@@ -1566,8 +1572,8 @@ extern "C" int bmx_attention_paged(const bmx_bf16* q, const bmx_paged_kv* cache,
       // Shares for the places that the shared rows' tiles leave of a round, so that
       // none waits for a place -- if that is a quarter of them and they get four
       // pairs each at most.  (Us, so / always kFewGrid: 64 tokens over 4096 shared rows
-      // 30.6 / 32.9, 32 over 8192 25.6 / 28.5, 160 over 512 29.6 / 33.5; 160 over 2048, 6.7
-      // pairs each, 48.0 / 39.7; 64 over 2048 with 500 to 3000 of their own 85.7 / 84.4.)
+      // 28.1 / 31.5, 32 over 8192 26.7 / 28.8, 160 over 2048 36.3 / 41.0; 160 over 512 or
+      // 32768, 64 over 2048 with 500 to 3000 of their own alike.)
       const int left = kFewGrid - pre % kFewGrid;
       const int few_grid = 4 * left >= kFewGrid && pairs <= 4 * left ? left : kFewGrid;
       if (shared) hipLaunchKernelGGL(with_shared, dim3(pre + few_grid), dim3(256), lds, st, p, pre);

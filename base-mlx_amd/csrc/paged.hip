@@ -80,7 +80,7 @@ __global__ void __launch_bounds__(256) qk_norm_rope_paged_kernel(const AppendPar
   }
   const int at = min(seg + lane, B - 1);
   const int s0 = p.b.starts[at], s1 = p.b.starts[at + 1], ln = p.b.lens[at];
-  const uint64_t m = __ballot(seg + lane < B && lane < step * 64 && s0 <= t);
+  const uint64_t m = __ballot(seg + lane < B && s0 <= t);
   if (m == 0) return;
   const int own = __popcll(m) - 1, b = seg + own;
   const PagedSeq sq = paged_seq(__builtin_amdgcn_readlane(s0, own), __builtin_amdgcn_readlane(s1, own),

@@ -22,7 +22,7 @@ def dirty(n_heads, n_kv_heads, batch, shared):
 
 
 @pytest.mark.parametrize("n", [1, 6, 14])
-@pytest.mark.parametrize("tokens,first", [(6144, 6100), (6144, 3072), (6144, 0), (6200, 5), (20000, 19900)])
+@pytest.mark.parametrize("tokens,first", [(6144, 6100), (6144, 3071), (6144, 0), (6200, 5), (20000, 19900)])
 def test_few_rows_of_many_behind_shared_ones(gpu, n, tokens, first):
     """Two sequences of n tokens somewhere among many packed rows."""
     hq, hkv, shared, new = 8, 2, 32, [n, n]
