@@ -794,7 +794,7 @@ constexpr int kSchedMfma = 0x8, kSchedRead = 0x100, kSchedValu = 0x402;
 // chunk c lies at c ^ (4 (row % 4) + row / 4 % 4), which keeps both kinds of
 // read off each other's banks.  64 KB of LDS and up to 256 registers: two
 // workgroups share a CU, one's exponentials beside the other's products.
-// One prompt of 4096 tokens, 32 heads: 200 to 217 us (boxes differ; the kernel 208),
+// One prompt of 4096 tokens, 32 heads: 200 to 217 us (cards differ; the kernel 208),
 // 137 GFLOP at 0.66 PFLOP/s, where a large matrix product reaches 1.12; the two
 // pieces of the weights make it 206 GFLOP of products, 0.99.  The matrix cores are
 // busy 51 % of the cycles and the vector units 46 %: the two overlap only in part.

@@ -439,7 +439,7 @@ int bmx_qk_norm_rope_paged(const bmx_bf16 *q, const bmx_bf16 *k, const bmx_bf16 
  * new tokens has at least that many rows before them.
  * A token that sees no row, or whose every score is -inf, gets zeros.  A row that
  * a query does not see leaves it alone to the last bit, whatever it holds, and so
- * do the other queries; one that it sees, with a score above -inf and a value that
+ * does what other queries hold; one that it sees, with a score above -inf and a value that
  * is not finite, makes that dimension of its output not finite.  Softmax statistics and
  * sums are fp32, weights enter the products with 16 bits, whatever else is in the
  * batch, and values as they are.  The order of every sum
