@@ -25,13 +25,13 @@
 // The merges fold in what comes of them.
 //
 // Scores are in base 2: p = 2^(s c - m), c = |scale| log2 e (a negative scale
-// flips q's signs).  The running m is 2^16 above a row's largest score, and follows
-// it only once that is 2^8 ahead, each row by itself: sums and outputs are fp32
-// either way, and the rescaling of the outputs all but vanishes.  Weights of at most 2^-8, and 2^-16
-// where m has followed, keep the sums of 2^15 rows of values of 2^120 in range (of
-// 256 next to bf16's largest); values of 2^-100 still have 2^-116, above the
-// smallest normal.  With one bf16 piece of p, outputs
-// were off by 0.0024 of their norm where their own rounding is 0.0017, so p has
+// flips q's signs).  The running m is set 2^16 above a row's largest score, and
+// anew only once that has grown by 2^8, each row by itself: sums and outputs are
+// fp32 either way, and the rescaling of the outputs all but vanishes.  Weights of
+// at most 2^-8, and 2^-16 where m was just set, keep the sums of 2^15 rows of values
+// of 2^120 in range (of 256 next to bf16's largest); values of 2^-100 still have
+// 2^-116, above the smallest normal.  With one bf16 piece of p, outputs were off by
+// 0.0024 of their norm where their own rounding is 0.0017, so p has
 // more bits: two bf16 pieces (16 bits), in every kernel, so that a token's
 // precision does not depend on what else is in its batch, and V stays the bf16
 // that it is, of any size.  (Tiles with p and V in fp16 save the second product,
@@ -50,7 +50,7 @@ namespace {
 constexpr int kD = kPagedDim;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kAbove = 16.0f;  // log2 by which m is set above the largest score
-constexpr float kLazy = 8.0f;    // log2 by which it may lag behind that
+constexpr float kLazy = 8.0f;    // log2 by which that may grow before m is set anew
 constexpr float kLeast = 1.17549435e-38f;  // of c: a scale of 0 leaves a hidden key's -inf what it is
 
 typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8_t;
@@ -512,7 +512,8 @@ __device__ __forceinline__ void few_run(const PagedAttn& p, FewLds& lds, int wg,
         for (int e = 1; e < 8; e++) mx = fmaxf(mx, sc[nt][e >> 2][e & 3]);
         mx = max_xor32(max_xor16(mx)) * p.c2;
         if (__any(mx > m[nt] + (kLazy - kAbove))) {
-          const float m1 = mx > m[nt] + (kLazy - kAbove) ? mx + kAbove : m[nt], alpha = __builtin_amdgcn_exp2f(m[nt] - finite_max(m1));
+          const float m1 = mx > m[nt] + (kLazy - kAbove) ? mx + kAbove : m[nt];
+          const float alpha = __builtin_amdgcn_exp2f(m[nt] - finite_max(m1));
           m[nt] = m1;
           l[nt] *= alpha;
 #pragma unroll
@@ -949,7 +950,8 @@ __device__ __forceinline__ void tile_run(const PagedAttn& p, char* lds, const Pa
     for (int r = 1; r < 16 * NK; r++) mx = fmaxf(mx, sc[r >> 4][r & 15]);
     mx = max_xor32(mx) * p.c2;
     if (__any(mx > m + (kLazy - kAbove))) {
-      const float m1 = mx > m + (kLazy - kAbove) ? mx + kAbove : m, alpha = __builtin_amdgcn_exp2f(m - finite_max(m1));
+      const float m1 = mx > m + (kLazy - kAbove) ? mx + kAbove : m;
+      const float alpha = __builtin_amdgcn_exp2f(m - finite_max(m1));
       m = m1;
       l *= alpha;
 #pragma unroll
@@ -1164,8 +1166,8 @@ __global__ void __launch_bounds__(64 * NW, 2) paged_tile_kernel(const PagedAttn 
 }
 
 // Up to 64 query rows of a pair, in blocks of 64 keys by shares as few_run: two
-// row groups of waves, each by two waves that take half of a block's keys.  16 sequences of 5 tokens, 40 rows
-// each, over 300 to 3000 rows: 29 us (the kernel 23.1), 79 MB at 3.4 TB/s: bound by
+// row groups of waves, each by two waves that take half of a block's keys.  16
+// sequences of 5 tokens, 40 rows each, over 300 to 3000 rows: 29 us (the kernel 23.1), 79 MB at 3.4 TB/s: bound by
 // the softmax between loads that LDS holds one block ahead.
 __device__ __forceinline__ void mid_run(const PagedAttn& p, char* lds, int wg, int wgs) {
   int* const tmp = reinterpret_cast<int*>(lds + kTileLds);
@@ -1382,8 +1384,8 @@ __global__ void __launch_bounds__(256) paged_tile_merge_kernel(const PagedAttn p
 constexpr int kFewRows = 64;
 // Of these up to 32 go straight from memory to registers, more through LDS: 64 rows
 // that way need more than 256 registers (36 us for 16 sequences of 5 tokens of 64
-// heads over 8, where the other takes 29).  Up to 16 rows that way is the faster
-// one; from 17 to 32 the two are within 15 % (us, that way / this, 8 kv heads, 64-row
+// heads over 8, where the other takes 29).  Up to 16 rows that way alone hands its
+// parts over without a launch; from 17 to 32 the two are within 15 % (us, that way / this, 8 kv heads, 64-row
 // pages: 16 sequences of 300 to 3000 rows, 20 query rows a pair 27.4 / 23.9, 32 of them
 // 28.7 / 25.0; 64 of 500 to 4000, 32 108 / 107; one over 4096, 20 16.9 / 16.2, over 131000,
 // 32 110 / 107; 16 behind 2048 shared rows, 20 24.6 / 24.2).
